@@ -10,7 +10,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("F2CGT_B200_LIB") or os.path.join(_PKG, "libf2cgt_b200.so")  # override: another build of the same ABI
 
 # dtype tags of include/f2cgt_b200.h
-U8, I8, I16, I32, I64, F16, F32, F64 = range(8)
+U8, I8, I16, I32, I64, F16, F32, F64, BF16 = range(9)
 MEAN, SUM = 0, 1
 L2, COSINE = 0, 1
 SCORER_EXACT, SCORER_TENSOR, NO_WAITS = 0x100, 0x200, 0x400
@@ -34,6 +34,10 @@ class Minibatch(C.Structure):  # f2c_minibatch
                 ("rng_offset", C.c_uint64), ("unique", C.c_void_p), ("sub_indptr", C.c_void_p * MAX_HOPS), ("ids", C.c_void_p * MAX_HOPS),
                 ("local", C.c_void_p * MAX_HOPS), ("node_map", C.c_void_p), ("header", C.c_void_p), ("workspace", C.c_void_p),
                 ("workspace_bytes", C.c_int64), ("epoch", C.c_uint32)]
+
+
+class MuonMatrix(C.Structure):  # f2c_muon_matrix
+    _fields_ = [("weight", C.c_void_p), ("grad", C.c_void_p), ("momentum", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64)]
 
 
 class F2CError(RuntimeError):
@@ -106,11 +110,21 @@ SIGNATURES = {
     "f2c_sample_block": [p, p, p, ci, i64, ci, u64, u64, p, p, p, p, p, p, i64, p],
     "f2c_sample_minibatch_workspace": [i64, i64, ci, C.POINTER(ci)],
     "f2c_sample_minibatch": [C.POINTER(Minibatch), p],
+    "f2c_int8_quantize": [p, i64, i64, p, i64, i64, ci, i64, p, i64, p, p],
+    "f2c_int8_mm_workspace": [p, i64, p, i64, i64, i64, i64],
+    "f2c_int8_mm": [p, i64, p, p, i64, p, p, ci, p, ci, i64, i64, i64, p, i64, p],
+    "f2c_int8_linear_workspace": [p, i64, i64, i64, i64],
+    "f2c_int8_linear": [p, i64, i64, p, i64, i64, ci, p, i64, p, p, ci, p, ci, i64, i64, p, i64, p],
+    "f2c_orthogonalize_workspace": [ci, i64, i64, i64],
+    "f2c_orthogonalize": [p, p, ci, i64, i64, i64, p, ci, f32, p, i64, p],
+    "f2c_muon_workspace": [C.POINTER(MuonMatrix), ci, ci],
+    "f2c_muon_step": [C.POINTER(MuonMatrix), ci, ci, f32, f32, ci, f32, p, ci, f32, p, i64, p],
     "f2c_last_error": [],
     "f2c_version": [],
 }
 _RESTYPE = {"f2c_last_error": C.c_char_p, "f2c_kmeans_assign_workspace": C.c_int64, "f2c_kmeans_fit_workspace": C.c_int64, "f2c_sq_statistics_workspace": C.c_int64,
-            "f2c_relabel_capacity": C.c_int64,
+            "f2c_relabel_capacity": C.c_int64, "f2c_int8_mm_workspace": C.c_int64, "f2c_int8_linear_workspace": C.c_int64,
+            "f2c_orthogonalize_workspace": C.c_int64, "f2c_muon_workspace": C.c_int64,
             "f2c_sample_block_workspace": C.c_int64, "f2c_sample_minibatch_workspace": C.c_int64, "f2c_peer_hot_first_cold_id": C.c_int64}
 
 for _name, _args in SIGNATURES.items():

@@ -2,6 +2,7 @@
 // the SQ decode expression and the Philox generator used by dropout.
 #pragma once
 #include <cuda_runtime.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -31,11 +32,12 @@ static inline bool is_sq_bits(int b) { return b == 1 || b == 2 || b == 4 || b ==
 static inline int dtype_size(int dt) {
   switch (dt) {
     case F2C_U8: case F2C_I8: return 1;
-    case F2C_I16: case F2C_F16: return 2;
+    case F2C_I16: case F2C_F16: case F2C_BF16: return 2;
     case F2C_I32: case F2C_F32: return 4;
     default: return 8;
   }
 }
+static inline bool is_float_dtype(int dt) { return dt == F2C_F32 || dt == F2C_F16 || dt == F2C_BF16; }
 static inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -119,6 +121,15 @@ __device__ __forceinline__ uint4 ldg_nc_u128(const void* p) {
 __device__ __forceinline__ void stg_cs_f4(float* p, float4 v) {
   asm volatile("st.global.cs.v4.f32 [%0], {%1,%2,%3,%4};" :: "l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
+
+// Values of the floating-point types as single precision, and back (round to even).
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // SQ decode of one element.  The expression is the reference's, term by term
 // (src/sq_quantization.cu:137-152 == src/fusion_spmm.cu:199-223), compiled with the same default

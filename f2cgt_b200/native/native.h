@@ -42,6 +42,7 @@ inline int dtype_tag(at::ScalarType t) {
     case at::kHalf: return F2C_F16;
     case at::kFloat: return F2C_F32;
     case at::kDouble: return F2C_F64;
+    case at::kBFloat16: return F2C_BF16;
     default: return -1;
   }
 }
@@ -113,7 +114,7 @@ inline auto unlocked(F&& body) {
 }
 
 
-extern PyMethodDef g_sage_methods[], g_loader_methods[];  // sage.cpp, loader.cpp
+extern PyMethodDef g_sage_methods[], g_loader_methods[], g_dense_methods[];  // sage.cpp, loader.cpp, dense.cpp
 
 void arguments(const char* name, Py_ssize_t got, Py_ssize_t want);
 

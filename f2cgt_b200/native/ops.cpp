@@ -268,7 +268,7 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods
 
 PyMODINIT_FUNC PyInit__native(void) {
   PyObject* m = PyModule_Create(&f2c_native::g_module);
-  for (PyMethodDef* more : {f2c_native::g_sage_methods, f2c_native::g_loader_methods})
+  for (PyMethodDef* more : {f2c_native::g_sage_methods, f2c_native::g_loader_methods, f2c_native::g_dense_methods})
     if (m != nullptr && PyModule_AddFunctions(m, more) != 0) Py_CLEAR(m);
   return m;
 }

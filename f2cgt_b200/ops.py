@@ -324,6 +324,47 @@ def dropout_inplace(output, p, is_training, seed=None, offset=0, scale=False):
     return output
 
 
+# ------------------------------------------------------------------ 8-bit products
+def int8_quantize(x, x2=None):
+    """Rows to int8: ``(codes, scales)`` with ``scale = max|row| / 127`` and ``code = round-to-even(value / scale)``, both in single
+    precision.  ``x``: float32 / float16 / bfloat16 [m, k] with contiguous rows; ``x2``: more columns of the same rows (one scale for
+    both).  The codes' rows start on 16-byte boundaries, where ``int8_mm`` reads them in place.  Used on activations per row
+    (token, node) and on a Linear weight [out, in] per output channel.  A zero row has scale 0; one with a NaN or an infinity scale NaN."""
+    return _native.int8_quantize(x, x2)
+
+
+def int8_mm(codes, scales, w_codes, w_scales, bias=None, relu=False, out_dtype=torch.float32):
+    """``act(scales[:, None] * w_scales * (codes @ w_codes.T) + bias)``: int8 [m, k] and [n, k], float32 scales and bias, an exact
+    integer sum (k <= 131071), float32 / float16 / bfloat16 [m, n] out, rounded once."""
+    return _native.int8_mm(codes, scales, w_codes, w_scales, bias, relu, out_dtype)
+
+
+def int8_linear(x, w_codes, w_scales, bias=None, relu=False, x2=None, out_dtype=None):
+    """``int8_mm(*int8_quantize(x, x2), w_codes, w_scales, bias, relu)`` in one call; the result has the dtype of ``x`` unless
+    ``out_dtype`` says otherwise.  With ``x2`` it is a whole SAGE layer (examples/conv.py:62-76): own rows and neighbours' means side
+    by side against ``fc_self | fc_neigh``.  For answering with trained weights: there is no gradient."""
+    return _native.int8_linear(x, x2, w_codes, w_scales, bias, relu, out_dtype)
+
+
+# ------------------------------------------------------------------ orthogonalised updates
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # quintic of Jordan et al., Muon (2024): singular values to about 0.7 .. 1.2 in five steps
+
+
+def orthogonalize(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, out=None):
+    """Newton-Schulz steps on every matrix of ``g`` [..., rows, cols] (float32 / float16 / bfloat16, contiguous): from
+    ``X = G / (|G| + eps)``, ``X <- (a I + b A + c A^2) X`` with ``A = X X^T`` - singular values go to one, singular vectors stay.
+    ``coefficients``: (a, b, c), or one such triple for every step.  ``out`` may be ``g``.  Sums and norms are held in 32 bits or
+    more, float32 matrices to about 22 bits throughout, 16-bit ones to 11 or more."""
+    return _native.orthogonalize(g, steps, coefficients, eps, out)
+
+
+def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """One step of Muon (momentum, orthogonalised update) over lists of matrices, in place: ``m <- momentum m + g``,
+    ``u = g + momentum m`` (``nesterov``) or ``m``, ``w <- w (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u)``.
+    Weights and gradients float32 / float16 / bfloat16 (one dtype), momenta float32; call under ``torch.no_grad()``."""
+    _native.muon_step(weights, grads, momenta, lr, momentum, nesterov, weight_decay, steps, coefficients, eps)
+
+
 # ------------------------------------------------------------------ k-means
 def pairwise_distance(x, y, metric):
     """src/kmeans.cu:102-118.  x [n,d], y [k,d] fp32 -> [n,k] squared-L2 or cosine distance."""

@@ -35,7 +35,8 @@ extern "C" {
 #endif
 
 typedef enum {
-  F2C_U8 = 0, F2C_I8 = 1, F2C_I16 = 2, F2C_I32 = 3, F2C_I64 = 4, F2C_F16 = 5, F2C_F32 = 6, F2C_F64 = 7
+  F2C_U8 = 0, F2C_I8 = 1, F2C_I16 = 2, F2C_I32 = 3, F2C_I64 = 4, F2C_F16 = 5, F2C_F32 = 6, F2C_F64 = 7,
+  F2C_BF16 = 8   /* the 8-bit products and the orthogonalised updates only */
 } f2c_dtype;
 
 typedef enum { F2C_MEAN = 0, F2C_SUM = 1 } f2c_reduce;   /* the reference only has mean */
@@ -398,6 +399,53 @@ typedef struct {
 } f2c_minibatch;
 int64_t f2c_sample_minibatch_workspace(int64_t n_nodes, int64_t n_seeds, int n_hops, const int* num_pick_host);
 int f2c_sample_minibatch(const f2c_minibatch* args, void* stream);
+
+/* ---- 8-bit products: the Linear layers of a trained network (fc_self, fc_neigh of examples/conv.py:62-76) in int8 ----
+ * Codes and scale of a row x of floating-point numbers: scale = max|x| / 127, code = round-to-even(x / scale), both quotients in
+ * single precision.  A row of zeros has scale 0 and codes 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so
+ * what is computed from it is NaN.
+ * f2c_int8_quantize: rows are the k1 columns of x1 followed by the k2 columns of x2 (x2 NULL and k2 0: x1 alone), dtype F32, F16
+ * or BF16, row strides ld1, ld2 in elements; codes [m, k1 + k2] with row stride ldq in bytes (a multiple of 16 and a 16-byte aligned
+ * start let f2c_int8_mm read them where they are; bytes between the columns and ldq are left as they are), scales [m]. */
+int f2c_int8_quantize(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, int64_t m,
+                      int8_t* codes, int64_t ldq, float* scales, void* stream);
+/* out [m, n] = act(scales[i] * w_scales[j] * sum_t codes[i, t] w[j, t] + bias[j]); codes [m, k] and w [n, k] int8 with row strides
+ * ldq, ldw, out F32, F16 or BF16, rounded once, bias [n] float or NULL, relu != 0: negative values become 0 (a NaN stays one).
+ * The sum is exact (int32), k <= 131071.  workspace: f2c_int8_mm_workspace(...) bytes, 256-byte aligned; 0 where both operands
+ * start on 16 bytes and their row strides are multiples of 16. */
+int64_t f2c_int8_mm_workspace(const int8_t* codes, int64_t ldq, const int8_t* w, int64_t ldw, int64_t m, int64_t n, int64_t k);
+int f2c_int8_mm(const int8_t* codes, int64_t ldq, const float* scales, const int8_t* w, int64_t ldw, const float* w_scales,
+                const float* bias, int relu, void* out, int out_dtype, int64_t m, int64_t n, int64_t k, void* workspace,
+                int64_t workspace_bytes, void* stream);
+/* f2c_int8_quantize and f2c_int8_mm in one call; out has the dtype of the rows unless out_dtype says otherwise. */
+int64_t f2c_int8_linear_workspace(const int8_t* w, int64_t ldw, int64_t m, int64_t n, int64_t k);
+int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, const int8_t* w,
+                    int64_t ldw, const float* w_scales, const float* bias, int relu, void* out, int out_dtype, int64_t m, int64_t n,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- orthogonalised updates of weight matrices (beside Adam, examples/train_graphsage_nodeclass.py:56) ----
+ * Newton-Schulz steps: X = G / (|G|_F + eps), then for every step's coefficients (a, b, c): X <- (a I + b A + c A^2) X, A = X X^T
+ * (for more rows than columns the transposed matrix is meant).  coefficients_host: 3 * steps floats.  Refused are coefficients under
+ * which a singular value could leave [0, 7.9] or a factor a + b s^2 + c s^4 the range of magnitude 60: values are held in half
+ * precision (pairs of it where more is needed).  Matrices that hold a NaN or an infinity become NaN.
+ * f2c_orthogonalize: g and out [batch, rows, cols], dtype F32, F16 or BF16; out may be g.
+ * f2c_muon_step: for every matrix of the list  m <- momentum m + g;  u = nesterov ? g + momentum m : m;
+ *   w <- w (1 - lr decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u),  in place; w and g of `dtype` (F32, F16 or BF16), m float.
+ *   The list (host memory) is read during the call.  Matrices of one step must not overlap.
+ * workspace: the bytes that the _workspace function names, 256-byte aligned. */
+typedef struct {
+  void* weight;
+  const void* grad;
+  float* momentum;
+  int64_t rows, cols;
+} f2c_muon_matrix;
+#define F2C_MAX_NS_STEPS 16
+int64_t f2c_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t cols);
+int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t batch, int64_t rows, int64_t cols, const float* coefficients_host,
+                      int steps, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int count, int dtype);
+int f2c_muon_step(const f2c_muon_matrix* list_host, int count, int dtype, float lr, float momentum, int nesterov, float decay,
+                  const float* coefficients_host, int steps, float eps, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
