@@ -1,55 +1,247 @@
-// out [m, n] = act(s[i] ws[j] sum_t q[i, t] w[j, t] + b[j]) in 8-bit integers (f2c_int8_mm, f2c_int8_linear).
+// out [m, n] = act(s[i] ws[j] sum_t q[i, t] w[j, t] + b[j]) in 8-bit integers on the 5th-generation tensor cores (f2c_int8_mm,
+// f2c_int8_linear).
 //
-// One 64 x 64 tile of the output per CTA, 16 columns of both operands in shared memory at a time, four-element dot products.
+// A tile of the product has 128 channels (rows of w, the lanes of TMEM) and up to 256 rows of q (its columns), whatever m: the weights are
+// what few rows have to read, and they fill the MMA's 128 rows; an epilogue thread has one channel, whose scale and bias stay in
+// registers, and a warp writes 32 neighbouring channels of a row of out without staging them.  128 columns of K come per step with TMA
+// (128-byte swizzle, zeros behind the operands' edges) through a ring of stages; the int32 accumulators of two tiles alternate in TMEM.
+//  * Rows per tile: so many that the tiles of one round over the SMs have equal work (see plan()).
+//  * Short K and few channel tiles: a CTA keeps its channels' weights in shared memory and only the rows travel.
+//  * Few tiles and a long K: the CTAs of a cluster each take a part of K and add their sums over distributed shared memory, which is exact
+//    and in any order the same.
+// Every wait is bounded: when one runs out the CTA's roles all leave, what it has not finished becomes NaN, copies and products in flight are
+// waited for, the error word is raised and TMEM is freed.
 #include "int8_mm.cuh"
+#include "tcgen05.cuh"
 
 namespace f2c {
 namespace i8 {
 
-constexpr int kTile = 64, kStep = 16, kThreads = 256;
+using namespace t5;
+
+constexpr int kThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
+constexpr int kM = 128, kK = 128, kMaxN = 256;
+constexpr int kABytes = kM * kK;
+constexpr int kMaxStages = 12;
+constexpr size_t kRoom = kSmemLimit - 8192;  // dynamic shared memory: what barriers and scales leave, less the alignment of its start
 
 struct Params {
-  const int8_t *a, *b;
-  int64_t lda, ldb;
   const float *a_scales, *b_scales, *bias;
   void* out;
-  int64_t m, n, k;
-  int relu;
+  int64_t m;
+  int n, steps;             // steps of K
+  int channel_tiles, tile_rows, items;
+  int stages, resident, split, relu;
+  int weights_first;        // the kernel before this one does not make the weights
+  int* error;
+};
+
+struct Bars {
+  uint64_t full[kMaxStages], empty[kMaxStages], weights, drain, acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int failed;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) mm_kernel(const Params p) {
-  dependency_wait();
-  release_dependents();
-  __shared__ __align__(16) int8_t as[kTile][kStep + 4], bs[kTile][kStep + 4];
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
-  const int64_t row0 = (int64_t)blockIdx.x * kTile, col0 = (int64_t)blockIdx.y * kTile;
-  int acc[4][4] = {};
-  for (int64_t t0 = 0; t0 < p.k; t0 += kStep) {
-    for (int e = tid; e < kTile * kStep; e += kThreads) {
-      const int r = e / kStep, t = e % kStep;
-      const bool in = t0 + t < p.k;
-      as[r][t] = in && row0 + r < p.m ? p.a[(row0 + r) * p.lda + t0 + t] : 0;
-      bs[r][t] = in && col0 + r < p.n ? p.b[(col0 + r) * p.ldb + t0 + t] : 0;
+__global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ CUtensorMap w, const Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ Bars bars;
+  __shared__ __align__(16) float scales_s[4][kMaxN];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const int rank = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, stride = (int)gridDim.x / p.split;
+  const int step0 = (int)((int64_t)p.steps * rank / p.split), steps = (int)((int64_t)p.steps * (rank + 1) / p.split) - step0;
+  const uint32_t b_bytes = (uint32_t)p.tile_rows * kK;
+  unsigned char* ring = smem + (p.resident ? (size_t)steps * kABytes : 0);
+  const uint32_t stage_bytes = b_bytes + (p.resident ? 0u : (uint32_t)kABytes);
+  volatile int* failed = &bars.failed;
+
+  if (wid == 1) alloc_tmem(&bars.tmem);
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) { init_bar(bars.full + s, 1); init_bar(bars.empty + s, 1); }
+    init_bar(&bars.weights, 1);
+    init_bar(&bars.drain, 1);
+    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, 4); }
+    fence_bars();
+    bars.failed = 0;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = bars.tmem;
+  int s = 0;
+  uint32_t round = 0;
+
+  if (wid == 0) {
+    // ================= loads
+    if (lane == 0) {
+      prefetch_map(&codes);
+      prefetch_map(&w);
+      if (!p.weights_first) dependency_wait();
+      int ahead = 0;  // stages whose weights have been asked for
+      if (p.resident) {
+        expect(&bars.weights, (uint32_t)steps * kABytes);
+        for (int i = 0; i < steps; ++i) tma_load(&w, smem_u32(smem + (size_t)i * kABytes), &bars.weights, (step0 + i) * kK, first % p.channel_tiles * kM);
+      } else if (p.weights_first) {
+        for (; ahead < min(p.stages, steps); ++ahead) {
+          expect(bars.full + ahead, stage_bytes);
+          tma_load(&w, smem_u32(ring + (size_t)ahead * stage_bytes), bars.full + ahead, (step0 + ahead) * kK, first % p.channel_tiles * kM);
+        }
+      }
+      if (p.weights_first) dependency_wait();
+      release_dependents();
+      for (int item = first; item < p.items; item += stride) {
+        const int channel0 = item % p.channel_tiles * kM, row0 = item / p.channel_tiles * p.tile_rows;
+        for (int i = 0; i < steps; ++i) {
+          if (round > 0 && !wait_bar(bars.empty + s, (round - 1) & 1, failed)) { item = p.items; break; }
+          unsigned char* stage = ring + (size_t)s * stage_bytes;
+          const bool asked = round == 0 && s < ahead;
+          if (!asked) expect(bars.full + s, stage_bytes);
+          if (!asked && !p.resident) tma_load(&w, smem_u32(stage), bars.full + s, (step0 + i) * kK, channel0);
+          tma_load(&codes, smem_u32(stage + (p.resident ? 0 : kABytes)), bars.full + s, (step0 + i) * kK, row0);
+          if (++s == p.stages) { s = 0; ++round; }
+        }
+        if (item >= p.items) break;
+      }
     }
-    __syncthreads();
+  } else if (wid == 1) {
+    // ================= MMAs
+    if (lane == 0) {
+      const uint32_t idesc = instruction(kSumS32, kFormatS8, kM, (uint32_t)p.tile_rows);
+      bool ok = !p.resident || wait_bar(&bars.weights, 0, failed);
+      uint32_t t = 0;
+      for (int item = first; ok && item < p.items; item += stride, ++t) {
+        const uint32_t buf = t & 1u;
+        if (t >= 2) ok = wait_bar(bars.acc_empty + buf, ((t >> 1) - 1) & 1, failed);
+        fence_after();
+        for (int i = 0; ok && i < steps; ++i) {
+          ok = wait_bar(bars.full + s, round & 1, failed);
+          if (!ok) break;
+          fence_after();
+          const uint32_t stage = smem_u32(ring + (size_t)s * stage_bytes);
+          const uint32_t a_addr = p.resident ? smem_u32(smem + (size_t)i * kABytes) : stage;
+          const uint32_t b_addr = p.resident ? stage : stage + kABytes;
 #pragma unroll
-    for (int q = 0; q < kStep; q += 4)
+          for (int q = 0; q < kK / 32; ++q) mma_i8(tmem + buf * kMaxN, desc_k(a_addr + q * 32), desc_k(b_addr + q * 32), idesc, i + q != 0 ? 1u : 0u);
+          commit(bars.empty + s);
+          if (++s == p.stages) { s = 0; ++round; }
+        }
+        if (ok) commit(bars.acc_full + buf);
+      }
+    }
+  } else {
+    // ================= epilogue: warp w owns the TMEM lanes of its quarter, thread = channel
+    const int quarter = wid & 3;
+    float* row_scale = scales_s[quarter];
+    uint32_t t = 0;
+    dependency_wait();
+    for (int item = first; item < p.items; item += stride, ++t) {
+      const uint32_t buf = t & 1u;
+      const int channel = item % p.channel_tiles * kM + quarter * 32 + lane;
+      const int64_t row0 = (int64_t)(item / p.channel_tiles) * p.tile_rows;
+      const int rows = (int)min((int64_t)p.tile_rows, p.m - row0);
+      const bool mine = channel < p.n;
+      const float w_scale = mine ? __ldg(p.b_scales + channel) : 0.0f, bias = mine && p.bias != nullptr ? __ldg(p.bias + channel) : 0.0f;
+      for (int c = lane; c < rows; c += 32) row_scale[c] = __ldg(p.a_scales + row0 + c);
+      __syncwarp();
+      const bool lost = steps > 0 && !__all_sync(0xffffffffu, wait_bar(bars.acc_full + buf, (t >> 1) & 1, failed));
+      fence_after();
+      const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kMaxN;
+      if (p.split > 1) {
+        // the ring is free: this CTA's sums go there, [row][channel]
+        uint32_t* part = reinterpret_cast<uint32_t*>(smem);
+        for (int c0 = 0; c0 < rows; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld32(at + (uint32_t)c0, r);
+          tmem_wait(r);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < rows) part[(c0 + j) * kM + quarter * 32 + lane] = r[j];
+        }
+        break;
+      }
+      T* out = (T*)p.out + row0 * p.n + channel;
+      for (int c0 = 0; c0 < rows; c0 += 32) {
+        uint32_t r[32];
+        if (steps > 0) {
+          tmem_ld32(at + (uint32_t)c0, r);
+          tmem_wait(r);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __dp4a(*reinterpret_cast<const int*>(&as[ty + 16 * i][q]), *reinterpret_cast<const int*>(&bs[tx + 16 * j][q]), acc[i][j]);
+          for (int j = 0; j < 32; ++j) r[j] = 0u;
+        }
+        if (c0 + 32 >= rows) {  // the accumulators have been read
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(bars.acc_empty + buf);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          float v = fmaf((float)(int)r[j], row_scale[c0 + j] * w_scale, bias);
+          if (p.relu && v <= 0.0f) v = 0.0f;  // a NaN stays one, as in torch.relu
+          if (lost) v = __int_as_float(0x7fffffff);
+          if (mine && c0 + j < rows) out[(int64_t)(c0 + j) * p.n] = from_float<T>(v);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  if (p.split > 1) {
+    // a cluster has one tile; its CTAs share the rows
+    __syncwarp();
+    cluster_barrier();
+    bool lost = false;
+    for (int q = 0; q < p.split; ++q) lost |= peer_u32(peer_address(smem_u32(&bars.failed), (uint32_t)q)) != 0u;
+    if (wid >= 2) {
+      const int quarter = wid & 3, channel = first % p.channel_tiles * kM + quarter * 32 + lane;
+      const int64_t row0 = (int64_t)(first / p.channel_tiles) * p.tile_rows;
+      const int rows = (int)min((int64_t)p.tile_rows, p.m - row0);
+      const bool mine = channel < p.n;
+      const float w_scale = mine ? __ldg(p.b_scales + channel) : 0.0f, bias = mine && p.bias != nullptr ? __ldg(p.bias + channel) : 0.0f;
+      const float* row_scale = scales_s[quarter];
+      const uint32_t part = smem_u32(smem) + 4u * (uint32_t)(quarter * 32 + lane);
+      for (int c = rank; c < rows; c += p.split) {
+        int sum = 0;
+        for (int q = 0; q < p.split; ++q) sum += (int)peer_u32(peer_address(part + (uint32_t)c * (4u * kM), (uint32_t)q));
+        float v = fmaf((float)sum, row_scale[c] * w_scale, bias);
+        if (p.relu && v <= 0.0f) v = 0.0f;
+        if (lost) v = __int_as_float(0x7fffffff);
+        if (mine) ((T*)p.out)[(row0 + c) * p.n + channel] = from_float<T>(v);
+      }
+    }
+    __syncwarp();
+    cluster_barrier();  // nobody's shared memory goes while another reads it
+  }
+  fence_before();
+  __syncthreads();
+  if (bars.failed) {
+    // copies in flight write to this CTA's shared memory, MMAs in flight read it and write its TMEM: wait (bounded) for what was issued
+    volatile int expired = 0;
+    if (tid == 0) {
+      if (p.resident) wait_bar(&bars.weights, 0, &expired);
+      for (int q = 0; q < p.stages; ++q) {
+        const uint32_t uses = round + (q < s ? 1u : 0u);
+        if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, &expired);
+      }
+    } else if (tid == 32) {
+      commit(&bars.drain);
+      wait_bar(&bars.drain, 0, &expired);
+    }
     __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = row0 + ty + 16 * i, c = col0 + tx + 16 * j;
-      if (r >= p.m || c >= p.n) continue;
-      float v = (float)acc[i][j] * (p.a_scales[r] * p.b_scales[c]);
-      if (p.bias != nullptr) v += p.bias[c];
-      ((T*)p.out)[r * p.n + c] = from_float<T>(p.relu && v <= 0.0f ? 0.0f : v);
-    }
+  if (wid == 1) {
+    fence_after();
+    free_tmem(tmem);
+  }
+  if (tid == 0 && bars.failed) report_wait(p.error, 4);
+}
+
+// Copies codes to rows that start on 16 bytes.
+__global__ void __launch_bounds__(256) align_kernel(const int8_t* __restrict__ src, int64_t ld, int64_t k, int8_t* __restrict__ dst, int64_t aligned_ld, int64_t rows) {
+  dependency_wait();
+  release_dependents();
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
+    for (int64_t t = threadIdx.x; t < k; t += 256) dst[row * aligned_ld + t] = src[row * ld + t];
 }
 
 static int check(const char* op, int64_t m, int64_t n, int64_t k, int out_dtype) {
@@ -60,21 +252,111 @@ static int check(const char* op, int64_t m, int64_t n, int64_t k, int out_dtype)
   return F2C_OK;
 }
 
-static int mm(const char* op, const Params& p, int out_dtype, cudaStream_t st) {
-  const dim3 grid((unsigned)ceil_div(p.m, kTile), (unsigned)ceil_div(p.n, kTile));
-  auto* kern = out_dtype == F2C_F32 ? mm_kernel<float> : out_dtype == F2C_F16 ? mm_kernel<__half> : mm_kernel<__nv_bfloat16>;
-  launch_dependent(kern, grid, kThreads, 0, st, p);
-  return check_launch(op);
+static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+static int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }
+static bool in_place(const int8_t* p, int64_t ld, int64_t rows) { return aligned(p, 16) && (rows <= 1 || ld % 16 == 0); }
+
+struct Operand {
+  const int8_t* p;
+  int64_t ld, rows;
+};
+
+// The operand where TMA can read it: its own memory, or a copy in the workspace (which moves on).
+static Operand readable(const Operand& o, int64_t k, char*& ws, cudaStream_t st) {
+  const int64_t ld = round16(k);
+  if (k == 0 || in_place(o.p, o.ld, o.rows)) return Operand{o.p, o.rows > 1 ? o.ld : ld, o.rows};
+  int8_t* copy = (int8_t*)ws;
+  ws += round256(o.rows * ld);
+  launch_dependent(align_kernel, dim3((unsigned)(o.rows < 4096 ? o.rows : 4096)), 256, 0, st, o.p, o.ld, k, copy, ld, o.rows);
+  return Operand{copy, ld, o.rows};
 }
 
-static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+struct Plan {
+  int channel_tiles, tile_rows, items, steps, split, resident, stages;
+  unsigned grid;
+  size_t smem;
+};
+
+static_assert(sizeof(Bars) + 4 * kMaxN * 4 + 256 <= 8192, "static shared memory");
+
+static Plan plan(int64_t m, int64_t n, int64_t k, int sms) {
+  Plan p{};
+  p.channel_tiles = (int)ceil_div(n, kM);
+  p.steps = (int)ceil_div(k, kK);
+  p.split = 1;
+  // Rows per tile: with r rounds over the SMs that one channel tile gets, ceil(m / (r SMs)) rows to the next 16; the r of least work,
+  // a tile counted as 32 rows more than it has.
+  const int64_t per = sms >= p.channel_tiles ? sms / p.channel_tiles : 1;
+  int64_t least = 0;
+  for (int64_t r = ceil_div(m, per * kMaxN), last = r + 3; r <= last; ++r) {
+    const int64_t rows = round16(ceil_div(m, per * r));
+    const int64_t work = r * (rows + 32);
+    if (least == 0 || work < least) {
+      least = work;
+      p.tile_rows = (int)rows;
+    }
+  }
+  const int64_t row_tiles = ceil_div(m, p.tile_rows);
+  const int64_t items = row_tiles * p.channel_tiles;
+  p.items = (int)items;
+  const size_t room = kRoom - 1024;
+  const size_t b_bytes = (size_t)p.tile_rows * kK, weights = (size_t)p.steps * kABytes;
+  if (items < sms && p.steps > 1) {
+    // parts of K of at least two steps, as long as there are SMs for them
+    while (p.split < 8 && items * p.split * 2 <= sms && p.steps >= p.split * 4) p.split *= 2;
+  }
+  int64_t clusters = items;
+  if (p.split == 1 && items > sms) clusters = sms;
+  if (p.split == 1 && sms >= p.channel_tiles && weights + 4 * b_bytes <= room) {
+    p.resident = 1;
+    const int64_t whole = (int64_t)sms / p.channel_tiles * p.channel_tiles;  // a CTA stays with its channels
+    if (clusters > whole) clusters = whole;
+  }
+  const size_t stage = b_bytes + (p.resident ? 0 : kABytes), fixed = p.resident ? weights : 0;
+  p.stages = (int)((room - fixed) / stage);
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.smem = fixed + p.stages * stage + 1024;
+  const size_t parts = p.split > 1 ? (size_t)p.tile_rows * kM * 4 + 1024 : 0;
+  if (p.smem < parts) p.smem = parts;
+  if (p.smem < 120 * 1024) p.smem = 120 * 1024;  // one CTA per SM: it owns all of TMEM
+  p.grid = (unsigned)(clusters * p.split);
+  return p;
+}
+
+struct Job {
+  Operand a, b;
+  const float *a_scales, *b_scales, *bias;
+  void* out;
+  int64_t k;
+  int relu, out_dtype, weights_first;
+};
+
+static int mm(const char* op, const Job& j, cudaStream_t st) {
+  const Plan pl = plan(j.a.rows, j.b.rows, j.k, current_sm_count());
+  CUtensorMap maps[2] = {};
+  if (j.k > 0) {
+    const bool ok = make_map(maps, j.a.p, 1, j.a.rows, j.k, j.a.ld, pl.tile_rows) && make_map(maps + 1, j.b.p, 1, j.b.rows, j.k, j.b.ld, kM);
+    F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
+  }
+  Params p{j.a_scales, j.b_scales, j.bias, j.out, j.a.rows, (int)j.b.rows, pl.steps, pl.channel_tiles, pl.tile_rows, pl.items,
+           pl.stages, pl.resident, pl.split, j.relu, j.weights_first, stream_error_word()};
+  auto* kern = j.out_dtype == F2C_F32 ? mm_kernel<float> : j.out_dtype == F2C_F16 ? mm_kernel<__half> : mm_kernel<__nv_bfloat16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRoom);
+  if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  launch_dependent_cluster(kern, dim3(pl.grid), kThreads, pl.smem, (unsigned)pl.split, st, maps[0], maps[1], p);
+  return check_launch(op);
+}
 
 }  // namespace i8
 }  // namespace f2c
 
 using namespace f2c;
 
-extern "C" int64_t f2c_int8_mm_workspace(const int8_t*, int64_t, const int8_t*, int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t f2c_int8_mm_workspace(const int8_t* codes, int64_t ldq, const int8_t* w, int64_t ldw, int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || n < 1 || k < 1) return 0;
+  const int64_t ld = i8::round16(k);
+  return (i8::in_place(codes, ldq, m) ? 0 : i8::round256(m * ld)) + (i8::in_place(w, ldw, n) ? 0 : i8::round256(n * ld));
+}
 
 extern "C" int f2c_int8_mm(const int8_t* codes, int64_t ldq, const float* scales, const int8_t* w, int64_t ldw, const float* w_scales,
                            const float* bias, int relu, void* out, int out_dtype, int64_t m, int64_t n, int64_t k, void* workspace,
@@ -84,11 +366,22 @@ extern "C" int f2c_int8_mm(const int8_t* codes, int64_t ldq, const float* scales
   F2C_REQUIRE((m <= 1 || ldq >= k) && (n <= 1 || ldw >= k), F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
   if (m == 0 || n == 0) return F2C_OK;
   F2C_REQUIRE(out && scales && w_scales && (k == 0 || (codes && w)), F2C_ERR_INVALID, "%s: null pointer", op);
-  return i8::mm(op, i8::Params{codes, w, ldq, ldw, scales, w_scales, bias, out, m, n, k, relu}, out_dtype, (cudaStream_t)stream);
+  const int64_t need = f2c_int8_mm_workspace(codes, ldq, w, ldw, m, n, k);
+  F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,
+              "%s: workspace too small or not 256-byte aligned", op);
+  cudaStream_t st = (cudaStream_t)stream;
+  char* ws = (char*)workspace;
+  i8::Job j{};
+  j.a = i8::readable(i8::Operand{codes, ldq, m}, k, ws, st);
+  j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);
+  j.a_scales = scales; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype;
+  return i8::mm(op, j, st);
 }
 
-extern "C" int64_t f2c_int8_linear_workspace(const int8_t*, int64_t, int64_t m, int64_t, int64_t k) {
-  return m < 0 || k < 0 ? 0 : i8::round256(4 * m) + m * ((k + 15) / 16 * 16);
+extern "C" int64_t f2c_int8_linear_workspace(const int8_t* w, int64_t ldw, int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || n < 1 || k < 0) return 0;
+  const int64_t ld = i8::round16(k);
+  return i8::round256(4 * m) + i8::round256(m * ld) + (k == 0 || i8::in_place(w, ldw, n) ? 0 : i8::round256(n * ld));
 }
 
 extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, const int8_t* w,
@@ -104,9 +397,17 @@ extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const vo
   F2C_REQUIRE(out && w_scales && (k == 0 || w), F2C_ERR_INVALID, "%s: null pointer", op);
   F2C_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= f2c_int8_linear_workspace(w, ldw, m, n, k), F2C_ERR_INVALID,
               "%s: workspace too small or not 256-byte aligned", op);
-  float* scales = (float*)workspace;
-  int8_t* codes = (int8_t*)workspace + i8::round256(4 * m);
-  const int64_t ldq = (k + 15) / 16 * 16;
-  if (const int rc = i8::quantize(r, codes, ldq, scales, (cudaStream_t)stream)) return rc;
-  return i8::mm(op, i8::Params{codes, w, ldq, ldw, scales, w_scales, bias, out, m, n, k, relu}, out_dtype, (cudaStream_t)stream);
+  cudaStream_t st = (cudaStream_t)stream;
+  char* ws = (char*)workspace;
+  float* scales = (float*)ws;
+  ws += i8::round256(4 * m);
+  int8_t* codes = (int8_t*)ws;
+  const int64_t ldq = i8::round16(k);
+  ws += i8::round256(m * ldq);
+  i8::Job j{};
+  j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);  // before the rows: the product may then ask for weights while these are encoded
+  if (const int rc = i8::quantize(r, codes, ldq, scales, st)) return rc;
+  j.a = i8::Operand{codes, ldq, m};
+  j.a_scales = scales; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype; j.weights_first = 1;
+  return i8::mm(op, j, st);
 }
