@@ -19,11 +19,11 @@ namespace i8 {
 
 using namespace t5;
 
-constexpr int kThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
+constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: MMA, then the epilogue's
 constexpr int kM = 128, kK = 128, kMaxN = 256;
 constexpr int kABytes = kM * kK;
 constexpr int kMaxStages = 12;
-constexpr size_t kRoom = kSmemLimit - 8192;  // dynamic shared memory: what barriers and scales leave, less the alignment of its start
+constexpr size_t kRoom = kSmemLimit - 10240;  // dynamic shared memory: what barriers and scales leave, less the alignment of its start
 
 struct Params {
   const float *a_scales, *b_scales, *bias;
@@ -42,11 +42,37 @@ struct Bars {
   int failed;
 };
 
+// scale * sum + bias, not below `floor`; a NaN stays one
+__device__ __forceinline__ float finish(int sum, float scale, float bias, float floor) {
+  const float v = fmaf((float)sum, scale, bias);
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(floor));
+  return r;
+}
+
+// One channel of 32 rows of out, `rows` of which exist.
+template <typename T>
+__device__ __forceinline__ void store_rows(T* out, int64_t ld, const uint32_t (&r)[32], const float* row_scale, float w_scale, float bias, float floor, int rows) {
+  if (rows >= 32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(row_scale + j);
+      const float of[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e, out += ld) *out = from_float<T>(finish((int)r[j + e], of[e] * w_scale, bias, floor));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j, out += ld)
+      if (j < rows) *out = from_float<T>(finish((int)r[j], row_scale[j] * w_scale, bias, floor));
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ CUtensorMap w, const Params p) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
-  __shared__ __align__(16) float scales_s[4][kMaxN];
+  __shared__ __align__(16) float scales_s[kEpilogueWarps][kMaxN];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
   const int rank = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, stride = (int)gridDim.x / p.split;
@@ -61,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
     for (int s = 0; s < p.stages; ++s) { init_bar(bars.full + s, 1); init_bar(bars.empty + s, 1); }
     init_bar(&bars.weights, 1);
     init_bar(&bars.drain, 1);
-    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, 4); }
+    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps); }
     fence_bars();
     bars.failed = 0;
   }
@@ -130,9 +156,10 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
       }
     }
   } else {
-    // ================= epilogue: warp w owns the TMEM lanes of its quarter, thread = channel
-    const int quarter = wid & 3;
-    float* row_scale = scales_s[quarter];
+    // ================= epilogue: a warp has the TMEM lanes of its quarter and every other 32 rows of the tile, thread = channel
+    const int quarter = wid & 3, half = (wid - 2) >> 2;
+    float* row_scale = scales_s[wid - 2];
+    const float floor = p.relu ? 0.0f : __int_as_float(0xff800000);
     uint32_t t = 0;
     dependency_wait();
     for (int item = first; item < p.items; item += stride, ++t) {
@@ -147,21 +174,8 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
       const bool lost = steps > 0 && !__all_sync(0xffffffffu, wait_bar(bars.acc_full + buf, (t >> 1) & 1, failed));
       fence_after();
       const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kMaxN;
-      if (p.split > 1) {
-        // the ring is free: this CTA's sums go there, [row][channel]
-        uint32_t* part = reinterpret_cast<uint32_t*>(smem);
-        for (int c0 = 0; c0 < rows; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld32(at + (uint32_t)c0, r);
-          tmem_wait(r);
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c0 + j < rows) part[(c0 + j) * kM + quarter * 32 + lane] = r[j];
-        }
-        break;
-      }
-      T* out = (T*)p.out + row0 * p.n + channel;
-      for (int c0 = 0; c0 < rows; c0 += 32) {
+      uint32_t* part = reinterpret_cast<uint32_t*>(smem) + quarter * 32 + lane;  // split: the ring is free, this CTA's sums go there, [row][channel]
+      for (int c0 = half * 32; c0 < rows; c0 += 64) {
         uint32_t r[32];
         if (steps > 0) {
           tmem_ld32(at + (uint32_t)c0, r);
@@ -170,20 +184,19 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = 0u;
         }
-        if (c0 + 32 >= rows) {  // the accumulators have been read
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive(bars.acc_empty + buf);
-        }
+        if (p.split > 1) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          float v = fmaf((float)(int)r[j], row_scale[c0 + j] * w_scale, bias);
-          if (p.relu && v <= 0.0f) v = 0.0f;  // a NaN stays one, as in torch.relu
-          if (lost) v = __int_as_float(0x7fffffff);
-          if (mine && c0 + j < rows) out[(int64_t)(c0 + j) * p.n] = from_float<T>(v);
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < rows) part[(c0 + j) * kM] = r[j];
+        } else if (mine) {
+          store_rows((T*)p.out + (row0 + c0) * p.n + channel, (int64_t)p.n, r, row_scale + c0, w_scale, lost ? __int_as_float(0x7fffffff) : bias, floor, rows - c0);
         }
         __syncwarp();
       }
+      // the accumulators have been read
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(bars.acc_empty + buf);
     }
   }
   if (p.split > 1) {
@@ -193,20 +206,18 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
     bool lost = false;
     for (int q = 0; q < p.split; ++q) lost |= peer_u32(peer_address(smem_u32(&bars.failed), (uint32_t)q)) != 0u;
     if (wid >= 2) {
-      const int quarter = wid & 3, channel = first % p.channel_tiles * kM + quarter * 32 + lane;
+      const int quarter = wid & 3, half = (wid - 2) >> 2, channel = first % p.channel_tiles * kM + quarter * 32 + lane;
       const int64_t row0 = (int64_t)(first / p.channel_tiles) * p.tile_rows;
       const int rows = (int)min((int64_t)p.tile_rows, p.m - row0);
       const bool mine = channel < p.n;
-      const float w_scale = mine ? __ldg(p.b_scales + channel) : 0.0f, bias = mine && p.bias != nullptr ? __ldg(p.bias + channel) : 0.0f;
-      const float* row_scale = scales_s[quarter];
+      const float w_scale = mine ? __ldg(p.b_scales + channel) : 0.0f;
+      const float bias = lost ? __int_as_float(0x7fffffff) : mine && p.bias != nullptr ? __ldg(p.bias + channel) : 0.0f;
+      const float floor = p.relu ? 0.0f : __int_as_float(0xff800000);
       const uint32_t part = smem_u32(smem) + 4u * (uint32_t)(quarter * 32 + lane);
-      for (int c = rank; c < rows; c += p.split) {
+      for (int c = 2 * rank + half; c < rows; c += 2 * p.split) {
         int sum = 0;
         for (int q = 0; q < p.split; ++q) sum += (int)peer_u32(peer_address(part + (uint32_t)c * (4u * kM), (uint32_t)q));
-        float v = fmaf((float)sum, row_scale[c] * w_scale, bias);
-        if (p.relu && v <= 0.0f) v = 0.0f;
-        if (lost) v = __int_as_float(0x7fffffff);
-        if (mine) ((T*)p.out)[(row0 + c) * p.n + channel] = from_float<T>(v);
+        if (mine) ((T*)p.out)[(row0 + c) * p.n + channel] = from_float<T>(finish(sum, scales_s[wid - 2][c] * w_scale, bias, floor));
       }
     }
     __syncwarp();
@@ -277,7 +288,7 @@ struct Plan {
   size_t smem;
 };
 
-static_assert(sizeof(Bars) + 4 * kMaxN * 4 + 256 <= 8192, "static shared memory");
+static_assert(sizeof(Bars) + kEpilogueWarps * kMaxN * 4 + 256 <= 10240, "static shared memory");
 
 static Plan plan(int64_t m, int64_t n, int64_t k, int sms) {
   Plan p{};
