@@ -2,6 +2,7 @@
 #include <stddef.h>
 
 #include <mutex>
+#include <vector>
 
 #include "common.cuh"
 #include "stream_pipe.cuh"
@@ -44,6 +45,26 @@ int current_sm_count() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
   return sm_count(dev);
+}
+
+int allow_smem(const char* what, const void* kernel, int bytes) {
+  struct Known { const void* kernel; int device, bytes; };
+  static std::mutex mu;
+  static std::vector<Known> known;
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  if (e == cudaSuccess) {
+    for (const Known& k : known)
+      if (k.kernel == kernel && k.device == dev && k.bytes == bytes) return F2C_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  }
+  if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  try {
+    known.push_back(Known{kernel, dev, bytes});
+  } catch (...) {  // asked again next time
+  }
+  return F2C_OK;
 }
 
 // The record that kernels with bounded waits raise when a wait runs out; one per device (it lives in the device image).

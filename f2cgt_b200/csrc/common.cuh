@@ -20,6 +20,8 @@ int set_error(int status, const char* fmt, ...);
 int check_launch(const char* what);
 int sm_count(int device);  // multiprocessors of `device` (queried once per device)
 int current_sm_count();     // the same for the current device
+// Lets `kernel` have that much dynamic shared memory on the current device (asked of the runtime once).
+int allow_smem(const char* what, const void* kernel, int bytes);
 
 #define F2C_REQUIRE(cond, status, ...)                 \
   do {                                                 \

@@ -12,17 +12,12 @@
 // Every wait is bounded: when one runs out the CTA's roles all leave, what it has not finished becomes NaN, copies and products in flight are
 // waited for, the error word is raised and TMEM is freed.
 #include "int8_mm.cuh"
-#include "tcgen05.cuh"
 
 namespace f2c {
 namespace i8 {
 
-using namespace t5;
-
 constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: MMA, then the epilogue's
-constexpr int kM = 128, kK = 128, kMaxN = 256;
-constexpr int kABytes = kM * kK;
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 12, kMaxSplit = 8;
 constexpr size_t kRoom = kSmemLimit - 10240;  // dynamic shared memory: what barriers and scales leave, less the alignment of its start
 
 struct Params {
@@ -32,6 +27,8 @@ struct Params {
   int n, steps;             // steps of K
   int channel_tiles, tile_rows, items;
   int stages, resident, split, relu;
+  int tmem, accumulators;   // columns of an accumulator, and how many
+  int parts_at, share_log;  // clusters: where the sums are in shared memory, and of how many rows
   int weights_first;        // the kernel before this one does not make the weights
   int* error;
 };
@@ -39,37 +36,11 @@ struct Params {
 struct Bars {
   uint64_t full[kMaxStages], empty[kMaxStages], weights, drain, acc_full[2], acc_empty[2];
   uint32_t tmem;
-  int failed;
+  int failed, lost;  // lost: of any CTA of the cluster
 };
 
-// scale * sum + bias, not below `floor`; a NaN stays one
-__device__ __forceinline__ float finish(int sum, float scale, float bias, float floor) {
-  const float v = fmaf((float)sum, scale, bias);
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(floor));
-  return r;
-}
-
-// One channel of 32 rows of out, `rows` of which exist.
 template <typename T>
-__device__ __forceinline__ void store_rows(T* out, int64_t ld, const uint32_t (&r)[32], const float* row_scale, float w_scale, float bias, float floor, int rows) {
-  if (rows >= 32) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 s = *reinterpret_cast<const float4*>(row_scale + j);
-      const float of[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e, out += ld) *out = from_float<T>(finish((int)r[j + e], of[e] * w_scale, bias, floor));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j, out += ld)
-      if (j < rows) *out = from_float<T>(finish((int)r[j], row_scale[j] * w_scale, bias, floor));
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ CUtensorMap w, const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ CUtensorMap w, const Params p) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
   __shared__ __align__(16) float scales_s[kEpilogueWarps][kMaxN];
@@ -82,7 +53,7 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
   const uint32_t stage_bytes = b_bytes + (p.resident ? 0u : (uint32_t)kABytes);
   volatile int* failed = &bars.failed;
 
-  if (wid == 1) alloc_tmem(&bars.tmem);
+  if (wid == 1) alloc_tmem(&bars.tmem, (uint32_t)p.tmem * p.accumulators);
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) { init_bar(bars.full + s, 1); init_bar(bars.empty + s, 1); }
     init_bar(&bars.weights, 1);
@@ -90,11 +61,15 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
     for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps); }
     fence_bars();
     bars.failed = 0;
+    bars.lost = 0;
   }
   fence_before();
   __syncthreads();
   fence_after();
+  if (p.split > 1) cluster_barrier();  // all are here before the first tells another its sums
   const uint32_t tmem = bars.tmem;
+  const int share = 1 << p.share_log;  // rows whose sums a CTA of a cluster adds up
+  const uint32_t parts = smem_u32(smem) + (uint32_t)p.parts_at;
   int s = 0;
   uint32_t round = 0;
 
@@ -148,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
           const uint32_t a_addr = p.resident ? smem_u32(smem + (size_t)i * kABytes) : stage;
           const uint32_t b_addr = p.resident ? stage : stage + kABytes;
 #pragma unroll
-          for (int q = 0; q < kK / 32; ++q) mma_i8(tmem + buf * kMaxN, desc_k(a_addr + q * 32), desc_k(b_addr + q * 32), idesc, i + q != 0 ? 1u : 0u);
+          for (int q = 0; q < kK / 32; ++q) mma_i8(tmem + buf * (uint32_t)p.tmem, desc_k(a_addr + q * 32), desc_k(b_addr + q * 32), idesc, i + q != 0 ? 1u : 0u);
           commit(bars.empty + s);
           if (++s == p.stages) { s = 0; ++round; }
         }
@@ -173,8 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
       __syncwarp();
       const bool lost = steps > 0 && !__all_sync(0xffffffffu, wait_bar(bars.acc_full + buf, (t >> 1) & 1, failed));
       fence_after();
-      const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kMaxN;
-      uint32_t* part = reinterpret_cast<uint32_t*>(smem) + quarter * 32 + lane;  // split: the ring is free, this CTA's sums go there, [row][channel]
+      const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)p.tmem;
       for (int c0 = half * 32; c0 < rows; c0 += 64) {
         uint32_t r[32];
         if (steps > 0) {
@@ -185,14 +159,17 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
           for (int j = 0; j < 32; ++j) r[j] = 0u;
         }
         if (p.split > 1) {
+          // row c goes to CTA c / share, there [this CTA][c % share][channel]
+          const uint32_t to = parts + 4u * (uint32_t)(rank * share * kM + quarter * 32 + lane);
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (c0 + j < rows) part[(c0 + j) * kM] = r[j];
+            if (c0 + j < rows) peer_store(peer_address(to + (uint32_t)((c0 + j) & (share - 1)) * (4u * kM), (uint32_t)(c0 + j) >> p.share_log), r[j]);
         } else if (mine) {
           store_rows((T*)p.out + (row0 + c0) * p.n + channel, (int64_t)p.n, r, row_scale + c0, w_scale, lost ? __int_as_float(0x7fffffff) : bias, floor, rows - c0);
         }
         __syncwarp();
       }
+      if (p.split > 1 && lost && lane < p.split) peer_store(peer_address(smem_u32(&bars.lost), (uint32_t)lane), 1u);
       // the accumulators have been read
       fence_before();
       __syncwarp();
@@ -200,28 +177,29 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
     }
   }
   if (p.split > 1) {
-    // a cluster has one tile; its CTAs share the rows
+    // a cluster has one tile, whose rows its CTAs share: all sums have been told when all have got here
     __syncwarp();
     cluster_barrier();
-    bool lost = false;
-    for (int q = 0; q < p.split; ++q) lost |= peer_u32(peer_address(smem_u32(&bars.failed), (uint32_t)q)) != 0u;
     if (wid >= 2) {
       const int quarter = wid & 3, half = (wid - 2) >> 2, channel = first % p.channel_tiles * kM + quarter * 32 + lane;
       const int64_t row0 = (int64_t)(first / p.channel_tiles) * p.tile_rows;
       const int rows = (int)min((int64_t)p.tile_rows, p.m - row0);
       const bool mine = channel < p.n;
       const float w_scale = mine ? __ldg(p.b_scales + channel) : 0.0f;
-      const float bias = lost ? __int_as_float(0x7fffffff) : mine && p.bias != nullptr ? __ldg(p.bias + channel) : 0.0f;
+      const float bias = bars.lost ? __int_as_float(0x7fffffff) : mine && p.bias != nullptr ? __ldg(p.bias + channel) : 0.0f;
       const float floor = p.relu ? 0.0f : __int_as_float(0xff800000);
-      const uint32_t part = smem_u32(smem) + 4u * (uint32_t)(quarter * 32 + lane);
-      for (int c = 2 * rank + half; c < rows; c += 2 * p.split) {
+      const int* part = reinterpret_cast<const int*>(smem + p.parts_at) + quarter * 32 + lane;
+#pragma unroll 2
+      for (int i = half; i < share; i += 2) {
+        const int c = rank * share + i;
+        if (c >= rows) break;
         int sum = 0;
-        for (int q = 0; q < p.split; ++q) sum += (int)peer_u32(peer_address(part + (uint32_t)c * (4u * kM), (uint32_t)q));
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; ++q)
+          if (q < p.split) sum += part[(q * share + i) * kM];
         if (mine) ((T*)p.out)[(row0 + c) * p.n + channel] = from_float<T>(finish(sum, scales_s[wid - 2][c] * w_scale, bias, floor));
       }
     }
-    __syncwarp();
-    cluster_barrier();  // nobody's shared memory goes while another reads it
   }
   fence_before();
   __syncthreads();
@@ -242,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) mm_kernel(const __grid_constant__
   }
   if (wid == 1) {
     fence_after();
-    free_tmem(tmem);
+    free_tmem(tmem, (uint32_t)p.tmem * p.accumulators);
   }
   if (tid == 0 && bars.failed) report_wait(p.error, 4);
 }
@@ -255,25 +233,8 @@ __global__ void __launch_bounds__(256) align_kernel(const int8_t* __restrict__ s
     for (int64_t t = threadIdx.x; t < k; t += 256) dst[row * aligned_ld + t] = src[row * ld + t];
 }
 
-static int check(const char* op, int64_t m, int64_t n, int64_t k, int out_dtype) {
-  F2C_REQUIRE(m >= 0 && n >= 0 && k >= 0, F2C_ERR_INVALID, "%s: negative size", op);
-  F2C_REQUIRE(is_float_dtype(out_dtype), F2C_ERR_UNSUPPORTED, "%s: the output must be float32, float16 or bfloat16", op);
-  F2C_REQUIRE(k <= kMaxK, F2C_ERR_LIMIT, "%s: more than %d columns", op, kMaxK);
-  F2C_REQUIRE(m <= kMaxRows && n <= (1 << 21), F2C_ERR_LIMIT, "%s: too many rows", op);
-  return F2C_OK;
-}
-
-static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
-static int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }
-static bool in_place(const int8_t* p, int64_t ld, int64_t rows) { return aligned(p, 16) && (rows <= 1 || ld % 16 == 0); }
-
-struct Operand {
-  const int8_t* p;
-  int64_t ld, rows;
-};
-
 // The operand where TMA can read it: its own memory, or a copy in the workspace (which moves on).
-static Operand readable(const Operand& o, int64_t k, char*& ws, cudaStream_t st) {
+Operand readable(const Operand& o, int64_t k, char*& ws, cudaStream_t st) {
   const int64_t ld = round16(k);
   if (k == 0 || in_place(o.p, o.ld, o.rows)) return Operand{o.p, o.rows > 1 ? o.ld : ld, o.rows};
   int8_t* copy = (int8_t*)ws;
@@ -282,40 +243,46 @@ static Operand readable(const Operand& o, int64_t k, char*& ws, cudaStream_t st)
   return Operand{copy, ld, o.rows};
 }
 
-struct Plan {
-  int channel_tiles, tile_rows, items, steps, split, resident, stages;
-  unsigned grid;
-  size_t smem;
-};
-
 static_assert(sizeof(Bars) + kEpilogueWarps * kMaxN * 4 + 256 <= 10240, "static shared memory");
 
-static Plan plan(int64_t m, int64_t n, int64_t k, int sms) {
+int check(const char* op, int64_t m, int64_t n, int64_t k, int out_dtype) {
+  F2C_REQUIRE(m >= 0 && n >= 0 && k >= 0, F2C_ERR_INVALID, "%s: negative size", op);
+  F2C_REQUIRE(is_float_dtype(out_dtype), F2C_ERR_UNSUPPORTED, "%s: the output must be float32, float16 or bfloat16", op);
+  F2C_REQUIRE(k <= kMaxK, F2C_ERR_LIMIT, "%s: more than %d columns", op, kMaxK);
+  F2C_REQUIRE(m <= kMaxRows && n <= (1 << 21), F2C_ERR_LIMIT, "%s: too many rows", op);
+  return F2C_OK;
+}
+
+Plan plan(int64_t m, int64_t n, int64_t k, int sms) {
   Plan p{};
   p.channel_tiles = (int)ceil_div(n, kM);
   p.steps = (int)ceil_div(k, kK);
-  p.split = 1;
-  // Rows per tile: with r rounds over the SMs that one channel tile gets, ceil(m / (r SMs)) rows to the next 16; the r of least work,
-  // a tile counted as 32 rows more than it has.
-  const int64_t per = sms >= p.channel_tiles ? sms / p.channel_tiles : 1;
+  // Rows per tile and parts of K: the pair of least cycles.  A step of K takes the longer of its bytes at 56 a cycle (what an SM was seen
+  // to get from L2 with all others at it) and its MMAs; the results 12 cycles a row, beside the next tile's steps; a tile 1000 more;
+  // the exchange between the parts of K 2000 and 16 a row.  (59,000 x 128 x 256: 9.2 us with 256 rows, 10.0 with 96, 11.6 with 64; 2000 x 1000 x 500:
+  // 5.5 us with 128, 6.5 with 64, 6.4 with 256.)
+  const size_t room = kRoom - 1024, weights = (size_t)p.steps * kABytes;
   int64_t least = 0;
-  for (int64_t r = ceil_div(m, per * kMaxN), last = r + 3; r <= last; ++r) {
-    const int64_t rows = round16(ceil_div(m, per * r));
-    const int64_t work = r * (rows + 32);
-    if (least == 0 || work < least) {
-      least = work;
-      p.tile_rows = (int)rows;
+  for (const int rows : {16, 32, 64, 128, 192, 256}) {
+    if (rows == 16 && m > 16) continue;  // as many steps for the weights as 32
+    const int64_t items = ceil_div(m, rows) * p.channel_tiles;
+    for (int split = 1; split <= kMaxSplit; split *= 2) {
+      if (split > 1 && (items * split > sms || p.steps < 2 * split || rows == 192)) break;
+      const int64_t rounds = ceil_div(items * split, sms), steps = ceil_div(p.steps, split);
+      const bool resident = split == 1 && sms >= p.channel_tiles && weights + 4 * rows * kK <= room;
+      const int64_t bytes = rows * kK + (resident ? 0 : kABytes), step = bytes / 56 > 2 * rows ? bytes / 56 : 2 * rows;
+      const int64_t tile = steps * step > 12 * rows ? steps * step : 12 * rows;
+      const int64_t cycles = rounds * (tile + 1000) + 12 * rows + (resident ? (int64_t)weights / 56 : 0) + (split > 1 ? 2000 + 16 * rows : 0);
+      if (least != 0 && cycles >= least) continue;
+      least = cycles;
+      p.tile_rows = rows;
+      p.split = split;
     }
+    if (rows >= m) break;
   }
-  const int64_t row_tiles = ceil_div(m, p.tile_rows);
-  const int64_t items = row_tiles * p.channel_tiles;
+  const int64_t items = ceil_div(m, p.tile_rows) * p.channel_tiles;
   p.items = (int)items;
-  const size_t room = kRoom - 1024;
-  const size_t b_bytes = (size_t)p.tile_rows * kK, weights = (size_t)p.steps * kABytes;
-  if (items < sms && p.steps > 1) {
-    // parts of K of at least two steps, as long as there are SMs for them
-    while (p.split < 8 && items * p.split * 2 <= sms && p.steps >= p.split * 4) p.split *= 2;
-  }
+  const size_t b_bytes = (size_t)p.tile_rows * kK;
   int64_t clusters = items;
   if (p.split == 1 && items > sms) clusters = sms;
   if (p.split == 1 && sms >= p.channel_tiles && weights + 4 * b_bytes <= room) {
@@ -323,26 +290,22 @@ static Plan plan(int64_t m, int64_t n, int64_t k, int sms) {
     const int64_t whole = (int64_t)sms / p.channel_tiles * p.channel_tiles;  // a CTA stays with its channels
     if (clusters > whole) clusters = whole;
   }
-  const size_t stage = b_bytes + (p.resident ? 0 : kABytes), fixed = p.resident ? weights : 0;
+  p.grid = (unsigned)(clusters * p.split);
+  p.tmem = 32;
+  while (p.tmem < p.tile_rows) p.tmem *= 2;
+  const size_t parts = p.split > 1 ? (size_t)p.tile_rows * kM * 4 : 0;
+  const size_t stage = b_bytes + (p.resident ? 0 : kABytes), fixed = (p.resident ? weights : 0) + parts;
+  const int64_t most = p.rounds() * ceil_div(p.steps, p.split);
   p.stages = (int)((room - fixed) / stage);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
+  if (p.stages > most) p.stages = (int)(most > 0 ? most : 1);
+  p.parts_at = (int)(p.stages * stage);  // (never resident)
+  while ((p.split << p.share_log) < p.tile_rows) ++p.share_log;
   p.smem = fixed + p.stages * stage + 1024;
-  const size_t parts = p.split > 1 ? (size_t)p.tile_rows * kM * 4 + 1024 : 0;
-  if (p.smem < parts) p.smem = parts;
-  if (p.smem < 120 * 1024) p.smem = 120 * 1024;  // one CTA per SM: it owns all of TMEM
-  p.grid = (unsigned)(clusters * p.split);
   return p;
 }
 
-struct Job {
-  Operand a, b;
-  const float *a_scales, *b_scales, *bias;
-  void* out;
-  int64_t k;
-  int relu, out_dtype, weights_first;
-};
-
-static int mm(const char* op, const Job& j, cudaStream_t st) {
+int mm(const char* op, const Job& j, cudaStream_t st) {
   const Plan pl = plan(j.a.rows, j.b.rows, j.k, current_sm_count());
   CUtensorMap maps[2] = {};
   if (j.k > 0) {
@@ -350,10 +313,9 @@ static int mm(const char* op, const Job& j, cudaStream_t st) {
     F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
   }
   Params p{j.a_scales, j.b_scales, j.bias, j.out, j.a.rows, (int)j.b.rows, pl.steps, pl.channel_tiles, pl.tile_rows, pl.items,
-           pl.stages, pl.resident, pl.split, j.relu, j.weights_first, stream_error_word()};
+           pl.stages, pl.resident, pl.split, j.relu, pl.tmem, pl.rounds() > 1 ? 2 : 1, pl.parts_at, pl.share_log, j.weights_first, stream_error_word()};
   auto* kern = j.out_dtype == F2C_F32 ? mm_kernel<float> : j.out_dtype == F2C_F16 ? mm_kernel<__half> : mm_kernel<__nv_bfloat16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRoom);
-  if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom)) return rc;
   launch_dependent_cluster(kern, dim3(pl.grid), kThreads, pl.smem, (unsigned)pl.split, st, maps[0], maps[1], p);
   return check_launch(op);
 }
@@ -386,13 +348,16 @@ extern "C" int f2c_int8_mm(const int8_t* codes, int64_t ldq, const float* scales
   j.a = i8::readable(i8::Operand{codes, ldq, m}, k, ws, st);
   j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);
   j.a_scales = scales; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype;
+  if (i8::is_few(m, n, k)) return i8::few(op, i8::Rows{j.a.p, nullptr, j.a.ld, 0, k, 0, m, F2C_I8}, j, st);
   return i8::mm(op, j, st);
 }
 
-extern "C" int64_t f2c_int8_linear_workspace(const int8_t* w, int64_t ldw, int64_t m, int64_t n, int64_t k) {
-  if (m < 1 || n < 1 || k < 0) return 0;
-  const int64_t ld = i8::round16(k);
-  return i8::round256(4 * m) + i8::round256(m * ld) + (k == 0 || i8::in_place(w, ldw, n) ? 0 : i8::round256(n * ld));
+extern "C" int64_t f2c_int8_linear_workspace(int64_t k1, int64_t k2, int dtype, const int8_t* w, int64_t ldw, int64_t m, int64_t n) {
+  const int64_t k = k1 + k2, ld = i8::round16(k);
+  if (m < 1 || n < 1 || k < 0 || k > i8::kMaxK) return 0;
+  const i8::Rows r{nullptr, nullptr, k1, k2, k1, k2, m, dtype};
+  const int64_t rows = i8::few_encodes(r, n) ? 0 : i8::round256(4 * m) + i8::round256(m * ld);
+  return rows + (k == 0 || i8::in_place(w, ldw, n) ? 0 : i8::round256(n * ld));
 }
 
 extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, const int8_t* w,
@@ -406,19 +371,26 @@ extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const vo
   F2C_REQUIRE(n <= 1 || ldw >= k, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
   if (m == 0 || n == 0) return F2C_OK;
   F2C_REQUIRE(out && w_scales && (k == 0 || w), F2C_ERR_INVALID, "%s: null pointer", op);
-  F2C_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= f2c_int8_linear_workspace(w, ldw, m, n, k), F2C_ERR_INVALID,
+  const int64_t need = f2c_int8_linear_workspace(k1, k2, dtype, w, ldw, m, n);
+  F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,
               "%s: workspace too small or not 256-byte aligned", op);
   cudaStream_t st = (cudaStream_t)stream;
   char* ws = (char*)workspace;
+  i8::Job j{};
+  j.a_scales = nullptr; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype;
+  if (i8::few_encodes(r, n)) {
+    j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);
+    return i8::few(op, r, j, st);
+  }
   float* scales = (float*)ws;
   ws += i8::round256(4 * m);
   int8_t* codes = (int8_t*)ws;
   const int64_t ldq = i8::round16(k);
   ws += i8::round256(m * ldq);
-  i8::Job j{};
   j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);  // before the rows: the product may then ask for weights while these are encoded
   if (const int rc = i8::quantize(r, codes, ldq, scales, st)) return rc;
   j.a = i8::Operand{codes, ldq, m};
-  j.a_scales = scales; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype; j.weights_first = 1;
+  j.a_scales = scales; j.weights_first = 1;
+  if (i8::is_few(m, n, k)) return i8::few(op, i8::Rows{codes, nullptr, ldq, 0, k, 0, m, F2C_I8}, j, st);
   return i8::mm(op, j, st);
 }

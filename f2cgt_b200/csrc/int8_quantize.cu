@@ -9,123 +9,76 @@
 namespace f2c {
 namespace i8q {
 
-constexpr int kThreads = 256, kKept = 4;  // vectors of a row that a thread keeps
+constexpr int kThreads = 256;
 
-template <int BYTES> struct Raw;
-template <> struct Raw<16> { using type = uint4; };
-template <> struct Raw<4> { using type = uint32_t; };
-template <> struct Raw<2> { using type = uint16_t; };
-template <int BYTES> struct Out;
-template <> struct Out<8> { using type = uint2; };
-template <> struct Out<4> { using type = uint32_t; };
-template <> struct Out<2> { using type = uint16_t; };
-template <> struct Out<1> { using type = uint8_t; };
-
-// BYTES of T's, V of them
-template <typename T, int BYTES>
-struct Vector {
-  static constexpr int V = BYTES / (int)sizeof(T);
-  using R = typename Raw<BYTES>::type;
-  union { R raw; T v[V]; };
-  __device__ __forceinline__ Vector() : raw() {}
-};
-
-// The code of v, in the low byte.  inv 0: divide.
-__device__ __forceinline__ uint32_t code_of(float v, float scale, float inv) {
-  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to even and leaves the integer in the low bits
-  const float t = v * inv, shifted = t + kRound;
-  uint32_t code = __float_as_uint(shifted);
-  if (inv == 0.0f || fabsf(t - (shifted - kRound)) > 0.4999f)
-    code = __float_as_uint(fminf(fmaxf(rintf(__fdiv_rn(v, scale)), -127.0f), 127.0f) + kRound);
-  return code & 0xffu;
-}
-
-template <typename T, int BYTES, int THREADS>
+// THREADS per row, of whose vectors each keeps KEPT
+template <typename T, int BYTES, int THREADS, int KEPT>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const i8::Rows r, int8_t* __restrict__ codes, int64_t ldq, float* __restrict__ scales) {
-  using Vec = Vector<T, BYTES>;
+  using Vec = i8::Vector<T, BYTES>;
+  using R = typename i8::Words<BYTES>::type;
   constexpr int V = Vec::V;
-  using O = typename Out<V>::type;
   dependency_wait();
   release_dependents();
   const int at = threadIdx.x % THREADS;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / THREADS) + threadIdx.x / THREADS;
   if (row >= r.m) return;  // all threads of a warp
   const int n1 = (int)(r.k1 / V), n = n1 + (int)(r.k2 / V);
-  const typename Vec::R* x1 = reinterpret_cast<const typename Vec::R*>((const T*)r.x1 + row * r.ld1);
-  const typename Vec::R* x2 = reinterpret_cast<const typename Vec::R*>((const T*)r.x2 + row * r.ld2) - n1;
+  const R* x1 = reinterpret_cast<const R*>((const T*)r.x1 + row * r.ld1);
+  const R* x2 = reinterpret_cast<const R*>((const T*)r.x2 + row * r.ld2) - n1;
   auto read = [&](int i) {
     Vec v;
     v.raw = __ldg(i < n1 ? x1 + i : x2 + i);
     return v;
   };
-  float top = 0.0f;
-  bool bad = false;
+  i8::Largest<T> part;
   auto look = [&](const Vec& v) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float a = fabsf(to_float(v.v[e]));
-      bad |= !(a <= 3.4028235e38f);
-      top = fmaxf(top, a);
-    }
+    for (int e = 0; e < Vec::W; ++e) part.add(v.w[e]);
   };
-  Vec kept[kKept];
+  Vec kept[KEPT];
 #pragma unroll
-  for (int q = 0; q < kKept; ++q)
+  for (int q = 0; q < KEPT; ++q)
     if (at + q * THREADS < n) kept[q] = read(at + q * THREADS);
 #pragma unroll
-  for (int q = 0; q < kKept; ++q) look(kept[q]);
-  for (int i = at + kKept * THREADS; i < n; i += THREADS) look(read(i));
-  uint32_t bits = bad ? 0xffffffffu : __float_as_uint(top);
-  bits = __reduce_max_sync(0xffffffffu, bits);
+  for (int q = 0; q < KEPT; ++q) look(kept[q]);
+  for (int i = at + KEPT * THREADS; i < n; i += THREADS) look(read(i));
+  uint32_t largest = __reduce_max_sync(0xffffffffu, part.of_float());
   if (THREADS > 32) {
     __shared__ uint32_t of_warp[kThreads / 32];
-    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = bits;
+    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = largest;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) bits = max(bits, of_warp[w]);
+    for (int w = 0; w < kThreads / 32; ++w) largest = max(largest, of_warp[w]);
   }
-  bad = bits == 0xffffffffu;
-  const float scale = bad ? __int_as_float(0x7fffffff) : __fdiv_rn(__uint_as_float(bits), 127.0f);
-  const bool zero = bad || scale == 0.0f;
-  const float inv = zero || scale < 1e-37f ? 0.0f : __frcp_rn(scale);  // (the reciprocal of less has no place, or few bits)
-  O* out = reinterpret_cast<O*>(codes + row * ldq);
-  auto write = [&](int i, const Vec& v) {
-    uint32_t word[V > 4 ? 2 : 1] = {};
-    if (!zero) {
+  const i8::Scale s = i8::scale_of(largest);
+  int8_t* out = codes + row * ldq;
 #pragma unroll
-      for (int e = 0; e < V; ++e) word[e / 4] |= code_of(to_float(v.v[e]), scale, inv) << (e % 4 * 8);
-    }
-    if constexpr (V == 8) out[i] = make_uint2(word[0], word[1]);
-    else out[i] = (O)word[0];
-  };
-#pragma unroll
-  for (int q = 0; q < kKept; ++q)
-    if (at + q * THREADS < n) write(at + q * THREADS, kept[q]);
-  for (int i = at + kKept * THREADS; i < n; i += THREADS) write(i, read(i));
-  if (at == 0) scales[row] = scale;
+  for (int q = 0; q < KEPT; ++q)
+    if (at + q * THREADS < n) i8::write<T, BYTES>(out + (at + q * THREADS) * V, kept[q], s);
+  for (int i = at + KEPT * THREADS; i < n; i += THREADS) i8::write<T, BYTES>(out + i * V, read(i), s);
+  if (at == 0) scales[row] = s.scale;
 }
 
 template <typename T, int BYTES>
 static void launch(const i8::Rows& r, int8_t* codes, int64_t ldq, float* scales, cudaStream_t st) {
-  if ((r.k1 + r.k2) * (int64_t)sizeof(T) > 32 * kKept * BYTES)
-    launch_dependent(quantize_kernel<T, BYTES, kThreads>, dim3((unsigned)r.m), kThreads, 0, st, r, codes, ldq, scales);
+  const int64_t vectors = (r.k1 + r.k2) * (int64_t)sizeof(T) / BYTES;
+  const dim3 warps((unsigned)ceil_div(r.m, kThreads / 32));
+  // A row up to 16 vectors a lane long is a warp's; where rows are few, one of more than two vectors a lane has a CTA.
+  if (vectors > 512 || (vectors > 64 && r.m < 1024))
+    launch_dependent(quantize_kernel<T, BYTES, kThreads, 4>, dim3((unsigned)r.m), kThreads, 0, st, r, codes, ldq, scales);
+  else if (vectors <= 64)
+    launch_dependent(quantize_kernel<T, BYTES, 32, 2>, warps, kThreads, 0, st, r, codes, ldq, scales);
+  else if (vectors <= 128)
+    launch_dependent(quantize_kernel<T, BYTES, 32, 4>, warps, kThreads, 0, st, r, codes, ldq, scales);
   else
-    launch_dependent(quantize_kernel<T, BYTES, 32>, dim3((unsigned)ceil_div(r.m, kThreads / 32)), kThreads, 0, st, r, codes, ldq, scales);
-}
-
-// Rows whose starts and lengths, and those of their codes, allow reads of `bytes`.
-template <typename T>
-static bool fits(const i8::Rows& r, const int8_t* codes, int64_t ldq, int bytes) {
-  const int64_t v = bytes / (int64_t)sizeof(T);
-  return aligned(r.x1, bytes) && aligned(r.x2, bytes) && aligned(codes, v) && r.k1 % v == 0 && r.k2 % v == 0 &&
-         (r.m <= 1 || (r.ld1 % v == 0 && r.ld2 % v == 0 && ldq % v == 0));
+    launch_dependent(quantize_kernel<T, BYTES, 32, 16>, warps, kThreads, 0, st, r, codes, ldq, scales);
 }
 
 template <typename T>
 static void any(const i8::Rows& r, int8_t* codes, int64_t ldq, float* scales, cudaStream_t st) {
-  if (fits<T>(r, codes, ldq, 16)) return launch<T, 16>(r, codes, ldq, scales, st);
+  if (r.fits(16, codes, ldq)) return launch<T, 16>(r, codes, ldq, scales, st);
   if constexpr (sizeof(T) == 2) {
-    if (!fits<T>(r, codes, ldq, 4)) return launch<T, 2>(r, codes, ldq, scales, st);
+    if (!r.fits(4, codes, ldq)) return launch<T, 2>(r, codes, ldq, scales, st);
   }
   launch<T, 4>(r, codes, ldq, scales, st);
 }

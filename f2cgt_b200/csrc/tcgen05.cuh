@@ -44,13 +44,14 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 // ordinary writes to shared memory, before copies and MMAs that read it
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// ---------------------------------------------------------------- TMEM (all 512 columns: one CTA per SM)
-__device__ __forceinline__ void alloc_tmem(uint32_t* at) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)), "r"(512u) : "memory");
+// ---------------------------------------------------------------- TMEM
+// `columns`: a power of two from 32 to 512.  Where the SM's other CTAs hold too many, the allocation waits for them: none of them waits for this one.
+__device__ __forceinline__ void alloc_tmem(uint32_t* at, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)), "r"(columns) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void free_tmem(uint32_t tmem) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+__device__ __forceinline__ void free_tmem(uint32_t tmem, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
 // 32 columns from `taddr` on, of the 32 lanes that the warp owns
@@ -118,11 +119,7 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t peer_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
+__device__ __forceinline__ void peer_store(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 
 // Tensor map of a row-major matrix [rows, cols] of `bytes`-byte elements (16-byte aligned start and row stride), boxes of box_rows x
 // 128 bytes with the 128-byte swizzle, zeros outside the matrix.  False when the driver refuses it.
