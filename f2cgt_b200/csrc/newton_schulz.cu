@@ -1,167 +1,694 @@
 // Newton-Schulz steps on stacks of matrices (f2c_orthogonalize) and the optimiser step around them (f2c_muon_step):
-//   X = G / (|G|_F + eps);   A = X X^T,  B = a I + b A + c A^2,  X <- B X   for every step.
+//   X = G / (|G|_F + eps);   A = X X^T,  R = b A + c A^2,  X <- a X + R X   for every step.
 //
-// Matrices with more rows than columns are worked on transposed.  Values, sums and norms in single precision, the norm's sum in double.
+// Products.  Three per step, on the 5th-generation tensor cores, one launch each (product_kernel).  A tile of a product has 128 rows (the
+// lanes of TMEM) and up to 256 columns.  A and A^2 are symmetric: tiles wholly below the diagonal are left out, what lies on or above it is written
+// twice.  Nothing is transposed in memory: an operand whose rows run along M or N instead of K is one that the MMA takes as it is, so a
+// matrix of more rows than columns, which is worked on transposed, is read the other way round.  The sums' factors, b A, a X and - in the
+// last step - the optimiser's update are the epilogue's.
+//
+// Precision.  Operands are half precision times a power of two for each matrix and step, chosen by a bound on the matrix' norm so that
+// the largest values stay a factor of 30 away from infinity and the smallest keep their bits; sums are single precision, the norm's double.
+//  * 16-bit matrices.  The first X is exact, A and R are rounded to 11 bits (R multiplies from the left: its rounding turns the singular
+//    vectors by 2^-12 of R's size).  X's own rounding is noise of full rank, which the following steps multiply by up to the product of their
+//    factors a, 3.4445^4 = 140 after the first, while large singular values only go to one: where that product is over 16, X is a pair of
+//    half precision numbers (22 bits) and R X two products.  For matrices of rank 8 the result is 2.6e-3 off then, and 2.6e-2 without.
+//  * 32-bit matrices.  All operands are pairs, a product is three (high by high, high by low, low by high): 22 bits throughout.  The tensor
+//    cores cut sums off instead of rounding them, for every 16 elements of K.  So the two small products have an accumulator of their own, the
+//    large one's sum is taken out every 128 elements and added up in registers, and a X is not in it.  (Rank 3, 400 x 600: 2.5e-4 off without
+//    any of this, 2e-4 without the taking out.)
 #include <math.h>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace f2c {
 namespace ns {
 
-constexpr int kThreads = 256, kTile = 64, kStep = 16, kParts = 64;
+using namespace t5;
 
-struct Source {     // what a matrix is read from, and what its result does
+constexpr int kParts = 64, kLoadThreads = 256;
+constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: MMA, then the epilogue's
+constexpr int kChunk = 2;                    // steps of K after which float32's sums are taken out of the tensor cores' hands
+constexpr int kM = 128, kK = 64, kMaxN = 256, kMaxStages = 8, kMaxList = 64;
+constexpr size_t kRoom = kSmemLimit - 1024;  // dynamic shared memory
+constexpr int kScaleLog = 10;                // norms are brought to 2^10
+
+// ---------------------------------------------------------------- what is read and written
+struct Matrices {  // of one shape: a stack, or a list
   const void* g;
-  void* out;        // orthogonalize: the result; muon: the weights
-  float* momentum;  // null: g is orthogonalised itself
-  float mu, keep, gain;  // w <- keep w - gain X
+  void* out;              // the result; optimiser: the weights
+  float* momentum;        // null: g is orthogonalised itself
+  f2c_muon_matrix list[kMaxList];
+  int listed;
+  int64_t size;           // elements of a matrix
+  float mu, keep, gain;   // w <- keep w - gain X
   int nesterov;
+  template <typename T> __device__ __forceinline__ const T* grad(int z) const { return listed ? (const T*)list[z].grad : (const T*)g + z * size; }
+  template <typename T> __device__ __forceinline__ T* result(int z) const { return listed ? (T*)list[z].weight : (T*)out + z * size; }
+  __device__ __forceinline__ float* moment(int z) const { return listed ? list[z].momentum : nullptr; }
 };
 
-// u of element i, and the momentum's update
-template <typename T>
-__device__ __forceinline__ float update(const Source& s, int64_t i) {
-  const float g = to_float(((const T*)s.g)[i]);
-  if (s.momentum == nullptr) return g;
-  const float m = fmaf(s.mu, s.momentum[i], g);
-  s.momentum[i] = m;
-  return s.nesterov ? fmaf(s.mu, m, g) : m;
+// Factors of a step, for a matrix.
+struct Factors {
+  float gram, poly_b, poly_c, apply, own;  // As = gram Xs Xs^T; Rs = poly_c As^2 + poly_b As; the next Xs = own Xs + apply Rs Xs
+};
+
+struct Steps {
+  int count;
+  float co[3 * F2C_MAX_NS_STEPS];
+  float top[F2C_MAX_NS_STEPS + 1];   // no singular value is larger in front of step t, if none was larger than one at first
+  float factor[F2C_MAX_NS_STEPS];    // and none is multiplied by more
+  float eps;
+};
+
+__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + min(max(e, -126), 127)) << 23); }
+// 2^e is the smallest power that is not below v > 0
+__device__ __forceinline__ int log2_above(float v) {
+  int e;
+  const float f = frexpf(v, &e);
+  return f == 0.5f ? e - 1 : e;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) load_kernel(const Source s, float* x, double* parts, int64_t rows, int64_t cols) {
+template <typename T, int V> struct alignas(V * sizeof(T)) Chunk { T v[V]; };
+
+// u of V elements from i on
+template <typename T, int V, bool UPDATE>
+__device__ __forceinline__ void direction(const Matrices& s, int z, int64_t i, float (&u)[V]) {
+  const Chunk<T, V> g = *reinterpret_cast<const Chunk<T, V>*>(s.template grad<T>(z) + i);
+  float* momentum = s.moment(z);
+  if (momentum == nullptr) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) u[e] = to_float(g.v[e]);
+    return;
+  }
+  Chunk<float, V> m = *reinterpret_cast<const Chunk<float, V>*>(momentum + i);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if (UPDATE) m.v[e] = fmaf(s.mu, m.v[e], to_float(g.v[e]));
+    u[e] = s.nesterov ? fmaf(s.mu, m.v[e], to_float(g.v[e])) : m.v[e];
+  }
+  if (UPDATE) *reinterpret_cast<Chunk<float, V>*>(momentum + i) = m;
+}
+
+// Momentum, and the squares' sums of kParts parts of every matrix.
+template <typename T, int V>
+__global__ void __launch_bounds__(kLoadThreads) norm_kernel(const __grid_constant__ Matrices s, double* parts) {
   dependency_wait();
   release_dependents();
-  const int64_t size = rows * cols, base = (int64_t)blockIdx.y * size;
+  const int z = blockIdx.y;
   double sum = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < size; i += (int64_t)kParts * kThreads) {
-    const float u = update<T>(s, base + i);
-    sum += (double)u * u;
-    x[base + (rows <= cols ? i : i % cols * rows + i / cols)] = u;
+  for (int64_t i = ((int64_t)blockIdx.x * kLoadThreads + threadIdx.x) * V; i < s.size; i += (int64_t)kParts * kLoadThreads * V) {
+    float u[V];
+    direction<T, V, true>(s, z, i, u);
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum = fma((double)u[e], (double)u[e], sum);
   }
-  __shared__ double sums[kThreads];
-  sums[threadIdx.x] = sum;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __shared__ double sums[kLoadThreads / 32];
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
   __syncthreads();
-  for (int o = kThreads / 2; o > 0; o >>= 1) {
-    if (threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-    __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kLoadThreads / 32; ++w) sum += sums[w];
+    parts[z * kParts + blockIdx.x] = sum;
   }
-  if (threadIdx.x == 0) parts[blockIdx.y * kParts + blockIdx.x] = sums[0];
 }
 
-__global__ void __launch_bounds__(kThreads) scale_kernel(float* x, const double* parts, int64_t size, float eps) {
+// X as half precision (and what that leaves, where `low` is given), and the steps' factors.
+template <typename T, int V>
+__global__ void __launch_bounds__(kLoadThreads) planes_kernel(const __grid_constant__ Matrices s, const __grid_constant__ Steps st, const double* parts,
+                                                              __half* high, __half* low, int64_t rows, int64_t cols, int64_t ld, Factors* table) {
   dependency_wait();
   release_dependents();
-  double sum = 0.0;
-  for (int i = 0; i < kParts; ++i) sum += parts[blockIdx.y * kParts + i];
-  // a matrix that is not finite becomes NaN
-  const float by = sum <= 1e300 ? (float)(1.0 / (sqrt(sum) + (double)eps)) : __int_as_float(0x7fffffff);
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < size; i += (int64_t)kParts * kThreads) x[blockIdx.y * size + i] *= by;
+  const int z = blockIdx.y;
+  __shared__ double norm_s;
+  if (threadIdx.x < 32) {
+    double sum = parts[z * kParts + threadIdx.x] + parts[z * kParts + 32 + threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x == 0) norm_s = sqrt(sum);
+  }
+  __syncthreads();
+  const double norm = norm_s;
+  const bool finite = norm <= 1e300;
+  int e = 0;
+  if (finite && norm > 0.0) (void)frexp(norm, &e);  // norm < 2^e
+  const int up = kScaleLog + 1 - e;
+  // u 2^up in two factors: the power itself may be out of range.  A matrix that is not finite becomes NaN.
+  const float by = power2(up / 2), more = finite ? power2(up - up / 2) : __int_as_float(0x7fffffff);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    float kappa = (float)(exp2((double)-up) / (norm + (double)st.eps));  // X = kappa Xs
+    float bound = (float)(norm / (norm + (double)st.eps));
+    for (int t = 0; t < st.count; ++t) {
+      const float a = st.co[3 * t], b = st.co[3 * t + 1], c = st.co[3 * t + 2];
+      const int lead = bound > 0.0f && bound <= 64.0f ? log2_above(bound) : 0;
+      const int a_log = min(kScaleLog - 2 * lead, 100);  // As = 2^a_log A
+      Factors f;
+      if (c != 0.0f) {
+        f.gram = power2(a_log) * kappa * kappa;
+        f.poly_b = b * power2(kScaleLog - a_log);
+        f.poly_c = c * power2(kScaleLog - a_log) * power2(-a_log);
+      } else {  // R itself
+        f.gram = b * power2(kScaleLog) * kappa * kappa;
+        f.poly_b = f.poly_c = 0.0f;
+      }
+      bound = fminf(st.top[t + 1], bound * st.factor[t]);
+      const bool last = t + 1 == st.count;
+      const float next = last ? 1.0f : power2((bound > 0.0f && bound <= 64.0f ? log2_above(bound) : 0) - kScaleLog);
+      f.apply = kappa * power2(-kScaleLog) / next;
+      f.own = a * (kappa / next);
+      kappa = next;
+      table[z * F2C_MAX_NS_STEPS + t] = f;
+    }
+    if (st.count == 0) table[z * F2C_MAX_NS_STEPS].apply = kappa;
+  }
+  __half* const hi = high + z * rows * ld;
+  __half* const lo = low + z * rows * ld;
+  for (int64_t i = ((int64_t)blockIdx.x * kLoadThreads + threadIdx.x) * V; i < s.size; i += (int64_t)gridDim.x * kLoadThreads * V) {
+    float u[V];
+    direction<T, V, false>(s, z, i, u);
+    const int64_t at = ld == cols ? i : i / cols * ld + i % cols;
+    Chunk<__half, V> h, l;
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+      const float v = u[q] * by * more;
+      h.v[q] = __float2half_rn(v);
+      l.v[q] = __float2half_rn(v - __half2float(h.v[q]));
+    }
+    *reinterpret_cast<Chunk<__half, V>*>(hi + at) = h;
+    if (low != nullptr) *reinterpret_cast<Chunk<__half, V>*>(lo + at) = l;
+  }
 }
 
-// D [p, q] = c L R + b C + a I with L [p, k] and R [k, q] (R given as [q, k] when turned)
-__global__ void __launch_bounds__(kThreads) product_kernel(const float* l, const float* r, const float* add, float* d, int p, int q, int k, int turned,
-                                                           float c, float b, float a) {
-  dependency_wait();
-  release_dependents();
-  __shared__ float ls[kStep][kTile + 1], rs[kStep][kTile + 1];
-  l += (int64_t)blockIdx.z * p * k;
-  r += (int64_t)blockIdx.z * q * k;
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16, row0 = blockIdx.x * kTile, col0 = blockIdx.y * kTile;
-  float acc[4][4] = {};
-  for (int t0 = 0; t0 < k; t0 += kStep) {
-    for (int e = tid; e < kTile * kStep; e += kThreads) {
-      const int x = e / kStep, t = e % kStep, y = e % kTile, u = e / kTile;
-      ls[t][x] = row0 + x < p && t0 + t < k ? l[(int64_t)(row0 + x) * k + t0 + t] : 0.0f;
-      if (turned) rs[t][x] = col0 + x < q && t0 + t < k ? r[(int64_t)(col0 + x) * k + t0 + t] : 0.0f;
-      else rs[u][y] = col0 + y < q && t0 + u < k ? r[(int64_t)(t0 + u) * q + col0 + y] : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < kStep; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(ls[t][ty + 16 * i], rs[t][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int x = row0 + ty + 16 * i, y = col0 + tx + 16 * j;
-      if (x >= p || y >= q) continue;
-      const int64_t at = ((int64_t)blockIdx.z * p + x) * q + y;
-      float v = c * acc[i][j];
-      if (add != nullptr) v += b * add[at];
-      d[at] = x == y ? v + a : v;
-    }
+// No steps: X itself is the result.
+template <typename T>
+__device__ __forceinline__ void finish(const Matrices& s, T* out, float x) {
+  *out = from_float<T>(s.listed ? s.keep * to_float(*out) - s.gain * x : x);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) store_kernel(const Source s, const float* x, int64_t rows, int64_t cols) {
+__global__ void __launch_bounds__(kLoadThreads) store_kernel(const __grid_constant__ Matrices s, const __half* high, const __half* low, int64_t rows, int64_t cols,
+                                                             int64_t ld, const Factors* table) {
   dependency_wait();
   release_dependents();
-  const int64_t size = rows * cols, base = (int64_t)blockIdx.y * size;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < size; i += (int64_t)kParts * kThreads) {
-    const float v = x[base + (rows <= cols ? i : i % cols * rows + i / cols)];
-    T* o = (T*)s.out + base + i;
-    *o = from_float<T>(s.momentum == nullptr ? v : s.keep * to_float(*o) - s.gain * v);
+  const int z = blockIdx.y;
+  const float kappa = table[z * F2C_MAX_NS_STEPS].apply;
+  for (int64_t i = (int64_t)blockIdx.x * kLoadThreads + threadIdx.x; i < s.size; i += (int64_t)gridDim.x * kLoadThreads) {
+    const int64_t at = z * rows * ld + i / cols * ld + i % cols;
+    finish(s, s.template result<T>(z) + i, kappa * (__half2float(high[at]) + (low != nullptr ? __half2float(low[at]) : 0.0f)));
   }
 }
 
+// ---------------------------------------------------------------- products
+enum Mode { kGram, kPoly, kApply, kFinal };
+
+struct Operand {
+  int rows;     // of a tile
+  int turned;   // its rows run along K
+  int planes;   // 1 or 2
+  __host__ __device__ int bytes() const { return rows * kK * 2; }
+};
+
+struct Params {
+  Operand a, b;
+  int m, n, steps;                 // M, N of the product; steps of K
+  int row_tiles, col_tiles, items; // row tiles along M; items of one matrix
+  int batch, stages, accumulators, tmem;  // accumulators: of 16-bit matrices; tmem: columns of one
+  int symmetric;
+  const Factors* factors;          // of this step
+  const __half *add_high, *add_low;  // kPoly: As; kApply, kFinal: Xs
+  __half *high, *low;              // result [n][m] (kGram and kPoly: symmetric); low null: none; ld and stack also Xs'
+  int64_t ld, stack;               // elements between rows, and between matrices
+  int* error;
+};
+
+struct Bars {
+  uint64_t full[kMaxStages], empty[kMaxStages], drain, acc_full[2], acc_empty[2], small_empty[2];
+  uint32_t tmem;
+  int failed;
+};
+
+struct Maps { CUtensorMap a[2], b[2]; };  // high, low
+
+struct Tile { int z, row, col; };
+// Tile `item` of the list.  Symmetric products: row tile i starts with the column tile that its diagonal is in.
+__device__ __forceinline__ Tile tile_of(const Params& p, int item) {
+  Tile t;
+  t.z = item / p.items;
+  int i = item % p.items;
+  if (!p.symmetric) {
+    t.row = i / p.col_tiles;
+    t.col = i % p.col_tiles;
+    return t;
+  }
+  t.row = 0;
+  for (int first = 0;; first = t.row * kM / p.b.rows) {
+    if (i < p.col_tiles - first) {
+      t.col = first + i;
+      return t;
+    }
+    i -= p.col_tiles - first;
+    ++t.row;
+  }
+}
+
+__device__ __forceinline__ uint64_t descriptor(const Operand& o, uint32_t addr, int q) {  // of 16 elements of K, the q-th in a step
+  return o.turned ? desc_mn(addr + (uint32_t)q * 2048u, kK * 128) : desc_k(addr + (uint32_t)q * 32u);
+}
+
+__device__ __forceinline__ void load_operand(const Operand& o, const CUtensorMap* map, uint32_t dst, const uint64_t* bar, int k0, int at, int z) {
+  if (!o.turned) {
+    tma_load(map, dst, bar, k0, at, z);
+  } else {
+    for (int c = 0; c < o.rows / 64; ++c) tma_load(map, dst + (uint32_t)c * (kK * 128), bar, at + c * 64, k0, z);
+  }
+}
+
+// One row's 32 values of the product from column `col` on, to where they belong.
+template <int MODE, typename T>
+__device__ __forceinline__ void store_values(const Params& p, const Matrices& s, const Factors& f, int z, int row, int col, const uint32_t (&r)[32], bool lost) {
+  if (row >= p.m) return;
+  const float nan = __int_as_float(0x7fffffff);
+  const __half* const add_high = MODE != kGram ? p.add_high + z * p.stack : nullptr;
+  const __half* const add_low = MODE != kGram && p.add_low != nullptr ? p.add_low + z * p.stack : nullptr;
+  const auto added = [&](int64_t at) {  // what is at [column][row] of the other matrix (As is symmetric)
+    const float high = __half2float(__ldg(add_high + at));
+    return add_low != nullptr ? high + __half2float(__ldg(add_low + at)) : high;
+  };
+  if constexpr (MODE == kFinal) {
+    T* out = s.template result<T>(z) + (int64_t)col * p.m + row;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (col + j >= p.n) break;
+      const float v = fmaf(f.own, added((int64_t)(col + j) * p.ld + row), __uint_as_float(r[j]) * f.apply);
+      finish(s, out + (int64_t)j * p.m, lost ? nan : v);
+    }
+  } else {
+    __half* const high = p.high + z * p.stack;
+    __half* const low = p.low != nullptr ? p.low + z * p.stack : nullptr;
+    union { __half h[32]; uint4 v[4]; } hi, lo;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float v = __uint_as_float(r[j]);
+      const bool in = col + j < p.n;
+      v *= MODE == kGram ? f.gram : MODE == kPoly ? f.poly_c : f.apply;
+      if (MODE != kGram && in) v = fmaf(MODE == kPoly ? f.poly_b : f.own, added((int64_t)(col + j) * p.ld + row), v);
+      if (lost) v = nan;
+      hi.h[j] = __float2half_rn(v);
+      lo.h[j] = __float2half_rn(v - __half2float(hi.h[j]));
+      if (in && (MODE == kApply || col + j >= row)) {
+        const int64_t at = (int64_t)(col + j) * p.ld + row;
+        high[at] = hi.h[j];
+        if (low != nullptr) low[at] = lo.h[j];
+      }
+    }
+    if constexpr (MODE != kApply) {  // the same on the other side of the diagonal
+      const int64_t at = (int64_t)row * p.ld + col;
+      if (col > row) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (col + 8 * q >= p.n) break;
+          *reinterpret_cast<uint4*>(high + at + 8 * q) = hi.v[q];
+          if (low != nullptr) *reinterpret_cast<uint4*>(low + at + 8 * q) = lo.v[q];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          if (col + j <= row || col + j >= p.n) continue;
+          high[at + j] = hi.h[j];
+          if (low != nullptr) low[at + j] = lo.h[j];
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void add(uint32_t (&sum)[32], const uint32_t (&r)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(r[j]));
+}
+
+template <int MODE, typename T>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, const __grid_constant__ Matrices s) {
+  constexpr bool kWide = sizeof(T) == 4;  // pairs by pairs: see above
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ Bars bars;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const int total = p.items * p.batch;
+  const uint32_t a_bytes = (uint32_t)p.a.bytes(), b_bytes = (uint32_t)p.b.bytes();
+  const uint32_t b_at = a_bytes * p.a.planes, stage_bytes = b_at + b_bytes * p.b.planes;
+  volatile int* failed = &bars.failed;
+
+  if (wid == 1) alloc_tmem(&bars.tmem, (uint32_t)p.tmem * (kWide ? 4u : (uint32_t)p.accumulators));
+  if (tid == 0) {
+    for (int q = 0; q < p.stages; ++q) { init_bar(bars.full + q, 1); init_bar(bars.empty + q, 1); }
+    init_bar(&bars.drain, 1);
+    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps); init_bar(bars.small_empty + b, kEpilogueWarps); }
+    fence_bars();
+    bars.failed = 0;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = bars.tmem;
+  int slot = 0;
+  uint32_t round = 0;
+
+  if (wid == 0) {
+    // ================= loads
+    if (lane == 0) {
+      dependency_wait();
+      release_dependents();
+      for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        const Tile t = tile_of(p, item);
+        int i = 0;
+        for (; i < p.steps; ++i) {
+          if (round > 0 && !wait_bar(bars.empty + slot, (round - 1) & 1, failed)) break;
+          const uint32_t stage = smem_u32(smem + (size_t)slot * stage_bytes);
+          expect(bars.full + slot, stage_bytes);
+          for (int q = 0; q < p.a.planes; ++q) load_operand(p.a, maps.a + q, stage + q * a_bytes, bars.full + slot, i * kK, t.row * kM, t.z);
+          for (int q = 0; q < p.b.planes; ++q) load_operand(p.b, maps.b + q, stage + b_at + q * b_bytes, bars.full + slot, i * kK, t.col * p.b.rows, t.z);
+          if (++slot == p.stages) { slot = 0; ++round; }
+        }
+        if (i < p.steps) break;
+      }
+    }
+  } else if (wid == 1) {
+    // ================= MMAs
+    if (lane == 0) {
+      const uint32_t idesc = instruction(kSumF32, kFormatF16, kM, (uint32_t)p.b.rows) | (p.a.turned ? kTurnedA : 0u) | (p.b.turned ? kTurnedB : 0u);
+      bool ok = true;
+      uint32_t t = 0, chunk = 0;
+      for (int item = blockIdx.x; ok && item < total; item += gridDim.x, ++t) {
+        const uint32_t turn = t / (uint32_t)p.accumulators, buf = t % (uint32_t)p.accumulators;
+        uint32_t acc = tmem + buf * (uint32_t)p.tmem;                      // 16-bit matrices: all sums of the tile
+        const uint32_t small = tmem + (2u + (t & 1u)) * (uint32_t)p.tmem;  // float32: those of the small products
+        if constexpr (kWide) {
+          if (t >= 2) ok = wait_bar(bars.small_empty + (t & 1u), ((t >> 1) - 1) & 1, failed);
+        } else {
+          if (turn > 0) ok = wait_bar(bars.acc_empty + buf, (turn - 1) & 1, failed);
+        }
+        for (int i = 0; ok && i < p.steps; ++i) {
+          const bool fresh = kWide && i % kChunk == 0;
+          if (fresh) {
+            if (chunk >= 2) ok = wait_bar(bars.acc_empty + (chunk & 1u), ((chunk >> 1) - 1) & 1, failed);
+            acc = tmem + (chunk & 1u) * (uint32_t)p.tmem;
+          }
+          ok = ok && wait_bar(bars.full + slot, round & 1, failed);
+          if (!ok) break;
+          fence_after();
+          const uint32_t a = smem_u32(smem + (size_t)slot * stage_bytes), b = a + b_at;
+#pragma unroll
+          for (int q = 0; q < kK / 16; ++q) {
+            const uint64_t a_high = descriptor(p.a, a, q), b_high = descriptor(p.b, b, q);
+            mma_f16(acc, a_high, b_high, idesc, (fresh || i == 0) && q == 0 ? 0u : 1u);
+            if (p.a.planes > 1) mma_f16(kWide ? small : acc, descriptor(p.a, a + a_bytes, q), b_high, idesc, kWide && i + q == 0 ? 0u : 1u);
+            if (p.b.planes > 1) mma_f16(kWide ? small : acc, a_high, descriptor(p.b, b + b_bytes, q), idesc, 1u);
+          }
+          commit(bars.empty + slot);
+          if (++slot == p.stages) { slot = 0; ++round; }
+          if (kWide && (i % kChunk == kChunk - 1 || i + 1 == p.steps)) {
+            commit(bars.acc_full + (chunk & 1u));
+            ++chunk;
+          }
+        }
+        if (!kWide && ok) commit(bars.acc_full + buf);
+      }
+    }
+  } else {
+    // ================= epilogue: a warp has the TMEM lanes of its quarter and half of the columns, thread = row
+    const int quarter = wid & 3, half = (wid - 2) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    uint32_t t = 0, chunk = 0;
+    bool lost = false;
+    dependency_wait();
+    for (int item = blockIdx.x; item < total; item += gridDim.x, ++t) {
+      const Tile at = tile_of(p, item);
+      const int row0 = at.row * kM + quarter * 32, col0 = at.col * p.b.rows;
+      const Factors f = p.factors[at.z * F2C_MAX_NS_STEPS];
+      if constexpr (kWide) {
+        // sums of kChunk steps each are added up here, where additions round
+        uint32_t sum[2][32] = {};
+        const int width = p.b.rows / 2, first = half * width;
+        for (int i = 0; i < p.steps; i += kChunk, ++chunk) {
+          lost = lost || !__all_sync(0xffffffffu, wait_bar(bars.acc_full + (chunk & 1u), (chunk >> 1) & 1, failed));
+          fence_after();
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (c * 32 >= width) break;
+            uint32_t r[32];
+            tmem_ld32(lanes + (chunk & 1u) * (uint32_t)p.tmem + (uint32_t)(first + c * 32), r);
+            tmem_wait(r);
+            add(sum[c], r);
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(bars.acc_empty + (chunk & 1u));
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c * 32 >= width) break;
+          uint32_t r[32];
+          tmem_ld32(lanes + (2u + (t & 1u)) * (uint32_t)p.tmem + (uint32_t)(first + c * 32), r);
+          tmem_wait(r);
+          add(sum[c], r);
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(bars.small_empty + (t & 1u));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int col = col0 + first + c * 32;
+          if (c * 32 >= width || col >= p.n || (p.symmetric && col + 31 < row0)) continue;  // (wholly below the diagonal)
+          store_values<MODE, T>(p, s, f, at.z, row0 + lane, col, sum[c], lost);
+        }
+        __syncwarp();
+      } else {
+        const uint32_t turn = t / (uint32_t)p.accumulators, buf = t % (uint32_t)p.accumulators;
+        const int cols = min(p.b.rows, p.n - col0);
+        lost = lost || !__all_sync(0xffffffffu, wait_bar(bars.acc_full + buf, turn & 1, failed));
+        fence_after();
+        for (int c0 = half * 32; c0 < cols; c0 += 64) {
+          if (p.symmetric && col0 + c0 + 31 < row0) continue;
+          uint32_t r[32];
+          tmem_ld32(lanes + buf * (uint32_t)p.tmem + (uint32_t)c0, r);
+          tmem_wait(r);
+          store_values<MODE, T>(p, s, f, at.z, row0 + lane, col0 + c0, r, lost);
+          __syncwarp();
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(bars.acc_empty + buf);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (bars.failed) {
+    // copies in flight write to this CTA's shared memory, MMAs in flight read it and write its TMEM: wait (bounded) for what was issued
+    volatile int expired = 0;
+    if (tid == 0) {
+      for (int q = 0; q < p.stages; ++q) {
+        const uint32_t uses = round + (q < slot ? 1u : 0u);
+        if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, &expired);
+      }
+    } else if (tid == 32) {
+      commit(&bars.drain);
+      wait_bar(&bars.drain, 0, &expired);
+    }
+    __syncthreads();
+  }
+  if (wid == 1) {
+    fence_after();
+    free_tmem(tmem, (uint32_t)p.tmem * (kWide ? 4u : (uint32_t)p.accumulators));
+  }
+  if (tid == 0 && bars.failed) report_wait(p.error, 5);
+}
+
+// ---------------------------------------------------------------- host
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
 struct Shape {
   int64_t batch, rows, cols;
   int64_t p() const { return rows < cols ? rows : cols; }
-  int64_t q() const { return rows < cols ? cols : rows; }
+  int64_t ldx() const { return (cols + 7) / 8 * 8; }
+  int64_t ldp() const { return (p() + 7) / 8 * 8; }
+  int64_t x_bytes() const { return round256(2 * batch * rows * ldx()); }
+  int64_t p_bytes() const { return round256(2 * batch * p() * ldp()); }
 };
 
-static int64_t workspace(const Shape& s) {
-  return 2 * round256(4 * s.batch * s.rows * s.cols) + 2 * round256(4 * s.batch * s.p() * s.p()) + round256(8 * s.batch * kParts);
+// Planes of X in front of a step: 2 for float32; otherwise see above (`exact`: the first X is).
+static int x_planes(const Steps& st, int t, bool wide, bool exact) {
+  if (wide) return 2;
+  if (t == 0 && exact) return 1;
+  double gain = 1.0;
+  for (int q = t; q < st.count; ++q) {
+    const double a = fabs((double)st.co[3 * q]);
+    gain *= a > 1.0 ? a : 1.0;
+  }
+  return gain > 16.0 ? 2 : 1;
 }
 
-static int run(const char* op, const Source& src, int dtype, const Shape& s, const float* co, int steps, float eps, char* ws, cudaStream_t st) {
-  float* x = (float*)ws;
-  float* x2 = (float*)(ws += round256(4 * s.batch * s.rows * s.cols));
-  float* a = (float*)(ws += round256(4 * s.batch * s.rows * s.cols));
-  float* b = (float*)(ws += round256(4 * s.batch * s.p() * s.p()));
-  double* parts = (double*)(ws + round256(4 * s.batch * s.p() * s.p()));
-  const dim3 grid(kParts, (unsigned)s.batch);
-  const int p = (int)s.p(), q = (int)s.q();
-  auto* load = dtype == F2C_F32 ? load_kernel<float> : dtype == F2C_F16 ? load_kernel<__half> : load_kernel<__nv_bfloat16>;
-  auto* store = dtype == F2C_F32 ? store_kernel<float> : dtype == F2C_F16 ? store_kernel<__half> : store_kernel<__nv_bfloat16>;
-  launch_dependent(load, grid, kThreads, 0, st, src, x, parts, s.rows, s.cols);
-  launch_dependent(scale_kernel, grid, kThreads, 0, st, x, (const double*)parts, s.rows * s.cols, eps);
-  const unsigned tp = (unsigned)ceil_div(p, kTile), tq = (unsigned)ceil_div(q, kTile), z = (unsigned)s.batch;
-  for (int t = 0; t < steps; ++t, co += 3) {
-    launch_dependent(product_kernel, dim3(tp, tp, z), kThreads, 0, st, (const float*)x, (const float*)x, (const float*)nullptr, a, p, p, q, 1, 1.0f, 0.0f, 0.0f);
-    launch_dependent(product_kernel, dim3(tp, tp, z), kThreads, 0, st, (const float*)a, (const float*)a, (const float*)a, b, p, p, p, 1, co[2], co[1], co[0]);
-    launch_dependent(product_kernel, dim3(tp, tq, z), kThreads, 0, st, (const float*)b, (const float*)x, (const float*)nullptr, x2, p, q, p, 0, 1.0f, 0.0f, 0.0f);
-    float* swap = x;
-    x = x2;
-    x2 = swap;
+static int64_t workspace(const Shape& s, bool wide) {
+  return 4 * s.x_bytes() + (wide ? 4 : 2) * s.p_bytes() + round256(8 * s.batch * kParts) + round256((int64_t)sizeof(Factors) * F2C_MAX_NS_STEPS * s.batch);
+}
+
+struct Planes {
+  __half *high, *low;
+};
+
+// Columns of a tile: as many as leave every SM a tile, or so few that more SMs than not have one.
+static int tile_columns(int64_t rows_m, int64_t cols_n, int64_t batch, bool symmetric, int most, int sms) {
+  for (int n = most; n > 64; n /= 2) {
+    int64_t items = 0;
+    const int64_t rt = ceil_div(rows_m, kM), ct = ceil_div(cols_n, n);
+    if (symmetric) for (int64_t i = 0; i < rt; ++i) items += ct - i * kM / n;
+    else items = rt * ct;
+    if (items * batch >= sms) return n;
   }
-  launch_dependent(store, grid, kThreads, 0, st, src, (const float*)x, s.rows, s.cols);
+  return 64;
+}
+
+struct Product {
+  Planes a, b;
+  int a_planes, b_planes, a_turned, b_turned;
+  int64_t a_rows, a_cols, a_ld, b_rows, b_cols, b_ld;  // the operands' matrices as they lie
+  int64_t m, n, k;
+  bool symmetric;
+};
+
+template <int MODE, typename T>
+static int multiply(const char* op, const Product& x, Params p, const Matrices& s, int64_t batch, cudaStream_t st) {
+  const int sms = current_sm_count();
+  p.m = (int)x.m; p.n = (int)x.n;
+  p.steps = (int)ceil_div(x.k, kK);
+  p.symmetric = x.symmetric;
+  p.batch = (int)batch;
+  p.a = Operand{kM, x.a_turned, x.a_planes};
+  p.b = Operand{tile_columns(x.m, x.n, batch, x.symmetric, sizeof(T) == 4 ? 128 : kMaxN, sms), x.b_turned, x.b_planes};
+  p.row_tiles = (int)ceil_div(x.m, kM);
+  p.col_tiles = (int)ceil_div(x.n, p.b.rows);
+  p.items = p.row_tiles * p.col_tiles;
+  if (x.symmetric) {
+    p.items = 0;
+    for (int i = 0; i < p.row_tiles; ++i) p.items += p.col_tiles - i * kM / p.b.rows;
+  }
+  const int64_t total = (int64_t)p.items * batch;
+  F2C_REQUIRE(total < (1ll << 31), F2C_ERR_LIMIT, "%s: too many tiles", op);
+  const unsigned grid = (unsigned)(total < sms ? total : sms);
+  p.tmem = p.b.rows;
+  p.accumulators = total > grid ? 2 : 1;
+  p.error = stream_error_word();
+  const size_t stage = (size_t)p.a.bytes() * p.a.planes + (size_t)p.b.bytes() * p.b.planes, room = kRoom - 1024;
+  p.stages = (int)(room / stage);
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  Maps maps;
+  const __half* ap[2] = {x.a.high, x.a.low};
+  const __half* bp[2] = {x.b.high, x.b.low};
+  bool ok = true;
+  for (int q = 0; q < 2; ++q) {
+    ok = ok && make_stack_map(maps.a + q, ap[q < x.a_planes ? q : 0], batch, x.a_rows, x.a_cols, 2 * x.a_ld, x.a_turned ? kK : kM);
+    ok = ok && make_stack_map(maps.b + q, bp[q < x.b_planes ? q : 0], batch, x.b_rows, x.b_cols, 2 * x.b_ld, x.b_turned ? kK : p.b.rows);
+  }
+  F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
+  auto* kern = product_kernel<MODE, T>;
+  if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom)) return rc;
+  launch_dependent(kern, dim3(grid), kThreads, p.stages * stage + 1024, st, maps, p, s);
   return check_launch(op);
 }
 
-// Singular values start in [0, 1].  What keeps the half-precision operands in range: no step may take one out of [0, 7.9], nor multiply by more than 60.
-static int check(const char* op, int dtype, const float* co, int steps, float eps) {
+template <typename T>
+static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps& st, char* ws, cudaStream_t stream) {
+  constexpr bool kWide = sizeof(T) == 4;
+  const bool exact = !kWide && src.listed == 0, tall = s.rows > s.cols;
+  auto take = [&](int64_t bytes) { char* at = ws; ws += bytes; return at; };
+  Planes x[2], a{}, r{};
+  for (Planes& q : x) { q.high = (__half*)take(s.x_bytes()); q.low = (__half*)take(s.x_bytes()); }
+  for (Planes* q : {&a, &r}) { q->high = (__half*)take(s.p_bytes()); q->low = kWide ? (__half*)take(s.p_bytes()) : nullptr; }
+  double* parts = (double*)take(round256(8 * s.batch * kParts));
+  Factors* table = (Factors*)take(0);
+  src.size = s.rows * s.cols;
+  bool four = s.cols % 4 == 0 && aligned(src.g, 4 * sizeof(T));
+  for (int i = 0; i < src.listed; ++i) four = four && aligned(src.list[i].grad, 4 * sizeof(T)) && aligned(src.list[i].momentum, 16);
+  const dim3 grid(kParts, (unsigned)s.batch);
+  int planes = st.count == 0 ? (exact ? 1 : 2) : x_planes(st, 0, kWide, exact);
+  __half* low = planes > 1 ? x[0].low : nullptr;
+  if (four) {
+    launch_dependent(norm_kernel<T, 4>, grid, kLoadThreads, 0, stream, src, parts);
+    launch_dependent(planes_kernel<T, 4>, grid, kLoadThreads, 0, stream, src, st, (const double*)parts, x[0].high, low, s.rows, s.cols, s.ldx(), table);
+  } else {
+    launch_dependent(norm_kernel<T, 1>, grid, kLoadThreads, 0, stream, src, parts);
+    launch_dependent(planes_kernel<T, 1>, grid, kLoadThreads, 0, stream, src, st, (const double*)parts, x[0].high, low, s.rows, s.cols, s.ldx(), table);
+  }
+  if (const int rc = check_launch(op)) return rc;
+  if (st.count == 0) {
+    launch_dependent(store_kernel<T>, grid, kLoadThreads, 0, stream, src, (const __half*)x[0].high, (const __half*)low, s.rows, s.cols, s.ldx(), (const Factors*)table);
+    return check_launch(op);
+  }
+  const int64_t p = s.p();
+  const int inner = kWide ? 2 : 1;
+  for (int t = 0; t < st.count; ++t) {
+    const bool last = t + 1 == st.count, poly = st.co[3 * t + 2] != 0.0f;
+    // A = X X^T: of a tall matrix, whose transpose X is, the rows run along K
+    Product gram{x[t & 1], x[t & 1], inner, inner, tall, tall, s.rows, s.cols, s.ldx(), s.rows, s.cols, s.ldx(), p, p, tall ? s.rows : s.cols, true};
+    Params g{};
+    g.factors = table + t;
+    g.high = poly ? a.high : r.high; g.low = poly ? a.low : r.low;
+    g.ld = s.ldp(); g.stack = p * s.ldp();
+    if (const int rc = multiply<kGram, T>(op, gram, g, src, s.batch, stream)) return rc;
+    if (poly) {
+      Product square{a, a, inner, inner, 0, 0, p, p, s.ldp(), p, p, s.ldp(), p, p, p, true};
+      Params q = g;
+      q.add_high = a.high; q.add_low = a.low;
+      q.high = r.high; q.low = r.low;
+      if (const int rc = multiply<kPoly, T>(op, square, q, src, s.batch, stream)) return rc;
+    }
+    // the rows of the next X are columns of this product, so that a warp writes 32 neighbours
+    const int next = last ? 1 : x_planes(st, t + 1, kWide, exact);
+    Product apply = tall ? Product{r, x[t & 1], inner, planes, 0, 0, p, p, s.ldp(), s.rows, s.cols, s.ldx(), p, s.rows, p, false}
+                         : Product{x[t & 1], r, planes, inner, 1, 0, s.rows, s.cols, s.ldx(), p, p, s.ldp(), s.cols, p, p, false};
+    Params q{};
+    q.factors = table + t;
+    q.add_high = x[t & 1].high; q.add_low = planes > 1 ? x[t & 1].low : nullptr;
+    q.high = x[(t + 1) & 1].high; q.low = next > 1 ? x[(t + 1) & 1].low : nullptr;
+    q.ld = s.ldx(); q.stack = s.rows * s.ldx();
+    if (const int rc = last ? multiply<kFinal, T>(op, apply, q, src, s.batch, stream) : multiply<kApply, T>(op, apply, q, src, s.batch, stream)) return rc;
+    planes = next;
+  }
+  return F2C_OK;
+}
+
+static int run(const char* op, Matrices& src, int dtype, const Shape& s, const Steps& st, char* ws, cudaStream_t stream) {
+  if (dtype == F2C_F32) return run_typed<float>(op, src, s, st, ws, stream);
+  if (dtype == F2C_F16) return run_typed<__half>(op, src, s, st, ws, stream);
+  return run_typed<__nv_bfloat16>(op, src, s, st, ws, stream);
+}
+
+// Singular values start in [0, 1].  What keeps the half-precision operands in range: no step may take one out of [0, 7.9], and R has none over 60.
+static int check(const char* op, int dtype, const float* co, int steps, float eps, Steps* st) {
   F2C_REQUIRE(is_float_dtype(dtype), F2C_ERR_UNSUPPORTED, "%s: matrices must be float32, float16 or bfloat16", op);
   F2C_REQUIRE(steps >= 0 && steps <= F2C_MAX_NS_STEPS, F2C_ERR_LIMIT, "%s: 0 to %d steps", op, F2C_MAX_NS_STEPS);
   F2C_REQUIRE(steps == 0 || co, F2C_ERR_INVALID, "%s: null pointer", op);
   F2C_REQUIRE(eps >= 0.0f && eps <= 3.4028235e38f, F2C_ERR_INVALID, "%s: eps must not be negative", op);
+  st->count = steps;
+  st->eps = eps;
   double top = 1.0;
+  st->top[0] = 1.0f;
   for (int t = 0; t < steps; ++t, co += 3) {
-    double factor = 0.0, next = 0.0;
+    double factor = 0.0, next = 0.0, r = 0.0;
     for (int i = 0; i <= 1024; ++i) {
-      const double v = top * i / 1024, f = fabs(co[0] + v * v * (co[1] + v * v * co[2]));
+      const double v = top * i / 1024, w = v * v * (co[1] + v * v * co[2]), f = fabs(co[0] + w);
+      if (!(fabs(w) <= r)) r = fabs(w);
       if (!(f <= factor)) factor = f;
       if (!(v * f <= next)) next = v * f;
     }
-    F2C_REQUIRE(factor <= 60.0 && next <= 7.9, F2C_ERR_LIMIT, "%s: the coefficients of step %d let the matrix grow too far", op, t);
+    F2C_REQUIRE(r <= 60.0 && next <= 7.9, F2C_ERR_LIMIT, "%s: the coefficients of step %d let the matrix grow too far", op, t);
     top = next;
+    for (int i = 0; i < 3; ++i) st->co[3 * t + i] = co[i];
+    st->factor[t] = (float)factor;
+    st->top[t + 1] = (float)top;
   }
   return F2C_OK;
 }
@@ -177,29 +704,46 @@ static int check_shape(const char* op, const Shape& s) {
 
 using namespace f2c;
 
-extern "C" int64_t f2c_orthogonalize_workspace(int, int64_t batch, int64_t rows, int64_t cols) {
-  return batch < 1 || rows < 1 || cols < 1 ? 0 : ns::workspace(ns::Shape{batch, rows, cols});
+extern "C" int64_t f2c_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t cols) {
+  return batch < 1 || rows < 1 || cols < 1 ? 0 : ns::workspace(ns::Shape{batch, rows, cols}, dtype == F2C_F32);
 }
 
 extern "C" int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t batch, int64_t rows, int64_t cols, const float* coefficients_host,
                                  int steps, float eps, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* op = "orthogonalize";
   const ns::Shape s{batch, rows, cols};
+  ns::Steps st{};
   if (const int rc = ns::check_shape(op, s)) return rc;
-  if (const int rc = ns::check(op, dtype, coefficients_host, steps, eps)) return rc;
+  if (const int rc = ns::check(op, dtype, coefficients_host, steps, eps, &st)) return rc;
   if (batch == 0 || rows == 0 || cols == 0) return F2C_OK;
   F2C_REQUIRE(g && out, F2C_ERR_INVALID, "%s: null pointer", op);
-  F2C_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= ns::workspace(s), F2C_ERR_INVALID,
+  F2C_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= ns::workspace(s, dtype == F2C_F32), F2C_ERR_INVALID,
               "%s: workspace too small or not 256-byte aligned", op);
-  return ns::run(op, ns::Source{g, out, nullptr, 0, 0, 0, 0}, dtype, s, coefficients_host, steps, eps, (char*)workspace, (cudaStream_t)stream);
+  ns::Matrices src{};
+  src.g = g;
+  src.out = out;
+  return ns::run(op, src, dtype, s, st, (char*)workspace, (cudaStream_t)stream);
 }
 
-extern "C" int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int count, int) {
+// Matrices of the list that have the shape of number i, from i on: into `src`, up to kMaxList.  False when an earlier one was their first.
+static bool group_of(const f2c_muon_matrix* list, int count, int i, ns::Matrices* src) {
+  const auto same = [&](int j) { return list[j].rows == list[i].rows && list[j].cols == list[i].cols; };
+  if (list[i].rows == 0 || list[i].cols == 0) return false;
+  int before = 0;
+  for (int j = 0; j < i; ++j) before += same(j);
+  if (before % ns::kMaxList != 0) return false;
+  src->listed = 0;
+  for (int j = i; j < count && src->listed < ns::kMaxList; ++j)
+    if (same(j)) src->list[src->listed++] = list[j];
+  return true;
+}
+
+extern "C" int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int count, int dtype) {
   int64_t most = 0;
+  ns::Matrices src{};
   for (int i = 0; list_host != nullptr && i < count; ++i) {
-    const ns::Shape s{1, list_host[i].rows, list_host[i].cols};
-    if (s.rows < 1 || s.cols < 1) continue;
-    const int64_t bytes = ns::workspace(s);
+    if (list_host[i].rows < 0 || list_host[i].cols < 0 || !group_of(list_host, count, i, &src)) continue;
+    const int64_t bytes = ns::workspace(ns::Shape{src.listed, list_host[i].rows, list_host[i].cols}, dtype == F2C_F32);
     most = bytes > most ? bytes : most;
   }
   return most;
@@ -208,8 +752,9 @@ extern "C" int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int coun
 extern "C" int f2c_muon_step(const f2c_muon_matrix* list_host, int count, int dtype, float lr, float momentum, int nesterov, float decay,
                              const float* coefficients_host, int steps, float eps, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* op = "muon_step";
+  ns::Steps st{};
   F2C_REQUIRE(count >= 0 && (count == 0 || list_host), F2C_ERR_INVALID, "%s: bad list", op);
-  if (const int rc = ns::check(op, dtype, coefficients_host, steps, eps)) return rc;
+  if (const int rc = ns::check(op, dtype, coefficients_host, steps, eps, &st)) return rc;
   for (int i = 0; i < count; ++i) {
     const f2c_muon_matrix& m = list_host[i];
     if (const int rc = ns::check_shape(op, ns::Shape{1, m.rows, m.cols})) return rc;
@@ -218,12 +763,15 @@ extern "C" int f2c_muon_step(const f2c_muon_matrix* list_host, int count, int dt
   const int64_t need = f2c_muon_workspace(list_host, count, dtype);
   F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,
               "%s: workspace too small or not 256-byte aligned", op);
+  ns::Matrices src{};
+  src.mu = momentum;
+  src.keep = (float)(1.0 - (double)lr * decay);
+  src.nesterov = nesterov;
   for (int i = 0; i < count; ++i) {
-    const f2c_muon_matrix& m = list_host[i];
-    if (m.rows == 0 || m.cols == 0) continue;
-    const double gain = (double)lr * sqrt(m.rows > m.cols ? (double)m.rows / (double)m.cols : 1.0);
-    const ns::Source src{m.grad, m.weight, m.momentum, momentum, (float)(1.0 - (double)lr * decay), (float)gain, nesterov};
-    if (const int rc = ns::run(op, src, dtype, ns::Shape{1, m.rows, m.cols}, coefficients_host, steps, eps, (char*)workspace, (cudaStream_t)stream)) return rc;
+    if (!group_of(list_host, count, i, &src)) continue;
+    const ns::Shape s{src.listed, list_host[i].rows, list_host[i].cols};
+    src.gain = (float)((double)lr * sqrt(s.rows > s.cols ? (double)s.rows / (double)s.cols : 1.0));
+    if (const int rc = ns::run(op, src, dtype, s, st, (char*)workspace, (cudaStream_t)stream)) return rc;
   }
   return F2C_OK;
 }

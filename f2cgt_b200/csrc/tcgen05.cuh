@@ -84,6 +84,14 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
   return ((uint64_t)hi << 32) | lo;
 }
 
+// Rows of 128 bytes along M or N, one row for every element of K: K row r of 64 elements at 128 r, the next 64 elements `chunk` bytes further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t chunk) {
+  const uint32_t lo = ((addr & 0x3FFFFu) >> 4) | ((chunk >> 4) << 16);
+  const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)hi << 32) | lo;
+}
+
+constexpr uint32_t kTurnedA = 1u << 15, kTurnedB = 1u << 16;  // of an instruction: the operand lies along M or N
 constexpr uint32_t kFormatF16 = 0, kFormatS8 = 1, kSumF32 = 1, kSumS32 = 2;
 __device__ __forceinline__ constexpr uint32_t instruction(uint32_t sum, uint32_t format, uint32_t m, uint32_t n) {
   return (sum << 4) | (format << 7) | (format << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
@@ -97,6 +105,14 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, 
       : "memory");
 }
 
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc),
+      "r"(accumulate), "r"(0u)
+      : "memory");
+}
+
 // arrives at the barrier when all MMAs issued so far by this thread are complete
 __device__ __forceinline__ void commit(const uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -106,6 +122,11 @@ __device__ __forceinline__ void commit(const uint64_t* bar) {
 __device__ __forceinline__ void tma_load(const CUtensorMap* map, uint32_t dst, const uint64_t* bar, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tma_load(const CUtensorMap* map, uint32_t dst, const uint64_t* bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
@@ -124,6 +145,8 @@ __device__ __forceinline__ void peer_store(uint32_t addr, uint32_t v) { asm vola
 // Tensor map of a row-major matrix [rows, cols] of `bytes`-byte elements (16-byte aligned start and row stride), boxes of box_rows x
 // 128 bytes with the 128-byte swizzle, zeros outside the matrix.  False when the driver refuses it.
 bool make_map(CUtensorMap* map, const void* base, int bytes, int64_t rows, int64_t cols, int64_t row_bytes, int box_rows);
+// The same for a stack of `batch` half-precision matrices, `rows` rows apart.
+bool make_stack_map(CUtensorMap* map, const void* base, int64_t batch, int64_t rows, int64_t cols, int64_t row_bytes, int box_rows);
 
 }  // namespace t5
 }  // namespace f2c

@@ -426,7 +426,7 @@ int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int
 /* ---- orthogonalised updates of weight matrices (beside Adam, examples/train_graphsage_nodeclass.py:56) ----
  * Newton-Schulz steps: X = G / (|G|_F + eps), then for every step's coefficients (a, b, c): X <- (a I + b A + c A^2) X, A = X X^T
  * (for more rows than columns the transposed matrix is meant).  coefficients_host: 3 * steps floats.  Refused are coefficients under
- * which a singular value could leave [0, 7.9] or a factor a + b s^2 + c s^4 the range of magnitude 60: values are held in half
+ * which a singular value s could leave [0, 7.9], or b s^2 + c s^4 exceed 60: values are held in half
  * precision (pairs of it where more is needed).  Matrices that hold a NaN or an infinity become NaN.
  * f2c_orthogonalize: g and out [batch, rows, cols], dtype F32, F16 or BF16; out may be g.
  * f2c_muon_step: for every matrix of the list  m <- momentum m + g;  u = nesterov ? g + momentum m : m;
