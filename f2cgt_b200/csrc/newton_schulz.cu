@@ -26,7 +26,7 @@ namespace ns {
 
 using namespace t5;
 
-constexpr int kParts = 64, kLoadThreads = 256;
+constexpr int kMaxParts = 1024, kLoadThreads = 256;  // parts of a matrix' norm
 constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: MMA, then the epilogue's
 constexpr int kChunk = 2;                    // steps of K after which float32's sums are taken out of the tensor cores' hands
 constexpr int kM = 128, kK = 64, kMaxN = 256, kMaxStages = 8, kMaxList = 64;
@@ -90,14 +90,14 @@ __device__ __forceinline__ void direction(const Matrices& s, int z, int64_t i, f
   if (UPDATE) *reinterpret_cast<Chunk<float, V>*>(momentum + i) = m;
 }
 
-// Momentum, and the squares' sums of kParts parts of every matrix.
+// Momentum, and the squares' sums of gridDim.x parts of every matrix.
 template <typename T, int V>
 __global__ void __launch_bounds__(kLoadThreads) norm_kernel(const __grid_constant__ Matrices s, double* parts) {
   dependency_wait();
   release_dependents();
   const int z = blockIdx.y;
   double sum = 0.0;
-  for (int64_t i = ((int64_t)blockIdx.x * kLoadThreads + threadIdx.x) * V; i < s.size; i += (int64_t)kParts * kLoadThreads * V) {
+  for (int64_t i = ((int64_t)blockIdx.x * kLoadThreads + threadIdx.x) * V; i < s.size; i += (int64_t)gridDim.x * kLoadThreads * V) {
     float u[V];
     direction<T, V, true>(s, z, i, u);
 #pragma unroll
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kLoadThreads) norm_kernel(const __grid_constan
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int w = 1; w < kLoadThreads / 32; ++w) sum += sums[w];
-    parts[z * kParts + blockIdx.x] = sum;
+    parts[z * kMaxParts + blockIdx.x] = sum;
   }
 }
 
@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(kLoadThreads) planes_kernel(const __grid_const
   const int z = blockIdx.y;
   __shared__ double norm_s;
   if (threadIdx.x < 32) {
-    double sum = parts[z * kParts + threadIdx.x] + parts[z * kParts + 32 + threadIdx.x];
+    double sum = 0.0;
+    for (int q = threadIdx.x; q < gridDim.x; q += 32) sum += parts[z * kMaxParts + q];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (threadIdx.x == 0) norm_s = sqrt(sum);
@@ -183,11 +184,6 @@ __global__ void __launch_bounds__(kLoadThreads) planes_kernel(const __grid_const
 
 // No steps: X itself is the result.
 template <typename T>
-__device__ __forceinline__ void finish(const Matrices& s, T* out, float x) {
-  *out = from_float<T>(s.listed ? s.keep * to_float(*out) - s.gain * x : x);
-}
-
-template <typename T>
 __global__ void __launch_bounds__(kLoadThreads) store_kernel(const __grid_constant__ Matrices s, const __half* high, const __half* low, int64_t rows, int64_t cols,
                                                              int64_t ld, const Factors* table) {
   dependency_wait();
@@ -196,7 +192,9 @@ __global__ void __launch_bounds__(kLoadThreads) store_kernel(const __grid_consta
   const float kappa = table[z * F2C_MAX_NS_STEPS].apply;
   for (int64_t i = (int64_t)blockIdx.x * kLoadThreads + threadIdx.x; i < s.size; i += (int64_t)gridDim.x * kLoadThreads) {
     const int64_t at = z * rows * ld + i / cols * ld + i % cols;
-    finish(s, s.template result<T>(z) + i, kappa * (__half2float(high[at]) + (low != nullptr ? __half2float(low[at]) : 0.0f)));
+    const float x = kappa * (__half2float(high[at]) + (low != nullptr ? __half2float(low[at]) : 0.0f));
+    T* const out = s.template result<T>(z) + i;
+    *out = from_float<T>(s.listed ? s.keep * to_float(*out) - s.gain * x : x);
   }
 }
 
@@ -265,61 +263,84 @@ __device__ __forceinline__ void load_operand(const Operand& o, const CUtensorMap
   }
 }
 
-// One row's 32 values of the product from column `col` on, to where they belong.
-template <int MODE, typename T>
-__device__ __forceinline__ void store_values(const Params& p, const Matrices& s, const Factors& f, int z, int row, int col, const uint32_t (&r)[32], bool lost) {
-  if (row >= p.m) return;
-  const float nan = __int_as_float(0x7fffffff);
-  const __half* const add_high = MODE != kGram ? p.add_high + z * p.stack : nullptr;
-  const __half* const add_low = MODE != kGram && p.add_low != nullptr ? p.add_low + z * p.stack : nullptr;
-  const auto added = [&](int64_t at) {  // what is at [column][row] of the other matrix (As is symmetric)
-    const float high = __half2float(__ldg(add_high + at));
-    return add_low != nullptr ? high + __half2float(__ldg(add_low + at)) : high;
-  };
-  if constexpr (MODE == kFinal) {
-    T* out = s.template result<T>(z) + (int64_t)col * p.m + row;
+// 32 values at `ld` from one another, as many as there are: all on the way before the first is used
+template <typename T>
+__device__ __forceinline__ void gather(const T* from, int64_t ld, int count, float (&v)[32]) {
+  T raw[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (col + j >= p.n) break;
-      const float v = fmaf(f.own, added((int64_t)(col + j) * p.ld + row), __uint_as_float(r[j]) * f.apply);
-      finish(s, out + (int64_t)j * p.m, lost ? nan : v);
-    }
+  for (int j = 0; j < 32; ++j) raw[j] = from[min(j, count - 1) * ld];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = to_float(raw[j]);
+}
+
+template <typename T>
+__device__ __forceinline__ void scatter(T* to, int64_t ld, int count, bool mine, const T (&v)[32]) {
+  if (__all_sync(0xffffffffu, mine) && count == 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) to[j * ld] = v[j];
   } else {
-    __half* const high = p.high + z * p.stack;
-    __half* const low = p.low != nullptr ? p.low + z * p.stack : nullptr;
-    union { __half h[32]; uint4 v[4]; } hi, lo;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      float v = __uint_as_float(r[j]);
-      const bool in = col + j < p.n;
-      v *= MODE == kGram ? f.gram : MODE == kPoly ? f.poly_c : f.apply;
-      if (MODE != kGram && in) v = fmaf(MODE == kPoly ? f.poly_b : f.own, added((int64_t)(col + j) * p.ld + row), v);
-      if (lost) v = nan;
-      hi.h[j] = __float2half_rn(v);
-      lo.h[j] = __float2half_rn(v - __half2float(hi.h[j]));
-      if (in && (MODE == kApply || col + j >= row)) {
-        const int64_t at = (int64_t)(col + j) * p.ld + row;
-        high[at] = hi.h[j];
-        if (low != nullptr) low[at] = lo.h[j];
-      }
+    for (int j = 0; j < 32; ++j)
+      if (mine && j < count) to[j * ld] = v[j];
+  }
+}
+
+// A lane's row of the product, 32 values from column `col` on (which exists), to where they belong; called by whole warps, whose rows start
+// at `row0`.  A warp reads and writes 32 neighbours at a time: [column][row].  Symmetric: also [row][column], where the chunk lies above
+// the diagonal; in the chunk with the diagonal the product has both sides.
+template <int MODE, typename T>
+__device__ __forceinline__ void store_values(const Params& p, const Matrices& s, const Factors& f, int z, int row0, int col, const uint32_t (&r)[32], bool lost) {
+  const int row = row0 + (threadIdx.x & 31), count = min(32, p.n - col);
+  const bool mine = row < p.m;
+  const int64_t stack = z * p.stack, at = stack + (int64_t)col * p.ld + min(row, p.m - 1);
+  const float by = lost ? __int_as_float(0x7fffffff) : MODE == kGram ? f.gram : MODE == kPoly ? f.poly_c : f.apply;
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * by;
+  if constexpr (MODE != kGram) {
+    const float other = MODE == kPoly ? f.poly_b : f.own;
+    float more[32];
+    gather(p.add_high + at, p.ld, count, more);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = fmaf(other, more[j], v[j]);
+    if (p.add_low != nullptr) {
+      gather(p.add_low + at, p.ld, count, more);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = fmaf(other, more[j], v[j]);
     }
-    if constexpr (MODE != kApply) {  // the same on the other side of the diagonal
-      const int64_t at = (int64_t)row * p.ld + col;
-      if (col > row) {
+  }
+  if constexpr (MODE == kFinal) {
+    T* const out = s.template result<T>(z) + (int64_t)col * p.m + min(row, p.m - 1);
+    T o[32];
+    if (s.listed) {
+      float w[32];
+      gather(out, (int64_t)p.m, count, w);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (col + 8 * q >= p.n) break;
-          *reinterpret_cast<uint4*>(high + at + 8 * q) = hi.v[q];
-          if (low != nullptr) *reinterpret_cast<uint4*>(low + at + 8 * q) = lo.v[q];
-        }
-      } else {
+      for (int j = 0; j < 32; ++j) v[j] = s.keep * w[j] - s.gain * v[j];
+    }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (col + j <= row || col + j >= p.n) continue;
-          high[at + j] = hi.h[j];
-          if (low != nullptr) low[at + j] = lo.h[j];
-        }
+    for (int j = 0; j < 32; ++j) o[j] = from_float<T>(v[j]);
+    scatter(out, (int64_t)p.m, count, mine, o);
+  } else {
+    union Half { __half h[32]; uint4 v[4]; };
+    Half half;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) half.h[j] = __float2half_rn(v[j]);
+    const int64_t across = stack + (int64_t)row * p.ld + col;
+    const bool above = MODE != kApply && col > row0 && mine;
+    const auto store = [&](__half* to) {
+      scatter(to + at, p.ld, count, mine, half.h);
+      if (above) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (8 * q < count) *reinterpret_cast<uint4*>(to + across + 8 * q) = half.v[q];
       }
+    };
+    store(p.high);
+    if (p.low != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) half.h[j] = __float2half_rn(v[j] - __half2float(half.h[j]));
+      store(p.low);
     }
   }
 }
@@ -462,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         for (int c = 0; c < 2; ++c) {
           const int col = col0 + first + c * 32;
           if (c * 32 >= width || col >= p.n || (p.symmetric && col + 31 < row0)) continue;  // (wholly below the diagonal)
-          store_values<MODE, T>(p, s, f, at.z, row0 + lane, col, sum[c], lost);
+          store_values<MODE, T>(p, s, f, at.z, row0, col, sum[c], lost);
         }
         __syncwarp();
       } else {
@@ -475,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           uint32_t r[32];
           tmem_ld32(lanes + buf * (uint32_t)p.tmem + (uint32_t)c0, r);
           tmem_wait(r);
-          store_values<MODE, T>(p, s, f, at.z, row0 + lane, col0 + c0, r, lost);
+          store_values<MODE, T>(p, s, f, at.z, row0, col0 + c0, r, lost);
           __syncwarp();
         }
         fence_before();
@@ -532,7 +553,7 @@ static int x_planes(const Steps& st, int t, bool wide, bool exact) {
 }
 
 static int64_t workspace(const Shape& s, bool wide) {
-  return 4 * s.x_bytes() + (wide ? 4 : 2) * s.p_bytes() + round256(8 * s.batch * kParts) + round256((int64_t)sizeof(Factors) * F2C_MAX_NS_STEPS * s.batch);
+  return 4 * s.x_bytes() + (wide ? 4 : 2) * s.p_bytes() + round256(8 * s.batch * kMaxParts) + round256((int64_t)sizeof(Factors) * F2C_MAX_NS_STEPS * s.batch);
 }
 
 struct Planes {
@@ -607,12 +628,15 @@ static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps&
   Planes x[2], a{}, r{};
   for (Planes& q : x) { q.high = (__half*)take(s.x_bytes()); q.low = (__half*)take(s.x_bytes()); }
   for (Planes* q : {&a, &r}) { q->high = (__half*)take(s.p_bytes()); q->low = kWide ? (__half*)take(s.p_bytes()) : nullptr; }
-  double* parts = (double*)take(round256(8 * s.batch * kParts));
+  double* parts = (double*)take(round256(8 * s.batch * kMaxParts));
   Factors* table = (Factors*)take(0);
   src.size = s.rows * s.cols;
   bool four = s.cols % 4 == 0 && aligned(src.g, 4 * sizeof(T));
   for (int i = 0; i < src.listed; ++i) four = four && aligned(src.list[i].grad, 4 * sizeof(T)) && aligned(src.list[i].momentum, 16);
-  const dim3 grid(kParts, (unsigned)s.batch);
+  // 16 elements a thread, more of matrices over 4 M elements
+  int64_t cut = ceil_div(src.size, 16 * kLoadThreads);
+  if (cut > kMaxParts) cut = kMaxParts;
+  const dim3 grid((unsigned)cut, (unsigned)s.batch);
   int planes = st.count == 0 ? (exact ? 1 : 2) : x_planes(st, 0, kWide, exact);
   __half* low = planes > 1 ? x[0].low : nullptr;
   if (four) {
