@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
   const uint32_t b_bytes = (uint32_t)p.tile_rows * kK;
   unsigned char* ring = smem + (p.resident ? (size_t)steps * kABytes : 0);
   const uint32_t stage_bytes = b_bytes + (p.resident ? 0u : (uint32_t)kABytes);
-  volatile int* failed = &bars.failed;
+  uint32_t left = kWaitLimit;
 
   if (wid == 1) alloc_tmem(&bars.tmem, (uint32_t)p.tmem * p.accumulators);
   if (tid == 0) {
@@ -91,43 +91,45 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
       }
       if (p.weights_first) dependency_wait();
       release_dependents();
-      for (int item = first; item < p.items; item += stride) {
+      const uint32_t ring0 = smem_u32(ring), codes_at = p.resident ? 0u : (uint32_t)kABytes;
+      for (int item = first; item < p.items && left != 0u; item += stride) {
         const int channel0 = item % p.channel_tiles * kM, row0 = item / p.channel_tiles * p.tile_rows;
-        for (int i = 0; i < steps; ++i) {
-          if (round > 0 && !wait_bar(bars.empty + s, (round - 1) & 1, failed)) { item = p.items; break; }
-          unsigned char* stage = ring + (size_t)s * stage_bytes;
-          const bool asked = round == 0 && s < ahead;
-          if (!asked) expect(bars.full + s, stage_bytes);
-          if (!asked && !p.resident) tma_load(&w, smem_u32(stage), bars.full + s, (step0 + i) * kK, channel0);
-          tma_load(&codes, smem_u32(stage + (p.resident ? 0 : kABytes)), bars.full + s, (step0 + i) * kK, row0);
-          if (++s == p.stages) { s = 0; ++round; }
+        for (int i = 0; i < steps && left != 0u; ++i) {
+          if (round > 0) wait_bar(bars.empty + s, (round - 1) & 1, left);
+          if (left != 0u) {
+            const uint32_t stage = ring0 + (uint32_t)s * stage_bytes;
+            if (round > 0 || s >= ahead) {
+              expect(bars.full + s, stage_bytes);
+              if (!p.resident) tma_load(&w, stage, bars.full + s, (step0 + i) * kK, channel0);
+            }
+            tma_load(&codes, stage + codes_at, bars.full + s, (step0 + i) * kK, row0);
+            if (++s == p.stages) { s = 0; ++round; }
+          }
         }
-        if (item >= p.items) break;
       }
     }
   } else if (wid == 1) {
     // ================= MMAs
     if (lane == 0) {
       const uint32_t idesc = instruction(kSumS32, kFormatS8, kM, (uint32_t)p.tile_rows);
-      bool ok = !p.resident || wait_bar(&bars.weights, 0, failed);
+      const uint32_t a_low = desc_low(smem_u32(p.resident ? smem : ring), kChunkAlongK), b_low = desc_low(smem_u32(ring) + (p.resident ? 0 : kABytes), kChunkAlongK);
+      if (p.resident) wait_bar(&bars.weights, 0, left);
       uint32_t t = 0;
-      for (int item = first; ok && item < p.items; item += stride, ++t) {
-        const uint32_t buf = t & 1u;
-        if (t >= 2) ok = wait_bar(bars.acc_empty + buf, ((t >> 1) - 1) & 1, failed);
-        fence_after();
-        for (int i = 0; ok && i < steps; ++i) {
-          ok = wait_bar(bars.full + s, round & 1, failed);
-          if (!ok) break;
-          fence_after();
-          const uint32_t stage = smem_u32(ring + (size_t)s * stage_bytes);
-          const uint32_t a_addr = p.resident ? smem_u32(smem + (size_t)i * kABytes) : stage;
-          const uint32_t b_addr = p.resident ? stage : stage + kABytes;
+      for (int item = first; item < p.items && left != 0u; item += stride, ++t) {
+        const uint32_t buf = t & 1u, acc = tmem + buf * (uint32_t)p.tmem;
+        if (t >= 2) wait_bar(bars.acc_empty + buf, ((t >> 1) - 1) & 1, left);
+        for (int i = 0; i < steps && left != 0u; ++i) {
+          wait_bar(bars.full + s, round & 1, left);
+          if (left != 0u) {
+            fence_after();
+            const uint32_t at = (uint32_t)s * (stage_bytes >> 4), a = a_low + (p.resident ? (uint32_t)i * (kABytes >> 4) : at), b = b_low + at;
 #pragma unroll
-          for (int q = 0; q < kK / 32; ++q) mma_i8(tmem + buf * (uint32_t)p.tmem, desc_k(a_addr + q * 32), desc_k(b_addr + q * 32), idesc, i + q != 0 ? 1u : 0u);
-          commit(bars.empty + s);
-          if (++s == p.stages) { s = 0; ++round; }
+            for (uint32_t q = 0; q < kK / 32; ++q) mma_i8(acc, desc(a + q * kStepAlongK), desc(b + q * kStepAlongK), idesc, i + (int)q != 0 ? 1u : 0u);
+            commit(bars.empty + s);
+            if (++s == p.stages) { s = 0; ++round; }
+          }
         }
-        if (ok) commit(bars.acc_full + buf);
+        if (left != 0u) commit(bars.acc_full + buf);
       }
     }
   } else {
@@ -146,7 +148,8 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
       const float w_scale = mine ? __ldg(p.b_scales + channel) : 0.0f, bias = mine && p.bias != nullptr ? __ldg(p.bias + channel) : 0.0f;
       for (int c = lane; c < rows; c += 32) row_scale[c] = __ldg(p.a_scales + row0 + c);
       __syncwarp();
-      const bool lost = steps > 0 && !__all_sync(0xffffffffu, wait_bar(bars.acc_full + buf, (t >> 1) & 1, failed));
+      if (steps > 0) wait_bar(bars.acc_full + buf, (t >> 1) & 1, left);
+      const bool lost = __any_sync(0xffffffffu, left == 0u);
       fence_after();
       const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)p.tmem;
       for (int c0 = half * 32; c0 < rows; c0 += 64) {
@@ -176,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
       if (lane == 0) arrive(bars.acc_empty + buf);
     }
   }
+  if (left == 0u) bars.failed = 1;
   if (p.split > 1) {
     // a cluster has one tile, whose rows its CTAs share: all sums have been told when all have got here
     __syncwarp();
@@ -205,16 +209,16 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
   __syncthreads();
   if (bars.failed) {
     // copies in flight write to this CTA's shared memory, MMAs in flight read it and write its TMEM: wait (bounded) for what was issued
-    volatile int expired = 0;
+    left = kWaitLimit;
     if (tid == 0) {
-      if (p.resident) wait_bar(&bars.weights, 0, &expired);
+      if (p.resident) wait_bar(&bars.weights, 0, left);
       for (int q = 0; q < p.stages; ++q) {
         const uint32_t uses = round + (q < s ? 1u : 0u);
-        if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, &expired);
+        if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
       }
     } else if (tid == 32) {
       commit(&bars.drain);
-      wait_bar(&bars.drain, 0, &expired);
+      wait_bar(&bars.drain, 0, left);
     }
     __syncthreads();
   }

@@ -14,9 +14,9 @@
 //    factors a, 3.4445^4 = 140 after the first, while large singular values only go to one: where that product is over 16, X is a pair of
 //    half precision numbers (22 bits) and R X two products.  For matrices of rank 8 the result is 2.6e-3 off then, and 2.6e-2 without.
 //  * 32-bit matrices.  All operands are pairs, a product is three (high by high, high by low, low by high): 22 bits throughout.  The tensor
-//    cores cut sums off instead of rounding them, for every 16 elements of K.  So the two small products have an accumulator of their own, the
-//    large one's sum is taken out every 128 elements and added up in registers, and a X is not in it.  (Rank 3, 400 x 600: 2.5e-4 off without
-//    any of this, 2e-4 without the taking out.)
+//    cores cut sums off instead of rounding them, for every 16 elements of K.  So the sums are taken out every 64 elements and added up in
+//    registers, the small products are in front of the large one, and a X is not in the sum.  (Rank 3, 400 x 600: 2.5e-4 off without any of this,
+//    2e-4 without the taking out.)
 #include <math.h>
 
 #include "tcgen05.cuh"
@@ -27,8 +27,10 @@ namespace ns {
 using namespace t5;
 
 constexpr int kMaxParts = 1024, kLoadThreads = 256;  // parts of a matrix' norm
-constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;  // warp 0: TMA, warp 1: MMA, then the epilogue's
-constexpr int kChunk = 2;                    // steps of K after which float32's sums are taken out of the tensor cores' hands
+constexpr int kFirstEpilogueWarp = 4, kEpilogueWarps = 8, kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);  // warp 0: TMA, warp 1: MMA
+// float32: 128 sums a thread.  What a CTA is launched with, 168 registers a thread, is shared out anew.
+constexpr int kRegisters = 168, kFewRegisters = 40, kManyRegisters = 232;
+static_assert(32 * (kFirstEpilogueWarp * kFewRegisters + kEpilogueWarps * kManyRegisters) <= kThreads * kRegisters, "registers of a CTA");
 constexpr int kM = 128, kK = 64, kMaxN = 256, kMaxStages = 8, kMaxList = 64;
 constexpr size_t kRoom = kSmemLimit - 1024;  // dynamic shared memory
 constexpr int kScaleLog = 10;                // norms are brought to 2^10
@@ -202,17 +204,19 @@ __global__ void __launch_bounds__(kLoadThreads) store_kernel(const __grid_consta
 enum Mode { kGram, kPoly, kApply, kFinal };
 
 struct Operand {
-  int rows;     // of a tile
+  int rows;     // of a CTA's part of a tile
   int turned;   // its rows run along K
   int planes;   // 1 or 2
-  __host__ __device__ int bytes() const { return rows * kK * 2; }
+  __host__ __device__ int bytes(int chunks) const { return rows * kK * 2 * chunks; }
 };
 
 struct Params {
   Operand a, b;
   int m, n, steps;                 // M, N of the product; steps of K
   int row_tiles, col_tiles, items; // row tiles along M; items of one matrix
-  int batch, stages, accumulators, tmem;  // accumulators: of 16-bit matrices; tmem: columns of one
+  int batch, stages;
+  int chunks;                      // of 64 elements of K in a stage (of which there are `steps`)
+  int ctas;                        // that share a tile: of 128 rows each
   int symmetric;
   const Factors* factors;          // of this step
   const __half *add_high, *add_low;  // kPoly: As; kApply, kFinal: Xs
@@ -222,7 +226,7 @@ struct Params {
 };
 
 struct Bars {
-  uint64_t full[kMaxStages], empty[kMaxStages], drain, acc_full[2], acc_empty[2], small_empty[2];
+  uint64_t full[kMaxStages], empty[kMaxStages], drain, acc_full[2], acc_empty[2];
   uint32_t tmem;
   int failed;
 };
@@ -241,25 +245,13 @@ __device__ __forceinline__ Tile tile_of(const Params& p, int item) {
     return t;
   }
   t.row = 0;
-  for (int first = 0;; first = t.row * kM / p.b.rows) {
+  for (int first = 0;; first = t.row * kM / p.b.rows) {  // (rows and columns of a tile have the same factor, ctas)
     if (i < p.col_tiles - first) {
       t.col = first + i;
       return t;
     }
     i -= p.col_tiles - first;
     ++t.row;
-  }
-}
-
-__device__ __forceinline__ uint64_t descriptor(const Operand& o, uint32_t addr, int q) {  // of 16 elements of K, the q-th in a step
-  return o.turned ? desc_mn(addr + (uint32_t)q * 2048u, kK * 128) : desc_k(addr + (uint32_t)q * 32u);
-}
-
-__device__ __forceinline__ void load_operand(const Operand& o, const CUtensorMap* map, uint32_t dst, const uint64_t* bar, int k0, int at, int z) {
-  if (!o.turned) {
-    tma_load(map, dst, bar, k0, at, z);
-  } else {
-    for (int c = 0; c < o.rows / 64; ++c) tma_load(map, dst + (uint32_t)c * (kK * 128), bar, at + c * 64, k0, z);
   }
 }
 
@@ -350,180 +342,211 @@ __device__ __forceinline__ void add(uint32_t (&sum)[32], const uint32_t (&r)[32]
   for (int j = 0; j < 32; ++j) sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(r[j]));
 }
 
-template <int MODE, typename T>
+// CTAS 2: the two CTAs of a cluster work on 256 rows, each with 128 of them and half of the columns' operand in its shared memory; the
+// first one issues the MMAs for both.
+template <int MODE, typename T, int CTAS>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, const __grid_constant__ Matrices s) {
   constexpr bool kWide = sizeof(T) == 4;  // pairs by pairs: see above
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const int rank = (int)blockIdx.x % CTAS, first = (int)blockIdx.x / CTAS, stride = (int)gridDim.x / CTAS;
   const int total = p.items * p.batch;
-  const uint32_t a_bytes = (uint32_t)p.a.bytes(), b_bytes = (uint32_t)p.b.bytes();
+  const uint32_t a_bytes = (uint32_t)p.a.bytes(p.chunks), b_bytes = (uint32_t)p.b.bytes(p.chunks);  // of a plane of a stage
   const uint32_t b_at = a_bytes * p.a.planes, stage_bytes = b_at + b_bytes * p.b.planes;
-  volatile int* failed = &bars.failed;
+  const int columns = p.b.rows * CTAS;  // of a tile
+  const uint32_t tmem_columns = (uint32_t)columns * 2;  // two accumulators
+  uint32_t left = kWaitLimit;
 
-  if (wid == 1) alloc_tmem(&bars.tmem, (uint32_t)p.tmem * (kWide ? 4u : (uint32_t)p.accumulators));
+  if (wid == 1) {
+    if (CTAS == 2) alloc_tmem_pair(&bars.tmem, tmem_columns);
+    else alloc_tmem(&bars.tmem, tmem_columns);
+  }
   if (tid == 0) {
     for (int q = 0; q < p.stages; ++q) { init_bar(bars.full + q, 1); init_bar(bars.empty + q, 1); }
     init_bar(&bars.drain, 1);
-    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps); init_bar(bars.small_empty + b, kEpilogueWarps); }
+    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps * CTAS); }
     fence_bars();
     bars.failed = 0;
   }
   fence_before();
   __syncthreads();
+  if (CTAS == 2) cluster_barrier();  // the other one's barriers are there
   fence_after();
   const uint32_t tmem = bars.tmem;
   int slot = 0;
   uint32_t round = 0;
 
-  if (wid == 0) {
-    // ================= loads
-    if (lane == 0) {
+  if (wid < kFirstEpilogueWarp) {
+    if constexpr (kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    if (wid != 1 && lane == 0) {
+      // ================= loads: a thread of its own for each operand, and one for their low planes
       dependency_wait();
-      release_dependents();
-      for (int item = blockIdx.x; item < total; item += gridDim.x) {
+      if (wid == 0) release_dependents();
+      const bool high = wid != 3, of_a = high ? wid == 0 : p.a.planes > 1, of_b = high ? wid == 2 : p.b.planes > 1;
+      const uint32_t smem0 = smem_u32(smem) + (high ? 0u : a_bytes), b_low_at = b_at - (high ? 0u : a_bytes) + (high ? 0u : b_bytes);
+      const uint32_t bars0 = CTAS == 2 ? peer_address(smem_u32(bars.full), 0) : smem_u32(bars.full);
+      const int depth = p.chunks * kK;
+      const auto load = [&](const Operand& o, const CUtensorMap* map, uint32_t dst, uint32_t bar, int k, int at, int z) {
+        const int boxes = o.turned ? o.rows / 64 : p.chunks, box_bytes = o.turned ? depth * 128 : o.rows * 128;
+        int x = o.turned ? at : k;
+        const int y = o.turned ? k : at;
+        for (int c = 0; c < boxes; ++c, x += 64, dst += (uint32_t)box_bytes) {
+          if (CTAS == 2) tma_load_pair(map, dst, bar, x, y, z);
+          else tma_load(map, dst, bar, x, y, z);
+        }
+      };
+      for (int item = of_a || of_b ? first : total; item < total && left != 0u; item += stride) {
         const Tile t = tile_of(p, item);
-        int i = 0;
-        for (; i < p.steps; ++i) {
-          if (round > 0 && !wait_bar(bars.empty + slot, (round - 1) & 1, failed)) break;
-          const uint32_t stage = smem_u32(smem + (size_t)slot * stage_bytes);
-          expect(bars.full + slot, stage_bytes);
-          for (int q = 0; q < p.a.planes; ++q) load_operand(p.a, maps.a + q, stage + q * a_bytes, bars.full + slot, i * kK, t.row * kM, t.z);
-          for (int q = 0; q < p.b.planes; ++q) load_operand(p.b, maps.b + q, stage + b_at + q * b_bytes, bars.full + slot, i * kK, t.col * p.b.rows, t.z);
-          if (++slot == p.stages) { slot = 0; ++round; }
+        const int a_row = (t.row * CTAS + rank) * kM, b_row = t.col * columns + rank * p.b.rows;
+        for (int i = 0; i < p.steps && left != 0u; ++i) {
+          if (round > 0) wait_bar(bars.empty + slot, (round - 1) & 1, left);
+          if (left != 0u) {
+            const uint32_t stage = smem0 + (uint32_t)slot * stage_bytes, bar = bars0 + (uint32_t)slot * 8u;
+            if (wid == 0 && rank == 0) expect(bars.full + slot, stage_bytes * CTAS);
+            if (of_a) load(p.a, high ? &maps.a[0] : &maps.a[1], stage, bar, i * depth, a_row, t.z);
+            if (of_b) load(p.b, high ? &maps.b[0] : &maps.b[1], stage + b_low_at, bar, i * depth, b_row, t.z);
+            if (++slot == p.stages) { slot = 0; ++round; }
+          }
         }
-        if (i < p.steps) break;
       }
-    }
-  } else if (wid == 1) {
-    // ================= MMAs
-    if (lane == 0) {
-      const uint32_t idesc = instruction(kSumF32, kFormatF16, kM, (uint32_t)p.b.rows) | (p.a.turned ? kTurnedA : 0u) | (p.b.turned ? kTurnedB : 0u);
-      bool ok = true;
-      uint32_t t = 0, chunk = 0;
-      for (int item = blockIdx.x; ok && item < total; item += gridDim.x, ++t) {
-        const uint32_t turn = t / (uint32_t)p.accumulators, buf = t % (uint32_t)p.accumulators;
-        uint32_t acc = tmem + buf * (uint32_t)p.tmem;                      // 16-bit matrices: all sums of the tile
-        const uint32_t small = tmem + (2u + (t & 1u)) * (uint32_t)p.tmem;  // float32: those of the small products
-        if constexpr (kWide) {
-          if (t >= 2) ok = wait_bar(bars.small_empty + (t & 1u), ((t >> 1) - 1) & 1, failed);
-        } else {
-          if (turn > 0) ok = wait_bar(bars.acc_empty + buf, (turn - 1) & 1, failed);
-        }
-        for (int i = 0; ok && i < p.steps; ++i) {
-          const bool fresh = kWide && i % kChunk == 0;
-          if (fresh) {
-            if (chunk >= 2) ok = wait_bar(bars.acc_empty + (chunk & 1u), ((chunk >> 1) - 1) & 1, failed);
-            acc = tmem + (chunk & 1u) * (uint32_t)p.tmem;
-          }
-          ok = ok && wait_bar(bars.full + slot, round & 1, failed);
-          if (!ok) break;
-          fence_after();
-          const uint32_t a = smem_u32(smem + (size_t)slot * stage_bytes), b = a + b_at;
+    } else if (wid == 1 && lane == 0 && rank == 0) {
+      // ================= MMAs
+      const uint32_t idesc = instruction(kSumF32, kFormatF16, kM * CTAS, (uint32_t)columns) | (p.a.turned ? kTurnedA : 0u) | (p.b.turned ? kTurnedB : 0u);
+      const auto done = [&](const uint64_t* bar) {
+        if (CTAS == 2) commit_pair(bar);
+        else commit(bar);
+      };
+      const uint32_t low = desc_low(smem_u32(smem), 0), a_low = low | desc_low(0, p.a.turned ? p.chunks * kK * 128 : kChunkAlongK);
+      const uint32_t b_low = (low | desc_low(0, p.b.turned ? p.chunks * kK * 128 : kChunkAlongK)) + (b_at >> 4);
+      const uint32_t a_step = p.a.turned ? kStepTurned : kStepAlongK, b_step = p.b.turned ? kStepTurned : kStepAlongK;
+      const uint32_t a_chunk = p.a.turned ? 4 * kStepTurned : (uint32_t)p.a.rows * 8u, b_chunk = p.b.turned ? 4 * kStepTurned : (uint32_t)p.b.rows * 8u;
+      const auto product = [&](uint32_t acc, uint32_t a, uint32_t b, bool more) {  // of a stage
+        for (int c = 0; c < p.chunks; ++c, a += a_chunk, b += b_chunk) {
 #pragma unroll
-          for (int q = 0; q < kK / 16; ++q) {
-            const uint64_t a_high = descriptor(p.a, a, q), b_high = descriptor(p.b, b, q);
-            mma_f16(acc, a_high, b_high, idesc, (fresh || i == 0) && q == 0 ? 0u : 1u);
-            if (p.a.planes > 1) mma_f16(kWide ? small : acc, descriptor(p.a, a + a_bytes, q), b_high, idesc, kWide && i + q == 0 ? 0u : 1u);
-            if (p.b.planes > 1) mma_f16(kWide ? small : acc, a_high, descriptor(p.b, b + b_bytes, q), idesc, 1u);
-          }
-          commit(bars.empty + slot);
-          if (++slot == p.stages) { slot = 0; ++round; }
-          if (kWide && (i % kChunk == kChunk - 1 || i + 1 == p.steps)) {
-            commit(bars.acc_full + (chunk & 1u));
-            ++chunk;
+          for (uint32_t q = 0; q < kK / 16; ++q) {
+            const uint32_t on = more || c + (int)q != 0 ? 1u : 0u;
+            if (CTAS == 2) mma_f16_pair(acc, desc(a + q * a_step), desc(b + q * b_step), idesc, on);
+            else mma_f16(acc, desc(a + q * a_step), desc(b + q * b_step), idesc, on);
           }
         }
-        if (!kWide && ok) commit(bars.acc_full + buf);
+      };
+      uint32_t n = 0;  // accumulations begun: one a tile, or (float32) one a step
+      uint32_t acc = tmem;
+      for (int item = first; item < total && left != 0u; item += stride) {
+        for (int i = 0; i < p.steps && left != 0u; ++i) {
+          const bool fresh = kWide || i == 0;
+          if (fresh) {
+            acc = tmem + (n & 1u) * (uint32_t)columns;
+            if (n >= 2) wait_bar(bars.acc_empty + (n & 1u), ((n >> 1) - 1) & 1, left);
+          }
+          wait_bar(bars.full + slot, round & 1, left);
+          if (left != 0u) {
+            fence_after();
+            const uint32_t at = (uint32_t)slot * (stage_bytes >> 4), a = a_low + at, b = b_low + at;
+            // the small products first: what is cut off their sums is as small as they are
+            if (p.a.planes > 1) product(acc, a + (a_bytes >> 4), b, !fresh);
+            if (p.b.planes > 1) product(acc, a, b + (b_bytes >> 4), !fresh || p.a.planes > 1);
+            product(acc, a, b, !fresh || p.a.planes > 1 || p.b.planes > 1);
+            done(bars.empty + slot);
+            if (++slot == p.stages) { slot = 0; ++round; }
+            if (kWide || i + 1 == p.steps) {
+              done(bars.acc_full + (n & 1u));
+              ++n;
+            }
+          }
+        }
       }
     }
   } else {
     // ================= epilogue: a warp has the TMEM lanes of its quarter and half of the columns, thread = row
-    const int quarter = wid & 3, half = (wid - 2) >> 2;
+    if constexpr (kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    const int quarter = wid & 3, half = (wid - kFirstEpilogueWarp) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    uint32_t t = 0, chunk = 0;
-    bool lost = false;
+    const auto leave = [&](uint32_t buf) {  // the accumulator has been read
+      fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CTAS == 2) peer_arrive(peer_address(smem_u32(bars.acc_empty + buf), 0));
+        else arrive(bars.acc_empty + buf);
+      }
+    };
+    uint32_t n = 0;
     dependency_wait();
-    for (int item = blockIdx.x; item < total; item += gridDim.x, ++t) {
+    for (int item = first; item < total; item += stride) {
       const Tile at = tile_of(p, item);
-      const int row0 = at.row * kM + quarter * 32, col0 = at.col * p.b.rows;
+      const int row0 = (at.row * CTAS + rank) * kM + quarter * 32, col0 = at.col * columns;
       const Factors f = p.factors[at.z * F2C_MAX_NS_STEPS];
       if constexpr (kWide) {
-        // sums of kChunk steps each are added up here, where additions round
-        uint32_t sum[2][32] = {};
-        const int width = p.b.rows / 2, first = half * width;
-        for (int i = 0; i < p.steps; i += kChunk, ++chunk) {
-          lost = lost || !__all_sync(0xffffffffu, wait_bar(bars.acc_full + (chunk & 1u), (chunk >> 1) & 1, failed));
+        // the sums of the steps are added up here, where additions round
+        uint32_t sum[4][32] = {};
+        const int width = columns / 2, mine = half * width;
+        for (int i = 0; i < p.steps; ++i, ++n) {
+          const uint32_t turn = n >> 1, buf = n & 1u;
+          wait_bar(bars.acc_full + buf, turn & 1, left);
+          __syncwarp();
           fence_after();
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 4; ++c) {
             if (c * 32 >= width) break;
             uint32_t r[32];
-            tmem_ld32(lanes + (chunk & 1u) * (uint32_t)p.tmem + (uint32_t)(first + c * 32), r);
+            tmem_ld32(lanes + buf * (uint32_t)columns + (uint32_t)(mine + c * 32), r);
             tmem_wait(r);
             add(sum[c], r);
           }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive(bars.acc_empty + (chunk & 1u));
+          leave(buf);
         }
+        const bool lost = __any_sync(0xffffffffu, left == 0u);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (c * 32 >= width) break;
-          uint32_t r[32];
-          tmem_ld32(lanes + (2u + (t & 1u)) * (uint32_t)p.tmem + (uint32_t)(first + c * 32), r);
-          tmem_wait(r);
-          add(sum[c], r);
-        }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) arrive(bars.small_empty + (t & 1u));
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = col0 + first + c * 32;
+        for (int c = 0; c < 4; ++c) {
+          const int col = col0 + mine + c * 32;
           if (c * 32 >= width || col >= p.n || (p.symmetric && col + 31 < row0)) continue;  // (wholly below the diagonal)
           store_values<MODE, T>(p, s, f, at.z, row0, col, sum[c], lost);
         }
         __syncwarp();
       } else {
-        const uint32_t turn = t / (uint32_t)p.accumulators, buf = t % (uint32_t)p.accumulators;
-        const int cols = min(p.b.rows, p.n - col0);
-        lost = lost || !__all_sync(0xffffffffu, wait_bar(bars.acc_full + buf, turn & 1, failed));
+        const uint32_t turn = n >> 1, buf = n & 1u;
+        const int cols = min(columns, p.n - col0);
+        wait_bar(bars.acc_full + buf, turn & 1, left);
+        const bool lost = __any_sync(0xffffffffu, left == 0u);
         fence_after();
         for (int c0 = half * 32; c0 < cols; c0 += 64) {
           if (p.symmetric && col0 + c0 + 31 < row0) continue;
           uint32_t r[32];
-          tmem_ld32(lanes + buf * (uint32_t)p.tmem + (uint32_t)c0, r);
+          tmem_ld32(lanes + buf * (uint32_t)columns + (uint32_t)c0, r);
           tmem_wait(r);
           store_values<MODE, T>(p, s, f, at.z, row0, col0 + c0, r, lost);
           __syncwarp();
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) arrive(bars.acc_empty + buf);
+        leave(buf);
+        ++n;
       }
     }
   }
+  if (left == 0u) bars.failed = 1;
+  __syncwarp();
   fence_before();
   __syncthreads();
-  if (bars.failed) {
-    // copies in flight write to this CTA's shared memory, MMAs in flight read it and write its TMEM: wait (bounded) for what was issued
-    volatile int expired = 0;
+  if (bars.failed && rank == 0) {
+    // copies in flight write to shared memory, MMAs in flight read it and write TMEM, of both CTAs: wait (bounded) for what was issued
+    left = kWaitLimit;
     if (tid == 0) {
       for (int q = 0; q < p.stages; ++q) {
         const uint32_t uses = round + (q < slot ? 1u : 0u);
-        if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, &expired);
+        if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
       }
     } else if (tid == 32) {
       commit(&bars.drain);
-      wait_bar(&bars.drain, 0, &expired);
+      wait_bar(&bars.drain, 0, left);
     }
     __syncthreads();
   }
+  if (CTAS == 2) cluster_barrier();
   if (wid == 1) {
     fence_after();
-    free_tmem(tmem, (uint32_t)p.tmem * (kWide ? 4u : (uint32_t)p.accumulators));
+    if (CTAS == 2) free_tmem_pair(tmem, tmem_columns);
+    else free_tmem(tmem, tmem_columns);
   }
   if (tid == 0 && bars.failed) report_wait(p.error, 5);
 }
@@ -560,16 +583,24 @@ struct Planes {
   __half *high, *low;
 };
 
-// Columns of a tile: as many as leave every SM a tile, or so few that more SMs than not have one.
-static int tile_columns(int64_t rows_m, int64_t cols_n, int64_t batch, bool symmetric, int most, int sms) {
-  for (int n = most; n > 64; n /= 2) {
-    int64_t items = 0;
-    const int64_t rt = ceil_div(rows_m, kM), ct = ceil_div(cols_n, n);
-    if (symmetric) for (int64_t i = 0; i < rt; ++i) items += ct - i * kM / n;
-    else items = rt * ct;
-    if (items * batch >= sms) return n;
-  }
-  return 64;
+// Tiles of one matrix' product.
+static int64_t tiles(int64_t m, int64_t n, int rows, int columns, bool symmetric) {
+  const int64_t rt = ceil_div(m, rows), ct = ceil_div(n, columns);
+  if (!symmetric) return rt * ct;
+  int64_t items = 0;
+  for (int64_t i = 0; i < rt; ++i) items += ct - i * rows / columns;
+  return items;
+}
+
+struct Tiling { int ctas, columns; };
+
+// Tiles of 256 x 256 for two CTAs, which read a third less for a product than CTAs of their own with 128 x 256, where there are enough of them; else 128 rows and
+// as many columns as leave every SM a tile.
+static Tiling tiling(int64_t m, int64_t n, int64_t batch, bool symmetric, int sms) {
+  if (tiles(m, n, 2 * kM, kMaxN, symmetric) * batch >= sms / 2) return Tiling{2, kMaxN};
+  for (int columns = kMaxN; columns > 64; columns /= 2)
+    if (tiles(m, n, kM, columns, symmetric) * batch >= sms) return Tiling{1, columns};
+  return Tiling{1, 64};
 }
 
 struct Product {
@@ -584,25 +615,22 @@ template <int MODE, typename T>
 static int multiply(const char* op, const Product& x, Params p, const Matrices& s, int64_t batch, cudaStream_t st) {
   const int sms = current_sm_count();
   p.m = (int)x.m; p.n = (int)x.n;
-  p.steps = (int)ceil_div(x.k, kK);
+  p.chunks = x.a_planes + x.b_planes > 2 ? 1 : 2;  // eight MMAs to a wait at least
+  p.steps = (int)ceil_div(x.k, kK * p.chunks);
   p.symmetric = x.symmetric;
   p.batch = (int)batch;
+  const Tiling shape = tiling(x.m, x.n, batch, x.symmetric, sms);
+  p.ctas = shape.ctas;
   p.a = Operand{kM, x.a_turned, x.a_planes};
-  p.b = Operand{tile_columns(x.m, x.n, batch, x.symmetric, sizeof(T) == 4 ? 128 : kMaxN, sms), x.b_turned, x.b_planes};
-  p.row_tiles = (int)ceil_div(x.m, kM);
-  p.col_tiles = (int)ceil_div(x.n, p.b.rows);
-  p.items = p.row_tiles * p.col_tiles;
-  if (x.symmetric) {
-    p.items = 0;
-    for (int i = 0; i < p.row_tiles; ++i) p.items += p.col_tiles - i * kM / p.b.rows;
-  }
-  const int64_t total = (int64_t)p.items * batch;
-  F2C_REQUIRE(total < (1ll << 31), F2C_ERR_LIMIT, "%s: too many tiles", op);
-  const unsigned grid = (unsigned)(total < sms ? total : sms);
-  p.tmem = p.b.rows;
-  p.accumulators = total > grid ? 2 : 1;
+  p.b = Operand{shape.columns / shape.ctas, x.b_turned, x.b_planes};
+  p.row_tiles = (int)ceil_div(x.m, kM * shape.ctas);
+  p.col_tiles = (int)ceil_div(x.n, shape.columns);
+  p.items = (int)tiles(x.m, x.n, kM * shape.ctas, shape.columns, x.symmetric);
+  const int64_t total = (int64_t)p.items * batch, places = sms / shape.ctas;
+  F2C_REQUIRE(total < (1ll << 30), F2C_ERR_LIMIT, "%s: too many tiles", op);
+  const unsigned grid = (unsigned)((total < places ? total : places) * shape.ctas);
   p.error = stream_error_word();
-  const size_t stage = (size_t)p.a.bytes() * p.a.planes + (size_t)p.b.bytes() * p.b.planes, room = kRoom - 1024;
+  const size_t stage = (size_t)p.a.bytes(p.chunks) * p.a.planes + (size_t)p.b.bytes(p.chunks) * p.b.planes, room = kRoom - 1024;
   p.stages = (int)(room / stage);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   Maps maps;
@@ -610,13 +638,13 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
   const __half* bp[2] = {x.b.high, x.b.low};
   bool ok = true;
   for (int q = 0; q < 2; ++q) {
-    ok = ok && make_stack_map(maps.a + q, ap[q < x.a_planes ? q : 0], batch, x.a_rows, x.a_cols, 2 * x.a_ld, x.a_turned ? kK : kM);
-    ok = ok && make_stack_map(maps.b + q, bp[q < x.b_planes ? q : 0], batch, x.b_rows, x.b_cols, 2 * x.b_ld, x.b_turned ? kK : p.b.rows);
+    ok = ok && make_stack_map(maps.a + q, ap[q < x.a_planes ? q : 0], batch, x.a_rows, x.a_cols, 2 * x.a_ld, x.a_turned ? kK * p.chunks : kM);
+    ok = ok && make_stack_map(maps.b + q, bp[q < x.b_planes ? q : 0], batch, x.b_rows, x.b_cols, 2 * x.b_ld, x.b_turned ? kK * p.chunks : p.b.rows);
   }
   F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
-  auto* kern = product_kernel<MODE, T>;
-  if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom)) return rc;
-  launch_dependent(kern, dim3(grid), kThreads, p.stages * stage + 1024, st, maps, p, s);
+  auto* kern = shape.ctas == 2 ? product_kernel<MODE, T, 2> : product_kernel<MODE, T, 1>;
+  if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom, sizeof(T) == 4 ? kRegisters : 0)) return rc;
+  launch_dependent_cluster(kern, dim3(grid), kThreads, p.stages * stage + 1024, (unsigned)shape.ctas, st, maps, p, s);
   return check_launch(op);
 }
 

@@ -11,7 +11,7 @@ int* stream_error_word();
 namespace t5 {
 
 constexpr size_t kSmemLimit = 227 * 1024;
-constexpr uint32_t kWaitLimit = 1u << 22;  // tries of a wait, each of which may take the hardware's own time
+constexpr uint32_t kWaitLimit = 1u << 20, kWaitHint = 1000;  // tries, and nanoseconds that one may take
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -25,18 +25,17 @@ __device__ __forceinline__ void expect(const uint64_t* bar, uint32_t bytes) {
 }
 __device__ __forceinline__ void fence_bars() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 
-// false when the limit ran out or another role of the CTA has given up
-__device__ __forceinline__ bool wait_bar(const uint64_t* bar, uint32_t parity, volatile int* failed) {
-  uint32_t done = 0;
-  for (uint32_t it = 0; it < kWaitLimit; ++it) {
+// Waits for a phase, or until `left`, the tries that a role has for all its waits, is 0: then it gives up, and its loops end.  (They end by their
+// conditions alone: a `break` behind the wait took the thread 120 cycles more, three quarters of what there is for a step's loads.)
+__device__ __forceinline__ void wait_bar(const uint64_t* bar, uint32_t parity, uint32_t& left) {
+  const uint32_t at = smem_u32(bar);
+  uint32_t done;
+  do {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (done) return true;
-    if ((it & 255u) == 255u && *failed) return false;
-  }
-  *failed = 1;
-  return false;
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done) : "r"(at), "r"(parity), "r"(kWaitHint) : "memory");
+    left -= done ? 0u : 1u;
+  } while (!done && left != 0u);
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -52,6 +51,15 @@ __device__ __forceinline__ void alloc_tmem(uint32_t* at, uint32_t columns) {
 }
 __device__ __forceinline__ void free_tmem(uint32_t tmem, uint32_t columns) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+
+// The same in both CTAs of a pair, by one warp of each.
+__device__ __forceinline__ void alloc_tmem_pair(uint32_t* at, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void free_tmem_pair(uint32_t tmem, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
 // 32 columns from `taddr` on, of the 32 lanes that the warp owns
@@ -76,20 +84,15 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
 }
 
 // ---------------------------------------------------------------- MMAs
-// Operands in shared memory, 128-byte swizzle, atoms of 8 x 128 bytes that start on 1024.
-// Rows of 128 bytes along K: row r at 128 r.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-  const uint32_t lo = ((addr & 0x3FFFFu) >> 4) | (1u << 16);
-  const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-  return ((uint64_t)hi << 32) | lo;
-}
-
-// Rows of 128 bytes along M or N, one row for every element of K: K row r of 64 elements at 128 r, the next 64 elements `chunk` bytes further.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t chunk) {
-  const uint32_t lo = ((addr & 0x3FFFFu) >> 4) | ((chunk >> 4) << 16);
-  const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-  return ((uint64_t)hi << 32) | lo;
-}
+// Operands in shared memory, 128-byte swizzle, atoms of 8 x 128 bytes that start on 1024.  A descriptor's low word holds the address in 16 bytes, to
+// which offsets are added as they are: the thread that issues MMAs has few cycles for each.
+//  * along K: row r of 128 bytes at 128 r, 32 bytes of K to an MMA
+//  * along M or N, one row for every element of K: K row r of 64 elements at 128 r, the next 64 elements `chunk` bytes further; 16 K rows to an MMA
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t chunk) { return ((addr & 0x3FFFFu) >> 4) | ((chunk >> 4) << 16); }
+constexpr uint32_t kChunkAlongK = 16;                                     // (has no meaning there)
+constexpr uint32_t kStepAlongK = 32 >> 4, kStepTurned = 16 * 128 >> 4;    // from one MMA's operand to the next
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);    // 1024 bytes from atom to atom, sm_100, 128-byte swizzle
+__device__ __forceinline__ uint64_t desc(uint32_t low) { return ((uint64_t)kDescHigh << 32) | low; }
 
 constexpr uint32_t kTurnedA = 1u << 15, kTurnedB = 1u << 16;  // of an instruction: the operand lies along M or N
 constexpr uint32_t kFormatF16 = 0, kFormatS8 = 1, kSumF32 = 1, kSumS32 = 2;
@@ -113,6 +116,20 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b,
       : "memory");
 }
 
+// Over both CTAs of a pair: half of the rows of A and of the columns of B in the shared memory of each, at the same offsets.
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}\n" ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc),
+      "r"(accumulate), "r"(0u)
+      : "memory");
+}
+// arrives at the barrier, in both CTAs of a pair, when all MMAs of the pair issued so far by this thread are complete
+__device__ __forceinline__ void commit_pair(const uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+               : "memory");
+}
+
 // arrives at the barrier when all MMAs issued so far by this thread are complete
 __device__ __forceinline__ void commit(const uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -124,9 +141,15 @@ __device__ __forceinline__ void tma_load(const CUtensorMap* map, uint32_t dst, c
                "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ void tma_load(const CUtensorMap* map, uint32_t dst, const uint64_t* bar, int x, int y, int z) {
+__device__ __forceinline__ void tma_load(const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-               "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+// The same in a pair of CTAs: `bar`, at which the bytes are counted, is a cluster address and may be the other one's.
+__device__ __forceinline__ void tma_load_pair(const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
@@ -139,6 +162,9 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
+}
+__device__ __forceinline__ void peer_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void peer_store(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 
