@@ -75,62 +75,59 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
 
   if (wid == 0) {
     // ================= loads
-    if (lane == 0) {
+    const bool mine = elected() != 0u;
+    if (mine) {
       prefetch_map(&codes);
       prefetch_map(&w);
-      if (!p.weights_first) dependency_wait();
-      int ahead = 0;  // stages whose weights have been asked for
-      if (p.resident) {
-        expect(&bars.weights, (uint32_t)steps * kABytes);
-        for (int i = 0; i < steps; ++i) tma_load(&w, smem_u32(smem + (size_t)i * kABytes), &bars.weights, (step0 + i) * kK, first % p.channel_tiles * kM);
-      } else if (p.weights_first) {
-        for (; ahead < min(p.stages, steps); ++ahead) {
-          expect(bars.full + ahead, stage_bytes);
-          tma_load(&w, smem_u32(ring + (size_t)ahead * stage_bytes), bars.full + ahead, (step0 + ahead) * kK, first % p.channel_tiles * kM);
-        }
+    }
+    __syncwarp();
+    if (!p.weights_first) dependency_wait();
+    const uint32_t ring0 = smem_u32(ring), codes_at = p.resident ? 0u : (uint32_t)kABytes, bars0 = smem_u32(bars.full);
+    int ahead = 0;  // stages whose weights have been asked for
+    if (p.resident) {
+      expect_if(mine, &bars.weights, (uint32_t)steps * kABytes);
+      for (int i = 0; i < steps; ++i) tma_load(mine, &w, smem_u32(smem) + (uint32_t)i * kABytes, smem_u32(&bars.weights), (step0 + i) * kK, first % p.channel_tiles * kM);
+    } else if (p.weights_first) {
+      for (; ahead < min(p.stages, steps); ++ahead) {
+        expect_if(mine, bars.full + ahead, stage_bytes);
+        tma_load(mine, &w, ring0 + (uint32_t)ahead * stage_bytes, bars0 + 8u * (uint32_t)ahead, (step0 + ahead) * kK, first % p.channel_tiles * kM);
       }
-      if (p.weights_first) dependency_wait();
-      release_dependents();
-      const uint32_t ring0 = smem_u32(ring), codes_at = p.resident ? 0u : (uint32_t)kABytes;
-      for (int item = first; item < p.items && left != 0u; item += stride) {
-        const int channel0 = item % p.channel_tiles * kM, row0 = item / p.channel_tiles * p.tile_rows;
-        for (int i = 0; i < steps && left != 0u; ++i) {
-          if (round > 0) wait_bar(bars.empty + s, (round - 1) & 1, left);
-          if (left != 0u) {
-            const uint32_t stage = ring0 + (uint32_t)s * stage_bytes;
-            if (round > 0 || s >= ahead) {
-              expect(bars.full + s, stage_bytes);
-              if (!p.resident) tma_load(&w, stage, bars.full + s, (step0 + i) * kK, channel0);
-            }
-            tma_load(&codes, stage + codes_at, bars.full + s, (step0 + i) * kK, row0);
-            if (++s == p.stages) { s = 0; ++round; }
-          }
-        }
+    }
+    if (p.weights_first) dependency_wait();
+    release_dependents();
+    for (int item = first; item < p.items; item += stride) {
+      const int channel0 = item % p.channel_tiles * kM, row0 = item / p.channel_tiles * p.tile_rows;
+      for (int i = 0; i < steps; ++i) {
+        if (round > 0) wait_bar(bars.empty + s, (round - 1) & 1, left);
+        const bool go = mine && left != 0u, fresh = go && (round > 0 || s >= ahead);
+        const uint32_t stage = ring0 + (uint32_t)s * stage_bytes, bar = bars0 + 8u * (uint32_t)s;
+        expect_if(fresh, bars.full + s, stage_bytes);
+        tma_load(fresh && !p.resident, &w, stage, bar, (step0 + i) * kK, channel0);
+        tma_load(go, &codes, stage + codes_at, bar, (step0 + i) * kK, row0);
+        if (++s == p.stages) { s = 0; ++round; }
       }
     }
   } else if (wid == 1) {
     // ================= MMAs
-    if (lane == 0) {
-      const uint32_t idesc = instruction(kSumS32, kFormatS8, kM, (uint32_t)p.tile_rows);
-      const uint32_t a_low = desc_low(smem_u32(p.resident ? smem : ring), kChunkAlongK), b_low = desc_low(smem_u32(ring) + (p.resident ? 0 : kABytes), kChunkAlongK);
-      if (p.resident) wait_bar(&bars.weights, 0, left);
-      uint32_t t = 0;
-      for (int item = first; item < p.items && left != 0u; item += stride, ++t) {
-        const uint32_t buf = t & 1u, acc = tmem + buf * (uint32_t)p.tmem;
-        if (t >= 2) wait_bar(bars.acc_empty + buf, ((t >> 1) - 1) & 1, left);
-        for (int i = 0; i < steps && left != 0u; ++i) {
-          wait_bar(bars.full + s, round & 1, left);
-          if (left != 0u) {
-            fence_after();
-            const uint32_t at = (uint32_t)s * (stage_bytes >> 4), a = a_low + (p.resident ? (uint32_t)i * (kABytes >> 4) : at), b = b_low + at;
+    const bool mine = elected() != 0u;
+    const uint32_t idesc = instruction(kSumS32, kFormatS8, kM, (uint32_t)p.tile_rows);
+    const uint32_t a_low = desc_low(smem_u32(p.resident ? smem : ring), kChunkAlongK), b_low = desc_low(smem_u32(ring) + (p.resident ? 0 : kABytes), kChunkAlongK);
+    if (p.resident) wait_bar(&bars.weights, 0, left);
+    uint32_t t = 0;
+    for (int item = first; item < p.items; item += stride, ++t) {
+      const uint32_t buf = t & 1u, acc = tmem + buf * (uint32_t)p.tmem;
+      if (t >= 2) wait_bar(bars.acc_empty + buf, ((t >> 1) - 1) & 1, left);
+      for (int i = 0; i < steps; ++i) {
+        wait_bar(bars.full + s, round & 1, left);
+        fence_after();
+        const bool go = mine && left != 0u;
+        const uint32_t at = (uint32_t)s * (stage_bytes >> 4), a = a_low + (p.resident ? (uint32_t)i * (kABytes >> 4) : at), b = b_low + at;
 #pragma unroll
-            for (uint32_t q = 0; q < kK / 32; ++q) mma_i8(acc, desc(a + q * kStepAlongK), desc(b + q * kStepAlongK), idesc, i + (int)q != 0 ? 1u : 0u);
-            commit(bars.empty + s);
-            if (++s == p.stages) { s = 0; ++round; }
-          }
-        }
-        if (left != 0u) commit(bars.acc_full + buf);
+        for (uint32_t q = 0; q < kK / 32; ++q) mma_i8(go, acc, desc(a + q * kStepAlongK), desc(b + q * kStepAlongK), idesc, i + (int)q != 0);
+        commit(go, bars.empty + s);
+        if (++s == p.stages) { s = 0; ++round; }
       }
+      commit(mine && left != 0u, bars.acc_full + buf);
     }
   } else {
     // ================= epilogue: a warp has the TMEM lanes of its quarter and every other 32 rows of the tile, thread = channel
@@ -217,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
         if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
       }
     } else if (tid == 32) {
-      commit(&bars.drain);
+      commit(true, &bars.drain);
       wait_bar(&bars.drain, 0, left);
     }
     __syncthreads();

@@ -380,81 +380,83 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 
   if (wid < kFirstEpilogueWarp) {
     if constexpr (kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
-    if (wid != 1 && lane == 0) {
-      // ================= loads: a thread of its own for each operand, and one for their low planes
+    const bool mine = elected() != 0u;
+    if (wid != 1) {
+      // ================= loads: a warp of its own for each operand, and one for their low planes
       dependency_wait();
       if (wid == 0) release_dependents();
       const bool high = wid != 3, of_a = high ? wid == 0 : p.a.planes > 1, of_b = high ? wid == 2 : p.b.planes > 1;
-      const uint32_t smem0 = smem_u32(smem) + (high ? 0u : a_bytes), b_low_at = b_at - (high ? 0u : a_bytes) + (high ? 0u : b_bytes);
+      const uint32_t smem0 = smem_u32(smem), a_at = high ? 0u : a_bytes, b_from = b_at + (high ? 0u : b_bytes);
       const uint32_t bars0 = CTAS == 2 ? peer_address(smem_u32(bars.full), 0) : smem_u32(bars.full);
       const int depth = p.chunks * kK;
-      const auto load = [&](const Operand& o, const CUtensorMap* map, uint32_t dst, uint32_t bar, int k, int at, int z) {
+      const auto load = [&](bool go, const Operand& o, const CUtensorMap* map, uint32_t dst, uint32_t bar, int k, int at, int z) {
         const int boxes = o.turned ? o.rows / 64 : p.chunks, box_bytes = o.turned ? depth * 128 : o.rows * 128;
         int x = o.turned ? at : k;
         const int y = o.turned ? k : at;
         for (int c = 0; c < boxes; ++c, x += 64, dst += (uint32_t)box_bytes) {
-          if (CTAS == 2) tma_load_pair(map, dst, bar, x, y, z);
-          else tma_load(map, dst, bar, x, y, z);
+          if (CTAS == 2) tma_load_pair(go, map, dst, bar, x, y, z);
+          else tma_load(go, map, dst, bar, x, y, z);
         }
       };
-      for (int item = of_a || of_b ? first : total; item < total && left != 0u; item += stride) {
+      const CUtensorMap *a_map = high ? &maps.a[0] : &maps.a[1], *b_map = high ? &maps.b[0] : &maps.b[1];
+      for (int item = of_a || of_b ? first : total; item < total; item += stride) {
         const Tile t = tile_of(p, item);
         const int a_row = (t.row * CTAS + rank) * kM, b_row = t.col * columns + rank * p.b.rows;
-        for (int i = 0; i < p.steps && left != 0u; ++i) {
+        for (int i = 0; i < p.steps; ++i) {
           if (round > 0) wait_bar(bars.empty + slot, (round - 1) & 1, left);
-          if (left != 0u) {
-            const uint32_t stage = smem0 + (uint32_t)slot * stage_bytes, bar = bars0 + (uint32_t)slot * 8u;
-            if (wid == 0 && rank == 0) expect(bars.full + slot, stage_bytes * CTAS);
-            if (of_a) load(p.a, high ? &maps.a[0] : &maps.a[1], stage, bar, i * depth, a_row, t.z);
-            if (of_b) load(p.b, high ? &maps.b[0] : &maps.b[1], stage + b_low_at, bar, i * depth, b_row, t.z);
-            if (++slot == p.stages) { slot = 0; ++round; }
-          }
+          const bool go = mine && left != 0u;
+          const uint32_t stage = smem0 + (uint32_t)slot * stage_bytes, bar = bars0 + (uint32_t)slot * 8u;
+          expect_if(go && wid == 0 && rank == 0, bars.full + slot, stage_bytes * CTAS);
+          if (of_a) load(go, p.a, a_map, stage + a_at, bar, i * depth, a_row, t.z);
+          if (of_b) load(go, p.b, b_map, stage + b_from, bar, i * depth, b_row, t.z);
+          if (++slot == p.stages) { slot = 0; ++round; }
         }
       }
-    } else if (wid == 1 && lane == 0 && rank == 0) {
+    } else if (rank == 0) {
       // ================= MMAs
       const uint32_t idesc = instruction(kSumF32, kFormatF16, kM * CTAS, (uint32_t)columns) | (p.a.turned ? kTurnedA : 0u) | (p.b.turned ? kTurnedB : 0u);
-      const auto done = [&](const uint64_t* bar) {
-        if (CTAS == 2) commit_pair(bar);
-        else commit(bar);
+      const auto done = [&](bool go, const uint64_t* bar) {
+        if (CTAS == 2) commit_pair(go, bar);
+        else commit(go, bar);
       };
       const uint32_t low = desc_low(smem_u32(smem), 0), a_low = low | desc_low(0, p.a.turned ? p.chunks * kK * 128 : kChunkAlongK);
       const uint32_t b_low = (low | desc_low(0, p.b.turned ? p.chunks * kK * 128 : kChunkAlongK)) + (b_at >> 4);
       const uint32_t a_step = p.a.turned ? kStepTurned : kStepAlongK, b_step = p.b.turned ? kStepTurned : kStepAlongK;
       const uint32_t a_chunk = p.a.turned ? 4 * kStepTurned : (uint32_t)p.a.rows * 8u, b_chunk = p.b.turned ? 4 * kStepTurned : (uint32_t)p.b.rows * 8u;
-      const auto product = [&](uint32_t acc, uint32_t a, uint32_t b, bool more) {  // of a stage
-        for (int c = 0; c < p.chunks; ++c, a += a_chunk, b += b_chunk) {
-#pragma unroll
-          for (uint32_t q = 0; q < kK / 16; ++q) {
-            const uint32_t on = more || c + (int)q != 0 ? 1u : 0u;
-            if (CTAS == 2) mma_f16_pair(acc, desc(a + q * a_step), desc(b + q * b_step), idesc, on);
-            else mma_f16(acc, desc(a + q * a_step), desc(b + q * b_step), idesc, on);
-          }
-        }
-      };
+      // The products of a stage: the small ones first (what is cut off their sums is as small as they are), then the large one.
+      const uint32_t a_small = a_bytes >> 4, b_small = b_bytes >> 4;
+      const int products = p.a.planes + p.b.planes - 1;
       uint32_t n = 0;  // accumulations begun: one a tile, or (float32) one a step
       uint32_t acc = tmem;
-      for (int item = first; item < total && left != 0u; item += stride) {
-        for (int i = 0; i < p.steps && left != 0u; ++i) {
-          const bool fresh = kWide || i == 0;
+      for (int item = first; item < total; item += stride) {
+        for (int i = 0; i < p.steps; ++i) {
+          const bool fresh = kWide || i == 0, last = kWide || i + 1 == p.steps;
           if (fresh) {
             acc = tmem + (n & 1u) * (uint32_t)columns;
             if (n >= 2) wait_bar(bars.acc_empty + (n & 1u), ((n >> 1) - 1) & 1, left);
           }
           wait_bar(bars.full + slot, round & 1, left);
-          if (left != 0u) {
-            fence_after();
-            const uint32_t at = (uint32_t)slot * (stage_bytes >> 4), a = a_low + at, b = b_low + at;
-            // the small products first: what is cut off their sums is as small as they are
-            if (p.a.planes > 1) product(acc, a + (a_bytes >> 4), b, !fresh);
-            if (p.b.planes > 1) product(acc, a, b + (b_bytes >> 4), !fresh || p.a.planes > 1);
-            product(acc, a, b, !fresh || p.a.planes > 1 || p.b.planes > 1);
-            done(bars.empty + slot);
-            if (++slot == p.stages) { slot = 0; ++round; }
-            if (kWide || i + 1 == p.steps) {
-              done(bars.acc_full + (n & 1u));
-              ++n;
+          fence_after();
+          const bool go = mine && left != 0u;
+          const uint32_t at = (uint32_t)slot * (stage_bytes >> 4);
+          bool more = !fresh;
+          for (int q = 0; q < products; ++q) {
+            const bool large = q + 1 == products, of_a = !large && q == 0 && p.a.planes > 1;  // the small product with A's low plane, or B's
+            uint32_t a = a_low + at + (of_a ? a_small : 0u), b = b_low + at + (large || of_a ? 0u : b_small);
+            for (int c = 0; c < p.chunks; ++c, a += a_chunk, b += b_chunk) {
+#pragma unroll
+              for (uint32_t e = 0; e < kK / 16; ++e) {
+                if (CTAS == 2) mma_f16_pair(go, acc, desc(a + e * a_step), desc(b + e * b_step), idesc, more || e != 0);
+                else mma_f16(go, acc, desc(a + e * a_step), desc(b + e * b_step), idesc, more || e != 0);
+              }
+              more = true;
             }
+          }
+          done(go, bars.empty + slot);
+          if (++slot == p.stages) { slot = 0; ++round; }
+          if (last) {
+            done(go, bars.acc_full + (n & 1u));
+            ++n;
           }
         }
       }
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
       }
     } else if (tid == 32) {
-      commit(&bars.drain);
+      commit(true, &bars.drain);
       wait_bar(&bars.drain, 0, left);
     }
     __syncthreads();
@@ -594,13 +596,25 @@ static int64_t tiles(int64_t m, int64_t n, int rows, int columns, bool symmetric
 
 struct Tiling { int ctas, columns; };
 
-// Tiles of 256 x 256 for two CTAs, which read a third less for a product than CTAs of their own with 128 x 256, where there are enough of them; else 128 rows and
-// as many columns as leave every SM a tile.
-static Tiling tiling(int64_t m, int64_t n, int64_t batch, bool symmetric, int sms) {
-  if (tiles(m, n, 2 * kM, kMaxN, symmetric) * batch >= sms / 2) return Tiling{2, kMaxN};
-  for (int columns = kMaxN; columns > 64; columns /= 2)
-    if (tiles(m, n, kM, columns, symmetric) * batch >= sms) return Tiling{1, columns};
-  return Tiling{1, 64};
+// The tiles of least cycles: rounds over the SMs of a tile's stages, which take the longer of their MMAs (half a cycle a column, 46 cycles at least,
+// and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of float32 to take the sums out.
+static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, int sms) {
+  const int products = planes_a + planes_b - 1, chunks = products > 1 ? 1 : 2;
+  Tiling best{1, 64};
+  int64_t least = 0;
+  for (const Tiling t : {Tiling{2, 256}, Tiling{2, 128}, Tiling{1, 256}, Tiling{1, 128}, Tiling{1, 64}}) {
+    const int64_t total = tiles(m, n, kM * t.ctas, t.columns, symmetric) * batch, rounds = ceil_div(total, sms / t.ctas), steps = ceil_div(k, kK * chunks);
+    const int64_t mma = products * chunks * 4 * (t.columns / 2 > 46 ? t.columns / 2 : 46), bytes = (int64_t)chunks * 128 * (kM * planes_a + t.columns / t.ctas * planes_b);
+    int64_t step = mma > bytes / 100 ? mma : bytes / 100;
+    const int64_t issue = products * chunks * 4 * 46 + (wide ? 400 : 250), taken = wide ? 250 + 3 * t.columns : 0;
+    if (step < issue) step = issue;
+    if (step < taken) step = taken;
+    const int64_t cycles = rounds * (steps * step + (wide ? 12 * t.columns : 0)) + 12 * t.columns;
+    if (least != 0 && cycles >= least) continue;
+    least = cycles;
+    best = t;
+  }
+  return best;
 }
 
 struct Product {
@@ -619,7 +633,7 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
   p.steps = (int)ceil_div(x.k, kK * p.chunks);
   p.symmetric = x.symmetric;
   p.batch = (int)batch;
-  const Tiling shape = tiling(x.m, x.n, batch, x.symmetric, sms);
+  const Tiling shape = tiling(x.a_planes, x.b_planes, x.m, x.n, x.k, batch, x.symmetric, sizeof(T) == 4, sms);
   p.ctas = shape.ctas;
   p.a = Operand{kM, x.a_turned, x.a_planes};
   p.b = Operand{shape.columns / shape.ctas, x.b_turned, x.b_planes};

@@ -23,10 +23,25 @@ __device__ __forceinline__ void arrive(const uint64_t* bar) { asm volatile("mbar
 __device__ __forceinline__ void expect(const uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+// whether this lane of a whole warp is the one to issue
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ void expect_if(bool go, const uint64_t* bar, uint32_t bytes) {
+  asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t@g mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(smem_u32(bar)),
+               "r"(bytes), "r"((uint32_t)go)
+               : "memory");
+}
 __device__ __forceinline__ void fence_bars() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 
-// Waits for a phase, or until `left`, the tries that a role has for all its waits, is 0: then it gives up, and its loops end.  (They end by their
-// conditions alone: a `break` behind the wait took the thread 120 cycles more, three quarters of what there is for a step's loads.)
+// How the roles that issue copies and MMAs are written: whole warps run their loops, whose conditions no wait decides, and `go` - this lane is the
+// one that issues, and no wait of the role has run out - is a predicate of every instruction that does something.  Then the compiler keeps
+// descriptors and addresses in uniform registers.  (With one thread in a loop that a failed wait leaves, a wait took 180 cycles instead of 60 and an
+// MMA 60 to 90 instead of 46: more than the MMA itself up to 128 columns.)
+
+// Waits for a phase, or until `left`, the tries that a role has for all its waits, is 0: then it has given up, and later waits try once.
 __device__ __forceinline__ void wait_bar(const uint64_t* bar, uint32_t parity, uint32_t& left) {
   const uint32_t at = smem_u32(bar);
   uint32_t done;
@@ -100,56 +115,59 @@ __device__ __forceinline__ constexpr uint32_t instruction(uint32_t sum, uint32_t
   return (sum << 4) | (format << 7) | (format << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc),
-      "r"(accumulate), "r"(0u)
-      : "memory");
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc),
-      "r"(accumulate), "r"(0u)
-      : "memory");
-}
-
-// Over both CTAs of a pair: half of the rows of A and of the columns of B in the shared memory of each, at the same offsets.
-__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}\n" ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc),
-      "r"(accumulate), "r"(0u)
-      : "memory");
-}
-// arrives at the barrier, in both CTAs of a pair, when all MMAs of the pair issued so far by this thread are complete
-__device__ __forceinline__ void commit_pair(const uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
-               : "memory");
-}
+#define F2C_MMA(name, form, lanes)                                                                                              \
+  __device__ __forceinline__ void name(bool go, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {  \
+    asm volatile(                                                                                                              \
+        "{\n\t.reg .pred p, g;\n\tsetp.ne.b32 g, %6, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                              \
+        "@g tcgen05.mma." form " [%0], %1, %2, %3, {" lanes "}, p;\n\t}\n" ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc),           \
+        "r"((uint32_t)accumulate), "r"(0u), "r"((uint32_t)go)                                                                 \
+        : "memory");                                                                                                           \
+  }
+F2C_MMA(mma_i8, "cta_group::1.kind::i8", "%5, %5, %5, %5")
+F2C_MMA(mma_f16, "cta_group::1.kind::f16", "%5, %5, %5, %5")
+// over both CTAs of a pair: half of the rows of A and of the columns of B in the shared memory of each, at the same offsets
+F2C_MMA(mma_i8_pair, "cta_group::2.kind::i8", "%5, %5, %5, %5, %5, %5, %5, %5")
+F2C_MMA(mma_f16_pair, "cta_group::2.kind::f16", "%5, %5, %5, %5, %5, %5, %5, %5")
+#undef F2C_MMA
 
 // arrives at the barrier when all MMAs issued so far by this thread are complete
-__device__ __forceinline__ void commit(const uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void commit(bool go, const uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %1, 0;\n\t"
+               "@g tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)), "r"((uint32_t)go)
+               : "memory");
+}
+// the same of the MMAs of a pair, at the barriers of both CTAs
+__device__ __forceinline__ void commit_pair(bool go, const uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t"
+               "@g tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n" ::"r"(smem_u32(bar)),
+               "h"((uint16_t)3), "r"((uint32_t)go)
+               : "memory");
 }
 
 // ---------------------------------------------------------------- TMA
-__device__ __forceinline__ void tma_load(const CUtensorMap* map, uint32_t dst, const uint64_t* bar, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-               "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+__device__ __forceinline__ void tma_load(bool go, const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y) {
+  asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %5, 0;\n\t"
+               "@g cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}\n" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(bar), "r"((uint32_t)go)
                : "memory");
 }
-__device__ __forceinline__ void tma_load(const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+__device__ __forceinline__ void tma_load(bool go, const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y, int z) {
+  asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %6, 0;\n\t"
+               "@g cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}\n" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"((uint32_t)go)
                : "memory");
 }
 // The same in a pair of CTAs: `bar`, at which the bytes are counted, is a cluster address and may be the other one's.
-__device__ __forceinline__ void tma_load_pair(const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+__device__ __forceinline__ void tma_load_pair(bool go, const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y) {
+  asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %5, 0;\n\t"
+               "@g cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];\n\t}\n" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(bar), "r"((uint32_t)go)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_pair(bool go, const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y, int z) {
+  asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %6, 0;\n\t"
+               "@g cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];\n\t}\n" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"((uint32_t)go)
                : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
