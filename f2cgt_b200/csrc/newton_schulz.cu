@@ -19,78 +19,18 @@
 //    2e-4 without the taking out.)
 #include <math.h>
 
-#include "tcgen05.cuh"
+#include "newton_schulz.cuh"
 
 namespace f2c {
 namespace ns {
-
-using namespace t5;
 
 constexpr int kMaxParts = 1024, kLoadThreads = 256;  // parts of a matrix' norm
 constexpr int kFirstEpilogueWarp = 4, kEpilogueWarps = 8, kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);  // warp 0: TMA, warp 1: MMA
 // float32: 128 sums a thread.  What a CTA is launched with, 168 registers a thread, is shared out anew.
 constexpr int kRegisters = 168, kFewRegisters = 40, kManyRegisters = 232;
 static_assert(32 * (kFirstEpilogueWarp * kFewRegisters + kEpilogueWarps * kManyRegisters) <= kThreads * kRegisters, "registers of a CTA");
-constexpr int kM = 128, kK = 64, kMaxN = 256, kMaxStages = 8, kMaxList = 64;
+constexpr int kM = 128, kK = 64, kMaxN = 256, kMaxStages = 8;
 constexpr size_t kRoom = kSmemLimit - 1024;  // dynamic shared memory
-constexpr int kScaleLog = 10;                // norms are brought to 2^10
-
-// ---------------------------------------------------------------- what is read and written
-struct Matrices {  // of one shape: a stack, or a list
-  const void* g;
-  void* out;              // the result; optimiser: the weights
-  float* momentum;        // null: g is orthogonalised itself
-  f2c_muon_matrix list[kMaxList];
-  int listed;
-  int64_t size;           // elements of a matrix
-  float mu, keep, gain;   // w <- keep w - gain X
-  int nesterov;
-  template <typename T> __device__ __forceinline__ const T* grad(int z) const { return listed ? (const T*)list[z].grad : (const T*)g + z * size; }
-  template <typename T> __device__ __forceinline__ T* result(int z) const { return listed ? (T*)list[z].weight : (T*)out + z * size; }
-  __device__ __forceinline__ float* moment(int z) const { return listed ? list[z].momentum : nullptr; }
-};
-
-// Factors of a step, for a matrix.
-struct Factors {
-  float gram, poly_b, poly_c, apply, own;  // As = gram Xs Xs^T; Rs = poly_c As^2 + poly_b As; the next Xs = own Xs + apply Rs Xs
-};
-
-struct Steps {
-  int count;
-  float co[3 * F2C_MAX_NS_STEPS];
-  float top[F2C_MAX_NS_STEPS + 1];   // no singular value is larger in front of step t, if none was larger than one at first
-  float factor[F2C_MAX_NS_STEPS];    // and none is multiplied by more
-  float eps;
-};
-
-__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + min(max(e, -126), 127)) << 23); }
-// 2^e is the smallest power that is not below v > 0
-__device__ __forceinline__ int log2_above(float v) {
-  int e;
-  const float f = frexpf(v, &e);
-  return f == 0.5f ? e - 1 : e;
-}
-
-template <typename T, int V> struct alignas(V * sizeof(T)) Chunk { T v[V]; };
-
-// u of V elements from i on
-template <typename T, int V, bool UPDATE>
-__device__ __forceinline__ void direction(const Matrices& s, int z, int64_t i, float (&u)[V]) {
-  const Chunk<T, V> g = *reinterpret_cast<const Chunk<T, V>*>(s.template grad<T>(z) + i);
-  float* momentum = s.moment(z);
-  if (momentum == nullptr) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) u[e] = to_float(g.v[e]);
-    return;
-  }
-  Chunk<float, V> m = *reinterpret_cast<const Chunk<float, V>*>(momentum + i);
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if (UPDATE) m.v[e] = fmaf(s.mu, m.v[e], to_float(g.v[e]));
-    u[e] = s.nesterov ? fmaf(s.mu, m.v[e], to_float(g.v[e])) : m.v[e];
-  }
-  if (UPDATE) *reinterpret_cast<Chunk<float, V>*>(momentum + i) = m;
-}
 
 // Momentum, and the squares' sums of gridDim.x parts of every matrix.
 template <typename T, int V>
@@ -135,36 +75,11 @@ __global__ void __launch_bounds__(kLoadThreads) planes_kernel(const __grid_const
   __syncthreads();
   const double norm = norm_s;
   const bool finite = norm <= 1e300;
-  int e = 0;
-  if (finite && norm > 0.0) (void)frexp(norm, &e);  // norm < 2^e
-  const int up = kScaleLog + 1 - e;
+  const int up = scale_up(norm);
   // u 2^up in two factors: the power itself may be out of range.  A matrix that is not finite becomes NaN.
   const float by = power2(up / 2), more = finite ? power2(up - up / 2) : __int_as_float(0x7fffffff);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    float kappa = (float)(exp2((double)-up) / (norm + (double)st.eps));  // X = kappa Xs
-    float bound = (float)(norm / (norm + (double)st.eps));
-    for (int t = 0; t < st.count; ++t) {
-      const float a = st.co[3 * t], b = st.co[3 * t + 1], c = st.co[3 * t + 2];
-      const int lead = bound > 0.0f && bound <= 64.0f ? log2_above(bound) : 0;
-      const int a_log = min(kScaleLog - 2 * lead, 100);  // As = 2^a_log A
-      Factors f;
-      if (c != 0.0f) {
-        f.gram = power2(a_log) * kappa * kappa;
-        f.poly_b = b * power2(kScaleLog - a_log);
-        f.poly_c = c * power2(kScaleLog - a_log) * power2(-a_log);
-      } else {  // R itself
-        f.gram = b * power2(kScaleLog) * kappa * kappa;
-        f.poly_b = f.poly_c = 0.0f;
-      }
-      bound = fminf(st.top[t + 1], bound * st.factor[t]);
-      const bool last = t + 1 == st.count;
-      const float next = last ? 1.0f : power2((bound > 0.0f && bound <= 64.0f ? log2_above(bound) : 0) - kScaleLog);
-      f.apply = kappa * power2(-kScaleLog) / next;
-      f.own = a * (kappa / next);
-      kappa = next;
-      table[z * F2C_MAX_NS_STEPS + t] = f;
-    }
-    if (st.count == 0) table[z * F2C_MAX_NS_STEPS].apply = kappa;
+    make_factors(st, norm, up, table + z * F2C_MAX_NS_STEPS);
   }
   __half* const hi = high + z * rows * ld;
   __half* const lo = low + z * rows * ld;
@@ -196,7 +111,7 @@ __global__ void __launch_bounds__(kLoadThreads) store_kernel(const __grid_consta
     const int64_t at = z * rows * ld + i / cols * ld + i % cols;
     const float x = kappa * (__half2float(high[at]) + (low != nullptr ? __half2float(low[at]) : 0.0f));
     T* const out = s.template result<T>(z) + i;
-    *out = from_float<T>(s.listed ? s.keep * to_float(*out) - s.gain * x : x);
+    *out = from_float<T>(s.listed ? s.keep * to_float(*out) - s.gain(rows, cols) * x : x);
   }
 }
 
@@ -222,6 +137,7 @@ struct Params {
   const __half *add_high, *add_low;  // kPoly: As; kApply, kFinal: Xs
   __half *high, *low;              // result [n][m] (kGram and kPoly: symmetric); low null: none; ld and stack also Xs'
   int64_t ld, stack;               // elements between rows, and between matrices
+  float gain;                      // kFinal, optimiser: times the result
   int* error;
 };
 
@@ -308,7 +224,7 @@ __device__ __forceinline__ void store_values(const Params& p, const Matrices& s,
       float w[32];
       gather(out, (int64_t)p.m, count, w);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = s.keep * w[j] - s.gain * v[j];
+      for (int j = 0; j < 32; ++j) v[j] = s.keep * w[j] - p.gain * v[j];
     }
 #pragma unroll
     for (int j = 0; j < 32; ++j) o[j] = from_float<T>(v[j]);
@@ -717,6 +633,7 @@ static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps&
                          : Product{x[t & 1], r, planes, inner, 1, 0, s.rows, s.cols, s.ldx(), p, p, s.ldp(), s.cols, p, p, false};
     Params q{};
     q.factors = table + t;
+    q.gain = src.lr * (float)sqrt(s.rows > s.cols ? (double)s.rows / (double)s.cols : 1.0);
     q.add_high = x[t & 1].high; q.add_low = planes > 1 ? x[t & 1].low : nullptr;
     q.high = x[(t + 1) & 1].high; q.low = next > 1 ? x[(t + 1) & 1].low : nullptr;
     q.ld = s.ldx(); q.stack = s.rows * s.ldx();
@@ -727,6 +644,10 @@ static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps&
 }
 
 static int run(const char* op, Matrices& src, int dtype, const Shape& s, const Steps& st, char* ws, cudaStream_t stream) {
+  if (is_small(s.rows, s.cols)) {
+    src.size = s.rows * s.cols;
+    return small(op, src, (int)s.batch, s.rows, s.cols, dtype, st, stream);
+  }
   if (dtype == F2C_F32) return run_typed<float>(op, src, s, st, ws, stream);
   if (dtype == F2C_F16) return run_typed<__half>(op, src, s, st, ws, stream);
   return run_typed<__nv_bfloat16>(op, src, s, st, ws, stream);
@@ -771,7 +692,7 @@ static int check_shape(const char* op, const Shape& s) {
 using namespace f2c;
 
 extern "C" int64_t f2c_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t cols) {
-  return batch < 1 || rows < 1 || cols < 1 ? 0 : ns::workspace(ns::Shape{batch, rows, cols}, dtype == F2C_F32);
+  return batch < 1 || rows < 1 || cols < 1 || ns::is_small(rows, cols) ? 0 : ns::workspace(ns::Shape{batch, rows, cols}, dtype == F2C_F32);
 }
 
 extern "C" int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t batch, int64_t rows, int64_t cols, const float* coefficients_host,
@@ -783,7 +704,8 @@ extern "C" int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t ba
   if (const int rc = ns::check(op, dtype, coefficients_host, steps, eps, &st)) return rc;
   if (batch == 0 || rows == 0 || cols == 0) return F2C_OK;
   F2C_REQUIRE(g && out, F2C_ERR_INVALID, "%s: null pointer", op);
-  F2C_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= ns::workspace(s, dtype == F2C_F32), F2C_ERR_INVALID,
+  const int64_t need = f2c_orthogonalize_workspace(dtype, batch, rows, cols);
+  F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,
               "%s: workspace too small or not 256-byte aligned", op);
   ns::Matrices src{};
   src.g = g;
@@ -791,16 +713,21 @@ extern "C" int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t ba
   return ns::run(op, src, dtype, s, st, (char*)workspace, (cudaStream_t)stream);
 }
 
-// Matrices of the list that have the shape of number i, from i on: into `src`, up to kMaxList.  False when an earlier one was their first.
+// The matrices that are done together with number i of the list, from it on, up to kMaxList: all small ones, or those of its shape.  False when an earlier
+// one was their first.
 static bool group_of(const f2c_muon_matrix* list, int count, int i, ns::Matrices* src) {
-  const auto same = [&](int j) { return list[j].rows == list[i].rows && list[j].cols == list[i].cols; };
+  const bool small = ns::is_small(list[i].rows, list[i].cols);
+  const auto with = [&](int j) {
+    if (list[j].rows == 0 || list[j].cols == 0) return false;
+    return small ? ns::is_small(list[j].rows, list[j].cols) : list[j].rows == list[i].rows && list[j].cols == list[i].cols;
+  };
   if (list[i].rows == 0 || list[i].cols == 0) return false;
   int before = 0;
-  for (int j = 0; j < i; ++j) before += same(j);
+  for (int j = 0; j < i; ++j) before += with(j);
   if (before % ns::kMaxList != 0) return false;
   src->listed = 0;
   for (int j = i; j < count && src->listed < ns::kMaxList; ++j)
-    if (same(j)) src->list[src->listed++] = list[j];
+    if (with(j)) src->list[src->listed++] = list[j];
   return true;
 }
 
@@ -808,7 +735,7 @@ extern "C" int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int coun
   int64_t most = 0;
   ns::Matrices src{};
   for (int i = 0; list_host != nullptr && i < count; ++i) {
-    if (list_host[i].rows < 0 || list_host[i].cols < 0 || !group_of(list_host, count, i, &src)) continue;
+    if (list_host[i].rows < 0 || list_host[i].cols < 0 || ns::is_small(list_host[i].rows, list_host[i].cols) || !group_of(list_host, count, i, &src)) continue;
     const int64_t bytes = ns::workspace(ns::Shape{src.listed, list_host[i].rows, list_host[i].cols}, dtype == F2C_F32);
     most = bytes > most ? bytes : most;
   }
@@ -832,11 +759,11 @@ extern "C" int f2c_muon_step(const f2c_muon_matrix* list_host, int count, int dt
   ns::Matrices src{};
   src.mu = momentum;
   src.keep = (float)(1.0 - (double)lr * decay);
+  src.lr = lr;
   src.nesterov = nesterov;
   for (int i = 0; i < count; ++i) {
     if (!group_of(list_host, count, i, &src)) continue;
     const ns::Shape s{src.listed, list_host[i].rows, list_host[i].cols};
-    src.gain = (float)((double)lr * sqrt(s.rows > s.cols ? (double)s.rows / (double)s.cols : 1.0));
     if (const int rc = ns::run(op, src, dtype, s, st, (char*)workspace, (cudaStream_t)stream)) return rc;
   }
   return F2C_OK;
