@@ -230,10 +230,10 @@ __device__ __forceinline__ void store_values(const Params& p, const Matrices& s,
     for (int j = 0; j < 32; ++j) o[j] = from_float<T>(v[j]);
     scatter(out, (int64_t)p.m, count, mine, o);
   } else {
-    union Half { __half h[32]; uint4 v[4]; };
+    union Half { __half h[32]; __half2 p[16]; uint4 v[4]; __device__ Half() {} };
     Half half;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) half.h[j] = __float2half_rn(v[j]);
+    for (int j = 0; j < 16; ++j) half.p[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
     const int64_t across = stack + (int64_t)row * p.ld + col;
     const bool above = MODE != kApply && col > row0 && mine;
     const auto store = [&](__half* to) {
@@ -247,7 +247,10 @@ __device__ __forceinline__ void store_values(const Params& p, const Matrices& s,
     store(p.high);
     if (p.low != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) half.h[j] = __float2half_rn(v[j] - __half2float(half.h[j]));
+      for (int j = 0; j < 16; ++j) {
+        const float2 f = __half22float2(half.p[j]);
+        half.p[j] = __floats2half2_rn(v[2 * j] - f.x, v[2 * j + 1] - f.y);
+      }
       store(p.low);
     }
   }

@@ -40,11 +40,10 @@ struct Steps {
 };
 
 __device__ __forceinline__ float power2(int e) { return __int_as_float((127 + min(max(e, -126), 127)) << 23); }
-// 2^e is the smallest power that is not below v > 0
+// 2^e is the smallest power that is not below v > 0 (v not subnormal)
 __device__ __forceinline__ int log2_above(float v) {
-  int e;
-  const float f = frexpf(v, &e);
-  return f == 0.5f ? e - 1 : e;
+  const uint32_t bits = __float_as_uint(v);
+  return (int)(bits >> 23) - 127 + ((bits & 0x7fffffu) != 0u ? 1 : 0);
 }
 
 template <typename T, int V> struct alignas(V * sizeof(T)) Chunk { T v[V]; };
@@ -70,18 +69,19 @@ __device__ __forceinline__ void direction(const Matrices& s, int z, int64_t i, f
 
 // Powers of two: X = u 2^up brings a norm to [2^10, 2^11).
 __device__ __forceinline__ int scale_up(double norm) {
-  int e = 0;
-  if (norm <= 1e300 && norm > 0.0) (void)frexp(norm, &e);  // norm < 2^e
+  if (!(norm <= 1e300 && norm > 0.0)) return kScaleLog + 1;
+  const int e = (__double2hiint(norm) >> 20) - 1022;  // norm < 2^e
   return kScaleLog + 1 - e;
 }
 
 // The steps' factors for a matrix of that norm; without steps, `apply` of the first is the result's.
 __device__ __forceinline__ void make_factors(const Steps& st, double norm, int up, Factors* table) {
-  float kappa = (float)(exp2((double)-up) / (norm + (double)st.eps));  // X = kappa Xs
-  float bound = (float)(norm / (norm + (double)st.eps));
+  const double by = 1.0 / (norm + (double)st.eps);
+  float kappa = (float)(by * __hiloint2double((1023 - up) << 20, 0));  // X = kappa Xs; 2^-up
+  float bound = (float)(norm * by);
   for (int t = 0; t < st.count; ++t) {
     const float a = st.co[3 * t], b = st.co[3 * t + 1], c = st.co[3 * t + 2];
-    const int lead = bound > 0.0f && bound <= 64.0f ? log2_above(bound) : 0;
+    const int lead = bound > 1e-37f && bound <= 64.0f ? log2_above(bound) : 0;
     const int a_log = min(kScaleLog - 2 * lead, 100);  // As = 2^a_log A
     Factors f;
     if (c != 0.0f) {
@@ -94,7 +94,7 @@ __device__ __forceinline__ void make_factors(const Steps& st, double norm, int u
     }
     bound = fminf(st.top[t + 1], bound * st.factor[t]);
     const bool last = t + 1 == st.count;
-    const float next = last ? 1.0f : power2((bound > 0.0f && bound <= 64.0f ? log2_above(bound) : 0) - kScaleLog);
+    const float next = last ? 1.0f : power2((bound > 1e-37f && bound <= 64.0f ? log2_above(bound) : 0) - kScaleLog);
     f.apply = kappa * power2(-kScaleLog) / next;
     f.own = a * (kappa / next);
     kappa = next;

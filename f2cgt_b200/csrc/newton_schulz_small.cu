@@ -34,31 +34,37 @@ struct Shared {
 __device__ __forceinline__ uint32_t place(uint32_t plane, int r, int c) {
   return plane + (uint32_t)((c >> 6) * kPiece + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2);
 }
-__device__ __forceinline__ void store8(uint32_t at, const __half (&h)[8]) {
-  union { __half h[8]; uint4 v; } u;
+// Eight columns from c on as half precision, and what that leaves.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& high, uint32_t& low) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  high = *reinterpret_cast<const uint32_t*>(&h);
+  low = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ void store_pair(uint32_t high, uint32_t low, bool both, int r, int c, const float (&v)[8]) {
+  uint32_t h[4], l[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) u.h[e] = h[e];
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u.v.x), "r"(u.v.y), "r"(u.v.z), "r"(u.v.w) : "memory");
+  for (int e = 0; e < 4; ++e) split2(v[2 * e], v[2 * e + 1], h[e], l[e]);
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(high, r, c)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+  if (both) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(low, r, c)), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
 }
 __device__ __forceinline__ void load8(uint32_t at, float (&v)[8]) {
-  union { __half h[8]; uint32_t w[4]; } u;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.w[0]), "=r"(u.w[1]), "=r"(u.w[2]), "=r"(u.w[3]) : "r"(at) : "memory");
+  uint32_t w[4];
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = __half2float(u.h[e]);
-}
-// eight columns from c on as half precision, and what that leaves
-__device__ __forceinline__ void store_pair(uint32_t high, uint32_t low, bool both, int r, int c, const float (&v)[8]) {
-  __half h[8], l[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    h[e] = __float2half_rn(v[e]);
-    l[e] = __float2half_rn(v[e] - __half2float(h[e]));
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+    v[2 * e] = f.x;
+    v[2 * e + 1] = f.y;
   }
-  store8(place(high, r, c), h);
-  if (both) store8(place(low, r, c), l);
 }
 
-template <typename T>
+// V elements of a matrix, which lie in one row of it
+template <typename T, int V> struct alignas(V * sizeof(T)) Few { T v[V]; };
+
+// V: elements read and written at a time
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constant__ Matrices s, const __grid_constant__ Steps st, int64_t stack_rows, int64_t stack_cols, int* error) {
   constexpr bool kWide = sizeof(T) == 4;
   extern __shared__ unsigned char smem_raw[];
@@ -82,20 +88,43 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
   dependency_wait();
   release_dependents();
 
-  // ================= the norm, and X
+  // ================= the norm, and X: a thread's elements stay in registers in between
   const T* const grad = s.template grad<T>(z);
   float* const momentum = s.moment(z);
-  const bool nesterov = s.nesterov != 0;
+  constexpr int kMost = kRows * kCols / kThreads / V, kBlock = kMost < 16 ? kMost / 2 : 16;  // of a thread, and on their way at once
+  const int count = size / V;
+  float u[kMost][V];
   double sum = 0.0;
-#pragma unroll 4
-  for (int i = tid; i < size; i += kThreads) {
-    float u = to_float(grad[i]);
-    if (momentum != nullptr) {
-      const float m = fmaf(s.mu, momentum[i], u);
-      momentum[i] = m;
-      u = nesterov ? fmaf(s.mu, m, u) : m;
+#pragma unroll
+  for (int b = 0; b < kMost; b += kBlock) {
+    if (b * kThreads >= count) break;
+#pragma unroll
+    for (int j = b; j < b + kBlock; ++j) {
+      Few<T, V> g{};
+      if (j * kThreads + tid < count) g = reinterpret_cast<const Few<T, V>*>(grad)[j * kThreads + tid];
+#pragma unroll
+      for (int e = 0; e < V; ++e) u[j][e] = to_float(g.v[e]);
     }
-    sum = fma((double)u, (double)u, sum);
+    if (momentum != nullptr) {
+      Few<float, V> m[kBlock];
+#pragma unroll
+      for (int j = 0; j < kBlock; ++j)
+        if ((b + j) * kThreads + tid < count) m[j] = reinterpret_cast<const Few<float, V>*>(momentum)[(b + j) * kThreads + tid];
+#pragma unroll
+      for (int j = 0; j < kBlock; ++j) {
+        if ((b + j) * kThreads + tid >= count) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          m[j].v[e] = fmaf(s.mu, m[j].v[e], u[b + j][e]);
+          u[b + j][e] = s.nesterov ? fmaf(s.mu, m[j].v[e], u[b + j][e]) : m[j].v[e];
+        }
+        reinterpret_cast<Few<float, V>*>(momentum)[(b + j) * kThreads + tid] = m[j];
+      }
+    }
+#pragma unroll
+    for (int j = b; j < b + kBlock; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum = fma((double)u[j][e], (double)u[j][e], sum);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -110,19 +139,53 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
   const int up = scale_up(norm);
   if (tid == 0) make_factors(st, norm, up, sh.factors);
   const float by = power2(up / 2), more = norm <= 1e300 ? power2(up - up / 2) : __int_as_float(0x7fffffff);
-#pragma unroll 4
-  for (int i = tid; i < size; i += kThreads) {
-    float u = to_float(grad[i]);
-    if (momentum != nullptr) {
-      const float m = momentum[i];
-      u = nesterov ? fmaf(s.mu, m, u) : m;
+  // V elements from i on are at (i / cols, i % cols); from one of a thread's to the next the pair moves by a fixed one
+  const int first_r = tid * V / cols, first_c = tid * V - first_r * cols, dr = kThreads * V / cols, dc = kThreads * V - dr * cols;
+  int r = first_r, c = first_c;
+  const auto move = [&]() {
+    r += dr;
+    c += dc;
+    if (c >= cols) {
+      c -= cols;
+      ++r;
     }
-    const float v = u * by * more;
-    const int row = i / cols, col = i - row * cols, r = tall ? col : row, c = tall ? row : col;
-    const __half h = __float2half_rn(v), l = __float2half_rn(v - __half2float(h));
-    const uint32_t at = place(smem + kXAt, r, c);
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(__half_as_ushort(h)) : "memory");
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + kXPlane), "h"(__half_as_ushort(l)) : "memory");
+  };
+#pragma unroll
+  for (int b = 0; b < kMost; b += kBlock) {
+    if (b * kThreads >= count) break;
+#pragma unroll
+    for (int j = b; j < b + kBlock; ++j, move()) {
+      if (j * kThreads + tid >= count) continue;
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = u[j][e] * by * more;
+      if constexpr (V == 4) {
+        uint32_t h[2], l[2];
+        split2(v[0], v[1], h[0], l[0]);
+        split2(v[2], v[3], h[1], l[1]);
+        if (!tall) {
+          const uint32_t at = place(smem + kXAt, r, c);
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(h[0]), "r"(h[1]) : "memory");
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + kXPlane), "r"(l[0]), "r"(l[1]) : "memory");
+        } else {  // four rows: every lane starts with another of them, so that 32 lanes meet eight bank groups
+          const int turn = (lane >> 1) & 3;
+          const uint64_t h4 = (uint64_t)h[1] << 32 | h[0], l4 = (uint64_t)l[1] << 32 | l[0];
+          const uint64_t hr = turn == 0 ? h4 : h4 >> (16 * turn) | h4 << (64 - 16 * turn), lr = turn == 0 ? l4 : l4 >> (16 * turn) | l4 << (64 - 16 * turn);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t at = place(smem + kXAt, c + ((e + turn) & 3), r);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((uint16_t)(hr >> (16 * e))) : "memory");
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + kXPlane), "h"((uint16_t)(lr >> (16 * e))) : "memory");
+          }
+        }
+      } else {
+        uint32_t h, l;
+        split2(v[0], 0.0f, h, l);
+        const uint32_t at = place(smem + kXAt, tall ? c : r, tall ? r : c);
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((uint16_t)h) : "memory");
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + kXPlane), "h"((uint16_t)l) : "memory");
+      }
+    }
   }
   fence_async();
   __syncthreads();
@@ -141,14 +204,19 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
       const uint32_t idesc = instruction(kSumF32, kFormatF16, kRows, (uint32_t)n) | (b_turned ? kTurnedB : 0u);
       const uint32_t a_plane = a == smem + kXAt ? kXPlane : kAPlane;
       const uint32_t a_low = desc_low(a, kChunkAlongK), b_low = desc_low(b, b_turned ? kPiece : kChunkAlongK);
+      const uint32_t b_step = b_turned ? kStepTurned : kStepAlongK;
       bool on = false;
       for (int t = 0; t < a_planes + b_planes - 1; ++t) {
         const bool large = t + 2 == a_planes + b_planes, of_a = !large && t == 0 && a_planes > 1;
         const uint32_t at = a_low + (of_a ? a_plane >> 4 : 0u), bt = b_low + (large || of_a ? 0u : b_plane >> 4);
-        for (int e = 0; e < k16; ++e, on = true) {  // 16 of K: 32 bytes of a row, 64 columns to a piece; turned: 16 rows
-          const uint32_t along = (uint32_t)((e >> 2) * (kPiece >> 4) + (e & 3) * (int)kStepAlongK);
-          mma_f16(go, acc, desc(at + along), desc(bt + (b_turned ? (uint32_t)e * kStepTurned : along)), idesc, on);
+        uint32_t ae = at, be = bt;
+        int e = 0;
+        for (; e + 4 <= k16; e += 4, ae += kPiece >> 4, be += b_turned ? 4 * kStepTurned : kPiece >> 4, on = true) {  // a piece, or 64 rows of one
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i)  // 16 of K: 32 bytes of a row; turned: 16 rows
+            mma_f16(go, acc, desc(ae + i * kStepAlongK), desc(be + i * b_step), idesc, on || i != 0);
         }
+        for (; e < k16; ++e, ae += kStepAlongK, be += b_step, on = true) mma_f16(go, acc, desc(ae), desc(be), idesc, on);
       }
       commit(go, &sh.done);
     }
@@ -206,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
     product(tmem + kApplyAt, smem + kAAt, inner, smem + kXAt, 2, kXPlane, true, q16, p16 / 16);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int x0 = group * 64 + half * 32;  // of 256
+      const int x0 = (group + 4 * half) * 32;  // of 256
       if (x0 >= q16) continue;
       uint32_t r[32];
       tmem_ld32(lanes + kApplyAt + (uint32_t)x0, r);
@@ -231,8 +299,8 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
 #pragma unroll
     for (int j = 0; j < kCols / 4; j += 8) {
       float h[8], l[8];
-      load8(place(smem + kXAt, row, group * 64 + j), h);
-      load8(place(smem + kXAt + kXPlane, row, group * 64 + j), l);
+      load8(place(smem + kXAt, row, (group + 4 * (j >> 5)) * 32 + (j & 31)), h);
+      load8(place(smem + kXAt + kXPlane, row, (group + 4 * (j >> 5)) * 32 + (j & 31)), l);
 #pragma unroll
       for (int e = 0; e < 8; ++e) kept[j + e] = kappa * (h[e] + l[e]);
     }
@@ -244,17 +312,35 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
   __syncthreads();
   const bool lost = sh.failed != 0;
 #pragma unroll
-  for (int j = 0; j < kCols / 4; ++j)
-    if (row < p && group * 64 + j < q) result[row * kPitch + group * 64 + j] = kept[j];
+  for (int j = 0; j < kCols / 4; ++j) {
+    const int column = (group + 4 * (j >> 5)) * 32 + (j & 31);
+    if (row < p && column < q) result[row * kPitch + column] = kept[j];
+  }
   __syncthreads();
   T* const out = s.template result<T>(z);
-  const float gain = s.listed ? s.gain(rows, cols) : 0.0f;
-#pragma unroll 4
-  for (int i = tid; i < size; i += kThreads) {
-    const int r = i / cols, c = i - r * cols;
-    float v = result[tall ? c * kPitch + r : r * kPitch + c];
-    if (s.listed) v = s.keep * to_float(out[i]) - gain * v;
-    out[i] = from_float<T>(lost ? __int_as_float(0x7fffffff) : v);
+  const float gain = s.listed ? s.gain(rows, cols) : 0.0f, nan = __int_as_float(0x7fffffff);
+  r = first_r;
+  c = first_c;
+#pragma unroll
+  for (int b = 0; b < kMost; b += kBlock) {
+    if (b * kThreads >= count) break;
+    Few<T, V> w[kBlock];
+    if (s.listed) {
+#pragma unroll
+      for (int j = 0; j < kBlock; ++j)
+        if ((b + j) * kThreads + tid < count) w[j] = reinterpret_cast<const Few<T, V>*>(out)[(b + j) * kThreads + tid];
+    }
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j, move()) {
+      if ((b + j) * kThreads + tid >= count) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float v = result[tall ? (c + e) * kPitch + r : r * kPitch + c + e];
+        if (s.listed) v = s.keep * to_float(w[j].v[e]) - gain * v;
+        w[j].v[e] = from_float<T>(lost ? nan : v);
+      }
+      reinterpret_cast<Few<T, V>*>(out)[(b + j) * kThreads + tid] = w[j];
+    }
   }
   if (lost && wid == 0) {  // MMAs in flight read shared memory and write TMEM: wait (bounded) for them
     left = kWaitLimit;
@@ -269,13 +355,23 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
   if (lost && tid == 0) report_wait(error, 6);
 }
 
-template <typename T>
+template <typename T, int V>
 static int launch(const char* op, const Matrices& s, int count, int64_t rows, int64_t cols, const Steps& st, cudaStream_t stream) {
-  auto* kern = small_kernel<T>;
+  auto* kern = small_kernel<T, V>;
   constexpr int bytes = kBytes + 1024;
   if (const int rc = allow_smem(op, (const void*)kern, bytes)) return rc;
   launch_dependent(kern, dim3((unsigned)count), kThreads, bytes, stream, s, st, rows, cols, stream_error_word());
   return check_launch(op);
+}
+
+template <typename T>
+static int by_width(const char* op, const Matrices& s, int count, int64_t rows, int64_t cols, const Steps& st, cudaStream_t stream) {
+  bool four = s.listed || (cols % 4 == 0 && aligned(s.g, 4 * sizeof(T)) && aligned(s.out, 4 * sizeof(T)));
+  for (int i = 0; i < s.listed; ++i) {
+    const f2c_muon_matrix& m = s.list[i];
+    four = four && m.cols % 4 == 0 && aligned(m.grad, 4 * sizeof(T)) && aligned(m.weight, 4 * sizeof(T)) && aligned(m.momentum, 16);
+  }
+  return four ? launch<T, 4>(op, s, count, rows, cols, st, stream) : launch<T, 1>(op, s, count, rows, cols, st, stream);
 }
 
 }  // namespace nss
@@ -288,9 +384,9 @@ bool is_small(int64_t rows, int64_t cols) {
 }
 
 int small(const char* op, const Matrices& s, int count, int64_t rows, int64_t cols, int dtype, const Steps& st, cudaStream_t stream) {
-  if (dtype == F2C_F32) return nss::launch<float>(op, s, count, rows, cols, st, stream);
-  if (dtype == F2C_F16) return nss::launch<__half>(op, s, count, rows, cols, st, stream);
-  return nss::launch<__nv_bfloat16>(op, s, count, rows, cols, st, stream);
+  if (dtype == F2C_F32) return nss::by_width<float>(op, s, count, rows, cols, st, stream);
+  if (dtype == F2C_F16) return nss::by_width<__half>(op, s, count, rows, cols, st, stream);
+  return nss::by_width<__nv_bfloat16>(op, s, count, rows, cols, st, stream);
 }
 
 }  // namespace ns
