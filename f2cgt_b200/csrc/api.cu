@@ -47,7 +47,7 @@ int current_sm_count() {
   return sm_count(dev);
 }
 
-int allow_smem(const char* what, const void* kernel, int bytes, int registers) {
+int allow_smem(const char* what, const void* kernel, int bytes) {
   struct Known { const void* kernel; int device, bytes; };
   static std::mutex mu;
   static std::vector<Known> known;
@@ -58,10 +58,6 @@ int allow_smem(const char* what, const void* kernel, int bytes, int registers) {
     for (const Known& k : known)
       if (k.kernel == kernel && k.device == dev && k.bytes == bytes) return F2C_OK;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    cudaFuncAttributes attr;
-    if (e == cudaSuccess && registers != 0) e = cudaFuncGetAttributes(&attr, kernel);
-    if (e == cudaSuccess && registers != 0 && attr.numRegs < registers)
-      return set_error(F2C_ERR_CUDA, "%s: a kernel was built with %d registers, %d are needed", what, attr.numRegs, registers);
   }
   if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   try {

@@ -20,9 +20,8 @@ int set_error(int status, const char* fmt, ...);
 int check_launch(const char* what);
 int sm_count(int device);  // multiprocessors of `device` (queried once per device)
 int current_sm_count();     // the same for the current device
-// Lets `kernel` have that much dynamic shared memory on the current device (asked of the runtime once).  `registers`, unless 0: what its threads have
-// to be launched with (a kernel that shares them out anew would wait for more forever).
-int allow_smem(const char* what, const void* kernel, int bytes, int registers = 0);
+// Lets `kernel` have that much dynamic shared memory on the current device (asked of the runtime once).
+int allow_smem(const char* what, const void* kernel, int bytes);
 
 #define F2C_REQUIRE(cond, status, ...)                 \
   do {                                                 \

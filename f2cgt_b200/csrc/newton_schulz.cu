@@ -14,7 +14,7 @@
 //    factors a, 3.4445^4 = 140 after the first, while large singular values only go to one: where that product is over 16, X is a pair of
 //    half precision numbers (22 bits) and R X two products.  For matrices of rank 8 the result is 2.6e-3 off then, and 2.6e-2 without.
 //  * 32-bit matrices.  All operands are pairs, a product is three (high by high, high by low, low by high): 22 bits throughout.  The tensor
-//    cores cut sums off instead of rounding them, for every 16 elements of K.  So the sums are taken out every 64 elements and added up in
+//    cores cut sums off instead of rounding them, for every 16 elements of K.  So the sums are taken out every 128 elements and added up in
 //    registers, the small products are in front of the large one, and a X is not in the sum.  (Rank 3, 400 x 600: 2.5e-4 off without any of this,
 //    2e-4 without the taking out.)
 #include <math.h>
@@ -26,10 +26,7 @@ namespace ns {
 
 constexpr int kMaxParts = 1024, kLoadThreads = 256;  // parts of a matrix' norm
 constexpr int kFirstEpilogueWarp = 4, kEpilogueWarps = 8, kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);  // warp 0: TMA, warp 1: MMA
-// float32: 128 sums a thread.  What a CTA is launched with, 168 registers a thread, is shared out anew.
-constexpr int kRegisters = 168, kFewRegisters = 40, kManyRegisters = 232;
-static_assert(32 * (kFirstEpilogueWarp * kFewRegisters + kEpilogueWarps * kManyRegisters) <= kThreads * kRegisters, "registers of a CTA");
-constexpr int kM = 128, kK = 64, kMaxN = 256, kMaxStages = 8;
+constexpr int kM = 128, kK = 64, kMaxSums = 128, kMaxStages = 8;
 constexpr size_t kRoom = kSmemLimit - 1024;  // dynamic shared memory
 
 // Momentum, and the squares' sums of gridDim.x parts of every matrix.
@@ -298,7 +295,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   uint32_t round = 0;
 
   if (wid < kFirstEpilogueWarp) {
-    if constexpr (kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
     const bool mine = elected() != 0u;
     if (wid != 1) {
       // ================= loads: a warp of its own for each operand, and one for their low planes
@@ -345,44 +341,46 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       // The products of a stage: the small ones first (what is cut off their sums is as small as they are), then the large one.
       const uint32_t a_small = a_bytes >> 4, b_small = b_bytes >> 4;
       const int products = p.a.planes + p.b.planes - 1;
+      // Waits for a step are made behind the MMAs and commits of the one before, some of which the tensor cores still have to do meanwhile.
+      const int mine_items = total > first ? (total - first + stride - 1) / stride : 0, all = mine_items * p.steps;
       uint32_t n = 0;  // accumulations begun: one a tile, or (float32) one a step
-      uint32_t acc = tmem;
-      for (int item = first; item < total; item += stride) {
-        for (int i = 0; i < p.steps; ++i) {
-          const bool fresh = kWide || i == 0, last = kWide || i + 1 == p.steps;
-          if (fresh) {
-            acc = tmem + (n & 1u) * (uint32_t)columns;
-            if (n >= 2) wait_bar(bars.acc_empty + (n & 1u), ((n >> 1) - 1) & 1, left);
-          }
-          wait_bar(bars.full + slot, round & 1, left);
-          fence_after();
-          const bool go = mine && left != 0u;
-          const uint32_t at = (uint32_t)slot * (stage_bytes >> 4);
-          bool more = !fresh;
-          for (int q = 0; q < products; ++q) {
-            const bool large = q + 1 == products, of_a = !large && q == 0 && p.a.planes > 1;  // the small product with A's low plane, or B's
-            uint32_t a = a_low + at + (of_a ? a_small : 0u), b = b_low + at + (large || of_a ? 0u : b_small);
-            for (int c = 0; c < p.chunks; ++c, a += a_chunk, b += b_chunk) {
+      int done_steps = 0, i = 0;
+      const auto wait_full = [&]() { wait_bar(bars.full + slot, round & 1, left); };
+      const auto wait_acc = [&]() {  // of accumulation n
+        if (n >= 2) wait_bar(bars.acc_empty + (n & 1u), ((n >> 1) - 1) & 1, left);
+      };
+      if (all > 0) wait_full();
+      for (; done_steps < all; ++done_steps) {
+        const bool fresh = kWide || i == 0, last = kWide || i + 1 == p.steps, more_steps = done_steps + 1 < all;
+        if (++i == p.steps) i = 0;
+        fence_after();
+        const bool go = mine && left != 0u;
+        const uint32_t at = (uint32_t)slot * (stage_bytes >> 4), acc = tmem + (n & 1u) * (uint32_t)columns;
+        const uint64_t *const empty = bars.empty + slot, *const full_acc = bars.acc_full + (n & 1u);
+        if (++slot == p.stages) { slot = 0; ++round; }
+        if (last) ++n;
+        bool more = !fresh;
+        for (int q = 0; q < products; ++q) {
+          const bool large = q + 1 == products, of_a = !large && q == 0 && p.a.planes > 1;  // the small product with A's low plane, or B's
+          uint32_t a = a_low + at + (of_a ? a_small : 0u), b = b_low + at + (large || of_a ? 0u : b_small);
+          for (int c = 0; c < p.chunks; ++c, a += a_chunk, b += b_chunk) {
 #pragma unroll
-              for (uint32_t e = 0; e < kK / 16; ++e) {
-                if (CTAS == 2) mma_f16_pair(go, acc, desc(a + e * a_step), desc(b + e * b_step), idesc, more || e != 0);
-                else mma_f16(go, acc, desc(a + e * a_step), desc(b + e * b_step), idesc, more || e != 0);
-              }
-              more = true;
+            for (uint32_t e = 0; e < kK / 16; ++e) {
+              if (CTAS == 2) mma_f16_pair(go, acc, desc(a + e * a_step), desc(b + e * b_step), idesc, more || e != 0);
+              else mma_f16(go, acc, desc(a + e * a_step), desc(b + e * b_step), idesc, more || e != 0);
             }
-          }
-          done(go, bars.empty + slot);
-          if (++slot == p.stages) { slot = 0; ++round; }
-          if (last) {
-            done(go, bars.acc_full + (n & 1u));
-            ++n;
+            more = true;
+            if (products > 1 && q == 0 && c == 0 && more_steps && last) wait_acc();
           }
         }
+        done(go, empty);
+        if (last) done(go, full_acc);
+        if (products == 1 && more_steps && last) wait_acc();
+        if (more_steps) wait_full();
       }
     }
   } else {
     // ================= epilogue: a warp has the TMEM lanes of its quarter and half of the columns, thread = row
-    if constexpr (kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int quarter = wid & 3, half = (wid - kFirstEpilogueWarp) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const auto leave = [&](uint32_t buf) {  // the accumulator has been read
@@ -401,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const Factors f = p.factors[at.z * F2C_MAX_NS_STEPS];
       if constexpr (kWide) {
         // the sums of the steps are added up here, where additions round
-        uint32_t sum[4][32] = {};
+        uint32_t sum[2][32] = {};
         const int width = columns / 2, mine = half * width;
         for (int i = 0; i < p.steps; ++i, ++n) {
           const uint32_t turn = n >> 1, buf = n & 1u;
@@ -409,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           __syncwarp();
           fence_after();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             if (c * 32 >= width) break;
             uint32_t r[32];
             tmem_ld32(lanes + buf * (uint32_t)columns + (uint32_t)(mine + c * 32), r);
@@ -420,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         }
         const bool lost = __any_sync(0xffffffffu, left == 0u);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           const int col = col0 + mine + c * 32;
           if (c * 32 >= width || col >= p.n || (p.symmetric && col + 31 < row0)) continue;  // (wholly below the diagonal)
           store_values<MODE, T>(p, s, f, at.z, row0, col, sum[c], lost);
@@ -513,15 +511,20 @@ static int64_t tiles(int64_t m, int64_t n, int rows, int columns, bool symmetric
   return items;
 }
 
+// Pieces of 64 elements of K in a stage.  float32, whose sums are taken out after every stage: two (2048 x 8192: 2.59 ms a step, 2.81 with one);
+// 16-bit matrices: one (4096 x 4096: 1.36 ms, 1.49 with two, of which fewer stages fit).
+static int chunks_of(bool wide) { return wide ? 2 : 1; }
+
 struct Tiling { int ctas, columns; };
 
 // The tiles of least cycles: rounds over the SMs of a tile's stages, which take the longer of their MMAs (half a cycle a column, 46 cycles at least,
 // and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of float32 to take the sums out.
 static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, int sms) {
-  const int products = planes_a + planes_b - 1, chunks = products > 1 ? 1 : 2;
+  const int products = planes_a + planes_b - 1, chunks = chunks_of(wide);
   Tiling best{1, 64};
   int64_t least = 0;
   for (const Tiling t : {Tiling{2, 256}, Tiling{2, 128}, Tiling{1, 256}, Tiling{1, 128}, Tiling{1, 64}}) {
+    if (wide && t.columns > kMaxSums) continue;
     const int64_t total = tiles(m, n, kM * t.ctas, t.columns, symmetric) * batch, rounds = ceil_div(total, sms / t.ctas), steps = ceil_div(k, kK * chunks);
     const int64_t mma = products * chunks * 4 * (t.columns / 2 > 46 ? t.columns / 2 : 46), bytes = (int64_t)chunks * 128 * (kM * planes_a + t.columns / t.ctas * planes_b);
     int64_t step = mma > bytes / 100 ? mma : bytes / 100;
@@ -548,7 +551,7 @@ template <int MODE, typename T>
 static int multiply(const char* op, const Product& x, Params p, const Matrices& s, int64_t batch, cudaStream_t st) {
   const int sms = current_sm_count();
   p.m = (int)x.m; p.n = (int)x.n;
-  p.chunks = x.a_planes + x.b_planes > 2 ? 1 : 2;  // eight MMAs to a wait at least
+  p.chunks = chunks_of(sizeof(T) == 4);
   p.steps = (int)ceil_div(x.k, kK * p.chunks);
   p.symmetric = x.symmetric;
   p.batch = (int)batch;
@@ -576,7 +579,7 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
   }
   F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
   auto* kern = shape.ctas == 2 ? product_kernel<MODE, T, 2> : product_kernel<MODE, T, 1>;
-  if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom, sizeof(T) == 4 ? kRegisters : 0)) return rc;
+  if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom)) return rc;
   launch_dependent_cluster(kern, dim3(grid), kThreads, p.stages * stage + 1024, (unsigned)shape.ctas, st, maps, p, s);
   return check_launch(op);
 }
