@@ -191,8 +191,8 @@ __device__ __forceinline__ void scatter(T* to, int64_t ld, int count, bool mine,
 }
 
 // A lane's row of the product, 32 values from column `col` on (which exists), to where they belong; called by whole warps, whose rows start
-// at `row0`.  A warp reads and writes 32 neighbours at a time: [column][row].  Symmetric: also [row][column], where the chunk lies above
-// the diagonal; in the chunk with the diagonal the product has both sides.
+// at `row0`.  A warp reads and writes 32 neighbours at a time: [column][row].  Symmetric, where half of the tiles are
+// made: also [row][column] of what lies above the diagonal; a chunk with the diagonal has both sides.
 template <int MODE, typename T>
 __device__ __forceinline__ void store_values(const Params& p, const Matrices& s, const Factors& f, int z, int row0, int col, const uint32_t (&r)[32], bool lost) {
   const int row = row0 + (threadIdx.x & 31), count = min(32, p.n - col);
@@ -232,7 +232,7 @@ __device__ __forceinline__ void store_values(const Params& p, const Matrices& s,
 #pragma unroll
     for (int j = 0; j < 16; ++j) half.p[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
     const int64_t across = stack + (int64_t)row * p.ld + col;
-    const bool above = MODE != kApply && col > row0 && mine;
+    const bool above = p.symmetric && col > row0 && mine;
     const auto store = [&](__half* to) {
       scatter(to + at, p.ld, count, mine, half.h);
       if (above) {
@@ -298,6 +298,11 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     const bool mine = elected() != 0u;
     if (wid != 1) {
       // ================= loads: a warp of its own for each operand, and one for their low planes
+      if (mine) {
+        prefetch_map(&maps.a[wid == 3]);
+        prefetch_map(&maps.b[wid == 3]);
+      }
+      __syncwarp();
       dependency_wait();
       if (wid == 0) release_dependents();
       const bool high = wid != 3, of_a = high ? wid == 0 : p.a.planes > 1, of_b = high ? wid == 2 : p.b.planes > 1;
@@ -553,7 +558,6 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
   p.m = (int)x.m; p.n = (int)x.n;
   p.chunks = chunks_of(sizeof(T) == 4);
   p.steps = (int)ceil_div(x.k, kK * p.chunks);
-  p.symmetric = x.symmetric;
   p.batch = (int)batch;
   const Tiling shape = tiling(x.a_planes, x.b_planes, x.m, x.n, x.k, batch, x.symmetric, sizeof(T) == 4, sms);
   p.ctas = shape.ctas;
@@ -561,7 +565,9 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
   p.b = Operand{shape.columns / shape.ctas, x.b_turned, x.b_planes};
   p.row_tiles = (int)ceil_div(x.m, kM * shape.ctas);
   p.col_tiles = (int)ceil_div(x.n, shape.columns);
-  p.items = (int)tiles(x.m, x.n, kM * shape.ctas, shape.columns, x.symmetric);
+  // (where all tiles are done at once, the half of them would save nothing but cost the second writing)
+  p.symmetric = x.symmetric && tiles(x.m, x.n, kM * shape.ctas, shape.columns, false) * batch > sms / shape.ctas;
+  p.items = (int)tiles(x.m, x.n, kM * shape.ctas, shape.columns, p.symmetric != 0);
   const int64_t total = (int64_t)p.items * batch, places = sms / shape.ctas;
   F2C_REQUIRE(total < (1ll << 30), F2C_ERR_LIMIT, "%s: too many tiles", op);
   const unsigned grid = (unsigned)((total < places ? total : places) * shape.ctas);
