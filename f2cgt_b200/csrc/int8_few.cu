@@ -119,10 +119,17 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const Params p) {
       const Scale s = scale_of(__reduce_max_sync(0xffffffffu, largest[i].of_float()));
       if (lane == 0) scale_s[r] = s.scale;
       int8_t* to = codes_s + r * pitch;
+      const auto some = [&](int v) { return v < n ? (n - v + 31) / 32 : 0; };
 #pragma unroll
-      for (int q = 0; q < kKept; ++q)
-        if (lane + 32 * q < n) write<T, BYTES>(to + (lane + 32 * q) * V, kept[i][q], s);
-      for (int v = lane + 32 * kKept; v < n; v += 32) write<T, BYTES>(to + v * V, read(i, v), s);
+      for (int q = 0; q < kKept; q += Vec::G)
+        if (lane + 32 * q < n) write<T, BYTES>(to + (lane + 32 * q) * V, 32 * V, some(lane + 32 * q), kept[i] + q, s);
+      for (int v = lane + 32 * kKept; v < n; v += 32 * Vec::G) {
+        Vec x[Vec::G];
+#pragma unroll
+        for (int g = 0; g < Vec::G; ++g)
+          if (v + 32 * g < n) x[g] = read(i, v + 32 * g);
+        write<T, BYTES>(to + v * V, 32 * V, some(v), x, s);
+      }
       for (int t = p.k + lane; t < units * kUnit; t += 32) to[t] = 0;
     }
     __syncthreads();

@@ -352,46 +352,3 @@ extern "C" int f2c_int8_mm(const int8_t* codes, int64_t ldq, const float* scales
   if (i8::is_few(m, n, k)) return i8::few(op, i8::Rows{j.a.p, nullptr, j.a.ld, 0, k, 0, m, F2C_I8}, j, st);
   return i8::mm(op, j, st);
 }
-
-extern "C" int64_t f2c_int8_linear_workspace(int64_t k1, int64_t k2, int dtype, const int8_t* w, int64_t ldw, int64_t m, int64_t n) {
-  const int64_t k = k1 + k2, ld = i8::round16(k);
-  if (m < 1 || n < 1 || k < 0 || k > i8::kMaxK) return 0;
-  const i8::Rows r{nullptr, nullptr, k1, k2, k1, k2, m, dtype};
-  const int64_t rows = i8::few_encodes(r, n) ? 0 : i8::round256(4 * m) + i8::round256(m * ld);
-  return rows + (k == 0 || i8::in_place(w, ldw, n) ? 0 : i8::round256(n * ld));
-}
-
-extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, const int8_t* w,
-                               int64_t ldw, const float* w_scales, const float* bias, int relu, void* out, int out_dtype, int64_t m, int64_t n,
-                               void* workspace, int64_t workspace_bytes, void* stream) {
-  const char* op = "int8_linear";
-  const i8::Rows r{x1, x2, ld1, ld2, k1, k2, m, dtype};
-  const int64_t k = k1 + k2;
-  if (const int rc = i8::check_rows(op, r)) return rc;
-  if (const int rc = i8::check(op, m, n, k, out_dtype)) return rc;
-  F2C_REQUIRE(n <= 1 || ldw >= k, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
-  if (m == 0 || n == 0) return F2C_OK;
-  F2C_REQUIRE(out && w_scales && (k == 0 || w), F2C_ERR_INVALID, "%s: null pointer", op);
-  const int64_t need = f2c_int8_linear_workspace(k1, k2, dtype, w, ldw, m, n);
-  F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,
-              "%s: workspace too small or not 256-byte aligned", op);
-  cudaStream_t st = (cudaStream_t)stream;
-  char* ws = (char*)workspace;
-  i8::Job j{};
-  j.a_scales = nullptr; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype;
-  if (i8::few_encodes(r, n)) {
-    j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);
-    return i8::few(op, r, j, st);
-  }
-  float* scales = (float*)ws;
-  ws += i8::round256(4 * m);
-  int8_t* codes = (int8_t*)ws;
-  const int64_t ldq = i8::round16(k);
-  ws += i8::round256(m * ldq);
-  j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);  // before the rows: the product may then ask for weights while these are encoded
-  if (const int rc = i8::quantize(r, codes, ldq, scales, st)) return rc;
-  j.a = i8::Operand{codes, ldq, m};
-  j.a_scales = scales; j.weights_first = 1;
-  if (i8::is_few(m, n, k)) return i8::few(op, i8::Rows{codes, nullptr, ldq, 0, k, 0, m, F2C_I8}, j, st);
-  return i8::mm(op, j, st);
-}

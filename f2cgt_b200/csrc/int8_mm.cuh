@@ -1,4 +1,4 @@
-// What the 8-bit products share between their files (int8_quantize.cu, int8_mm.cu, int8_few.cu).
+// What the 8-bit products share between their files (int8_quantize.cu, int8_mm.cu, int8_few.cu, int8_linear.cu).
 #pragma once
 #include "tcgen05.cuh"
 
@@ -115,14 +115,16 @@ struct Largest {
   }
 };
 
-template <int BYTES> struct Words;  // a vector of BYTES, and the word of its codes
+template <int BYTES> struct Words;  // a vector of BYTES
 template <> struct Words<16> { using type = uint4; };
+template <> struct Words<8> { using type = uint2; };
 template <> struct Words<4> { using type = uint32_t; };
 template <> struct Words<2> { using type = uint16_t; };
 
 template <typename T, int BYTES>
 struct Vector {
   static constexpr int V = BYTES / (int)sizeof(T), W = BYTES < 4 ? 1 : BYTES / 4;
+  static constexpr int G = V < 4 ? 4 / V : 1;  // vectors that are encoded together: four values share a branch
   union { typename Words<BYTES>::type raw; uint32_t w[W]; T v[V]; };
   __device__ __forceinline__ Vector() {
 #pragma unroll
@@ -130,22 +132,33 @@ struct Vector {
   }
 };
 
-// codes of a vector to its place
+// The codes of G vectors to their places, `step` bytes apart; the first `count` of them.
 template <typename T, int BYTES>
-__device__ __forceinline__ void write(int8_t* to, const Vector<T, BYTES>& v, const Scale& s) {
-  constexpr int V = Vector<T, BYTES>::V, N = V < 4 ? V : 4;
-  uint32_t word[V < 4 ? 1 : V / 4];
+__device__ __forceinline__ void write(int8_t* to, int step, int count, const Vector<T, BYTES>* v, const Scale& s) {
+  constexpr int V = Vector<T, BYTES>::V, G = Vector<T, BYTES>::G;
+  if constexpr (G == 1) {
+    uint32_t word[V / 4];
 #pragma unroll
-  for (int g = 0; g < V; g += N) {
-    float f[N];
+    for (int g = 0; g < V; g += 4) {
+      const float f[4] = {to_float(v->v[g]), to_float(v->v[g + 1]), to_float(v->v[g + 2]), to_float(v->v[g + 3])};
+      word[g / 4] = codes_of(f, s);
+    }
+    if (count > 0) {
+      if constexpr (V == 8) *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[1]);
+      else *reinterpret_cast<uint32_t*>(to) = word[0];
+    }
+  } else {
+    float f[4];
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = to_float(v.v[g + e]);
-    word[g / N] = codes_of(f, s);
+    for (int e = 0; e < 4; ++e) f[e] = to_float(v[e / V].v[e % V]);
+    const uint32_t word = codes_of(f, s);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (g >= count) break;
+      if constexpr (V == 2) *reinterpret_cast<uint16_t*>(to + g * step) = (uint16_t)(word >> (16 * g));
+      else to[g * step] = (int8_t)(word >> (8 * g));
+    }
   }
-  if constexpr (V == 8) *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[1]);
-  else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(to) = word[0];
-  else if constexpr (V == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)word[0];
-  else *to = (int8_t)word[0];
 }
 
 // ---------------------------------------------------------------- results

@@ -52,22 +52,33 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const i8::Rows r, in
   }
   const i8::Scale s = i8::scale_of(largest);
   int8_t* out = codes + row * ldq;
+  // of vectors at, at + THREADS, ...: G at a time
+  const auto left = [&](int i) { return i < n ? (n - i + THREADS - 1) / THREADS : 0; };
 #pragma unroll
-  for (int q = 0; q < KEPT; ++q)
-    if (at + q * THREADS < n) i8::write<T, BYTES>(out + (at + q * THREADS) * V, kept[q], s);
-  for (int i = at + KEPT * THREADS; i < n; i += THREADS) i8::write<T, BYTES>(out + i * V, read(i), s);
+  for (int q = 0; q < KEPT; q += Vec::G)
+    if (at + q * THREADS < n) i8::write<T, BYTES>(out + (at + q * THREADS) * V, THREADS * V, left(at + q * THREADS), kept + q, s);
+  for (int i = at + KEPT * THREADS; i < n; i += Vec::G * THREADS) {
+    Vec v[Vec::G];
+#pragma unroll
+    for (int g = 0; g < Vec::G; ++g)
+      if (i + g * THREADS < n) v[g] = read(i + g * THREADS);
+    i8::write<T, BYTES>(out + i * V, THREADS * V, left(i), v, s);
+  }
   if (at == 0) scales[row] = s.scale;
 }
+
+// two vectors a lane, or as many as are encoded together
+template <typename T, int BYTES> struct Vec2 { static constexpr int kept = i8::Vector<T, BYTES>::G > 2 ? 4 : 2; };
 
 template <typename T, int BYTES>
 static void launch(const i8::Rows& r, int8_t* codes, int64_t ldq, float* scales, cudaStream_t st) {
   const int64_t vectors = (r.k1 + r.k2) * (int64_t)sizeof(T) / BYTES;
   const dim3 warps((unsigned)ceil_div(r.m, kThreads / 32));
-  // A row up to 16 vectors a lane long is a warp's; where rows are few, one of more than two vectors a lane has a CTA.
-  if (vectors > 512 || (vectors > 64 && r.m < 1024))
+  // A row up to 16 vectors a lane long is a warp's; where rows are few, one of more than four vectors a lane has a CTA.
+  if (vectors > 512 || (vectors > 128 && r.m < 1024))
     launch_dependent(quantize_kernel<T, BYTES, kThreads, 4>, dim3((unsigned)r.m), kThreads, 0, st, r, codes, ldq, scales);
   else if (vectors <= 64)
-    launch_dependent(quantize_kernel<T, BYTES, 32, 2>, warps, kThreads, 0, st, r, codes, ldq, scales);
+    launch_dependent(quantize_kernel<T, BYTES, 32, Vec2<T, BYTES>::kept>, warps, kThreads, 0, st, r, codes, ldq, scales);
   else if (vectors <= 128)
     launch_dependent(quantize_kernel<T, BYTES, 32, 4>, warps, kThreads, 0, st, r, codes, ldq, scales);
   else
@@ -77,6 +88,7 @@ static void launch(const i8::Rows& r, int8_t* codes, int64_t ldq, float* scales,
 template <typename T>
 static void any(const i8::Rows& r, int8_t* codes, int64_t ldq, float* scales, cudaStream_t st) {
   if (r.fits(16, codes, ldq)) return launch<T, 16>(r, codes, ldq, scales, st);
+  if (r.fits(8, codes, ldq)) return launch<T, 8>(r, codes, ldq, scales, st);
   if constexpr (sizeof(T) == 2) {
     if (!r.fits(4, codes, ldq)) return launch<T, 2>(r, codes, ldq, scales, st);
   }
