@@ -10,6 +10,7 @@
 * ``SAGEConv`` - mean SAGE layer for hidden features (what the reference takes from DGL), aggregation through
   ``spmm_csr`` with a backward pass over the transposed block.
 * ``SAGE`` - examples/models.py:10-42: ReLU + dropout between layers.
+* ``Int8SAGE`` - a trained network answering in 8-bit integers.
 * ``GPUSamplingDataloader`` - examples/dataloader.py:154-192: per minibatch, hops in reversed(fan_out) order from the
   seeds with ``csr_sampling`` + ``tensor_relabel``; yields (input_nodes, output_nodes, blocks).
 
@@ -398,6 +399,38 @@ class SAGE(nn.Module):
         tf32 = _PRODUCT_DTYPE is None and torch.backends.cuda.matmul.allow_tf32
         return ops._native.sage_net(h_self, h_neigh, [b["indptr"] for b in blocks[1:]], [b["indices_local"] for b in blocks[1:]], rows, padded,
                                     weights, p, tf32, _PRODUCT_DTYPE)
+
+
+class Int8SAGE:
+    """A trained ``SAGE`` network that answers in 8-bit integers: every layer is one product of its rows, own and neighbours' mean side by side,
+    with ``fc_self | fc_neigh`` (``ops.int8_linear``), the weights quantised once, per output channel.  Aggregation, decoding and the hidden
+    rows are as in the float network; there is no dropout and no gradient.
+
+        answer = sage.Int8SAGE(model)(blocks)
+    """
+
+    def __init__(self, model):
+        self.first_input = model.layers[0].sm
+        self.layers = []
+        with torch.no_grad():
+            for layer in model.layers:
+                weight = torch.cat([layer.fc_self.weight, layer.fc_neigh.weight], dim=1)
+                bias = layer.fc_self.bias
+                self.layers.append(ops.int8_quantize(weight) + (bias.detach().float().clone() if bias is not None else None,))
+
+    @torch.no_grad()
+    def __call__(self, blocks):
+        if len(blocks) != len(self.layers):
+            raise RuntimeError(f"the network has {len(self.layers)} layers, there are {len(blocks)} blocks")
+        h = None
+        for i, ((codes, scales, bias), block) in enumerate(zip(self.layers, blocks)):
+            if i == 0:
+                sm, neighbours, dst = block.get("first_layer_input") or self.first_input.for_block(block)
+                own, mean = sm.decode_rows(dst), sm.aggregate(block["indptr"], neighbours)
+            else:
+                own, mean = h[:block["dst_nodes"].numel()], ops.spmm_csr(h, block["indptr"], block["indices_local"])
+            h = ops.int8_linear(own, codes, scales, bias, relu=i + 1 < len(self.layers), x2=mean)
+        return h
 
 
 def _hooked(module):

@@ -111,7 +111,7 @@ class DirectFusedAdam:
 
 
 def train(preset="small", table="replicated", rank=0, world=1, local_rank=0, epochs=3, min_timed_steps=0, batch_size=1024, lr=0.003,
-          dropout=0.5, index_dtype="int64", max_steps=0, precision="tf32", ahead=True):
+          dropout=0.5, index_dtype="int64", max_steps=0, precision="tf32", ahead=True, optimizer="adam", muon_lr=0.02, answer_int8=False):
     """Train on the preset's synthetic data inside an already initialised process (and, for world > 1 or a sharded table,
     process group); returns the record rank 0 reports (every rank gets it).  The first epoch is a discarded warm-up; when
     ``min_timed_steps`` is set, enough further epochs are run to time at least that many steps per rank.  Per-phase device
@@ -119,12 +119,15 @@ def train(preset="small", table="replicated", rank=0, world=1, local_rank=0, epo
     tf32_before = torch.backends.cuda.matmul.allow_tf32
     try:
         return _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batch_size, lr, dropout, index_dtype, max_steps, precision,
-                      ahead)
+                      ahead, optimizer, muon_lr, answer_int8)
     finally:
         torch.backends.cuda.matmul.allow_tf32 = tf32_before
 
 
-def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batch_size, lr, dropout, index_dtype, max_steps, precision, ahead):
+def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batch_size, lr, dropout, index_dtype, max_steps, precision, ahead,
+           optimizer_name, muon_lr, answer_int8):
+    if optimizer_name not in ("adam", "muon"):
+        raise ValueError("optimizer must be adam or muon")
     cfg = PRESETS[preset]
     device = torch.device("cuda", local_rank)
     idt = torch.int32 if index_dtype == "int32" else torch.int64
@@ -150,7 +153,10 @@ def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batc
     # Adam lr 0.003 with an exponential decay of 0.978 per epoch (examples/train_graphsage_nodeclass.py:56-57); one fused
     # kernel for all parameters (the model is tiny)
     gamma = 0.978
-    if DirectFusedAdam.available():
+    if optimizer_name == "muon":
+        from f2cgt_b200.muon import Muon
+        optimizer, scheduler = Muon(net.parameters(), lr=muon_lr, adam_lr=lr), None
+    elif DirectFusedAdam.available():
         optimizer, scheduler = DirectFusedAdam(net.parameters(), lr=lr), None
     else:
         optimizer = torch.optim.Adam(net.parameters(), lr=lr, fused=True)
@@ -242,6 +248,13 @@ def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batc
         sm = stats.clone(); dist.all_reduce(sm, op=dist.ReduceOp.SUM)
         stats = torch.cat([mx[:1], sm[1:2], mx[2:]])
     stats = stats.tolist()
+    int8 = None
+    if answer_int8:
+        net.eval()
+        with torch.no_grad():
+            want = net(blocks)
+        got = sage.Int8SAGE(net)(blocks)
+        int8 = {"relative_error": float((got - want).norm() / want.norm()), "same_class": float((got.argmax(1) == want.argmax(1)).float().mean())}
     if hasattr(cm, "close"):
         torch.cuda.synchronize()
         cm.close()
@@ -252,7 +265,7 @@ def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batc
         "breakdown_ms": {k: round(v, 4) for k, v in zip(phases, stats[2:])},
         "first_layer_edges_per_s": stats[1] / stats[0], "loss_last_step_per_epoch": [round(v, 4) for v in losses],
         "config": {k: (list(v) if isinstance(v, tuple) else v) for k, v in cfg.items()}, "index_dtype": index_dtype,
-        "precision": precision, "blocks_built_ahead": bool(ahead), "table": table, "data": "synthetic", "scaling": "strong (train ids split over ranks)",
+        "precision": precision, "optimizer": optimizer_name, **({"int8": int8} if int8 is not None else {}), "blocks_built_ahead": bool(ahead), "table": table, "data": "synthetic", "scaling": "strong (train ids split over ranks)",
         "timing": "wall clock around barrier + synchronize delimited epochs, first epoch discarded, max over ranks; breakdown = CUDA "
                   "events on the current stream, mean per step, max over ranks"}
 
@@ -291,6 +304,10 @@ def main():
     ap.add_argument("--min-timed-steps", type=int, default=0, help="run enough epochs to time at least this many steps")
     ap.add_argument("--precision", default="tf32", choices=["tf32", "fp32", "bf16"],
                     help="tf32: fp32 storage, tf32 tensor-core products (default); fp32: plain; bf16: product operands in bf16")
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"],
+                    help="muon: orthogonalised updates of the weight matrices (learning rate --muon-lr), Adam for the biases")
+    ap.add_argument("--muon-lr", type=float, default=0.02)
+    ap.add_argument("--answer-int8", action="store_true", help="also answer the last minibatch in 8-bit integers and report the difference")
     ap.add_argument("--no-pin", action="store_true", help="do not give every rank its own share of the node's CPUs")
     ap.add_argument("--no-ahead", action="store_true", help="build every minibatch inside its step instead of one step early on a side stream")
     ap.add_argument("--table", default="replicated", choices=["replicated", "sharded", "sharded_peer"],
@@ -311,7 +328,7 @@ def main():
             os.environ.setdefault("MASTER_PORT", "29577")
         dist.init_process_group("nccl", device_id=device, rank=rank, world_size=world)
     rec = train(args.preset, args.table, rank, world, local_rank, args.epochs, args.min_timed_steps, args.batch_size, args.lr,
-                args.dropout, args.index_dtype, args.max_steps, args.precision, not args.no_ahead)
+                args.dropout, args.index_dtype, args.max_steps, args.precision, not args.no_ahead, args.optimizer, args.muon_lr, args.answer_int8)
     if rank == 0:
         print(json.dumps(rec), flush=True)
     if dist.is_initialized():
