@@ -9,12 +9,13 @@
 //
 // Precision.  Operands are half precision times a power of two for each matrix and step, chosen by a bound on the matrix' norm so that
 // the largest values stay a factor of 30 away from infinity and the smallest keep their bits; sums are single precision, the norm's double.
-//  * 16-bit matrices.  The first X is exact, A and R are rounded to 11 bits (R multiplies from the left: its rounding turns the singular
-//    vectors by 2^-12 of R's size).  X's own rounding is noise of full rank, which the following steps multiply by up to the product of their
+//  * bfloat16.  The first X is exact, A and R are rounded to 11 bits (R multiplies from the left: its rounding turns the singular
+//    vectors by 2^-12 of R's size), or pairs where they have no more than 256 rows (the fewer, the less do roundings cancel out: 43 x 42 in bfloat16
+//    3.0e-3 off without, of which the result's own rounding is 1.7e-3).  X's own rounding is noise of full rank, which the following steps multiply by up to the product of their
 //    factors a, 3.4445^4 = 140 after the first, while large singular values only go to one: where that product is over 16, X is a pair of
 //    half precision numbers (22 bits) and R X two products.  For matrices of rank 8 the result is 2.6e-3 off then, and 2.6e-2 without.
-//  * 32-bit matrices.  All operands are pairs, a product is three (high by high, high by low, low by high): 22 bits throughout.  The tensor
-//    cores cut sums off instead of rounding them, for every 16 elements of K.  So the sums are taken out every 128 elements and added up in
+//  * float32, and float16, whose own 11 bits the result has to keep.  All operands are pairs, a product is three (high by high, high by low, low by high): 22 bits throughout.  The tensor
+//    cores cut sums off instead of rounding them, for every 16 elements of K.  So the sums are taken out every 64 or 128 elements and added up in
 //    registers, the small products are in front of the large one, and a X is not in the sum.  (Rank 3, 400 x 600: 2.5e-4 off without any of this,
 //    2e-4 without the taking out.)
 #include <math.h>
@@ -262,7 +263,7 @@ __device__ __forceinline__ void add(uint32_t (&sum)[32], const uint32_t (&r)[32]
 // first one issues the MMAs for both.
 template <int MODE, typename T, int CTAS>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, const __grid_constant__ Matrices s) {
-  constexpr bool kWide = sizeof(T) == 4;  // pairs by pairs: see above
+  constexpr bool kWide = is_wide<T>;  // pairs by pairs: see above
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const int products = p.a.planes + p.b.planes - 1;
       // Waits for a step are made behind the MMAs and commits of the one before, some of which the tensor cores still have to do meanwhile.
       const int mine_items = total > first ? (total - first + stride - 1) / stride : 0, all = mine_items * p.steps;
-      uint32_t n = 0;  // accumulations begun: one a tile, or (float32) one a step
+      uint32_t n = 0;  // accumulations begun: one a tile, or (pairs) one a step
       int done_steps = 0, i = 0;
       const auto wait_full = [&]() { wait_bar(bars.full + slot, round & 1, left); };
       const auto wait_acc = [&]() {  // of accumulation n
@@ -484,10 +485,11 @@ struct Shape {
   int64_t ldx() const { return (cols + 7) / 8 * 8; }
   int64_t ldp() const { return (p() + 7) / 8 * 8; }
   int64_t x_bytes() const { return round256(2 * batch * rows * ldx()); }
+  bool fine(bool wide) const { return wide || p() <= 256; }  // A and R are pairs
   int64_t p_bytes() const { return round256(2 * batch * p() * ldp()); }
 };
 
-// Planes of X in front of a step: 2 for float32; otherwise see above (`exact`: the first X is).
+// Planes of X in front of a step: 2 where all operands are pairs; otherwise see above (`exact`: the first X is).
 static int x_planes(const Steps& st, int t, bool wide, bool exact) {
   if (wide) return 2;
   if (t == 0 && exact) return 1;
@@ -500,7 +502,7 @@ static int x_planes(const Steps& st, int t, bool wide, bool exact) {
 }
 
 static int64_t workspace(const Shape& s, bool wide) {
-  return 4 * s.x_bytes() + (wide ? 4 : 2) * s.p_bytes() + round256(8 * s.batch * kMaxParts) + round256((int64_t)sizeof(Factors) * F2C_MAX_NS_STEPS * s.batch);
+  return 4 * s.x_bytes() + (s.fine(wide) ? 4 : 2) * s.p_bytes() + round256(8 * s.batch * kMaxParts) + round256((int64_t)sizeof(Factors) * F2C_MAX_NS_STEPS * s.batch);
 }
 
 struct Planes {
@@ -516,16 +518,17 @@ static int64_t tiles(int64_t m, int64_t n, int rows, int columns, bool symmetric
   return items;
 }
 
-// Pieces of 64 elements of K in a stage.  float32, whose sums are taken out after every stage: two (2048 x 8192: 2.59 ms a step, 2.81 with one);
-// 16-bit matrices: one (4096 x 4096: 1.36 ms, 1.49 with two, of which fewer stages fit).
-static int chunks_of(bool wide) { return wide ? 2 : 1; }
+// Pieces of 64 elements of K in a stage.  Pairs, whose sums are taken out after every stage: two (2048 x 8192 float32: 2.59 ms a step, 2.81 with one), but
+// one for R X while it is short, where what is cut off the sums is what counts (1500 x 300: 3.1e-6 off with two).  bfloat16: one (4096 x 4096: 1.36 ms,
+// 1.49 with two, of which fewer stages fit).
+static int chunks_of(bool wide, bool apply, int64_t k) { return wide && !(apply && k <= 1024) ? 2 : 1; }
 
 struct Tiling { int ctas, columns; };
 
 // The tiles of least cycles: rounds over the SMs of a tile's stages, which take the longer of their MMAs (half a cycle a column, 46 cycles at least,
-// and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of float32 to take the sums out.
-static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, int sms) {
-  const int products = planes_a + planes_b - 1, chunks = chunks_of(wide);
+// and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of pairs to take the sums out.
+static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, bool apply, int sms) {
+  const int products = planes_a + planes_b - 1, chunks = chunks_of(wide, apply, k);
   Tiling best{1, 64};
   int64_t least = 0;
   for (const Tiling t : {Tiling{2, 256}, Tiling{2, 128}, Tiling{1, 256}, Tiling{1, 128}, Tiling{1, 64}}) {
@@ -556,10 +559,11 @@ template <int MODE, typename T>
 static int multiply(const char* op, const Product& x, Params p, const Matrices& s, int64_t batch, cudaStream_t st) {
   const int sms = current_sm_count();
   p.m = (int)x.m; p.n = (int)x.n;
-  p.chunks = chunks_of(sizeof(T) == 4);
+  constexpr bool kApplies = MODE == kApply || MODE == kFinal;
+  p.chunks = chunks_of(is_wide<T>, kApplies, x.k);
   p.steps = (int)ceil_div(x.k, kK * p.chunks);
   p.batch = (int)batch;
-  const Tiling shape = tiling(x.a_planes, x.b_planes, x.m, x.n, x.k, batch, x.symmetric, sizeof(T) == 4, sms);
+  const Tiling shape = tiling(x.a_planes, x.b_planes, x.m, x.n, x.k, batch, x.symmetric, is_wide<T>, kApplies, sms);
   p.ctas = shape.ctas;
   p.a = Operand{kM, x.a_turned, x.a_planes};
   p.b = Operand{shape.columns / shape.ctas, x.b_turned, x.b_planes};
@@ -592,12 +596,12 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
 
 template <typename T>
 static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps& st, char* ws, cudaStream_t stream) {
-  constexpr bool kWide = sizeof(T) == 4;
-  const bool exact = !kWide && src.listed == 0, tall = s.rows > s.cols;
+  constexpr bool kWide = is_wide<T>;
+  const bool exact = sizeof(T) == 2 && src.listed == 0, tall = s.rows > s.cols;
   auto take = [&](int64_t bytes) { char* at = ws; ws += bytes; return at; };
   Planes x[2], a{}, r{};
   for (Planes& q : x) { q.high = (__half*)take(s.x_bytes()); q.low = (__half*)take(s.x_bytes()); }
-  for (Planes* q : {&a, &r}) { q->high = (__half*)take(s.p_bytes()); q->low = kWide ? (__half*)take(s.p_bytes()) : nullptr; }
+  for (Planes* q : {&a, &r}) { q->high = (__half*)take(s.p_bytes()); q->low = s.fine(kWide) ? (__half*)take(s.p_bytes()) : nullptr; }
   double* parts = (double*)take(round256(8 * s.batch * kMaxParts));
   Factors* table = (Factors*)take(0);
   src.size = s.rows * s.cols;
@@ -622,11 +626,11 @@ static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps&
     return check_launch(op);
   }
   const int64_t p = s.p();
-  const int inner = kWide ? 2 : 1;
+  const int gram_planes = kWide ? 2 : 1, inner = s.fine(kWide) ? 2 : 1;  // of X in A = X X^T, and of A and R
   for (int t = 0; t < st.count; ++t) {
     const bool last = t + 1 == st.count, poly = st.co[3 * t + 2] != 0.0f;
     // A = X X^T: of a tall matrix, whose transpose X is, the rows run along K
-    Product gram{x[t & 1], x[t & 1], inner, inner, tall, tall, s.rows, s.cols, s.ldx(), s.rows, s.cols, s.ldx(), p, p, tall ? s.rows : s.cols, true};
+    Product gram{x[t & 1], x[t & 1], gram_planes, gram_planes, tall, tall, s.rows, s.cols, s.ldx(), s.rows, s.cols, s.ldx(), p, p, tall ? s.rows : s.cols, true};
     Params g{};
     g.factors = table + t;
     g.high = poly ? a.high : r.high; g.low = poly ? a.low : r.low;
@@ -704,7 +708,7 @@ static int check_shape(const char* op, const Shape& s) {
 using namespace f2c;
 
 extern "C" int64_t f2c_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t cols) {
-  return batch < 1 || rows < 1 || cols < 1 || ns::is_small(rows, cols) ? 0 : ns::workspace(ns::Shape{batch, rows, cols}, dtype == F2C_F32);
+  return batch < 1 || rows < 1 || cols < 1 || ns::is_small(rows, cols) ? 0 : ns::workspace(ns::Shape{batch, rows, cols}, dtype != F2C_BF16);
 }
 
 extern "C" int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t batch, int64_t rows, int64_t cols, const float* coefficients_host,
@@ -748,7 +752,7 @@ extern "C" int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int coun
   ns::Matrices src{};
   for (int i = 0; list_host != nullptr && i < count; ++i) {
     if (list_host[i].rows < 0 || list_host[i].cols < 0 || ns::is_small(list_host[i].rows, list_host[i].cols) || !group_of(list_host, count, i, &src)) continue;
-    const int64_t bytes = ns::workspace(ns::Shape{src.listed, list_host[i].rows, list_host[i].cols}, dtype == F2C_F32);
+    const int64_t bytes = ns::workspace(ns::Shape{src.listed, list_host[i].rows, list_host[i].cols}, dtype != F2C_BF16);
     most = bytes > most ? bytes : most;
   }
   return most;

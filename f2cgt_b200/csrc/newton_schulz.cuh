@@ -26,6 +26,10 @@ struct Matrices {  // of one shape: a stack, or a list
   __device__ __forceinline__ float* moment(int z) const { return listed ? list[z].momentum : nullptr; }
 };
 
+// Types whose matrices are held in pairs of half precision throughout (newton_schulz.cu).
+template <typename T> constexpr bool is_wide = true;
+template <> constexpr bool is_wide<__nv_bfloat16> = false;
+
 // Factors of a step, for a matrix.
 struct Factors {
   float gram, poly_b, poly_c, apply, own;  // As = gram Xs Xs^T; Rs = poly_c As^2 + poly_b As; the next Xs = own Xs + apply Rs Xs

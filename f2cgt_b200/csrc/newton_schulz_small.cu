@@ -6,7 +6,8 @@
 // X X^T, and the same bytes, read as rows along N, for R X.  A thread has a row of X, A and R and a quarter of its columns; what the next
 // product reads goes from TMEM through registers to shared memory.
 // What bounds it is the chain of 15 products, each with its MMAs, the reading of its sums and a barrier (128 x 128 float32: 24 MMAs of 64 cycles
-// in some 2500).  Precision is as in newton_schulz.cu: float32 in pairs throughout, 16-bit matrices with A and R in one plane; X is always a pair.
+// in some 2500).  Precision is as in newton_schulz.cu: everything in pairs, but that bfloat16's
+// X X^T takes the high planes alone.
 #include "newton_schulz.cuh"
 
 namespace f2c {
@@ -42,12 +43,12 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& high, uint32_
   high = *reinterpret_cast<const uint32_t*>(&h);
   low = *reinterpret_cast<const uint32_t*>(&l);
 }
-__device__ __forceinline__ void store_pair(uint32_t high, uint32_t low, bool both, int r, int c, const float (&v)[8]) {
+__device__ __forceinline__ void store_pair(uint32_t high, uint32_t low, int r, int c, const float (&v)[8]) {
   uint32_t h[4], l[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) split2(v[2 * e], v[2 * e + 1], h[e], l[e]);
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(high, r, c)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-  if (both) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(low, r, c)), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(low, r, c)), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
 }
 __device__ __forceinline__ void load8(uint32_t at, float (&v)[8]) {
   uint32_t w[4];
@@ -66,7 +67,7 @@ template <typename T, int V> struct alignas(V * sizeof(T)) Few { T v[V]; };
 // V: elements read and written at a time
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constant__ Matrices s, const __grid_constant__ Steps st, int64_t stack_rows, int64_t stack_cols, int* error) {
-  constexpr bool kWide = sizeof(T) == 4;
+  constexpr bool kWide = is_wide<T>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Shared sh;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
     fence_before();
     __syncthreads();
   };
-  const int inner = kWide ? 2 : 1;
+  constexpr int kGramPlanes = kWide ? 2 : 1;
   float kept[kCols / 4];  // of the result: a thread's columns
 #pragma unroll
   for (int j = 0; j < kCols / 4; ++j) kept[j] = 0.0f;
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
     const Factors f = sh.factors[t];
     const bool poly = st.co[3 * t + 2] != 0.0f, last = t + 1 == st.count;
     // A = X X^T
-    product(tmem + kGramAt, smem + kXAt, inner, smem + kXAt, inner, kXPlane, false, p16, q16 / 16);
+    product(tmem + kGramAt, smem + kXAt, kGramPlanes, smem + kXAt, kGramPlanes, kXPlane, false, p16, q16 / 16);
     const int c0 = group * 32;  // of 128
     uint32_t a[32];
     if (c0 < p16) {
@@ -250,12 +251,12 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(a[j + e]) * f.gram;
-        store_pair(smem + kAAt, smem + kAAt + kAPlane, kWide, row, c0 + j, v);
+        store_pair(smem + kAAt, smem + kAAt + kAPlane, row, c0 + j, v);
       }
     }
     next();
     if (poly) {  // R = c A^2 + b A
-      product(tmem + kSquareAt, smem + kAAt, inner, smem + kAAt, inner, kAPlane, false, p16, p16 / 16);
+      product(tmem + kSquareAt, smem + kAAt, 2, smem + kAAt, 2, kAPlane, false, p16, p16 / 16);
       if (c0 < p16) {
         uint32_t r[32];
         tmem_ld32(lanes + kSquareAt + (uint32_t)c0, r);
@@ -265,13 +266,13 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = fmaf(f.poly_c, __uint_as_float(r[j + e]), f.poly_b * (__uint_as_float(a[j + e]) * f.gram));
-          store_pair(smem + kAAt, smem + kAAt + kAPlane, kWide, row, c0 + j, v);
+          store_pair(smem + kAAt, smem + kAAt + kAPlane, row, c0 + j, v);
         }
       }
       next();
     }
     // X <- a X + R X: X's rows run along K here
-    product(tmem + kApplyAt, smem + kAAt, inner, smem + kXAt, 2, kXPlane, true, q16, p16 / 16);
+    product(tmem + kApplyAt, smem + kAAt, 2, smem + kXAt, 2, kXPlane, true, q16, p16 / 16);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int x0 = (group + 4 * half) * 32;  // of 256
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
           v[e] = fmaf(f.own, h[e], fmaf(f.own, l[e], __uint_as_float(r[j + e]) * f.apply));
           kept[half * 32 + j + e] = v[e];
         }
-        if (!last) store_pair(smem + kXAt, smem + kXAt + kXPlane, true, row, x0 + j, v);
+        if (!last) store_pair(smem + kXAt, smem + kXAt + kXPlane, row, x0 + j, v);
       }
     }
     if (!last) next();
