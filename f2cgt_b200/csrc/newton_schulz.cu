@@ -519,16 +519,17 @@ static int64_t tiles(int64_t m, int64_t n, int rows, int columns, bool symmetric
 }
 
 // Pieces of 64 elements of K in a stage.  Pairs, whose sums are taken out after every stage: two (2048 x 8192 float32: 2.59 ms a step, 2.81 with one), but
-// one for R X while it is short, where what is cut off the sums is what counts (1500 x 300: 3.1e-6 off with two).  bfloat16: one (4096 x 4096: 1.36 ms,
-// 1.49 with two, of which fewer stages fit).
-static int chunks_of(bool wide, bool apply, int64_t k) { return wide && !(apply && k <= 1024) ? 2 : 1; }
+// one of matrices of up to 1024 rows or columns, whose products are short anyway: the cutting off makes sums smaller, all alike, and
+// the fewer singular values there are, the more it counts (1500 x 300: 3.3e-6 off with two).  bfloat16: one (4096 x 4096: 1.36 ms, 1.49 with two,
+// of which fewer stages fit).
+static int chunks_of(bool wide, int64_t p) { return wide && p > 1024 ? 2 : 1; }
 
 struct Tiling { int ctas, columns; };
 
 // The tiles of least cycles: rounds over the SMs of a tile's stages, which take the longer of their MMAs (half a cycle a column, 46 cycles at least,
 // and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of pairs to take the sums out.
-static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, bool apply, int sms) {
-  const int products = planes_a + planes_b - 1, chunks = chunks_of(wide, apply, k);
+static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, int64_t p, int sms) {
+  const int products = planes_a + planes_b - 1, chunks = chunks_of(wide, p);
   Tiling best{1, 64};
   int64_t least = 0;
   for (const Tiling t : {Tiling{2, 256}, Tiling{2, 128}, Tiling{1, 256}, Tiling{1, 128}, Tiling{1, 64}}) {
@@ -553,17 +554,17 @@ struct Product {
   int64_t a_rows, a_cols, a_ld, b_rows, b_cols, b_ld;  // the operands' matrices as they lie
   int64_t m, n, k;
   bool symmetric;
+  int64_t smaller = 0;                 // side of the matrices
 };
 
 template <int MODE, typename T>
 static int multiply(const char* op, const Product& x, Params p, const Matrices& s, int64_t batch, cudaStream_t st) {
   const int sms = current_sm_count();
   p.m = (int)x.m; p.n = (int)x.n;
-  constexpr bool kApplies = MODE == kApply || MODE == kFinal;
-  p.chunks = chunks_of(is_wide<T>, kApplies, x.k);
+  p.chunks = chunks_of(is_wide<T>, x.smaller);
   p.steps = (int)ceil_div(x.k, kK * p.chunks);
   p.batch = (int)batch;
-  const Tiling shape = tiling(x.a_planes, x.b_planes, x.m, x.n, x.k, batch, x.symmetric, is_wide<T>, kApplies, sms);
+  const Tiling shape = tiling(x.a_planes, x.b_planes, x.m, x.n, x.k, batch, x.symmetric, is_wide<T>, x.smaller, sms);
   p.ctas = shape.ctas;
   p.a = Operand{kM, x.a_turned, x.a_planes};
   p.b = Operand{shape.columns / shape.ctas, x.b_turned, x.b_planes};
@@ -635,18 +636,21 @@ static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps&
     g.factors = table + t;
     g.high = poly ? a.high : r.high; g.low = poly ? a.low : r.low;
     g.ld = s.ldp(); g.stack = p * s.ldp();
+    gram.smaller = p;
     if (const int rc = multiply<kGram, T>(op, gram, g, src, s.batch, stream)) return rc;
     if (poly) {
       Product square{a, a, inner, inner, 0, 0, p, p, s.ldp(), p, p, s.ldp(), p, p, p, true};
       Params q = g;
       q.add_high = a.high; q.add_low = a.low;
       q.high = r.high; q.low = r.low;
+      square.smaller = p;
       if (const int rc = multiply<kPoly, T>(op, square, q, src, s.batch, stream)) return rc;
     }
     // the rows of the next X are columns of this product, so that a warp writes 32 neighbours
     const int next = last ? 1 : x_planes(st, t + 1, kWide, exact);
     Product apply = tall ? Product{r, x[t & 1], inner, planes, 0, 0, p, p, s.ldp(), s.rows, s.cols, s.ldx(), p, s.rows, p, false}
                          : Product{x[t & 1], r, planes, inner, 1, 0, s.rows, s.cols, s.ldx(), p, p, s.ldp(), s.cols, p, p, false};
+    apply.smaller = p;
     Params q{};
     q.factors = table + t;
     q.gain = src.lr * (float)sqrt(s.rows > s.cols ? (double)s.rows / (double)s.cols : 1.0);
