@@ -5,13 +5,16 @@
 // what few rows have to read, and they fill the MMA's 128 rows; an epilogue thread has one channel, whose scale and bias stay in
 // registers, and a warp writes 32 neighbouring channels of a row of out without staging them.  128 columns of K come per step with TMA
 // (128-byte swizzle, zeros behind the operands' edges) through a ring of stages; the int32 accumulators of two tiles alternate in TMEM.
-//  * Rows per tile: so many that the tiles of one round over the SMs have equal work (see plan()).
-//  * Short K and few channel tiles: a CTA keeps its channels' weights in shared memory and only the rows travel.
+//  * Rows per tile: so many that the SMs have equal work in few rounds (see plan()).
+//  * Many tiles and a long K: pairs of CTAs share a tile of 256 channels, so that each fetches half of the rows: 32 KB for a step of K instead of 48.
 //  * Few tiles and a long K: the CTAs of a cluster each take a part of K and add their sums over distributed shared memory, which is exact
 //    and in any order the same.
 // Every wait is bounded: when one runs out the CTA's roles all leave, what it has not finished becomes NaN, copies and products in flight are
 // waited for, the error word is raised and TMEM is freed.
 #include "int8_mm.cuh"
+
+#include <algorithm>
+#include <climits>
 
 namespace f2c {
 namespace i8 {
@@ -26,7 +29,7 @@ struct Params {
   int64_t m;
   int n, steps;             // steps of K
   int channel_tiles, tile_rows, items;
-  int stages, resident, split, relu;
+  int stages, split, relu;
   int tmem, accumulators;   // columns of an accumulator, and how many
   int parts_at, share_log;  // clusters: where the sums are in shared memory, and of how many rows
   int weights_first;        // the kernel before this one does not make the weights
@@ -34,39 +37,45 @@ struct Params {
 };
 
 struct Bars {
-  uint64_t full[kMaxStages], empty[kMaxStages], weights, drain, acc_full[2], acc_empty[2];
+  uint64_t full[kMaxStages], empty[kMaxStages], drain, acc_full[2], acc_empty[2];
   uint32_t tmem;
   int failed, lost;  // lost: of any CTA of the cluster
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ CUtensorMap w, const Params p) {
+// CTAS 2: the two CTAs of a cluster work on 256 channels, each with 128 of them and half of the tile's rows in its shared memory; the first one
+// issues the MMAs for both.
+template <typename T, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS == 1 ? 2 : 1) mm_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ CUtensorMap w, const Params p) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
   __shared__ __align__(16) float scales_s[kEpilogueWarps][kMaxN];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
-  const int rank = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, stride = (int)gridDim.x / p.split;
-  const int step0 = (int)((int64_t)p.steps * rank / p.split), steps = (int)((int64_t)p.steps * (rank + 1) / p.split) - step0;
-  const uint32_t b_bytes = (uint32_t)p.tile_rows * kK;
-  unsigned char* ring = smem + (p.resident ? (size_t)steps * kABytes : 0);
-  const uint32_t stage_bytes = b_bytes + (p.resident ? 0u : (uint32_t)kABytes);
+  const int split = CTAS == 1 ? p.split : 1, group = split * CTAS;
+  const int rank = (int)blockIdx.x % group, first = (int)blockIdx.x / group, stride = (int)gridDim.x / group;
+  const int part = CTAS == 1 ? rank : 0;  // of K
+  const int step0 = (int)((int64_t)p.steps * part / split), steps = (int)((int64_t)p.steps * (part + 1) / split) - step0;
+  const int tile_channels = kM * CTAS, b_rows = p.tile_rows / CTAS, own_channels = CTAS == 1 ? 0 : rank * kM, own_rows = CTAS == 1 ? 0 : rank * b_rows;
+  const uint32_t b_bytes = (uint32_t)b_rows * kK;
+  const uint32_t stage_bytes = (uint32_t)kABytes + b_bytes;
   uint32_t left = kWaitLimit;
 
-  if (wid == 1) alloc_tmem(&bars.tmem, (uint32_t)p.tmem * p.accumulators);
+  if (wid == 1) {
+    if (CTAS == 2) alloc_tmem_pair(&bars.tmem, (uint32_t)p.tmem * p.accumulators);
+    else alloc_tmem(&bars.tmem, (uint32_t)p.tmem * p.accumulators);
+  }
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) { init_bar(bars.full + s, 1); init_bar(bars.empty + s, 1); }
-    init_bar(&bars.weights, 1);
     init_bar(&bars.drain, 1);
-    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps); }
+    for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps * CTAS); }
     fence_bars();
     bars.failed = 0;
     bars.lost = 0;
   }
   fence_before();
   __syncthreads();
+  if (group > 1) cluster_barrier();  // all are here before the first tells another its sums, or that it has loaded
   fence_after();
-  if (p.split > 1) cluster_barrier();  // all are here before the first tells another its sums
   const uint32_t tmem = bars.tmem;
   const int share = 1 << p.share_log;  // rows whose sums a CTA of a cluster adds up
   const uint32_t parts = smem_u32(smem) + (uint32_t)p.parts_at;
@@ -82,52 +91,60 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
     }
     __syncwarp();
     if (!p.weights_first) dependency_wait();
-    const uint32_t ring0 = smem_u32(ring), codes_at = p.resident ? 0u : (uint32_t)kABytes, bars0 = smem_u32(bars.full);
+    const uint32_t ring = smem_u32(smem), bars0 = CTAS == 2 ? peer_address(smem_u32(bars.full), 0) : smem_u32(bars.full);
+    const auto load = [&](bool go, const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int y) {
+      if (CTAS == 2) tma_load_pair(go, map, dst, bar, x, y);
+      else tma_load(go, map, dst, bar, x, y);
+    };
+    const bool counts = CTAS == 1 || rank == 0;  // the first one's barriers count the bytes of both
     int ahead = 0;  // stages whose weights have been asked for
-    if (p.resident) {
-      expect_if(mine, &bars.weights, (uint32_t)steps * kABytes);
-      for (int i = 0; i < steps; ++i) tma_load(mine, &w, smem_u32(smem) + (uint32_t)i * kABytes, smem_u32(&bars.weights), (step0 + i) * kK, first % p.channel_tiles * kM);
-    } else if (p.weights_first) {
+    if (p.weights_first) {
       for (; ahead < min(p.stages, steps); ++ahead) {
-        expect_if(mine, bars.full + ahead, stage_bytes);
-        tma_load(mine, &w, ring0 + (uint32_t)ahead * stage_bytes, bars0 + 8u * (uint32_t)ahead, (step0 + ahead) * kK, first % p.channel_tiles * kM);
+        expect_if(mine && counts, bars.full + ahead, stage_bytes * CTAS);
+        load(mine, &w, ring + (uint32_t)ahead * stage_bytes, bars0 + 8u * (uint32_t)ahead, (step0 + ahead) * kK, first % p.channel_tiles * tile_channels + own_channels);
       }
+      dependency_wait();
     }
-    if (p.weights_first) dependency_wait();
     release_dependents();
     for (int item = first; item < p.items; item += stride) {
-      const int channel0 = item % p.channel_tiles * kM, row0 = item / p.channel_tiles * p.tile_rows;
+      const int channel0 = item % p.channel_tiles * tile_channels + own_channels, row0 = item / p.channel_tiles * p.tile_rows + own_rows;
       for (int i = 0; i < steps; ++i) {
         if (round > 0) wait_bar(bars.empty + s, (round - 1) & 1, left);
         const bool go = mine && left != 0u, fresh = go && (round > 0 || s >= ahead);
-        const uint32_t stage = ring0 + (uint32_t)s * stage_bytes, bar = bars0 + 8u * (uint32_t)s;
-        expect_if(fresh, bars.full + s, stage_bytes);
-        tma_load(fresh && !p.resident, &w, stage, bar, (step0 + i) * kK, channel0);
-        tma_load(go, &codes, stage + codes_at, bar, (step0 + i) * kK, row0);
+        const uint32_t stage = ring + (uint32_t)s * stage_bytes, bar = bars0 + 8u * (uint32_t)s;
+        expect_if(fresh && counts, bars.full + s, stage_bytes * CTAS);
+        load(fresh, &w, stage, bar, (step0 + i) * kK, channel0);
+        load(go, &codes, stage + (uint32_t)kABytes, bar, (step0 + i) * kK, row0);
         if (++s == p.stages) { s = 0; ++round; }
       }
     }
   } else if (wid == 1) {
     // ================= MMAs
     const bool mine = elected() != 0u;
-    const uint32_t idesc = instruction(kSumS32, kFormatS8, kM, (uint32_t)p.tile_rows);
-    const uint32_t a_low = desc_low(smem_u32(p.resident ? smem : ring), kChunkAlongK), b_low = desc_low(smem_u32(ring) + (p.resident ? 0 : kABytes), kChunkAlongK);
-    if (p.resident) wait_bar(&bars.weights, 0, left);
+    const uint32_t idesc = instruction(kSumS32, kFormatS8, kM * CTAS, (uint32_t)p.tile_rows);
+    const uint32_t a_low = desc_low(smem_u32(smem), kChunkAlongK), b_low = a_low + (kABytes >> 4);
+    const auto done = [&](bool go, const uint64_t* bar) {
+      if (CTAS == 2) commit_pair(go, bar);
+      else commit(go, bar);
+    };
     uint32_t t = 0;
-    for (int item = first; item < p.items; item += stride, ++t) {
+    for (int item = CTAS == 1 || rank == 0 ? first : p.items; item < p.items; item += stride, ++t) {
       const uint32_t buf = t & 1u, acc = tmem + buf * (uint32_t)p.tmem;
       if (t >= 2) wait_bar(bars.acc_empty + buf, ((t >> 1) - 1) & 1, left);
       for (int i = 0; i < steps; ++i) {
         wait_bar(bars.full + s, round & 1, left);
         fence_after();
         const bool go = mine && left != 0u;
-        const uint32_t at = (uint32_t)s * (stage_bytes >> 4), a = a_low + (p.resident ? (uint32_t)i * (kABytes >> 4) : at), b = b_low + at;
+        const uint32_t at = (uint32_t)s * (stage_bytes >> 4), a = a_low + at, b = b_low + at;
 #pragma unroll
-        for (uint32_t q = 0; q < kK / 32; ++q) mma_i8(go, acc, desc(a + q * kStepAlongK), desc(b + q * kStepAlongK), idesc, i + (int)q != 0);
-        commit(go, bars.empty + s);
+        for (uint32_t q = 0; q < kK / 32; ++q) {
+          if (CTAS == 2) mma_i8_pair(go, acc, desc(a + q * kStepAlongK), desc(b + q * kStepAlongK), idesc, i + (int)q != 0);
+          else mma_i8(go, acc, desc(a + q * kStepAlongK), desc(b + q * kStepAlongK), idesc, i + (int)q != 0);
+        }
+        done(go, bars.empty + s);
         if (++s == p.stages) { s = 0; ++round; }
       }
-      commit(mine && left != 0u, bars.acc_full + buf);
+      done(mine && left != 0u, bars.acc_full + buf);
     }
   } else {
     // ================= epilogue: a warp has the TMEM lanes of its quarter and every other 32 rows of the tile, thread = channel
@@ -138,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
     dependency_wait();
     for (int item = first; item < p.items; item += stride, ++t) {
       const uint32_t buf = t & 1u;
-      const int channel = item % p.channel_tiles * kM + quarter * 32 + lane;
+      const int channel = item % p.channel_tiles * tile_channels + own_channels + quarter * 32 + lane;
       const int64_t row0 = (int64_t)(item / p.channel_tiles) * p.tile_rows;
       const int rows = (int)min((int64_t)p.tile_rows, p.m - row0);
       const bool mine = channel < p.n;
@@ -158,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = 0u;
         }
-        if (p.split > 1) {
+        if (split > 1) {
           // row c goes to CTA c / share, there [this CTA][c % share][channel]
           const uint32_t to = parts + 4u * (uint32_t)(rank * share * kM + quarter * 32 + lane);
 #pragma unroll
@@ -169,15 +186,18 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
         }
         __syncwarp();
       }
-      if (p.split > 1 && lost && lane < p.split) peer_store(peer_address(smem_u32(&bars.lost), (uint32_t)lane), 1u);
+      if (split > 1 && lost && lane < split) peer_store(peer_address(smem_u32(&bars.lost), (uint32_t)lane), 1u);
       // the accumulators have been read
       fence_before();
       __syncwarp();
-      if (lane == 0) arrive(bars.acc_empty + buf);
+      if (lane == 0) {
+        if (CTAS == 2) peer_arrive(peer_address(smem_u32(bars.acc_empty + buf), 0));
+        else arrive(bars.acc_empty + buf);
+      }
     }
   }
   if (left == 0u) bars.failed = 1;
-  if (p.split > 1) {
+  if (split > 1) {
     // a cluster has one tile, whose rows its CTAs share: all sums have been told when all have got here
     __syncwarp();
     cluster_barrier();
@@ -197,18 +217,17 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
         int sum = 0;
 #pragma unroll
         for (int q = 0; q < kMaxSplit; ++q)
-          if (q < p.split) sum += part[(q * share + i) * kM];
+          if (q < split) sum += part[(q * share + i) * kM];
         if (mine) ((T*)p.out)[(row0 + c) * p.n + channel] = from_float<T>(finish(sum, scales_s[wid - 2][c] * w_scale, bias, floor));
       }
     }
   }
   fence_before();
   __syncthreads();
-  if (bars.failed) {
-    // copies in flight write to this CTA's shared memory, MMAs in flight read it and write its TMEM: wait (bounded) for what was issued
+  if (bars.failed && (CTAS == 1 || rank == 0)) {
+    // copies in flight write to shared memory, MMAs in flight read it and write TMEM, of both CTAs of a pair: wait (bounded) for what was issued
     left = kWaitLimit;
     if (tid == 0) {
-      if (p.resident) wait_bar(&bars.weights, 0, left);
       for (int q = 0; q < p.stages; ++q) {
         const uint32_t uses = round + (q < s ? 1u : 0u);
         if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
@@ -219,9 +238,11 @@ __global__ void __launch_bounds__(kThreads, 2) mm_kernel(const __grid_constant__
     }
     __syncthreads();
   }
+  if (CTAS == 2) cluster_barrier();
   if (wid == 1) {
     fence_after();
-    free_tmem(tmem, (uint32_t)p.tmem * p.accumulators);
+    if (CTAS == 2) free_tmem_pair(tmem, (uint32_t)p.tmem * p.accumulators);
+    else free_tmem(tmem, (uint32_t)p.tmem * p.accumulators);
   }
   if (tid == 0 && bars.failed) report_wait(p.error, 4);
 }
@@ -256,68 +277,77 @@ int check(const char* op, int64_t m, int64_t n, int64_t k, int out_dtype) {
 
 Plan plan(int64_t m, int64_t n, int64_t k, int sms) {
   Plan p{};
-  p.channel_tiles = (int)ceil_div(n, kM);
+  const int channel_tiles = (int)ceil_div(n, kM);
   p.steps = (int)ceil_div(k, kK);
-  // Rows per tile and parts of K: the pair of least cycles.  A step of K takes the longer of its bytes at 56 a cycle (what an SM was seen
-  // to get from L2 with all others at it) and its MMAs; the results 12 cycles a row, beside the next tile's steps; a tile 1000 more;
-  // the exchange between the parts of K 2000 and 16 a row.  (59,000 x 128 x 256: 9.2 us with 256 rows, 10.0 with 96, 11.6 with 64; 2000 x 1000 x 500:
-  // 5.5 us with 128, 6.5 with 64, 6.4 with 256.)
-  const size_t room = kRoom - 1024, weights = (size_t)p.steps * kABytes;
-  int64_t least = 0;
-  for (const int rows : {16, 32, 64, 128, 192, 256}) {
-    if (rows == 16 && m > 16) continue;  // as many steps for the weights as 32
-    const int64_t items = ceil_div(m, rows) * p.channel_tiles;
-    for (int split = 1; split <= kMaxSplit; split *= 2) {
-      if (split > 1 && (items * split > sms || p.steps < 2 * split || rows == 192)) break;
-      const int64_t rounds = ceil_div(items * split, sms), steps = ceil_div(p.steps, split);
-      const bool resident = split == 1 && sms >= p.channel_tiles && weights + 4 * rows * kK <= room;
-      const int64_t bytes = rows * kK + (resident ? 0 : kABytes), step = bytes / 56 > 2 * rows ? bytes / 56 : 2 * rows;
-      const int64_t tile = steps * step > 12 * rows ? steps * step : 12 * rows;
-      const int64_t cycles = rounds * (tile + 1000) + 12 * rows + (resident ? (int64_t)weights / 56 : 0) + (split > 1 ? 2000 + 16 * rows : 0);
-      if (least != 0 && cycles >= least) continue;
-      least = cycles;
-      p.tile_rows = rows;
-      p.split = split;
-    }
+  // Rows per tile, CTAs that share them and parts of K: the choice of least cycles.
+  const size_t room = kRoom - 1024;
+  int64_t least = INT64_MAX;
+  const auto consider = [&](int rows, int ctas, int split) {
+    Plan q{};
+    q.steps = p.steps;
+    q.tile_rows = rows;
+    q.ctas = ctas;
+    q.split = split;
+    q.channel_tiles = (channel_tiles + ctas - 1) / ctas;
+    q.items = (int)(ceil_div(m, rows) * q.channel_tiles);
+    const int most = sms / (ctas * split);  // at a time
+    const int at_once = q.items < most ? q.items : most;
+    const size_t b_bytes = (size_t)rows / ctas * kK, parts = split > 1 ? (size_t)rows * kM * 4 : 0;
+    q.grid = (unsigned)(at_once * ctas * split);
+    const size_t stage = kABytes + b_bytes;
+    const int steps = (q.steps + split - 1) / split, rounds = (q.items + at_once - 1) / at_once;
+    q.accumulators = rounds > 1 ? 2 : 1;
+    q.stages = (int)((room - parts) / stage);
+    if (q.stages > kMaxStages) q.stages = kMaxStages;
+    // A step of K takes the longest of its bytes at 56 a cycle (what an SM was seen to get from L2 with all others at it; 100 where half of them
+    // have none), its MMAs, and the 2800 cycles that memory was seen to take under load shared among the stages; the results 12 cycles a row,
+    // beside the next tile's steps; a tile 1000; the exchange between the parts of K 2000 and 16 a row; a pair 100 a step and 1500.  What it chooses between, measured:
+    //   16384 x 4096 x 4096 (m x n x k): 189 us with 256 rows and a CTA, 165 with a pair; 30000 x 400 x 3000: 45 and 38
+    //   512 x 4096 x 4096: 9.8 us with 128 rows and a CTA, 10.3 with a pair, 12.4 with 192 rows, 13.5 with 64
+    //   59,000 x 128 x 256: 8.4 us with 224 rows, 8.9 with 256, 10.1 with 128; 20,000 x 128 x 256: 4.6 with 160, 4.9 with 192, 5.9 with 128
+    //   32 x 4096 x 4096: 6.0 us in four parts of K, 6.3 in two, 7.0 in one; 128 x 4096 x 4096: 7.6 in one, 8.8 in two (64 rows)
+    // (Weights kept in shared memory over a CTA's tiles made no difference of 2% anywhere.)
+    const int rate = 2 * (int)q.grid > sms ? 56 : 100, step = std::max(std::max((int)stage / rate + (ctas > 1 ? 100 : 0), 2 * rows), 2800 / q.stages);
+    const int64_t tile = std::max((int64_t)steps * step, (int64_t)12 * rows);
+    const int64_t cycles = rounds * (tile + 1000) + 12 * rows + (split > 1 ? 2000 + 16 * rows : 0) + (ctas > 1 ? 1500 : 0);
+    if (cycles >= least) return;
+    least = cycles;
+    if ((int64_t)q.stages > (int64_t)rounds * steps) q.stages = rounds * steps > 0 ? rounds * steps : 1;
+    q.tmem = 32;
+    while (q.tmem < rows) q.tmem *= 2;
+    q.parts_at = (int)(q.stages * stage);
+    while ((split << q.share_log) < rows) ++q.share_log;
+    q.smem = parts + q.stages * stage + 1024;
+    p = q;
+  };
+  const bool fine = ceil_div(m, 64) * channel_tiles > sms;
+  for (int rows = m > 16 ? 32 : 16; rows <= kMaxN; rows += fine && rows >= 64 ? 32 : rows) {  // (16 rows: as many steps for the weights as 32)
+    const int64_t items = ceil_div(m, rows) * channel_tiles;
+    const bool power = (rows & (rows - 1)) == 0;
+    consider(rows, 1, 1);
+    // (clusters do not fill the machine: 128 CTAs in clusters of 8, or 140 in clusters of 4, ran in two rounds)
+    for (int split = 2; split <= kMaxSplit && power && items * split <= sms * (split < 8 ? 7 : 6) / 8 && p.steps >= 2 * split; split *= 2) consider(rows, 1, split);
+    if (rows >= 64 && channel_tiles > 1) consider(rows, 2, 1);
     if (rows >= m) break;
   }
-  const int64_t items = ceil_div(m, p.tile_rows) * p.channel_tiles;
-  p.items = (int)items;
-  const size_t b_bytes = (size_t)p.tile_rows * kK;
-  int64_t clusters = items;
-  if (p.split == 1 && items > sms) clusters = sms;
-  if (p.split == 1 && sms >= p.channel_tiles && weights + 4 * b_bytes <= room) {
-    p.resident = 1;
-    const int64_t whole = (int64_t)sms / p.channel_tiles * p.channel_tiles;  // a CTA stays with its channels
-    if (clusters > whole) clusters = whole;
-  }
-  p.grid = (unsigned)(clusters * p.split);
-  p.tmem = 32;
-  while (p.tmem < p.tile_rows) p.tmem *= 2;
-  const size_t parts = p.split > 1 ? (size_t)p.tile_rows * kM * 4 : 0;
-  const size_t stage = b_bytes + (p.resident ? 0 : kABytes), fixed = (p.resident ? weights : 0) + parts;
-  const int64_t most = p.rounds() * ceil_div(p.steps, p.split);
-  p.stages = (int)((room - fixed) / stage);
-  if (p.stages > kMaxStages) p.stages = kMaxStages;
-  if (p.stages > most) p.stages = (int)(most > 0 ? most : 1);
-  p.parts_at = (int)(p.stages * stage);  // (never resident)
-  while ((p.split << p.share_log) < p.tile_rows) ++p.share_log;
-  p.smem = fixed + p.stages * stage + 1024;
   return p;
 }
+
+template <int CTAS>
+auto mm_kernel_of(int dtype) { return dtype == F2C_F32 ? mm_kernel<float, CTAS> : dtype == F2C_F16 ? mm_kernel<__half, CTAS> : mm_kernel<__nv_bfloat16, CTAS>; }
 
 int mm(const char* op, const Job& j, cudaStream_t st) {
   const Plan pl = plan(j.a.rows, j.b.rows, j.k, current_sm_count());
   CUtensorMap maps[2] = {};
   if (j.k > 0) {
-    const bool ok = make_map(maps, j.a.p, 1, j.a.rows, j.k, j.a.ld, pl.tile_rows) && make_map(maps + 1, j.b.p, 1, j.b.rows, j.k, j.b.ld, kM);
+    const bool ok = make_map(maps, j.a.p, 1, j.a.rows, j.k, j.a.ld, pl.tile_rows / pl.ctas) && make_map(maps + 1, j.b.p, 1, j.b.rows, j.k, j.b.ld, kM);
     F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
   }
   Params p{j.a_scales, j.b_scales, j.bias, j.out, j.a.rows, (int)j.b.rows, pl.steps, pl.channel_tiles, pl.tile_rows, pl.items,
-           pl.stages, pl.resident, pl.split, j.relu, pl.tmem, pl.rounds() > 1 ? 2 : 1, pl.parts_at, pl.share_log, j.weights_first, stream_error_word()};
-  auto* kern = j.out_dtype == F2C_F32 ? mm_kernel<float> : j.out_dtype == F2C_F16 ? mm_kernel<__half> : mm_kernel<__nv_bfloat16>;
+           pl.stages, pl.split, j.relu, pl.tmem, pl.accumulators, pl.parts_at, pl.share_log, j.weights_first, stream_error_word()};
+  auto* kern = pl.ctas == 2 ? mm_kernel_of<2>(j.out_dtype) : mm_kernel_of<1>(j.out_dtype);
   if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom)) return rc;
-  launch_dependent_cluster(kern, dim3(pl.grid), kThreads, pl.smem, (unsigned)pl.split, st, maps[0], maps[1], p);
+  launch_dependent_cluster(kern, dim3(pl.grid), kThreads, pl.smem, (unsigned)(pl.split * pl.ctas), st, maps[0], maps[1], p);
   return check_launch(op);
 }
 

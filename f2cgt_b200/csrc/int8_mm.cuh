@@ -31,20 +31,18 @@ static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 static int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }
 static bool in_place(const int8_t* p, int64_t ld, int64_t rows) { return aligned(p, 16) && (rows <= 1 || ld % 16 == 0); }
 
-
 struct Operand {
   const int8_t* p;
   int64_t ld, rows;
 };
 
-
 struct Plan {
-  int channel_tiles, tile_rows, items, steps, split, resident, stages;
+  int channel_tiles, tile_rows, items, steps, split, stages;
+  int ctas;  // that share a tile's channels: 1, or 2 with twice as many
   int parts_at, share_log;
-  int tmem;  // columns of one accumulator: a power of two
+  int tmem, accumulators;  // columns of one accumulator: a power of two; and how many, two where a CTA has more than one tile
   unsigned grid;
   size_t smem;
-  int64_t rounds() const { return ceil_div((int64_t)items * split, grid); }  // tiles of the CTA that has most
 };
 
 struct Job {

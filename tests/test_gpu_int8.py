@@ -146,6 +146,13 @@ def test_products(m, n, k, out):
     check(y, q, s, wq, ws, b if with_bias else None, relu)
 
 
+# many tiles and a long K, where pairs of CTAs share one: odd numbers of channel tiles (the last half of a pair has none), tails everywhere
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("m,n,k", [(4000, 700, 1600), (7001, 1100, 1333), (20001, 390, 1500)])
+def test_many_tiles_and_a_long_k(m, n, k, out):
+    test_products(m, n, k, out)
+
+
 def test_extreme_codes_do_not_overflow():
     for m, n in ((3, 5), (200, 130)):
         q, w = torch.full((m, 131071), -128, dtype=torch.int8), torch.full((n, 131071), -128, dtype=torch.int8)
