@@ -126,10 +126,10 @@ struct Operand {
 struct Params {
   Operand a, b;
   int m, n, steps;                 // M, N of the product; steps of K
-  int row_tiles, col_tiles, items; // row tiles along M; items of one matrix
+  int col_tiles, items;            // of one matrix
   int batch, stages;
   int chunks;                      // of 64 elements of K in a stage (of which there are `steps`)
-  int ctas;                        // that share a tile: of 128 rows each
+  int split, parts_at;             // CTAs that take parts of K, and where in shared memory they put their sums together
   int symmetric;
   const Factors* factors;          // of this step
   const __half *add_high, *add_low;  // kPoly: As; kApply, kFinal: Xs
@@ -142,7 +142,7 @@ struct Params {
 struct Bars {
   uint64_t full[kMaxStages], empty[kMaxStages], drain, acc_full[2], acc_empty[2];
   uint32_t tmem;
-  int failed;
+  int failed, lost;  // lost: of any CTA of the cluster
 };
 
 struct Maps { CUtensorMap a[2], b[2]; };  // high, low
@@ -260,15 +260,18 @@ __device__ __forceinline__ void add(uint32_t (&sum)[32], const uint32_t (&r)[32]
 }
 
 // CTAS 2: the two CTAs of a cluster work on 256 rows, each with 128 of them and half of the columns' operand in its shared memory; the
-// first one issues the MMAs for both.
-template <int MODE, typename T, int CTAS>
+// first one issues the MMAs for both.  SPLIT: the CTAs of a cluster each take a part of K, put their sums together over distributed shared
+// memory, and each has some of the columns' results to write (a kernel of its own: with both ways in one the registers spilled, 1.2 us a launch).
+template <int MODE, typename T, int CTAS, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, const __grid_constant__ Matrices s) {
   constexpr bool kWide = is_wide<T>;  // pairs by pairs: see above
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
-  const int rank = (int)blockIdx.x % CTAS, first = (int)blockIdx.x / CTAS, stride = (int)gridDim.x / CTAS;
+  const int split = SPLIT ? p.split : 1, group = CTAS * split, member = (int)blockIdx.x % group;
+  const int rank = SPLIT ? 0 : member, part = SPLIT ? member : 0, first = (int)blockIdx.x / group, stride = (int)gridDim.x / group;
+  const int step0 = p.steps * part / split, steps = p.steps * (part + 1) / split - step0;
   const int total = p.items * p.batch;
   const uint32_t a_bytes = (uint32_t)p.a.bytes(p.chunks), b_bytes = (uint32_t)p.b.bytes(p.chunks);  // of a plane of a stage
   const uint32_t b_at = a_bytes * p.a.planes, stage_bytes = b_at + b_bytes * p.b.planes;
@@ -286,10 +289,11 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kEpilogueWarps * CTAS); }
     fence_bars();
     bars.failed = 0;
+    bars.lost = 0;
   }
   fence_before();
   __syncthreads();
-  if (CTAS == 2) cluster_barrier();  // the other one's barriers are there
+  if (group > 1) cluster_barrier();  // the other ones' barriers and shared memory are there
   fence_after();
   const uint32_t tmem = bars.tmem;
   int slot = 0;
@@ -323,13 +327,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       for (int item = of_a || of_b ? first : total; item < total; item += stride) {
         const Tile t = tile_of(p, item);
         const int a_row = (t.row * CTAS + rank) * kM, b_row = t.col * columns + rank * p.b.rows;
-        for (int i = 0; i < p.steps; ++i) {
+        for (int i = 0; i < steps; ++i) {
           if (round > 0) wait_bar(bars.empty + slot, (round - 1) & 1, left);
           const bool go = mine && left != 0u;
           const uint32_t stage = smem0 + (uint32_t)slot * stage_bytes, bar = bars0 + (uint32_t)slot * 8u;
           expect_if(go && wid == 0 && rank == 0, bars.full + slot, stage_bytes * CTAS);
-          if (of_a) load(go, p.a, a_map, stage + a_at, bar, i * depth, a_row, t.z);
-          if (of_b) load(go, p.b, b_map, stage + b_from, bar, i * depth, b_row, t.z);
+          if (of_a) load(go, p.a, a_map, stage + a_at, bar, (step0 + i) * depth, a_row, t.z);
+          if (of_b) load(go, p.b, b_map, stage + b_from, bar, (step0 + i) * depth, b_row, t.z);
           if (++slot == p.stages) { slot = 0; ++round; }
         }
       }
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const uint32_t a_small = a_bytes >> 4, b_small = b_bytes >> 4;
       const int products = p.a.planes + p.b.planes - 1;
       // Waits for a step are made behind the MMAs and commits of the one before, some of which the tensor cores still have to do meanwhile.
-      const int mine_items = total > first ? (total - first + stride - 1) / stride : 0, all = mine_items * p.steps;
+      const int mine_items = total > first ? (total - first + stride - 1) / stride : 0, all = mine_items * steps;
       uint32_t n = 0;  // accumulations begun: one a tile, or (pairs) one a step
       int done_steps = 0, i = 0;
       const auto wait_full = [&]() { wait_bar(bars.full + slot, round & 1, left); };
@@ -357,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       };
       if (all > 0) wait_full();
       for (; done_steps < all; ++done_steps) {
-        const bool fresh = kWide || i == 0, last = kWide || i + 1 == p.steps, more_steps = done_steps + 1 < all;
-        if (++i == p.steps) i = 0;
+        const bool fresh = kWide || i == 0, last = kWide || i + 1 == steps, more_steps = done_steps + 1 < all;
+        if (++i == steps) i = 0;
         fence_after();
         const bool go = mine && left != 0u;
         const uint32_t at = (uint32_t)slot * (stage_bytes >> 4), acc = tmem + (n & 1u) * (uint32_t)columns;
@@ -397,6 +401,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         else arrive(bars.acc_empty + buf);
       }
     };
+    // In parts of K: 32 columns of sums to the CTA whose they are, there [this CTA][column][row]
+    const auto tell = [&](int c0, const uint32_t (&r)[32]) {
+      const int share = columns / split, owner = c0 / share;
+      const uint32_t to = peer_address(smem_u32(smem) + (uint32_t)p.parts_at + 4u * (uint32_t)((part * share + c0 - owner * share) * kM + quarter * 32 + lane), (uint32_t)owner);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) peer_store(to + (uint32_t)(j * kM) * 4u, r[j]);
+    };
+    const auto tell_lost = [&](bool lost) {
+      if (lost && lane < split) peer_store(peer_address(smem_u32(&bars.lost), (uint32_t)lane), 1u);
+    };
     uint32_t n = 0;
     dependency_wait();
     for (int item = first; item < total; item += stride) {
@@ -407,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         // the sums of the steps are added up here, where additions round
         uint32_t sum[2][32] = {};
         const int width = columns / 2, mine = half * width;
-        for (int i = 0; i < p.steps; ++i, ++n) {
+        for (int i = 0; i < steps; ++i, ++n) {
           const uint32_t turn = n >> 1, buf = n & 1u;
           wait_bar(bars.acc_full + buf, turn & 1, left);
           __syncwarp();
@@ -427,8 +441,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         for (int c = 0; c < 2; ++c) {
           const int col = col0 + mine + c * 32;
           if (c * 32 >= width || col >= p.n || (p.symmetric && col + 31 < row0)) continue;  // (wholly below the diagonal)
-          store_values<MODE, T>(p, s, f, at.z, row0, col, sum[c], lost);
+          if constexpr (SPLIT) tell(mine + c * 32, sum[c]);
+          else store_values<MODE, T>(p, s, f, at.z, row0, col, sum[c], lost);
         }
+        if constexpr (SPLIT) tell_lost(lost);
         __syncwarp();
       } else {
         const uint32_t turn = n >> 1, buf = n & 1u;
@@ -441,9 +457,11 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           uint32_t r[32];
           tmem_ld32(lanes + buf * (uint32_t)columns + (uint32_t)c0, r);
           tmem_wait(r);
-          store_values<MODE, T>(p, s, f, at.z, row0, col0 + c0, r, lost);
+          if constexpr (SPLIT) tell(c0, r);
+          else store_values<MODE, T>(p, s, f, at.z, row0, col0 + c0, r, lost);
           __syncwarp();
         }
+        if constexpr (SPLIT) tell_lost(lost);
         leave(buf);
         ++n;
       }
@@ -451,6 +469,33 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   }
   if (left == 0u) bars.failed = 1;
   __syncwarp();
+  if constexpr (SPLIT) {
+    // a cluster has one tile, whose columns its CTAs share: all sums have been told when all have got here, and are added in the order of K
+    cluster_barrier();
+    if (wid >= kFirstEpilogueWarp) {
+      const int quarter = wid & 3, half = (wid - kFirstEpilogueWarp) >> 2, share = columns / split;
+      const Tile at = tile_of(p, first);
+      const int row0 = at.row * kM + quarter * 32;
+      const Factors f = p.factors[at.z * F2C_MAX_NS_STEPS];
+      const bool lost = bars.lost != 0;
+      const float* told = reinterpret_cast<const float*>(smem + p.parts_at) + quarter * 32 + lane;
+      for (int c0 = half * 32; c0 < share; c0 += 64) {
+        const int col = at.col * columns + part * share + c0;
+        if (col >= p.n) continue;
+        uint32_t sum[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sum[j] = __float_as_uint(told[(c0 + j) * kM]);
+        for (int q = 1; q < split; ++q) {
+          uint32_t more[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) more[j] = __float_as_uint(told[(q * share + c0 + j) * kM]);
+          add(sum, more);
+        }
+        store_values<MODE, T>(p, s, f, at.z, row0, col, sum, lost);
+      }
+    }
+    __syncwarp();
+  }
   fence_before();
   __syncthreads();
   if (bars.failed && rank == 0) {
@@ -524,23 +569,27 @@ static int64_t tiles(int64_t m, int64_t n, int rows, int columns, bool symmetric
 // of which fewer stages fit).
 static int chunks_of(bool wide, int64_t p) { return wide && p > 1024 ? 2 : 1; }
 
-struct Tiling { int ctas, columns; };
+struct Tiling { int ctas, columns, split; };
 
 // The tiles of least cycles: rounds over the SMs of a tile's stages, which take the longer of their MMAs (half a cycle a column, 46 cycles at least,
-// and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of pairs to take the sums out.
+// and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of pairs to take the sums out; parts of K
+// 2500 and 8 a column, where their clusters fit the machine at once (200 x 2000 float32: 188 us in parts, 248 without; 1031 x 602: 206 and 236; 500 x 500: 181 and 197;
+// 200 x 2000 bfloat16: 148 and 166; 300 x 500 has few parts either way: 172 and 177).
 static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, int64_t p, int sms) {
   const int products = planes_a + planes_b - 1, chunks = chunks_of(wide, p);
-  Tiling best{1, 64};
+  Tiling best{1, 64, 1};
   int64_t least = 0;
-  for (const Tiling t : {Tiling{2, 256}, Tiling{2, 128}, Tiling{1, 256}, Tiling{1, 128}, Tiling{1, 64}}) {
+  for (const Tiling t : {Tiling{2, 256, 1}, Tiling{2, 128, 1}, Tiling{1, 256, 1}, Tiling{1, 128, 1}, Tiling{1, 64, 1}, Tiling{1, 128, 4}, Tiling{1, 128, 2}, Tiling{1, 64, 2}}) {
     if (wide && t.columns > kMaxSums) continue;
-    const int64_t total = tiles(m, n, kM * t.ctas, t.columns, symmetric) * batch, rounds = ceil_div(total, sms / t.ctas), steps = ceil_div(k, kK * chunks);
+    const int64_t total = tiles(m, n, kM * t.ctas, t.columns, symmetric && t.split == 1) * batch, rounds = ceil_div(total, sms / t.ctas);
+    const int64_t all = ceil_div(k, kK * chunks), steps = ceil_div(all, t.split);
+    if (t.split > 1 && (total * t.split > sms * 7 / 8 || all < 2 * t.split)) continue;
     const int64_t mma = products * chunks * 4 * (t.columns / 2 > 46 ? t.columns / 2 : 46), bytes = (int64_t)chunks * 128 * (kM * planes_a + t.columns / t.ctas * planes_b);
     int64_t step = mma > bytes / 100 ? mma : bytes / 100;
     const int64_t issue = products * chunks * 4 * 46 + (wide ? 400 : 250), taken = wide ? 250 + 3 * t.columns : 0;
     if (step < issue) step = issue;
     if (step < taken) step = taken;
-    const int64_t cycles = rounds * (steps * step + (wide ? 12 * t.columns : 0)) + 12 * t.columns;
+    const int64_t cycles = rounds * (steps * step + (wide ? 12 * t.columns : 0)) + 12 * t.columns / t.split + (t.split > 1 ? 2500 + 8 * t.columns : 0);
     if (least != 0 && cycles >= least) continue;
     least = cycles;
     best = t;
@@ -565,21 +614,21 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
   p.steps = (int)ceil_div(x.k, kK * p.chunks);
   p.batch = (int)batch;
   const Tiling shape = tiling(x.a_planes, x.b_planes, x.m, x.n, x.k, batch, x.symmetric, is_wide<T>, x.smaller, sms);
-  p.ctas = shape.ctas;
+  p.split = shape.split;
   p.a = Operand{kM, x.a_turned, x.a_planes};
   p.b = Operand{shape.columns / shape.ctas, x.b_turned, x.b_planes};
-  p.row_tiles = (int)ceil_div(x.m, kM * shape.ctas);
   p.col_tiles = (int)ceil_div(x.n, shape.columns);
   // (where all tiles are done at once, the half of them would save nothing but cost the second writing)
   p.symmetric = x.symmetric && tiles(x.m, x.n, kM * shape.ctas, shape.columns, false) * batch > sms / shape.ctas;
   p.items = (int)tiles(x.m, x.n, kM * shape.ctas, shape.columns, p.symmetric != 0);
-  const int64_t total = (int64_t)p.items * batch, places = sms / shape.ctas;
+  const int64_t total = (int64_t)p.items * batch, places = sms / (shape.ctas * shape.split);
   F2C_REQUIRE(total < (1ll << 30), F2C_ERR_LIMIT, "%s: too many tiles", op);
-  const unsigned grid = (unsigned)((total < places ? total : places) * shape.ctas);
+  const unsigned grid = (unsigned)((total < places ? total : places) * shape.ctas * shape.split);
   p.error = stream_error_word();
-  const size_t stage = (size_t)p.a.bytes(p.chunks) * p.a.planes + (size_t)p.b.bytes(p.chunks) * p.b.planes, room = kRoom - 1024;
-  p.stages = (int)(room / stage);
+  const size_t stage = (size_t)p.a.bytes(p.chunks) * p.a.planes + (size_t)p.b.bytes(p.chunks) * p.b.planes, parts = shape.split > 1 ? (size_t)shape.columns * kM * 4 : 0;
+  p.stages = (int)((kRoom - 1024 - parts) / stage);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.parts_at = (int)(p.stages * stage);
   Maps maps;
   const __half* ap[2] = {x.a.high, x.a.low};
   const __half* bp[2] = {x.b.high, x.b.low};
@@ -589,9 +638,9 @@ static int multiply(const char* op, const Product& x, Params p, const Matrices& 
     ok = ok && make_stack_map(maps.b + q, bp[q < x.b_planes ? q : 0], batch, x.b_rows, x.b_cols, 2 * x.b_ld, x.b_turned ? kK * p.chunks : p.b.rows);
   }
   F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
-  auto* kern = shape.ctas == 2 ? product_kernel<MODE, T, 2> : product_kernel<MODE, T, 1>;
+  auto* kern = shape.ctas == 2 ? product_kernel<MODE, T, 2, false> : shape.split > 1 ? product_kernel<MODE, T, 1, true> : product_kernel<MODE, T, 1, false>;
   if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom)) return rc;
-  launch_dependent_cluster(kern, dim3(grid), kThreads, p.stages * stage + 1024, (unsigned)shape.ctas, st, maps, p, s);
+  launch_dependent_cluster(kern, dim3(grid), kThreads, p.stages * stage + parts + 1024, (unsigned)(shape.ctas * shape.split), st, maps, p, s);
   return check_launch(op);
 }
 

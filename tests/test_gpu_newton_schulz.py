@@ -75,6 +75,18 @@ def test_matrices_of_few_large_singular_values(rows, cols, kind, dtype):
     near(ops.orthogonalize(g), define(g), g.dtype)
 
 
+# few tiles and a long K, of which the CTAs of a cluster take parts
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(200, 2000), (1501, 64), (1000, 1031), (33, 2999)])
+def test_long_sums(rows, cols, dtype):
+    test_against_the_formula(rows, cols, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_zero_and_not_finite_among_long_sums(dtype):
+    test_zero_and_matrices_that_are_not_finite_leave_the_others_alone(70, 1200, dtype)
+
+
 @pytest.mark.parametrize("rows,cols", [(40, 60), (128, 130), (300, 200)])
 def test_scale_does_not_matter(rows, cols):
     g = matrices(1, rows, cols, torch.float32)
