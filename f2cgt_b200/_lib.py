@@ -113,7 +113,7 @@ SIGNATURES = {
     "f2c_int8_quantize": [p, i64, i64, p, i64, i64, ci, i64, p, i64, p, p],
     "f2c_int8_mm_workspace": [p, i64, p, i64, i64, i64, i64],
     "f2c_int8_mm": [p, i64, p, p, i64, p, p, ci, p, ci, i64, i64, i64, p, i64, p],
-    "f2c_int8_linear_workspace": [i64, i64, ci, p, i64, i64, i64],
+    "f2c_int8_linear_workspace": [p, i64, i64, p, i64, i64, ci, p, i64, i64, i64],
     "f2c_int8_linear": [p, i64, i64, p, i64, i64, ci, p, i64, p, p, ci, p, ci, i64, i64, p, i64, p],
     "f2c_orthogonalize_workspace": [ci, i64, i64, i64],
     "f2c_orthogonalize": [p, p, ci, i64, i64, i64, p, ci, f32, p, i64, p],

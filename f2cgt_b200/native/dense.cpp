@@ -160,7 +160,8 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, x2, 
       const int64_t m = r.m(), cols = w.n();
       const int8_t* wp = (const int8_t*)w.w->const_data_ptr();
       out = empty({m, cols}, type, r.x1->device());
-      const int64_t bytes = f2c_int8_linear_workspace(r.k1(), r.k2(), dtype_tag(r.x1->scalar_type()), wp, row_stride(*w.w), m, cols);
+      const int64_t bytes = f2c_int8_linear_workspace(r.x1->const_data_ptr(), row_stride(*r.x1), r.k1(), r.p2(), r.ld2(), r.k2(),
+                                                      dtype_tag(r.x1->scalar_type()), wp, row_stride(*w.w), m, cols);
       at::Tensor ws;
       if (bytes > 0) ws = empty({bytes}, at::kByte, r.x1->device());
       return f2c_int8_linear(r.x1->const_data_ptr(), row_stride(*r.x1), r.k1(), r.p2(), r.ld2(), r.k2(), dtype_tag(r.x1->scalar_type()), wp,

@@ -417,8 +417,10 @@ int64_t f2c_int8_mm_workspace(const int8_t* codes, int64_t ldq, const int8_t* w,
 int f2c_int8_mm(const int8_t* codes, int64_t ldq, const float* scales, const int8_t* w, int64_t ldw, const float* w_scales,
                 const float* bias, int relu, void* out, int out_dtype, int64_t m, int64_t n, int64_t k, void* workspace,
                 int64_t workspace_bytes, void* stream);
-/* f2c_int8_quantize and f2c_int8_mm in one call; out has the dtype of the rows unless out_dtype says otherwise. */
-int64_t f2c_int8_linear_workspace(int64_t k1, int64_t k2, int dtype, const int8_t* w, int64_t ldw, int64_t m, int64_t n);
+/* f2c_int8_quantize and f2c_int8_mm in one call; dtype is the rows', out_dtype the result's.  The workspace depends on
+ * where the operands start and on their strides: ask with those of the call (256-byte aligned). */
+int64_t f2c_int8_linear_workspace(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, const int8_t* w,
+                                  int64_t ldw, int64_t m, int64_t n);
 int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int64_t ld2, int64_t k2, int dtype, const int8_t* w,
                     int64_t ldw, const float* w_scales, const float* bias, int relu, void* out, int out_dtype, int64_t m, int64_t n,
                     void* workspace, int64_t workspace_bytes, void* stream);

@@ -40,9 +40,16 @@ def test_workspaces_of_the_8_bit_products():
     assert lib.f2c_int8_mm_workspace(AT, 16, AT, 16, 100, 50, 16) == 0
     assert lib.f2c_int8_mm_workspace(AT, 17, AT, 16, 100, 50, 16) == 1792  # 1600 bytes of codes, to the next 256
     assert lib.f2c_int8_mm_workspace(AT + 4, 16, AT, 19, 100, 50, 19) == 3328 + 1792  # and 32 a row of both
-    assert lib.f2c_int8_linear_workspace(256, 0, _lib.F32, AT, 256, 1, 172) == 0
-    assert lib.f2c_int8_linear_workspace(256, 0, _lib.F32, AT, 256, 100000, 172) == 400128 + 25600000
-    assert lib.f2c_int8_linear_workspace(256, 0, _lib.F32, AT, 256, 0, 172) == 0
+    assert lib.f2c_int8_linear_workspace(AT, 256, 256, None, 0, 0, _lib.F32, AT, 256, 1, 172) == 0
+    assert lib.f2c_int8_linear_workspace(AT, 256, 256, None, 0, 0, _lib.F32, AT, 256, 100000, 172) == 400128 + 25600000
+    assert lib.f2c_int8_linear_workspace(AT, 256, 256, None, 0, 0, _lib.F32, AT, 256, 0, 172) == 0
+    # rows that cannot be encoded on the way, by their start, their stride or their length, need a place for their codes
+    codes = 4096 + 1024 * 256
+    assert lib.f2c_int8_linear_workspace(AT, 256, 256, None, 0, 0, _lib.F32, AT, 256, 1024, 172) == 0
+    assert lib.f2c_int8_linear_workspace(AT + 4, 256, 256, None, 0, 0, _lib.F32, AT, 256, 1024, 172) == codes
+    assert lib.f2c_int8_linear_workspace(AT, 257, 256, None, 0, 0, _lib.F32, AT, 256, 1024, 172) == codes
+    assert lib.f2c_int8_linear_workspace(AT, 128, 128, AT + 8, 128, 128, _lib.F32, AT, 256, 1024, 172) == codes
+    assert lib.f2c_int8_linear_workspace(AT, 254, 254, None, 0, 0, _lib.F32, AT, 256, 1024, 172) == codes
 
 
 COEFFICIENTS = (C.c_float * 15)(*[3.4445, -4.7750, 2.0315] * 5)

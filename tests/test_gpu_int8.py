@@ -8,7 +8,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from f2cgt_b200 import ops  # noqa: E402
+from f2cgt_b200 import _lib, ops  # noqa: E402
 
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 HALF_ULP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
@@ -180,6 +180,26 @@ def test_strided_and_unaligned_operands(m, n, k):
     off = lambda t: torch.cat([torch.zeros(1), t]).cuda()[1:]  # noqa: E731
     y = ops.int8_mm(torch.from_numpy(q).cuda(), off(torch.from_numpy(s)), wq.cuda(), off(ws), off(b))
     check(y, q, s, wq, ws, b, False)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 172, 256), (40, 70, 96), (1024, 172, 256), (300, 41, 602), (2000, 300, 1000)])
+def test_workspaces_are_kept_to(m, n, k):
+    lib, stream = _lib.lib, torch.cuda.current_stream().cuda_stream
+    x, (wq, ws, _) = rows(m, k, torch.float32, 4), weights(n, k)
+    q, s = define(x)
+    for lead, gap in ((0, 0), (1, 0), (0, 1), (4, 4)):
+        xs = torch.zeros(m, lead + k + gap).cuda()
+        xs[:, lead:lead + k] = x.cuda()
+        wide = torch.zeros(n, lead + k + gap, dtype=torch.int8).cuda()
+        wide[:, lead:lead + k] = wq.cuda()
+        scales, out = ws.cuda(), torch.empty(m, n).cuda()
+        xp, wp, ld = xs.data_ptr() + 4 * lead, wide.data_ptr() + lead, lead + k + gap
+        need = lib.f2c_int8_linear_workspace(xp, ld, k, None, 0, 0, _lib.F32, wp, ld, m, n)
+        space = torch.full((need + 65536,), 85, dtype=torch.uint8).cuda()
+        assert lib.f2c_int8_linear(xp, ld, k, None, 0, 0, _lib.F32, wp, ld, scales.data_ptr(), None, 0, out.data_ptr(), _lib.F32, m, n,
+                                   space.data_ptr() if need else None, need, stream) == 0
+        assert (space[need:] == 85).all()
+        check(out, q, s, wq, ws, None, False)
 
 
 def test_no_columns_no_rows():
