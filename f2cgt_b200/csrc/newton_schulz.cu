@@ -440,12 +440,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           leave(buf);
         }
         const bool lost = __any_sync(0xffffffffu, left == 0u);
-#pragma unroll
+        // (one copy of the code that stores, whose fetching from memory counts in a short launch)
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           const int col = col0 + mine + c * 32;
-          if (c * 32 >= width || col >= p.n || (p.symmetric && col + 31 < row0)) continue;  // (wholly below the diagonal)
-          if constexpr (SPLIT) tell(mine + c * 32, sum[c]);
-          else store_values<MODE, T>(p, s, f, at.z, row0, col, sum[c], lost);
+          if (c * 32 < width && col < p.n && !(p.symmetric && col + 31 < row0)) {  // (not wholly below the diagonal)
+            if constexpr (SPLIT) tell(mine + c * 32, sum[0]);
+            else store_values<MODE, T>(p, s, f, at.z, row0, col, sum[0], lost);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[0][j] = sum[1][j];
         }
         if constexpr (SPLIT) tell_lost(lost);
         __syncwarp();
