@@ -2,7 +2,7 @@
 //   X = G / (|G|_F + eps);   A = X X^T,  R = b A + c A^2,  X <- a X + R X   for every step.
 //
 // What bounds it: the tensor cores where matrices are large (4096 x 4096 bfloat16: 1.32 ms for five steps, products of 1.3 PFLOP/s; 2048 x 2048 and
-// 2048 x 8192 float32, three products for one: 2.2 ms), and the latency of 17 launches where they are not (1031 x 602 float32: 205 us).
+// 2048 x 8192 float32, three products for one: 2.3 to 2.4 ms), and the latency of 17 launches where they are not (1031 x 602 float32: 181 us).
 //
 // Products.  Three per step, on the 5th-generation tensor cores, one launch each (product_kernel).  A tile of a product has 128 rows (the
 // lanes of TMEM) and up to 256 columns.  A and A^2 are symmetric: tiles wholly below the diagonal are left out, what lies on or above it is written
@@ -232,27 +232,24 @@ __device__ __forceinline__ void store_values(const Params& p, const Matrices& s,
     scatter(out, (int64_t)p.m, count, mine, o);
   } else {
     union Half { __half h[32]; __half2 p[16]; uint4 v[4]; __device__ Half() {} };
-    Half half;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) half.p[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
     const int64_t across = stack + (int64_t)row * p.ld + col;
     const bool above = p.symmetric && col > row0 && mine;
-    const auto store = [&](__half* to) {
+    // One copy of the code for both planes: a short launch waits for its instructions to come from memory (1031 x 602 float32: 184 us, 205 with
+    // two; 1500 x 1500 bfloat16: 224 and 243; long ones 1% the other way).  The reading in one copy keeps fewer loads on the way (12 x 1024 x 1024
+    // bfloat16: 516 us, 437 so).
+#pragma unroll 1
+    for (__half* to = p.high; to != nullptr; to = to == p.high ? p.low : nullptr) {
+      Half half;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) half.p[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
       scatter(to + at, p.ld, count, mine, half.h);
       if (above) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (8 * q < count) *reinterpret_cast<uint4*>(to + across + 8 * q) = half.v[q];
       }
-    };
-    store(p.high);
-    if (p.low != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float2 f = __half22float2(half.p[j]);
-        half.p[j] = __floats2half2_rn(v[2 * j] - f.x, v[2 * j + 1] - f.y);
-      }
-      store(p.low);
+      for (int j = 0; j < 32; ++j) v[j] -= __half2float(half.h[j]);  // what the low plane has to hold
     }
   }
 }
@@ -440,7 +437,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           leave(buf);
         }
         const bool lost = __any_sync(0xffffffffu, left == 0u);
-        // (one copy of the code that stores, whose fetching from memory counts in a short launch)
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           const int col = col0 + mine + c * 32;
@@ -580,8 +576,8 @@ struct Tiling { int ctas, columns, split; };
 
 // The tiles of least cycles: rounds over the SMs of a tile's stages, which take the longer of their MMAs (half a cycle a column, 46 cycles at least,
 // and 250 for the waits) and their bytes at 100 a cycle; 12 cycles a column for the results of the last one, and of pairs to take the sums out; parts of K
-// 2500 and 8 a column, where their clusters fit the machine at once (200 x 2000 float32: 188 us in parts, 248 without; 1031 x 602: 206 and 236; 500 x 500: 181 and 197;
-// 200 x 2000 bfloat16: 148 and 166; 300 x 500 has few parts either way: 172 and 177).
+// 2500 and 8 a column, where their clusters fit the machine at once (five steps of 200 x 2000 float32 took 188 us in parts and 248 without, of 1031 x 602
+// 206 and 236, of 500 x 500 181 and 197, of 200 x 2000 bfloat16 148 and 166, before the code that stores results was made shorter).
 static Tiling tiling(const int planes_a, const int planes_b, int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric, bool wide, int64_t p, int sms) {
   const int products = planes_a + planes_b - 1, chunks = chunks_of(wide, p);
   Tiling best{1, 64, 1};
