@@ -41,7 +41,12 @@ __device__ __forceinline__ void fence_bars() { asm volatile("fence.mbarrier_init
 // descriptors and addresses in uniform registers.  (With one thread in a loop that a failed wait leaves, a wait took 180 cycles instead of 60 and an
 // MMA 60 to 90 instead of 46: more than the MMA itself up to 128 columns.)
 
-// Waits for a phase, or until `left`, the tries that a role has for all its waits, is 0: then it has given up, and later waits try once.
+// Whether a wait that has tried goes on: not with the phase complete, and not with `left`, the tries that a role has for all its waits, used up.
+// A role without tries has given up for good: later waits try once.
+__host__ __device__ __forceinline__ bool tries_again(bool done, uint32_t& left) {
+  if (done || left == 0u) return false;
+  return --left != 0u;
+}
 __device__ __forceinline__ void wait_bar(const uint64_t* bar, uint32_t parity, uint32_t& left) {
   const uint32_t at = smem_u32(bar);
   uint32_t done;
@@ -49,8 +54,7 @@ __device__ __forceinline__ void wait_bar(const uint64_t* bar, uint32_t parity, u
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(done) : "r"(at), "r"(parity), "r"(kWaitHint) : "memory");
-    left -= done ? 0u : 1u;
-  } while (!done && left != 0u);
+  } while (tries_again(done != 0u, left));
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
