@@ -20,6 +20,7 @@ struct Params {
   const float *b_scales, *bias;
   void* out;
   int n, steps, channel_tiles, tile_rows, tmem, relu;
+  uint32_t tries;  // of a role's bounded waits; 0: nothing is issued
   int* error;
 };
 
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_kernel(const __grid_consta
   const int rows = (int)min((int64_t)p.tile_rows, p.x.m - row0);
   const uint32_t b_bytes = (uint32_t)p.tile_rows * kK;
   unsigned char* codes = smem + (size_t)p.steps * kABytes;  // [step][row][128], behind the weights
-  uint32_t left = kWaitLimit;
+  uint32_t left = p.tries;
 
   if (wid == 1) alloc_tmem(&bars.tmem, (uint32_t)p.tmem);
   if (tid == 0) {
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_kernel(const __grid_consta
   dependency_wait();
   if (wid == 0) {
     // ================= weights
-    const bool mine = elected() != 0u;
+    const bool mine = elected() != 0u && left != 0u;
     release_dependents();
     for (int i = 0; i < p.steps; ++i) {
       expect_if(mine, bars.full + i, kABytes);
@@ -146,13 +147,13 @@ __global__ void __launch_bounds__(kThreads, 2) linear_kernel(const __grid_consta
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (bars.failed) {
+  if (bars.failed && p.tries != 0u) {
     // copies in flight write to shared memory, MMAs in flight read it and write TMEM: wait (bounded) for what was issued
-    left = kWaitLimit;
-    if (tid == 0) {
+    left = p.tries;
+    if (wid == 0) {
       for (int i = 0; i < p.steps; ++i) wait_bar(bars.full + i, 0, left);
-    } else if (tid == 32) {
-      commit(true, &bars.drain);
+    } else if (wid == 1) {
+      commit(elected() != 0u, &bars.drain);  // by who issued them
       wait_bar(&bars.drain, 0, left);
     }
     __syncthreads();
@@ -200,7 +201,7 @@ static cudaError_t by_output(int out_dtype, const CUtensorMap& map, const Params
 static int run(const char* op, const Rows& x, const Job& j, const Plan& pl, cudaStream_t st) {
   CUtensorMap map;
   F2C_REQUIRE(make_map(&map, j.b.p, 1, j.b.rows, j.k, j.b.ld, kM), F2C_ERR_CUDA, "%s: tensor map", op);
-  const Params p{x, j.b_scales, j.bias, j.out, (int)j.b.rows, pl.steps, pl.channel_tiles, pl.tile_rows, pl.tmem, j.relu, stream_error_word()};
+  const Params p{x, j.b_scales, j.bias, j.out, (int)j.b.rows, pl.steps, pl.channel_tiles, pl.tile_rows, pl.tmem, j.relu, j.tries, stream_error_word()};
   const size_t smem = (size_t)pl.steps * (kABytes + (size_t)pl.tile_rows * kK) + 1024;
   const cudaError_t e = x.dtype == F2C_F32   ? by_output<float>(j.out_dtype, map, p, pl.grid, smem, st)
                         : x.dtype == F2C_F16 ? by_output<__half>(j.out_dtype, map, p, pl.grid, smem, st)
@@ -243,7 +244,8 @@ extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const vo
   cudaStream_t st = (cudaStream_t)stream;
   char* ws = (char*)workspace;
   i8::Job j{};
-  j.a_scales = nullptr; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype;
+  j.a_scales = nullptr; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.out_dtype = out_dtype;
+  j.activation(relu);
   if (i8::few_encodes(r, n)) {
     j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);
     return i8::few(op, r, j, st);

@@ -35,6 +35,7 @@ struct Params {
   int tmem, accumulators;   // columns of an accumulator, and how many
   int parts_at, share_log;  // clusters: where the sums are in shared memory, and of how many rows
   int weights_first;        // the kernel before this one does not make the weights
+  uint32_t tries;           // of a role's bounded waits; 0: nothing is issued
   int* error;
 };
 
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(kThreads, CTAS == 1 ? 2 : 1) mm_kernel(const _
   const int tile_channels = kM * CTAS, b_rows = p.tile_rows / CTAS, own_channels = CTAS == 1 ? 0 : rank * kM, own_rows = CTAS == 1 ? 0 : rank * b_rows;
   const uint32_t b_bytes = (uint32_t)b_rows * kK;
   const uint32_t stage_bytes = (uint32_t)kABytes + b_bytes;
-  uint32_t left = kWaitLimit;
+  uint32_t left = p.tries;
 
   if (wid == 1) {
     if (CTAS == 2) alloc_tmem_pair(&bars.tmem, (uint32_t)p.tmem * p.accumulators);
@@ -102,8 +103,8 @@ __global__ void __launch_bounds__(kThreads, CTAS == 1 ? 2 : 1) mm_kernel(const _
     int ahead = 0;  // stages whose weights have been asked for
     if (p.weights_first) {
       for (; ahead < min(p.stages, steps); ++ahead) {
-        expect_if(mine && counts, bars.full + ahead, stage_bytes * CTAS);
-        load(mine, &w, ring + (uint32_t)ahead * stage_bytes, bars0 + 8u * (uint32_t)ahead, (step0 + ahead) * kK, first % p.channel_tiles * tile_channels + own_channels);
+        expect_if(mine && left != 0u && counts, bars.full + ahead, stage_bytes * CTAS);
+        load(mine && left != 0u, &w, ring + (uint32_t)ahead * stage_bytes, bars0 + 8u * (uint32_t)ahead, (step0 + ahead) * kK, first % p.channel_tiles * tile_channels + own_channels);
       }
       dependency_wait();
     }
@@ -226,16 +227,18 @@ __global__ void __launch_bounds__(kThreads, CTAS == 1 ? 2 : 1) mm_kernel(const _
   }
   fence_before();
   __syncthreads();
-  if (bars.failed && (CTAS == 1 || rank == 0)) {
+  if (bars.failed && p.tries != 0u && (CTAS == 1 || rank == 0)) {
     // copies in flight write to shared memory, MMAs in flight read it and write TMEM, of both CTAs of a pair: wait (bounded) for what was issued
-    left = kWaitLimit;
-    if (tid == 0) {
+    left = p.tries;
+    if (wid == 0) {
       for (int q = 0; q < p.stages; ++q) {
         const uint32_t uses = round + (q < s ? 1u : 0u);
         if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
       }
-    } else if (tid == 32) {
-      commit(true, &bars.drain);
+    } else if (wid == 1) {
+      const bool mine = elected() != 0u;  // who issued them
+      if (CTAS == 2) commit_pair(mine, &bars.drain, 1);
+      else commit(mine, &bars.drain);
       wait_bar(&bars.drain, 0, left);
     }
     __syncthreads();
@@ -346,7 +349,7 @@ int mm(const char* op, const Job& j, cudaStream_t st) {
     F2C_REQUIRE(ok, F2C_ERR_CUDA, "%s: tensor map", op);
   }
   Params p{j.a_scales, j.b_scales, j.bias, j.out, j.a.rows, (int)j.b.rows, pl.steps, pl.channel_tiles, pl.tile_rows, pl.items,
-           pl.stages, pl.split, j.relu, pl.tmem, pl.accumulators, pl.parts_at, pl.share_log, j.weights_first, stream_error_word()};
+           pl.stages, pl.split, j.relu, pl.tmem, pl.accumulators, pl.parts_at, pl.share_log, j.weights_first, j.tries, stream_error_word()};
   auto* kern = pl.ctas == 2 ? mm_kernel_of<2>(j.out_dtype) : mm_kernel_of<1>(j.out_dtype);
   if (const int rc = allow_smem(op, (const void*)kern, (int)kRoom)) return rc;
   launch_dependent_cluster(kern, dim3(pl.grid), kThreads, pl.smem, (unsigned)(pl.split * pl.ctas), st, maps[0], maps[1], p);
@@ -380,7 +383,8 @@ extern "C" int f2c_int8_mm(const int8_t* codes, int64_t ldq, const float* scales
   i8::Job j{};
   j.a = i8::readable(i8::Operand{codes, ldq, m}, k, ws, st);
   j.b = i8::readable(i8::Operand{w, ldw, n}, k, ws, st);
-  j.a_scales = scales; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.relu = relu; j.out_dtype = out_dtype;
+  j.a_scales = scales; j.b_scales = w_scales; j.bias = bias; j.out = out; j.k = k; j.out_dtype = out_dtype;
+  j.activation(relu);
   if (i8::is_few(m, n, k)) return i8::few(op, i8::Rows{j.a.p, nullptr, j.a.ld, 0, k, 0, m, F2C_I8}, j, st);
   return i8::mm(op, j, st);
 }

@@ -51,6 +51,11 @@ struct Job {
   void* out;
   int64_t k;
   int relu, out_dtype, weights_first;
+  uint32_t tries;  // of the kernels' bounded waits
+  void activation(int flags) {  // relu, or with F2C_NO_WAITS
+    relu = (flags & ~F2C_NO_WAITS) != 0;
+    tries = flags & F2C_NO_WAITS ? 0u : kWaitLimit;
+  }
 };
 
 int check(const char* op, int64_t m, int64_t n, int64_t k, int out_dtype);

@@ -139,6 +139,7 @@ struct Params {
   __half *high, *low;              // result [n][m] (kGram and kPoly: symmetric); low null: none; ld and stack also Xs'
   int64_t ld, stack;               // elements between rows, and between matrices
   float gain;                      // kFinal, optimiser: times the result
+  uint32_t tries;                  // of a role's bounded waits; 0: nothing is issued
   int* error;
 };
 
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   const uint32_t b_at = a_bytes * p.a.planes, stage_bytes = b_at + b_bytes * p.b.planes;
   const int columns = p.b.rows * CTAS;  // of a tile
   const uint32_t tmem_columns = (uint32_t)columns * 2;  // two accumulators
-  uint32_t left = kWaitLimit;
+  uint32_t left = p.tries;
 
   if (wid == 1) {
     if (CTAS == 2) alloc_tmem_pair(&bars.tmem, tmem_columns);
@@ -501,16 +502,18 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   }
   fence_before();
   __syncthreads();
-  if (bars.failed && rank == 0) {
+  if (bars.failed && p.tries != 0u && rank == 0) {
     // copies in flight write to shared memory, MMAs in flight read it and write TMEM, of both CTAs: wait (bounded) for what was issued
-    left = kWaitLimit;
-    if (tid == 0) {
+    left = p.tries;
+    if (wid == 0) {
       for (int q = 0; q < p.stages; ++q) {
         const uint32_t uses = round + (q < slot ? 1u : 0u);
         if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
       }
-    } else if (tid == 32) {
-      commit(true, &bars.drain);
+    } else if (wid == 1) {
+      const bool mine = elected() != 0u;  // who issued them
+      if (CTAS == 2) commit_pair(mine, &bars.drain, 1);
+      else commit(mine, &bars.drain);
       wait_bar(&bars.drain, 0, left);
     }
     __syncthreads();
@@ -686,6 +689,7 @@ static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps&
     Product gram{x[t & 1], x[t & 1], gram_planes, gram_planes, tall, tall, s.rows, s.cols, s.ldx(), s.rows, s.cols, s.ldx(), p, p, tall ? s.rows : s.cols, true};
     Params g{};
     g.factors = table + t;
+    g.tries = st.tries;
     g.high = poly ? a.high : r.high; g.low = poly ? a.low : r.low;
     g.ld = s.ldp(); g.stack = p * s.ldp();
     gram.smaller = p;
@@ -705,6 +709,7 @@ static int run_typed(const char* op, Matrices& src, const Shape& s, const Steps&
     apply.smaller = p;
     Params q{};
     q.factors = table + t;
+    q.tries = st.tries;
     q.gain = src.lr * (float)sqrt(s.rows > s.cols ? (double)s.rows / (double)s.cols : 1.0);
     q.add_high = x[t & 1].high; q.add_low = planes > 1 ? x[t & 1].low : nullptr;
     q.high = x[(t + 1) & 1].high; q.low = next > 1 ? x[(t + 1) & 1].low : nullptr;
@@ -728,6 +733,8 @@ static int run(const char* op, Matrices& src, int dtype, const Shape& s, const S
 // Singular values start in [0, 1].  What keeps the half-precision operands in range: no step may take one out of [0, 7.9], and R has none over 60.
 static int check(const char* op, int dtype, const float* co, int steps, float eps, Steps* st) {
   F2C_REQUIRE(is_float_dtype(dtype), F2C_ERR_UNSUPPORTED, "%s: matrices must be float32, float16 or bfloat16", op);
+  st->tries = steps & F2C_NO_WAITS ? 0u : kWaitLimit;
+  steps &= ~F2C_NO_WAITS;
   F2C_REQUIRE(steps >= 0 && steps <= F2C_MAX_NS_STEPS, F2C_ERR_LIMIT, "%s: 0 to %d steps", op, F2C_MAX_NS_STEPS);
   F2C_REQUIRE(steps == 0 || co, F2C_ERR_INVALID, "%s: null pointer", op);
   F2C_REQUIRE(eps >= 0.0f && eps <= 3.4028235e38f, F2C_ERR_INVALID, "%s: eps must not be negative", op);

@@ -24,7 +24,7 @@ static_assert(kRows * kPitch * 4 <= kBytes, "the result lies where X, A and R we
 constexpr uint32_t kGramAt = 0, kSquareAt = 128, kApplyAt = 256;     // columns of TMEM
 
 struct Shared {
-  uint64_t done;
+  uint64_t done, drain;
   uint32_t tmem;
   int failed;
   double sums[kThreads / 32];
@@ -76,11 +76,12 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
   const int rows = (int)(s.listed ? s.list[z].rows : stack_rows), cols = (int)(s.listed ? s.list[z].cols : stack_cols), size = rows * cols;
   const bool tall = rows > cols;
   const int p = tall ? cols : rows, q = tall ? rows : cols, p16 = (p + 15) / 16 * 16, q16 = (q + 15) / 16 * 16;
-  uint32_t left = kWaitLimit;
+  uint32_t left = st.tries;
 
   if (wid == 0) alloc_tmem(&sh.tmem, 512);
   if (tid == 0) {
     init_bar(&sh.done, 1);
+    init_bar(&sh.drain, 1);
     fence_bars();
     sh.failed = 0;
   }
@@ -343,10 +344,10 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
       reinterpret_cast<Few<T, V>*>(out)[(b + j) * kThreads + tid] = w[j];
     }
   }
-  if (lost && wid == 0) {  // MMAs in flight read shared memory and write TMEM: wait (bounded) for them
-    left = kWaitLimit;
-    commit(issues, &sh.done);
-    wait_bar(&sh.done, phase & 1u, left);
+  if (lost && st.tries != 0u && wid == 0) {  // MMAs in flight read shared memory and write TMEM: wait (bounded) for them
+    left = st.tries;
+    commit(issues, &sh.drain);
+    wait_bar(&sh.drain, 0, left);
     __syncwarp();
   }
   if (wid == 0) {

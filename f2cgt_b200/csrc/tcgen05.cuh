@@ -140,11 +140,11 @@ __device__ __forceinline__ void commit(bool go, const uint64_t* bar) {
                "@g tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)), "r"((uint32_t)go)
                : "memory");
 }
-// the same of the MMAs of a pair, at the barriers of both CTAs
-__device__ __forceinline__ void commit_pair(bool go, const uint64_t* bar) {
+// the same of the MMAs of a pair, at the barriers of its CTAs in `mask`
+__device__ __forceinline__ void commit_pair(bool go, const uint64_t* bar, uint16_t mask = 3) {
   asm volatile("{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t"
                "@g tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n" ::"r"(smem_u32(bar)),
-               "h"((uint16_t)3), "r"((uint32_t)go)
+               "h"(mask), "r"((uint32_t)go)
                : "memory");
 }
 
