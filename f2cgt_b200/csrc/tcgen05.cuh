@@ -41,11 +41,12 @@ __device__ __forceinline__ void fence_bars() { asm volatile("fence.mbarrier_init
 // descriptors and addresses in uniform registers.  (With one thread in a loop that a failed wait leaves, a wait took 180 cycles instead of 60 and an
 // MMA 60 to 90 instead of 46: more than the MMA itself up to 128 columns.)
 
-// Whether a wait that has tried goes on: not with the phase complete, and not with `left`, the tries that a role has for all its waits, used up.
-// A role without tries has given up for good: later waits try once.
+// Whether a wait that has tried goes on: not with the phase complete, and not with `left`, its tries, used up.  Every wait of a role has kWaitLimit of
+// them, however many waits a long product takes; a role that has none has given up for good, and later waits try once.
 __host__ __device__ __forceinline__ bool tries_again(bool done, uint32_t& left) {
-  if (done || left == 0u) return false;
-  return --left != 0u;
+  if (left == 0u) return false;
+  left = done ? kWaitLimit : left - 1u;
+  return !done && left != 0u;
 }
 __device__ __forceinline__ void wait_bar(const uint64_t* bar, uint32_t parity, uint32_t& left) {
   const uint32_t at = smem_u32(bar);

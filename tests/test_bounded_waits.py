@@ -44,3 +44,16 @@ def test_a_role_that_has_given_up_tries_once(tmp_path):
   printf("%u %llu %llu %u", kWaitLimit, first, then, left);
 """)
     assert first == limit and then == 6 and last == 0
+
+
+@pytest.mark.skipif(not os.path.exists(NVCC), reason="no CUDA compiler")
+def test_waits_that_end_leave_later_ones_their_tries(tmp_path):
+    """A hundred waits, each of which ends at its last try, and one that never does."""
+    limit, before, after, last = counts(tmp_path, """
+  uint32_t left = kWaitLimit;
+  for (int i = 0; i < 100; ++i) wait(left, kWaitLimit);
+  const uint32_t before = left;
+  const unsigned long long after = wait(left, 0);
+  printf("%u %u %llu %u", kWaitLimit, before, after, left);
+""")
+    assert before == limit and after == limit and last == 0
