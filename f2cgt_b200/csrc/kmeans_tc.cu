@@ -10,7 +10,6 @@ namespace tc {
 template <int C, int NB, bool NO_WAITS = false>
 __global__ void __launch_bounds__(kThreads, 1) kmeans_tc_kernel(const __grid_constant__ Params p) {
   dependency_wait();
-  release_dependents();
   run<C, NB, NO_WAITS>(p);
 }
 

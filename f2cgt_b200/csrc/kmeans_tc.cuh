@@ -766,6 +766,7 @@ __device__ __forceinline__ void run(const P& p) {
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (!FIT) release_dependents();  // (a fit is launched on its own)
   }
   constexpr int kStagers = 16;  // warps that stage the centres; the last of the producers prepare the A ring
   constexpr int STEPS = (N / kStagers + L::R - 1) / L::R;  // reads that make a warp's share of the centres

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 1) small_kernel(const __grid_constan
   for (int i = tid; i < kBytes / 16; i += kThreads)
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(smem + 16u * (uint32_t)i), "r"(0u) : "memory");
   dependency_wait();
-  release_dependents();
+  if (wid == 0) release_dependents();  // the warp that has allocated
 
   // ================= the norm, and X: a thread's elements stay in registers in between
   const T* const grad = s.template grad<T>(z);

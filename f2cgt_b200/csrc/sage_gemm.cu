@@ -122,7 +122,6 @@ __global__ void __launch_bounds__(kThreads, 1) sage_forward_kernel(const __grid_
                                                                    const __grid_constant__ CUtensorMap w1, const __grid_constant__ CUtensorMap w2,
                                                                    const Params p) {
   dependency_wait();
-  release_dependents();
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
   __shared__ __align__(16) float epi_s[4 * kEpiFloats];
@@ -142,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) sage_forward_kernel(const __grid_
   if (wid == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    release_dependents();
   }
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) { init_bar(bars.full + s, 1); init_bar(bars.empty + s, 1); }
