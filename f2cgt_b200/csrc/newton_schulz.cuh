@@ -41,7 +41,7 @@ struct Steps {
   float top[F2C_MAX_NS_STEPS + 1];   // no singular value is larger in front of step t, if none was larger than one at first
   float factor[F2C_MAX_NS_STEPS];    // and none is multiplied by more
   float eps;
-  uint32_t tries;                    // of a role's bounded waits; 0: no MMA or tensor copy is issued
+  uint32_t tries;                    // of a role's bounded waits; 0: no MMA or tensor copy is issued (product_kernel: and the waits run out)
 };
 
 __device__ __forceinline__ float power2(int e) { return __int_as_float((127 + min(max(e, -126), 127)) << 23); }

@@ -11,7 +11,9 @@ int* stream_error_word();
 namespace t5 {
 
 constexpr size_t kSmemLimit = 227 * 1024;
-constexpr uint32_t kWaitLimit = 1u << 20, kWaitHint = 1000;  // tries, and nanoseconds that one may take
+// Tries of a wait, and nanoseconds after which one may end; they took 4 us each (a wait that ran out after 2^20: 4.2 s).  The longest wait that can
+// end is for the sums of a tile, milliseconds.
+constexpr uint32_t kWaitLimit = 1u << 18, kWaitHint = 1000;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -41,21 +43,22 @@ __device__ __forceinline__ void fence_bars() { asm volatile("fence.mbarrier_init
 // descriptors and addresses in uniform registers.  (With one thread in a loop that a failed wait leaves, a wait took 180 cycles instead of 60 and an
 // MMA 60 to 90 instead of 46: more than the MMA itself up to 128 columns.)
 
-// Whether a wait that has tried goes on: not with the phase complete, and not with `left`, its tries, used up.  Every wait of a role has kWaitLimit of
-// them, however many waits a long product takes; a role that has none has given up for good, and later waits try once.
-__host__ __device__ __forceinline__ bool tries_again(bool done, uint32_t& left) {
-  if (left == 0u) return false;
-  left = done ? kWaitLimit : left - 1u;
-  return !done && left != 0u;
+// Whether a wait that has tried goes on: not with the phase complete, and not with kWaitLimit tries `spent` (a number of the wait's own, however many
+// waits a long product takes).  One that runs out leaves `left` 0: the role has given up for good, and later waits try once.
+__host__ __device__ __forceinline__ bool tries_again(bool done, uint32_t& spent, uint32_t& left) {
+  if (done || left == 0u) return false;
+  if (++spent < kWaitLimit) return true;
+  left = 0u;
+  return false;
 }
 __device__ __forceinline__ void wait_bar(const uint64_t* bar, uint32_t parity, uint32_t& left) {
   const uint32_t at = smem_u32(bar);
-  uint32_t done;
+  uint32_t done, spent = 0;
   do {
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(done) : "r"(at), "r"(parity), "r"(kWaitHint) : "memory");
-  } while (tries_again(done != 0u, left));
+  } while (tries_again(done != 0u, spent, left));
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }

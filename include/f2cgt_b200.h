@@ -45,7 +45,8 @@ typedef enum { F2C_L2 = 0, F2C_COSINE = 1 } f2c_metric;  /* src/kmeans.cu:16-22,
  * without one the library picks by shape.  Both give the same labels. */
 #define F2C_SCORER_EXACT 0x100   /* fp32 FMA scorer */
 #define F2C_SCORER_TENSOR 0x200  /* tcgen05 scorer + exact re-score of undecided points (needs a workspace) */
-/* For tests of what follows a bounded wait that has run out: all those of the call's tensor-core kernels run out at once.
+/* For tests of what follows a bounded wait that has run out: all those of the call's tensor-core kernels run out, at once or (Newton-Schulz
+ * products of matrices that one SM does not hold) after about a second.
  * f2c_kmeans_assign and f2c_kmeans_fit_iterate (in `metric`): same results.  f2c_int8_mm and f2c_int8_linear (in `relu`),
  * f2c_orthogonalize and f2c_muon_step (in `steps`): results of NaN and a device status, where such kernels are used. */
 #define F2C_NO_WAITS 0x400

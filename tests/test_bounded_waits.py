@@ -15,7 +15,8 @@ using namespace f2c::t5;
 // tries of a wait whose phase completes with number `when` (0: never)
 static unsigned long long wait(uint32_t& left, unsigned long long when) {
   unsigned long long n = 0;
-  do ++n; while (n < (1ull << 25) && tries_again(n == when, left));
+  uint32_t spent = 0;
+  do ++n; while (n < (1ull << 25) && tries_again(n == when, spent, left));
   return n;
 }
 int main() {

@@ -1,5 +1,6 @@
-"""GPU: what the dense operators leave behind a bounded wait that has run out.  ``F2C_NO_WAITS`` makes all of a call's run out at once, before
-anything is issued: results are NaN, the device status has the kernel's code, and the next ordinary call has the bits of the one before."""
+"""GPU: what the dense operators leave behind a bounded wait that has run out.  With ``F2C_NO_WAITS`` nothing is issued that a wait could be for,
+and all run out (at once, or those of a product of matrices that one SM does not hold after their full limit): results are NaN, the device
+status has the kernel's code, and the next ordinary call has the bits of the one before."""
 import ctypes
 
 import pytest
@@ -63,7 +64,7 @@ def test_8_bit_layers(m, n, k, code, dtype):
 
 
 # one CTA a matrix; a CTA a tile, parts of K, pairs of CTAs with half of the symmetric products
-@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("batch,rows,cols,code", [(3, 100, 128, 6), (2, 128, 200, 6), (1, 300, 400, 5), (1, 1031, 602, 5), (6, 520, 700, 5), (2, 1500, 1100, 5)])
 def test_orthogonalised_matrices(batch, rows, cols, code, dtype):
     g = torch.randn(batch, rows, cols, generator=torch.Generator(device="cuda").manual_seed(rows), device="cuda").to(dtype)
@@ -72,7 +73,7 @@ def test_orthogonalised_matrices(batch, rows, cols, code, dtype):
     out = torch.zeros_like(g)
     need = lib.f2c_orthogonalize_workspace(TAGS[dtype], batch, rows, cols)
     space = torch.zeros(max(need, 1), dtype=torch.uint8, device="cuda")
-    for steps in (1, 3):
+    for steps in (1, 3) if code == 6 else (1,):
         out.zero_()
         check(lib.f2c_orthogonalize(g.data_ptr(), out.data_ptr(), TAGS[dtype], batch, rows, cols, COEFFICIENTS, steps | _lib.NO_WAITS, 1e-7,
                                     space.data_ptr() if need else None, need, stream()))
@@ -90,6 +91,6 @@ def test_weights_of_an_optimiser_step(rows, cols, code):
     one = (_lib.MuonMatrix * 1)(_lib.MuonMatrix(w.data_ptr(), g.data_ptr(), momentum.data_ptr(), rows, cols))
     need = lib.f2c_muon_workspace(one, 1, _lib.F32)
     space = torch.zeros(max(need, 1), dtype=torch.uint8, device="cuda")
-    check(lib.f2c_muon_step(one, 1, _lib.F32, 0.02, 0.95, 1, 0.0, COEFFICIENTS, 5 | _lib.NO_WAITS, 1e-7, space.data_ptr() if need else None, need, stream()))
+    check(lib.f2c_muon_step(one, 1, _lib.F32, 0.02, 0.95, 1, 0.0, COEFFICIENTS, 1 | _lib.NO_WAITS, 1e-7, space.data_ptr() if need else None, need, stream()))
     lost(w, code)
     assert torch.equal(momentum, g)
