@@ -63,7 +63,7 @@ struct Weights {
   const float* b() const { return bias != nullptr ? bias->const_data_ptr<float>() : nullptr; }
 };
 
-Weights weights(PyObject* w, PyObject* s, PyObject* b, const at::Tensor& x, int64_t k) {
+Weights weights(PyObject* w, PyObject* s, PyObject* b, const at::Tensor& x, int64_t k, const char* op) {
   Weights r;
   r.w = &matrix(w, "w_codes", bit(F2C_I8));
   r.scales = &tensor(s, "w_scales", kF32);
@@ -71,10 +71,12 @@ Weights weights(PyObject* w, PyObject* s, PyObject* b, const at::Tensor& x, int6
   if (r.scales->dim() != 1 || r.scales->size(0) != r.n()) fail(PyExc_RuntimeError, "w_scales must be [n]");
   same_device(*r.w, x, "w_codes");
   same_device(*r.scales, x, "w_scales");
+  no_gradient(*r.scales, op, "w_scales");
   if (b != Py_None) {
     r.bias = &tensor(b, "bias", kF32);
     if (r.bias->dim() != 1 || r.bias->size(0) != r.n()) fail(PyExc_RuntimeError, "bias must be [n]");
     same_device(*r.bias, x, "bias");
+    no_gradient(*r.bias, op, "bias");
   }
   return r;
 }
@@ -128,7 +130,8 @@ PyObject* int8_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {  // codes, scal
     const at::Tensor& s = tensor(a[1], "scales", kF32);
     if (s.dim() != 1 || s.size(0) != q.size(0)) fail(PyExc_RuntimeError, "scales must be [m]");
     same_device(s, q, "scales");
-    const Weights w = weights(a[2], a[3], a[4], q, q.size(1));
+    no_gradient(s, "int8_mm", "scales");
+    const Weights w = weights(a[2], a[3], a[4], q, q.size(1), "int8_mm");
     const bool relu = truth(a[5]);
     const at::ScalarType type = float_type(a[6], at::kFloat);
     at::Tensor out;
@@ -151,7 +154,7 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, x2, 
   return guarded([&]() -> PyObject* {
     arguments("int8_linear", n, 7);
     const Rows r = rows(a[0], a[1], "int8_linear");
-    const Weights w = weights(a[2], a[3], a[4], *r.x1, r.k1() + r.k2());
+    const Weights w = weights(a[2], a[3], a[4], *r.x1, r.k1() + r.k2(), "int8_linear");
     const bool relu = truth(a[5]);
     const at::ScalarType type = float_type(a[6], r.x1->scalar_type());
     at::Tensor out;
@@ -255,7 +258,7 @@ PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (first == nullptr) first = &w;
       const at::Tensor& g = tensor(PySequence_Fast_GET_ITEM(seq[1].o, i), "grads", bit(dtype_tag(w.scalar_type())));
       const at::Tensor& m = tensor(PySequence_Fast_GET_ITEM(seq[2].o, i), "momenta", kF32);
-      no_gradient(w, "muon_step", "a weight");
+      no_gradient(w, "muon_step", "a weight"); no_gradient(g, "muon_step", "a gradient"); no_gradient(m, "muon_step", "a momentum");
       if (w.scalar_type() != first->scalar_type()) fail(PyExc_RuntimeError, "weights must have one dtype");
       if (w.dim() != 2 || g.sizes() != w.sizes() || m.sizes() != w.sizes()) fail(PyExc_RuntimeError, "weights, grads and momenta must be matrices of one shape");
       same_device(w, *first, "a weight"); same_device(g, *first, "a gradient"); same_device(m, *first, "a momentum");
