@@ -3,6 +3,7 @@
 
 #include <vector>
 
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/grad_mode.h>
 
 namespace f2c_native {
@@ -31,6 +32,8 @@ void same_device(const at::Tensor& t, const at::Tensor& other, const char* name)
 void no_gradient(const at::Tensor& t, const char* op, const char* name) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     fail(PyExc_RuntimeError, "%s has no gradient: %s requires one (detach it, or call under torch.no_grad())", op, name);
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    fail(PyExc_RuntimeError, "%s has no forward-mode derivative: %s has a tangent", op, name);
 }
 
 struct Rows {

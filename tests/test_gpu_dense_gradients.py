@@ -32,3 +32,18 @@ def test_inputs_that_require_a_gradient(which, name):
         call(**asking)
     with torch.no_grad():
         call(**asking)
+
+
+@pytest.mark.parametrize("which,name", INPUTS)
+def test_inputs_with_a_tangent(which, name):
+    from torch.autograd import forward_ad
+    op, inputs, call = calls()[which]
+    with forward_ad.dual_level():
+        call(**inputs)
+        dual = dict(inputs, **{name: forward_ad.make_dual(inputs[name], torch.ones_like(inputs[name]))})
+        with pytest.raises(RuntimeError, match=f"{op} has no forward-mode derivative"):
+            call(**dual)
+        with torch.no_grad(), pytest.raises(RuntimeError):  # which leaves that mode alone
+            call(**dual)
+        with forward_ad._set_fwd_grad_enabled(False):
+            call(**dual)
