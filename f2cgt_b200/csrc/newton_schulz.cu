@@ -23,6 +23,9 @@
 //    2e-4 without the taking out.)
 #include <math.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "newton_schulz.cuh"
 
 namespace f2c {
@@ -811,6 +814,30 @@ static bool group_of(const f2c_muon_matrix* list, int count, int i, ns::Matrices
   return true;
 }
 
+// Whether anything of the list that is written shares memory with anything else of it: the matrices of a launch are worked on at the same time.
+static bool overlaps(const f2c_muon_matrix* list, int count, int dtype) {
+  struct Range { uintptr_t from, to; bool written; };
+  std::vector<Range> all;
+  all.reserve(3 * (size_t)count);
+  for (int i = 0; i < count; ++i) {
+    const f2c_muon_matrix& m = list[i];
+    const uintptr_t size = (uintptr_t)m.rows * (uintptr_t)m.cols;
+    if (size == 0) continue;
+    const auto put = [&](const void* p, size_t item, bool written) { all.push_back(Range{(uintptr_t)p, (uintptr_t)p + size * item, written}); };
+    put(m.weight, dtype_size(dtype), true);
+    put(m.grad, dtype_size(dtype), false);
+    put(m.momentum, 4, true);
+  }
+  std::sort(all.begin(), all.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+  uintptr_t end = 0, written_end = 0;  // of those that begin before
+  for (const Range& r : all) {
+    if (r.from < (r.written ? end : written_end)) return true;
+    end = std::max(end, r.to);
+    if (r.written) written_end = std::max(written_end, r.to);
+  }
+  return false;
+}
+
 extern "C" int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int count, int dtype) {
   int64_t most = 0;
   ns::Matrices src{};
@@ -832,6 +859,11 @@ extern "C" int f2c_muon_step(const f2c_muon_matrix* list_host, int count, int dt
     const f2c_muon_matrix& m = list_host[i];
     if (const int rc = ns::check_shape(op, ns::Shape{1, m.rows, m.cols})) return rc;
     F2C_REQUIRE(m.rows == 0 || m.cols == 0 || (m.weight && m.grad && m.momentum), F2C_ERR_INVALID, "%s: null pointer", op);
+  }
+  try {
+    F2C_REQUIRE(!overlaps(list_host, count, dtype), F2C_ERR_INVALID, "%s: a weight or momentum shares memory with another tensor of the step", op);
+  } catch (...) {
+    return set_error(F2C_ERR_LIMIT, "%s: no host memory for a list of %d matrices", op, count);
   }
   const int64_t need = f2c_muon_workspace(list_host, count, dtype);
   F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,

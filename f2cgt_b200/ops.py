@@ -361,7 +361,8 @@ def orthogonalize(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, out=None):
 def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """One step of Muon (momentum, orthogonalised update) over lists of matrices, in place: ``m <- momentum m + g``,
     ``u = g + momentum m`` (``nesterov``) or ``m``, ``w <- w (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u)``.
-    Weights and gradients float32 / float16 / bfloat16 (one dtype), momenta float32; call under ``torch.no_grad()``."""
+    Weights and gradients float32 / float16 / bfloat16 (one dtype), momenta float32; call under ``torch.no_grad()``.  A weight or a momentum
+    must not share memory with another tensor of the lists (a weight listed twice is refused)."""
     _native.muon_step(weights, grads, momenta, lr, momentum, nesterov, weight_decay, steps, coefficients, eps)
 
 

@@ -435,7 +435,7 @@ int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int
  * f2c_orthogonalize: g and out [batch, rows, cols], dtype F32, F16 or BF16; out may be g.
  * f2c_muon_step: for every matrix of the list  m <- momentum m + g;  u = nesterov ? g + momentum m : m;
  *   w <- w (1 - lr decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u),  in place; w and g of `dtype` (F32, F16 or BF16), m float.
- *   The list (host memory) is read during the call.  Matrices of one step must not overlap.
+ *   The list (host memory) is read during the call.  Refused: a weight or momentum that shares memory with another tensor of the list.
  * workspace: the bytes that the _workspace function names, 256-byte aligned. */
 typedef struct {
   void* weight;

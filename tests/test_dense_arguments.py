@@ -91,3 +91,22 @@ def test_workspaces_of_the_updates():
     large = _lib.MuonMatrix(AT, AT, AT, 300, 400)
     assert lib.f2c_muon_workspace((_lib.MuonMatrix * 2)(small, small), 2, _lib.F32) == 0
     assert lib.f2c_muon_workspace((_lib.MuonMatrix * 3)(large, small, large), 3, _lib.F32) == two
+
+
+A, B, G, M = (0x1000000 * i for i in range(1, 5))  # 300 x 300 float32 are 360,000 bytes
+
+
+@pytest.mark.parametrize("list_", [
+    [(A, G, M, 300, 300), (A, G + 400_000, M + 400_000, 300, 300)], [(A, G, M, 300, 300), (B, G, M, 300, 300)], [(A, A, M, 300, 300)], [(A, G, A, 300, 300)],
+    [(A, G, G, 300, 300)], [(A, G, M, 300, 300), (A + 359_996, G, M + 400_000, 300, 300)], [(A, G, M, 300, 300), (B, A + 4, M + 400_000, 20, 20)],
+    [(A, G, M, 1, 1), (B, G, M, 1, 1)], [(A, G, M, 300, 300), (B, M + 100, M + 400_000, 20, 20)], [(B, G, M, 20, 20), (A, G, B - 16, 20, 20)]])
+def test_matrices_of_a_step_that_share_memory_are_refused(list_):
+    assert step(list_) == INVALID and b"shares memory" in lib.f2c_last_error()
+
+
+@pytest.mark.parametrize("list_", [
+    [(A, G, M, 300, 300), (A + 360_000, G + 360_000, M + 360_000, 300, 300)], [(A, G, M, 300, 300), (B, G, M + 360_000, 300, 300)],
+    [(A, G, M, 300, 300), (B, G + 100, M + 360_000, 20, 20)], [(A, A, A, 0, 300), (B, B, B, 300, 0)]])
+def test_neighbours_and_shared_gradients_are_not(list_):
+    assert step(list_, work=0) == (0 if 0 in list_[0] else INVALID)
+    assert 0 in list_[0] or b"workspace" in lib.f2c_last_error()
