@@ -787,6 +787,8 @@ extern "C" int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t ba
   if (const int rc = ns::check(op, dtype, coefficients_host, steps, eps, &st)) return rc;
   if (batch == 0 || rows == 0 || cols == 0) return F2C_OK;
   F2C_REQUIRE(g && out, F2C_ERR_INVALID, "%s: null pointer", op);
+  const uintptr_t from = (uintptr_t)g, to = (uintptr_t)out, bytes = (uintptr_t)batch * (uintptr_t)rows * (uintptr_t)cols * dtype_size(dtype);
+  F2C_REQUIRE(from == to || from + bytes <= to || to + bytes <= from, F2C_ERR_INVALID, "%s: out shares a part of g's memory", op);
   const int64_t need = f2c_orthogonalize_workspace(dtype, batch, rows, cols);
   F2C_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), F2C_ERR_INVALID,
               "%s: workspace too small or not 256-byte aligned", op);

@@ -353,7 +353,7 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # quintic of Jordan et al., Muon (202
 def orthogonalize(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, out=None):
     """Newton-Schulz steps on every matrix of ``g`` [..., rows, cols] (float32 / float16 / bfloat16, contiguous): from
     ``X = G / (|G| + eps)``, ``X <- (a I + b A + c A^2) X`` with ``A = X X^T`` - singular values go to one, singular vectors stay.
-    ``coefficients``: (a, b, c), or one such triple for every step.  ``out`` may be ``g``.  Sums and norms are held in 32 bits or
+    ``coefficients``: (a, b, c), or one such triple for every step.  ``out`` may be ``g``, or share no memory with it.  Sums and norms are held in 32 bits or
     more, float32 and float16 matrices to about 22 bits throughout, bfloat16 ones to 11 or more."""
     return _native.orthogonalize(g, steps, coefficients, eps, out)
 

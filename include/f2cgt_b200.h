@@ -432,7 +432,7 @@ int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const void* x2, int
  * (for more rows than columns the transposed matrix is meant).  coefficients_host: 3 * steps floats.  Refused are coefficients under
  * which a singular value s could leave [0, 7.9], or b s^2 + c s^4 exceed 60: values are held in half
  * precision (pairs of it where more is needed).  Matrices that hold a NaN or an infinity become NaN.
- * f2c_orthogonalize: g and out [batch, rows, cols], dtype F32, F16 or BF16; out may be g.
+ * f2c_orthogonalize: g and out [batch, rows, cols], dtype F32, F16 or BF16; out may be g, or share nothing with it.
  * f2c_muon_step: for every matrix of the list  m <- momentum m + g;  u = nesterov ? g + momentum m : m;
  *   w <- w (1 - lr decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u),  in place; w and g of `dtype` (F32, F16 or BF16), m float.
  *   The list (host memory) is read during the call.  Refused: a weight or momentum that shares memory with another tensor of the list.

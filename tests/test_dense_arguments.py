@@ -110,3 +110,17 @@ def test_matrices_of_a_step_that_share_memory_are_refused(list_):
 def test_neighbours_and_shared_gradients_are_not(list_):
     assert step(list_, work=0) == (0 if 0 in list_[0] else INVALID)
     assert 0 in list_[0] or b"workspace" in lib.f2c_last_error()
+
+
+@pytest.mark.parametrize("rows,cols", [(30, 50), (300, 300)])
+@pytest.mark.parametrize("dtype,item", [(_lib.F32, 4), (_lib.BF16, 2)])
+def test_results_that_share_a_part_of_the_matrices_are_refused(rows, cols, dtype, item):
+    size = 2 * rows * cols * item
+    for at in (item, size // 2, size - item):
+        for g, out in ((A, A + at), (A + at, A)):
+            assert orthogonalize(dtype=dtype, batch=2, rows=rows, cols=cols, g=g, out=out) == INVALID
+            assert b"memory" in lib.f2c_last_error()
+    if rows == 300:  # (goes on to what is refused next)
+        for g, out in ((A, A), (A, A + size), (A + size, A)):
+            assert orthogonalize(dtype=dtype, batch=2, rows=rows, cols=cols, g=g, out=out, work=0) == INVALID
+            assert b"workspace" in lib.f2c_last_error()

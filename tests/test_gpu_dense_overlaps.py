@@ -23,3 +23,18 @@ def test_matrices_of_a_step(shape):
     views = [[f[:size].view(shape), f[size:].view(shape)] for f in flat]
     ops.muon_step(*views, 0.1)
     assert torch.equal(views[0][0], w) and torch.equal(views[0][1], v) and torch.equal(views[2][0], m) and torch.equal(views[2][1], n)
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 96), (300, 200)])
+def test_results_of_matrices(rows, cols):
+    stack = torch.randn(4, rows, cols, device="cuda")
+    kept = stack.clone()
+    want = ops.orthogonalize(stack)
+    for g, out in ((stack[:3], stack[1:]), (stack[1:], stack[:3]), (stack[0], stack.view(-1)[4:4 + rows * cols].view(rows, cols))):
+        with pytest.raises(RuntimeError, match="memory"):
+            ops.orthogonalize(g, out=out)
+    assert torch.equal(stack, kept)
+    ops.orthogonalize(stack[:2], out=stack[2:])
+    assert torch.equal(stack[2:], want[:2]) and torch.equal(stack[:2], kept[:2])
+    ops.orthogonalize(stack[:2], out=stack[:2])
+    assert torch.equal(stack[:2], want[:2])
