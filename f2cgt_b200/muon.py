@@ -10,7 +10,8 @@ from . import ops
 
 class Muon:
     """``params``: parameters on one device; matrices (float32, float16 or bfloat16) are orthogonalised, the others (float32) go to Adam with
-    ``adam_lr``.  ``lr`` times ``sqrt(max(1, rows / cols))`` is the size of an update's singular values.  Momenta are float32.
+    ``adam_lr``, which moves with ``lr`` (a schedule sets ``lr`` alone; of ``lr=0`` there is no ratio to keep, and Adam's rate stays ``adam_lr``).
+    ``lr`` times ``sqrt(max(1, rows / cols))`` is the size of an update's singular values.  Momenta are float32.
     Matrices without a gradient are left alone."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=ops.NEWTON_SCHULZ, eps=1e-7,
@@ -26,7 +27,7 @@ class Muon:
         self.steps, self.coefficients, self.eps = int(steps), coefficients, float(eps)
         others = [p for p in params if p.dim() != 2]
         self.adam = DirectFusedAdam(others, lr=adam_lr) if others else None
-        self._lr, self._adam_ratio = float(lr), float(adam_lr) / float(lr) if lr else 0.0
+        self._lr, self._adam_ratio = float(lr), float(adam_lr) / float(lr) if lr else None
 
     @property
     def lr(self):
@@ -35,7 +36,7 @@ class Muon:
     @lr.setter
     def lr(self, value):  # a schedule moves both learning rates
         self._lr = float(value)
-        if self.adam is not None:
+        if self.adam is not None and self._adam_ratio is not None:
             self.adam.lr = self._lr * self._adam_ratio
 
     def zero_grad(self, set_to_none=True):

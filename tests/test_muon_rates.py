@@ -1,0 +1,37 @@
+"""CPU: the learning rates of Muon, on parameters that are no matrices (which Adam updates)."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+def muon(**kw):
+    from f2cgt_b200.muon import Muon
+    return Muon([torch.zeros(3, requires_grad=True)], **kw)
+
+
+def moved(optimizer):
+    """what one step changes a parameter by, of gradients of one: Adam's rate"""
+    p = optimizer.adam.params[0]
+    before = p.detach().clone()
+    p.grad = torch.ones_like(p)
+    optimizer.step()
+    return float((before - p.detach()).max())
+
+
+def test_adam_s_rate_moves_with_the_rate():
+    o = muon(lr=0.02, adam_lr=0.004)
+    assert moved(o) == pytest.approx(0.004, rel=1e-5)
+    o.lr = 0.01
+    assert moved(o) == pytest.approx(0.002, rel=1e-4)
+    o.lr = 0.0
+    assert moved(o) == 0.0
+    o.lr = 0.02
+    assert moved(o) == pytest.approx(0.004, rel=1e-4)
+
+
+def test_a_rate_of_zero_at_first_leaves_adam_s_alone():
+    o = muon(lr=0.0, adam_lr=0.004)
+    assert moved(o) == pytest.approx(0.004, rel=1e-5)
+    for lr in (0.001, 0.01, 0.02):
+        o.lr = lr
+        assert o.lr == lr and moved(o) == pytest.approx(0.004, rel=1e-4)
