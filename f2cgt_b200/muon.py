@@ -65,7 +65,7 @@ class Muon:
     def state_dict(self):
         state = dict(lr=self._lr, momenta=self.momenta)
         if self.adam is not None:
-            state.update(exp_avg=self.adam.exp_avg, exp_avg_sq=self.adam.exp_avg_sq, adam_steps=self.adam.steps[0])
+            state.update(adam_lr=self.adam.lr, adam_ratio=self._adam_ratio, exp_avg=self.adam.exp_avg, exp_avg_sq=self.adam.exp_avg_sq, adam_steps=self.adam.steps[0])
         return state
 
     def load_state_dict(self, state):
@@ -81,3 +81,5 @@ class Muon:
         for mine, given in pairs:
             mine.copy_(given)
         self.lr = state["lr"]
+        if self.adam is not None and "adam_lr" in state:  # (states of before have no rate of Adam's)
+            self.adam.lr, self._adam_ratio = float(state["adam_lr"]), state["adam_ratio"]

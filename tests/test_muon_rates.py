@@ -35,3 +35,23 @@ def test_a_rate_of_zero_at_first_leaves_adam_s_alone():
     for lr in (0.001, 0.01, 0.02):
         o.lr = lr
         assert o.lr == lr and moved(o) == pytest.approx(0.004, rel=1e-4)
+
+
+@pytest.mark.parametrize("first,then", [((0.02, 0.004), (0.5, 0.3)), ((0.02, 0.004), (0.0, 0.3)), ((0.0, 0.004), (0.5, 0.3))])
+def test_a_state_goes_on_with_its_own_rates(first, then):
+    """in an optimiser that was built with others"""
+    a, b = (muon(lr=lr, adam_lr=adam_lr) for lr, adam_lr in (first, then))
+    a.lr = 0.01
+    moved(a)
+    b.load_state_dict(a.state_dict())
+    assert b.lr == 0.01 and b.adam.lr == a.adam.lr
+    for lr in (0.01, 0.03, 0.0, 0.02):
+        a.lr = b.lr = lr
+        assert b.adam.lr == a.adam.lr and moved(b) == pytest.approx(moved(a), rel=1e-5)
+
+
+def test_a_state_without_adam_s_rate_is_taken():
+    a, b = muon(lr=0.02, adam_lr=0.004), muon(lr=0.01, adam_lr=0.004)
+    state = {k: v for k, v in a.state_dict().items() if k not in ("adam_lr", "adam_ratio")}
+    b.load_state_dict(state)
+    assert b.lr == 0.02 and b.adam.lr == pytest.approx(0.008)
