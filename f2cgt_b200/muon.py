@@ -8,6 +8,15 @@ import torch
 from . import ops
 
 
+def _adam_step(adam):
+    """``DirectFusedAdam.step`` for a torch that does not expose the fused kernel."""
+    (beta1, beta2), count = adam.betas, adam.steps[0].add_(1)
+    for p, m, v in zip(adam.params, adam.exp_avg, adam.exp_avg_sq):
+        m.lerp_(p.grad, 1 - beta1)
+        v.mul_(beta2).addcmul_(p.grad, p.grad, value=1 - beta2)
+        p.sub_(m / (1 - beta1 ** count) * adam.lr / ((v / (1 - beta2 ** count)).sqrt() + adam.eps))
+
+
 class Muon:
     """``params``: parameters on one device; matrices (float32, float16 or bfloat16) are orthogonalised, the others (float32) go to Adam with
     ``adam_lr``, which moves with ``lr`` (a schedule sets ``lr`` alone; of ``lr=0`` there is no ratio to keep, and Adam's rate stays ``adam_lr``).
@@ -60,7 +69,10 @@ class Muon:
         if self.adam is not None and any(p.grad is not None for p in self.adam.params):
             if any(p.grad is None for p in self.adam.params):
                 raise RuntimeError("Muon: the parameters that are no matrices are updated together: one of them has no gradient")
-            self.adam.step()
+            if self.adam.available():
+                self.adam.step()
+            else:
+                _adam_step(self.adam)
 
     def state_dict(self):
         state = dict(lr=self._lr, momenta=self.momenta)

@@ -55,3 +55,21 @@ def test_a_state_without_adam_s_rate_is_taken():
     state = {k: v for k, v in a.state_dict().items() if k not in ("adam_lr", "adam_ratio")}
     b.load_state_dict(state)
     assert b.lr == 0.02 and b.adam.lr == pytest.approx(0.008)
+
+
+def test_a_torch_without_the_fused_kernel(monkeypatch):
+    """The same updates, to the rounding of a step of 0.004 on values of one: 10 steps, 2^-23 of one each and of the steps themselves."""
+    def run():
+        g = torch.Generator().manual_seed(0)
+        o = muon(lr=0.02, adam_lr=0.004)
+        p = o.adam.params[0]
+        with torch.no_grad():
+            p.copy_(torch.rand(3, generator=g))
+        for _ in range(10):
+            p.grad = torch.randn(3, generator=g)
+            o.step()
+        return p.detach().clone()
+
+    want = run()
+    monkeypatch.delattr(torch, "_fused_adam_")
+    assert float((run() - want).abs().max()) <= 20 * 2.0 ** -23
