@@ -2,9 +2,9 @@
 //
 // A CTA has 16 rows and 16 to 128 channels; its eight warps share out channels (16 each) and parts of K, whose sums they add in shared
 // memory.  A lane reads 16 neighbouring columns of a channel straight into registers, so that all of a warp's weights are on their way at
-// once and, where the kernel before cannot have made them, before that has ended.  The rows' codes are put into shared memory, or made
-// there: then a warp has two rows, finds their largest magnitudes and encodes them.  The sums are four-element dot products, 256 products a
-// cycle and SM; the warp-wide 8-bit MMA has about 25 here (16 x 4096 x 4096: 17.7 us with it).  What bounds it is latency: launch, loads, sums (1 x 172 x 256: 2.8 us).
+// once.  The rows' codes are put into shared memory, or made there: then a warp has two rows, finds their largest magnitudes and encodes them.
+// The sums are four-element dot products, 256 products a cycle and SM; the warp-wide 8-bit MMA has about 25 here (16 x 4096 x 4096: 17.7 us with
+// it).  What bounds it is latency: launch, loads, sums (1 x 172 x 256: 2.8 us).
 #include "int8_mm.cuh"
 
 namespace f2c {
@@ -25,7 +25,6 @@ struct Params {
   void* out;
   int n, k, relu;
   int k_parts;            // warps that share a channel's K
-  int weights_first;
 };
 
 // 16 columns from t on of a row of a matrix whose last byte is in front of `end`; zeros behind the row
@@ -74,10 +73,9 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const Params p) {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) to[g] = u < units ? read16(w[g], u * kUnit + at, p.k, end) : make_uint4(0u, 0u, 0u, 0u);
   };
-  if (!p.weights_first) dependency_wait();
+  dependency_wait();
 #pragma unroll
   for (int q = 0; q < kAhead; ++q) weights(part + q * p.k_parts, b[q]);
-  if (p.weights_first) dependency_wait();
   release_dependents();
 
   const int pitch = units * kUnit + 64;  // rows that follow one another start in different halves of the banks
@@ -236,7 +234,7 @@ bool few_encodes(const Rows& x, int64_t n) {
 
 int few(const char* op, const Rows& x, const Job& j, cudaStream_t st) {
   const int64_t k = j.k, n = j.b.rows;
-  i8f::Params p{x, j.b.p, j.b.ld, j.a_scales, j.b_scales, j.bias, j.out, (int)n, (int)k, j.relu, i8f::k_parts(x.m, n, k), j.weights_first};
+  i8f::Params p{x, j.b.p, j.b.ld, j.a_scales, j.b_scales, j.bias, j.out, (int)n, (int)k, j.relu, i8f::k_parts(x.m, n, k)};
   const dim3 grid((unsigned)ceil_div(x.m, i8f::kRows), (unsigned)ceil_div(n, i8f::kWarps / p.k_parts * 8 * i8f::kGroups));
   const size_t smem = (size_t)i8f::kRows * (ceil_div(k, i8f::kUnit) * i8f::kUnit + 64);
   const cudaError_t e = x.dtype == F2C_I8    ? i8f::by_output<int8_t>(j.out_dtype, p, grid, smem, st)

@@ -264,6 +264,5 @@ extern "C" int f2c_int8_linear(const void* x1, int64_t ld1, int64_t k1, const vo
   if (const int rc = i8::quantize(r, codes, ldq, scales, st)) return rc;
   j.a = i8::Operand{codes, ldq, m};
   j.a_scales = scales; j.weights_first = 1;
-  if (i8::is_few(m, n, k)) return i8::few(op, i8::Rows{codes, nullptr, ldq, 0, k, 0, m, F2C_I8}, j, st);
   return i8::mm(op, j, st);
 }
