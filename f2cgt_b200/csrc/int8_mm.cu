@@ -10,7 +10,7 @@
 //  * Few tiles and a long K: the CTAs of a cluster each take a part of K and add their sums over distributed shared memory, which is exact
 //    and in any order the same.
 // Large products are bound by the tensor cores (16,384 x 4096 x 4096: 166 us, 3.3 POP/s, the tensor pipe busy 94% of the time), those of short K by
-// memory (59,000 x 128 x 256 to float32: 10.0 us, 4.6 TB/s), small ones by latency (16 x 4096 x 4096 with the codes of its rows: 7.1 us).
+// memory (59,000 x 128 x 256 to float32: 10.6 us a call, 4.3 TB/s), small ones by latency (16 x 4096 x 4096 with the codes of its rows: 7.3 us).
 // Every wait is bounded: when one runs out the CTA's roles all leave, what it has not finished becomes NaN, copies and products in flight are
 // waited for, the error word is raised and TMEM is freed.
 #include "int8_mm.cuh"
@@ -306,11 +306,12 @@ Plan plan(int64_t m, int64_t n, int64_t k, int sms) {
     if (q.stages > kMaxStages) q.stages = kMaxStages;
     // A step of K takes the longest of its bytes at 56 a cycle (what an SM was seen to get from L2 with all others at it; 100 where half of them
     // have none), its MMAs, and the 2800 cycles that memory was seen to take under load shared among the stages; the results 12 cycles a row,
-    // beside the next tile's steps; a tile 1000; the exchange between the parts of K 2000 and 16 a row; a pair 100 a step and 1500.  What it chooses between, measured:
-    //   16384 x 4096 x 4096 (m x n x k): 189 us with 256 rows and a CTA, 165 with a pair; 30000 x 400 x 3000: 45 and 38
-    //   512 x 4096 x 4096: 9.8 us with 128 rows and a CTA, 10.3 with a pair, 12.4 with 192 rows, 13.5 with 64
-    //   59,000 x 128 x 256: 8.4 us with 224 rows, 8.9 with 256, 10.1 with 128; 20,000 x 128 x 256: 4.6 with 160, 4.9 with 192, 5.9 with 128
-    //   32 x 4096 x 4096: 6.0 us in four parts of K, 6.3 in two, 7.0 in one; 128 x 4096 x 4096: 7.6 in one, 8.8 in two (64 rows)
+    // beside the next tile's steps; a tile 1000; the exchange between the parts of K 2000 and 16 a row; a pair 100 a step and 1500.  What it chooses between, measured
+    // (calls in a graph, to bfloat16 but for *, which is to float32; inputs and results that L2 does not hold):
+    //   16384 x 4096 x 4096 (m x n x k): 192 us with 256 rows and a CTA, 164 with a pair; 30000 x 400 x 3000: 46, 39, and 37 with 224 rows and a pair
+    //   512 x 4096 x 4096: 11.3 us with 128 rows and a CTA, 10.7 with a pair, 13.2 with 192 rows, 13.8 with 64
+    //   59,000 x 128 x 256 *: 11.8 us with 224 rows, 11.9 with 256, 13.0 with 128; 20,000 x 128 x 256 *: 6.0 with 160, 6.2 with 192, 7.7 with 128
+    //   32 x 4096 x 4096: 7.5 us in four parts of K, 7.9 in two, 8.0 in one; 128 x 4096 x 4096 (64 rows): 8.5 in one, 10.0 in two
     // (Weights kept in shared memory over a CTA's tiles made no difference of 2% anywhere.)
     const int rate = 2 * (int)q.grid > sms ? 56 : 100, step = std::max(std::max((int)stage / rate + (ctas > 1 ? 100 : 0), 2 * rows), 2800 / q.stages);
     const int64_t tile = std::max((int64_t)steps * step, (int64_t)12 * rows);

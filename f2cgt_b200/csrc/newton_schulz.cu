@@ -11,7 +11,8 @@
 // last step - the optimiser's update are the epilogue's.
 //
 // Precision.  Operands are half precision times a power of two for each matrix and step, chosen by a bound on the matrix' norm so that
-// the largest values stay a factor of 30 away from infinity and the smallest keep their bits; sums are single precision, the norm's double.
+// the smallest values keep their bits and the largest have room: X and A stay below 2^11, R below 60 * 2^10 for any coefficients that are
+// accepted (infinity is 2^16; of the default ones R stays below 2.9 * 2^10).  Sums are single precision, the norm's double.
 //  * bfloat16.  The first X is exact, A and R are rounded to 11 bits (R multiplies from the left: its rounding turns the singular
 //    vectors by 2^-12 of R's size), or pairs where they have no more than 256 rows (the fewer, the less do roundings cancel out: 43 x 42 in bfloat16
 //    3.0e-3 off without, of which the result's own rounding is 1.7e-3).  X's own rounding is noise of full rank, which the following steps multiply by up to the product of their

@@ -1,12 +1,12 @@
 // Newton-Schulz steps on matrices that one SM can hold: up to 128 x 256 (or transposed), each in a CTA, all of them in one launch (the weight matrices of a
-// GraphSAGE network are of this size).
+// GraphSAGE network of 128 columns are of this size; those of 256 x 256 are not).
 //
 // X (its smaller side down, the larger one along) stays in shared memory as two planes of half precision, A and then R beside it; the sums are in
 // TMEM: 128 columns for X X^T, 128 for A^2, 256 for R X.  X is laid out in pieces of 64 columns, rows of 128 bytes (128-byte swizzle): along K for
 // X X^T, and the same bytes, read as rows along N, for R X.  A thread has a row of X, A and R and a quarter of its columns; what the next
 // product reads goes from TMEM through registers to shared memory.
-// What bounds it is the chain of 15 products, each with its MMAs, the reading of its sums and a barrier (128 x 128 float32: 24 MMAs of 64 cycles
-// in some 2500; five steps 43.5 us).  Precision is as in newton_schulz.cu: everything in pairs, but that bfloat16's
+// What bounds it is the chain of 15 products, each with its MMAs, the reading of its sums and a barrier (128 x 128 float32: five steps 43.5 us, so 2.8 us
+// or some 5300 cycles a product, of which its 24 MMAs take 64 each).  Precision is as in newton_schulz.cu: everything in pairs, but that bfloat16's
 // X X^T takes the high planes alone.
 #include "newton_schulz.cuh"
 

@@ -1,6 +1,7 @@
 """Muon for the weight matrices of a network: momentum, and updates whose singular values are all about one.
 
-The step itself is ``ops.muon_step`` - one launch for all matrices of a GraphSAGE network.  What is no matrix (biases) is updated by Adam, in the
+The step itself is ``ops.muon_step``: one launch for all matrices up to 128 x 256 (or transposed), 17 launches for those of each larger
+shape.  A GraphSAGE network of 128 columns takes 53 us, one of 256 columns 185.  What is no matrix (biases) is updated by Adam, in the
 fused kernel ``train_graphsage.DirectFusedAdam`` calls.  Like that class it is a plain object: ``step()``, ``zero_grad()``, ``lr``.
 """
 import torch
