@@ -1,0 +1,166 @@
+// Rows four columns a lane (layer_norm.cu, layer_norm_backward.cu, checkpoint.cu), and activations in 8 bits:
+// of every row, 128 columns at a time - four of each lane of a warp - are a group with codes 0 .. 255,
+//   low = min,  step = (max - low) / 255,  code = round-to-even((x - low) / step),  value = low + step * code,
+// the differences and quotients as single precision has them, so that every implementation of the definition gives the same codes.
+// A group whose max - low is not finite (it holds a NaN or an infinity, or more than the type's range) has codes 0 and values NaN.
+#pragma once
+#include "common.cuh"
+
+namespace f2c {
+namespace ckpt {
+
+constexpr int kGroup = F2C_CHECKPOINT_GROUP;  // columns of a warp, four a lane
+static_assert(kGroup == 128, "a group is what a warp holds");
+constexpr int64_t kMaxRows = 1ll << 31, kMaxColumns = 1 << 20;
+
+// Four columns of a row as they are in memory.  ACCESS: bytes of a load or store, by what the rows' alignment and length allow.
+template <typename T, int ACCESS>
+struct alignas(4 * sizeof(T)) Four {
+  static constexpr int kEach = ACCESS / (int)sizeof(T), kPieces = 4 / kEach;
+  T v[4];
+
+  // the row's columns from `at` on, of which `left` (which may be negative) exist; zeros for the others
+  __device__ __forceinline__ void load(const T* at, int left) {
+    if constexpr (ACCESS == 16) {
+      const uint4 w = ldg_nc_u128_if(at, left > 0);
+      *reinterpret_cast<uint4*>(v) = w;
+    } else if constexpr (kPieces == 1) {
+      *reinterpret_cast<uint2*>(v) = ldg_nc_u64_if(at, left > 0);
+    } else {
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const bool here = p * kEach < left;
+        if constexpr (ACCESS == 8) *reinterpret_cast<uint2*>(v + p * kEach) = here ? __ldg(reinterpret_cast<const uint2*>(at) + p) : make_uint2(0u, 0u);
+        else if constexpr (ACCESS == 4) *reinterpret_cast<uint32_t*>(v + p * kEach) = here ? __ldg(reinterpret_cast<const uint32_t*>(at) + p) : 0u;
+        else *reinterpret_cast<uint16_t*>(v + p) = here ? __ldg(reinterpret_cast<const uint16_t*>(at) + p) : (uint16_t)0;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* at, int left) const {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      if (p * kEach >= left) continue;
+      if constexpr (ACCESS == 16) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(v);
+      else if constexpr (ACCESS == 8) *reinterpret_cast<uint2*>(at + p * kEach) = *reinterpret_cast<const uint2*>(v + p * kEach);
+      else if constexpr (ACCESS == 4) *reinterpret_cast<uint32_t*>(at + p * kEach) = *reinterpret_cast<const uint32_t*>(v + p * kEach);
+      else at[p] = v[p];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = to_float(v[e]);
+  }
+  __device__ __forceinline__ void set(const float (&f)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = from_float<T>(f[e]);
+  }
+};
+
+// Bytes of an access that rows of `item`-byte elements starting at `p`, `ld` elements apart and d long, allow; at most four elements.
+static inline int access_of(const void* p, int64_t ld, int64_t m, int64_t d, int item) {
+  int a = 4 * item;
+  while (a > item && (!aligned(p, a) || d * item % a != 0 || (m > 1 && ld * item % a != 0))) a /= 2;
+  return a;
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float warp_min_nan(float v) {
+  float r;
+  asm volatile("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+struct Scale { float step, low; };
+
+// Codes of a group, four columns a lane of which `left` exist (the others' codes are 0); by whole warps.  The quotient is a product with the
+// reciprocal, which is at most 255 * 3 * 2^-24 = 4.6e-5 off; only where it lies so near to a tie that this could matter, or where the step is so
+// small that the reciprocal is none, is the division made.
+__device__ __forceinline__ uint32_t encode(const float (&x)[4], int left, Scale& s) {
+  float low = __int_as_float(0x7f800000), high = -low;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    low = min_nan(low, e < left ? x[e] : low);
+    high = max_nan(high, e < left ? x[e] : high);
+  }
+  low = warp_min_nan(low);
+  high = warp_max_nan(high);
+  const float range = high - low;
+  if (!(range <= 3.402823466e38f)) {  // infinite, or no number
+    s.step = s.low = __int_as_float(0x7fffffff);
+    return 0u;
+  }
+  s.low = low;
+  s.step = range / 255.0f;
+  if (s.step == 0.0f) return 0u;
+  const bool small = s.step < 1e-35f;
+  const float by = 1.0f / s.step;
+  uint32_t codes = 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float over = x[e] - low;
+    float q = over * by;
+    const float r = rintf(q);
+    if (small || fabsf(fabsf(q - r) - 0.5f) < 1e-4f) q = rintf(over / s.step);
+    else q = r;
+    if (e < left) codes |= (uint32_t)fminf(q, 255.0f) << (8 * e);
+  }
+  return codes;
+}
+
+__device__ __forceinline__ void decode(uint32_t codes, Scale s, float (&x)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = fmaf(s.step, (float)((codes >> (8 * e)) & 255u), s.low);
+}
+
+__device__ __forceinline__ Scale load_scale(const float* at) {
+  const float2 v = __ldg(reinterpret_cast<const float2*>(at));
+  return Scale{v.x, v.y};
+}
+__device__ __forceinline__ void store_scale(float* at, Scale s) { *reinterpret_cast<float2*>(at) = make_float2(s.step, s.low); }
+
+// Codes, their row stride in bytes, and [rows][groups][step, low].
+struct Codes {
+  uint8_t* codes;
+  int64_t ld;
+  float* scales;
+  int64_t groups;
+};
+
+// What the entry points refuse of codes: rows start on 16 bytes, with room for whole 16 bytes, and scales on 8.
+int check_codes(const char* op, const uint8_t* codes, int64_t ldq, const float* scales, int64_t m, int64_t d);
+int check_sizes(const char* op, int dtype, int64_t m, int64_t d);
+
+}  // namespace ckpt
+}  // namespace f2c
+
+// a type and an access width as template arguments
+#define F2C_BY_ROWS(run, dtype, access, ...)                                   \
+  do {                                                                         \
+    if (dtype == F2C_F32) {                                                    \
+      if (access == 16) run<float, 16>(__VA_ARGS__);                           \
+      else if (access == 8) run<float, 8>(__VA_ARGS__);                        \
+      else run<float, 4>(__VA_ARGS__);                                         \
+    } else if (dtype == F2C_F16) {                                             \
+      if (access == 8) run<__half, 8>(__VA_ARGS__);                            \
+      else if (access == 4) run<__half, 4>(__VA_ARGS__);                       \
+      else run<__half, 2>(__VA_ARGS__);                                        \
+    } else {                                                                   \
+      if (access == 8) run<__nv_bfloat16, 8>(__VA_ARGS__);                     \
+      else if (access == 4) run<__nv_bfloat16, 4>(__VA_ARGS__);                \
+      else run<__nv_bfloat16, 2>(__VA_ARGS__);                                 \
+    }                                                                          \
+  } while (0)

@@ -1,0 +1,381 @@
+// Layer norm's backward pass (f2c_layer_norm_backward).  With h = (x - mean) rstd and g = dy where the ReLU was open (everywhere without one):
+//   dx = rstd (g w - mean(g w) - h mean(g w h)),   dweight = sum over rows of g h,   dbias = sum over rows of g.
+// x is the rows themselves or their 8-bit codes (checkpoint.cuh), decoded on the way.
+//
+// Bound by reading dy and x and writing dx.  A lane has the same columns of every row that its warp (or CTA) takes, so the sums over rows stay in
+// registers; each CTA leaves one part of them, and a second launch adds the parts up in their order: no atomics, the same bits every time.
+// What a row needs is on the way while the row before it is worked on.
+#include <type_traits>
+
+#include "checkpoint.cuh"
+
+namespace f2c {
+namespace ln {
+
+using ckpt::Four;
+using ckpt::kGroup;
+
+struct Back {
+  const void* dy;
+  int64_t ldy;
+  const void* x;               // or
+  ckpt::Codes codes;
+  int64_t ldx, m;
+  int d;
+  const float *mean, *rstd;
+  const uint8_t* active;       // null: no ReLU
+  const float* weight;         // null: 1
+  void* dx;                    // [m, d]
+  float* parts;                // [CTAs][2][d]
+};
+
+// A lane's four columns of a row, on their way
+template <typename T, int ACCESS, bool CODES>
+struct Columns {
+  using Kept = typename std::conditional<CODES, uint32_t, Four<T, ACCESS>>::type;
+  Four<T, ACCESS> dy;
+  Kept x;
+  ckpt::Scale s;
+  uint32_t open;
+
+  __device__ __forceinline__ void load(const Back& a, int64_t row, int chunk, bool here) {
+    const int lane = threadIdx.x & 31, col = chunk * kGroup + 4 * lane, left = here ? a.d - col : 0;
+    dy.load((const T*)a.dy + row * a.ldy + col, left);
+    if constexpr (CODES) {
+      x = ldg_nc_u32_if(a.codes.codes + row * a.codes.ld + col, left > 0);
+      s = here && chunk < a.codes.groups ? ckpt::load_scale(a.codes.scales + 2 * (row * a.codes.groups + chunk)) : ckpt::Scale{0.0f, 0.0f};
+    } else {
+      x.load((const T*)a.x + row * a.ldx + col, left);
+    }
+    open = 15u;
+    if (a.active != nullptr) open = left > 0 ? (uint32_t)__ldg(a.active + row * ((a.d + 7) >> 3) + (col >> 3)) >> (4 * (lane & 1)) : 0u;
+  }
+  // g and h; columns that do not exist have neither
+  __device__ __forceinline__ void get(float mean, float rstd, int left, float (&g)[4], float (&h)[4]) const {
+    dy.get(g);
+    if constexpr (CODES) ckpt::decode(x, s, h);
+    else x.get(h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (!((open >> e) & 1u)) g[e] = 0.0f;
+      h[e] = e < left ? (h[e] - mean) * rstd : 0.0f;
+    }
+  }
+};
+
+__device__ __forceinline__ void weights_of(const Back& a, int chunk, float (&w)[4]) {
+  const int col = chunk * kGroup + 4 * (threadIdx.x & 31);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = col + e < a.d ? (a.weight != nullptr ? __ldg(a.weight + col + e) : 1.0f) : 0.0f;
+}
+
+__device__ __forceinline__ void warp_sum2(float& u, float& v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    u += __shfl_xor_sync(0xffffffffu, u, o);
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+}
+
+// WARPS warps have a row of up to WARPS * CHUNKS * 128 columns: one warp (eight rows to a CTA), or a CTA's.
+template <typename T, int ACCESS, bool CODES, int WARPS, int CHUNKS, int THREADS>
+__global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant__ Back a) {
+  constexpr int kRows = THREADS / 32 / WARPS;  // of a CTA at a time
+  constexpr bool kAlone = WARPS == 1;
+  __shared__ float sums[2][2][kAlone ? 1 : WARPS];
+  __shared__ float joined[kAlone ? 2 * CHUNKS * kGroup : 1][kAlone ? kRows + 1 : 1];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % WARPS;
+  const int64_t stride = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + warp / WARPS;
+  Columns<T, ACCESS, CODES> next[CHUNKS];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  const auto fetch = [&](int64_t r) {
+    const bool here = r < a.m;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) next[c].load(a, r, member + c * WARPS, here);
+    if (here) {
+      next_mean = __ldg(a.mean + r);
+      next_rstd = __ldg(a.rstd + r);
+    }
+  };
+  fetch(row);
+  float w[CHUNKS][4], dw[CHUNKS][4], db[CHUNKS][4];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    weights_of(a, member + c * WARPS, w[c]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dw[c][e] = db[c][e] = 0.0f;
+  }
+  const float n = (float)a.d;
+  // (WARPS > 1: row is the CTA's, and all its threads leave together)
+  for (int turn = 0; row < a.m; row += stride, turn ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
+    Columns<T, ACCESS, CODES> now[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) now[c] = next[c];
+    fetch(row + stride);
+    float u = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      float g[4], h[4];
+      now[c].get(mean, rstd, a.d - (member + c * WARPS) * kGroup - 4 * lane, g, h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dw[c][e] = fmaf(g[e], h[e], dw[c][e]);
+        db[c][e] += g[e];
+        const float gw = g[e] * w[c][e];
+        u += gw;
+        v = fmaf(gw, h[e], v);
+      }
+    }
+    warp_sum2(u, v);
+    if constexpr (!kAlone) {
+      if (lane == 0) {
+        sums[turn][0][member] = u;
+        sums[turn][1][member] = v;
+      }
+      __syncthreads();  // (the other turn's sums are read before the next one)
+      u = v = 0.0f;
+#pragma unroll
+      for (int q = 0; q < WARPS; ++q) {
+        u += sums[turn][0][q];
+        v += sums[turn][1][q];
+      }
+    }
+    u /= n;
+    v /= n;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = (member + c * WARPS) * kGroup + 4 * lane, left = a.d - col;
+      float g[4], h[4];
+      now[c].get(mean, rstd, left, g, h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[e] = rstd * (fmaf(g[e], w[c][e], -u) - h[e] * v);
+      Four<T, ACCESS> out;
+      out.set(g);
+      out.store((T*)a.dx + row * a.d + col, left);
+    }
+  }
+  float* const part = a.parts + (int64_t)blockIdx.x * 2 * a.d;
+  if constexpr (kAlone) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        joined[c * kGroup + 4 * lane + e][warp] = dw[c][e];
+        joined[CHUNKS * kGroup + c * kGroup + 4 * lane + e][warp] = db[c][e];
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * a.d; i += THREADS) {
+      const int from = i < a.d ? i : CHUNKS * kGroup + i - a.d;
+      float sum = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kRows; ++q) sum += joined[from][q];
+      part[i] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int col = (member + c * WARPS) * kGroup + 4 * lane;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < a.d) {
+          part[col + e] = dw[c][e];
+          part[a.d + col + e] = db[c][e];
+        }
+    }
+  }
+}
+
+// Rows that a CTA's registers do not hold: dx alone, each row read twice; the sums over rows are columns_kernel's.
+template <typename T, int ACCESS, bool CODES>
+__global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Back a) {
+  constexpr int kWarps = 16;
+  __shared__ float sums[2][kWarps];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.d + kGroup - 1) / kGroup;
+  const int64_t row = blockIdx.x;
+  const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row), n = (float)a.d;
+  float u = 0.0f, v = 0.0f;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int c = warp; c < chunks; c += kWarps) {
+      Columns<T, ACCESS, CODES> now;
+      now.load(a, row, c, true);
+      float g[4], h[4], w[4];
+      const int col = c * kGroup + 4 * lane, left = a.d - col;
+      now.get(mean, rstd, left, g, h);
+      weights_of(a, c, w);
+      if (pass == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u = fmaf(g[e], w[e], u);
+          v = fmaf(g[e] * w[e], h[e], v);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = rstd * (fmaf(g[e], w[e], -u) - h[e] * v);
+        Four<T, ACCESS> out;
+        out.set(g);
+        out.store((T*)a.dx + row * a.d + col, left);
+      }
+    }
+    if (pass == 0) {
+      warp_sum2(u, v);
+      if (lane == 0) {
+        sums[0][warp] = u;
+        sums[1][warp] = v;
+      }
+      __syncthreads();
+      u = v = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kWarps; ++q) {
+        u += sums[0][q];
+        v += sums[1][q];
+      }
+      u /= n;
+      v /= n;
+    }
+  }
+}
+
+// The sums of such rows: a CTA has 128 columns of every gridDim.x-th stretch of eight rows.
+template <typename T, int ACCESS, bool CODES>
+__global__ void __launch_bounds__(256) columns_kernel(const __grid_constant__ Back a) {
+  __shared__ float joined[2 * kGroup][9];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.y * kGroup + 4 * lane;
+  float dw[4] = {}, db[4] = {};
+  for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < a.m; row += (int64_t)gridDim.x * 8) {
+    Columns<T, ACCESS, CODES> now;
+    now.load(a, row, blockIdx.y, true);
+    float g[4], h[4];
+    now.get(__ldg(a.mean + row), __ldg(a.rstd + row), a.d - col, g, h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dw[e] = fmaf(g[e], h[e], dw[e]);
+      db[e] += g[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    joined[4 * lane + e][warp] = dw[e];
+    joined[kGroup + 4 * lane + e][warp] = db[e];
+  }
+  __syncthreads();
+  const int which = threadIdx.x / kGroup, c = threadIdx.x % kGroup, at = blockIdx.y * kGroup + c;
+  float sum = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) sum += joined[which * kGroup + c][q];
+  if (at < a.d) a.parts[((int64_t)blockIdx.x * 2 + which) * a.d + at] = sum;
+}
+
+// The parts' sums: 32 columns a CTA, a 32nd of the parts a warp.
+__global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ parts, int count, int d, float* __restrict__ dweight, float* __restrict__ dbias) {
+  __shared__ float of[32][33];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = blockIdx.x * 32 + lane;
+  float sum = 0.0f;
+  if (at < 2 * d)
+    for (int p = warp; p < count; p += 32) sum += parts[(int64_t)p * 2 * d + at];
+  of[warp][lane] = sum;
+  __syncthreads();
+  if (warp != 0) return;
+  sum = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 32; ++q) sum += of[q][lane];
+  if (at < d) {
+    if (dweight != nullptr) dweight[at] = sum;
+  } else if (at < 2 * d && dbias != nullptr) {
+    dbias[at - d] = sum;
+  }
+}
+
+// How the rows are dealt out: columns that a CTA's registers hold, and CTAs.
+struct Deal {
+  int warps, chunks, threads;  // warps 0: too long
+  int ctas;
+};
+static Deal deal(int64_t m, int64_t d) {
+  Deal r;
+  if (d <= kGroup) r = {1, 1, 256, 6};
+  else if (d <= 2 * kGroup) r = {1, 2, 256, 4};
+  else if (d <= 4 * kGroup) r = {1, 4, 256, 2};
+  else if (d <= 8 * kGroup) r = {8, 1, 256, 6};
+  else if (d <= 32 * kGroup) r = {8, 4, 256, 2};
+  else if (d <= 64 * kGroup) r = {16, 4, 512, 1};
+  else r = {0, 1, 256, 1};
+  const int rows = r.warps == 0 ? 8 : r.threads / 32 / r.warps;
+  int64_t ctas = ceil_div(m, rows), most = (int64_t)kSmCount * r.ctas;  // (a constant: results do not depend on the device's count)
+  if (r.warps == 0) most = 64;
+  r.ctas = (int)(ctas < most ? ctas : most);
+  return r;
+}
+
+template <typename T, int ACCESS, bool CODES>
+static void run_source(const Back& a, const Deal& how, cudaStream_t st) {
+  const dim3 grid((unsigned)how.ctas);
+  if (how.warps == 1 && how.chunks == 1) launch_dependent(backward_kernel<T, ACCESS, CODES, 1, 1, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 1 && how.chunks == 2) launch_dependent(backward_kernel<T, ACCESS, CODES, 1, 2, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 1) launch_dependent(backward_kernel<T, ACCESS, CODES, 1, 4, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 8 && how.chunks == 1) launch_dependent(backward_kernel<T, ACCESS, CODES, 8, 1, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 8) launch_dependent(backward_kernel<T, ACCESS, CODES, 8, 4, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 16) launch_dependent(backward_kernel<T, ACCESS, CODES, 16, 4, 512>, grid, 512, 0, st, a);
+  else {
+    launch_dependent(long_kernel<T, ACCESS, CODES>, dim3((unsigned)a.m), 512, 0, st, a);
+    launch_dependent(columns_kernel<T, ACCESS, CODES>, dim3((unsigned)how.ctas, (unsigned)ceil_div(a.d, kGroup)), 256, 0, st, a);
+  }
+}
+template <typename T, int ACCESS>
+static void run(const Back& a, const Deal& how, cudaStream_t st) {
+  if (a.codes.codes != nullptr) run_source<T, ACCESS, true>(a, how, st);
+  else run_source<T, ACCESS, false>(a, how, st);
+}
+
+}  // namespace ln
+}  // namespace f2c
+
+using namespace f2c;
+
+extern "C" int64_t f2c_layer_norm_backward_workspace(int64_t m, int64_t d) {
+  if (m <= 0 || d <= 0 || m >= ckpt::kMaxRows || d > ckpt::kMaxColumns) return 0;
+  return ceil_div((int64_t)ln::deal(m, d).ctas * 2 * d * 4, 256) * 256;
+}
+
+extern "C" int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, const void* x, int64_t ldx, const uint8_t* codes, int64_t ldq, const float* scales,
+                                       const float* mean, const float* rstd, const uint8_t* active, const float* weight, int64_t m, int64_t d, void* dx,
+                                       float* dweight, float* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* op = "layer_norm_backward";
+  if (const int rc = ckpt::check_sizes(op, dtype, m, d)) return rc;
+  F2C_REQUIRE(x == nullptr || codes == nullptr, F2C_ERR_INVALID, "%s: rows or their codes, not both", op);
+  if (codes || scales)
+    if (const int rc = ckpt::check_codes(op, codes, ldq, scales, m, d)) return rc;
+  if (d == 0) return F2C_OK;
+  F2C_REQUIRE(m == 0 || ((x || codes) && dy && mean && rstd && dx), F2C_ERR_INVALID, "%s: null pointer", op);
+  F2C_REQUIRE(m <= 1 || (ldy >= d && (x == nullptr || ldx >= d)), F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
+  F2C_REQUIRE(m < ckpt::kMaxRows, F2C_ERR_LIMIT, "%s: 2^31 rows", op);
+  const int64_t need = f2c_layer_norm_backward_workspace(m, d);
+  F2C_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 256)), F2C_ERR_INVALID, "%s: the workspace must have %lld bytes, 256-byte aligned", op,
+              (long long)need);
+  cudaStream_t st = (cudaStream_t)stream;
+  const ln::Deal how = ln::deal(m, d);
+  if (m > 0) {
+    const ln::Back a{dy, ldy, x, ckpt::Codes{const_cast<uint8_t*>(codes), ldq, const_cast<float*>(scales), ceil_div(d, ckpt::kGroup)}, ldx, m, (int)d, mean, rstd, active,
+                     weight, dx, (float*)workspace};
+    const int item = dtype_size(dtype);
+    int access = ckpt::access_of(dy, ldy, m, d, item), other = ckpt::access_of(dx, d, m, d, item);
+    access = other < access ? other : access;
+    if (x != nullptr) {
+      other = ckpt::access_of(x, ldx, m, d, item);
+      access = other < access ? other : access;
+    }
+    F2C_BY_ROWS(ln::run, dtype, access, a, how, st);
+    if (const int rc = check_launch(op)) return rc;
+  }
+  launch_dependent(ln::join_kernel, dim3((unsigned)ceil_div(2 * d, 32)), 1024, 0, st, (const float*)workspace, m > 0 ? how.ctas : 0, (int)d, dweight, dbias);
+  return check_launch(op);
+}

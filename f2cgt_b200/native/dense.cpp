@@ -3,38 +3,8 @@
 
 #include <vector>
 
-#include <c10/core/AutogradState.h>
-#include <torch/csrc/autograd/grad_mode.h>
-
 namespace f2c_native {
 namespace {
-
-constexpr unsigned kFloats = bit(F2C_F32) | bit(F2C_F16) | bit(F2C_BF16);
-
-// A CUDA matrix of one of `allowed` dtypes with contiguous rows, at any distance that keeps them apart.
-const at::Tensor& matrix(PyObject* o, const char* name, unsigned allowed) {
-  if (!THPVariable_Check(o)) fail(PyExc_TypeError, "%s must be a torch.Tensor", name);
-  const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.is_cuda()) fail(PyExc_RuntimeError, "%s must be a CUDA tensor", name);
-  const int tag = dtype_tag(t.scalar_type());
-  if (tag < 0 || !(allowed & bit(tag))) fail(PyExc_RuntimeError, "%s has unsupported dtype %s", name, c10::toString(t.scalar_type()));
-  if (t.dim() != 2) fail(PyExc_RuntimeError, "%s must be 2-D", name);
-  if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1))) fail(PyExc_RuntimeError, "%s must have contiguous rows", name);
-  return t;
-}
-
-int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
-
-void same_device(const at::Tensor& t, const at::Tensor& other, const char* name) {
-  if (t.device() != other.device()) fail(PyExc_RuntimeError, "%s is on another device", name);
-}
-
-void no_gradient(const at::Tensor& t, const char* op, const char* name) {
-  if (t.requires_grad() && at::GradMode::is_enabled())
-    fail(PyExc_RuntimeError, "%s has no gradient: %s requires one (detach it, or call under torch.no_grad())", op, name);
-  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
-    fail(PyExc_RuntimeError, "%s has no forward-mode derivative: %s has a tangent", op, name);
-}
 
 struct Rows {
   const at::Tensor* x1 = nullptr;
@@ -91,12 +61,6 @@ at::ScalarType float_type(PyObject* o, at::ScalarType otherwise) {
   const int tag = dtype_tag(t);
   if (tag < 0 || !(kFloats & bit(tag))) fail(PyExc_RuntimeError, "out_dtype %s is unsupported", c10::toString(t));
   return t;
-}
-
-bool truth(PyObject* o) {
-  const int v = PyObject_IsTrue(o);
-  if (v < 0) throw PythonError{};
-  return v != 0;
 }
 
 PyObject* pair(at::Tensor a, at::Tensor b) {

@@ -6,8 +6,10 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/f2cgt_b200.h"
@@ -80,6 +82,39 @@ inline double real(PyObject* o) {
   return v;
 }
 
+constexpr unsigned kFloats = bit(F2C_F32) | bit(F2C_F16) | bit(F2C_BF16);
+
+// A CUDA matrix of one of `allowed` dtypes with contiguous rows, at any distance that keeps them apart.
+inline const at::Tensor& matrix(PyObject* o, const char* name, unsigned allowed) {
+  if (!THPVariable_Check(o)) fail(PyExc_TypeError, "%s must be a torch.Tensor", name);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda()) fail(PyExc_RuntimeError, "%s must be a CUDA tensor", name);
+  const int tag = dtype_tag(t.scalar_type());
+  if (tag < 0 || !(allowed & bit(tag))) fail(PyExc_RuntimeError, "%s has unsupported dtype %s", name, c10::toString(t.scalar_type()));
+  if (t.dim() != 2) fail(PyExc_RuntimeError, "%s must be 2-D", name);
+  if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1))) fail(PyExc_RuntimeError, "%s must have contiguous rows", name);
+  return t;
+}
+
+inline int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+inline void same_device(const at::Tensor& t, const at::Tensor& other, const char* name) {
+  if (t.device() != other.device()) fail(PyExc_RuntimeError, "%s is on another device", name);
+}
+
+inline void no_gradient(const at::Tensor& t, const char* op, const char* name) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    fail(PyExc_RuntimeError, "%s has no gradient: %s requires one (detach it, or call under torch.no_grad())", op, name);
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    fail(PyExc_RuntimeError, "%s has no forward-mode derivative: %s has a tangent", op, name);
+}
+
+inline bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PythonError{};
+  return v != 0;
+}
+
 inline cudaStream_t stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 inline at::Tensor empty(at::IntArrayRef size, at::ScalarType dtype, const at::Device& device) {
@@ -114,7 +149,7 @@ inline auto unlocked(F&& body) {
 }
 
 
-extern PyMethodDef g_sage_methods[], g_loader_methods[], g_dense_methods[];  // sage.cpp, loader.cpp, dense.cpp
+extern PyMethodDef g_sage_methods[], g_loader_methods[], g_dense_methods[], g_learn_methods[];  // sage.cpp, loader.cpp, dense.cpp, learn.cpp
 
 void arguments(const char* name, Py_ssize_t got, Py_ssize_t want);
 

@@ -13,6 +13,8 @@ Differences, all additive:
 
 torch is used for memory and streams only; every computation is a kernel of libf2cgt_b200.so.
 """
+import collections
+
 import torch
 
 from . import _lib
@@ -364,6 +366,49 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     Weights and gradients float32 / float16 / bfloat16 (one dtype), momenta float32; call under ``torch.no_grad()``.  A weight or a momentum
     must not share memory with another tensor of the lists (a weight listed twice is refused)."""
     _native.muon_step(weights, grads, momenta, lr, momentum, nesterov, weight_decay, steps, coefficients, eps)
+
+
+# ------------------------------------------------------------------ activations in 8 bits, layer norm
+# Rows in 8 bits, 128 columns (a group) with a step and a lowest value of their own: ``codes`` uint8 [rows, cols], each row on 16 bytes, ``scales``
+# float32 [rows, groups, 2] (step, lowest value).
+Int8Checkpoint = collections.namedtuple("Int8Checkpoint", "codes scales")
+# What layer_norm_backward needs of layer_norm_train: the rows (a tensor, or an Int8Checkpoint of them), their means and reciprocal deviations,
+# and one bit a value for the ReLU (uint8 [rows, ceil(cols / 8)], None without one).
+NormSaved = collections.namedtuple("NormSaved", "x mean rstd active")
+
+
+def checkpoint_int8(x):
+    """Rows of ``x`` [rows, cols] (float32 / float16 / bfloat16) as an ``Int8Checkpoint``, for keeping activations until the backward pass
+    in a quarter (half) of their memory.  Of every 128 columns of a row ``step = (max - min) / 255`` and ``code = round-to-even((x - min) / step)``,
+    in single precision: values are at most half a step off.  128 columns that hold a NaN or an infinity, or whose range is more than float32 has, come back as NaN."""
+    return Int8Checkpoint(*_native.checkpoint_int8(x))
+
+
+def checkpoint_values(checkpoint, dtype=torch.float32):
+    """The rows that an ``Int8Checkpoint`` stands for: ``min + step * code``, rounded once to ``dtype``."""
+    return _native.checkpoint_values(checkpoint[0], checkpoint[1], dtype)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over every row of ``x`` [rows, cols] (float32 / float16 / bfloat16), then ReLU if asked for;
+    ``weight`` and ``bias`` float32 [cols] or None.  Statistics are single precision, the result is rounded once.  It has no gradient by itself:
+    ``layer_norm_train`` keeps what ``layer_norm_backward`` needs, ``sage.LayerNorm`` is the module over them."""
+    return _native.layer_norm(x, weight, bias, eps, relu, 0)[0]
+
+
+def layer_norm_train(x, weight=None, bias=None, eps=1e-5, relu=False, int8=False):
+    """``(layer_norm(x, ...), NormSaved)``.  With ``int8`` what is kept of the rows is their 8-bit codes (those of ``checkpoint_int8``, made in
+    the same pass), and the gradients are those of the rows that the codes stand for; the result is that of the rows themselves either way."""
+    y, mean, rstd, active, codes, scales = _native.layer_norm(x, weight, bias, eps, relu, 2 if int8 else 1)
+    return y, NormSaved(Int8Checkpoint(codes, scales) if int8 else x, mean, rstd, active)
+
+
+def layer_norm_backward(dy, saved, weight=None):
+    """``(dx, dweight, dbias)`` of ``layer_norm_train``: ``dx`` in the dtype of ``dy`` (that of the rows), the others float32 sums over the rows,
+    added up in the same order every time."""
+    kept = saved.x
+    x, scales = (kept, None) if isinstance(kept, torch.Tensor) else (kept[0], kept[1])
+    return _native.layer_norm_backward(dy, x, scales, saved.mean, saved.rstd, saved.active, weight)
 
 
 # ------------------------------------------------------------------ k-means

@@ -36,7 +36,7 @@ extern "C" {
 
 typedef enum {
   F2C_U8 = 0, F2C_I8 = 1, F2C_I16 = 2, F2C_I32 = 3, F2C_I64 = 4, F2C_F16 = 5, F2C_F32 = 6, F2C_F64 = 7,
-  F2C_BF16 = 8   /* the 8-bit products and the orthogonalised updates only */
+  F2C_BF16 = 8   /* what works on the dense half of a network only: 8-bit products, orthogonalised updates, norms, 8-bit activations, learned rows */
 } f2c_dtype;
 
 typedef enum { F2C_MEAN = 0, F2C_SUM = 1 } f2c_reduce;   /* the reference only has mean */
@@ -450,6 +450,31 @@ int f2c_orthogonalize(const void* g, void* out, int dtype, int64_t batch, int64_
 int64_t f2c_muon_workspace(const f2c_muon_matrix* list_host, int count, int dtype);
 int f2c_muon_step(const f2c_muon_matrix* list_host, int count, int dtype, float lr, float momentum, int nesterov, float decay,
                   const float* coefficients_host, int steps, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- what a deeper network trains with: activations in 8 bits, layer norm ----
+ * 8-bit activations.  Of every row, F2C_CHECKPOINT_GROUP columns at a time (the last group may have fewer) have
+ *   low = min,  step = (max - low) / 255,  code = round-to-even((x - low) / step),  value = low + step * code,
+ * differences and quotients in single precision.  Equal values have step 0 and codes 0.  A group that holds a NaN or an infinity, or whose
+ * range is more than single precision has, has codes 0, step and low NaN: its values are NaN.
+ * codes [m, d] uint8, rows ldq bytes apart: start and ldq multiples of 16, ldq >= d (bytes between the columns and the next four are written,
+ * and never used); scales [m, ceil(d / group), 2] float: step, low.  Rows x and out: dtype F32, F16 or BF16, strides in elements. */
+#define F2C_CHECKPOINT_GROUP 128
+int f2c_checkpoint_int8(const void* x, int64_t ldx, int dtype, int64_t m, int64_t d, uint8_t* codes, int64_t ldq, float* scales, void* stream);
+int f2c_checkpoint_values(const uint8_t* codes, int64_t ldq, const float* scales, int64_t m, int64_t d, void* out, int64_t ldo, int out_dtype,
+                          void* stream);
+/* y [m, d] = (x - mean) rstd weight + bias of every row, rstd = 1 / sqrt(mean((x - mean)^2) + eps); relu != 0: negative values become 0 (a NaN
+ * stays one).  x and y of `dtype`, everything else float; weight, bias [d] or NULL (1, 0).  Wanted for the backward pass, or NULL: mean and
+ * rstd [m]; active [m, ceil(d / 8)]: bit c % 8 of byte c / 8 says that y was positive before rounding (bits behind the columns are 0); codes and
+ * scales: x in 8 bits, as f2c_checkpoint_int8 has it. */
+int f2c_layer_norm(const void* x, int64_t ldx, int dtype, int64_t m, int64_t d, const float* weight, const float* bias, float eps, int relu, void* y,
+                   float* mean, float* rstd, uint8_t* active, uint8_t* codes, int64_t ldq, float* scales, void* stream);
+/* Gradients of it.  x or codes (with scales), mean, rstd and active (NULL: no ReLU) as f2c_layer_norm left them; dy and dx (and x) of `dtype`, dx
+ * [m, d]; dweight, dbias [d] float or NULL, 0 without rows.  Sums are single precision and always in the same order.  workspace:
+ * f2c_layer_norm_backward_workspace(m, d) bytes, 256-byte aligned. */
+int64_t f2c_layer_norm_backward_workspace(int64_t m, int64_t d);
+int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, const void* x, int64_t ldx, const uint8_t* codes, int64_t ldq, const float* scales,
+                            const float* mean, const float* rstd, const uint8_t* active, const float* weight, int64_t m, int64_t d, void* dx,
+                            float* dweight, float* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

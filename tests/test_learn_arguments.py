@@ -1,0 +1,47 @@
+"""CPU: layer norm, 8-bit activations and learned rows refuse bad arguments before any CUDA call, and do nothing on nothing."""
+import pytest
+
+from f2cgt_b200 import _lib
+
+lib = _lib.lib
+OK, INVALID, UNSUPPORTED, LIMIT = 0, 1, 2, 4
+AT = 0x10000  # an address that is never looked at
+
+
+def encode(x=AT, ldx=40, dtype=_lib.F32, m=4, d=40, codes=AT, ldq=48, scales=AT):
+    return lib.f2c_checkpoint_int8(x, ldx, dtype, m, d, codes, ldq, scales, None)
+
+
+def values(codes=AT, ldq=48, scales=AT, m=4, d=40, out=AT, ldo=40, dtype=_lib.F32):
+    return lib.f2c_checkpoint_values(codes, ldq, scales, m, d, out, ldo, dtype, None)
+
+
+def norm(x=AT, ldx=40, dtype=_lib.F32, m=4, d=40, eps=1e-5, y=AT, mean=0, rstd=0, active=0, codes=0, ldq=0, scales=0):
+    return lib.f2c_layer_norm(x, ldx, dtype, m, d, 0, 0, eps, 0, y, mean, rstd, active, codes, ldq, scales, None)
+
+
+def backward(dy=AT, ldy=40, dtype=_lib.F32, x=AT, ldx=40, codes=0, ldq=0, scales=0, mean=AT, rstd=AT, m=4, d=40, dx=AT, work=AT, size=1 << 30):
+    return lib.f2c_layer_norm_backward(dy, ldy, dtype, x, ldx, codes, ldq, scales, mean, rstd, 0, 0, m, d, dx, AT, AT, work, size, None)
+
+
+@pytest.mark.parametrize("call,status", [
+    (lambda: encode(dtype=_lib.F64), UNSUPPORTED), (lambda: encode(m=-1), INVALID), (lambda: encode(d=(1 << 20) + 1, ldx=1 << 21, ldq=1 << 21), LIMIT), (lambda: encode(ldx=39), INVALID),
+    (lambda: encode(x=0), INVALID), (lambda: encode(codes=0), INVALID), (lambda: encode(codes=AT + 8), INVALID), (lambda: encode(ldq=40), INVALID), (lambda: encode(ldq=32), INVALID),
+    (lambda: encode(scales=0), INVALID), (lambda: encode(scales=AT + 4), INVALID), (lambda: encode(m=1 << 30, d=1 << 10, ldx=1 << 10, ldq=1 << 10), LIMIT),
+    (lambda: encode(m=0, x=0, codes=0, scales=0), OK), (lambda: encode(d=0, x=0, codes=0, scales=0), OK),
+    (lambda: values(dtype=_lib.I8), UNSUPPORTED), (lambda: values(out=0), INVALID), (lambda: values(ldo=39), INVALID), (lambda: values(codes=AT + 4), INVALID), (lambda: values(m=0, out=0), OK),
+    (lambda: norm(dtype=_lib.I32), UNSUPPORTED), (lambda: norm(eps=-1e-9), INVALID), (lambda: norm(eps=float("nan")), INVALID), (lambda: norm(mean=AT), INVALID), (lambda: norm(x=0), INVALID),
+    (lambda: norm(y=0), INVALID), (lambda: norm(ldx=39), INVALID), (lambda: norm(codes=AT), INVALID), (lambda: norm(codes=AT, ldq=40, scales=AT), INVALID),
+    (lambda: norm(m=1 << 31), LIMIT), (lambda: norm(m=0, x=0, y=0), OK), (lambda: norm(d=0, x=0, y=0), OK),
+    (lambda: backward(dtype=_lib.U8), UNSUPPORTED), (lambda: backward(x=0), INVALID), (lambda: backward(codes=AT, ldq=48, scales=AT), INVALID), (lambda: backward(dy=0), INVALID),
+    (lambda: backward(mean=0), INVALID), (lambda: backward(rstd=0), INVALID), (lambda: backward(dx=0), INVALID), (lambda: backward(ldy=39), INVALID), (lambda: backward(ldx=39), INVALID),
+    (lambda: backward(work=0), INVALID), (lambda: backward(work=AT + 16), INVALID), (lambda: backward(size=100), INVALID), (lambda: backward(d=0), OK)])
+def test_norms_and_8_bit_activations(call, status):
+    assert call() == status
+    assert status == OK or b"checkpoint" in lib.f2c_last_error() or b"layer_norm" in lib.f2c_last_error()
+
+
+def test_workspaces_of_the_norms_gradient():
+    assert lib.f2c_layer_norm_backward_workspace(0, 128) == 0 and lib.f2c_layer_norm_backward_workspace(10, 0) == 0
+    assert lib.f2c_layer_norm_backward_workspace(8, 128) == 1024  # one CTA's two sums of 128 columns
+    assert lib.f2c_layer_norm_backward_workspace(1 << 20, 128) >= 148 * 1024
