@@ -1,0 +1,580 @@
+// Rows of a table by ids, scaled (f2c_embedding), and the table's gradient (f2c_embedding_backward).
+//
+// The lookup is bound by reading and writing the rows.  The gradient of row r is the sum of dy over the places i with ids[i] = r, in their order: the
+// places are sorted by id (stable), every warp adds up a stretch of them, and a segment that lies in several stretches is put together by
+// a last launch.  No atomics on values: the same bits every time.  Sums are single precision, rounded once.
+//
+// Sorting.  Up to 4096 places each place counts the ones in front of it, in one launch: the keys are few enough that all pairs cost
+// less than further launches.  Beyond, digits of up to 11 bits from the lowest on: counts of every tile of 2048 places, their sums over tiles, and the
+// placing, in which a warp ranks 32 places at a time by their equals in it.  As many digits as the table has rows need.
+#include "checkpoint.cuh"
+
+namespace f2c {
+namespace emb {
+
+using ckpt::Four;
+using ckpt::kGroup;
+
+constexpr int kThreads = 256, kWarps = kThreads / 32, kAhead = 4;
+constexpr int64_t kMaxRows = (1ll << 31) - 2, kMaxPlaces = 1ll << 30, kMaxColumns = 1 << 20;
+
+// ---------------------------------------------------------------- lookup
+// A thread has kAhead vectors of ACCESS bytes of the result, all loads before the first use.
+template <typename T, typename I, int ACCESS>
+__global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ table, int64_t ld, int64_t rows, int vectors, const I* __restrict__ ids, int64_t m, float scale,
+                                                          T* __restrict__ out) {
+  constexpr int V = ACCESS / (int)sizeof(T);
+  struct alignas(ACCESS) Vec { T v[V]; };
+  dependency_wait();
+  release_dependents();
+  const int64_t first = (int64_t)blockIdx.x * (kThreads * kAhead), row0 = first / vectors;
+  const uint32_t rest = (uint32_t)(first - row0 * vectors) + threadIdx.x;
+  Vec v[kAhead];
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    const uint32_t at = rest + a * kThreads;
+    const int64_t row = row0 + at / (uint32_t)vectors;
+    const int64_t id = row < m ? (int64_t)__ldg(ids + row) : -1;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[a].v[e] = from_float<T>(0.0f);
+    if ((uint64_t)id < (uint64_t)rows) v[a] = *(reinterpret_cast<const Vec*>(table + id * ld) + at % (uint32_t)vectors);
+  }
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    const int64_t row = row0 + (rest + a * kThreads) / (uint32_t)vectors;
+    if (row >= m) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[a].v[e] = from_float<T>(to_float(v[a].v[e]) * scale);
+    *(reinterpret_cast<Vec*>(out) + first + threadIdx.x + a * kThreads) = v[a];
+  }
+}
+
+// ---------------------------------------------------------------- sorting
+constexpr int kItems = 8, kTile = kThreads * kItems, kMaxBits = 11, kFew = 4096;
+
+// A row's number, or the number of rows where the id is outside the table.
+template <typename I>
+__device__ __forceinline__ uint32_t key_of(const I* ids, int64_t i, uint32_t rows) {
+  const int64_t id = (int64_t)__ldg(ids + i);
+  return (uint64_t)id < (uint64_t)rows ? (uint32_t)id : rows;
+}
+
+struct Pairs { uint32_t *key, *place; };
+
+// Few places: a warp finds the ranks of four at a time.
+template <typename I>
+__global__ void __launch_bounds__(kThreads) rank_kernel(const I* __restrict__ ids, int m, uint32_t rows, Pairs out) {
+  __shared__ uint32_t keys[kFew];
+  dependency_wait();
+  release_dependents();
+  for (int i = threadIdx.x; i < m; i += kThreads) keys[i] = key_of(ids, i, rows);
+  __syncthreads();
+  const int lane = threadIdx.x & 31, first = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * 4;
+  uint32_t mine[4];
+  int before[4] = {};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) mine[q] = keys[min(first + q, m - 1)];
+  for (int j = lane; j < m; j += 32) {
+    const uint32_t k = keys[j];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) before[q] += k < mine[q] || (k == mine[q] && j < first + q);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int rank = __reduce_add_sync(0xffffffffu, before[q]);
+    if (lane == 0 && first + q < m) {
+      out.key[rank] = mine[q];
+      out.place[rank] = (uint32_t)(first + q);
+    }
+  }
+}
+
+struct Digit { int shift, bits; };
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, Digit d) { return (key >> d.shift) & ((1u << d.bits) - 1u); }
+
+// counts [digit][tile].  FIRST: keys come from ids.
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kThreads) count_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t m, uint32_t rows, Digit d, uint32_t* __restrict__ counts,
+                                                         int tiles) {
+  __shared__ uint32_t here[1 << kMaxBits];
+  dependency_wait();
+  release_dependents();
+  for (int b = threadIdx.x; b < 1 << d.bits; b += kThreads) here[b] = 0u;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kItems; ++q) {
+    const int64_t i = (int64_t)blockIdx.x * kTile + q * kThreads + threadIdx.x;
+    if (i < m) atomicAdd(here + digit_of(FIRST ? key_of(ids, i, rows) : keys[i], d), 1u);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < 1 << d.bits; b += kThreads) counts[(int64_t)b * tiles + blockIdx.x] = here[b];
+}
+
+// A warp to a digit: its counts become those of the tiles in front, and their sum goes to `totals`.
+__global__ void __launch_bounds__(kThreads) tiles_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, int tiles, int bins) {
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, bin = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (bin >= bins) return;
+  uint32_t* const of = counts + (int64_t)bin * tiles;
+  uint32_t before = 0u;
+  for (int t = 0; t < tiles; t += 32) {
+    const uint32_t own = t + lane < tiles ? of[t + lane] : 0u;
+    uint32_t sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (t + lane < tiles) of[t + lane] = before + sum - own;
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) totals[bin] = before;
+}
+
+// `mine` of every thread becomes the sum of those of the threads in front.
+__device__ __forceinline__ uint32_t block_before(uint32_t mine, uint32_t* of_warp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) of_warp[warp] = sum;
+  __syncthreads();
+  uint32_t before = sum - mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w)
+    if (w < warp) before += of_warp[w];
+  return before;
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ ids, Pairs in, int64_t m, uint32_t rows, Digit d, const uint32_t* __restrict__ counts,
+                                                         const uint32_t* __restrict__ totals, int tiles, Pairs out) {
+  constexpr int kBins = 1 << kMaxBits, kEach = kBins / kThreads;
+  __shared__ uint16_t of_warp[kWarps][kBins];  // a tile has 2048 places
+  __shared__ uint32_t base[kBins], sums[kWarps];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << d.bits;
+  for (int i = threadIdx.x; i < kWarps * kBins / 2; i += kThreads) reinterpret_cast<uint32_t*>(of_warp)[i] = 0u;
+  {  // where each digit's places of this tile start
+    uint32_t own[kEach], sum = 0u;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int b = threadIdx.x * kEach + e;
+      own[e] = b < bins ? __ldg(totals + b) : 0u;
+      sum += own[e];
+    }
+    uint32_t before = block_before(sum, sums);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int b = threadIdx.x * kEach + e;
+      if (b < bins) base[b] = before + __ldg(counts + (int64_t)b * tiles + blockIdx.x);
+      before += own[e];
+    }
+  }
+  __syncthreads();
+  uint32_t key[kItems], place[kItems], rank[kItems];
+  const int64_t first = (int64_t)blockIdx.x * kTile + warp * (32 * kItems) + lane;
+#pragma unroll
+  for (int q = 0; q < kItems; ++q) {
+    const int64_t i = first + 32 * q;
+    key[q] = i < m ? (FIRST ? key_of(ids, i, rows) : in.key[i]) : 0u;
+    place[q] = i < m ? (FIRST ? (uint32_t)i : in.place[i]) : 0u;
+  }
+#pragma unroll
+  for (int q = 0; q < kItems; ++q) {
+    const bool here = first + 32 * q < m;
+    const uint32_t digit = digit_of(key[q], d), all = __ballot_sync(0xffffffffu, here);
+    uint32_t equal = 0u, before = 0u;
+    if (here) {
+      equal = __match_any_sync(all, digit);
+      before = of_warp[warp][digit];
+    }
+    __syncwarp();
+    if (here && (equal & ((1u << lane) - 1u)) == 0u) of_warp[warp][digit] = (uint16_t)(before + __popc(equal));
+    __syncwarp();
+    rank[q] = before + __popc(equal & ((1u << lane) - 1u));
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += kThreads) {
+    uint32_t before = 0u;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t own = of_warp[w][b];
+      of_warp[w][b] = (uint16_t)before;
+      before += own;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kItems; ++q)
+    if (first + 32 * q < m) {
+      const uint32_t digit = digit_of(key[q], d), to = base[digit] + of_warp[warp][digit] + rank[q];
+      out.key[to] = key[q];
+      out.place[to] = place[q];
+    }
+}
+
+// ---------------------------------------------------------------- sums over segments
+// Stretches of up to 32 sorted places, a warp's each.
+struct Segments {
+  const uint32_t *key, *place;  // sorted
+  int64_t m;
+  uint32_t rows;                // keys of places without a row
+  int stretch;                  // 8 to 32
+  int64_t stretches;
+  // only the rows that were looked up: numbers of segments in front of a stretch in its tile, and of those that begin in each tile
+  const uint32_t *in_tile, *of_tile;
+  int tiles;
+  int64_t* looked_up;           // null: the whole table
+  int64_t* count;
+};
+
+// Whether a segment begins at sorted place i.
+__device__ __forceinline__ bool begins(const uint32_t* key, int64_t i, int64_t m, uint32_t rows) {
+  return i < m && key[i] < rows && (i == 0 || key[i - 1] != key[i]);
+}
+
+// Numbers the segments: a CTA to a tile of 2048 places.
+__global__ void __launch_bounds__(kThreads) number_kernel(const uint32_t* __restrict__ key, int64_t m, uint32_t rows, int stretch, uint32_t* __restrict__ in_tile,
+                                                          uint32_t* __restrict__ of_tile, int64_t* __restrict__ looked_up) {
+  __shared__ uint32_t sums[kWarps];
+  dependency_wait();
+  release_dependents();
+  const int64_t first = (int64_t)blockIdx.x * kTile + threadIdx.x * kItems;
+  uint32_t own = 0u;
+#pragma unroll
+  for (int q = 0; q < kItems; ++q) {
+    own += begins(key, first + q, m, rows);
+    if (first + q < m) looked_up[first + q] = -1;  // (those that there are are written by the next launch)
+  }
+  const uint32_t before = block_before(own, sums);
+  // a thread's eight places are one stretch, or a part of one
+  if (first < m && first % stretch == 0) in_tile[first / stretch] = before;
+  if (threadIdx.x == kThreads - 1) of_tile[blockIdx.x] = before + own;
+}
+
+constexpr int kRowsAhead = 8;
+
+// What a stretch leaves: sums of the segment that it only continues (head) and of the one that goes on behind it (tail), and the tail's row (-1: none).
+struct Open {
+  float *head, *tail;  // [stretches][width]
+  int64_t* row;        // [stretches]
+  int64_t width;
+};
+
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__ dy, int64_t ld, int d, float scale, const __grid_constant__ Segments s, const __grid_constant__ Open open,
+                                                           T* __restrict__ out) {
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t c = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (c >= s.stretches) return;
+  const int64_t start = c * s.stretch;
+  const int n = (int)min((int64_t)s.stretch, s.m - start), col = blockIdx.y * kGroup + 4 * lane, left = d - col;
+  const uint32_t key = lane < n ? s.key[start + lane] : s.rows, place = lane < n ? s.place[start + lane] : 0u;
+  const uint32_t above = __shfl_up_sync(0xffffffffu, key, 1);
+  const uint32_t before = lane == 0 && start > 0 ? s.key[start - 1] : s.rows;
+  const uint32_t behind = start + n < s.m ? s.key[start + n] : s.rows;
+  const uint32_t first = __ballot_sync(0xffffffffu, lane < n && (lane == 0 ? start == 0 || before != key : above != key));
+  const int kept = __popc(__ballot_sync(0xffffffffu, key < s.rows));  // the places of no row are behind all others
+  int64_t number = 0;  // of the next segment that begins here
+  if (s.looked_up != nullptr) {
+    uint32_t tiles_before = 0u, all = 0u;
+    const int tile = (int)(start / kTile);
+    for (int t = lane; t < s.tiles; t += 32) {
+      const uint32_t v = s.of_tile[t];
+      all += v;
+      if (t < tile) tiles_before += v;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    number = (int64_t)__reduce_add_sync(0xffffffffu, tiles_before) + s.in_tile[c];
+    if (c == 0 && blockIdx.y == 0 && lane == 0) *s.count = all;
+    // rows behind the last segment's are zero
+    for (int64_t r = max(start, (int64_t)all); r < start + n; ++r) {
+      Four<T, ACCESS> zero;
+      const float none[4] = {};
+      zero.set(none);
+      zero.store(out + r * d + col, left);
+    }
+  }
+  float acc[4] = {};
+  bool head = (first & 1u) == 0u, opened = false;
+  const auto flush = [&](int last) {  // the segment whose last place here is `last`
+    const uint32_t k = __shfl_sync(0xffffffffu, key, last);
+    const bool goes_on = last == n - 1 && behind == k;
+    const int64_t row = s.looked_up != nullptr ? (head ? 0 : number) : (int64_t)k;
+    if (!head && s.looked_up != nullptr) {
+      if (lane == 0 && blockIdx.y == 0) s.looked_up[row] = (int64_t)k;
+      ++number;
+    }
+    if (head || goes_on) {
+      float* const to = (head ? open.head : open.tail) + c * open.width + blockIdx.y * kGroup + 4 * lane;
+      *reinterpret_cast<float4*>(to) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (!head) {
+        opened = true;
+        if (lane == 0 && blockIdx.y == 0) open.row[c] = row;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= scale;
+      Four<T, ACCESS> v;
+      v.set(acc);
+      v.store(out + row * d + col, left);
+    }
+    head = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = 0.0f;
+  };
+  for (int t0 = 0; t0 < kept; t0 += kRowsAhead) {
+    Four<T, ACCESS> v[kRowsAhead];
+#pragma unroll
+    for (int q = 0; q < kRowsAhead; ++q) {
+      const int64_t at = __shfl_sync(0xffffffffu, place, (t0 + q) & 31);
+      v[q].load(dy + at * ld + col, t0 + q < kept ? left : 0);
+    }
+#pragma unroll
+    for (int q = 0; q < kRowsAhead; ++q) {
+      const int t = t0 + q;
+      if (t >= kept) break;
+      if (t > 0 && ((first >> t) & 1u)) flush(t - 1);
+      float f[4];
+      v[q].get(f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += f[e];
+    }
+  }
+  if (kept > 0) flush(kept - 1);
+  if (!opened && lane == 0 && blockIdx.y == 0) open.row[c] = -1;
+}
+
+// Puts the segments together that lie in several stretches: the tail of the one in which they begin, then heads.  A warp does a short one by
+// itself, the whole CTA a long one.
+constexpr int kShort = 16;
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, const __grid_constant__ Segments s, const __grid_constant__ Open open, T* __restrict__ out) {
+  __shared__ float sums[kWarps][kGroup];
+  __shared__ int64_t long_row[kWarps];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.y * kGroup + 4 * lane;
+  const int64_t c0 = (int64_t)blockIdx.x * kWarps, c = c0 + warp;
+  const int64_t row = c < s.stretches ? open.row[c] : -1;
+  const auto key_of_tail = [&](int64_t q) { return s.key[(q + 1) * s.stretch - 1]; };
+  const auto goes_on = [&](int64_t q, uint32_t key) { return q < s.stretches && s.key[q * s.stretch] == key; };
+  const auto add = [&](float (&acc)[4], const float* from, int64_t q) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(from + q * open.width + blockIdx.y * kGroup + 4 * lane));
+    acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
+  };
+  const auto write = [&](int64_t to, float (&acc)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= scale;
+    Four<T, ACCESS> v;
+    v.set(acc);
+    v.store(out + to * d + col, d - col);
+  };
+  bool is_long = false;
+  if (row >= 0) {
+    const uint32_t key = key_of_tail(c);
+    is_long = goes_on(c + kShort, key);
+    if (!is_long) {
+      float acc[4] = {};
+      add(acc, open.tail, c);
+      for (int64_t q = c + 1; goes_on(q, key); ++q) add(acc, open.head, q);
+      write(row, acc);
+    }
+  }
+  if (lane == 0) long_row[warp] = is_long ? row : -1;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    if (long_row[w] < 0) continue;  // for all threads alike
+    const uint32_t key = key_of_tail(c0 + w);
+    float acc[4] = {};
+    if (warp == 0) add(acc, open.tail, c0 + w);
+    int64_t q = c0 + w + 1 + warp;
+    for (; goes_on(q + 3 * kWarps, key); q += 4 * kWarps) {  // (stretches of a segment lie side by side)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) add(acc, open.head, q + u * kWarps);
+    }
+    for (; goes_on(q, key); q += kWarps) add(acc, open.head, q);
+    *reinterpret_cast<float4*>(&sums[warp][4 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (warp == 0) {
+      float all[4] = {};
+#pragma unroll
+      for (int u = 0; u < kWarps; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) all[e] += sums[u][4 * lane + e];
+      write(long_row[w], all);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- host
+template <typename T, typename I, int ACCESS>
+static void lookup_as(const void* table, int64_t ld, int64_t rows, int64_t d, const void* ids, int64_t m, float scale, void* out, cudaStream_t st) {
+  const int vectors = (int)(d * (int64_t)sizeof(T) / ACCESS);
+  launch_dependent(lookup_kernel<T, I, ACCESS>, dim3((unsigned)ceil_div(m * vectors, kThreads * kAhead)), kThreads, 0, st, (const T*)table, ld, rows, vectors, (const I*)ids, m, scale,
+                   (T*)out);
+}
+template <typename T, typename I>
+static void lookup(const void* table, int64_t ld, int64_t rows, int64_t d, const void* ids, int64_t m, float scale, void* out, cudaStream_t st) {
+  int access = 16;
+  while (access > (int)sizeof(T) && (!aligned(table, access) || !aligned(out, access) || d * (int64_t)sizeof(T) % access != 0 || ld * (int64_t)sizeof(T) % access != 0)) access /= 2;
+  if (access == 16) lookup_as<T, I, 16>(table, ld, rows, d, ids, m, scale, out, st);
+  else if (access == 8) lookup_as<T, I, 8>(table, ld, rows, d, ids, m, scale, out, st);
+  else if (access == 4 || sizeof(T) == 4) lookup_as<T, I, 4>(table, ld, rows, d, ids, m, scale, out, st);
+  else if constexpr (sizeof(T) == 2) lookup_as<T, I, 2>(table, ld, rows, d, ids, m, scale, out, st);
+}
+
+// What a gradient needs of the workspace, in bytes from its start.
+struct Plan {
+  int64_t m, d;
+  int stretch, tiles, bits, passes;
+  int64_t stretches, width;
+  int64_t key[2], place[2], counts, totals, in_tile, of_tile, head, tail, row, bytes;
+};
+static Plan plan(int64_t m, int64_t rows, int64_t d) {
+  Plan p{};
+  p.m = m;
+  p.d = d;
+  // Short stretches where there are few places: a stretch's rows are added one after the other.
+  p.stretch = m <= 16384 ? 8 : 32;
+  p.tiles = (int)ceil_div(m, kTile);
+  int bits = 1;
+  while ((rows >> bits) != 0) ++bits;
+  p.passes = m <= kFew ? 0 : (bits + kMaxBits - 1) / kMaxBits;
+  p.bits = p.passes == 0 ? 0 : (bits + p.passes - 1) / p.passes;
+  p.stretches = ceil_div(m, p.stretch);
+  p.width = ceil_div(d, kGroup) * kGroup;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += ceil_div(bytes, 256) * 256;
+    return from;
+  };
+  for (int b = 0; b < (p.passes > 1 ? 2 : 1); ++b) {
+    p.key[b] = take(4 * m);
+    p.place[b] = take(4 * m);
+  }
+  if (p.passes > 0) {
+    p.counts = take(((int64_t)4 << p.bits) * p.tiles);
+    p.totals = take((int64_t)4 << p.bits);
+  }
+  p.in_tile = take(4 * p.stretches);
+  p.of_tile = take(4 * (int64_t)p.tiles);
+  p.head = take(4 * p.stretches * p.width);
+  p.tail = take(4 * p.stretches * p.width);
+  p.row = take(8 * p.stretches);
+  p.bytes = at;
+  return p;
+}
+
+// Sorts the places; the pairs' final place.
+template <typename I>
+static Pairs sort(const Plan& p, const I* ids, uint32_t rows, char* ws, cudaStream_t st) {
+  Pairs pairs[2];
+  for (int b = 0; b < 2; ++b) pairs[b] = Pairs{(uint32_t*)(ws + p.key[b]), (uint32_t*)(ws + p.place[b])};
+  if (p.passes == 0) {
+    launch_dependent(rank_kernel<I>, dim3((unsigned)ceil_div(p.m, 4 * kWarps)), kThreads, 0, st, ids, (int)p.m, rows, pairs[0]);
+    return pairs[0];
+  }
+  uint32_t *const counts = (uint32_t*)(ws + p.counts), *const totals = (uint32_t*)(ws + p.totals);
+  int to = p.passes & 1 ? 0 : 1;  // so that the last pass ends in pairs[0]
+  for (int q = 0; q < p.passes; ++q, to ^= 1) {
+    const Digit d{q * p.bits, p.bits};
+    const Pairs in = pairs[to ^ 1], out = pairs[to];
+    if (q == 0) launch_dependent(count_kernel<I, true>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, (const uint32_t*)nullptr, p.m, rows, d, counts, p.tiles);
+    else launch_dependent(count_kernel<I, false>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, (const uint32_t*)in.key, p.m, rows, d, counts, p.tiles);
+    launch_dependent(tiles_kernel, dim3((unsigned)ceil_div((int64_t)1 << p.bits, kWarps)), kThreads, 0, st, counts, totals, p.tiles, 1 << p.bits);
+    if (q == 0) launch_dependent(place_kernel<I, true>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, in, p.m, rows, d, (const uint32_t*)counts, (const uint32_t*)totals, p.tiles, out);
+    else launch_dependent(place_kernel<I, false>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, in, p.m, rows, d, (const uint32_t*)counts, (const uint32_t*)totals, p.tiles, out);
+  }
+  return pairs[0];
+}
+
+template <typename T, int ACCESS>
+static void add_up(const Plan& p, const void* dy, int64_t ld, float scale, const Segments& s, const Open& open, void* out, cudaStream_t st) {
+  const dim3 grid((unsigned)ceil_div(p.stretches, kWarps), (unsigned)ceil_div(p.d, kGroup));
+  launch_dependent(segment_kernel<T, ACCESS>, grid, kThreads, 0, st, (const T*)dy, ld, (int)p.d, scale, s, open, (T*)out);
+  launch_dependent(join_kernel<T, ACCESS>, grid, kThreads, 0, st, (int)p.d, scale, s, open, (T*)out);
+}
+
+static int check(const char* op, int dtype, int index_dtype, int64_t m, int64_t rows, int64_t d) {
+  F2C_REQUIRE(is_float_dtype(dtype), F2C_ERR_UNSUPPORTED, "%s: rows must be float32, float16 or bfloat16", op);
+  F2C_REQUIRE(is_index_dtype(index_dtype), F2C_ERR_UNSUPPORTED, "%s: ids must be int32 or int64", op);
+  F2C_REQUIRE(m >= 0 && rows >= 0 && d >= 0, F2C_ERR_INVALID, "%s: negative size", op);
+  F2C_REQUIRE(m <= kMaxPlaces && rows <= kMaxRows && d <= kMaxColumns && m * ceil_div(d, kGroup) <= 1ll << 33, F2C_ERR_LIMIT,
+              "%s: more than 2^30 ids, 2^31 - 2 rows, 2^20 columns or 2^33 pieces of 128 columns", op);
+  return F2C_OK;
+}
+
+}  // namespace emb
+}  // namespace f2c
+
+using namespace f2c;
+
+extern "C" int f2c_embedding(const void* table, int64_t ld, int dtype, int64_t rows, int64_t d, const void* ids, int index_dtype, int64_t m, float scale, void* out, void* stream) {
+  const char* op = "embedding";
+  if (const int rc = emb::check(op, dtype, index_dtype, m, rows, d)) return rc;
+  if (m == 0 || d == 0) return F2C_OK;
+  F2C_REQUIRE((table || rows == 0) && ids && out, F2C_ERR_INVALID, "%s: null pointer", op);
+  F2C_REQUIRE(rows <= 1 || ld >= d, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool wide = index_dtype == F2C_I64;
+  if (dtype == F2C_F32) (wide ? emb::lookup<float, int64_t> : emb::lookup<float, int32_t>)(table, ld, rows, d, ids, m, scale, out, st);
+  else if (dtype == F2C_F16) (wide ? emb::lookup<__half, int64_t> : emb::lookup<__half, int32_t>)(table, ld, rows, d, ids, m, scale, out, st);
+  else (wide ? emb::lookup<__nv_bfloat16, int64_t> : emb::lookup<__nv_bfloat16, int32_t>)(table, ld, rows, d, ids, m, scale, out, st);
+  return check_launch(op);
+}
+
+extern "C" int64_t f2c_embedding_backward_workspace(int64_t m, int64_t rows, int64_t d) {
+  if (m <= 0 || rows < 0 || d <= 0 || m > emb::kMaxPlaces || rows > emb::kMaxRows || d > emb::kMaxColumns) return 0;
+  return emb::plan(m, rows, d).bytes;
+}
+
+extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, const void* ids, int index_dtype, int64_t m, int64_t rows, int64_t d, float scale, void* grad,
+                                      int64_t* looked_up, int64_t* count, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* op = "embedding_backward";
+  if (const int rc = emb::check(op, dtype, index_dtype, m, rows, d)) return rc;
+  const bool dense = count == nullptr;
+  cudaStream_t st = (cudaStream_t)stream;
+  F2C_REQUIRE(dense || looked_up || m == 0, F2C_ERR_INVALID, "%s: null pointer", op);
+  if (dense && rows > 0 && d > 0) {
+    F2C_REQUIRE(grad, F2C_ERR_INVALID, "%s: null pointer", op);
+    F2C_REQUIRE(rows * d <= 1ll << 40, F2C_ERR_LIMIT, "%s: more than 2^40 values", op);
+  }
+  if (m > 0 && d > 0) {
+    F2C_REQUIRE(dy && ids && (grad || (dense && rows == 0)), F2C_ERR_INVALID, "%s: null pointer", op);
+    F2C_REQUIRE(m == 1 || ldy >= d, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
+    const int64_t need = f2c_embedding_backward_workspace(m, rows, d);
+    F2C_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 256), F2C_ERR_INVALID, "%s: the workspace must have %lld bytes, 256-byte aligned", op, (long long)need);
+  }
+  if (dense && rows > 0 && d > 0) {
+    const cudaError_t e = cudaMemsetAsync(grad, 0, (size_t)(rows * d * dtype_size(dtype)), st);
+    if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  }
+  if (!dense && (m == 0 || d == 0)) {
+    cudaError_t e = cudaMemsetAsync(count, 0, 8, st);
+    if (e == cudaSuccess && m > 0) e = cudaMemsetAsync(looked_up, 0xff, (size_t)m * 8, st);
+    if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  }
+  if (m == 0 || d == 0 || (dense && rows == 0)) return F2C_OK;
+  char* const ws = (char*)workspace;
+  const emb::Plan p = emb::plan(m, rows, d);
+  const emb::Pairs sorted = index_dtype == F2C_I64 ? emb::sort(p, (const int64_t*)ids, (uint32_t)rows, ws, st) : emb::sort(p, (const int32_t*)ids, (uint32_t)rows, ws, st);
+  uint32_t *const in_tile = (uint32_t*)(ws + p.in_tile), *const of_tile = (uint32_t*)(ws + p.of_tile);
+  if (!dense)
+    launch_dependent(emb::number_kernel, dim3((unsigned)p.tiles), emb::kThreads, 0, st, (const uint32_t*)sorted.key, m, (uint32_t)rows, p.stretch, in_tile, of_tile, looked_up);
+  const emb::Segments s{sorted.key, sorted.place, m, (uint32_t)rows, p.stretch, p.stretches, in_tile, of_tile, p.tiles, dense ? nullptr : looked_up, count};
+  const emb::Open open{(float*)(ws + p.head), (float*)(ws + p.tail), (int64_t*)(ws + p.row), p.width};
+  const int item = dtype_size(dtype), from = ckpt::access_of(dy, ldy, m, d, item), to = ckpt::access_of(grad, d, dense ? rows : m, d, item);
+  F2C_BY_ROWS(emb::add_up, dtype, (from < to ? from : to), p, dy, ldy, scale, s, open, grad, st);
+  return check_launch(op);
+}

@@ -198,12 +198,78 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {  //
   });
 }
 
+// Ids of any shape, without gaps; the dtype is checked.
+const at::Tensor& ids_of(PyObject* o, const at::Tensor& other) {
+  const at::Tensor& ids = tensor(o, "ids", kIndex);
+  same_device(ids, other, "ids");
+  return ids;
+}
+
+PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {  // table, ids, scale
+  return guarded([&]() -> PyObject* {
+    arguments("embedding", n, 3);
+    const at::Tensor& table = matrix(a[0], "table", kFloats);
+    no_gradient(table, "embedding", "table");
+    const at::Tensor& ids = ids_of(a[1], table);
+    const double scale = real(a[2]);
+    at::Tensor out;
+    check_status(unlocked([&] {
+      c10::cuda::CUDAGuard guard(table.device());
+      c10::DimVector shape(ids.sizes());
+      shape.push_back(table.size(1));
+      out = empty(shape, table.scalar_type(), table.device());
+      return f2c_embedding(table.const_data_ptr(), row_stride(table), dtype_tag(table.scalar_type()), table.size(0), table.size(1), ids.const_data_ptr(),
+                           dtype_tag(ids.scalar_type()), ids.numel(), (float)scale, out.mutable_data_ptr(), stream_of(table));
+    }));
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// dy, ids, n_rows, scale, whether only the rows that were looked up -> the table's gradient; or looked_up, rows, count
+PyObject* embedding_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const char* op = "embedding_backward";
+    arguments(op, n, 5);
+    if (!THPVariable_Check(a[0])) fail(PyExc_TypeError, "dy must be a torch.Tensor");
+    const at::Tensor& given = THPVariable_Unpack(a[0]);
+    // (a matrix may have its rows further apart)
+    const at::Tensor& dy = given.dim() == 2 ? matrix(a[0], "dy", kFloats) : tensor(a[0], "dy", kFloats);
+    no_gradient(dy, op, "dy");
+    const at::Tensor& ids = ids_of(a[1], dy);
+    const int64_t rows = integer(a[2]);
+    const double scale = real(a[3]);
+    const bool sparse = truth(a[4]);
+    if (dy.dim() != ids.dim() + 1 || dy.sizes().slice(0, ids.dim()) != ids.sizes()) fail(PyExc_RuntimeError, "dy must be a row for every id");
+    if (rows < 0) fail(PyExc_RuntimeError, "n_rows must not be negative");
+    const int64_t m = ids.numel(), d = dy.size(-1);
+    at::Tensor grad, looked_up, count;
+    check_status(unlocked([&] {
+      c10::cuda::CUDAGuard guard(dy.device());
+      grad = empty({sparse ? m : rows, d}, dy.scalar_type(), dy.device());
+      if (sparse) {
+        looked_up = empty({m}, at::kLong, dy.device());
+        count = empty({1}, at::kLong, dy.device());
+      }
+      const int64_t bytes = f2c_embedding_backward_workspace(m, rows, d);
+      at::Tensor ws;
+      if (bytes > 0) ws = empty({bytes}, at::kByte, dy.device());
+      return f2c_embedding_backward(dy.const_data_ptr(), dy.dim() == 2 ? row_stride(dy) : d, dtype_tag(dy.scalar_type()), ids.const_data_ptr(), dtype_tag(ids.scalar_type()), m, rows,
+                                    d, (float)scale, grad.mutable_data_ptr(), sparse ? looked_up.mutable_data_ptr<int64_t>() : nullptr,
+                                    sparse ? count.mutable_data_ptr<int64_t>() : nullptr, bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(dy));
+    }));
+    if (!sparse) return THPVariable_Wrap(std::move(grad));
+    return tuple_of(std::move(looked_up), std::move(grad), std::move(count));
+  });
+}
+
 }  // namespace
 
 PyMethodDef g_learn_methods[] = {{"checkpoint_int8", (PyCFunction)(void*)checkpoint_int8, METH_FASTCALL, nullptr},
                                  {"checkpoint_values", (PyCFunction)(void*)checkpoint_values, METH_FASTCALL, nullptr},
                                  {"layer_norm", (PyCFunction)(void*)layer_norm, METH_FASTCALL, nullptr},
                                  {"layer_norm_backward", (PyCFunction)(void*)layer_norm_backward, METH_FASTCALL, nullptr},
+                                 {"embedding", (PyCFunction)(void*)embedding, METH_FASTCALL, nullptr},
+                                 {"embedding_backward", (PyCFunction)(void*)embedding_backward, METH_FASTCALL, nullptr},
                                  {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace f2c_native

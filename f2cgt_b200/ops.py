@@ -411,6 +411,28 @@ def layer_norm_backward(dy, saved, weight=None):
     return _native.layer_norm_backward(dy, x, scales, saved.mean, saved.rstd, saved.active, weight)
 
 
+# ------------------------------------------------------------------ learned rows
+def embedding(table, ids, scale=1.0):
+    """``scale * table[ids]``, rounded once: rows of ``table`` [rows, cols] (float32 / float16 / bfloat16) for ``ids`` of any shape (int32 / int64).  An
+    id outside the table - the -1 that pads a batch - is a row of zeros.  It has no gradient by itself: see ``embedding_backward``;
+    ``sage.NodeEmbedding`` is the module over them."""
+    return _native.embedding(table, ids, scale)
+
+
+def embedding_backward(grad_out, ids, n_rows, scale=1.0):
+    """Gradient of ``embedding(table, ids, scale)`` with respect to a table of ``n_rows`` rows, in the dtype of ``grad_out`` [*ids.shape, cols]: row r is
+    ``scale`` times the sum over the places where r was looked up, zero where it was not.  The places are sorted by id and summed in single precision, in the
+    same order every time (no atomics)."""
+    return _native.embedding_backward(grad_out, ids, n_rows, scale, False)
+
+
+def embedding_backward_rows(grad_out, ids, n_rows, scale=1.0):
+    """``embedding_backward`` for a table that is much larger than what is looked up: ``(looked_up, rows, count)`` with the distinct ids in
+    ascending order (int64 [n], n the number of ids; -1 behind them), their rows of the gradient [n, cols] (zeros behind them), and how many there are
+    (int64 [1]).  Nothing is read back to the host."""
+    return _native.embedding_backward(grad_out, ids, n_rows, scale, True)
+
+
 # ------------------------------------------------------------------ k-means
 def pairwise_distance(x, y, metric):
     """src/kmeans.cu:102-118.  x [n,d], y [k,d] fp32 -> [n,k] squared-L2 or cosine distance."""

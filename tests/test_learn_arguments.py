@@ -45,3 +45,31 @@ def test_workspaces_of_the_norms_gradient():
     assert lib.f2c_layer_norm_backward_workspace(0, 128) == 0 and lib.f2c_layer_norm_backward_workspace(10, 0) == 0
     assert lib.f2c_layer_norm_backward_workspace(8, 128) == 1024  # one CTA's two sums of 128 columns
     assert lib.f2c_layer_norm_backward_workspace(1 << 20, 128) >= 148 * 1024
+
+
+def lookup(table=AT, ld=8, dtype=_lib.F32, rows=10, d=8, ids=AT, index=_lib.I64, m=4, out=AT):
+    return lib.f2c_embedding(table, ld, dtype, rows, d, ids, index, m, 1.0, out, None)
+
+
+def rows_gradient(dy=AT, ldy=8, dtype=_lib.F32, ids=AT, index=_lib.I64, m=4, rows=10, d=8, grad=AT, looked_up=AT, count=AT, work=AT, size=1 << 40):
+    return lib.f2c_embedding_backward(dy, ldy, dtype, ids, index, m, rows, d, 1.0, grad, looked_up, count, work, size, None)
+
+
+@pytest.mark.parametrize("call,status", [
+    (lambda: lookup(dtype=_lib.F64), UNSUPPORTED), (lambda: lookup(index=_lib.I16), UNSUPPORTED), (lambda: lookup(m=-1), INVALID), (lambda: lookup(rows=1 << 31), LIMIT),
+    (lambda: lookup(m=(1 << 30) + 1), LIMIT), (lambda: lookup(m=1 << 30, d=1 << 12, ld=1 << 12), LIMIT), (lambda: lookup(d=(1 << 20) + 1, ld=1 << 21), LIMIT), (lambda: lookup(ld=7), INVALID), (lambda: lookup(table=0), INVALID),
+    (lambda: lookup(ids=0), INVALID), (lambda: lookup(out=0), INVALID), (lambda: lookup(m=0, ids=0, out=0), OK), (lambda: lookup(d=0, out=0), OK),
+    (lambda: rows_gradient(dtype=_lib.I8), UNSUPPORTED), (lambda: rows_gradient(index=_lib.U8), UNSUPPORTED), (lambda: rows_gradient(d=-1), INVALID), (lambda: rows_gradient(dy=0), INVALID),
+    (lambda: rows_gradient(ids=0), INVALID), (lambda: rows_gradient(grad=0), INVALID), (lambda: rows_gradient(looked_up=0), INVALID), (lambda: rows_gradient(ldy=7), INVALID),
+    (lambda: rows_gradient(work=0), INVALID), (lambda: rows_gradient(work=AT + 8), INVALID), (lambda: rows_gradient(size=1000), INVALID),
+    (lambda: rows_gradient(count=0, looked_up=0, rows=1 << 25, d=1 << 20, ldy=1 << 20, m=1), LIMIT), (lambda: rows_gradient(count=0, grad=0), INVALID),
+    (lambda: rows_gradient(count=0, rows=0, m=0, dy=0, ids=0, work=0, grad=0), OK)])
+def test_learned_rows(call, status):
+    assert call() == status
+    assert status == OK or b"embedding" in lib.f2c_last_error()
+
+
+def test_workspaces_of_learned_rows():
+    few, many, large = (lib.f2c_embedding_backward_workspace(m, rows, 128) for m, rows in ((100, 1000), (100_000, 1000), (100_000, 1 << 30)))
+    assert 0 < few < many < large and lib.f2c_embedding_backward_workspace(0, 10, 10) == 0
+    assert many < 100_000 * 128 * 4  # less than the rows themselves
