@@ -121,6 +121,8 @@ SIGNATURES = {
     "f2c_muon_step": [C.POINTER(MuonMatrix), ci, ci, f32, f32, ci, f32, p, ci, f32, p, i64, p],
     "f2c_checkpoint_int8": [p, i64, ci, i64, i64, p, i64, p, p],
     "f2c_checkpoint_values": [p, i64, p, i64, i64, p, i64, ci, p],
+    "f2c_checkpoint_weight_grad_workspace": [i64, i64, i64],
+    "f2c_checkpoint_weight_grad": [p, i64, ci, p, i64, p, i64, i64, i64, p, p, ci, p, i64, p],
     "f2c_layer_norm": [p, i64, ci, i64, i64, p, p, f32, ci, p, p, p, p, p, i64, p, p],
     "f2c_layer_norm_backward_workspace": [i64, i64],
     "f2c_layer_norm_backward": [p, i64, ci, p, i64, p, i64, p, p, p, p, p, i64, i64, p, p, p, p, i64, p],
@@ -132,7 +134,7 @@ SIGNATURES = {
 }
 _RESTYPE = {"f2c_last_error": C.c_char_p, "f2c_kmeans_assign_workspace": C.c_int64, "f2c_kmeans_fit_workspace": C.c_int64, "f2c_sq_statistics_workspace": C.c_int64,
             "f2c_relabel_capacity": C.c_int64, "f2c_int8_mm_workspace": C.c_int64, "f2c_int8_linear_workspace": C.c_int64,
-            "f2c_layer_norm_backward_workspace": C.c_int64, "f2c_embedding_backward_workspace": C.c_int64,
+            "f2c_checkpoint_weight_grad_workspace": C.c_int64, "f2c_layer_norm_backward_workspace": C.c_int64, "f2c_embedding_backward_workspace": C.c_int64,
             "f2c_orthogonalize_workspace": C.c_int64, "f2c_muon_workspace": C.c_int64,
             "f2c_sample_block_workspace": C.c_int64, "f2c_sample_minibatch_workspace": C.c_int64, "f2c_peer_hot_first_cold_id": C.c_int64}
 

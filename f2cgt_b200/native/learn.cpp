@@ -118,6 +118,31 @@ PyObject* checkpoint_values(PyObject*, PyObject* const* a, Py_ssize_t n) {  // c
   });
 }
 
+PyObject* checkpoint_weight_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {  // dy, codes, scales -> dw, db
+  return guarded([&]() -> PyObject* {
+    const char* op = "checkpoint_weight_grad";
+    arguments(op, n, 3);
+    const at::Tensor& dy = matrix(a[0], "dy", kFloats);
+    no_gradient(dy, op, "dy");
+    const Codes c = codes_of(a[1], a[2], op);
+    same_device(*c.codes, dy, "codes");
+    const int64_t m = dy.size(0), cols = dy.size(1), k = c.codes->size(1);
+    if (c.codes->size(0) != m) fail(PyExc_RuntimeError, "dy must have as many rows as the input that was kept");
+    at::Tensor dw, db;
+    check_status(unlocked([&] {
+      c10::cuda::CUDAGuard guard(dy.device());
+      dw = empty({cols, k}, dy.scalar_type(), dy.device());
+      db = empty({cols}, dy.scalar_type(), dy.device());
+      const int64_t bytes = f2c_checkpoint_weight_grad_workspace(m, cols, k);
+      at::Tensor ws;
+      if (bytes > 0) ws = empty({bytes}, at::kByte, dy.device());
+      return f2c_checkpoint_weight_grad(dy.const_data_ptr(), row_stride(dy), dtype_tag(dy.scalar_type()), c.q(), c.ld, c.s(), m, cols, k, dw.mutable_data_ptr(), db.mutable_data_ptr(), 0,
+                                        bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(dy));
+    }));
+    return tuple_of(std::move(dw), std::move(db));
+  });
+}
+
 // x, weight, bias, eps, relu, keep (0: nothing, 1: what goes with the rows, 2: and the rows in 8 bits)
 // -> y, mean, rstd, active, codes, scales (None: not wanted)
 PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -266,6 +291,7 @@ PyObject* embedding_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef g_learn_methods[] = {{"checkpoint_int8", (PyCFunction)(void*)checkpoint_int8, METH_FASTCALL, nullptr},
                                  {"checkpoint_values", (PyCFunction)(void*)checkpoint_values, METH_FASTCALL, nullptr},
+                                 {"checkpoint_weight_grad", (PyCFunction)(void*)checkpoint_weight_grad, METH_FASTCALL, nullptr},
                                  {"layer_norm", (PyCFunction)(void*)layer_norm, METH_FASTCALL, nullptr},
                                  {"layer_norm_backward", (PyCFunction)(void*)layer_norm_backward, METH_FASTCALL, nullptr},
                                  {"embedding", (PyCFunction)(void*)embedding, METH_FASTCALL, nullptr},

@@ -389,6 +389,13 @@ def checkpoint_values(checkpoint, dtype=torch.float32):
     return _native.checkpoint_values(checkpoint[0], checkpoint[1], dtype)
 
 
+def checkpoint_weight_grad(dy, checkpoint):
+    """``(dweight, dbias)`` of a linear layer ``y = x @ weight.T + bias`` whose input was kept as an ``Int8Checkpoint``: ``dy.T @ x`` and the sums of
+    ``dy``'s columns, in the dtype of ``dy`` [rows, n] (float32 / float16 / bfloat16), without writing ``x`` out.  On the tensor cores; ``dy`` times a step is
+    held to 24 bits (float32) or 16, sums are single precision in an order that the sizes alone decide."""
+    return _native.checkpoint_weight_grad(dy, checkpoint[0], checkpoint[1])
+
+
 def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over every row of ``x`` [rows, cols] (float32 / float16 / bfloat16), then ReLU if asked for;
     ``weight`` and ``bias`` float32 [cols] or None.  Statistics are single precision, the result is rounded once.  It has no gradient by itself:

@@ -48,7 +48,8 @@ typedef enum { F2C_L2 = 0, F2C_COSINE = 1 } f2c_metric;  /* src/kmeans.cu:16-22,
 /* For tests of what follows a bounded wait that has run out: all those of the call's tensor-core kernels run out, at once or (Newton-Schulz
  * products of matrices that one SM does not hold) after about a second.
  * f2c_kmeans_assign and f2c_kmeans_fit_iterate (in `metric`): same results.  f2c_int8_mm and f2c_int8_linear (in `relu`),
- * f2c_orthogonalize and f2c_muon_step (in `steps`): results of NaN and a device status, where such kernels are used. */
+ * f2c_orthogonalize and f2c_muon_step (in `steps`), f2c_checkpoint_weight_grad (in `flags`): results of NaN and a device status, where such kernels
+ * are used. */
 #define F2C_NO_WAITS 0x400
 
 typedef enum {
@@ -462,6 +463,14 @@ int f2c_muon_step(const f2c_muon_matrix* list_host, int count, int dtype, float 
 int f2c_checkpoint_int8(const void* x, int64_t ldx, int dtype, int64_t m, int64_t d, uint8_t* codes, int64_t ldq, float* scales, void* stream);
 int f2c_checkpoint_values(const uint8_t* codes, int64_t ldq, const float* scales, int64_t m, int64_t d, void* out, int64_t ldo, int out_dtype,
                           void* stream);
+/* Gradient of a linear layer y = x W^T + b from dy [m, n] (`dtype`: F32, F16 or BF16, row stride ldy) and x [m, k] in 8 bits:
+ *   dw [n, k] = dy^T x,  db [n] = the sums of dy's columns, both of `dtype`, rounded once; x is not written out.
+ * dy times a code's step is held to 24 bits for F32 and to 16 for the others, sums are single precision in an order that the sizes decide.
+ * Codes as f2c_checkpoint_int8 leaves them (every row has whole 16 bytes).  m < 2^31, n and k up to 2^17.  flags: 0, or F2C_NO_WAITS.
+ * workspace: f2c_checkpoint_weight_grad_workspace(m, n, k) bytes, 256-byte aligned.  A bounded wait that runs out reports 8 and leaves NaN. */
+int64_t f2c_checkpoint_weight_grad_workspace(int64_t m, int64_t n, int64_t k);
+int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype, const uint8_t* codes, int64_t ldq, const float* scales, int64_t m, int64_t n, int64_t k,
+                               void* dw, void* db, int flags, void* workspace, int64_t workspace_bytes, void* stream);
 /* y [m, d] = (x - mean) rstd weight + bias of every row, rstd = 1 / sqrt(mean((x - mean)^2) + eps); relu != 0: negative values become 0 (a NaN
  * stays one).  x and y of `dtype`, everything else float; weight, bias [d] or NULL (1, 0).  Wanted for the backward pass, or NULL: mean and
  * rstd [m]; active [m, ceil(d / 8)]: bit c % 8 of byte c / 8 says that y was positive before rounding (bits behind the columns are 0); codes and

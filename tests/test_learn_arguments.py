@@ -73,3 +73,23 @@ def test_workspaces_of_learned_rows():
     few, many, large = (lib.f2c_embedding_backward_workspace(m, rows, 128) for m, rows in ((100, 1000), (100_000, 1000), (100_000, 1 << 30)))
     assert 0 < few < many < large and lib.f2c_embedding_backward_workspace(0, 10, 10) == 0
     assert many < 100_000 * 128 * 4  # less than the rows themselves
+
+
+def weights(dy=AT, ldy=8, dtype=_lib.F32, codes=AT, ldq=48, scales=AT, m=4, n=8, k=40, dw=AT, db=AT, flags=0, work=AT, size=1 << 40):
+    return lib.f2c_checkpoint_weight_grad(dy, ldy, dtype, codes, ldq, scales, m, n, k, dw, db, flags, work, size, None)
+
+
+@pytest.mark.parametrize("call,status", [
+    (lambda: weights(dtype=_lib.F64), UNSUPPORTED), (lambda: weights(n=-1), INVALID), (lambda: weights(m=1 << 31), LIMIT), (lambda: weights(n=(1 << 17) + 1, ldy=1 << 18), LIMIT),
+    (lambda: weights(k=(1 << 17) + 1, ldq=1 << 18), LIMIT), (lambda: weights(flags=1), INVALID), (lambda: weights(codes=AT + 8), INVALID), (lambda: weights(ldq=40), INVALID), (lambda: weights(scales=0), INVALID),
+    (lambda: weights(dy=0), INVALID), (lambda: weights(dw=0), INVALID), (lambda: weights(db=0), INVALID), (lambda: weights(ldy=7), INVALID), (lambda: weights(k=0), INVALID),
+    (lambda: weights(m=10000, work=0), INVALID), (lambda: weights(m=10000, work=AT + 64), INVALID), (lambda: weights(m=10000, size=1 << 16), INVALID), (lambda: weights(n=0, dw=0, db=0), OK)])
+def test_weight_gradients(call, status):
+    assert call() == status
+    assert status == OK or b"checkpoint_weight_grad" in lib.f2c_last_error()
+
+
+def test_workspaces_of_weight_gradients():
+    size = lib.f2c_checkpoint_weight_grad_workspace
+    assert size(0, 8, 8) == size(8, 0, 8) == size(32, 128, 128) == 0  # one part
+    assert size(59_000, 128, 128) % (65536 + 512) == 0 and size(16_384, 4096, 4096) == 0
