@@ -11,6 +11,8 @@
   ``spmm_csr`` with a backward pass over the transposed block.
 * ``SAGE`` - examples/models.py:10-42: ReLU + dropout between layers.
 * ``Int8SAGE`` - a trained network answering in 8-bit integers.
+* ``LayerNorm``, ``NodeEmbedding`` - norm between layers and learned rows for nodes, as modules over ``ops``; ``SAGE`` takes both, and keeps
+  its activations in 8 bits until the backward pass where it is asked to.
 * ``GPUSamplingDataloader`` - examples/dataloader.py:154-192: per minibatch, hops in reversed(fan_out) order from the
   seeds with ``csr_sampling`` + ``tensor_relabel``; yields (input_nodes, output_nodes, blocks).
 
@@ -20,6 +22,7 @@ source nodes.
 """
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -274,6 +277,130 @@ class _SageLayer(torch.autograd.Function):
         return dh, None, None, None, None, dw_self, dw_neigh, db
 
 
+class _SageProduct8(torch.autograd.Function):
+    """``_SageProduct`` that keeps its inputs in 8 bits: the weights' gradients are those of the values that the codes stand for."""
+
+    @staticmethod
+    def forward(ctx, x_self, x_neigh, w_self, w_neigh, bias):
+        ctx.save_for_backward(*ops.checkpoint_int8(x_self), *ops.checkpoint_int8(x_neigh))
+        ctx.has_bias = bias is not None
+        return _addmm_(_affine(bias, x_self, w_self.t()), x_neigh, w_neigh.t())
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        kept, dy = ctx.saved_tensors, dy.contiguous()
+        dw_self, db = ops.checkpoint_weight_grad(dy, kept[:2])
+        return None, None, dw_self, ops.checkpoint_weight_grad(dy, kept[2:])[0], db if ctx.has_bias else None
+
+
+class _SageLayer8(torch.autograd.Function):
+    """``_SageLayer`` that keeps its own rows and their neighbours' means in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, h, indptr, indices, n_dst, m, w_self, w_neigh, bias):
+        neigh = ops.spmm_csr(h, indptr, indices, out_rows=m)
+        h_self = h[:m]
+        y = _addmm_(_affine(bias, h_self, w_self.t()), neigh, w_neigh.t())
+        ctx.save_for_backward(*ops.checkpoint_int8(h_self), *ops.checkpoint_int8(neigh), indptr, indices, w_self, w_neigh)
+        ctx.n_dst, ctx.m, ctx.n_src, ctx.has_bias = n_dst, m, h.shape[0], bias is not None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        kept, (indptr, indices, w_self, w_neigh), dy = ctx.saved_tensors[:4], ctx.saved_tensors[4:], dy.contiguous()
+        dw_self, db = ops.checkpoint_weight_grad(dy, kept[:2])
+        dw_neigh = ops.checkpoint_weight_grad(dy, kept[2:])[0]
+        dh = None
+        if ctx.needs_input_grad[0]:
+            dh = ops.spmm_csr_backward(_mm(dy, w_neigh)[:ctx.n_dst], indptr, indices, ctx.n_src)
+            _addmm_(dh[:ctx.m], dy, w_self)
+        return dh, None, None, None, None, dw_self, dw_neigh, db if ctx.has_bias else None
+
+
+class _ReluBits(torch.autograd.Function):
+    """ReLU that keeps a byte a value instead of its result."""
+
+    @staticmethod
+    def forward(ctx, x):
+        y = torch.relu(x)
+        ctx.save_for_backward(y > 0)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        return dy * ctx.saved_tensors[0]
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, relu, int8):
+        y, saved = ops.layer_norm_train(x, weight, bias, eps, relu, int8)
+        ctx.int8 = int8
+        ctx.save_for_backward(*(saved.x if int8 else (saved.x, None)), saved.mean, saved.rstd, saved.active, weight)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, scales, mean, rstd, active, weight = ctx.saved_tensors
+        saved = ops.NormSaved(ops.Int8Checkpoint(x, scales) if ctx.int8 else x, mean, rstd, active)
+        dx, dweight, dbias = ops.layer_norm_backward(dy.contiguous(), saved, weight)
+        need = ctx.needs_input_grad
+        return dx if need[0] else None, dweight if need[1] else None, dbias if need[2] else None, None, None, None
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over the rows of [rows, columns] (``ops.layer_norm``), followed by ReLU with ``relu=True``; with ``int8=True`` its input is kept
+    in 8 bits for the backward pass.  Weight and bias are float32; rows float32, float16 or bfloat16.  Differentiable once."""
+
+    def __init__(self, columns, eps=1e-5, relu=False, int8=False):
+        super().__init__()
+        self.weight, self.bias = nn.Parameter(torch.ones(columns)), nn.Parameter(torch.zeros(columns))
+        self.eps, self.relu, self.int8 = float(eps), bool(relu), bool(int8)
+
+    def forward(self, x):
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or self.bias.requires_grad):
+            return _LayerNorm.apply(x, self.weight, self.bias, self.eps, self.relu, self.int8)
+        return ops.layer_norm(x, self.weight, self.bias, self.eps, self.relu)
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale, sparse):
+        ctx.save_for_backward(ids)
+        ctx.shape, ctx.scale, ctx.sparse = table.shape, scale, sparse
+        return ops.embedding(table, ids, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        dy, n_rows = dy.contiguous(), ctx.shape[0]
+        if not ctx.sparse:
+            return ops.embedding_backward(dy, ids, n_rows, ctx.scale), None, None, None
+        looked_up, rows, count = ops.embedding_backward_rows(dy, ids, n_rows, ctx.scale)
+        count = int(count)  # the one host read: a sparse tensor's size is the host's
+        return torch.sparse_coo_tensor(looked_up[None, :count], rows[:count], ctx.shape, is_coalesced=True, check_invariants=False), None, None, None
+
+
+class NodeEmbedding(nn.Module):
+    """A learned row for every node: ``scale * weight[ids]`` (``ops.embedding``), zeros for ids outside the table.  The table's gradient is dense, or with
+    ``sparse=True`` a sparse tensor of the rows that were looked up, each once, as ``torch.optim.SparseAdam`` and ``SGD`` take it.  Differentiable once."""
+
+    def __init__(self, n_nodes, columns, scale=1.0, sparse=False, device=None, dtype=None):
+        super().__init__()
+        self.weight = nn.Parameter(torch.empty((n_nodes, columns), device=device, dtype=dtype))
+        nn.init.normal_(self.weight)
+        self.scale, self.sparse = float(scale), bool(sparse)
+
+    def forward(self, ids):
+        if torch.is_grad_enabled() and self.weight.requires_grad:
+            return _Embedding.apply(self.weight, ids, self.scale, self.sparse)
+        return ops.embedding(self.weight, ids, self.scale)
+
+
 class _MeanAggregate(torch.autograd.Function):
     """out[d] = mean over the block's neighbours of h[src]; backward adds grad / deg to every neighbour's row."""
 
@@ -290,8 +417,11 @@ class _MeanAggregate(torch.autograd.Function):
 
 
 class MySAGEConv(nn.Module):
-    def __init__(self, in_feats, out_feats, compression_manager, bias=True):
+    int8 = False
+
+    def __init__(self, in_feats, out_feats, compression_manager, bias=True, int8=False):
         super().__init__()
+        self.int8 = bool(int8)  # keep the inputs in 8 bits until the backward pass
         self.fc_neigh = nn.Linear(in_feats, out_feats, bias=False)
         self.fc_self = nn.Linear(in_feats, out_feats, bias=bias)
         self.sm = compression_manager
@@ -307,15 +437,18 @@ class MySAGEConv(nn.Module):
         m = _bucket(dst.numel())
         h_neigh = sm.aggregate(block["indptr"], neighbours, out_rows=m)  # raw codes in, no autograd through it
         h_self = sm.decode_rows(dst, out_rows=m)
-        return _SageProduct.apply(h_self, h_neigh, self.fc_self.weight, self.fc_neigh.weight, self.fc_self.bias)
+        return (_SageProduct8 if self.int8 else _SageProduct).apply(h_self, h_neigh, self.fc_self.weight, self.fc_neigh.weight, self.fc_self.bias)
 
     def forward(self, block, _unused=None):
         return self.forward_padded(block)[:block["dst_nodes"].numel()]
 
 
 class SAGEConv(nn.Module):
-    def __init__(self, in_feats, out_feats, bias=True):
+    int8 = False
+
+    def __init__(self, in_feats, out_feats, bias=True, int8=False):
         super().__init__()
+        self.int8 = bool(int8)
         self.fc_neigh = nn.Linear(in_feats, out_feats, bias=False)
         self.fc_self = nn.Linear(in_feats, out_feats, bias=bias)
         gain = nn.init.calculate_gain("relu")
@@ -328,32 +461,49 @@ class SAGEConv(nn.Module):
         n_dst = block["dst_nodes"].numel()
         h = h.float().contiguous()
         m = min(_bucket(n_dst), h.shape[0])
-        return _SageLayer.apply(h, block["indptr"], block["indices_local"], n_dst, m, self.fc_self.weight, self.fc_neigh.weight,
-                                self.fc_self.bias)
+        return (_SageLayer8 if self.int8 else _SageLayer).apply(h, block["indptr"], block["indices_local"], n_dst, m, self.fc_self.weight,
+                                                                self.fc_neigh.weight, self.fc_self.bias)
 
     def forward(self, block, h):
         return self.forward_padded(block, h)[:block["dst_nodes"].numel()]
 
 
 class SAGE(nn.Module):
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, dropout, cm):
+    """``norm``: layer norm in front of every ReLU.  ``activations="int8"``: what the layers, norms and ReLUs keep for the backward pass is in 8 bits or
+    less (dropout keeps its bytes); gradients are those of the kept values.  ``embedding``: a ``NodeEmbedding`` of ``in_feats`` columns whose rows are the
+    first layer's input in place of decoded features (``cm`` is None then)."""
+    int8 = False
+
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, dropout, cm, norm=False, activations="float", embedding=None):
         super().__init__()
+        if activations not in ("float", "int8"):
+            raise ValueError("activations must be float or int8")
+        if embedding is not None and (cm is not None or embedding.weight.shape[1] != in_feats):
+            raise ValueError("learned rows have in_feats columns and stand in place of the compressed features")
+        int8 = activations == "int8"
         self.layers = nn.ModuleList()
         for i in range(n_layers):
             in_dim = in_feats if i == 0 else n_hidden
             out_dim = n_classes if i == n_layers - 1 else n_hidden
-            self.layers.append(MySAGEConv(in_dim, out_dim, cm) if i == 0 else SAGEConv(in_dim, out_dim))
+            self.layers.append(MySAGEConv(in_dim, out_dim, cm, int8=int8) if i == 0 and embedding is None else SAGEConv(in_dim, out_dim, int8=int8))
         self.dropout = nn.Dropout(dropout)
+        if int8:
+            self.int8 = True
+        if norm:
+            self.norms = nn.ModuleList(LayerNorm(n_hidden, relu=True, int8=int8) for _ in range(n_layers - 1))
+        if embedding is not None:
+            self.embedding = embedding
 
     def forward(self, blocks, x=None):
         weights = self._plain_weights() if x is None and len(blocks) == len(self.layers) else None
         if weights is not None:
             return self._forward_as_one_node(blocks, weights)
-        h = x
+        norms, embedding = self._modules.get("norms"), self._modules.get("embedding")  # (not there unless asked for)
+        h = x if embedding is None else embedding(blocks[0]["src_nodes"])
         for i, (layer, block) in enumerate(zip(self.layers, blocks)):
             h = layer.forward_padded(block, h)
             if i != len(self.layers) - 1:
-                h = self.dropout(torch.relu(h))
+                h = self.dropout(norms[i](h) if norms is not None else _ReluBits.apply(h) if self.int8 else torch.relu(h))
         n_out = blocks[-1]["dst_nodes"].numel()
         return h if h.shape[0] == n_out else h[:n_out]
 
@@ -361,13 +511,15 @@ class SAGE(nn.Module):
         """[self, neigh, bias] of every layer, or None when the layers are not just these tensors (subclasses, hooks - those of
         all modules too -, parametrisations, other dtypes, autocast, forward-mode derivatives): then every layer is called on its
         own."""
+        if "norms" in self._modules or "embedding" in self._modules or self.int8:
+            return None
         if torch.is_autocast_enabled("cuda") or type(self.dropout) is not nn.Dropout or self.dropout.inplace or _hooked(self.dropout):
             return None
         if nn.modules.module._has_any_global_hook() or torch.autograd.forward_ad._current_level >= 0:
             return None
         weights = []
         for i, layer in enumerate(self.layers._modules.values()):
-            if type(layer) is not (SAGEConv if i else MySAGEConv) or _hooked(layer):
+            if type(layer) is not (SAGEConv if i else MySAGEConv) or _hooked(layer) or layer.int8:
                 return None
             parts = layer._modules
             fc_self, fc_neigh = parts["fc_self"], parts["fc_neigh"]
@@ -403,20 +555,25 @@ class SAGE(nn.Module):
 
 class Int8SAGE:
     """A trained ``SAGE`` network that answers in 8-bit integers: every layer is one product of its rows, own and neighbours' mean side by side,
-    with ``fc_self | fc_neigh`` (``ops.int8_linear``), the weights quantised once, per output channel.  Aggregation, decoding and the hidden
+    with ``fc_self | fc_neigh`` (``ops.int8_linear``), the weights quantised once, per output channel.  Aggregation, decoding, norms and the hidden
     rows are as in the float network; there is no dropout and no gradient.
 
         answer = sage.Int8SAGE(model)(blocks)
     """
 
     def __init__(self, model):
-        self.first_input = model.layers[0].sm
-        self.layers = []
+        norms, embedding = model._modules.get("norms"), model._modules.get("embedding")
+        self.first_input = model.layers[0].sm if embedding is None else None
+        self.layers, self.norms, self.embedding = [], None, None
         with torch.no_grad():
             for layer in model.layers:
                 weight = torch.cat([layer.fc_self.weight, layer.fc_neigh.weight], dim=1)
                 bias = layer.fc_self.bias
                 self.layers.append(ops.int8_quantize(weight) + (bias.detach().float().clone() if bias is not None else None,))
+            if norms is not None:
+                self.norms = [(n.weight.detach().clone(), n.bias.detach().clone(), n.eps) for n in norms]
+            if embedding is not None:  # (the table itself: it may fill most of the memory)
+                self.embedding = embedding.weight.detach(), embedding.scale
 
     @torch.no_grad()
     def __call__(self, blocks):
@@ -424,12 +581,17 @@ class Int8SAGE:
             raise RuntimeError(f"the network has {len(self.layers)} layers, there are {len(blocks)} blocks")
         h = None
         for i, ((codes, scales, bias), block) in enumerate(zip(self.layers, blocks)):
-            if i == 0:
+            if i == 0 and self.embedding is not None:
+                h = ops.embedding(self.embedding[0], block["src_nodes"], self.embedding[1]).float()
+            if i == 0 and self.embedding is None:
                 sm, neighbours, dst = block.get("first_layer_input") or self.first_input.for_block(block)
                 own, mean = sm.decode_rows(dst), sm.aggregate(block["indptr"], neighbours)
             else:
                 own, mean = h[:block["dst_nodes"].numel()], ops.spmm_csr(h, block["indptr"], block["indices_local"])
-            h = ops.int8_linear(own, codes, scales, bias, relu=i + 1 < len(self.layers), x2=mean)
+            hidden = i + 1 < len(self.layers)
+            h = ops.int8_linear(own, codes, scales, bias, relu=hidden and self.norms is None, x2=mean)
+            if hidden and self.norms is not None:
+                h = ops.layer_norm(h, *self.norms[i], relu=True)
         return h
 
 

@@ -111,7 +111,8 @@ class DirectFusedAdam:
 
 
 def train(preset="small", table="replicated", rank=0, world=1, local_rank=0, epochs=3, min_timed_steps=0, batch_size=1024, lr=0.003,
-          dropout=0.5, index_dtype="int64", max_steps=0, precision="tf32", ahead=True, optimizer="adam", muon_lr=0.02, answer_int8=False):
+          dropout=0.5, index_dtype="int64", max_steps=0, precision="tf32", ahead=True, optimizer="adam", muon_lr=0.02, answer_int8=False, norm=False,
+          activations="float", embedding=0):
     """Train on the preset's synthetic data inside an already initialised process (and, for world > 1 or a sharded table,
     process group); returns the record rank 0 reports (every rank gets it).  The first epoch is a discarded warm-up; when
     ``min_timed_steps`` is set, enough further epochs are run to time at least that many steps per rank.  Per-phase device
@@ -119,22 +120,27 @@ def train(preset="small", table="replicated", rank=0, world=1, local_rank=0, epo
     tf32_before = torch.backends.cuda.matmul.allow_tf32
     try:
         return _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batch_size, lr, dropout, index_dtype, max_steps, precision,
-                      ahead, optimizer, muon_lr, answer_int8)
+                      ahead, optimizer, muon_lr, answer_int8, norm, activations, embedding)
     finally:
         torch.backends.cuda.matmul.allow_tf32 = tf32_before
 
 
 def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batch_size, lr, dropout, index_dtype, max_steps, precision, ahead,
-           optimizer_name, muon_lr, answer_int8):
+           optimizer_name, muon_lr, answer_int8, norm, activations, embedding):
     if optimizer_name not in ("adam", "muon"):
         raise ValueError("optimizer must be adam or muon")
+    if embedding and (optimizer_name == "muon" or table != "replicated"):
+        raise ValueError("learned rows go with Adam and without a sharded table")
     cfg = PRESETS[preset]
     device = torch.device("cuda", local_rank)
     idt = torch.int32 if index_dtype == "int32" else torch.int64
     indptr, indices, labels, train_ids, cm = build_data(cfg, device, idt, table)
 
     torch.manual_seed(0)
-    model = sage.SAGE(cfg["feat"], cfg["hidden"], cfg["classes"], len(cfg["fan_out"]), dropout, cm).to(device)
+    if embedding:  # learned rows in place of the features
+        cm, rows = None, sage.NodeEmbedding(cfg["nodes"], embedding, device=device)
+    model = sage.SAGE(embedding or cfg["feat"], cfg["hidden"], cfg["classes"], len(cfg["fan_out"]), dropout, cm, norm=norm, activations=activations,
+                      embedding=rows if embedding else None).to(device)
     net = model
     flat_grad = None
     if world > 1:
@@ -198,7 +204,8 @@ def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batc
             input_nodes, output_nodes, blocks = next(it)
             y = labels[output_nodes]
             ev[1].record()
-            blocks[0]["first_layer_input"] = cm.for_block(blocks[0])  # sharded table: the row exchange of this minibatch
+            if cm is not None:
+                blocks[0]["first_layer_input"] = cm.for_block(blocks[0])  # sharded table: the row exchange of this minibatch
             ev[2].record()
             with sage.products_in(product_dtype):
                 pred = net(blocks)
@@ -265,7 +272,7 @@ def _train(preset, table, rank, world, local_rank, epochs, min_timed_steps, batc
         "breakdown_ms": {k: round(v, 4) for k, v in zip(phases, stats[2:])},
         "first_layer_edges_per_s": stats[1] / stats[0], "loss_last_step_per_epoch": [round(v, 4) for v in losses],
         "config": {k: (list(v) if isinstance(v, tuple) else v) for k, v in cfg.items()}, "index_dtype": index_dtype,
-        "precision": precision, "optimizer": optimizer_name, **({"int8": int8} if int8 is not None else {}), "blocks_built_ahead": bool(ahead), "table": table, "data": "synthetic", "scaling": "strong (train ids split over ranks)",
+        "precision": precision, "optimizer": optimizer_name, "norm": bool(norm), "activations": activations, "embedding": int(embedding), **({"int8": int8} if int8 is not None else {}), "blocks_built_ahead": bool(ahead), "table": table, "data": "synthetic", "scaling": "strong (train ids split over ranks)",
         "timing": "wall clock around barrier + synchronize delimited epochs, first epoch discarded, max over ranks; breakdown = CUDA "
                   "events on the current stream, mean per step, max over ranks"}
 
@@ -307,6 +314,9 @@ def main():
     ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"],
                     help="muon: orthogonalised updates of the weight matrices (learning rate --muon-lr), Adam for the biases")
     ap.add_argument("--muon-lr", type=float, default=0.02)
+    ap.add_argument("--norm", action="store_true", help="layer norm in front of every ReLU")
+    ap.add_argument("--activations", default="float", choices=["float", "int8"], help="int8: keep what the backward pass needs in 8 bits")
+    ap.add_argument("--embedding", type=int, default=0, help="train a row of that many columns for every node and use it in place of the features")
     ap.add_argument("--answer-int8", action="store_true", help="also answer the last minibatch in 8-bit integers and report the difference")
     ap.add_argument("--no-pin", action="store_true", help="do not give every rank its own share of the node's CPUs")
     ap.add_argument("--no-ahead", action="store_true", help="build every minibatch inside its step instead of one step early on a side stream")
@@ -328,7 +338,8 @@ def main():
             os.environ.setdefault("MASTER_PORT", "29577")
         dist.init_process_group("nccl", device_id=device, rank=rank, world_size=world)
     rec = train(args.preset, args.table, rank, world, local_rank, args.epochs, args.min_timed_steps, args.batch_size, args.lr,
-                args.dropout, args.index_dtype, args.max_steps, args.precision, not args.no_ahead, args.optimizer, args.muon_lr, args.answer_int8)
+                args.dropout, args.index_dtype, args.max_steps, args.precision, not args.no_ahead, args.optimizer, args.muon_lr, args.answer_int8,
+                args.norm, args.activations, args.embedding)
     if rank == 0:
         print(json.dumps(rec), flush=True)
     if dist.is_initialized():
