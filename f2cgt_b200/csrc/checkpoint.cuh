@@ -86,17 +86,52 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 
 struct Scale { float step, low; };
 
-// Codes of a group, four columns a lane of which `left` exist (the others' codes are 0); by whole warps.  The quotient is a product with the
-// reciprocal, which is at most 255 * 3 * 2^-24 = 4.6e-5 off; only where it lies so near to a tie that this could matter, or where the step is so
-// small that the reciprocal is none, is the division made.
-__device__ __forceinline__ uint32_t encode(const float (&x)[4], int left, Scale& s) {
-  float low = __int_as_float(0x7f800000), high = -low;
+// Two single-precision numbers at a time.
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_near(float v) {  // one unit in the last place off
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Codes of four columns of which `left` exist, by divisions.
+static __device__ __noinline__ uint32_t encode_by_division(float x0, float x1, float x2, float x3, float low, float step, int left) {
+  const float x[4] = {x0, x1, x2, x3};
+  uint32_t codes = 0u;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    low = min_nan(low, e < left ? x[e] : low);
-    high = max_nan(high, e < left ? x[e] : high);
+  for (int e = 0; e < 4; ++e)
+    if (e < left) codes |= (uint32_t)fminf(rintf((x[e] - low) / step), 255.0f) << (8 * e);
+  return codes;
+}
+
+// Codes of a group, four columns a lane of which `left` exist (the others' codes are 0); by whole warps.  The quotient is a product with the
+// reciprocal, at most 255 * 4 * 2^-24 = 6.1e-5 off what the division gives; only where it lies so near to a tie that this could matter, or where the
+// step is so small that the reciprocal is none, is the division made (one warp in forty; a division each took 60 us for 8192 x 4096 bfloat16).  2^23 + 2^22
+// added to a number below 2^22 rounds it to even and leaves it in the last bits.
+__device__ __forceinline__ uint32_t encode(const float (&given)[4], int left, Scale& s) {
+  float x[4] = {given[0], given[1], given[2], given[3]};
+  if (left < 4) {
+    if (left <= 0) x[0] = __int_as_float(0x7f800000);  // (below: nobody's extreme)
+#pragma unroll
+    for (int e = 1; e < 4; ++e) x[e] = e < left ? x[e] : x[0];
   }
-  low = warp_min_nan(low);
+  const float low = warp_min_nan(min_nan(min_nan(x[0], x[1]), min_nan(x[2], x[3])));
+  float high = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+  if (left <= 0) high = __int_as_float(0xff800000);
   high = warp_max_nan(high);
   const float range = high - low;
   if (!(range <= 3.402823466e38f)) {  // infinite, or no number
@@ -104,21 +139,29 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], int left, Scale&
     return 0u;
   }
   s.low = low;
-  s.step = range / 255.0f;
+  // range / 255 by two corrections with exact remainders; the ordinary division where they would not be exact
+  const bool plain = range > 1e-25f && range < 1e30f;
+  if (plain) s.step = div_exact_fast(range, 255.0f, 1.0f / 255.0f);
+  else s.step = range / 255.0f;
   if (s.step == 0.0f) return 0u;
-  const bool small = s.step < 1e-35f;
-  const float by = 1.0f / s.step;
-  uint32_t codes = 0u;
+  if (!plain) return encode_by_division(x[0], x[1], x[2], x[3], low, s.step, left);
+  const float by = reciprocal_near(s.step), magic = 12582912.0f;
+  const unsigned long long by2 = pair_of(by, by), low2 = pair_of(-low, -low), magic2 = pair_of(magic, magic), less2 = pair_of(-magic, -magic), minus2 = pair_of(-1.0f, -1.0f);
+  unsigned long long q[2] = {pair_of(x[0], x[1]), pair_of(x[2], x[3])}, m[2];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float over = x[e] - low;
-    float q = over * by;
-    const float r = rintf(q);
-    if (small || fabsf(fabsf(q - r) - 0.5f) < 1e-4f) q = rintf(over / s.step);
-    else q = r;
-    if (e < left) codes |= (uint32_t)fminf(q, 255.0f) << (8 * e);
+  for (int h = 0; h < 2; ++h) {
+    add2(q[h], low2);
+    q[h] = mul2(q[h], by2);
+    m[h] = q[h];
+    add2(m[h], magic2);
+    unsigned long long r = m[h];
+    add2(r, less2);
+    q[h] = fma2(r, minus2, q[h]);  // from the nearest whole number: exact
   }
-  return codes;
+  const float far = fmaxf(fmaxf(fabsf(lo32(q[0])), fabsf(hi32(q[0]))), fmaxf(fabsf(lo32(q[1])), fabsf(hi32(q[1]))));
+  if (far > 0.5f - 1e-4f && left > 0) return encode_by_division(x[0], x[1], x[2], x[3], low, s.step, left);
+  const uint32_t codes = __byte_perm(__byte_perm((uint32_t)m[0], (uint32_t)(m[0] >> 32), 0x0040), __byte_perm((uint32_t)m[1], (uint32_t)(m[1] >> 32), 0x0040), 0x5410);
+  return left >= 4 ? codes : left <= 0 ? 0u : codes & ((1u << (8 * left)) - 1u);
 }
 
 __device__ __forceinline__ void decode(uint32_t codes, Scale s, float (&x)[4]) {

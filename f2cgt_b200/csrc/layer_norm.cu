@@ -3,7 +3,8 @@
 //
 // Bound by reading and writing the rows.  A row's values stay in registers between the mean, the squares of the differences from it (no
 // cancellation of large means) and the result: a warp has rows up to 1024 columns long, several at a time where they are short so that enough loads are on
-// the way; a CTA has longer ones, and what its registers do not hold (beyond 16,384 columns) it reads again.
+// the way; a CTA has longer ones, one after the other, the next one's loads on the way and its columns' weights in registers; rows beyond 8192 columns it
+// reads again for every step.
 #include "checkpoint.cuh"
 
 namespace f2c {
@@ -76,7 +77,7 @@ constexpr int kThreads = 256;
 
 // ROWS rows of up to CHUNKS * 128 columns for every warp
 template <typename T, int ACCESS, int CHUNKS, int ROWS>
-__global__ void __launch_bounds__(kThreads) warp_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 2) warp_kernel(const __grid_constant__ Args a) {
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31;
@@ -89,9 +90,10 @@ __global__ void __launch_bounds__(kThreads) warp_kernel(const __grid_constant__ 
       const int col = c * kGroup + 4 * lane;
       raw[r][c].load((const T*)a.x + (first + r) * a.ldx + col, first + r < a.m ? a.d - col : 0);
     }
-  float w[CHUNKS][4], b[CHUNKS][4];
+  constexpr int kHeld = ROWS > 1 ? CHUNKS : 0;  // weights used more than once
+  float w[kHeld + 1][4], b[kHeld + 1][4];
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
+  for (int c = 0; c < kHeld; ++c) {
     const int col = c * kGroup + 4 * lane;
     of_columns(a.weight, col, a.d - col, 1.0f, w[c]);
     of_columns(a.bias, col, a.d - col, 0.0f, b[c]);
@@ -122,8 +124,15 @@ __global__ void __launch_bounds__(kThreads) warp_kernel(const __grid_constant__ 
       a.rstd[row] = rstd;
     }
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-      if (c * kGroup < a.d) finish<T, ACCESS>(a, row, c, x[c], mean, rstd, w[c], b[c]);
+    for (int c = 0; c < CHUNKS; ++c) {
+      if (c * kGroup >= a.d) break;
+      const int at = kHeld > 0 ? c : 0, col = c * kGroup + 4 * lane;
+      if constexpr (kHeld == 0) {
+        of_columns(a.weight, col, a.d - col, 1.0f, w[0]);
+        of_columns(a.bias, col, a.d - col, 0.0f, b[0]);
+      }
+      finish<T, ACCESS>(a, row, c, x[c], mean, rstd, w[at], b[at]);
+    }
   }
 }
 
@@ -138,59 +147,101 @@ __device__ __forceinline__ float block_sum(float v, float* of_warp) {
   return v;
 }
 
-// A row for every CTA: chunks warp, warp + THREADS / 32, ... are a warp's, KEPT of which it keeps.
+// A CTA has every gridDim.x-th row: chunks warp, warp + THREADS / 32, ... are a warp's, all of which it keeps.
 template <typename T, int ACCESS, int THREADS, int KEPT>
-__global__ void __launch_bounds__(THREADS) block_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __grid_constant__ Args a) {
   constexpr int kWarps = THREADS / 32;
+  __shared__ float of_warp[2][kWarps];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Four<T, ACCESS> next[KEPT];
+  const auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+      const int col = (warp + k * kWarps) * kGroup + 4 * lane;
+      next[k].load((const T*)a.x + row * a.ldx + col, row < a.m ? a.d - col : 0);
+    }
+  };
+  fetch(blockIdx.x);
+  float w[KEPT][4], b[KEPT][4];
+#pragma unroll
+  for (int k = 0; k < KEPT; ++k) {
+    const int col = (warp + k * kWarps) * kGroup + 4 * lane;
+    of_columns(a.weight, col, a.d - col, 1.0f, w[k]);
+    of_columns(a.bias, col, a.d - col, 0.0f, b[k]);
+  }
+  const float n = (float)a.d;
+  for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
+    float x[KEPT][4], sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+      next[k].get(x[k]);
+      sum += (x[k][0] + x[k][1]) + (x[k][2] + x[k][3]);
+    }
+    fetch(row + gridDim.x);
+    // (the barrier of one sum keeps the reads of the other's apart from the next row's writes)
+    const float mean = block_sum<THREADS>(sum, of_warp[0]) / n;
+    float squares = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float t = (warp + k * kWarps) * kGroup + 4 * lane + e < a.d ? x[k][e] - mean : 0.0f;
+        squares = fmaf(t, t, squares);
+      }
+    const float rstd = 1.0f / sqrtf(block_sum<THREADS>(squares, of_warp[1]) / n + a.eps);
+    if (threadIdx.x == 0 && a.mean != nullptr) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+      if ((warp + k * kWarps) * kGroup >= a.d) break;
+      finish<T, ACCESS>(a, row, warp + k * kWarps, x[k], mean, rstd, w[k], b[k]);
+    }
+  }
+}
+
+// Longer rows, one a CTA, read three times.
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args a) {
+  constexpr int kWarps = 16;
   __shared__ float of_warp[2][kWarps];
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.d + kGroup - 1) / kGroup;
   const int64_t row = blockIdx.x;
   const T* const from = (const T*)a.x + row * a.ldx;
-  Four<T, ACCESS> raw[KEPT];
-#pragma unroll
-  for (int k = 0; k < KEPT; ++k) {
-    const int col = (warp + k * kWarps) * kGroup + 4 * lane;
-    raw[k].load(from + col, a.d - col);
-  }
   const auto each = [&](auto&& body) {  // every chunk of this warp
-#pragma unroll
-    for (int k = 0; k < KEPT; ++k) {
-      if (warp + k * kWarps >= chunks) break;
-      float x[4];
-      raw[k].get(x);
-      body(warp + k * kWarps, x);
-    }
-    for (int c = warp + KEPT * kWarps; c < chunks; c += kWarps) {
-      Four<T, ACCESS> more;
+    for (int c = warp; c < chunks; c += kWarps) {
+      Four<T, ACCESS> v;
       float x[4];
       const int col = c * kGroup + 4 * lane;
-      more.load(from + col, a.d - col);
-      more.get(x);
-      body(c, x);
+      v.load(from + col, a.d - col);
+      v.get(x);
+      body(c, col, x);
     }
   };
   const float n = (float)a.d;
   float sum = 0.0f;
-  each([&](int, const float (&x)[4]) { sum += (x[0] + x[1]) + (x[2] + x[3]); });
-  const float mean = block_sum<THREADS>(sum, of_warp[0]) / n;
+  each([&](int, int, const float (&x)[4]) { sum += (x[0] + x[1]) + (x[2] + x[3]); });
+  const float mean = block_sum<512>(sum, of_warp[0]) / n;
   float squares = 0.0f;
-  each([&](int c, const float (&x)[4]) {
+  each([&](int, int col, const float (&x)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float t = c * kGroup + 4 * lane + e < a.d ? x[e] - mean : 0.0f;
+      const float t = col + e < a.d ? x[e] - mean : 0.0f;
       squares = fmaf(t, t, squares);
     }
   });
-  const float rstd = 1.0f / sqrtf(block_sum<THREADS>(squares, of_warp[1]) / n + a.eps);
+  const float rstd = 1.0f / sqrtf(block_sum<512>(squares, of_warp[1]) / n + a.eps);
   if (threadIdx.x == 0 && a.mean != nullptr) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
   }
-  each([&](int c, const float (&x)[4]) {
+  each([&](int c, int col, const float (&x)[4]) {
     float w[4], b[4];
-    const int col = c * kGroup + 4 * lane;
     of_columns(a.weight, col, a.d - col, 1.0f, w);
     of_columns(a.bias, col, a.d - col, 0.0f, b);
     finish<T, ACCESS>(a, row, c, x, mean, rstd, w, b);
@@ -202,14 +253,28 @@ static void by_warps(const Args& a, cudaStream_t st) {
   launch_dependent(warp_kernel<T, ACCESS, CHUNKS, ROWS>, dim3((unsigned)ceil_div(a.m, kThreads / 32 * ROWS)), kThreads, 0, st, a);
 }
 
+template <typename T, int ACCESS, int THREADS, int KEPT>
+static void by_ctas(const Args& a, int resident, cudaStream_t st) {
+  const int64_t most = (int64_t)resident * kSmCount;
+  launch_dependent(block_kernel<T, ACCESS, THREADS, KEPT>, dim3((unsigned)(a.m < most ? a.m : most)), THREADS, 0, st, a);
+}
+
 template <typename T, int ACCESS>
 static void run(const Args& a, cudaStream_t st) {
-  if (a.d <= kGroup) by_warps<T, ACCESS, 1, 4>(a, st);
-  else if (a.d <= 2 * kGroup) by_warps<T, ACCESS, 2, 2>(a, st);
-  else if (a.d <= 4 * kGroup) by_warps<T, ACCESS, 4, 1>(a, st);
-  else if (a.d <= 8 * kGroup) by_warps<T, ACCESS, 8, 1>(a, st);
-  else if (a.d <= 32 * kGroup) launch_dependent(block_kernel<T, ACCESS, 256, 4>, dim3((unsigned)a.m), 256, 0, st, a);
-  else launch_dependent(block_kernel<T, ACCESS, 512, 8>, dim3((unsigned)a.m), 512, 0, st, a);
+  switch ((a.d + kGroup - 1) / kGroup) {
+    case 1: return by_warps<T, ACCESS, 1, 4>(a, st);
+    case 2: return by_warps<T, ACCESS, 2, 2>(a, st);
+    case 3: return by_warps<T, ACCESS, 3, 1>(a, st);
+    case 4: return by_warps<T, ACCESS, 4, 1>(a, st);
+    case 5: return by_warps<T, ACCESS, 5, 1>(a, st);
+    case 6: return by_warps<T, ACCESS, 6, 1>(a, st);
+    case 7: case 8: return by_warps<T, ACCESS, 8, 1>(a, st);
+    default: break;
+  }
+  if (a.d <= 16 * kGroup) by_ctas<T, ACCESS, 256, 2>(a, 4, st);
+  else if (a.d <= 32 * kGroup) by_ctas<T, ACCESS, 256, 4>(a, 2, st);
+  else if (a.d <= 64 * kGroup) by_ctas<T, ACCESS, 512, 4>(a, 1, st);
+  else launch_dependent(long_kernel<T, ACCESS>, dim3((unsigned)a.m), 512, 0, st, a);
 }
 
 }  // namespace ln

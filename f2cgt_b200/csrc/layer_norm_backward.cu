@@ -77,16 +77,17 @@ __device__ __forceinline__ void warp_sum2(float& u, float& v) {
   }
 }
 
-// WARPS warps have a row of up to WARPS * CHUNKS * 128 columns: one warp (eight rows to a CTA), or a CTA's.
+// WARPS warps have a row of up to WARPS * CHUNKS * 128 columns: one warp, two, or all of a CTA.
 template <typename T, int ACCESS, bool CODES, int WARPS, int CHUNKS, int THREADS>
 __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant__ Back a) {
   constexpr int kRows = THREADS / 32 / WARPS;  // of a CTA at a time
   constexpr bool kAlone = WARPS == 1;
-  __shared__ float sums[2][2][kAlone ? 1 : WARPS];
-  __shared__ float joined[kAlone ? 2 * CHUNKS * kGroup : 1][kAlone ? kRows + 1 : 1];
+  constexpr int kColumns = WARPS * CHUNKS * kGroup;
+  __shared__ float sums[2][2][kAlone ? 1 : THREADS / 32];
+  __shared__ float joined[kRows > 1 ? 2 * kColumns : 1][kRows > 1 ? kRows + 1 : 1];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % WARPS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % WARPS, own = warp / WARPS * WARPS;
   const int64_t stride = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + warp / WARPS;
   Columns<T, ACCESS, CODES> next[CHUNKS];
@@ -101,15 +102,24 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
     }
   };
   fetch(row);
-  float w[CHUNKS][4], dw[CHUNKS][4], db[CHUNKS][4];
+  constexpr bool kHeld = WARPS < 16;  // (the widest rows' weights do not fit beside their sums: they are read again for every row)
+  float held[kHeld ? CHUNKS : 1][4], dw[CHUNKS][4], db[CHUNKS][4];
+  const auto weights = [&](int c, float (&w)[4]) {
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = held[c][e];
+    } else {
+      weights_of(a, member + c * WARPS, w);
+    }
+  };
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    weights_of(a, member + c * WARPS, w[c]);
+    if constexpr (kHeld) weights_of(a, member + c * WARPS, held[c]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) dw[c][e] = db[c][e] = 0.0f;
   }
   const float n = (float)a.d;
-  // (WARPS > 1: row is the CTA's, and all its threads leave together)
+  // (all warps of a row leave together)
   for (int turn = 0; row < a.m; row += stride, turn ^= 1) {
     const float mean = next_mean, rstd = next_rstd;
     Columns<T, ACCESS, CODES> now[CHUNKS];
@@ -119,13 +129,14 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
     float u = 0.0f, v = 0.0f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      float g[4], h[4];
+      float g[4], h[4], w[4];
       now[c].get(mean, rstd, a.d - (member + c * WARPS) * kGroup - 4 * lane, g, h);
+      weights(c, w);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         dw[c][e] = fmaf(g[e], h[e], dw[c][e]);
         db[c][e] += g[e];
-        const float gw = g[e] * w[c][e];
+        const float gw = g[e] * w[e];
         u += gw;
         v = fmaf(gw, h[e], v);
       }
@@ -133,15 +144,17 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
     warp_sum2(u, v);
     if constexpr (!kAlone) {
       if (lane == 0) {
-        sums[turn][0][member] = u;
-        sums[turn][1][member] = v;
+        sums[turn][0][warp] = u;
+        sums[turn][1][warp] = v;
       }
-      __syncthreads();  // (the other turn's sums are read before the next one)
+      // of the row's warps (the other turn's sums are read before the next one)
+      if constexpr (kRows == 1) __syncthreads();
+      else asm volatile("bar.sync %0, %1;" ::"r"(warp / WARPS + 1), "n"(WARPS * 32) : "memory");
       u = v = 0.0f;
 #pragma unroll
       for (int q = 0; q < WARPS; ++q) {
-        u += sums[turn][0][q];
-        v += sums[turn][1][q];
+        u += sums[turn][0][own + q];
+        v += sums[turn][1][own + q];
       }
     }
     u /= n;
@@ -149,27 +162,29 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int col = (member + c * WARPS) * kGroup + 4 * lane, left = a.d - col;
-      float g[4], h[4];
+      float g[4], h[4], w[4];
       now[c].get(mean, rstd, left, g, h);
+      weights(c, w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) g[e] = rstd * (fmaf(g[e], w[c][e], -u) - h[e] * v);
+      for (int e = 0; e < 4; ++e) g[e] = rstd * (fmaf(g[e], w[e], -u) - h[e] * v);
       Four<T, ACCESS> out;
       out.set(g);
       out.store((T*)a.dx + row * a.d + col, left);
     }
   }
   float* const part = a.parts + (int64_t)blockIdx.x * 2 * a.d;
-  if constexpr (kAlone) {
+  if constexpr (kRows > 1) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        joined[c * kGroup + 4 * lane + e][warp] = dw[c][e];
-        joined[CHUNKS * kGroup + c * kGroup + 4 * lane + e][warp] = db[c][e];
+        const int col = (member + c * WARPS) * kGroup + 4 * lane + e;
+        joined[col][warp / WARPS] = dw[c][e];
+        joined[kColumns + col][warp / WARPS] = db[c][e];
       }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * a.d; i += THREADS) {
-      const int from = i < a.d ? i : CHUNKS * kGroup + i - a.d;
+      const int from = i < a.d ? i : kColumns + i - a.d;
       float sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < kRows; ++q) sum += joined[from][q];
@@ -273,18 +288,22 @@ __global__ void __launch_bounds__(256) columns_kernel(const __grid_constant__ Ba
   if (at < a.d) a.parts[((int64_t)blockIdx.x * 2 + which) * a.d + at] = sum;
 }
 
-// The parts' sums: 32 columns a CTA, a 32nd of the parts a warp.
+// The parts' sums: eight columns a CTA, four parts a warp at a time.  (32 columns a CTA and a part a warp took 8 us for 888 parts of 256.)
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ parts, int count, int d, float* __restrict__ dweight, float* __restrict__ dbias) {
-  __shared__ float of[32][33];
+  __shared__ float of[32][8];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = blockIdx.x * 8 + (lane & 7);
   float sum = 0.0f;
-  if (at < 2 * d)
-    for (int p = warp; p < count; p += 32) sum += parts[(int64_t)p * 2 * d + at];
-  of[warp][lane] = sum;
+  if (at < 2 * d) {
+#pragma unroll 8
+    for (int p = warp * 4 + (lane >> 3); p < count; p += 128) sum += parts[(int64_t)p * 2 * d + at];
+  }
+  sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+  if (lane < 8) of[warp][lane] = sum;
   __syncthreads();
-  if (warp != 0) return;
+  if (threadIdx.x >= 8) return;
   sum = 0.0f;
 #pragma unroll
   for (int q = 0; q < 32; ++q) sum += of[q][lane];
@@ -302,11 +321,13 @@ struct Deal {
 };
 static Deal deal(int64_t m, int64_t d) {
   Deal r;
-  if (d <= kGroup) r = {1, 1, 256, 6};
-  else if (d <= 2 * kGroup) r = {1, 2, 256, 4};
-  else if (d <= 4 * kGroup) r = {1, 4, 256, 2};
-  else if (d <= 8 * kGroup) r = {8, 1, 256, 6};
-  else if (d <= 32 * kGroup) r = {8, 4, 256, 2};
+  if (d <= kGroup) r = {1, 1, 256, 3};
+  else if (d <= 2 * kGroup) r = {1, 2, 256, 2};
+  else if (d <= 4 * kGroup) r = {1, 4, 256, 1};
+  else if (d <= 6 * kGroup) r = {2, 3, 256, 2};
+  else if (d <= 8 * kGroup) r = {2, 4, 256, 1};
+  else if (d <= 16 * kGroup) r = {8, 2, 256, 2};
+  else if (d <= 32 * kGroup) r = {8, 4, 256, 1};
   else if (d <= 64 * kGroup) r = {16, 4, 512, 1};
   else r = {0, 1, 256, 1};
   const int rows = r.warps == 0 ? 8 : r.threads / 32 / r.warps;
@@ -322,7 +343,9 @@ static void run_source(const Back& a, const Deal& how, cudaStream_t st) {
   if (how.warps == 1 && how.chunks == 1) launch_dependent(backward_kernel<T, ACCESS, CODES, 1, 1, 256>, grid, 256, 0, st, a);
   else if (how.warps == 1 && how.chunks == 2) launch_dependent(backward_kernel<T, ACCESS, CODES, 1, 2, 256>, grid, 256, 0, st, a);
   else if (how.warps == 1) launch_dependent(backward_kernel<T, ACCESS, CODES, 1, 4, 256>, grid, 256, 0, st, a);
-  else if (how.warps == 8 && how.chunks == 1) launch_dependent(backward_kernel<T, ACCESS, CODES, 8, 1, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 2 && how.chunks == 3) launch_dependent(backward_kernel<T, ACCESS, CODES, 2, 3, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 2) launch_dependent(backward_kernel<T, ACCESS, CODES, 2, 4, 256>, grid, 256, 0, st, a);
+  else if (how.warps == 8 && how.chunks == 2) launch_dependent(backward_kernel<T, ACCESS, CODES, 8, 2, 256>, grid, 256, 0, st, a);
   else if (how.warps == 8) launch_dependent(backward_kernel<T, ACCESS, CODES, 8, 4, 256>, grid, 256, 0, st, a);
   else if (how.warps == 16) launch_dependent(backward_kernel<T, ACCESS, CODES, 16, 4, 512>, grid, 512, 0, st, a);
   else {
@@ -376,6 +399,6 @@ extern "C" int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, c
     F2C_BY_ROWS(ln::run, dtype, access, a, how, st);
     if (const int rc = check_launch(op)) return rc;
   }
-  launch_dependent(ln::join_kernel, dim3((unsigned)ceil_div(2 * d, 32)), 1024, 0, st, (const float*)workspace, m > 0 ? how.ctas : 0, (int)d, dweight, dbias);
+  launch_dependent(ln::join_kernel, dim3((unsigned)ceil_div(2 * d, 8)), 1024, 0, st, (const float*)workspace, m > 0 ? how.ctas : 0, (int)d, dweight, dbias);
   return check_launch(op);
 }

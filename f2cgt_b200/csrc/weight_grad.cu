@@ -25,7 +25,10 @@ namespace f2c {
 namespace wg {
 
 using namespace t5;
+using ckpt::fma2;
 using ckpt::kGroup;
+using ckpt::mul2;
+using ckpt::pair_of;
 
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kTile = 128, kRows = 32, kAhead = 2, kStages = 6;
@@ -41,7 +44,6 @@ struct Params {
   int64_t split_rows;     // a multiple of kRows
   void *dw, *db;          // (splits == 1) of dy's type
   float *part, *part_db;  // (splits > 1) [split][tile][32][128][4], [split][n_tiles * 128]
-  int vectors;            // dy's rows can be read 16 bytes at a time
   uint32_t tries;
   int* error;
 };
@@ -65,52 +67,50 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&w)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-// What a thread has of a stage: eight columns of a row of dy and of its codes, and their step and lowest value.
-template <typename T>
+// What a thread has of a stage: eight columns of a row of dy and of its codes, and their step and lowest value.  ACCESS: bytes of a load of dy.
+template <typename T, int ACCESS>
 struct Piece {
-  static constexpr int kWords = 2 * (int)sizeof(T);
+  static constexpr int kWords = 2 * (int)sizeof(T), kEach = ACCESS / (int)sizeof(T);
   uint32_t dy[kWords];
-  uint2 codes;
-  ckpt::Scale s;
+  uint2 codes, scale;
 
   __device__ __forceinline__ void load(const Params& p, int64_t row, bool here, int col, int code_col, int group) {
     const T* const from = (const T*)p.dy + row * p.ldy + col;
-    if (p.vectors) {  // (a row's last vector may reach over its end, where it is loaded value by value)
-      const bool whole = here && col + 8 <= p.n;
 #pragma unroll
-      for (int q = 0; q < kWords / 4; ++q) {
-        const uint4 v = ldg_nc_u128_if(from + q * (16 / (int)sizeof(T)), whole);
+    for (int q = 0; q < 8 / kEach; ++q) {
+      const bool go = here && col + q * kEach < p.n;
+      const T* const at = from + q * kEach;
+      if constexpr (ACCESS == 16) {
+        const uint4 v = ldg_nc_u128_if(at, go);
         dy[4 * q] = v.x; dy[4 * q + 1] = v.y; dy[4 * q + 2] = v.z; dy[4 * q + 3] = v.w;
+      } else if constexpr (ACCESS == 8) {
+        const uint2 v = ldg_nc_u64_if(at, go);
+        dy[2 * q] = v.x; dy[2 * q + 1] = v.y;
+      } else if constexpr (ACCESS == 4) {
+        dy[q] = ldg_nc_u32_if(at, go);
+      } else {
+        const uint32_t v = go ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at)) : 0u;
+        dy[q / 2] = q & 1 ? dy[q / 2] | v << 16 : v;
       }
-      if (here && !whole && col < p.n) one_by_one(from, p.n - col);
-    } else {
-#pragma unroll
-      for (int q = 0; q < kWords; ++q) dy[q] = 0u;
-      if (here) one_by_one(from, p.n - col);
     }
     codes = ldg_nc_u64_if(p.x.codes + row * p.x.ld + code_col, here && code_col < p.k);
-    const uint2 v = ldg_nc_u64_if(p.x.scales + 2 * (row * p.x.groups + group), here);
-    s = ckpt::Scale{__uint_as_float(v.x), __uint_as_float(v.y)};
+    scale = ldg_nc_u64_if(p.x.scales + 2 * (row * p.x.groups + group), here);
   }
-  __device__ __forceinline__ void one_by_one(const T* from, int count) {
+  __device__ __forceinline__ void get(unsigned long long (&d)[4]) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (e >= count) break;
-      if constexpr (sizeof(T) == 4) dy[e] = __ldg(reinterpret_cast<const uint32_t*>(from) + e);
-      else dy[e / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(from) + e) << (16 * (e & 1));
-    }
-  }
-  __device__ __forceinline__ void get(float (&d)[8]) const {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (sizeof(T) == 4) d[e] = __uint_as_float(dy[e]);
-      else if constexpr (std::is_same<T, __half>::value) d[e] = __half2float(__ushort_as_half((unsigned short)(dy[e / 2] >> (16 * (e & 1)))));
-      else d[e] = __uint_as_float(e & 1 ? dy[e / 2] & 0xffff0000u : dy[e / 2] << 16);
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(T) == 4) d[e] = pair_of(__uint_as_float(dy[2 * e]), __uint_as_float(dy[2 * e + 1]));
+      else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&dy[e]));
+        d[e] = pair_of(f.x, f.y);
+      } else {
+        d[e] = pair_of(__uint_as_float(dy[e] << 16), __uint_as_float(dy[e] & 0xffff0000u));
+      }
     }
   }
 };
 
-template <typename T>
+template <typename T, int ACCESS>
 __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_constant__ Params p) {
   constexpr int kPieces = Kind<T>::kPieces, kTaken = Kind<T>::kTaken;
   constexpr uint32_t kStage = (kPieces + 1) * kPlane;
@@ -139,11 +139,12 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
   dependency_wait();
   release_dependents();
 
-  float sum[32], of_low[8], of_bias[8];  // the tile's sums that this thread has, and over its rows and eight columns
+  float sum[32];
+  unsigned long long of_low[4], of_bias[4];  // the tile's sums that this thread has, and over its rows and eight columns
 #pragma unroll
   for (int j = 0; j < 32; ++j) sum[j] = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) of_low[e] = of_bias[e] = 0.0f;
+  for (int e = 0; e < 4; ++e) of_low[e] = of_bias[e] = 0ull;
   const int vec = tid & 15, at_row = tid >> 4;  // eight columns, and a row of a stage
   const int col = n0 + 8 * vec, code_col = group * kGroup + 8 * vec;
   // 16 bytes `vec` of row at_row, in the 128-byte swizzle
@@ -194,11 +195,11 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
   };
 
   // ================= dy and codes, as the MMAs take them
-  const auto fetch = [&](Piece<T>& v, int i) {
+  const auto fetch = [&](Piece<T, ACCESS>& v, int i) {
     const int64_t r = (int64_t)i * kRows + at_row;
     v.load(p, row0 + r, r < rows, col, code_col, group);
   };
-  Piece<T> ahead[kAhead];
+  Piece<T, ACCESS> ahead[kAhead];
 #pragma unroll
   for (int a = 0; a < kAhead; ++a) fetch(ahead[a], a);
   int s = 0, taken = 0;
@@ -208,15 +209,19 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
     for (int a = 0; a < kAhead; ++a) {
       const int i = i0 + a;
       if (i >= stages) break;
-      const Piece<T> v = ahead[a];
+      const Piece<T, ACCESS> v = ahead[a];
       fetch(ahead[a], i + kAhead);
-      float d[8];
+      unsigned long long d[4];
       v.get(d);
+      if (group == 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        of_low[e] = fmaf(v.s.low, d[e], of_low[e]);
-        of_bias[e] += d[e];
-        d[e] *= v.s.step;
+        for (int e = 0; e < 4; ++e) add2(of_bias[e], d[e]);
+      }
+      const unsigned long long step = pair_of(__uint_as_float(v.scale.x), __uint_as_float(v.scale.x)), low = pair_of(__uint_as_float(v.scale.y), __uint_as_float(v.scale.y));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        of_low[e] = fma2(low, d[e], of_low[e]);
+        d[e] = mul2(step, d[e]);
       }
       if (round > 0) wait_bar(bars.empty + s, (round - 1) & 1, left);
       const uint32_t at = place + (uint32_t)s * kStage;
@@ -225,11 +230,9 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = pack_bf16(d[2 * e], d[2 * e + 1]);
-          if (q + 1 < kPieces) {  // what is left: exact
-            d[2 * e] -= __uint_as_float(w[e] << 16);
-            d[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
-          }
+          w[e] = pack_bf16(lo32(d[e]), hi32(d[e]));
+          // what is left: exact
+          if (q + 1 < kPieces) d[e] = fma2(pair_of(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)), pair_of(-1.0f, -1.0f), d[e]);
         }
         store16(at + (uint32_t)q * kPlane, w);
       }
@@ -237,9 +240,9 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
 #pragma unroll
       for (int e = 0; e < 4; ++e) {  // 2^23 + q, less 2^23
         const uint32_t from = e < 2 ? v.codes.x : v.codes.y;
-        const float low = __uint_as_float(__byte_perm(from, 0x4B000000u, 0x7440 + (e & 1) * 2)) - 8388608.0f;
-        const float high = __uint_as_float(__byte_perm(from, 0x4B000000u, 0x7441 + (e & 1) * 2)) - 8388608.0f;
-        w[e] = pack_bf16(low, high);
+        unsigned long long q = pair_of(__uint_as_float(__byte_perm(from, 0x4B000000u, 0x7440 + (e & 1) * 2)), __uint_as_float(__byte_perm(from, 0x4B000000u, 0x7441 + (e & 1) * 2)));
+        add2(q, pair_of(-8388608.0f, -8388608.0f));
+        w[e] = pack_bf16(lo32(q), hi32(q));
       }
       store16(at + kPieces * kPlane, w);
       fence_async();
@@ -275,15 +278,15 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
   // of_low and of_bias over all rows: the ring's memory is free
   float(*const columns)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(smem);  // [warp]
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    of_low[e] += __shfl_xor_sync(0xffffffffu, of_low[e], 16);
-    of_bias[e] += __shfl_xor_sync(0xffffffffu, of_bias[e], 16);
+  for (int e = 0; e < 4; ++e) {
+    add2(of_low[e], __shfl_xor_sync(0xffffffffu, of_low[e], 16));
+    add2(of_bias[e], __shfl_xor_sync(0xffffffffu, of_bias[e], 16));
   }
   if (lane < 16) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      columns[wid][0][8 * lane + e] = of_low[e];
-      columns[wid][1][8 * lane + e] = of_bias[e];
+    for (int e = 0; e < 4; ++e) {
+      *reinterpret_cast<unsigned long long*>(&columns[wid][0][8 * lane + 2 * e]) = of_low[e];
+      *reinterpret_cast<unsigned long long*>(&columns[wid][1][8 * lane + 2 * e]) = of_bias[e];
     }
   }
   __syncthreads();
@@ -390,14 +393,28 @@ static Plan plan(int64_t m, int64_t n, int64_t k) {
   return p;
 }
 
-template <typename T>
-static int run(const char* op, Params p, const Plan& how, cudaStream_t st) {
+template <typename T, int ACCESS>
+static int run(const char* op, const Params& p, const Plan& how, cudaStream_t st) {
   constexpr int bytes = kStages * (Kind<T>::kPieces + 1) * kPlane + 1024;
   const int tiles = how.n_tiles * how.k_tiles;
-  if (const int rc = allow_smem(op, (const void*)weight_grad_kernel<T>, bytes)) return rc;
-  launch_dependent(weight_grad_kernel<T>, dim3((unsigned)(tiles * how.splits)), kThreads, bytes, st, p);
+  if (const int rc = allow_smem(op, (const void*)weight_grad_kernel<T, ACCESS>, bytes)) return rc;
+  launch_dependent(weight_grad_kernel<T, ACCESS>, dim3((unsigned)(tiles * how.splits)), kThreads, bytes, st, p);
   if (how.splits > 1) launch_dependent(join_kernel<T>, dim3((unsigned)(tiles * (kTile * kTile / 128) + how.n_tiles * 4)), 256, 0, st, p, tiles);
   return check_launch(op);
+}
+
+// by the widest loads that dy's rows allow
+template <typename T>
+static int run(const char* op, const Params& p, const Plan& how, cudaStream_t st) {
+  int access = 16;
+  const int64_t item = sizeof(T);
+  while (access > item && (!aligned(p.dy, access) || p.n * item % access != 0 || (p.m > 1 && p.ldy * item % access != 0))) access /= 2;
+  if (access == 16) return run<T, 16>(op, p, how, st);
+  if (access == 8) return run<T, 8>(op, p, how, st);
+  if constexpr (sizeof(T) == 2) {
+    if (access == 2) return run<T, 2>(op, p, how, st);
+  }
+  return run<T, 4>(op, p, how, st);
 }
 
 static bool too_large(int64_t m, int64_t n, int64_t k) { return m >= ckpt::kMaxRows || n > (1 << 17) || k > (1 << 17); }
@@ -435,9 +452,8 @@ extern "C" int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype
   const wg::Plan how = wg::plan(m, n, k);
   F2C_REQUIRE(how.bytes == 0 || (workspace && workspace_bytes >= how.bytes && aligned(workspace, 256)), F2C_ERR_INVALID,
               "%s: the workspace must have %lld bytes, 256-byte aligned", op, (long long)how.bytes);
-  const int item = dtype_size(dtype);
-  wg::Params p{dy, ldy, m, (int)n, (int)k, ckpt::Codes{const_cast<uint8_t*>(codes), ldq, const_cast<float*>(scales), ceil_div(k, ckpt::kGroup)}, how.n_tiles, how.splits, how.split_rows,
-               dw, db, (float*)workspace, (float*)((char*)workspace + how.part_bytes), aligned(dy, 16) && (m == 1 || ldy * item % 16 == 0),
+  const wg::Params p{dy, ldy, m, (int)n, (int)k, ckpt::Codes{const_cast<uint8_t*>(codes), ldq, const_cast<float*>(scales), ceil_div(k, ckpt::kGroup)}, how.n_tiles, how.splits, how.split_rows,
+               dw, db, (float*)workspace, (float*)((char*)workspace + how.part_bytes),
                (flags & F2C_NO_WAITS) ? 0u : t5::kWaitLimit, stream_error_word()};
   if (dtype == F2C_F32) return wg::run<float>(op, p, how, st);
   if (dtype == F2C_F16) return wg::run<__half>(op, p, how, st);
