@@ -10,8 +10,9 @@ namespace ckpt {
 constexpr int kThreads = 256, kWarps = kThreads / 32, kAhead = 4;
 
 struct Place { int64_t row; int group; };
-// group number `i` of all rows' groups (2^31 at most)
+// group number `i` of all rows' groups (2^31 at most), and the one behind it
 __device__ __forceinline__ Place place_of(int64_t i, uint32_t groups) { return Place{(int64_t)((uint32_t)i / groups), (int)((uint32_t)i % groups)}; }
+__device__ __forceinline__ Place behind(Place p, int groups) { return p.group + 1 < groups ? Place{p.row, p.group + 1} : Place{p.row + 1, 0}; }
 
 template <typename T, int ACCESS>
 __global__ void __launch_bounds__(kThreads) encode_kernel(const T* __restrict__ x, int64_t ldx, int64_t m, int d, Codes out) {
@@ -21,24 +22,27 @@ __global__ void __launch_bounds__(kThreads) encode_kernel(const T* __restrict__ 
   const int64_t total = m * out.groups, first = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kAhead;
   Four<T, ACCESS> v[kAhead];
   Place at[kAhead];
+  at[0] = place_of(first, (uint32_t)out.groups);
 #pragma unroll
   for (int a = 0; a < kAhead; ++a) {
-    at[a] = place_of(first + a, (uint32_t)out.groups);
+    if (a > 0) at[a] = behind(at[a - 1], (int)out.groups);
     const int col = at[a].group * kGroup + 4 * lane;
-    if (first + a < total) v[a].load(x + at[a].row * ldx + col, d - col);
+    v[a].load(x + at[a].row * ldx + col, first + a < total ? d - col : 0);
   }
+  Scale mine{0.0f, 0.0f};  // lane a: of group a
 #pragma unroll
   for (int a = 0; a < kAhead; ++a) {
-    if (first + a >= total) return;
-    float f[4];
+    if (first + a >= total) break;
+    f32x2 f[2];
     v[a].get(f);
     Scale s;
     const int col = at[a].group * kGroup + 4 * lane;
     const uint32_t codes = encode(f, d - col, s);
     // rows have room for whole 16 bytes: a word that starts in front of the row's end is there
     if (col < d) *reinterpret_cast<uint32_t*>(out.codes + at[a].row * out.ld + col) = codes;
-    if (lane == 0) store_scale(out.scales + 2 * (first + a), s);
+    if (lane == a) mine = s;
   }
+  if (lane < kAhead && first + lane < total) store_scale(out.scales + 2 * (first + lane), mine);
 }
 
 template <typename T, int ACCESS>
@@ -50,9 +54,10 @@ __global__ void __launch_bounds__(kThreads) values_kernel(const Codes in, T* __r
   uint32_t codes[kAhead];
   Scale s[kAhead];
   Place at[kAhead];
+  at[0] = place_of(first, (uint32_t)in.groups);
 #pragma unroll
   for (int a = 0; a < kAhead; ++a) {
-    at[a] = place_of(first + a, (uint32_t)in.groups);
+    if (a > 0) at[a] = behind(at[a - 1], (int)in.groups);
     const int col = at[a].group * kGroup + 4 * lane;
     if (first + a < total) {
       codes[a] = ldg_nc_u32_if(in.codes + at[a].row * in.ld + col, col < d);
@@ -62,7 +67,7 @@ __global__ void __launch_bounds__(kThreads) values_kernel(const Codes in, T* __r
 #pragma unroll
   for (int a = 0; a < kAhead; ++a) {
     if (first + a >= total) return;
-    float f[4];
+    f32x2 f[2];
     decode(codes[a], s[a], f);
     Four<T, ACCESS> v;
     v.set(f);

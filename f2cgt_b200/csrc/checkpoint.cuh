@@ -4,6 +4,8 @@
 // the differences and quotients as single precision has them, so that every implementation of the definition gives the same codes.
 // A group whose max - low is not finite (it holds a NaN or an infinity, or more than the type's range) has codes 0 and values NaN.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace f2c {
@@ -12,6 +14,29 @@ namespace ckpt {
 constexpr int kGroup = F2C_CHECKPOINT_GROUP;  // columns of a warp, four a lane
 static_assert(kGroup == 128, "a group is what a warp holds");
 constexpr int64_t kMaxRows = 1ll << 31, kMaxColumns = 1 << 20;
+
+// Two single-precision numbers in a register pair, and what is done to both by one instruction (add2, lo32 and hi32: common.cuh).
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair_of(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pair_of(v, v); }
+__device__ __forceinline__ f32x2 plus2(f32x2 a, f32x2 b) {
+  add2(a, b);
+  return a;
+}
 
 // Four columns of a row as they are in memory.  ACCESS: bytes of a load or store, by what the rows' alignment and length allow.
 template <typename T, int ACCESS>
@@ -46,13 +71,24 @@ struct alignas(4 * sizeof(T)) Four {
       else at[p] = v[p];
     }
   }
-  __device__ __forceinline__ void get(float (&f)[4]) const {
+  __device__ __forceinline__ void get(f32x2 (&f)[2]) const {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = to_float(v[e]);
+    for (int h = 0; h < 2; ++h) f[h] = pair_of(to_float(v[2 * h]), to_float(v[2 * h + 1]));
   }
-  __device__ __forceinline__ void set(const float (&f)[4]) {
+  __device__ __forceinline__ void set(const f32x2 (&f)[2]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = from_float<T>(f[e]);
+      for (int h = 0; h < 2; ++h) {
+        v[2 * h] = lo32(f[h]);
+        v[2 * h + 1] = hi32(f[h]);
+      }
+    } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<__half2*>(v + 2 * h) = __floats2half2_rn(lo32(f[h]), hi32(f[h]));
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<__nv_bfloat162*>(v + 2 * h) = __floats2bfloat162_rn(lo32(f[h]), hi32(f[h]));
+    }
   }
 };
 
@@ -63,6 +99,7 @@ static inline int access_of(const void* p, int64_t ld, int64_t m, int64_t d, int
   return a;
 }
 
+// of two or three, NaN where one is
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -71,6 +108,16 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ float warp_min_nan(float v) {
@@ -86,22 +133,6 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 
 struct Scale { float step, low; };
 
-// Two single-precision numbers at a time.
-__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ float reciprocal_near(float v) {  // one unit in the last place off
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -122,51 +153,56 @@ static __device__ __noinline__ uint32_t encode_by_division(float x0, float x1, f
 // reciprocal, at most 255 * 4 * 2^-24 = 6.1e-5 off what the division gives; only where it lies so near to a tie that this could matter, or where the
 // step is so small that the reciprocal is none, is the division made (one warp in forty; a division each took 60 us for 8192 x 4096 bfloat16).  2^23 + 2^22
 // added to a number below 2^22 rounds it to even and leaves it in the last bits.
-__device__ __forceinline__ uint32_t encode(const float (&given)[4], int left, Scale& s) {
-  float x[4] = {given[0], given[1], given[2], given[3]};
-  if (left < 4) {
-    if (left <= 0) x[0] = __int_as_float(0x7f800000);  // (below: nobody's extreme)
-#pragma unroll
-    for (int e = 1; e < 4; ++e) x[e] = e < left ? x[e] : x[0];
+__device__ __forceinline__ uint32_t encode(const f32x2 (&given)[2], int left, Scale& s) {
+  f32x2 x[2] = {given[0], given[1]};
+  float low = min_nan(min_nan(lo32(x[0]), hi32(x[0]), lo32(x[1])), hi32(x[1])), high = max_nan(max_nan(lo32(x[0]), hi32(x[0]), lo32(x[1])), hi32(x[1]));
+  if (left < 4) {  // the columns that are not there have the first one's value; without any, nobody's extreme
+    const float first = lo32(x[0]);
+    const float second = left > 1 ? hi32(x[0]) : first, third = left > 2 ? lo32(x[1]) : first;
+    x[0] = pair_of(first, second);
+    x[1] = pair_of(third, first);
+    low = left > 0 ? min_nan(first, second, third) : __int_as_float(0x7f800000);
+    high = left > 0 ? max_nan(first, second, third) : __int_as_float(0xff800000);
   }
-  const float low = warp_min_nan(min_nan(min_nan(x[0], x[1]), min_nan(x[2], x[3])));
-  float high = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
-  if (left <= 0) high = __int_as_float(0xff800000);
+  low = warp_min_nan(low);
   high = warp_max_nan(high);
   const float range = high - low;
-  if (!(range <= 3.402823466e38f)) {  // infinite, or no number
-    s.step = s.low = __int_as_float(0x7fffffff);
-    return 0u;
-  }
   s.low = low;
   // range / 255 by two corrections with exact remainders; the ordinary division where they would not be exact
+  s.step = div_exact_fast(range, 255.0f, 1.0f / 255.0f);
   const bool plain = range > 1e-25f && range < 1e30f;
-  if (plain) s.step = div_exact_fast(range, 255.0f, 1.0f / 255.0f);
-  else s.step = range / 255.0f;
-  if (s.step == 0.0f) return 0u;
-  if (!plain) return encode_by_division(x[0], x[1], x[2], x[3], low, s.step, left);
-  const float by = reciprocal_near(s.step), magic = 12582912.0f;
-  const unsigned long long by2 = pair_of(by, by), low2 = pair_of(-low, -low), magic2 = pair_of(magic, magic), less2 = pair_of(-magic, -magic), minus2 = pair_of(-1.0f, -1.0f);
-  unsigned long long q[2] = {pair_of(x[0], x[1]), pair_of(x[2], x[3])}, m[2];
+  if (!plain) {
+    if (!(range <= 3.402823466e38f)) {  // infinite, or no number
+      s.step = s.low = __int_as_float(0x7fffffff);
+      return 0u;
+    }
+    s.step = range / 255.0f;
+    if (s.step == 0.0f) return 0u;
+    return encode_by_division(lo32(x[0]), hi32(x[0]), lo32(x[1]), hi32(x[1]), low, s.step, left);
+  }
+  const f32x2 by = both(reciprocal_near(s.step)), less = both(-low), magic = both(12582912.0f), back = both(-12582912.0f), minus = both(-1.0f);
+  f32x2 q[2], m[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    add2(q[h], low2);
-    q[h] = mul2(q[h], by2);
-    m[h] = q[h];
-    add2(m[h], magic2);
-    unsigned long long r = m[h];
-    add2(r, less2);
-    q[h] = fma2(r, minus2, q[h]);  // from the nearest whole number: exact
+    q[h] = mul2(plus2(x[h], less), by);
+    m[h] = plus2(q[h], magic);
+    q[h] = fma2(plus2(m[h], back), minus, q[h]);  // from the nearest whole number: exact
   }
   const float far = fmaxf(fmaxf(fabsf(lo32(q[0])), fabsf(hi32(q[0]))), fmaxf(fabsf(lo32(q[1])), fabsf(hi32(q[1]))));
-  if (far > 0.5f - 1e-4f && left > 0) return encode_by_division(x[0], x[1], x[2], x[3], low, s.step, left);
+  if (far > 0.5f - 1e-4f) return encode_by_division(lo32(x[0]), hi32(x[0]), lo32(x[1]), hi32(x[1]), low, s.step, left);
   const uint32_t codes = __byte_perm(__byte_perm((uint32_t)m[0], (uint32_t)(m[0] >> 32), 0x0040), __byte_perm((uint32_t)m[1], (uint32_t)(m[1] >> 32), 0x0040), 0x5410);
   return left >= 4 ? codes : left <= 0 ? 0u : codes & ((1u << (8 * left)) - 1u);
 }
 
-__device__ __forceinline__ void decode(uint32_t codes, Scale s, float (&x)[4]) {
+// The codes as numbers: 2^23 + q, less 2^23.
+__device__ __forceinline__ void numbers_of(uint32_t codes, f32x2 (&q)[2]) {
+  q[0] = plus2(pair_of(__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7441))), both(-8388608.0f));
+  q[1] = plus2(pair_of(__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7443))), both(-8388608.0f));
+}
+__device__ __forceinline__ void decode(uint32_t codes, Scale s, f32x2 (&x)[2]) {
+  numbers_of(codes, x);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = fmaf(s.step, (float)((codes >> (8 * e)) & 255u), s.low);
+  for (int h = 0; h < 2; ++h) x[h] = fma2(both(s.step), x[h], both(s.low));
 }
 
 __device__ __forceinline__ Scale load_scale(const float* at) {

@@ -12,8 +12,13 @@
 namespace f2c {
 namespace emb {
 
+using ckpt::both;
+using ckpt::f32x2;
 using ckpt::Four;
 using ckpt::kGroup;
+using ckpt::mul2;
+using ckpt::pair_of;
+using ckpt::plus2;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kAhead = 4;
 constexpr int64_t kMaxRows = (1ll << 31) - 2, kMaxPlaces = 1ll << 30, kMaxColumns = 1 << 20;
@@ -298,12 +303,12 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
     // rows behind the last segment's are zero
     for (int64_t r = max(start, (int64_t)all); r < start + n; ++r) {
       Four<T, ACCESS> zero;
-      const float none[4] = {};
+      const f32x2 none[2] = {};
       zero.set(none);
       zero.store(out + r * d + col, left);
     }
   }
-  float acc[4] = {};
+  f32x2 acc[2] = {};
   bool head = (first & 1u) == 0u, opened = false;
   const auto flush = [&](int last) {  // the segment whose last place here is `last`
     const uint32_t k = __shfl_sync(0xffffffffu, key, last);
@@ -315,21 +320,20 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
     }
     if (head || goes_on) {
       float* const to = (head ? open.head : open.tail) + c * open.width + blockIdx.y * kGroup + 4 * lane;
-      *reinterpret_cast<float4*>(to) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<ulonglong2*>(to) = make_ulonglong2(acc[0], acc[1]);
       if (!head) {
         opened = true;
         if (lane == 0 && blockIdx.y == 0) open.row[c] = row;
       }
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] *= scale;
+      acc[0] = mul2(acc[0], both(scale));
+      acc[1] = mul2(acc[1], both(scale));
       Four<T, ACCESS> v;
       v.set(acc);
       v.store(out + row * d + col, left);
     }
     head = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = 0.0f;
+    acc[0] = acc[1] = 0ull;
   };
   for (int t0 = 0; t0 < kept; t0 += kRowsAhead) {
     Four<T, ACCESS> v[kRowsAhead];
@@ -343,10 +347,10 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
       const int t = t0 + q;
       if (t >= kept) break;
       if (t > 0 && ((first >> t) & 1u)) flush(t - 1);
-      float f[4];
+      f32x2 f[2];
       v[q].get(f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += f[e];
+      acc[0] = plus2(acc[0], f[0]);
+      acc[1] = plus2(acc[1], f[1]);
     }
   }
   if (kept > 0) flush(kept - 1);
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
 constexpr int kShort = 16;
 template <typename T, int ACCESS>
 __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, const __grid_constant__ Segments s, const __grid_constant__ Open open, T* __restrict__ out) {
-  __shared__ float sums[kWarps][kGroup];
+  __shared__ __align__(16) float sums[kWarps][kGroup];
   __shared__ int64_t long_row[kWarps];
   dependency_wait();
   release_dependents();
@@ -367,13 +371,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, cons
   const int64_t row = c < s.stretches ? open.row[c] : -1;
   const auto key_of_tail = [&](int64_t q) { return s.key[(q + 1) * s.stretch - 1]; };
   const auto goes_on = [&](int64_t q, uint32_t key) { return q < s.stretches && s.key[q * s.stretch] == key; };
-  const auto add = [&](float (&acc)[4], const float* from, int64_t q) {
+  const auto add = [&](f32x2 (&acc)[2], const float* from, int64_t q) {
     const float4 v = __ldg(reinterpret_cast<const float4*>(from + q * open.width + blockIdx.y * kGroup + 4 * lane));
-    acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
+    acc[0] = plus2(acc[0], pair_of(v.x, v.y));
+    acc[1] = plus2(acc[1], pair_of(v.z, v.w));
   };
-  const auto write = [&](int64_t to, float (&acc)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= scale;
+  const auto write = [&](int64_t to, f32x2 (&acc)[2]) {
+    acc[0] = mul2(acc[0], both(scale));
+    acc[1] = mul2(acc[1], both(scale));
     Four<T, ACCESS> v;
     v.set(acc);
     v.store(out + to * d + col, d - col);
@@ -383,7 +388,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, cons
     const uint32_t key = key_of_tail(c);
     is_long = goes_on(c + kShort, key);
     if (!is_long) {
-      float acc[4] = {};
+      f32x2 acc[2] = {};
       add(acc, open.tail, c);
       for (int64_t q = c + 1; goes_on(q, key); ++q) add(acc, open.head, q);
       write(row, acc);
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, cons
   for (int w = 0; w < kWarps; ++w) {
     if (long_row[w] < 0) continue;  // for all threads alike
     const uint32_t key = key_of_tail(c0 + w);
-    float acc[4] = {};
+    f32x2 acc[2] = {};
     if (warp == 0) add(acc, open.tail, c0 + w);
     int64_t q = c0 + w + 1 + warp;
     for (; goes_on(q + 3 * kWarps, key); q += 4 * kWarps) {  // (stretches of a segment lie side by side)
@@ -402,14 +407,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, cons
       for (int u = 0; u < 4; ++u) add(acc, open.head, q + u * kWarps);
     }
     for (; goes_on(q, key); q += kWarps) add(acc, open.head, q);
-    *reinterpret_cast<float4*>(&sums[warp][4 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    *reinterpret_cast<ulonglong2*>(&sums[warp][4 * lane]) = make_ulonglong2(acc[0], acc[1]);
     __syncthreads();
     if (warp == 0) {
-      float all[4] = {};
+      f32x2 all[2] = {};
 #pragma unroll
-      for (int u = 0; u < kWarps; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) all[e] += sums[u][4 * lane + e];
+      for (int u = 0; u < kWarps; ++u) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sums[u][4 * lane]);
+        all[0] = plus2(all[0], v.x);
+        all[1] = plus2(all[1], v.y);
+      }
       write(long_row[w], all);
     }
     __syncthreads();

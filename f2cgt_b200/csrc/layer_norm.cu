@@ -10,8 +10,14 @@
 namespace f2c {
 namespace ln {
 
+using ckpt::both;
+using ckpt::f32x2;
+using ckpt::fma2;
 using ckpt::Four;
 using ckpt::kGroup;
+using ckpt::mul2;
+using ckpt::pair_of;
+using ckpt::plus2;
 
 struct Args {
   const void* x;
@@ -33,38 +39,51 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // of four values of columns [at, at + 4) of a vector that starts anywhere
-__device__ __forceinline__ void of_columns(const float* w, int at, int left, float otherwise, float (&v)[4]) {
+__device__ __forceinline__ void of_columns(const float* w, int at, int left, float otherwise, f32x2 (&v)[2]) {
   if (w == nullptr || left <= 0) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = otherwise;
+    v[0] = v[1] = both(otherwise);
   } else if (left >= 4 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
     const float4 f = __ldg(reinterpret_cast<const float4*>(w + at));
-    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    v[0] = pair_of(f.x, f.y);
+    v[1] = pair_of(f.z, f.w);
   } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = e < left ? __ldg(w + at + e) : otherwise;
+    const float f0 = __ldg(w + at), f1 = left > 1 ? __ldg(w + at + 1) : otherwise, f2 = left > 2 ? __ldg(w + at + 2) : otherwise, f3 = left > 3 ? __ldg(w + at + 3) : otherwise;
+    v[0] = pair_of(f0, f1);
+    v[1] = pair_of(f2, f3);
   }
 }
 
+// Squares of the differences from the mean, of the columns that there are.
+__device__ __forceinline__ f32x2 add_squares(const f32x2 (&x)[2], f32x2 less, int left, f32x2 sum) {
+  f32x2 t[2] = {plus2(x[0], less), plus2(x[1], less)};
+  if (left < 4) {
+    t[0] = left > 1 ? t[0] : left > 0 ? pair_of(lo32(t[0]), 0.0f) : 0ull;
+    t[1] = left > 2 ? pair_of(lo32(t[1]), 0.0f) : 0ull;
+  }
+  return fma2(t[1], t[1], fma2(t[0], t[0], sum));
+}
+__device__ __forceinline__ float sum_of(f32x2 v) { return lo32(v) + hi32(v); }
+
 // Everything that a lane writes of four columns of a row; by whole warps.
 template <typename T, int ACCESS>
-__device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, const float (&x)[4], float mean, float rstd, const float (&w)[4], const float (&b)[4]) {
+__device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, const f32x2 (&x)[2], float mean, float rstd, const f32x2 (&w)[2], const f32x2 (&b)[2]) {
   const int lane = threadIdx.x & 31, col = chunk * kGroup + 4 * lane, left = a.d - col;
-  float z[4];
-  uint32_t bits = 0u;
+  f32x2 z[2];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    z[e] = fmaf((x[e] - mean) * rstd, w[e], b[e]);
-    if (e < left && z[e] > 0.0f) bits |= 1u << e;
-    if (a.relu && z[e] < 0.0f) z[e] = 0.0f;  // (a NaN stays one)
+  for (int h = 0; h < 2; ++h) z[h] = fma2(mul2(plus2(x[h], both(-mean)), both(rstd)), w[h], b[h]);
+  if (a.active != nullptr) {
+    uint32_t bits = (lo32(z[0]) > 0.0f) | (hi32(z[0]) > 0.0f) << 1 | (lo32(z[1]) > 0.0f) << 2 | (hi32(z[1]) > 0.0f) << 3;
+    if (left < 4) bits &= (1u << max(left, 0)) - 1u;
+    bits |= __shfl_down_sync(0xffffffffu, bits, 1) << 4;
+    if ((lane & 1) == 0 && left > 0) a.active[row * ((a.d + 7) >> 3) + (col >> 3)] = (uint8_t)bits;
+  }
+  if (a.relu) {  // (a NaN stays one)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) z[h] = pair_of(ckpt::max_nan(lo32(z[h]), 0.0f), ckpt::max_nan(hi32(z[h]), 0.0f));
   }
   Four<T, ACCESS> out;
   out.set(z);
   out.store((T*)a.y + row * a.d + col, left);
-  if (a.active != nullptr) {
-    bits |= __shfl_down_sync(0xffffffffu, bits, 1) << 4;
-    if ((lane & 1) == 0 && left > 0) a.active[row * ((a.d + 7) >> 3) + (col >> 3)] = (uint8_t)bits;
-  }
   if (a.codes.codes != nullptr) {
     ckpt::Scale s;
     const uint32_t q = ckpt::encode(x, left, s);
@@ -91,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 2) warp_kernel(const __grid_constant
       raw[r][c].load((const T*)a.x + (first + r) * a.ldx + col, first + r < a.m ? a.d - col : 0);
     }
   constexpr int kHeld = ROWS > 1 ? CHUNKS : 0;  // weights used more than once
-  float w[kHeld + 1][4], b[kHeld + 1][4];
+  f32x2 w[kHeld + 1][2], b[kHeld + 1][2];
 #pragma unroll
   for (int c = 0; c < kHeld; ++c) {
     const int col = c * kGroup + 4 * lane;
@@ -103,22 +122,16 @@ __global__ void __launch_bounds__(kThreads, 2) warp_kernel(const __grid_constant
   for (int r = 0; r < ROWS; ++r) {
     const int64_t row = first + r;
     if (row >= a.m) return;  // all threads of the warp
-    float x[CHUNKS][4], sum = 0.0f;
+    f32x2 x[CHUNKS][2], sum = 0ull, squares = 0ull;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       raw[r][c].get(x[c]);
-      sum += (x[c][0] + x[c][1]) + (x[c][2] + x[c][3]);
+      sum = plus2(plus2(sum, x[c][0]), x[c][1]);
     }
-    const float mean = warp_sum(sum) / n;
-    float squares = 0.0f;
+    const float mean = warp_sum(sum_of(sum)) / n;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float t = c * kGroup + 4 * lane + e < a.d ? x[c][e] - mean : 0.0f;
-        squares = fmaf(t, t, squares);
-      }
-    const float rstd = 1.0f / sqrtf(warp_sum(squares) / n + a.eps);
+    for (int c = 0; c < CHUNKS; ++c) squares = add_squares(x[c], both(-mean), a.d - c * kGroup - 4 * lane, squares);
+    const float rstd = 1.0f / sqrtf(warp_sum(sum_of(squares)) / n + a.eps);
     if (lane == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
@@ -164,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __g
     }
   };
   fetch(blockIdx.x);
-  float w[KEPT][4], b[KEPT][4];
+  f32x2 w[KEPT][2], b[KEPT][2];
 #pragma unroll
   for (int k = 0; k < KEPT; ++k) {
     const int col = (warp + k * kWarps) * kGroup + 4 * lane;
@@ -173,24 +186,18 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __g
   }
   const float n = (float)a.d;
   for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
-    float x[KEPT][4], sum = 0.0f;
+    f32x2 x[KEPT][2], sum = 0ull, squares = 0ull;
 #pragma unroll
     for (int k = 0; k < KEPT; ++k) {
       next[k].get(x[k]);
-      sum += (x[k][0] + x[k][1]) + (x[k][2] + x[k][3]);
+      sum = plus2(plus2(sum, x[k][0]), x[k][1]);
     }
     fetch(row + gridDim.x);
     // (the barrier of one sum keeps the reads of the other's apart from the next row's writes)
-    const float mean = block_sum<THREADS>(sum, of_warp[0]) / n;
-    float squares = 0.0f;
+    const float mean = block_sum<THREADS>(sum_of(sum), of_warp[0]) / n;
 #pragma unroll
-    for (int k = 0; k < KEPT; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float t = (warp + k * kWarps) * kGroup + 4 * lane + e < a.d ? x[k][e] - mean : 0.0f;
-        squares = fmaf(t, t, squares);
-      }
-    const float rstd = 1.0f / sqrtf(block_sum<THREADS>(squares, of_warp[1]) / n + a.eps);
+    for (int k = 0; k < KEPT; ++k) squares = add_squares(x[k], both(-mean), a.d - (warp + k * kWarps) * kGroup - 4 * lane, squares);
+    const float rstd = 1.0f / sqrtf(block_sum<THREADS>(sum_of(squares), of_warp[1]) / n + a.eps);
     if (threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
@@ -216,7 +223,7 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
   const auto each = [&](auto&& body) {  // every chunk of this warp
     for (int c = warp; c < chunks; c += kWarps) {
       Four<T, ACCESS> v;
-      float x[4];
+      f32x2 x[2];
       const int col = c * kGroup + 4 * lane;
       v.load(from + col, a.d - col);
       v.get(x);
@@ -224,24 +231,17 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
     }
   };
   const float n = (float)a.d;
-  float sum = 0.0f;
-  each([&](int, int, const float (&x)[4]) { sum += (x[0] + x[1]) + (x[2] + x[3]); });
-  const float mean = block_sum<512>(sum, of_warp[0]) / n;
-  float squares = 0.0f;
-  each([&](int, int col, const float (&x)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float t = col + e < a.d ? x[e] - mean : 0.0f;
-      squares = fmaf(t, t, squares);
-    }
-  });
-  const float rstd = 1.0f / sqrtf(block_sum<512>(squares, of_warp[1]) / n + a.eps);
+  f32x2 sum = 0ull, squares = 0ull;
+  each([&](int, int, const f32x2 (&x)[2]) { sum = plus2(plus2(sum, x[0]), x[1]); });
+  const float mean = block_sum<512>(sum_of(sum), of_warp[0]) / n;
+  each([&](int, int col, const f32x2 (&x)[2]) { squares = add_squares(x, both(-mean), a.d - col, squares); });
+  const float rstd = 1.0f / sqrtf(block_sum<512>(sum_of(squares), of_warp[1]) / n + a.eps);
   if (threadIdx.x == 0 && a.mean != nullptr) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
   }
-  each([&](int c, int col, const float (&x)[4]) {
-    float w[4], b[4];
+  each([&](int c, int col, const f32x2 (&x)[2]) {
+    f32x2 w[2], b[2];
     of_columns(a.weight, col, a.d - col, 1.0f, w);
     of_columns(a.bias, col, a.d - col, 0.0f, b);
     finish<T, ACCESS>(a, row, c, x, mean, rstd, w, b);

@@ -12,8 +12,14 @@
 namespace f2c {
 namespace ln {
 
+using ckpt::both;
+using ckpt::f32x2;
+using ckpt::fma2;
 using ckpt::Four;
 using ckpt::kGroup;
+using ckpt::mul2;
+using ckpt::pair_of;
+using ckpt::plus2;
 
 struct Back {
   const void* dy;
@@ -50,23 +56,27 @@ struct Columns {
     open = 15u;
     if (a.active != nullptr) open = left > 0 ? (uint32_t)__ldg(a.active + row * ((a.d + 7) >> 3) + (col >> 3)) >> (4 * (lane & 1)) : 0u;
   }
-  // g and h; columns that do not exist have neither
-  __device__ __forceinline__ void get(float mean, float rstd, int left, float (&g)[4], float (&h)[4]) const {
+  // g and h; columns that do not exist have no g (what they have for h meets nothing else)
+  __device__ __forceinline__ void get(bool masked, float mean, float rstd, f32x2 (&g)[2], f32x2 (&h)[2]) const {
     dy.get(g);
+    if (masked) {
+      g[0] = pair_of(open & 1u ? lo32(g[0]) : 0.0f, open & 2u ? hi32(g[0]) : 0.0f);
+      g[1] = pair_of(open & 4u ? lo32(g[1]) : 0.0f, open & 8u ? hi32(g[1]) : 0.0f);
+    }
     if constexpr (CODES) ckpt::decode(x, s, h);
     else x.get(h);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (!((open >> e) & 1u)) g[e] = 0.0f;
-      h[e] = e < left ? (h[e] - mean) * rstd : 0.0f;
-    }
+    for (int q = 0; q < 2; ++q) h[q] = mul2(plus2(h[q], both(-mean)), both(rstd));
   }
 };
 
-__device__ __forceinline__ void weights_of(const Back& a, int chunk, float (&w)[4]) {
+__device__ __forceinline__ void weights_of(const Back& a, int chunk, f32x2 (&w)[2]) {
   const int col = chunk * kGroup + 4 * (threadIdx.x & 31);
+  float f[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = col + e < a.d ? (a.weight != nullptr ? __ldg(a.weight + col + e) : 1.0f) : 0.0f;
+  for (int e = 0; e < 4; ++e) f[e] = col + e < a.d ? (a.weight != nullptr ? __ldg(a.weight + col + e) : 1.0f) : 0.0f;
+  w[0] = pair_of(f[0], f[1]);
+  w[1] = pair_of(f[2], f[3]);
 }
 
 __device__ __forceinline__ void warp_sum2(float& u, float& v) {
@@ -103,11 +113,11 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
   };
   fetch(row);
   constexpr bool kHeld = WARPS < 16;  // (the widest rows' weights do not fit beside their sums: they are read again for every row)
-  float held[kHeld ? CHUNKS : 1][4], dw[CHUNKS][4], db[CHUNKS][4];
-  const auto weights = [&](int c, float (&w)[4]) {
+  f32x2 held[kHeld ? CHUNKS : 1][2], dw[CHUNKS][2], db[CHUNKS][2];
+  const auto weights = [&](int c, f32x2 (&w)[2]) {
     if constexpr (kHeld) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = held[c][e];
+      for (int q = 0; q < 2; ++q) w[q] = held[c][q];
     } else {
       weights_of(a, member + c * WARPS, w);
     }
@@ -116,9 +126,10 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
   for (int c = 0; c < CHUNKS; ++c) {
     if constexpr (kHeld) weights_of(a, member + c * WARPS, held[c]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dw[c][e] = db[c][e] = 0.0f;
+    for (int q = 0; q < 2; ++q) dw[c][q] = db[c][q] = 0ull;
   }
   const float n = (float)a.d;
+  const bool masked = a.active != nullptr;
   // (all warps of a row leave together)
   for (int turn = 0; row < a.m; row += stride, turn ^= 1) {
     const float mean = next_mean, rstd = next_rstd;
@@ -126,21 +137,22 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) now[c] = next[c];
     fetch(row + stride);
-    float u = 0.0f, v = 0.0f;
+    f32x2 us = 0ull, vs = 0ull;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      float g[4], h[4], w[4];
-      now[c].get(mean, rstd, a.d - (member + c * WARPS) * kGroup - 4 * lane, g, h);
+      f32x2 g[2], h[2], w[2];
+      now[c].get(masked, mean, rstd, g, h);
       weights(c, w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        dw[c][e] = fmaf(g[e], h[e], dw[c][e]);
-        db[c][e] += g[e];
-        const float gw = g[e] * w[e];
-        u += gw;
-        v = fmaf(gw, h[e], v);
+      for (int q = 0; q < 2; ++q) {
+        dw[c][q] = fma2(g[q], h[q], dw[c][q]);
+        db[c][q] = plus2(db[c][q], g[q]);
+        const f32x2 gw = mul2(g[q], w[q]);
+        us = plus2(us, gw);
+        vs = fma2(gw, h[q], vs);
       }
     }
+    float u = lo32(us) + hi32(us), v = lo32(vs) + hi32(vs);
     warp_sum2(u, v);
     if constexpr (!kAlone) {
       if (lane == 0) {
@@ -162,11 +174,11 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int col = (member + c * WARPS) * kGroup + 4 * lane, left = a.d - col;
-      float g[4], h[4], w[4];
-      now[c].get(mean, rstd, left, g, h);
+      f32x2 g[2], h[2], w[2];
+      now[c].get(masked, mean, rstd, g, h);
       weights(c, w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) g[e] = rstd * (fmaf(g[e], w[e], -u) - h[e] * v);
+      for (int q = 0; q < 2; ++q) g[q] = mul2(both(rstd), fma2(h[q], both(-v), fma2(g[q], w[q], both(-u))));
       Four<T, ACCESS> out;
       out.set(g);
       out.store((T*)a.dx + row * a.d + col, left);
@@ -179,8 +191,8 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int col = (member + c * WARPS) * kGroup + 4 * lane + e;
-        joined[col][warp / WARPS] = dw[c][e];
-        joined[kColumns + col][warp / WARPS] = db[c][e];
+        joined[col][warp / WARPS] = e & 1 ? hi32(dw[c][e / 2]) : lo32(dw[c][e / 2]);
+        joined[kColumns + col][warp / WARPS] = e & 1 ? hi32(db[c][e / 2]) : lo32(db[c][e / 2]);
       }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * a.d; i += THREADS) {
@@ -197,8 +209,8 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (col + e < a.d) {
-          part[col + e] = dw[c][e];
-          part[a.d + col + e] = db[c][e];
+          part[col + e] = e & 1 ? hi32(dw[c][e / 2]) : lo32(dw[c][e / 2]);
+          part[a.d + col + e] = e & 1 ? hi32(db[c][e / 2]) : lo32(db[c][e / 2]);
         }
     }
   }
@@ -215,29 +227,33 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Back 
   const int64_t row = blockIdx.x;
   const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row), n = (float)a.d;
   float u = 0.0f, v = 0.0f;
+  f32x2 us = 0ull, vs = 0ull;
   for (int pass = 0; pass < 2; ++pass) {
     for (int c = warp; c < chunks; c += kWarps) {
       Columns<T, ACCESS, CODES> now;
       now.load(a, row, c, true);
-      float g[4], h[4], w[4];
+      f32x2 g[2], h[2], w[2];
       const int col = c * kGroup + 4 * lane, left = a.d - col;
-      now.get(mean, rstd, left, g, h);
+      now.get(a.active != nullptr, mean, rstd, g, h);
       weights_of(a, c, w);
       if (pass == 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          u = fmaf(g[e], w[e], u);
-          v = fmaf(g[e] * w[e], h[e], v);
+        for (int q = 0; q < 2; ++q) {
+          const f32x2 gw = mul2(g[q], w[q]);
+          us = plus2(us, gw);
+          vs = fma2(gw, h[q], vs);
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) g[e] = rstd * (fmaf(g[e], w[e], -u) - h[e] * v);
+        for (int q = 0; q < 2; ++q) g[q] = mul2(both(rstd), fma2(h[q], both(-v), fma2(g[q], w[q], both(-u))));
         Four<T, ACCESS> out;
         out.set(g);
         out.store((T*)a.dx + row * a.d + col, left);
       }
     }
     if (pass == 0) {
+      u = lo32(us) + hi32(us);
+      v = lo32(vs) + hi32(vs);
       warp_sum2(u, v);
       if (lane == 0) {
         sums[0][warp] = u;
@@ -262,23 +278,23 @@ __global__ void __launch_bounds__(256) columns_kernel(const __grid_constant__ Ba
   __shared__ float joined[2 * kGroup][9];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.y * kGroup + 4 * lane;
-  float dw[4] = {}, db[4] = {};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  f32x2 dw[2] = {}, db[2] = {};
   for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < a.m; row += (int64_t)gridDim.x * 8) {
     Columns<T, ACCESS, CODES> now;
     now.load(a, row, blockIdx.y, true);
-    float g[4], h[4];
-    now.get(__ldg(a.mean + row), __ldg(a.rstd + row), a.d - col, g, h);
+    f32x2 g[2], h[2];
+    now.get(a.active != nullptr, __ldg(a.mean + row), __ldg(a.rstd + row), g, h);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      dw[e] = fmaf(g[e], h[e], dw[e]);
-      db[e] += g[e];
+    for (int q = 0; q < 2; ++q) {
+      dw[q] = fma2(g[q], h[q], dw[q]);
+      db[q] = plus2(db[q], g[q]);
     }
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    joined[4 * lane + e][warp] = dw[e];
-    joined[kGroup + 4 * lane + e][warp] = db[e];
+    joined[4 * lane + e][warp] = e & 1 ? hi32(dw[e / 2]) : lo32(dw[e / 2]);
+    joined[kGroup + 4 * lane + e][warp] = e & 1 ? hi32(db[e / 2]) : lo32(db[e / 2]);
   }
   __syncthreads();
   const int which = threadIdx.x / kGroup, c = threadIdx.x % kGroup, at = blockIdx.y * kGroup + c;
