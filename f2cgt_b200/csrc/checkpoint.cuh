@@ -133,12 +133,6 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 
 struct Scale { float step, low; };
 
-__device__ __forceinline__ float reciprocal_near(float v) {  // one unit in the last place off
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // Codes of four columns of which `left` exist, by divisions.
 static __device__ __noinline__ uint32_t encode_by_division(float x0, float x1, float x2, float x3, float low, float step, int left) {
   const float x[4] = {x0, x1, x2, x3};
@@ -149,10 +143,10 @@ static __device__ __noinline__ uint32_t encode_by_division(float x0, float x1, f
   return codes;
 }
 
-// Codes of a group, four columns a lane of which `left` exist (the others' codes are 0); by whole warps.  The quotient is a product with the
-// reciprocal, at most 255 * 4 * 2^-24 = 6.1e-5 off what the division gives; only where it lies so near to a tie that this could matter, or where the
-// step is so small that the reciprocal is none, is the division made (one warp in forty; a division each took 60 us for 8192 x 4096 bfloat16).  2^23 + 2^22
-// added to a number below 2^22 rounds it to even and leaves it in the last bits.
+// Codes of a group, four columns a lane of which `left` exist (the others' codes are 0); by whole warps.  The quotients are what division gives: the
+// product with the correctly rounded reciprocal, and two corrections with exact remainders (Markstein).  (Corrected only where the product lay near a tie: rows
+// of 16-bit numbers, whose quotients are ties as often as not somewhere in a group, took twice the time.)  2^23 + 2^22 added to a number below 2^22 rounds it to
+// even and leaves it in the last bits.
 __device__ __forceinline__ uint32_t encode(const f32x2 (&given)[2], int left, Scale& s) {
   f32x2 x[2] = {given[0], given[1]};
   float low = min_nan(min_nan(lo32(x[0]), hi32(x[0]), lo32(x[1])), hi32(x[1])), high = max_nan(max_nan(lo32(x[0]), hi32(x[0]), lo32(x[1])), hi32(x[1]));
@@ -180,16 +174,16 @@ __device__ __forceinline__ uint32_t encode(const f32x2 (&given)[2], int left, Sc
     if (s.step == 0.0f) return 0u;
     return encode_by_division(lo32(x[0]), hi32(x[0]), lo32(x[1]), hi32(x[1]), low, s.step, left);
   }
-  const f32x2 by = both(reciprocal_near(s.step)), less = both(-low), magic = both(12582912.0f), back = both(-12582912.0f), minus = both(-1.0f);
-  f32x2 q[2], m[2];
+  const f32x2 by = both(__frcp_rn(s.step)), less = both(-low), minus = both(-s.step), magic = both(12582912.0f);
+  f32x2 m[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    q[h] = mul2(plus2(x[h], less), by);
-    m[h] = plus2(q[h], magic);
-    q[h] = fma2(plus2(m[h], back), minus, q[h]);  // from the nearest whole number: exact
+    const f32x2 over = plus2(x[h], less);
+    f32x2 q = mul2(over, by);
+    q = fma2(fma2(q, minus, over), by, q);
+    q = fma2(fma2(q, minus, over), by, q);
+    m[h] = plus2(q, magic);
   }
-  const float far = fmaxf(fmaxf(fabsf(lo32(q[0])), fabsf(hi32(q[0]))), fmaxf(fabsf(lo32(q[1])), fabsf(hi32(q[1]))));
-  if (far > 0.5f - 1e-4f) return encode_by_division(lo32(x[0]), hi32(x[0]), lo32(x[1]), hi32(x[1]), low, s.step, left);
   const uint32_t codes = __byte_perm(__byte_perm((uint32_t)m[0], (uint32_t)(m[0] >> 32), 0x0040), __byte_perm((uint32_t)m[1], (uint32_t)(m[1] >> 32), 0x0040), 0x5410);
   return left >= 4 ? codes : left <= 0 ? 0u : codes & ((1u << (8 * left)) - 1u);
 }

@@ -109,10 +109,10 @@ __global__ void __launch_bounds__(kThreads, 2) warp_kernel(const __grid_constant
       const int col = c * kGroup + 4 * lane;
       raw[r][c].load((const T*)a.x + (first + r) * a.ldx + col, first + r < a.m ? a.d - col : 0);
     }
-  constexpr int kHeld = ROWS > 1 ? CHUNKS : 0;  // weights used more than once
+  constexpr int kHeld = ROWS > 1 ? CHUNKS : 0;  // weights used more than once; otherwise the first chunk's
   f32x2 w[kHeld + 1][2], b[kHeld + 1][2];
 #pragma unroll
-  for (int c = 0; c < kHeld; ++c) {
+  for (int c = 0; c < (kHeld > 0 ? kHeld : 1); ++c) {
     const int col = c * kGroup + 4 * lane;
     of_columns(a.weight, col, a.d - col, 1.0f, w[c]);
     of_columns(a.bias, col, a.d - col, 0.0f, b[c]);
@@ -139,12 +139,22 @@ __global__ void __launch_bounds__(kThreads, 2) warp_kernel(const __grid_constant
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       if (c * kGroup >= a.d) break;
-      const int at = kHeld > 0 ? c : 0, col = c * kGroup + 4 * lane;
-      if constexpr (kHeld == 0) {
-        of_columns(a.weight, col, a.d - col, 1.0f, w[0]);
-        of_columns(a.bias, col, a.d - col, 0.0f, b[0]);
+      if constexpr (kHeld > 0) {
+        finish<T, ACCESS>(a, row, c, x[c], mean, rstd, w[c], b[c]);
+      } else {  // the next chunk's are on the way meanwhile
+        const int col = (c + 1) * kGroup + 4 * lane;
+        f32x2 w_next[2], b_next[2];
+        if (c + 1 < CHUNKS) {
+          of_columns(a.weight, col, a.d - col, 1.0f, w_next);
+          of_columns(a.bias, col, a.d - col, 0.0f, b_next);
+        }
+        finish<T, ACCESS>(a, row, c, x[c], mean, rstd, w[0], b[0]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          w[0][h] = w_next[h];
+          b[0][h] = b_next[h];
+        }
       }
-      finish<T, ACCESS>(a, row, c, x[c], mean, rstd, w[at], b[at]);
     }
   }
 }
