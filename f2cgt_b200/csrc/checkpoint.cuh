@@ -38,6 +38,23 @@ __device__ __forceinline__ f32x2 plus2(f32x2 a, f32x2 b) {
   return a;
 }
 
+// 0 without a load when !on; no branch.  (Narrow loads of neighbouring lanes share sectors: they may stay in L1.)
+__device__ __forceinline__ uint2 ld_u64_if(const void* p, bool on) {
+  uint2 v = make_uint2(0u, 0u);
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %3, 0;\n\t@q ld.global.nc.v2.u32 {%0,%1}, [%2];\n\t}" : "+r"(v.x), "+r"(v.y) : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_u32_if(const void* p, bool on) {
+  uint32_t v = 0u;
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.nc.u32 %0, [%1];\n\t}" : "+r"(v) : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+__device__ __forceinline__ uint16_t ld_u16_if(const void* p, bool on) {
+  uint16_t v = 0;
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.nc.u16 %0, [%1];\n\t}" : "+h"(v) : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+
 // Four columns of a row as they are in memory.  ACCESS: bytes of a load or store, by what the rows' alignment and length allow.
 template <typename T, int ACCESS>
 struct alignas(4 * sizeof(T)) Four {
@@ -55,9 +72,9 @@ struct alignas(4 * sizeof(T)) Four {
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) {
         const bool here = p * kEach < left;
-        if constexpr (ACCESS == 8) *reinterpret_cast<uint2*>(v + p * kEach) = here ? __ldg(reinterpret_cast<const uint2*>(at) + p) : make_uint2(0u, 0u);
-        else if constexpr (ACCESS == 4) *reinterpret_cast<uint32_t*>(v + p * kEach) = here ? __ldg(reinterpret_cast<const uint32_t*>(at) + p) : 0u;
-        else *reinterpret_cast<uint16_t*>(v + p) = here ? __ldg(reinterpret_cast<const uint16_t*>(at) + p) : (uint16_t)0;
+        if constexpr (ACCESS == 8) *reinterpret_cast<uint2*>(v + p * kEach) = ld_u64_if(at + p * kEach, here);
+        else if constexpr (ACCESS == 4) *reinterpret_cast<uint32_t*>(v + p * kEach) = ld_u32_if(at + p * kEach, here);
+        else *reinterpret_cast<uint16_t*>(v + p) = ld_u16_if(at + p, here);
       }
     }
   }

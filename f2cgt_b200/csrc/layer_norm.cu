@@ -23,6 +23,7 @@ struct Args {
   const void* x;
   int64_t ldx, m;
   int d;
+  float per_column;            // 1 / d
   const float *weight, *bias;  // null: 1, 0
   float eps;
   int relu;
@@ -64,10 +65,10 @@ __device__ __forceinline__ f32x2 add_squares(const f32x2 (&x)[2], f32x2 less, in
 }
 __device__ __forceinline__ float sum_of(f32x2 v) { return lo32(v) + hi32(v); }
 
-// Everything that a lane writes of four columns of a row; by whole warps.
+// Everything that a lane writes of four columns of a row, of which `left` exist; by whole warps.
 template <typename T, int ACCESS>
-__device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, const f32x2 (&x)[2], float mean, float rstd, const f32x2 (&w)[2], const f32x2 (&b)[2]) {
-  const int lane = threadIdx.x & 31, col = chunk * kGroup + 4 * lane, left = a.d - col;
+__device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, int left, const f32x2 (&x)[2], float mean, float rstd, const f32x2 (&w)[2], const f32x2 (&b)[2]) {
+  const int lane = threadIdx.x & 31, col = chunk * kGroup + 4 * lane;
   f32x2 z[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) z[h] = fma2(mul2(plus2(x[h], both(-mean)), both(rstd)), w[h], b[h]);
@@ -94,30 +95,26 @@ __device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, co
 
 constexpr int kThreads = 256;
 
-// ROWS rows of up to CHUNKS * 128 columns for every warp
-template <typename T, int ACCESS, int CHUNKS, int ROWS>
-__global__ void __launch_bounds__(kThreads, 2) warp_kernel(const __grid_constant__ Args a) {
+// ROWS rows of CHUNKS * 128 columns for every warp; the last chunk may have fewer, unless EVEN
+template <typename T, int ACCESS, int CHUNKS, int ROWS, bool EVEN>
+__global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 3 : 2) warp_kernel(const __grid_constant__ Args a) {
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * ROWS;
+  const auto left_of = [&](int c) { return EVEN || c + 1 < CHUNKS ? 4 : a.d - c * kGroup - 4 * lane; };
   Four<T, ACCESS> raw[ROWS][CHUNKS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      const int col = c * kGroup + 4 * lane;
-      raw[r][c].load((const T*)a.x + (first + r) * a.ldx + col, first + r < a.m ? a.d - col : 0);
-    }
-  constexpr int kHeld = ROWS > 1 ? CHUNKS : 0;  // weights used more than once; otherwise the first chunk's
-  f32x2 w[kHeld + 1][2], b[kHeld + 1][2];
+    for (int c = 0; c < CHUNKS; ++c) raw[r][c].load((const T*)a.x + (first + r) * a.ldx + c * kGroup + 4 * lane, first + r < a.m ? left_of(c) : 0);
+  constexpr int kHeld = ROWS > 1 ? CHUNKS : 1;  // of weights: all where they are used more than once, or the first chunk's
+  f32x2 w[kHeld][2], b[kHeld][2];
 #pragma unroll
-  for (int c = 0; c < (kHeld > 0 ? kHeld : 1); ++c) {
-    const int col = c * kGroup + 4 * lane;
-    of_columns(a.weight, col, a.d - col, 1.0f, w[c]);
-    of_columns(a.bias, col, a.d - col, 0.0f, b[c]);
+  for (int c = 0; c < kHeld; ++c) {
+    of_columns(a.weight, c * kGroup + 4 * lane, left_of(c), 1.0f, w[c]);
+    of_columns(a.bias, c * kGroup + 4 * lane, left_of(c), 0.0f, b[c]);
   }
-  const float n = (float)a.d;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int64_t row = first + r;
@@ -128,27 +125,25 @@ __global__ void __launch_bounds__(kThreads, 2) warp_kernel(const __grid_constant
       raw[r][c].get(x[c]);
       sum = plus2(plus2(sum, x[c][0]), x[c][1]);
     }
-    const float mean = warp_sum(sum_of(sum)) / n;
+    const float mean = warp_sum(sum_of(sum)) * a.per_column;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) squares = add_squares(x[c], both(-mean), a.d - c * kGroup - 4 * lane, squares);
-    const float rstd = 1.0f / sqrtf(warp_sum(sum_of(squares)) / n + a.eps);
+    for (int c = 0; c < CHUNKS; ++c) squares = add_squares(x[c], both(-mean), left_of(c), squares);
+    const float rstd = rsqrtf(fmaf(warp_sum(sum_of(squares)), a.per_column, a.eps));
     if (lane == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      if (c * kGroup >= a.d) break;
-      if constexpr (kHeld > 0) {
-        finish<T, ACCESS>(a, row, c, x[c], mean, rstd, w[c], b[c]);
-      } else {  // the next chunk's are on the way meanwhile
-        const int col = (c + 1) * kGroup + 4 * lane;
+      if constexpr (ROWS > 1) {
+        finish<T, ACCESS>(a, row, c, left_of(c), x[c], mean, rstd, w[c], b[c]);
+      } else {  // the next chunk's weights are on the way meanwhile
         f32x2 w_next[2], b_next[2];
         if (c + 1 < CHUNKS) {
-          of_columns(a.weight, col, a.d - col, 1.0f, w_next);
-          of_columns(a.bias, col, a.d - col, 0.0f, b_next);
+          of_columns(a.weight, (c + 1) * kGroup + 4 * lane, left_of(c + 1), 1.0f, w_next);
+          of_columns(a.bias, (c + 1) * kGroup + 4 * lane, left_of(c + 1), 0.0f, b_next);
         }
-        finish<T, ACCESS>(a, row, c, x[c], mean, rstd, w[0], b[0]);
+        finish<T, ACCESS>(a, row, c, left_of(c), x[c], mean, rstd, w[0], b[0]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           w[0][h] = w_next[h];
@@ -171,7 +166,7 @@ __device__ __forceinline__ float block_sum(float v, float* of_warp) {
 }
 
 // A CTA has every gridDim.x-th row: chunks warp, warp + THREADS / 32, ... are a warp's, all of which it keeps.
-template <typename T, int ACCESS, int THREADS, int KEPT>
+template <typename T, int ACCESS, int THREADS, int KEPT, bool EVEN>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __grid_constant__ Args a) {
   constexpr int kWarps = THREADS / 32;
   __shared__ float of_warp[2][kWarps];
@@ -186,6 +181,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __g
       next[k].load((const T*)a.x + row * a.ldx + col, row < a.m ? a.d - col : 0);
     }
   };
+  const int mine = max(0, min(KEPT, ((a.d + kGroup - 1) / kGroup - warp + kWarps - 1) / kWarps));  // chunks that there are
   fetch(blockIdx.x);
   f32x2 w[KEPT][2], b[KEPT][2];
 #pragma unroll
@@ -194,7 +190,6 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __g
     of_columns(a.weight, col, a.d - col, 1.0f, w[k]);
     of_columns(a.bias, col, a.d - col, 0.0f, b[k]);
   }
-  const float n = (float)a.d;
   for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
     f32x2 x[KEPT][2], sum = 0ull, squares = 0ull;
 #pragma unroll
@@ -204,18 +199,19 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __g
     }
     fetch(row + gridDim.x);
     // (the barrier of one sum keeps the reads of the other's apart from the next row's writes)
-    const float mean = block_sum<THREADS>(sum_of(sum), of_warp[0]) / n;
+    const float mean = block_sum<THREADS>(sum_of(sum), of_warp[0]) * a.per_column;
 #pragma unroll
-    for (int k = 0; k < KEPT; ++k) squares = add_squares(x[k], both(-mean), a.d - (warp + k * kWarps) * kGroup - 4 * lane, squares);
-    const float rstd = 1.0f / sqrtf(block_sum<THREADS>(sum_of(squares), of_warp[1]) / n + a.eps);
+    for (int k = 0; k < KEPT; ++k)
+      if (k < mine) squares = add_squares(x[k], both(-mean), EVEN ? 4 : a.d - (warp + k * kWarps) * kGroup - 4 * lane, squares);
+    const float rstd = rsqrtf(fmaf(block_sum<THREADS>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
     if (threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
 #pragma unroll
     for (int k = 0; k < KEPT; ++k) {
-      if ((warp + k * kWarps) * kGroup >= a.d) break;
-      finish<T, ACCESS>(a, row, warp + k * kWarps, x[k], mean, rstd, w[k], b[k]);
+      if (k >= mine) break;
+      finish<T, ACCESS>(a, row, warp + k * kWarps, EVEN ? 4 : a.d - (warp + k * kWarps) * kGroup - 4 * lane, x[k], mean, rstd, w[k], b[k]);
     }
   }
 }
@@ -240,12 +236,11 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
       body(c, col, x);
     }
   };
-  const float n = (float)a.d;
   f32x2 sum = 0ull, squares = 0ull;
   each([&](int, int, const f32x2 (&x)[2]) { sum = plus2(plus2(sum, x[0]), x[1]); });
-  const float mean = block_sum<512>(sum_of(sum), of_warp[0]) / n;
+  const float mean = block_sum<512>(sum_of(sum), of_warp[0]) * a.per_column;
   each([&](int, int col, const f32x2 (&x)[2]) { squares = add_squares(x, both(-mean), a.d - col, squares); });
-  const float rstd = 1.0f / sqrtf(block_sum<512>(sum_of(squares), of_warp[1]) / n + a.eps);
+  const float rstd = rsqrtf(fmaf(block_sum<512>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
   if (threadIdx.x == 0 && a.mean != nullptr) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
@@ -254,37 +249,44 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
     f32x2 w[2], b[2];
     of_columns(a.weight, col, a.d - col, 1.0f, w);
     of_columns(a.bias, col, a.d - col, 0.0f, b);
-    finish<T, ACCESS>(a, row, c, x, mean, rstd, w, b);
+    finish<T, ACCESS>(a, row, c, a.d - col, x, mean, rstd, w, b);
   });
 }
 
-template <typename T, int ACCESS, int CHUNKS, int ROWS>
+template <typename T, int ACCESS, int CHUNKS, int ROWS, bool EVEN>
 static void by_warps(const Args& a, cudaStream_t st) {
-  launch_dependent(warp_kernel<T, ACCESS, CHUNKS, ROWS>, dim3((unsigned)ceil_div(a.m, kThreads / 32 * ROWS)), kThreads, 0, st, a);
+  launch_dependent(warp_kernel<T, ACCESS, CHUNKS, ROWS, EVEN>, dim3((unsigned)ceil_div(a.m, kThreads / 32 * ROWS)), kThreads, 0, st, a);
 }
-
-template <typename T, int ACCESS, int THREADS, int KEPT>
+template <typename T, int ACCESS, int THREADS, int KEPT, bool EVEN>
 static void by_ctas(const Args& a, int resident, cudaStream_t st) {
   const int64_t most = (int64_t)resident * kSmCount;
-  launch_dependent(block_kernel<T, ACCESS, THREADS, KEPT>, dim3((unsigned)(a.m < most ? a.m : most)), THREADS, 0, st, a);
+  launch_dependent(block_kernel<T, ACCESS, THREADS, KEPT, EVEN>, dim3((unsigned)(a.m < most ? a.m : most)), THREADS, 0, st, a);
 }
 
-template <typename T, int ACCESS>
-static void run(const Args& a, cudaStream_t st) {
+template <typename T, int ACCESS, bool EVEN>
+static void by_size(const Args& a, cudaStream_t st) {
   switch ((a.d + kGroup - 1) / kGroup) {
-    case 1: return by_warps<T, ACCESS, 1, 4>(a, st);
-    case 2: return by_warps<T, ACCESS, 2, 2>(a, st);
-    case 3: return by_warps<T, ACCESS, 3, 1>(a, st);
-    case 4: return by_warps<T, ACCESS, 4, 1>(a, st);
-    case 5: return by_warps<T, ACCESS, 5, 1>(a, st);
-    case 6: return by_warps<T, ACCESS, 6, 1>(a, st);
-    case 7: case 8: return by_warps<T, ACCESS, 8, 1>(a, st);
+    case 1: return by_warps<T, ACCESS, 1, 4, EVEN>(a, st);
+    case 2: return by_warps<T, ACCESS, 2, 2, EVEN>(a, st);
+    case 3: return by_warps<T, ACCESS, 3, 1, EVEN>(a, st);
+    case 4: return by_warps<T, ACCESS, 4, 1, EVEN>(a, st);
+    case 5: return by_warps<T, ACCESS, 5, 1, EVEN>(a, st);
+    case 6: return by_warps<T, ACCESS, 6, 1, EVEN>(a, st);
+    case 7: return by_warps<T, ACCESS, 7, 1, EVEN>(a, st);
+    case 8: return by_warps<T, ACCESS, 8, 1, EVEN>(a, st);
     default: break;
   }
-  if (a.d <= 16 * kGroup) by_ctas<T, ACCESS, 256, 2>(a, 4, st);
-  else if (a.d <= 32 * kGroup) by_ctas<T, ACCESS, 256, 4>(a, 2, st);
-  else if (a.d <= 64 * kGroup) by_ctas<T, ACCESS, 512, 4>(a, 1, st);
+  if (a.d <= 16 * kGroup) by_ctas<T, ACCESS, 256, 2, EVEN>(a, 4, st);
+  else if (a.d <= 32 * kGroup) by_ctas<T, ACCESS, 256, 4, EVEN>(a, 2, st);
+  else if (a.d <= 64 * kGroup) by_ctas<T, ACCESS, 512, 4, EVEN>(a, 1, st);
   else launch_dependent(long_kernel<T, ACCESS>, dim3((unsigned)a.m), 512, 0, st, a);
+}
+template <typename T, int ACCESS>
+static void run(const Args& a, cudaStream_t st) {
+  if constexpr (ACCESS == 4 * (int)sizeof(T)) {
+    if (a.d % kGroup == 0) return by_size<T, ACCESS, true>(a, st);
+  }
+  by_size<T, ACCESS, false>(a, st);
 }
 
 }  // namespace ln
@@ -304,7 +306,7 @@ extern "C" int f2c_layer_norm(const void* x, int64_t ldx, int dtype, int64_t m, 
   F2C_REQUIRE(x && y, F2C_ERR_INVALID, "%s: null pointer", op);
   F2C_REQUIRE(m == 1 || ldx >= d, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
   F2C_REQUIRE(m < ckpt::kMaxRows, F2C_ERR_LIMIT, "%s: 2^31 rows", op);
-  const ln::Args a{x, ldx, m, (int)d, weight, bias, eps, relu, y, mean, rstd, active, ckpt::Codes{codes, ldq, scales, ceil_div(d, ckpt::kGroup)}};
+  const ln::Args a{x, ldx, m, (int)d, (float)(1.0 / (double)d), weight, bias, eps, relu, y, mean, rstd, active, ckpt::Codes{codes, ldq, scales, ceil_div(d, ckpt::kGroup)}};
   const int item = dtype_size(dtype), from = ckpt::access_of(x, ldx, m, d, item), to = ckpt::access_of(y, d, m, d, item);
   F2C_BY_ROWS(ln::run, dtype, (from < to ? from : to), a, (cudaStream_t)stream);
   return check_launch(op);
