@@ -5,8 +5,9 @@
 // a last launch.  No atomics on values: the same bits every time.  Sums are single precision, rounded once.
 //
 // Sorting.  Up to 4096 places each place counts the ones in front of it, in one launch: the keys are few enough that all pairs cost
-// less than further launches.  Beyond, digits of up to 11 bits from the lowest on: counts of every tile of 2048 places, their sums over tiles, and the
-// placing, in which a warp ranks 32 places at a time by their equals in it.  As many digits as the table has rows need.
+// less than further launches.  Beyond, digits of up to 11 bits from the lowest on: counts of every tile of 1024 places, their sums over tiles, and the
+// placing, in which a warp ranks 32 places at a time by their equals in it and counts the next digit where the places go.  As many digits as the table
+// has rows need.  All of it is latency - the first launch also clears what the others add to, and a whole table's gradient, on CTAs of its own.
 #include "checkpoint.cuh"
 
 namespace f2c {
@@ -55,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ 
 }
 
 // ---------------------------------------------------------------- sorting
-constexpr int kItems = 8, kTile = kThreads * kItems, kMaxBits = 11, kFew = 4096;
+constexpr int kItems = 4, kTile = kThreads * kItems, kMaxBits = 11, kFew = 4096;
 
 // A row's number, or the number of rows where the id is outside the table.
 template <typename I>
@@ -66,12 +67,32 @@ __device__ __forceinline__ uint32_t key_of(const I* ids, int64_t i, uint32_t row
 
 struct Pairs { uint32_t *key, *place; };
 
+// Memory that the first launch sets to zero on its CTAs behind the others, 16 bytes at a time: `whole` of them from a 16-byte boundary on, and single
+// bytes in front of and behind them.
+struct Clear {
+  uint8_t* at;
+  int64_t front, whole, behind;
+};
+struct Clears { Clear of[2]; };
+constexpr int kClearEach = 16;  // 16-byte words a thread
+__device__ __forceinline__ void clear(const Clears& c, int64_t cta, int64_t ctas) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const Clear& m = c.of[q];
+    uint4* const from = reinterpret_cast<uint4*>(m.at + m.front);
+    for (int64_t i = cta * kThreads + threadIdx.x; i < m.whole; i += ctas * kThreads) from[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (cta == 0 && threadIdx.x < m.front) m.at[threadIdx.x] = 0;
+    if (cta == 0 && threadIdx.x < m.behind) m.at[m.front + 16 * m.whole + threadIdx.x] = 0;
+  }
+}
+
 // Few places: a warp finds the ranks of four at a time.
 template <typename I>
-__global__ void __launch_bounds__(kThreads) rank_kernel(const I* __restrict__ ids, int m, uint32_t rows, Pairs out) {
+__global__ void __launch_bounds__(kThreads) rank_kernel(const I* __restrict__ ids, int m, uint32_t rows, Pairs out, int ctas, const __grid_constant__ Clears zero) {
   __shared__ uint32_t keys[kFew];
   dependency_wait();
   release_dependents();
+  if ((int)blockIdx.x >= ctas) return clear(zero, blockIdx.x - ctas, gridDim.x - ctas);
   for (int i = threadIdx.x; i < m; i += kThreads) keys[i] = key_of(ids, i, rows);
   __syncthreads();
   const int lane = threadIdx.x & 31, first = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * 4;
@@ -97,44 +118,58 @@ __global__ void __launch_bounds__(kThreads) rank_kernel(const I* __restrict__ id
 struct Digit { int shift, bits; };
 __device__ __forceinline__ uint32_t digit_of(uint32_t key, Digit d) { return (key >> d.shift) & ((1u << d.bits) - 1u); }
 
-// counts [digit][tile].  FIRST: keys come from ids.
-template <typename I, bool FIRST>
-__global__ void __launch_bounds__(kThreads) count_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t m, uint32_t rows, Digit d, uint32_t* __restrict__ counts,
-                                                         int tiles) {
+// counts [tile][digit] of the first digit
+template <typename I>
+__global__ void __launch_bounds__(kThreads) count_kernel(const I* __restrict__ ids, int64_t m, uint32_t rows, Digit d, uint32_t* __restrict__ counts, int tiles,
+                                                         const __grid_constant__ Clears zero) {
   __shared__ uint32_t here[1 << kMaxBits];
   dependency_wait();
   release_dependents();
+  if ((int)blockIdx.x >= tiles) return clear(zero, blockIdx.x - tiles, gridDim.x - tiles);
+  uint32_t key[kItems];
+  const int64_t first = (int64_t)blockIdx.x * kTile + threadIdx.x;
+#pragma unroll
+  for (int q = 0; q < kItems; ++q) key[q] = first + q * kThreads < m ? key_of(ids, first + q * kThreads, rows) : 0u;
   for (int b = threadIdx.x; b < 1 << d.bits; b += kThreads) here[b] = 0u;
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < kItems; ++q) {
-    const int64_t i = (int64_t)blockIdx.x * kTile + q * kThreads + threadIdx.x;
-    if (i < m) atomicAdd(here + digit_of(FIRST ? key_of(ids, i, rows) : keys[i], d), 1u);
-  }
+  for (int q = 0; q < kItems; ++q)
+    if (first + q * kThreads < m) atomicAdd(here + digit_of(key[q], d), 1u);
   __syncthreads();
-  for (int b = threadIdx.x; b < 1 << d.bits; b += kThreads) counts[(int64_t)b * tiles + blockIdx.x] = here[b];
+  for (int b = threadIdx.x; b < 1 << d.bits; b += kThreads) counts[((int64_t)blockIdx.x << d.bits) + b] = here[b];
 }
 
-// A warp to a digit: its counts become those of the tiles in front, and their sum goes to `totals`.
-__global__ void __launch_bounds__(kThreads) tiles_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, int tiles, int bins) {
+// A digit to a lane: its counts become those of the tiles in front, and their sum goes to `totals`.  Each of the CTA's warps has a stretch of the tiles.
+constexpr int kScanWarps = 32;
+__global__ void __launch_bounds__(32 * kScanWarps) tiles_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, int tiles, int bins) {
+  __shared__ uint32_t sums[kScanWarps][32];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, bin = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (bin >= bins) return;
-  uint32_t* const of = counts + (int64_t)bin * tiles;
-  uint32_t before = 0u;
-  for (int t = 0; t < tiles; t += 32) {
-    const uint32_t own = t + lane < tiles ? of[t + lane] : 0u;
-    uint32_t sum = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
-    }
-    if (t + lane < tiles) of[t + lane] = before + sum - own;
-    before += __shfl_sync(0xffffffffu, sum, 31);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bin = blockIdx.x * 32 + lane, each = (tiles + kScanWarps - 1) / kScanWarps;
+  const int from = min(tiles, warp * each), to = min(tiles, from + each);
+  uint32_t own = 0u;
+  if (bin < bins) {
+#pragma unroll 4
+    for (int t = from; t < to; ++t) own += counts[(int64_t)t * bins + bin];
   }
-  if (lane == 0) totals[bin] = before;
+  sums[warp][lane] = own;
+  __syncthreads();
+  uint32_t before = 0u, all = 0u;
+#pragma unroll
+  for (int w = 0; w < kScanWarps; ++w) {
+    const uint32_t v = sums[w][lane];
+    if (w < warp) before += v;
+    all += v;
+  }
+  if (bin >= bins) return;
+#pragma unroll 4
+  for (int t = from; t < to; ++t) {
+    uint32_t* const at = counts + (int64_t)t * bins + bin;
+    const uint32_t v = *at;
+    *at = before;
+    before += v;
+  }
+  if (warp == 0) totals[bin] = all;
 }
 
 // `mine` of every thread becomes the sum of those of the threads in front.
@@ -155,33 +190,17 @@ __device__ __forceinline__ uint32_t block_before(uint32_t mine, uint32_t* of_war
   return before;
 }
 
+// Puts a tile's places where the digit wants them; counts_next (null: none): counts of the next digit, of the tiles in which they end up.
 template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ ids, Pairs in, int64_t m, uint32_t rows, Digit d, const uint32_t* __restrict__ counts,
-                                                         const uint32_t* __restrict__ totals, int tiles, Pairs out) {
+                                                         const uint32_t* __restrict__ totals, Pairs out, Digit next, uint32_t* __restrict__ counts_next) {
   constexpr int kBins = 1 << kMaxBits, kEach = kBins / kThreads;
-  __shared__ uint16_t of_warp[kWarps][kBins];  // a tile has 2048 places
-  __shared__ uint32_t base[kBins], sums[kWarps];
+  __shared__ uint16_t of_warp[kWarps][kBins];  // a tile has 1024 places
+  __shared__ __align__(16) uint32_t base[kBins];
+  __shared__ uint32_t sums[kWarps];
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << d.bits;
-  for (int i = threadIdx.x; i < kWarps * kBins / 2; i += kThreads) reinterpret_cast<uint32_t*>(of_warp)[i] = 0u;
-  {  // where each digit's places of this tile start
-    uint32_t own[kEach], sum = 0u;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int b = threadIdx.x * kEach + e;
-      own[e] = b < bins ? __ldg(totals + b) : 0u;
-      sum += own[e];
-    }
-    uint32_t before = block_before(sum, sums);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int b = threadIdx.x * kEach + e;
-      if (b < bins) base[b] = before + __ldg(counts + (int64_t)b * tiles + blockIdx.x);
-      before += own[e];
-    }
-  }
-  __syncthreads();
   uint32_t key[kItems], place[kItems], rank[kItems];
   const int64_t first = (int64_t)blockIdx.x * kTile + warp * (32 * kItems) + lane;
 #pragma unroll
@@ -190,28 +209,47 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ i
     key[q] = i < m ? (FIRST ? key_of(ids, i, rows) : in.key[i]) : 0u;
     place[q] = i < m ? (FIRST ? (uint32_t)i : in.place[i]) : 0u;
   }
+  // where each digit's places of this tile start: eight digits (or as many as there are for everyone) a thread
+  const int each = bins >= kBins ? kEach : (bins + kThreads - 1) / kThreads;
+  uint32_t all[kEach], here[kEach], sum = 0u;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int b = threadIdx.x * each + e;
+    const bool mine = e < each && b < bins;
+    all[e] = mine ? __ldg(totals + b) : 0u;
+    here[e] = mine ? __ldg(counts + ((int64_t)blockIdx.x << d.bits) + b) : 0u;
+    sum += all[e];
+  }
+  for (int b = lane; b < bins / 2; b += 32) reinterpret_cast<uint32_t*>(of_warp[warp])[b] = 0u;  // (two digits at least)
+  uint32_t before = block_before(sum, sums);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int b = threadIdx.x * each + e;
+    if (e < each && b < bins) base[b] = before + here[e];
+    before += all[e];
+  }
 #pragma unroll
   for (int q = 0; q < kItems; ++q) {
-    const bool here = first + 32 * q < m;
-    const uint32_t digit = digit_of(key[q], d), all = __ballot_sync(0xffffffffu, here);
-    uint32_t equal = 0u, before = 0u;
-    if (here) {
-      equal = __match_any_sync(all, digit);
-      before = of_warp[warp][digit];
+    const bool there = first + 32 * q < m;
+    const uint32_t digit = digit_of(key[q], d), those = __ballot_sync(0xffffffffu, there);
+    uint32_t equal = 0u, so_far = 0u;
+    if (there) {
+      equal = __match_any_sync(those, digit);
+      so_far = of_warp[warp][digit];
     }
     __syncwarp();
-    if (here && (equal & ((1u << lane) - 1u)) == 0u) of_warp[warp][digit] = (uint16_t)(before + __popc(equal));
+    if (there && (equal & ((1u << lane) - 1u)) == 0u) of_warp[warp][digit] = (uint16_t)(so_far + __popc(equal));
     __syncwarp();
-    rank[q] = before + __popc(equal & ((1u << lane) - 1u));
+    rank[q] = so_far + __popc(equal & ((1u << lane) - 1u));
   }
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kThreads) {
-    uint32_t before = 0u;
+    uint32_t so_far = 0u;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const uint32_t own = of_warp[w][b];
-      of_warp[w][b] = (uint16_t)before;
-      before += own;
+      of_warp[w][b] = (uint16_t)so_far;
+      so_far += own;
     }
   }
   __syncthreads();
@@ -221,6 +259,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ i
       const uint32_t digit = digit_of(key[q], d), to = base[digit] + of_warp[warp][digit] + rank[q];
       out.key[to] = key[q];
       out.place[to] = place[q];
+      if (counts_next != nullptr) atomicAdd(counts_next + ((int64_t)(to / kTile) << next.bits) + digit_of(key[q], next), 1u);
     }
 }
 
@@ -244,7 +283,7 @@ __device__ __forceinline__ bool begins(const uint32_t* key, int64_t i, int64_t m
   return i < m && key[i] < rows && (i == 0 || key[i - 1] != key[i]);
 }
 
-// Numbers the segments: a CTA to a tile of 2048 places.
+// Numbers the segments: a CTA to a tile of 1024 places.
 __global__ void __launch_bounds__(kThreads) number_kernel(const uint32_t* __restrict__ key, int64_t m, uint32_t rows, int stretch, uint32_t* __restrict__ in_tile,
                                                           uint32_t* __restrict__ of_tile, int64_t* __restrict__ looked_up) {
   __shared__ uint32_t sums[kWarps];
@@ -258,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) number_kernel(const uint32_t* __rest
     if (first + q < m) looked_up[first + q] = -1;  // (those that there are are written by the next launch)
   }
   const uint32_t before = block_before(own, sums);
-  // a thread's eight places are one stretch, or a part of one
+  // a thread's four places are a part of one stretch
   if (first < m && first % stretch == 0) in_tile[first / stretch] = before;
   if (threadIdx.x == kThreads - 1) of_tile[blockIdx.x] = before + own;
 }
@@ -385,12 +424,15 @@ __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, cons
   };
   bool is_long = false;
   if (row >= 0) {
-    const uint32_t key = key_of_tail(c);
-    is_long = goes_on(c + kShort, key);
+    // (the stretches of a segment lie side by side)
+    const int count = __popc(__ballot_sync(0xffffffffu, goes_on(c + 1 + lane, key_of_tail(c))));
+    is_long = count >= kShort;
     if (!is_long) {
       f32x2 acc[2] = {};
       add(acc, open.tail, c);
-      for (int64_t q = c + 1; goes_on(q, key); ++q) add(acc, open.head, q);
+#pragma unroll
+      for (int q = 0; q < kShort; ++q)
+        if (q < count) add(acc, open.head, c + 1 + q);
       write(row, acc);
     }
   }
@@ -445,7 +487,7 @@ struct Plan {
   int64_t m, d;
   int stretch, tiles, bits, passes;
   int64_t stretches, width;
-  int64_t key[2], place[2], counts, totals, in_tile, of_tile, head, tail, row, bytes;
+  int64_t key[2], place[2], counts[2], count_bytes, totals, in_tile, of_tile, head, tail, row, bytes;
 };
 static Plan plan(int64_t m, int64_t rows, int64_t d) {
   Plan p{};
@@ -471,7 +513,8 @@ static Plan plan(int64_t m, int64_t rows, int64_t d) {
     p.place[b] = take(4 * m);
   }
   if (p.passes > 0) {
-    p.counts = take(((int64_t)4 << p.bits) * p.tiles);
+    p.count_bytes = ((int64_t)4 << p.bits) * p.tiles;
+    for (int b = 0; b < (p.passes > 1 ? 2 : 1); ++b) p.counts[b] = take(p.count_bytes);
     p.totals = take((int64_t)4 << p.bits);
   }
   p.in_tile = take(4 * p.stretches);
@@ -483,25 +526,42 @@ static Plan plan(int64_t m, int64_t rows, int64_t d) {
   return p;
 }
 
-// Sorts the places; the pairs' final place.
+static Clear clear_of(void* at, int64_t bytes) {
+  Clear c{(uint8_t*)at, 0, 0, 0};
+  c.front = (16 - (int64_t)(reinterpret_cast<uintptr_t>(at) & 15)) & 15;
+  if (c.front > bytes) c.front = bytes;
+  c.whole = (bytes - c.front) / 16;
+  c.behind = (bytes - c.front) % 16;
+  return c;
+}
+
+// Sorts the places (and clears `bytes` bytes from `zero` on beside it); the pairs' final place.
 template <typename I>
-static Pairs sort(const Plan& p, const I* ids, uint32_t rows, char* ws, cudaStream_t st) {
+static Pairs sort(const Plan& p, const I* ids, uint32_t rows, char* ws, void* zero, int64_t bytes, cudaStream_t st) {
   Pairs pairs[2];
   for (int b = 0; b < 2; ++b) pairs[b] = Pairs{(uint32_t*)(ws + p.key[b]), (uint32_t*)(ws + p.place[b])};
+  Clears clears{{clear_of(zero, bytes), clear_of(nullptr, 0)}};
+  if (p.passes > 1) clears.of[1] = clear_of(ws + p.counts[1], p.count_bytes);
+  const int64_t words = clears.of[0].whole + clears.of[1].whole;
+  const int64_t wanted = words == 0 && bytes == 0 ? 0 : ceil_div(words + 1, kThreads * kClearEach);
+  const unsigned more = (unsigned)(wanted < 8 * kSmCount ? wanted : 8 * kSmCount);
   if (p.passes == 0) {
-    launch_dependent(rank_kernel<I>, dim3((unsigned)ceil_div(p.m, 4 * kWarps)), kThreads, 0, st, ids, (int)p.m, rows, pairs[0]);
+    const int ctas = (int)ceil_div(p.m, 4 * kWarps);
+    launch_dependent(rank_kernel<I>, dim3(ctas + more), kThreads, 0, st, ids, (int)p.m, rows, pairs[0], ctas, clears);
     return pairs[0];
   }
-  uint32_t *const counts = (uint32_t*)(ws + p.counts), *const totals = (uint32_t*)(ws + p.totals);
+  uint32_t* const totals = (uint32_t*)(ws + p.totals);
   int to = p.passes & 1 ? 0 : 1;  // so that the last pass ends in pairs[0]
   for (int q = 0; q < p.passes; ++q, to ^= 1) {
-    const Digit d{q * p.bits, p.bits};
+    const Digit d{q * p.bits, p.bits}, next{(q + 1) * p.bits, p.bits};
     const Pairs in = pairs[to ^ 1], out = pairs[to];
-    if (q == 0) launch_dependent(count_kernel<I, true>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, (const uint32_t*)nullptr, p.m, rows, d, counts, p.tiles);
-    else launch_dependent(count_kernel<I, false>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, (const uint32_t*)in.key, p.m, rows, d, counts, p.tiles);
-    launch_dependent(tiles_kernel, dim3((unsigned)ceil_div((int64_t)1 << p.bits, kWarps)), kThreads, 0, st, counts, totals, p.tiles, 1 << p.bits);
-    if (q == 0) launch_dependent(place_kernel<I, true>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, in, p.m, rows, d, (const uint32_t*)counts, (const uint32_t*)totals, p.tiles, out);
-    else launch_dependent(place_kernel<I, false>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, in, p.m, rows, d, (const uint32_t*)counts, (const uint32_t*)totals, p.tiles, out);
+    uint32_t *const counts = (uint32_t*)(ws + p.counts[q & 1]), *const counts_next = q + 1 < p.passes ? (uint32_t*)(ws + p.counts[(q + 1) & 1]) : nullptr;
+    if (q == 0) launch_dependent(count_kernel<I>, dim3((unsigned)p.tiles + more), kThreads, 0, st, ids, p.m, rows, d, counts, p.tiles, clears);
+    launch_dependent(tiles_kernel, dim3((unsigned)ceil_div((int64_t)1 << p.bits, 32)), 32 * kScanWarps, 0, st, counts, totals, p.tiles, 1 << p.bits);
+    if (q == 0) launch_dependent(place_kernel<I, true>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, in, p.m, rows, d, (const uint32_t*)counts, (const uint32_t*)totals, out, next, counts_next);
+    else launch_dependent(place_kernel<I, false>, dim3((unsigned)p.tiles), kThreads, 0, st, ids, in, p.m, rows, d, (const uint32_t*)counts, (const uint32_t*)totals, out, next, counts_next);
+    // (a third digit's counts go where the first one's were)
+    if (q == 0 && p.passes > 2) (void)cudaMemsetAsync(counts, 0, (size_t)p.count_bytes, st);
   }
   return pairs[0];
 }
@@ -563,8 +623,9 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
     const int64_t need = f2c_embedding_backward_workspace(m, rows, d);
     F2C_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 256), F2C_ERR_INVALID, "%s: the workspace must have %lld bytes, 256-byte aligned", op, (long long)need);
   }
-  if (dense && rows > 0 && d > 0) {
-    const cudaError_t e = cudaMemsetAsync(grad, 0, (size_t)(rows * d * dtype_size(dtype)), st);
+  const int64_t bytes = dense ? rows * d * dtype_size(dtype) : 0;
+  if (bytes > 0 && m == 0) {
+    const cudaError_t e = cudaMemsetAsync(grad, 0, (size_t)bytes, st);
     if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
   }
   if (!dense && (m == 0 || d == 0)) {
@@ -575,7 +636,8 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
   if (m == 0 || d == 0 || (dense && rows == 0)) return F2C_OK;
   char* const ws = (char*)workspace;
   const emb::Plan p = emb::plan(m, rows, d);
-  const emb::Pairs sorted = index_dtype == F2C_I64 ? emb::sort(p, (const int64_t*)ids, (uint32_t)rows, ws, st) : emb::sort(p, (const int32_t*)ids, (uint32_t)rows, ws, st);
+  const emb::Pairs sorted = index_dtype == F2C_I64 ? emb::sort(p, (const int64_t*)ids, (uint32_t)rows, ws, grad, bytes, st)
+                                                       : emb::sort(p, (const int32_t*)ids, (uint32_t)rows, ws, grad, bytes, st);
   uint32_t *const in_tile = (uint32_t*)(ws + p.in_tile), *const of_tile = (uint32_t*)(ws + p.of_tile);
   if (!dense)
     launch_dependent(emb::number_kernel, dim3((unsigned)p.tiles), emb::kThreads, 0, st, (const uint32_t*)sorted.key, m, (uint32_t)rows, p.stretch, in_tile, of_tile, looked_up);
