@@ -121,7 +121,7 @@ SIGNATURES = {
     "f2c_muon_step": [C.POINTER(MuonMatrix), ci, ci, f32, f32, ci, f32, p, ci, f32, p, i64, p],
     "f2c_checkpoint_int8": [p, i64, ci, i64, i64, p, i64, p, p],
     "f2c_checkpoint_values": [p, i64, p, i64, i64, p, i64, ci, p],
-    "f2c_checkpoint_weight_grad_workspace": [i64, i64, i64],
+    "f2c_checkpoint_weight_grad_workspace": [p, i64, ci, i64, i64, i64],
     "f2c_checkpoint_weight_grad": [p, i64, ci, p, i64, p, i64, i64, i64, p, p, ci, p, i64, p],
     "f2c_layer_norm": [p, i64, ci, i64, i64, p, p, f32, ci, p, p, p, p, p, i64, p, p],
     "f2c_layer_norm_backward_workspace": [i64, i64],

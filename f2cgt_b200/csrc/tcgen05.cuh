@@ -190,7 +190,7 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void peer_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void peer_store(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 
-// Tensor map of a row-major matrix [rows, cols] of `bytes`-byte elements (16-byte aligned start and row stride), boxes of box_rows x
+// Tensor map of a row-major matrix [rows, cols] of `bytes`-byte elements (1, 2, or 4: single precision; 16-byte aligned start and row stride), boxes of box_rows x
 // 128 bytes with the 128-byte swizzle, zeros outside the matrix.  False when the driver refuses it.
 bool make_map(CUtensorMap* map, const void* base, int bytes, int64_t rows, int64_t cols, int64_t row_bytes, int box_rows);
 // The same for a stack of `batch` half-precision matrices, `rows` rows apart.

@@ -1,21 +1,22 @@
 // Gradient of a linear layer's weight and bias, its input kept in 8 bits (f2c_checkpoint_weight_grad):
-//   dW[i, j] = sum over rows r of dy[r, i] (low[r, g] + step[r, g] q[r, j]),   db[i] = sum over rows of dy[r, i],   g the group of column j,
-// on the 5th-generation tensor cores.  The input is never written out: with the factors taken to the other side,
-//   dW = (step dy)^T q + (low dy)^T 1,
-// the codes q = 0 .. 255 are bfloat16 numbers as they are, and step dy, rounded to single precision, is a sum of bfloat16 numbers: three of them hold
-// all 24 bits (float32 dy), two 16 (float16 and bfloat16 dy, whose result is rounded to 11 or 8).  The second term is one number for every i and
-// group, summed in registers on the way, as is db.
+//   dW[i, j] = sum over rows r of dy[r, i] x[r, j],  x[r, j] = low[r, g] + step[r, g] q[r, j],  g the group of column j;  db[i] = sum over rows of dy[r, i],
+// on the 5th-generation tensor cores.  The input is never written out: it is decoded between shared memory and the tensor cores.  32 rows of dy and of codes
+// at a time come with TMA through a ring of stages; four groups of four warps take the stages in turn, a thread has a column; one operand goes to TMEM by
+// way of their registers, the other one lies in shared memory along M or N, which the MMA takes as it is.
 //
-// A tile of dW has 128 columns of dy (the lanes of TMEM) and a group's 128 columns of q, so that all of a row's tile has one step.  Neither operand is
-// turned: their rows run along M and N, which the MMA takes as it is.  Sixteen warps load 32 rows of both, two stages ahead in registers, and
-// write them as bfloat16 to a ring in shared memory; the first of them also issues the MMAs, of a stage when it has written its part of the next (a
-// warp of its own would leave the others 96 registers instead of 128).
+//  * bfloat16 dy (rows_kernel).  dy is an operand as it is.  x is two bfloat16 numbers, 16 bits, of a product that is rounded to 8: two MMAs of
+//    128 columns of x (the lanes of TMEM) by 256 of dy for every 16 rows.
+//  * float32 and float16 dy (scaled_kernel).  With the factors taken to the other side, dW = (step dy)^T q + (low dy)^T 1: the codes 0 .. 255 are
+//    bfloat16 numbers as they are, and step dy, rounded to single precision, is a sum of three of them (all 24 bits; float32) or two (16 bits; float16, whose
+//    range bfloat16 has and float16 values of x might leave).  The second term is one number for every column of dy and group, summed in registers.  128
+//    columns of dy (the lanes) by a group.
 //
-// Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows.  So for float32 the two small parts of step dy have an
-// accumulator of their own, and sums are taken out every 256 rows and added up in registers, while the MMAs go on in the other half of TMEM.
+// Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows.  So for float32 they are taken out every 128 rows and added up in
+// registers, while the MMAs go on in the other half of the accumulators; elsewhere every 16,384 rows (float16), and once a part of at most 65,536 rows.
 //
 // Many rows and few tiles: the rows are dealt out over all SMs; each leaves its part of the sums, and a second launch adds them up in their order.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "checkpoint.cuh"
@@ -25,108 +26,127 @@ namespace f2c {
 namespace wg {
 
 using namespace t5;
+using ckpt::both;
+using ckpt::f32x2;
 using ckpt::fma2;
 using ckpt::kGroup;
 using ckpt::mul2;
 using ckpt::pair_of;
+using ckpt::plus2;
 
-constexpr int kWarps = 16, kThreads = 32 * kWarps;
-constexpr int kTile = 128, kRows = 32, kAhead = 2, kStages = 6;
-constexpr uint32_t kChunk = kRows * 128, kPlane = 2 * kChunk;  // 64 columns' rows, and a tile's
+constexpr int kGroups = 4, kWarps = 4 * kGroups, kThreads = 32 * (kWarps + 2);  // then a warp for the loads and one for the MMAs
+constexpr int kRows = 32, kStages = 8;
+constexpr uint32_t kBox = kRows * 128;  // a stage's rows of 128 bytes
 constexpr uint32_t kFormatBf16 = 1;
+constexpr int64_t kMaxSplitRows = 65536;
 
 struct Params {
-  const void* dy;
-  int64_t ldy, m;
+  const float* scales;
+  int64_t groups, m;
   int n, k;
-  ckpt::Codes x;
   int n_tiles, splits;
   int64_t split_rows;     // a multiple of kRows
   void *dw, *db;          // (splits == 1) of dy's type
-  float *part, *part_db;  // (splits > 1) [split][tile][32][128][4], [split][n_tiles * 128]
+  float *part, *part_db;  // (splits > 1) [split][tile][columns / 4][128][4], [split][n_tiles * columns of dy]
   uint32_t tries;
   int* error;
 };
 
 struct Bars {
-  uint64_t full[kStages], empty[kStages], drain, acc_full[2], acc_empty[2];
+  uint64_t full[kStages], empty[kStages], ready[kGroups], taken[kGroups], drain, acc_full[2], acc_empty[2];
   uint32_t tmem;
   int failed;
 };
 
-template <typename T> struct Kind { static constexpr int kPieces = 2, kTaken = 128; };  // stages between two takings out
-template <> struct Kind<float> { static constexpr int kPieces = 3, kTaken = 8; };
-static_assert(Kind<float>::kTaken >= kStages, "a ring's stages do not reach over two takings out");
+// The MMA whose first operand is in TMEM, two 16-bit elements of K to a column.
+__device__ __forceinline__ void mma_f16_tmem(bool go, uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, g;\n\tsetp.ne.b32 g, %6, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@g tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(0u),
+      "r"((uint32_t)go)
+      : "memory");
+}
+// 16 or 8 columns of the 32 lanes that the warp owns
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {  // round to even
+__device__ __forceinline__ uint32_t pack_bf16(f32x2 v) {  // round to even
   uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi32(v)), "f"(lo32(v)));
   return r;
 }
-__device__ __forceinline__ void store16(uint32_t at, const uint32_t (&w)[4]) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+// v less the two numbers of w: exact where they are v rounded
+__device__ __forceinline__ f32x2 less_bf16(f32x2 v, uint32_t w) { return fma2(pair_of(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), both(-1.0f), v); }
+__device__ __forceinline__ uint32_t lds_u8(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint4 lds_u128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ void sts_u128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// What a thread has of a stage: eight columns of a row of dy and of its codes, and their step and lowest value.  ACCESS: bytes of a load of dy.
-template <typename T, int ACCESS>
-struct Piece {
-  static constexpr int kWords = 2 * (int)sizeof(T), kEach = ACCESS / (int)sizeof(T);
-  uint32_t dy[kWords];
-  uint2 codes, scale;
-
-  __device__ __forceinline__ void load(const Params& p, int64_t row, bool here, int col, int code_col, int group) {
-    const T* const from = (const T*)p.dy + row * p.ldy + col;
-#pragma unroll
-    for (int q = 0; q < 8 / kEach; ++q) {
-      const bool go = here && col + q * kEach < p.n;
-      const T* const at = from + q * kEach;
-      if constexpr (ACCESS == 16) {
-        const uint4 v = ldg_nc_u128_if(at, go);
-        dy[4 * q] = v.x; dy[4 * q + 1] = v.y; dy[4 * q + 2] = v.z; dy[4 * q + 3] = v.w;
-      } else if constexpr (ACCESS == 8) {
-        const uint2 v = ldg_nc_u64_if(at, go);
-        dy[2 * q] = v.x; dy[2 * q + 1] = v.y;
-      } else if constexpr (ACCESS == 4) {
-        dy[q] = ldg_nc_u32_if(at, go);
-      } else {
-        const uint32_t v = go ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at)) : 0u;
-        dy[q / 2] = q & 1 ? dy[q / 2] | v << 16 : v;
-      }
-    }
-    codes = ldg_nc_u64_if(p.x.codes + row * p.x.ld + code_col, here && code_col < p.k);
-    scale = ldg_nc_u64_if(p.x.scales + 2 * (row * p.x.groups + group), here);
+// The steps and lowest values of a stage's rows, for a warp: lane r has row r's on the way a round ahead, and all get them from shared memory.
+struct Scales {
+  uint2 next;
+  __device__ __forceinline__ void fetch(const Params& p, int64_t row0, int64_t rows, int stage, int group) {
+    const int64_t r = (int64_t)stage * kRows + (threadIdx.x & 31);
+    next = ldg_nc_u64_if(p.scales + 2 * ((row0 + r) * p.groups + group), r < rows);
   }
-  __device__ __forceinline__ void get(unsigned long long (&d)[4]) const {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (sizeof(T) == 4) d[e] = pair_of(__uint_as_float(dy[2 * e]), __uint_as_float(dy[2 * e + 1]));
-      else if constexpr (std::is_same<T, __half>::value) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&dy[e]));
-        d[e] = pair_of(f.x, f.y);
-      } else {
-        d[e] = pair_of(__uint_as_float(dy[e] << 16), __uint_as_float(dy[e] & 0xffff0000u));
-      }
-    }
+  // [steps of 32 rows][lowest values]
+  __device__ __forceinline__ void tell(float* mine) const {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();  // (the ones before have been read)
+    mine[lane] = __uint_as_float(next.x);
+    mine[32 + lane] = __uint_as_float(next.y);
+    __syncwarp();
   }
 };
 
-template <typename T, int ACCESS>
-__global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_constant__ Params p) {
-  constexpr int kPieces = Kind<T>::kPieces, kTaken = Kind<T>::kTaken;
-  constexpr uint32_t kStage = (kPieces + 1) * kPlane;
-  constexpr uint32_t kAcc = kPieces == 3 ? 256 : 128;  // columns of TMEM: the sums, and those of the small parts
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ Bars bars;
-  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
-  const int tile = (int)blockIdx.x / p.splits, split = (int)blockIdx.x % p.splits, n0 = tile % p.n_tiles * kTile, group = tile / p.n_tiles;
-  const int64_t row0 = split * p.split_rows, rows = min(p.split_rows, p.m - row0);
-  const int stages = (int)((rows + kRows - 1) / kRows), takes = (stages + kTaken - 1) / kTaken;
-  uint32_t left = p.tries;
+struct Place {
+  int tile, split, n0, group;
+  int64_t row0, rows;
+  int stages;
+  __device__ __forceinline__ Place(const Params& p, int columns) {
+    tile = (int)blockIdx.x / p.splits;
+    split = (int)blockIdx.x % p.splits;
+    n0 = tile % p.n_tiles * columns;
+    group = tile / p.n_tiles;
+    row0 = split * p.split_rows;
+    rows = min(p.split_rows, p.m - row0);
+    stages = (int)((rows + kRows - 1) / kRows);
+  }
+};
 
-  if (wid == 0) alloc_tmem(&bars.tmem, 2 * kAcc);
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) { init_bar(bars.full + s, kWarps); init_bar(bars.empty + s, 1); }
+// Barriers and TMEM (512 columns: no other CTA that has any is on the SM, which the shared memory sees to)
+__device__ __forceinline__ void begin(Bars& bars, uint32_t empties) {
+  if (threadIdx.x / 32 == kWarps + 1) alloc_tmem(&bars.tmem, 512);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { init_bar(bars.full + s, 1); init_bar(bars.empty + s, empties); }
+    for (int g = 0; g < kGroups; ++g) { init_bar(bars.ready + g, 4); init_bar(bars.taken + g, 1); }
     init_bar(&bars.drain, 1);
     for (int b = 0; b < 2; ++b) { init_bar(bars.acc_full + b, 1); init_bar(bars.acc_empty + b, kWarps); }
     fence_bars();
@@ -135,201 +155,404 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_c
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = bars.tmem;
-  dependency_wait();
-  release_dependents();
+}
 
-  float sum[32];
-  unsigned long long of_low[4], of_bias[4];  // the tile's sums that this thread has, and over its rows and eight columns
-#pragma unroll
-  for (int j = 0; j < 32; ++j) sum[j] = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) of_low[e] = of_bias[e] = 0ull;
-  const int vec = tid & 15, at_row = tid >> 4;  // eight columns, and a row of a stage
-  const int col = n0 + 8 * vec, code_col = group * kGroup + 8 * vec;
-  // 16 bytes `vec` of row at_row, in the 128-byte swizzle
-  const uint32_t place = smem_u32(smem) + (uint32_t)(vec >> 3) * kChunk + (uint32_t)at_row * 128 + (uint32_t)(((vec & 7) ^ (at_row & 7)) << 4);
-  const int quarter = wid & 3, cols = wid >> 2;
-  const uint32_t acc_at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)cols * 32;
-
-  // ================= sums of kTaken stages out of TMEM
-  const auto take = [&](int t) {
-    wait_bar(bars.acc_full + (t & 1), (t >> 1) & 1, left);
-    fence_after();
-#pragma unroll
-    for (int part = 0; part < (kPieces == 3 ? 2 : 1); ++part) {
-      uint32_t r[32];
-      tmem_ld32(acc_at + (uint32_t)(t & 1) * kAcc + part * 128, r);
-      tmem_wait(r);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(r[j]);
-    }
-    fence_before();
-    __syncwarp();
-    if (lane == 0) arrive(bars.acc_empty + (t & 1));
-  };
-
-  // ================= MMAs of stage i, whose place in the ring is s
-  const bool mine = wid == 0 && elected() != 0u;
-  const uint32_t idesc = instruction(kSumF32, kFormatBf16, kTile, kTile) | kTurnedA | kTurnedB;
-  const uint32_t a_low = desc_low(smem_u32(smem), kChunk), b_low = a_low + (kPieces * kPlane >> 4);
-  const auto multiply = [&](int i, int s, uint32_t round) {
-    const int t = i / kTaken, in_take = i % kTaken;
-    const uint32_t acc = tmem + (uint32_t)(t & 1) * kAcc;
-    if (in_take == 0 && t >= 2) wait_bar(bars.acc_empty + (t & 1), ((t >> 1) - 1) & 1, left);
-    wait_bar(bars.full + s, round & 1, left);
-    fence_after();
-    const bool go = mine && left != 0u;
-    const uint32_t at = (uint32_t)s * (kStage >> 4), a = a_low + at, b = b_low + at;
-#pragma unroll
-    for (uint32_t q = 0; q < kRows / 16; ++q) {
-      mma_f16(go, acc, desc(a + q * kStepTurned), desc(b + q * kStepTurned), idesc, in_take != 0 || q != 0);
-#pragma unroll
-      for (uint32_t piece = 1; piece < kPieces; ++piece)
-        mma_f16(go, kPieces == 3 ? acc + 128 : acc, desc(a + piece * (kPlane >> 4) + q * kStepTurned), desc(b + q * kStepTurned), idesc,
-                kPieces == 2 || in_take != 0 || q != 0 || piece != 1);
-    }
-    commit(go, bars.empty + s);
-    if (in_take == kTaken - 1 || i == stages - 1) commit(go, bars.acc_full + (t & 1));
-    __syncwarp();
-  };
-
-  // ================= dy and codes, as the MMAs take them
-  const auto fetch = [&](Piece<T, ACCESS>& v, int i) {
-    const int64_t r = (int64_t)i * kRows + at_row;
-    v.load(p, row0 + r, r < rows, col, code_col, group);
-  };
-  Piece<T, ACCESS> ahead[kAhead];
-#pragma unroll
-  for (int a = 0; a < kAhead; ++a) fetch(ahead[a], a);
-  int s = 0, taken = 0;
-  uint32_t round = 0;
-  for (int i0 = 0; i0 < stages; i0 += kAhead) {
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int i = i0 + a;
-      if (i >= stages) break;
-      const Piece<T, ACCESS> v = ahead[a];
-      fetch(ahead[a], i + kAhead);
-      unsigned long long d[4];
-      v.get(d);
-      if (group == 0) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) add2(of_bias[e], d[e]);
-      }
-      const unsigned long long step = pair_of(__uint_as_float(v.scale.x), __uint_as_float(v.scale.x)), low = pair_of(__uint_as_float(v.scale.y), __uint_as_float(v.scale.y));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        of_low[e] = fma2(low, d[e], of_low[e]);
-        d[e] = mul2(step, d[e]);
-      }
-      if (round > 0) wait_bar(bars.empty + s, (round - 1) & 1, left);
-      const uint32_t at = place + (uint32_t)s * kStage;
-#pragma unroll
-      for (int q = 0; q < kPieces; ++q) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = pack_bf16(lo32(d[e]), hi32(d[e]));
-          // what is left: exact
-          if (q + 1 < kPieces) d[e] = fma2(pair_of(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)), pair_of(-1.0f, -1.0f), d[e]);
-        }
-        store16(at + (uint32_t)q * kPlane, w);
-      }
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // 2^23 + q, less 2^23
-        const uint32_t from = e < 2 ? v.codes.x : v.codes.y;
-        unsigned long long q = pair_of(__uint_as_float(__byte_perm(from, 0x4B000000u, 0x7440 + (e & 1) * 2)), __uint_as_float(__byte_perm(from, 0x4B000000u, 0x7441 + (e & 1) * 2)));
-        add2(q, pair_of(-8388608.0f, -8388608.0f));
-        w[e] = pack_bf16(lo32(q), hi32(q));
-      }
-      store16(at + kPieces * kPlane, w);
-      fence_async();
-      __syncwarp();
-      if (lane == 0) arrive(bars.full + s);
-      if (wid == 0 && i > 0) multiply(i - 1, s > 0 ? s - 1 : kStages - 1, s > 0 ? round : round - 1);
-      if (++s == kStages) { s = 0; ++round; }
-      // the sums are ready some time after the last of their stages has been handed over
-      if ((taken + 1) * kTaken + kStages <= i + 1) take(taken++);
-    }
+// The stages' loads, by a warp: `boxes` of dy, EACH columns apart, then the codes.
+template <int EACH>
+__device__ __forceinline__ void load_stages(const CUtensorMap* dy, const CUtensorMap* codes, Bars& bars, uint32_t ring, uint32_t stage_bytes, uint32_t codes_at, int boxes, const Place& at,
+                                            uint32_t& left, int& s, uint32_t& round) {
+  const bool mine = elected() != 0u;
+  if (mine) {
+    prefetch_map(dy);
+    prefetch_map(codes);
   }
-  if (wid == 0 && stages > 0) multiply(stages - 1, s > 0 ? s - 1 : kStages - 1, s > 0 ? round : round - 1);
-  while (taken < takes) take(taken++);
+  __syncwarp();
+  for (int i = 0; i < at.stages; ++i) {
+    if (round > 0) wait_bar(bars.empty + s, (round - 1) & 1, left);
+    const bool go = mine && left != 0u;
+    const uint32_t stage = ring + (uint32_t)s * stage_bytes, bar = smem_u32(bars.full + s);
+    const int row = (int)(at.row0 + (int64_t)i * kRows);
+    expect_if(go, bars.full + s, (uint32_t)(boxes + 1) * kBox);
+    for (int b = 0; b < boxes; ++b) tma_load(go, dy, stage + (uint32_t)b * kBox, bar, at.n0 + b * EACH, row);
+    tma_load(go, codes, stage + codes_at, bar, at.group * kGroup, row);
+    if (++s == kStages) { s = 0; ++round; }
+  }
+}
+
+// All roles are done; whether a wait of one of them has run out.
+__device__ __forceinline__ bool settle(Bars& bars, uint32_t left) {
   if (left == 0u) bars.failed = 1;
   fence_before();
   __syncthreads();
-  const bool lost = bars.failed != 0;
+  fence_after();
+  return bars.failed != 0;
+}
+// The way out, after the last read of TMEM: when a wait has run out, what was issued is waited for (bounded) before TMEM is freed.
+__device__ __forceinline__ void leave(const Params& p, Bars& bars, bool lost, int s, uint32_t round) {
+  const int wid = threadIdx.x >> 5;
   if (lost && p.tries != 0u) {
-    // MMAs in flight read shared memory and write TMEM: wait (bounded) for what was issued
-    left = p.tries;
-    if (wid == 0) {
+    uint32_t left = p.tries;
+    if (wid == kWarps) {
+      for (int q = 0; q < kStages; ++q) {
+        const uint32_t uses = round + (q < s ? 1u : 0u);
+        if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
+      }
+    } else if (wid == kWarps + 1) {
+      const bool mine = elected() != 0u;
       commit(mine, &bars.drain);
       wait_bar(&bars.drain, 0, left);
     }
-    __syncthreads();
   }
-  if (wid == 0) {
+  fence_before();
+  __syncthreads();
+  if (wid == kWarps + 1) {
     fence_after();
-    free_tmem(tmem, 2 * kAcc);
+    free_tmem(bars.tmem, 512);
   }
-  if (tid == 0 && lost) report_wait(p.error, 8);
+  if (threadIdx.x == 0 && lost) report_wait(p.error, 8);
+}
 
-  // of_low and of_bias over all rows: the ring's memory is free
-  float(*const columns)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(smem);  // [warp]
+// ---------------------------------------------------------------- bfloat16: x decoded, in TMEM; dy as it is
+constexpr int kWide = 256;                                           // columns of dy in a tile
+constexpr uint32_t kWideStage = (kWide / 64 + 1) * kBox;             // four boxes of 64 columns, and the codes
+constexpr int kWideSmem = kStages * kWideStage + 1024;
+
+__global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant__ CUtensorMap dy, const __grid_constant__ CUtensorMap codes, const __grid_constant__ Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ Bars bars;
+  __shared__ __align__(16) float scales_s[kWarps][64];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const Place at(p, kWide);
+  const int cols = min(kWide, p.n - at.n0), boxes = (cols + 63) / 64;
+  uint32_t left = p.tries;
+  int s = 0;
+  uint32_t round = 0;
+  begin(bars, 5);  // a stage is free when its MMAs are done and its group's warps have read it
+  const uint32_t tmem = bars.tmem, ring = smem_u32(smem), a_tmem = tmem + kWide;
+  const int quarter = wid & 3, set = wid >> 2;
+  f32x2 of_bias = 0ull;
+  dependency_wait();
+  release_dependents();
+
+  if (wid == kWarps) {
+    load_stages<64>(&dy, &codes, bars, ring, kWideStage, (kWide / 64) * kBox, boxes, at, left, s, round);
+  } else if (wid == kWarps + 1) {
+    // ================= MMAs
+    const bool mine = elected() != 0u;
+    const uint32_t idesc = instruction(kSumF32, kFormatBf16, 128, (uint32_t)(cols + 15) / 16 * 16) | kTurnedB, b_low = desc_low(ring, kBox);
+    for (int i = 0; i < at.stages; ++i) {
+      const int slot = i % kGroups;
+      wait_bar(bars.full + s, round & 1, left);
+      wait_bar(bars.ready + slot, (i / kGroups) & 1, left);
+      fence_after();
+      const bool go = mine && left != 0u;
+      const uint32_t b = b_low + (uint32_t)s * (kWideStage >> 4), a = a_tmem + (uint32_t)slot * 32;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    add2(of_low[e], __shfl_xor_sync(0xffffffffu, of_low[e], 16));
-    add2(of_bias[e], __shfl_xor_sync(0xffffffffu, of_bias[e], 16));
+      for (uint32_t q = 0; q < kRows / 16; ++q) {
+        mma_f16_tmem(go, tmem, a + 8 * q, desc(b + q * kStepTurned), idesc, i != 0 || q != 0);
+        mma_f16_tmem(go, tmem, a + 16 + 8 * q, desc(b + q * kStepTurned), idesc, true);
+      }
+      commit(go, bars.empty + s);
+      commit(go, bars.taken + slot);
+      if (++s == kStages) { s = 0; ++round; }
+    }
+    commit(mine && left != 0u, bars.acc_full);
+  } else {
+    // ================= x as two bfloat16 numbers: a column a thread, a stage a group
+    const int c = quarter * 32 + lane;
+    uint32_t column[8];  // of row j of eight, in the 128-byte swizzle
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) column[j] = ring + (kWide / 64) * kBox + j * 128 + ((((uint32_t)c >> 4) ^ j) << 4) + (c & 15);
+    const uint32_t to = a_tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)set * 32;
+    Scales scale;
+    scale.fetch(p, at.row0, at.rows, set, at.group);
+    int use = 0;
+    for (int i = set; i < at.stages; i += kGroups, ++use) {
+      s = i % kStages;
+      scale.tell(scales_s[wid]);
+      scale.fetch(p, at.row0, at.rows, i + kGroups, at.group);
+      wait_bar(bars.full + s, (uint32_t)(i / kStages) & 1, left);
+      const uint32_t stage = (uint32_t)s * kWideStage;
+      uint32_t q[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) q[r] = lds_u8(column[r & 7] + stage + (uint32_t)(r >> 3) * 1024);
+      if (at.group == 0) {  // two columns of dy a thread, over the stage's rows
+        const uint32_t box = ring + stage + (uint32_t)quarter * kBox;
+        if (quarter < boxes) {
+#pragma unroll 8
+          for (uint32_t r = 0; r < kRows; ++r) {
+            const uint32_t w = lds_u32(box + r * 128 + ((((uint32_t)lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            of_bias = plus2(of_bias, pair_of(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) arrive(bars.empty + s);
+      uint32_t high[16], low[16];
+#pragma unroll
+      for (int r = 0; r < kRows; r += 4) {
+        const float4 step = *reinterpret_cast<const float4*>(&scales_s[wid][r]), base = *reinterpret_cast<const float4*>(&scales_s[wid][32 + r]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f32x2 v = plus2(pair_of(__uint_as_float(q[r + 2 * h] | 0x4B000000u), __uint_as_float(q[r + 2 * h + 1] | 0x4B000000u)), both(-8388608.0f));
+          v = fma2(h ? pair_of(step.z, step.w) : pair_of(step.x, step.y), v, h ? pair_of(base.z, base.w) : pair_of(base.x, base.y));
+          high[r / 2 + h] = pack_bf16(v);
+          low[r / 2 + h] = pack_bf16(less_bf16(v, high[r / 2 + h]));
+        }
+      }
+      if (use > 0) wait_bar(bars.taken + set, (uint32_t)(use - 1) & 1, left);
+      fence_after();
+      tmem_st16(to, high);
+      tmem_st16(to + 16, low);
+      tmem_st_wait();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(bars.ready + set);
+    }
+    wait_bar(bars.acc_full, 0, left);
   }
-  if (lane < 16) {
+  const bool lost = settle(bars, left);
+  if (wid < kWarps) {  // a group has 64 columns of dy, a thread a column of x
+    const float none = lost ? __int_as_float(0x7fffffff) : 0.0f;
+    const int x_col = at.group * kGroup + quarter * 32 + lane;
+    for (int c0 = set * 64; c0 < min(cols, set * 64 + 64); c0 += 32) {
+      uint32_t r[32];
+      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0, r);
+      tmem_wait(r);
+      if (p.splits > 1) {
+        float4* const out = reinterpret_cast<float4*>(p.part) + ((int64_t)at.split * (gridDim.x / p.splits) + at.tile) * (kWide * 128 / 4) + c0 / 4 * 128 + quarter * 32 + lane;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      *reinterpret_cast<unsigned long long*>(&columns[wid][0][8 * lane + 2 * e]) = of_low[e];
-      *reinterpret_cast<unsigned long long*>(&columns[wid][1][8 * lane + 2 * e]) = of_bias[e];
+        for (int j = 0; j < 8; ++j)
+          out[j * 128] = make_float4(__uint_as_float(r[4 * j]) + none, __uint_as_float(r[4 * j + 1]) + none, __uint_as_float(r[4 * j + 2]) + none, __uint_as_float(r[4 * j + 3]) + none);
+      } else if (x_col < p.k) {
+        __nv_bfloat16* const out = (__nv_bfloat16*)p.dw + (int64_t)(at.n0 + c0) * p.k + x_col;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c0 + j < cols) out[(int64_t)j * p.k] = __float2bfloat16_rn(__uint_as_float(r[j]) + none);
+      }
     }
   }
+  leave(p, bars, lost, s, round);
+  if (at.group != 0) return;
+  float* const columns = reinterpret_cast<float*>(smem);  // [group][256]: the ring is free
+  if (wid < kWarps) *reinterpret_cast<f32x2*>(columns + set * kWide + quarter * 64 + 2 * lane) = of_bias;
   __syncthreads();
-  if (tid < 2 * kTile) {
-    float all = 0.0f;
+  if (tid < cols) {
+    float sum = lost ? __int_as_float(0x7fffffff) : 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) all += columns[w][tid >> 7][tid & 127];
-    columns[0][tid >> 7][tid & 127] = all;  // (read by this thread alone)
+    for (int g = 0; g < kGroups; ++g) sum += columns[g * kWide + tid];
+    if (p.splits > 1) p.part_db[(int64_t)at.split * p.n_tiles * kWide + at.n0 + tid] = sum;
+    else ((__nv_bfloat16*)p.db)[at.n0 + tid] = __float2bfloat16_rn(sum);
+  }
+}
+
+// ---------------------------------------------------------------- float32, float16: dy times the step, in TMEM; the codes as they are
+constexpr int kTile = 128;                     // columns of dy in a tile
+constexpr uint32_t kCodesBytes = 2 * kBox;     // a stage's codes as bfloat16
+
+// kTaken: stages between two takings out
+template <typename T> struct Kind;
+template <> struct Kind<float> {
+  static constexpr int kPieces = 3, kTaken = 4, kEach = 32;
+  static constexpr uint32_t kStage = 5 * kBox;
+};
+template <> struct Kind<__half> {
+  static constexpr int kPieces = 2, kTaken = 512, kEach = 64;
+  static constexpr uint32_t kStage = 3 * kBox;
+};
+template <typename T> constexpr int kTileSmem = kStages * Kind<T>::kStage + kGroups * kCodesBytes + 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_constant__ CUtensorMap dy, const __grid_constant__ CUtensorMap codes, const __grid_constant__ Params p) {
+  constexpr int kPieces = Kind<T>::kPieces, kTaken = Kind<T>::kTaken, kEach = Kind<T>::kEach;
+  constexpr uint32_t kStage = Kind<T>::kStage, kCodesAt = kStage - kBox;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ Bars bars;
+  __shared__ __align__(16) float scales_s[kWarps][64];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const Place at(p, kTile);
+  const int cols = min(kTile, p.n - at.n0), boxes = (cols + kEach - 1) / kEach, takes = (at.stages + kTaken - 1) / kTaken;
+  uint32_t left = p.tries;
+  int s = 0;
+  uint32_t round = 0;
+  begin(bars, 4);  // a stage is free when its group's warps have read it
+  const uint32_t tmem = bars.tmem, ring = smem_u32(smem), q_ring = ring + kStages * kStage, a_tmem = tmem + 2 * kTile;
+  const int quarter = wid & 3, set = wid >> 2;
+  float sum[32];
+  f32x2 of_low = 0ull, of_bias = 0ull;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) sum[j] = 0.0f;
+  dependency_wait();
+  release_dependents();
+
+  if (wid == kWarps) {
+    load_stages<kEach>(&dy, &codes, bars, ring, kStage, kCodesAt, boxes, at, left, s, round);
+  } else if (wid == kWarps + 1) {
+    // ================= MMAs
+    const bool mine = elected() != 0u;
+    const uint32_t idesc = instruction(kSumF32, kFormatBf16, kTile, kTile) | kTurnedB, b_low = desc_low(q_ring, kBox);
+    for (int i = 0; i < at.stages; ++i) {
+      const int slot = i % kGroups, t = i / kTaken, in_take = i % kTaken;
+      const uint32_t acc = tmem + (uint32_t)(t & 1) * kTile;
+      if (in_take == 0 && t >= 2) wait_bar(bars.acc_empty + (t & 1), ((t >> 1) - 1) & 1, left);
+      wait_bar(bars.ready + slot, (i / kGroups) & 1, left);
+      fence_after();
+      const bool go = mine && left != 0u;
+      const uint32_t b = b_low + (uint32_t)slot * (kCodesBytes >> 4), a = a_tmem + (uint32_t)slot * (16 * kPieces);
+#pragma unroll
+      for (uint32_t q = 0; q < kRows / 16; ++q)
+#pragma unroll
+        for (int piece = kPieces - 1; piece >= 0; --piece)  // the small ones first
+          mma_f16_tmem(go, acc, a + 16 * piece + 8 * q, desc(b + q * kStepTurned), idesc, in_take != 0 || q != 0 || piece != kPieces - 1);
+      commit(go, bars.taken + slot);
+      if (in_take == kTaken - 1 || i == at.stages - 1) commit(go, bars.acc_full + (t & 1));
+    }
+  } else {
+    const auto take = [&](int t) {  // sums out of TMEM: a group has 32 columns of the codes, a thread a column of dy
+      wait_bar(bars.acc_full + (t & 1), (t >> 1) & 1, left);
+      fence_after();
+      uint32_t r[32];
+      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((t & 1) * kTile + set * 32), r);
+      tmem_wait(r);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(r[j]);
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(bars.acc_empty + (t & 1));
+    };
+    // ================= dy times the step as bfloat16 numbers, a column a thread, a stage a group
+    const int c = quarter * 32 + lane;
+    uint32_t column[8];  // of row j of eight, in the 128-byte swizzle
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      if constexpr (sizeof(T) == 4) column[j] = ring + (uint32_t)quarter * kBox + j * 128 + ((((uint32_t)lane >> 2) ^ j) << 4) + (lane & 3) * 4;
+      else column[j] = ring + (uint32_t)(quarter >> 1) * kBox + j * 128 + (((((uint32_t)c & 63) >> 3) ^ j) << 4) + (c & 7) * 2;
+    }
+    // and codes: 32 of a row a thread
+    const uint32_t q_row = (uint32_t)(tid & 127) >> 2, q_part = tid & 3;
+    const uint32_t to = a_tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)set * (16 * kPieces);
+    Scales scale;
+    scale.fetch(p, at.row0, at.rows, set, at.group);
+    int use = 0, taken = 0;
+    for (int i = set; i < at.stages; i += kGroups, ++use) {
+      s = i % kStages;
+      scale.tell(scales_s[wid]);
+      scale.fetch(p, at.row0, at.rows, i + kGroups, at.group);
+      wait_bar(bars.full + s, (uint32_t)(i / kStages) & 1, left);
+      if (use > 0) wait_bar(bars.taken + set, (uint32_t)(use - 1) & 1, left);
+      fence_after();
+      const uint32_t stage = (uint32_t)s * kStage;
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {  // 16 codes
+        const uint4 q = lds_u128(ring + stage + kCodesAt + q_row * 128 + (((q_part * 2 + h) ^ (q_row & 7)) << 4));
+        const uint32_t box = q_ring + (uint32_t)set * kCodesBytes + (q_part >> 1) * kBox + q_row * 128, first = (q_part & 1) * 4 + 2 * h;
+        f32x2 a[2], b[2];
+        ckpt::numbers_of(q.x, a);
+        ckpt::numbers_of(q.y, b);
+        sts_u128(box + ((first ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
+        ckpt::numbers_of(q.z, a);
+        ckpt::numbers_of(q.w, b);
+        sts_u128(box + (((first + 1) ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
+      }
+      const bool mine = quarter * 32 < cols;  // (behind them nothing was loaded)
+      // 16 rows at a time: more did not fit into the registers beside the sums
+#pragma unroll 1
+      for (uint32_t half = 0; half < 2; ++half) {
+        f32x2 d[8];
+        const uint32_t from = stage + half * 2048;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const uint32_t even = column[r & 7] + from + (uint32_t)(r >> 3) * 1024, odd = column[(r + 1) & 7] + from + (uint32_t)(r >> 3) * 1024;
+          if (!mine) d[r / 2] = 0ull;
+          else if constexpr (sizeof(T) == 4) d[r / 2] = pair_of(__uint_as_float(lds_u32(even)), __uint_as_float(lds_u32(odd)));
+          else d[r / 2] = pair_of(__half2float(__ushort_as_half((unsigned short)lds_u16(even))), __half2float(__ushort_as_half((unsigned short)lds_u16(odd))));
+        }
+        if (at.group == 0) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) of_bias = plus2(of_bias, d[r]);
+        }
+        const float* const step_of = scales_s[wid] + half * 16;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const float4 step = *reinterpret_cast<const float4*>(step_of + r), base = *reinterpret_cast<const float4*>(step_of + 32 + r);
+          of_low = fma2(pair_of(base.x, base.y), d[r / 2], of_low);
+          of_low = fma2(pair_of(base.z, base.w), d[r / 2 + 1], of_low);
+          d[r / 2] = mul2(pair_of(step.x, step.y), d[r / 2]);
+          d[r / 2 + 1] = mul2(pair_of(step.z, step.w), d[r / 2 + 1]);
+        }
+#pragma unroll
+        for (int piece = 0; piece < kPieces; ++piece) {
+          uint32_t w[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            w[r] = pack_bf16(d[r]);
+            if (piece + 1 < kPieces) d[r] = less_bf16(d[r], w[r]);
+          }
+          tmem_st8(to + 16 * piece + 8 * half, w);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) arrive(bars.empty + s);
+      tmem_st_wait();
+      fence_async();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(bars.ready + set);
+      // sums of stages that were handed over a round ago
+      if ((taken + 1) * kTaken <= i) take(taken++);
+    }
+    while (taken < takes) take(taken++);
+  }
+  const bool lost = settle(bars, left);
+  leave(p, bars, lost, s, round);
+  float(*const columns)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(smem);  // [group]: the ring is free
+  if (wid < kWarps) {
+    columns[set][0][quarter * 32 + lane] = lo32(of_low) + hi32(of_low);
+    columns[set][1][quarter * 32 + lane] = lo32(of_bias) + hi32(of_bias);
   }
   __syncthreads();
+  if (wid >= kWarps) return;
   const int i = quarter * 32 + lane;
-  const float more = lost ? __int_as_float(0x7fffffff) : columns[0][0][i];
+  float more = lost ? __int_as_float(0x7fffffff) : 0.0f, bias = more;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    more += columns[g][0][i];
+    bias += columns[g][1][i];
+  }
 #pragma unroll
   for (int j = 0; j < 32; ++j) sum[j] += more;
   if (p.splits > 1) {
-    float4* const to = reinterpret_cast<float4*>(p.part) + ((int64_t)split * (gridDim.x / p.splits) + tile) * (kTile * kTile / 4) + cols * 8 * kTile + i;
+    float4* const out = reinterpret_cast<float4*>(p.part) + ((int64_t)at.split * (gridDim.x / p.splits) + at.tile) * (kTile * kTile / 4) + set * 8 * kTile + i;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) to[j * kTile] = make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
-    if (group == 0 && tid < kTile) p.part_db[(int64_t)split * p.n_tiles * kTile + n0 + tid] = columns[0][1][tid];
+    for (int j = 0; j < 8; ++j) out[j * kTile] = make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
+    if (at.group == 0 && set == 0) p.part_db[(int64_t)at.split * p.n_tiles * kTile + at.n0 + i] = bias;
     return;
   }
-  if (n0 + i < p.n) {
-    const int first = group * kGroup + cols * 32, count = p.k - first;
-    T* const to = (T*)p.dw + (int64_t)(n0 + i) * p.k + first;
+  if (i >= cols) return;
+  const int first = at.group * kGroup + set * 32, count = p.k - first;
+  T* const out = (T*)p.dw + (int64_t)(at.n0 + i) * p.k + first;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < count) to[j] = from_float<T>(sum[j]);
-  }
-  if (group == 0 && tid < kTile && n0 + tid < p.n) ((T*)p.db)[n0 + tid] = from_float<T>(columns[0][1][tid]);
+  for (int j = 0; j < 32; ++j)
+    if (j < count) out[j] = from_float<T>(sum[j]);
+  if (at.group == 0 && set == 0) ((T*)p.db)[at.n0 + i] = from_float<T>(bias);
 }
 
-// Adds the parts up: 32 columns of dy and four of q to a CTA, an eighth of the parts to a warp.  Behind the tiles' CTAs those of db.
+// Adds the parts up: 32 lanes and four columns of TMEM to a CTA, an eighth of the parts to a warp.  Behind the tiles' CTAs those of db.  The lanes are columns
+// of x (bfloat16) or of dy.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int tiles) {
+  constexpr bool kOfX = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kColumns = kOfX ? kWide : kTile, kPerTile = kColumns, kQuads = kColumns * 128 / 4;
   __shared__ float4 of[8][33];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_tile = kTile * kTile / 128;
-  const bool bias = (int)blockIdx.x >= tiles * per_tile;
-  if (bias) {
-    const int i = ((int)blockIdx.x - tiles * per_tile) * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if ((int)blockIdx.x >= tiles * kPerTile) {
+    const int i = ((int)blockIdx.x - tiles * kPerTile) * 32 + lane;
     float sum = 0.0f;
-    for (int s = warp; s < p.splits; s += 8) sum += p.part_db[(int64_t)s * p.n_tiles * kTile + i];
+    for (int s = warp; s < p.splits; s += 8) sum += p.part_db[(int64_t)s * p.n_tiles * kColumns + i];
     of[warp][lane].x = sum;
     __syncthreads();
     if (warp != 0 || i >= p.n) return;
@@ -339,17 +562,19 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
     ((T*)p.db)[i] = from_float<T>(sum);
     return;
   }
-  const int tile = blockIdx.x / per_tile, rest = blockIdx.x % per_tile, quad = rest / 4, i = rest % 4 * 32 + lane;
-  const float4* const from = reinterpret_cast<const float4*>(p.part) + (int64_t)tile * (kTile * kTile / 4) + quad * kTile + i;
+  const int tile = blockIdx.x / kPerTile, rest = blockIdx.x % kPerTile, quad = rest / 4, i = rest % 4 * 32 + lane;
+  const float4* const from = reinterpret_cast<const float4*>(p.part) + (int64_t)tile * kQuads + quad * 128 + i;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
   for (int s = warp; s < p.splits; s += 8) {
-    const float4 v = from[(int64_t)s * tiles * (kTile * kTile / 4)];
+    const float4 v = from[(int64_t)s * tiles * kQuads];
     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
   }
   of[warp][lane] = sum;
   __syncthreads();
-  const int n = tile % p.n_tiles * kTile + i, col = tile / p.n_tiles * kGroup + quad * 4;
-  if (warp != 0 || n >= p.n) return;
+  const int across = tile % p.n_tiles * kColumns, down = tile / p.n_tiles * kGroup;
+  const int n = across + (kOfX ? quad * 4 : i), col = down + (kOfX ? i : quad * 4);
+  if (warp != 0 || n >= p.n || col >= p.k) return;
   sum = of[0][lane];
 #pragma unroll
   for (int w = 1; w < 8; ++w) {
@@ -360,73 +585,95 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (col + e < p.k) to[e] = from_float<T>(v[e]);
+    if ((kOfX ? n : col) + e < (kOfX ? p.n : p.k)) to[kOfX ? (int64_t)e * p.k : e] = from_float<T>(v[e]);
+}
+
+// Copies dy to rows that start on 16 bytes, where TMA can read them.
+template <typename T>
+__global__ void __launch_bounds__(256) align_kernel(const T* __restrict__ src, int64_t ld, int64_t n, T* __restrict__ dst, int64_t aligned_ld, int64_t m) {
+  dependency_wait();
+  release_dependents();
+  const int64_t total = m * n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / n;
+    dst[row * aligned_ld + (i - row * n)] = src[row * ld + (i - row * n)];
+  }
 }
 
 struct Plan {
-  int n_tiles, k_tiles, splits;
-  int64_t split_rows, part_bytes, bytes;
+  int columns, n_tiles, k_tiles, splits;
+  int64_t split_rows, part_bytes, sum_bytes, copy_ld, bytes;  // copy_ld: 0 where dy can be read where it is
 };
 
-// How many ways the rows are split: the choice of least time, in cycles: a stage takes an SM 600, a tile's start and end 5000, the parts' way through
-// L2 and back 64 KB each at 4000 bytes a cycle for all SMs, and the launch that adds them up 4000.
-static Plan plan(int64_t m, int64_t n, int64_t k) {
+// How many ways the rows are split: the choice of least time, in cycles: a stage takes an SM 600 (when the tensor cores or shared memory are what bounds it;
+// together the SMs get no more than 3500 bytes a cycle), a tile's start and end 5000, the parts' way through L2 and back 4000 bytes a cycle for all
+// SMs, and the launch that adds them up 4000.
+static Plan plan(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k) {
   Plan p{};
-  p.n_tiles = (int)ceil_div(n, kTile);
+  const int64_t item = dtype_size(dtype);
+  p.columns = dtype == F2C_BF16 ? kWide : kTile;
+  p.n_tiles = (int)ceil_div(n, p.columns);
   p.k_tiles = (int)ceil_div(k, kGroup);
-  const int64_t tiles = (int64_t)p.n_tiles * p.k_tiles, stages = ceil_div(m, kRows);
+  const int64_t tiles = (int64_t)p.n_tiles * p.k_tiles, stages = ceil_div(m, kRows), tile_bytes = (int64_t)p.columns * 128 * 4;
+  const int64_t first = ceil_div(m, kMaxSplitRows);
   int64_t least = INT64_MAX;
-  for (int64_t s = 1; s <= std::min<int64_t>(stages, kSmCount); ++s) {
-    if (s > 1 && tiles * s > 2 * kSmCount) break;
+  for (int64_t s = first; s <= std::min<int64_t>(stages, std::max<int64_t>(first, kSmCount)); ++s) {
+    if (s > first && tiles * s > 2 * kSmCount) break;
     const int64_t each = ceil_div(stages, s);
-    if (s > 1 && ceil_div(stages, each) != s) continue;  // (the last ones would have none)
-    const int64_t cycles = ceil_div(tiles * s, kSmCount) * (each * 600 + 5000) + (s > 1 ? 4000 + tiles * s * 2 * 65536 / 4000 : 0);
+    if (s > first && ceil_div(stages, each) != s) continue;  // (the last ones would have none)
+    const int64_t rounds = ceil_div(tiles * s, kSmCount), stage_bytes = kRows * ((int64_t)p.columns * item / p.k_tiles + 128 / p.n_tiles);
+    const int64_t stage = std::max<int64_t>(600, std::min<int64_t>(tiles * s, kSmCount) * stage_bytes / 3500);
+    const int64_t cycles = rounds * (each * stage + 5000) + (s > 1 ? 4000 + tiles * s * 2 * tile_bytes / 4000 : 0);
     if (cycles >= least) continue;
     least = cycles;
-    p.splits = (int)s;
     p.split_rows = each * kRows;
+    p.splits = (int)ceil_div(stages, each);
   }
   if (p.splits > 1) {
-    p.part_bytes = tiles * p.splits * kTile * kTile * 4;
-    p.bytes = p.part_bytes + ceil_div((int64_t)p.splits * p.n_tiles * kTile * 4, 256) * 256;
+    p.part_bytes = tiles * p.splits * tile_bytes;
+    p.sum_bytes = ceil_div((int64_t)p.splits * p.n_tiles * p.columns * 4, 256) * 256;
+  }
+  p.bytes = p.part_bytes + p.sum_bytes;
+  if (!aligned(dy, 16) || (m > 1 && ldy * item % 16 != 0)) {
+    p.copy_ld = ceil_div(n * item, 16) * 16 / item;
+    p.bytes += ceil_div(m * p.copy_ld * item, 256) * 256;
   }
   return p;
 }
 
-template <typename T, int ACCESS>
-static int run(const char* op, const Params& p, const Plan& how, cudaStream_t st) {
-  constexpr int bytes = kStages * (Kind<T>::kPieces + 1) * kPlane + 1024;
+// A map of a row-major matrix for boxes of kRows rows of 128 bytes.
+static bool rows_map(CUtensorMap* map, const void* base, int64_t item, int64_t m, int64_t cols, int64_t ld) {
+  // (a lone row may have any stride)
+  const int64_t row_bytes = m > 1 ? ld * item : ceil_div(cols * item, 16) * 16;
+  return make_map(map, base, (int)item, m, cols, row_bytes, kRows);
+}
+
+template <typename T>
+static int run(const char* op, const CUtensorMap& dy, const CUtensorMap& codes, const Params& p, const Plan& how, cudaStream_t st) {
   const int tiles = how.n_tiles * how.k_tiles;
-  if (const int rc = allow_smem(op, (const void*)weight_grad_kernel<T, ACCESS>, bytes)) return rc;
-  launch_dependent(weight_grad_kernel<T, ACCESS>, dim3((unsigned)(tiles * how.splits)), kThreads, bytes, st, p);
-  if (how.splits > 1) launch_dependent(join_kernel<T>, dim3((unsigned)(tiles * (kTile * kTile / 128) + how.n_tiles * 4)), 256, 0, st, p, tiles);
+  const dim3 grid((unsigned)(tiles * how.splits));
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    if (const int rc = allow_smem(op, (const void*)rows_kernel, kWideSmem)) return rc;
+    launch_dependent(rows_kernel, grid, kThreads, kWideSmem, st, dy, codes, p);
+  } else {
+    if (const int rc = allow_smem(op, (const void*)scaled_kernel<T>, kTileSmem<T>)) return rc;
+    launch_dependent(scaled_kernel<T>, grid, kThreads, kTileSmem<T>, st, dy, codes, p);
+  }
+  if (how.splits > 1)
+    launch_dependent(join_kernel<T>, dim3((unsigned)(tiles * how.columns + how.n_tiles * how.columns / 32)), 256, 0, st, p, tiles);
   return check_launch(op);
 }
 
-// by the widest loads that dy's rows allow
-template <typename T>
-static int run(const char* op, const Params& p, const Plan& how, cudaStream_t st) {
-  int access = 16;
-  const int64_t item = sizeof(T);
-  while (access > item && (!aligned(p.dy, access) || p.n * item % access != 0 || (p.m > 1 && p.ldy * item % access != 0))) access /= 2;
-  if (access == 16) return run<T, 16>(op, p, how, st);
-  if (access == 8) return run<T, 8>(op, p, how, st);
-  if constexpr (sizeof(T) == 2) {
-    if (access == 2) return run<T, 2>(op, p, how, st);
-  }
-  return run<T, 4>(op, p, how, st);
-}
-
-static bool too_large(int64_t m, int64_t n, int64_t k) { return m >= ckpt::kMaxRows || n > (1 << 17) || k > (1 << 17); }
+static bool too_large(int64_t m, int64_t n, int64_t k) { return m >= ckpt::kMaxRows - kRows * kStages || n > (1 << 17) || k > (1 << 17); }
 
 }  // namespace wg
 }  // namespace f2c
 
 using namespace f2c;
 
-extern "C" int64_t f2c_checkpoint_weight_grad_workspace(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0 || wg::too_large(m, n, k)) return 0;
-  return wg::plan(m, n, k).bytes;
+extern "C" int64_t f2c_checkpoint_weight_grad_workspace(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0 || !is_float_dtype(dtype) || wg::too_large(m, n, k)) return 0;
+  return wg::plan(dy, ldy, dtype, m, n, k).bytes;
 }
 
 extern "C" int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype, const uint8_t* codes, int64_t ldq, const float* scales, int64_t m, int64_t n, int64_t k, void* dw,
@@ -434,7 +681,7 @@ extern "C" int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype
   const char* op = "checkpoint_weight_grad";
   if (const int rc = ckpt::check_sizes(op, dtype, m, k)) return rc;
   F2C_REQUIRE(n >= 0, F2C_ERR_INVALID, "%s: negative size", op);
-  F2C_REQUIRE(!wg::too_large(m, n, k), F2C_ERR_LIMIT, "%s: 2^31 rows, or more than 2^17 columns", op);
+  F2C_REQUIRE(!wg::too_large(m, n, k), F2C_ERR_LIMIT, "%s: 2^31 - 256 rows, or more than 2^17 columns", op);
   F2C_REQUIRE((flags & ~F2C_NO_WAITS) == 0, F2C_ERR_INVALID, "%s: unknown flags", op);
   if (const int rc = ckpt::check_codes(op, codes, ldq, scales, m, k)) return rc;
   if (n == 0) return F2C_OK;
@@ -443,19 +690,30 @@ extern "C" int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype
   F2C_REQUIRE(m <= 1 || ldy >= n, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
   F2C_REQUIRE(k > 0 || m == 0, F2C_ERR_INVALID, "%s: no columns", op);
   cudaStream_t st = (cudaStream_t)stream;
+  const int64_t item = dtype_size(dtype);
   if (m == 0) {
-    cudaError_t e = cudaMemsetAsync(db, 0, (size_t)(n * dtype_size(dtype)), st);
-    if (e == cudaSuccess && k > 0) e = cudaMemsetAsync(dw, 0, (size_t)(n * k * dtype_size(dtype)), st);
+    cudaError_t e = cudaMemsetAsync(db, 0, (size_t)(n * item), st);
+    if (e == cudaSuccess && k > 0) e = cudaMemsetAsync(dw, 0, (size_t)(n * k * item), st);
     if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
     return F2C_OK;
   }
-  const wg::Plan how = wg::plan(m, n, k);
+  const wg::Plan how = wg::plan(dy, ldy, dtype, m, n, k);
   F2C_REQUIRE(how.bytes == 0 || (workspace && workspace_bytes >= how.bytes && aligned(workspace, 256)), F2C_ERR_INVALID,
               "%s: the workspace must have %lld bytes, 256-byte aligned", op, (long long)how.bytes);
-  const wg::Params p{dy, ldy, m, (int)n, (int)k, ckpt::Codes{const_cast<uint8_t*>(codes), ldq, const_cast<float*>(scales), ceil_div(k, ckpt::kGroup)}, how.n_tiles, how.splits, how.split_rows,
-               dw, db, (float*)workspace, (float*)((char*)workspace + how.part_bytes),
-               (flags & F2C_NO_WAITS) ? 0u : t5::kWaitLimit, stream_error_word()};
-  if (dtype == F2C_F32) return wg::run<float>(op, p, how, st);
-  if (dtype == F2C_F16) return wg::run<__half>(op, p, how, st);
-  return wg::run<__nv_bfloat16>(op, p, how, st);
+  char* const ws = (char*)workspace;
+  if (how.copy_ld != 0) {
+    char* const copy = ws + how.part_bytes + how.sum_bytes;
+    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(m * n, 256), 16 * kSmCount));
+    if (item == 4) launch_dependent(wg::align_kernel<uint32_t>, grid, 256, 0, st, (const uint32_t*)dy, ldy, n, (uint32_t*)copy, how.copy_ld, m);
+    else launch_dependent(wg::align_kernel<uint16_t>, grid, 256, 0, st, (const uint16_t*)dy, ldy, n, (uint16_t*)copy, how.copy_ld, m);
+    dy = copy;
+    ldy = how.copy_ld;
+  }
+  CUtensorMap maps[2] = {};
+  F2C_REQUIRE(wg::rows_map(maps, dy, item, m, n, ldy) && wg::rows_map(maps + 1, codes, 1, m, k, ldq), F2C_ERR_CUDA, "%s: tensor map", op);
+  const wg::Params p{scales, ceil_div(k, ckpt::kGroup), m, (int)n, (int)k, how.n_tiles, how.splits, how.split_rows, dw, db, (float*)ws, (float*)(ws + how.part_bytes),
+                     (flags & F2C_NO_WAITS) ? 0u : t5::kWaitLimit, stream_error_word()};
+  if (dtype == F2C_F32) return wg::run<float>(op, maps[0], maps[1], p, how, st);
+  if (dtype == F2C_F16) return wg::run<__half>(op, maps[0], maps[1], p, how, st);
+  return wg::run<__nv_bfloat16>(op, maps[0], maps[1], p, how, st);
 }

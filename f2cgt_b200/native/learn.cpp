@@ -133,7 +133,7 @@ PyObject* checkpoint_weight_grad(PyObject*, PyObject* const* a, Py_ssize_t n) { 
       c10::cuda::CUDAGuard guard(dy.device());
       dw = empty({cols, k}, dy.scalar_type(), dy.device());
       db = empty({cols}, dy.scalar_type(), dy.device());
-      const int64_t bytes = f2c_checkpoint_weight_grad_workspace(m, cols, k);
+      const int64_t bytes = f2c_checkpoint_weight_grad_workspace(dy.const_data_ptr(), row_stride(dy), dtype_tag(dy.scalar_type()), m, cols, k);
       at::Tensor ws;
       if (bytes > 0) ws = empty({bytes}, at::kByte, dy.device());
       return f2c_checkpoint_weight_grad(dy.const_data_ptr(), row_stride(dy), dtype_tag(dy.scalar_type()), c.q(), c.ld, c.s(), m, cols, k, dw.mutable_data_ptr(), db.mutable_data_ptr(), 0,

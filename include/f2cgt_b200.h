@@ -465,10 +465,11 @@ int f2c_checkpoint_values(const uint8_t* codes, int64_t ldq, const float* scales
                           void* stream);
 /* Gradient of a linear layer y = x W^T + b from dy [m, n] (`dtype`: F32, F16 or BF16, row stride ldy) and x [m, k] in 8 bits:
  *   dw [n, k] = dy^T x,  db [n] = the sums of dy's columns, both of `dtype`, rounded once; x is not written out.
- * dy times a code's step is held to 24 bits for F32 and to 16 for the others, sums are single precision in an order that the sizes decide.
- * Codes as f2c_checkpoint_int8 leaves them (every row has whole 16 bytes).  m < 2^31, n and k up to 2^17.  flags: 0, or F2C_NO_WAITS.
- * workspace: f2c_checkpoint_weight_grad_workspace(m, n, k) bytes, 256-byte aligned.  A bounded wait that runs out reports 8 and leaves NaN. */
-int64_t f2c_checkpoint_weight_grad_workspace(int64_t m, int64_t n, int64_t k);
+ * dy times a code's step is held to 24 bits for F32 and to 16 for F16, x to 16 bits for BF16; sums are single precision in an order that the sizes decide.
+ * Codes as f2c_checkpoint_int8 leaves them (every row has whole 16 bytes).  m < 2^31 - 256, n and k up to 2^17.  flags: 0, or F2C_NO_WAITS.
+ * workspace: f2c_checkpoint_weight_grad_workspace(...) bytes, 256-byte aligned; it depends on where dy starts and on its stride (rows that do not start on
+ * 16 bytes are copied): ask with those of the call.  A bounded wait that runs out reports 8 and leaves NaN. */
+int64_t f2c_checkpoint_weight_grad_workspace(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k);
 int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype, const uint8_t* codes, int64_t ldq, const float* scales, int64_t m, int64_t n, int64_t k,
                                void* dw, void* db, int flags, void* workspace, int64_t workspace_bytes, void* stream);
 /* y [m, d] = (x - mean) rstd weight + bias of every row, rstd = 1 / sqrt(mean((x - mean)^2) + eps); relu != 0: negative values become 0 (a NaN
