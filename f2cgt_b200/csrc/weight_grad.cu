@@ -7,11 +7,11 @@
 //  * bfloat16 dy (rows_kernel).  dy is an operand as it is.  x is two bfloat16 numbers, 16 bits, of a product that is rounded to 8: two MMAs of
 //    128 columns of x (the lanes of TMEM) by 256 of dy for every 16 rows.
 //  * float32 and float16 dy (scaled_kernel).  With the factors taken to the other side, dW = (step dy)^T q + (low dy)^T 1: the codes 0 .. 255 are
-//    bfloat16 numbers as they are, and step dy, rounded to single precision, is a sum of three of them (all 24 bits; float32) or two (16 bits; float16, whose
-//    range bfloat16 has and float16 values of x might leave).  The second term is one number for every column of dy and group, summed in registers.  128
+//    bfloat16 numbers as they are, and step dy, rounded to single precision, is a sum of three of them (its 24 bits, eight each; float32) or two (16 bits;
+//    float16, whose range bfloat16 has and float16 values of x might leave).  The second term is one number for every column of dy and group, summed in registers.  128
 //    columns of dy (the lanes) by a group.
 //
-// Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows.  So for float32 they are taken out every 128 rows and added up in
+// Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows.  So for float32 they are taken out every 256 rows and added up in
 // registers, while the MMAs go on in the other half of the accumulators; elsewhere every 16,384 rows (float16), and once a part of at most 65,536 rows.
 //
 // Many rows and few tiles: the rows are dealt out over all SMs; each leaves its part of the sums, and a second launch adds them up in their order.
@@ -83,7 +83,9 @@ __device__ __forceinline__ uint32_t pack_bf16(f32x2 v) {  // round to even
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi32(v)), "f"(lo32(v)));
   return r;
 }
-// v less the two numbers of w: exact where they are v rounded
+// the same cut off
+__device__ __forceinline__ uint32_t cut_bf16(f32x2 v) { return __byte_perm((uint32_t)v, (uint32_t)(v >> 32), 0x7632); }
+// v less the two numbers of w: exact where they are v rounded or cut off
 __device__ __forceinline__ f32x2 less_bf16(f32x2 v, uint32_t w) { return fma2(pair_of(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), both(-1.0f), v); }
 __device__ __forceinline__ uint32_t lds_u8(uint32_t at) {
   uint32_t v;
@@ -354,7 +356,7 @@ constexpr uint32_t kCodesBytes = 2 * kBox;     // a stage's codes as bfloat16
 // kTaken: stages between two takings out
 template <typename T> struct Kind;
 template <> struct Kind<float> {
-  static constexpr int kPieces = 3, kTaken = 4, kEach = 32;
+  static constexpr int kPieces = 3, kTaken = 8, kEach = 32;
   static constexpr uint32_t kStage = 5 * kBox;
 };
 template <> struct Kind<__half> {
@@ -380,10 +382,9 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
   begin(bars, 4);  // a stage is free when its group's warps have read it
   const uint32_t tmem = bars.tmem, ring = smem_u32(smem), q_ring = ring + kStages * kStage, a_tmem = tmem + 2 * kTile;
   const int quarter = wid & 3, set = wid >> 2;
-  float sum[32];
-  f32x2 of_low = 0ull, of_bias = 0ull;
+  f32x2 sum[16], of_low = 0ull, of_bias = 0ull;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) sum[j] = 0.0f;
+  for (int j = 0; j < 16; ++j) sum[j] = 0ull;
   dependency_wait();
   release_dependents();
 
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
       tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((t & 1) * kTile + set * 32), r);
       tmem_wait(r);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(r[j]);
+      for (int j = 0; j < 16; ++j) sum[j] = plus2(sum[j], pair_of(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
       fence_before();
       __syncwarp();
       if (lane == 0) arrive(bars.acc_empty + (t & 1));
@@ -441,33 +442,23 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
       scale.tell(scales_s[wid]);
       scale.fetch(p, at.row0, at.rows, i + kGroups, at.group);
       wait_bar(bars.full + s, (uint32_t)(i / kStages) & 1, left);
-      if (use > 0) wait_bar(bars.taken + set, (uint32_t)(use - 1) & 1, left);
-      fence_after();
       const uint32_t stage = (uint32_t)s * kStage;
-#pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {  // 16 codes
-        const uint4 q = lds_u128(ring + stage + kCodesAt + q_row * 128 + (((q_part * 2 + h) ^ (q_row & 7)) << 4));
-        const uint32_t box = q_ring + (uint32_t)set * kCodesBytes + (q_part >> 1) * kBox + q_row * 128, first = (q_part & 1) * 4 + 2 * h;
-        f32x2 a[2], b[2];
-        ckpt::numbers_of(q.x, a);
-        ckpt::numbers_of(q.y, b);
-        sts_u128(box + ((first ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
-        ckpt::numbers_of(q.z, a);
-        ckpt::numbers_of(q.w, b);
-        sts_u128(box + (((first + 1) ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
-      }
       const bool mine = quarter * 32 < cols;  // (behind them nothing was loaded)
       // 16 rows at a time: more did not fit into the registers beside the sums
-#pragma unroll 1
+#pragma unroll
       for (uint32_t half = 0; half < 2; ++half) {
         f32x2 d[8];
         const uint32_t from = stage + half * 2048;
+        if (mine) {
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const uint32_t even = column[r & 7] + from + (uint32_t)(r >> 3) * 1024, odd = column[(r + 1) & 7] + from + (uint32_t)(r >> 3) * 1024;
-          if (!mine) d[r / 2] = 0ull;
-          else if constexpr (sizeof(T) == 4) d[r / 2] = pair_of(__uint_as_float(lds_u32(even)), __uint_as_float(lds_u32(odd)));
-          else d[r / 2] = pair_of(__half2float(__ushort_as_half((unsigned short)lds_u16(even))), __half2float(__ushort_as_half((unsigned short)lds_u16(odd))));
+          for (int r = 0; r < 16; r += 2) {
+            const uint32_t even = column[r & 7] + from + (uint32_t)(r >> 3) * 1024, odd = column[(r + 1) & 7] + from + (uint32_t)(r >> 3) * 1024;
+            if constexpr (sizeof(T) == 4) d[r / 2] = pair_of(__uint_as_float(lds_u32(even)), __uint_as_float(lds_u32(odd)));
+            else d[r / 2] = pair_of(__half2float(__ushort_as_half((unsigned short)lds_u16(even))), __half2float(__ushort_as_half((unsigned short)lds_u16(odd))));
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) d[r] = 0ull;
         }
         if (at.group == 0) {
 #pragma unroll
@@ -487,11 +478,27 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
           uint32_t w[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            w[r] = pack_bf16(d[r]);
+            w[r] = kPieces == 3 ? cut_bf16(d[r]) : pack_bf16(d[r]);  // (of three, what the last leaves is nothing)
             if (piece + 1 < kPieces) d[r] = less_bf16(d[r], w[r]);
+          }
+          if (piece == 0 && half == 0) {  // what the group handed over a round ago has been used
+            if (use > 0) wait_bar(bars.taken + set, (uint32_t)(use - 1) & 1, left);
+            fence_after();
           }
           tmem_st8(to + 16 * piece + 8 * half, w);
         }
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {  // 16 codes
+        const uint4 q = lds_u128(ring + stage + kCodesAt + q_row * 128 + (((q_part * 2 + h) ^ (q_row & 7)) << 4));
+        const uint32_t box = q_ring + (uint32_t)set * kCodesBytes + (q_part >> 1) * kBox + q_row * 128, first = (q_part & 1) * 4 + 2 * h;
+        f32x2 a[2], b[2];
+        ckpt::numbers_of(q.x, a);
+        ckpt::numbers_of(q.y, b);
+        sts_u128(box + ((first ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
+        ckpt::numbers_of(q.z, a);
+        ckpt::numbers_of(q.w, b);
+        sts_u128(box + (((first + 1) ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
       }
       __syncwarp();
       if (lane == 0) arrive(bars.empty + s);
@@ -522,11 +529,11 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
     bias += columns[g][1][i];
   }
 #pragma unroll
-  for (int j = 0; j < 32; ++j) sum[j] += more;
+  for (int j = 0; j < 16; ++j) sum[j] = plus2(sum[j], both(more));
   if (p.splits > 1) {
-    float4* const out = reinterpret_cast<float4*>(p.part) + ((int64_t)at.split * (gridDim.x / p.splits) + at.tile) * (kTile * kTile / 4) + set * 8 * kTile + i;
+    ulonglong2* const out = reinterpret_cast<ulonglong2*>(p.part) + ((int64_t)at.split * (gridDim.x / p.splits) + at.tile) * (kTile * kTile / 4) + set * 8 * kTile + i;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out[j * kTile] = make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
+    for (int j = 0; j < 8; ++j) out[j * kTile] = make_ulonglong2(sum[2 * j], sum[2 * j + 1]);
     if (at.group == 0 && set == 0) p.part_db[(int64_t)at.split * p.n_tiles * kTile + at.n0 + i] = bias;
     return;
   }
@@ -535,38 +542,39 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
   T* const out = (T*)p.dw + (int64_t)(at.n0 + i) * p.k + first;
 #pragma unroll
   for (int j = 0; j < 32; ++j)
-    if (j < count) out[j] = from_float<T>(sum[j]);
+    if (j < count) out[j] = from_float<T>(j & 1 ? hi32(sum[j / 2]) : lo32(sum[j / 2]));
   if (at.group == 0 && set == 0) ((T*)p.db)[at.n0 + i] = from_float<T>(bias);
 }
 
-// Adds the parts up: 32 lanes and four columns of TMEM to a CTA, an eighth of the parts to a warp.  Behind the tiles' CTAs those of db.  The lanes are columns
+// Adds the parts up: 32 lanes and four columns of TMEM to a CTA, every 16th part (or as many as there are) to a
+// warp.  Behind the tiles' CTAs those of db.  The lanes are columns
 // of x (bfloat16) or of dy.
+constexpr int kJoinWarps = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int tiles) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Params p, int tiles) {
   constexpr bool kOfX = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kColumns = kOfX ? kWide : kTile, kPerTile = kColumns, kQuads = kColumns * 128 / 4;
-  __shared__ float4 of[8][33];
+  __shared__ float4 of[kJoinWarps][33];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   if ((int)blockIdx.x >= tiles * kPerTile) {
     const int i = ((int)blockIdx.x - tiles * kPerTile) * 32 + lane;
     float sum = 0.0f;
-    for (int s = warp; s < p.splits; s += 8) sum += p.part_db[(int64_t)s * p.n_tiles * kColumns + i];
+    for (int s = warp; s < p.splits; s += warps) sum += p.part_db[(int64_t)s * p.n_tiles * kColumns + i];
     of[warp][lane].x = sum;
     __syncthreads();
     if (warp != 0 || i >= p.n) return;
     sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) sum += of[w][lane].x;
+    for (int w = 0; w < warps; ++w) sum += of[w][lane].x;
     ((T*)p.db)[i] = from_float<T>(sum);
     return;
   }
   const int tile = blockIdx.x / kPerTile, rest = blockIdx.x % kPerTile, quad = rest / 4, i = rest % 4 * 32 + lane;
   const float4* const from = reinterpret_cast<const float4*>(p.part) + (int64_t)tile * kQuads + quad * 128 + i;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int s = warp; s < p.splits; s += 8) {
+#pragma unroll 10
+  for (int s = warp; s < p.splits; s += warps) {
     const float4 v = from[(int64_t)s * tiles * kQuads];
     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
   }
@@ -576,8 +584,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   const int n = across + (kOfX ? quad * 4 : i), col = down + (kOfX ? i : quad * 4);
   if (warp != 0 || n >= p.n || col >= p.k) return;
   sum = of[0][lane];
-#pragma unroll
-  for (int w = 1; w < 8; ++w) {
+  for (int w = 1; w < warps; ++w) {
     const float4 v = of[w][lane];
     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
   }
@@ -605,9 +612,9 @@ struct Plan {
   int64_t split_rows, part_bytes, sum_bytes, copy_ld, bytes;  // copy_ld: 0 where dy can be read where it is
 };
 
-// How many ways the rows are split: the choice of least time, in cycles: a stage takes an SM 600 (when the tensor cores or shared memory are what bounds it;
-// together the SMs get no more than 3500 bytes a cycle), a tile's start and end 5000, the parts' way through L2 and back 4000 bytes a cycle for all
-// SMs, and the launch that adds them up 4000.
+// How many ways the rows are split: the choice of least time, in cycles: a stage takes an SM 560 (bfloat16: its MMAs), 1200 (float32) or 900 (float16: what
+// the groups do for it); together the SMs get no more than 3500 bytes a cycle; a tile's start and end 4000, the parts' way through L2 and back 4000 bytes a
+// cycle for all SMs, and the launch that adds them up 4000.
 static Plan plan(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k) {
   Plan p{};
   const int64_t item = dtype_size(dtype);
@@ -622,8 +629,8 @@ static Plan plan(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, i
     const int64_t each = ceil_div(stages, s);
     if (s > first && ceil_div(stages, each) != s) continue;  // (the last ones would have none)
     const int64_t rounds = ceil_div(tiles * s, kSmCount), stage_bytes = kRows * ((int64_t)p.columns * item / p.k_tiles + 128 / p.n_tiles);
-    const int64_t stage = std::max<int64_t>(600, std::min<int64_t>(tiles * s, kSmCount) * stage_bytes / 3500);
-    const int64_t cycles = rounds * (each * stage + 5000) + (s > 1 ? 4000 + tiles * s * 2 * tile_bytes / 4000 : 0);
+    const int64_t stage = std::max<int64_t>(dtype == F2C_BF16 ? 560 : dtype == F2C_F32 ? 1200 : 900, std::min<int64_t>(tiles * s, kSmCount) * stage_bytes / 3500);
+    const int64_t cycles = rounds * (each * stage + 4000) + (s > 1 ? 4000 + tiles * s * 2 * tile_bytes / 4000 : 0);
     if (cycles >= least) continue;
     least = cycles;
     p.split_rows = each * kRows;
@@ -660,7 +667,7 @@ static int run(const char* op, const CUtensorMap& dy, const CUtensorMap& codes, 
     launch_dependent(scaled_kernel<T>, grid, kThreads, kTileSmem<T>, st, dy, codes, p);
   }
   if (how.splits > 1)
-    launch_dependent(join_kernel<T>, dim3((unsigned)(tiles * how.columns + how.n_tiles * how.columns / 32)), 256, 0, st, p, tiles);
+    launch_dependent(join_kernel<T>, dim3((unsigned)(tiles * how.columns + how.n_tiles * how.columns / 32)), 32 * std::min(kJoinWarps, how.splits), 0, st, p, tiles);
   return check_launch(op);
 }
 
