@@ -195,7 +195,7 @@ template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ ids, Pairs in, int64_t m, uint32_t rows, Digit d, const uint32_t* __restrict__ counts,
                                                          const uint32_t* __restrict__ totals, Pairs out, Digit next, uint32_t* __restrict__ counts_next) {
   constexpr int kBins = 1 << kMaxBits, kEach = kBins / kThreads;
-  __shared__ uint16_t of_warp[kWarps][kBins];  // a tile has 1024 places
+  __shared__ __align__(16) uint16_t of_warp[kWarps][kBins];  // a tile has 1024 places
   __shared__ __align__(16) uint32_t base[kBins];
   __shared__ uint32_t sums[kWarps];
   dependency_wait();
@@ -232,23 +232,28 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ i
   for (int q = 0; q < kItems; ++q) {
     const bool there = first + 32 * q < m;
     const uint32_t digit = digit_of(key[q], d), those = __ballot_sync(0xffffffffu, there);
-    uint32_t equal = 0u, so_far = 0u;
-    if (there) {
-      equal = __match_any_sync(those, digit);
-      so_far = of_warp[warp][digit];
+    // the lanes with the same digit, bit by bit
+    uint32_t equal = those;
+#pragma unroll
+    for (int b = 0; b < kMaxBits; ++b) {
+      const bool one = (digit >> b) & 1u;
+      const uint32_t ones = __ballot_sync(0xffffffffu, one);
+      equal &= one ? ones : ~ones;
     }
+    const uint32_t so_far = there ? of_warp[warp][digit] : 0u;
     __syncwarp();
     if (there && (equal & ((1u << lane) - 1u)) == 0u) of_warp[warp][digit] = (uint16_t)(so_far + __popc(equal));
     __syncwarp();
     rank[q] = so_far + __popc(equal & ((1u << lane) - 1u));
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += kThreads) {
+  for (int b = threadIdx.x; b < bins / 2; b += kThreads) {  // two digits at once: their sums over the tile's warps stay below 2^16
     uint32_t so_far = 0u;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const uint32_t own = of_warp[w][b];
-      of_warp[w][b] = (uint16_t)so_far;
+      uint32_t* const at = reinterpret_cast<uint32_t*>(of_warp[w]) + b;
+      const uint32_t own = *at;
+      *at = so_far;
       so_far += own;
     }
   }
