@@ -3,8 +3,9 @@
 //
 // Bound by reading and writing the rows.  A row's values stay in registers between the mean, the squares of the differences from it (no
 // cancellation of large means) and the result: a warp has rows up to 1024 columns long, several at a time where they are short so that enough loads are on
-// the way; a CTA has longer ones, one after the other, the next one's loads on the way and its columns' weights in registers; rows beyond 8192 columns it
-// reads again for every step.
+// the way; a CTA of four warps (eight beyond 4096 columns) has longer ones, one after the other, the next one's loads on the way: five or six of them to an SM
+// (two of eight warps, their columns' weights in registers, waited more than they worked: 16,384 x 4096 bfloat16 64 us); rows beyond 8192 columns it reads
+// again for every step.
 #include "checkpoint.cuh"
 
 namespace f2c {
@@ -39,19 +40,25 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// of four values of columns [at, at + 4) of a vector that starts anywhere
+// Four values of a vector, at `w` those of this lane's first columns (null: `otherwise`), where all four exist and start on 16 bytes
+__device__ __forceinline__ void of_columns(const float* w, float otherwise, f32x2 (&v)[2]) {
+  float4 f = make_float4(otherwise, otherwise, otherwise, otherwise);
+  if (w != nullptr) f = __ldg(reinterpret_cast<const float4*>(w));
+  v[0] = pair_of(f.x, f.y);
+  v[1] = pair_of(f.z, f.w);
+}
+// the same of columns [at, at + 4) of a vector that starts anywhere.  (One by one in a function of its own: as a branch they were eight loads beside every two.)
+static __device__ __noinline__ float4 one_by_one(const float* w, int left, float otherwise) {
+  return make_float4(__ldg(w), left > 1 ? __ldg(w + 1) : otherwise, left > 2 ? __ldg(w + 2) : otherwise, left > 3 ? __ldg(w + 3) : otherwise);
+}
 __device__ __forceinline__ void of_columns(const float* w, int at, int left, float otherwise, f32x2 (&v)[2]) {
-  if (w == nullptr || left <= 0) {
-    v[0] = v[1] = both(otherwise);
-  } else if (left >= 4 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(w + at));
-    v[0] = pair_of(f.x, f.y);
-    v[1] = pair_of(f.z, f.w);
-  } else {
-    const float f0 = __ldg(w + at), f1 = left > 1 ? __ldg(w + at + 1) : otherwise, f2 = left > 2 ? __ldg(w + at + 2) : otherwise, f3 = left > 3 ? __ldg(w + at + 3) : otherwise;
-    v[0] = pair_of(f0, f1);
-    v[1] = pair_of(f2, f3);
+  float4 f = make_float4(otherwise, otherwise, otherwise, otherwise);
+  if (w != nullptr && left > 0) {
+    if (left >= 4 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) f = __ldg(reinterpret_cast<const float4*>(w + at));
+    else f = one_by_one(w + at, left, otherwise);
   }
+  v[0] = pair_of(f.x, f.y);
+  v[1] = pair_of(f.z, f.w);
 }
 
 // Squares of the differences from the mean, of the columns that there are.
@@ -66,13 +73,14 @@ __device__ __forceinline__ f32x2 add_squares(const f32x2 (&x)[2], f32x2 less, in
 __device__ __forceinline__ float sum_of(f32x2 v) { return lo32(v) + hi32(v); }
 
 // Everything that a lane writes of four columns of a row, of which `left` exist; by whole warps.
-template <typename T, int ACCESS>
-__device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, int left, const f32x2 (&x)[2], float mean, float rstd, const f32x2 (&w)[2], const f32x2 (&b)[2]) {
+// KEEP: with what is wanted for the backward pass beside the result.
+template <typename T, int ACCESS, bool KEEP>
+__device__ __forceinline__ void finish(const Args& a, T* y, int64_t row, int chunk, int left, const f32x2 (&x)[2], float mean, float rstd, const f32x2 (&w)[2], const f32x2 (&b)[2]) {
   const int lane = threadIdx.x & 31, col = chunk * kGroup + 4 * lane;
   f32x2 z[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) z[h] = fma2(mul2(plus2(x[h], both(-mean)), both(rstd)), w[h], b[h]);
-  if (a.active != nullptr) {
+  if (KEEP && a.active != nullptr) {
     uint32_t bits = (lo32(z[0]) > 0.0f) | (hi32(z[0]) > 0.0f) << 1 | (lo32(z[1]) > 0.0f) << 2 | (hi32(z[1]) > 0.0f) << 3;
     if (left < 4) bits &= (1u << max(left, 0)) - 1u;
     bits |= __shfl_down_sync(0xffffffffu, bits, 1) << 4;
@@ -84,8 +92,8 @@ __device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, in
   }
   Four<T, ACCESS> out;
   out.set(z);
-  out.store((T*)a.y + row * a.d + col, left);
-  if (a.codes.codes != nullptr) {
+  out.store(y, left);
+  if (KEEP && a.codes.codes != nullptr) {
     ckpt::Scale s;
     const uint32_t q = ckpt::encode(x, left, s);
     if (left > 0) *reinterpret_cast<uint32_t*>(a.codes.codes + row * a.codes.ld + col) = q;
@@ -96,7 +104,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t row, int chunk, in
 constexpr int kThreads = 256;
 
 // ROWS rows of CHUNKS * 128 columns for every warp; the last chunk may have fewer, unless EVEN
-template <typename T, int ACCESS, int CHUNKS, int ROWS, bool EVEN>
+template <typename T, int ACCESS, int CHUNKS, int ROWS, bool EVEN, bool KEEP>
 __global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 3 : 2) warp_kernel(const __grid_constant__ Args a) {
   dependency_wait();
   release_dependents();
@@ -105,16 +113,25 @@ __global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 3 : 2) warp_kernel(con
   const auto left_of = [&](int c) { return EVEN || c + 1 < CHUNKS ? 4 : a.d - c * kGroup - 4 * lane; };
   Four<T, ACCESS> raw[ROWS][CHUNKS];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r)
+  for (int r = 0; r < ROWS; ++r) {
+    const T* const x = (const T*)a.x + (first + r) * a.ldx + 4 * lane;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) raw[r][c].load((const T*)a.x + (first + r) * a.ldx + c * kGroup + 4 * lane, first + r < a.m ? left_of(c) : 0);
+    for (int c = 0; c < CHUNKS; ++c) raw[r][c].load(x + c * kGroup, first + r < a.m ? left_of(c) : 0);
+  }
   constexpr int kHeld = ROWS > 1 ? CHUNKS : 1;  // of weights: all where they are used more than once, or the first chunk's
   f32x2 w[kHeld][2], b[kHeld][2];
+  const float *const weight = EVEN && a.weight != nullptr ? a.weight + 4 * lane : a.weight, *const bias = EVEN && a.bias != nullptr ? a.bias + 4 * lane : a.bias;
+  const auto weights = [&](int c, f32x2 (&w)[2], f32x2 (&b)[2]) {
+    if constexpr (EVEN) {
+      of_columns(weight != nullptr ? weight + c * kGroup : nullptr, 1.0f, w);
+      of_columns(bias != nullptr ? bias + c * kGroup : nullptr, 0.0f, b);
+    } else {
+      of_columns(weight, c * kGroup + 4 * lane, left_of(c), 1.0f, w);
+      of_columns(bias, c * kGroup + 4 * lane, left_of(c), 0.0f, b);
+    }
+  };
 #pragma unroll
-  for (int c = 0; c < kHeld; ++c) {
-    of_columns(a.weight, c * kGroup + 4 * lane, left_of(c), 1.0f, w[c]);
-    of_columns(a.bias, c * kGroup + 4 * lane, left_of(c), 0.0f, b[c]);
-  }
+  for (int c = 0; c < kHeld; ++c) weights(c, w[c], b[c]);
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int64_t row = first + r;
@@ -129,21 +146,19 @@ __global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 3 : 2) warp_kernel(con
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) squares = add_squares(x[c], both(-mean), left_of(c), squares);
     const float rstd = rsqrtf(fmaf(warp_sum(sum_of(squares)), a.per_column, a.eps));
-    if (lane == 0 && a.mean != nullptr) {
+    if (KEEP && lane == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
+    T* const y = (T*)a.y + row * a.d + 4 * lane;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       if constexpr (ROWS > 1) {
-        finish<T, ACCESS>(a, row, c, left_of(c), x[c], mean, rstd, w[c], b[c]);
+        finish<T, ACCESS, KEEP>(a, y + c * kGroup, row, c, left_of(c), x[c], mean, rstd, w[c], b[c]);
       } else {  // the next chunk's weights are on the way meanwhile
         f32x2 w_next[2], b_next[2];
-        if (c + 1 < CHUNKS) {
-          of_columns(a.weight, (c + 1) * kGroup + 4 * lane, left_of(c + 1), 1.0f, w_next);
-          of_columns(a.bias, (c + 1) * kGroup + 4 * lane, left_of(c + 1), 0.0f, b_next);
-        }
-        finish<T, ACCESS>(a, row, c, left_of(c), x[c], mean, rstd, w[0], b[0]);
+        if (c + 1 < CHUNKS) weights(c + 1, w_next, b_next);
+        finish<T, ACCESS, KEEP>(a, y + c * kGroup, row, c, left_of(c), x[c], mean, rstd, w[0], b[0]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           w[0][h] = w_next[h];
@@ -159,37 +174,30 @@ __device__ __forceinline__ float block_sum(float v, float* of_warp) {
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.0f;
+  v = of_warp[threadIdx.x & (THREADS / 32 - 1)];
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) v += of_warp[w];
+  for (int o = THREADS / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
 // A CTA has every gridDim.x-th row: chunks warp, warp + THREADS / 32, ... are a warp's, all of which it keeps.
-template <typename T, int ACCESS, int THREADS, int KEPT, bool EVEN>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __grid_constant__ Args a) {
+template <typename T, int ACCESS, int THREADS, int KEPT, bool EVEN, bool KEEP>
+__global__ void __launch_bounds__(THREADS, (KEEP ? 640 : 768) / THREADS) block_kernel(const __grid_constant__ Args a) {
   constexpr int kWarps = THREADS / 32;
   __shared__ float of_warp[2][kWarps];
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Four<T, ACCESS> next[KEPT];
+  const int own = warp * kGroup + 4 * lane;  // this lane's first columns
   const auto fetch = [&](int64_t row) {
+    const T* const x = (const T*)a.x + row * a.ldx + own;
+    const int left = row < a.m ? a.d - own : 0;
 #pragma unroll
-    for (int k = 0; k < KEPT; ++k) {
-      const int col = (warp + k * kWarps) * kGroup + 4 * lane;
-      next[k].load((const T*)a.x + row * a.ldx + col, row < a.m ? a.d - col : 0);
-    }
+    for (int k = 0; k < KEPT; ++k) next[k].load(x + k * (kWarps * kGroup), left - k * (kWarps * kGroup));
   };
   const int mine = max(0, min(KEPT, ((a.d + kGroup - 1) / kGroup - warp + kWarps - 1) / kWarps));  // chunks that there are
   fetch(blockIdx.x);
-  f32x2 w[KEPT][2], b[KEPT][2];
-#pragma unroll
-  for (int k = 0; k < KEPT; ++k) {
-    const int col = (warp + k * kWarps) * kGroup + 4 * lane;
-    of_columns(a.weight, col, a.d - col, 1.0f, w[k]);
-    of_columns(a.bias, col, a.d - col, 0.0f, b[k]);
-  }
   for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
     f32x2 x[KEPT][2], sum = 0ull, squares = 0ull;
 #pragma unroll
@@ -204,20 +212,31 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) block_kernel(const __g
     for (int k = 0; k < KEPT; ++k)
       if (k < mine) squares = add_squares(x[k], both(-mean), EVEN ? 4 : a.d - (warp + k * kWarps) * kGroup - 4 * lane, squares);
     const float rstd = rsqrtf(fmaf(block_sum<THREADS>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
-    if (threadIdx.x == 0 && a.mean != nullptr) {
+    if (KEEP && threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
+    T* const y = (T*)a.y + row * a.d + own;
 #pragma unroll
     for (int k = 0; k < KEPT; ++k) {
       if (k >= mine) break;
-      finish<T, ACCESS>(a, row, warp + k * kWarps, EVEN ? 4 : a.d - (warp + k * kWarps) * kGroup - 4 * lane, x[k], mean, rstd, w[k], b[k]);
+      constexpr int kStep = kWarps * kGroup;
+      const int left = EVEN ? 4 : a.d - own - k * kStep;
+      f32x2 w[2], b[2];
+      if constexpr (EVEN) {
+        of_columns(a.weight != nullptr ? a.weight + own + k * kStep : nullptr, 1.0f, w);
+        of_columns(a.bias != nullptr ? a.bias + own + k * kStep : nullptr, 0.0f, b);
+      } else {
+        of_columns(a.weight, own + k * kStep, left, 1.0f, w);
+        of_columns(a.bias, own + k * kStep, left, 0.0f, b);
+      }
+      finish<T, ACCESS, KEEP>(a, y + k * kStep, row, warp + k * kWarps, left, x[k], mean, rstd, w, b);
     }
   }
 }
 
 // Longer rows, one a CTA, read three times.
-template <typename T, int ACCESS>
+template <typename T, int ACCESS, bool KEEP>
 __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args a) {
   constexpr int kWarps = 16;
   __shared__ float of_warp[2][kWarps];
@@ -241,7 +260,7 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
   const float mean = block_sum<512>(sum_of(sum), of_warp[0]) * a.per_column;
   each([&](int, int col, const f32x2 (&x)[2]) { squares = add_squares(x, both(-mean), a.d - col, squares); });
   const float rstd = rsqrtf(fmaf(block_sum<512>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
-  if (threadIdx.x == 0 && a.mean != nullptr) {
+  if (KEEP && threadIdx.x == 0 && a.mean != nullptr) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
   }
@@ -249,44 +268,45 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
     f32x2 w[2], b[2];
     of_columns(a.weight, col, a.d - col, 1.0f, w);
     of_columns(a.bias, col, a.d - col, 0.0f, b);
-    finish<T, ACCESS>(a, row, c, a.d - col, x, mean, rstd, w, b);
+    finish<T, ACCESS, KEEP>(a, (T*)a.y + row * a.d + col, row, c, a.d - col, x, mean, rstd, w, b);
   });
 }
 
-template <typename T, int ACCESS, int CHUNKS, int ROWS, bool EVEN>
+template <typename T, int ACCESS, int CHUNKS, int ROWS, bool EVEN, bool KEEP>
 static void by_warps(const Args& a, cudaStream_t st) {
-  launch_dependent(warp_kernel<T, ACCESS, CHUNKS, ROWS, EVEN>, dim3((unsigned)ceil_div(a.m, kThreads / 32 * ROWS)), kThreads, 0, st, a);
+  launch_dependent(warp_kernel<T, ACCESS, CHUNKS, ROWS, EVEN, KEEP>, dim3((unsigned)ceil_div(a.m, kThreads / 32 * ROWS)), kThreads, 0, st, a);
 }
-template <typename T, int ACCESS, int THREADS, int KEPT, bool EVEN>
+template <typename T, int ACCESS, int THREADS, int KEPT, bool EVEN, bool KEEP>
 static void by_ctas(const Args& a, int resident, cudaStream_t st) {
   const int64_t most = (int64_t)resident * kSmCount;
-  launch_dependent(block_kernel<T, ACCESS, THREADS, KEPT, EVEN>, dim3((unsigned)(a.m < most ? a.m : most)), THREADS, 0, st, a);
+  launch_dependent(block_kernel<T, ACCESS, THREADS, KEPT, EVEN, KEEP>, dim3((unsigned)(a.m < most ? a.m : most)), THREADS, 0, st, a);
 }
 
-template <typename T, int ACCESS, bool EVEN>
+template <typename T, int ACCESS, bool EVEN, bool KEEP>
 static void by_size(const Args& a, cudaStream_t st) {
   switch ((a.d + kGroup - 1) / kGroup) {
-    case 1: return by_warps<T, ACCESS, 1, 4, EVEN>(a, st);
-    case 2: return by_warps<T, ACCESS, 2, 2, EVEN>(a, st);
-    case 3: return by_warps<T, ACCESS, 3, 1, EVEN>(a, st);
-    case 4: return by_warps<T, ACCESS, 4, 1, EVEN>(a, st);
-    case 5: return by_warps<T, ACCESS, 5, 1, EVEN>(a, st);
-    case 6: return by_warps<T, ACCESS, 6, 1, EVEN>(a, st);
-    case 7: return by_warps<T, ACCESS, 7, 1, EVEN>(a, st);
-    case 8: return by_warps<T, ACCESS, 8, 1, EVEN>(a, st);
+    case 1: return by_warps<T, ACCESS, 1, 4, EVEN, KEEP>(a, st);
+    case 2: return by_warps<T, ACCESS, 2, 2, EVEN, KEEP>(a, st);
+    case 3: return by_warps<T, ACCESS, 3, 1, EVEN, KEEP>(a, st);
+    case 4: return by_warps<T, ACCESS, 4, 1, EVEN, KEEP>(a, st);
+    case 5: return by_warps<T, ACCESS, 5, 1, EVEN, KEEP>(a, st);
+    case 6: return by_warps<T, ACCESS, 6, 1, EVEN, KEEP>(a, st);
+    case 7: return by_warps<T, ACCESS, 7, 1, EVEN, KEEP>(a, st);
+    case 8: return by_warps<T, ACCESS, 8, 1, EVEN, KEEP>(a, st);
     default: break;
   }
-  if (a.d <= 16 * kGroup) by_ctas<T, ACCESS, 256, 2, EVEN>(a, 4, st);
-  else if (a.d <= 32 * kGroup) by_ctas<T, ACCESS, 256, 4, EVEN>(a, 2, st);
-  else if (a.d <= 64 * kGroup) by_ctas<T, ACCESS, 512, 4, EVEN>(a, 1, st);
-  else launch_dependent(long_kernel<T, ACCESS>, dim3((unsigned)a.m), 512, 0, st, a);
+  if (a.d <= 16 * kGroup) by_ctas<T, ACCESS, 128, 4, EVEN, KEEP>(a, KEEP ? 5 : 6, st);
+  else if (a.d <= 32 * kGroup) by_ctas<T, ACCESS, 128, 8, EVEN, KEEP>(a, KEEP ? 5 : 6, st);
+  else if (a.d <= 64 * kGroup) by_ctas<T, ACCESS, 256, 8, EVEN, KEEP>(a, KEEP ? 2 : 3, st);
+  else launch_dependent(long_kernel<T, ACCESS, KEEP>, dim3((unsigned)a.m), 512, 0, st, a);
 }
 template <typename T, int ACCESS>
 static void run(const Args& a, cudaStream_t st) {
+  const bool keep = a.mean != nullptr || a.active != nullptr || a.codes.codes != nullptr;
   if constexpr (ACCESS == 4 * (int)sizeof(T)) {
-    if (a.d % kGroup == 0) return by_size<T, ACCESS, true>(a, st);
+    if (a.d % kGroup == 0 && aligned(a.weight, 16) && aligned(a.bias, 16)) return keep ? by_size<T, ACCESS, true, true>(a, st) : by_size<T, ACCESS, true, false>(a, st);
   }
-  by_size<T, ACCESS, false>(a, st);
+  keep ? by_size<T, ACCESS, false, true>(a, st) : by_size<T, ACCESS, false, false>(a, st);
 }
 
 }  // namespace ln
