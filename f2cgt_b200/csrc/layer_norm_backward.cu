@@ -28,6 +28,7 @@ struct Back {
   ckpt::Codes codes;
   int64_t ldx, m;
   int d;
+  float per_column;            // 1 / d
   const float *mean, *rstd;
   const uint8_t* active;       // null: no ReLU
   const float* weight;         // null: 1
@@ -44,17 +45,33 @@ struct Columns {
   ckpt::Scale s;
   uint32_t open;
 
-  __device__ __forceinline__ void load(const Back& a, int64_t row, int chunk, bool here) {
-    const int lane = threadIdx.x & 31, col = chunk * kGroup + 4 * lane, left = here ? a.d - col : 0;
-    dy.load((const T*)a.dy + row * a.ldy + col, left);
-    if constexpr (CODES) {
-      x = ldg_nc_u32_if(a.codes.codes + row * a.codes.ld + col, left > 0);
-      s = here && chunk < a.codes.groups ? ckpt::load_scale(a.codes.scales + 2 * (row * a.codes.groups + chunk)) : ckpt::Scale{0.0f, 0.0f};
-    } else {
-      x.load((const T*)a.x + row * a.ldx + col, left);
+  // `at`: the row, from this lane's columns of its first chunk on; this chunk's are `step` columns further, of which `left` exist (none: nothing is loaded)
+  struct Row {
+    const T *dy, *x;
+    const uint8_t *codes, *active;
+    const float* scales;
+    __device__ __forceinline__ Row(const Back& a, int64_t row, int member) {
+      const int own = member * kGroup + 4 * (threadIdx.x & 31);
+      dy = (const T*)a.dy + row * a.ldy + own;
+      if constexpr (CODES) {
+        codes = a.codes.codes + row * a.codes.ld + own;
+        scales = a.codes.scales + 2 * (row * a.codes.groups + member);
+      } else {
+        x = (const T*)a.x + row * a.ldx + own;
+      }
+      active = a.active + row * ((a.d + 7) >> 3) + (own >> 3);
     }
-    open = 15u;
-    if (a.active != nullptr) open = left > 0 ? (uint32_t)__ldg(a.active + row * ((a.d + 7) >> 3) + (col >> 3)) >> (4 * (lane & 1)) : 0u;
+  };
+  __device__ __forceinline__ void load(const Row& at, int step, int left, bool masked) {
+    dy.load(at.dy + step, left);
+    if constexpr (CODES) {
+      x = ldg_nc_u32_if(at.codes + step, left > 0);
+      const uint2 v = ckpt::ld_u64_if(at.scales + 2 * (step / kGroup), left > 0);
+      s = ckpt::Scale{__uint_as_float(v.x), __uint_as_float(v.y)};
+    } else {
+      x.load(at.x + step, left);
+    }
+    open = masked && left > 0 ? (uint32_t)__ldg(at.active + (step >> 3)) >> (4 * (threadIdx.x & 1)) : 15u;
   }
   // g and h; columns that do not exist have no g (what they have for h meets nothing else)
   __device__ __forceinline__ void get(bool masked, float mean, float rstd, f32x2 (&g)[2], f32x2 (&h)[2]) const {
@@ -89,7 +106,7 @@ __device__ __forceinline__ void warp_sum2(float& u, float& v) {
 
 // WARPS warps have a row of up to WARPS * CHUNKS * 128 columns: one warp, two, or all of a CTA.
 template <typename T, int ACCESS, bool CODES, int WARPS, int CHUNKS, int THREADS>
-__global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant__ Back a) {
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : CHUNKS == 1 ? 3 : 2) backward_kernel(const __grid_constant__ Back a) {
   constexpr int kRows = THREADS / 32 / WARPS;  // of a CTA at a time
   constexpr bool kAlone = WARPS == 1;
   constexpr int kColumns = WARPS * CHUNKS * kGroup;
@@ -102,14 +119,15 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
   int64_t row = (int64_t)blockIdx.x * kRows + warp / WARPS;
   Columns<T, ACCESS, CODES> next[CHUNKS];
   float next_mean = 0.0f, next_rstd = 0.0f;
+  const bool masked = a.active != nullptr;
   const auto fetch = [&](int64_t r) {
-    const bool here = r < a.m;
+    if (r >= a.m) return;
+    const typename Columns<T, ACCESS, CODES>::Row at(a, r, member);
+    const int left = a.d - member * kGroup - 4 * lane;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) next[c].load(a, r, member + c * WARPS, here);
-    if (here) {
-      next_mean = __ldg(a.mean + r);
-      next_rstd = __ldg(a.rstd + r);
-    }
+    for (int c = 0; c < CHUNKS; ++c) next[c].load(at, c * WARPS * kGroup, left - c * WARPS * kGroup, masked);
+    next_mean = __ldg(a.mean + r);
+    next_rstd = __ldg(a.rstd + r);
   };
   fetch(row);
   constexpr bool kHeld = WARPS < 16;  // (the widest rows' weights do not fit beside their sums: they are read again for every row)
@@ -128,28 +146,25 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
 #pragma unroll
     for (int q = 0; q < 2; ++q) dw[c][q] = db[c][q] = 0ull;
   }
-  const float n = (float)a.d;
-  const bool masked = a.active != nullptr;
   // (all warps of a row leave together)
   for (int turn = 0; row < a.m; row += stride, turn ^= 1) {
-    const float mean = next_mean, rstd = next_rstd;
-    Columns<T, ACCESS, CODES> now[CHUNKS];
+    const float rstd = next_rstd;
+    f32x2 g[CHUNKS][2], h[CHUNKS][2];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) now[c] = next[c];
+    for (int c = 0; c < CHUNKS; ++c) next[c].get(masked, next_mean, rstd, g[c], h[c]);
     fetch(row + stride);
     f32x2 us = 0ull, vs = 0ull;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      f32x2 g[2], h[2], w[2];
-      now[c].get(masked, mean, rstd, g, h);
+      f32x2 w[2];
       weights(c, w);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        dw[c][q] = fma2(g[q], h[q], dw[c][q]);
-        db[c][q] = plus2(db[c][q], g[q]);
-        const f32x2 gw = mul2(g[q], w[q]);
-        us = plus2(us, gw);
-        vs = fma2(gw, h[q], vs);
+        dw[c][q] = fma2(g[c][q], h[c][q], dw[c][q]);
+        db[c][q] = plus2(db[c][q], g[c][q]);
+        g[c][q] = mul2(g[c][q], w[q]);
+        us = plus2(us, g[c][q]);
+        vs = fma2(g[c][q], h[c][q], vs);
       }
     }
     float u = lo32(us) + hi32(us), v = lo32(vs) + hi32(vs);
@@ -169,19 +184,17 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const __grid_constant
         v += sums[turn][1][own + q];
       }
     }
-    u /= n;
-    v /= n;
+    u *= a.per_column;
+    v *= a.per_column;
+    T* const dx = (T*)a.dx + row * a.d + member * kGroup + 4 * lane;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const int col = (member + c * WARPS) * kGroup + 4 * lane, left = a.d - col;
-      f32x2 g[2], h[2], w[2];
-      now[c].get(masked, mean, rstd, g, h);
-      weights(c, w);
+      constexpr int kStep = WARPS * kGroup;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) g[q] = mul2(both(rstd), fma2(h[q], both(-v), fma2(g[q], w[q], both(-u))));
+      for (int q = 0; q < 2; ++q) g[c][q] = mul2(both(rstd), fma2(h[c][q], both(-v), plus2(g[c][q], both(-u))));
       Four<T, ACCESS> out;
-      out.set(g);
-      out.store((T*)a.dx + row * a.d + col, left);
+      out.set(g[c]);
+      out.store(dx + c * kStep, a.d - member * kGroup - 4 * lane - c * kStep);
     }
   }
   float* const part = a.parts + (int64_t)blockIdx.x * 2 * a.d;
@@ -225,15 +238,16 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Back 
   release_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.d + kGroup - 1) / kGroup;
   const int64_t row = blockIdx.x;
-  const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row), n = (float)a.d;
+  const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row);
+  const typename Columns<T, ACCESS, CODES>::Row at(a, row, 0);
   float u = 0.0f, v = 0.0f;
   f32x2 us = 0ull, vs = 0ull;
   for (int pass = 0; pass < 2; ++pass) {
     for (int c = warp; c < chunks; c += kWarps) {
       Columns<T, ACCESS, CODES> now;
-      now.load(a, row, c, true);
       f32x2 g[2], h[2], w[2];
       const int col = c * kGroup + 4 * lane, left = a.d - col;
+      now.load(at, c * kGroup, left, a.active != nullptr);
       now.get(a.active != nullptr, mean, rstd, g, h);
       weights_of(a, c, w);
       if (pass == 0) {
@@ -266,8 +280,8 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Back 
         u += sums[0][q];
         v += sums[1][q];
       }
-      u /= n;
-      v /= n;
+      u *= a.per_column;
+      v *= a.per_column;
     }
   }
 }
@@ -282,7 +296,7 @@ __global__ void __launch_bounds__(256) columns_kernel(const __grid_constant__ Ba
   f32x2 dw[2] = {}, db[2] = {};
   for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < a.m; row += (int64_t)gridDim.x * 8) {
     Columns<T, ACCESS, CODES> now;
-    now.load(a, row, blockIdx.y, true);
+    now.load(typename Columns<T, ACCESS, CODES>::Row(a, row, blockIdx.y), 0, a.d - (int)blockIdx.y * kGroup - 4 * lane, a.active != nullptr);
     f32x2 g[2], h[2];
     now.get(a.active != nullptr, __ldg(a.mean + row), __ldg(a.rstd + row), g, h);
 #pragma unroll
@@ -339,11 +353,11 @@ static Deal deal(int64_t m, int64_t d) {
   Deal r;
   if (d <= kGroup) r = {1, 1, 256, 3};
   else if (d <= 2 * kGroup) r = {1, 2, 256, 2};
-  else if (d <= 4 * kGroup) r = {1, 4, 256, 1};
+  else if (d <= 4 * kGroup) r = {1, 4, 256, 2};
   else if (d <= 6 * kGroup) r = {2, 3, 256, 2};
-  else if (d <= 8 * kGroup) r = {2, 4, 256, 1};
+  else if (d <= 8 * kGroup) r = {2, 4, 256, 2};
   else if (d <= 16 * kGroup) r = {8, 2, 256, 2};
-  else if (d <= 32 * kGroup) r = {8, 4, 256, 1};
+  else if (d <= 32 * kGroup) r = {8, 4, 256, 2};
   else if (d <= 64 * kGroup) r = {16, 4, 512, 1};
   else r = {0, 1, 256, 1};
   const int rows = r.warps == 0 ? 8 : r.threads / 32 / r.warps;
@@ -403,7 +417,7 @@ extern "C" int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, c
   cudaStream_t st = (cudaStream_t)stream;
   const ln::Deal how = ln::deal(m, d);
   if (m > 0) {
-    const ln::Back a{dy, ldy, x, ckpt::Codes{const_cast<uint8_t*>(codes), ldq, const_cast<float*>(scales), ceil_div(d, ckpt::kGroup)}, ldx, m, (int)d, mean, rstd, active,
+    const ln::Back a{dy, ldy, x, ckpt::Codes{const_cast<uint8_t*>(codes), ldq, const_cast<float*>(scales), ceil_div(d, ckpt::kGroup)}, ldx, m, (int)d, (float)(1.0 / (double)d), mean, rstd, active,
                      weight, dx, (float*)workspace};
     const int item = dtype_size(dtype);
     int access = ckpt::access_of(dy, ldy, m, d, item), other = ckpt::access_of(dx, d, m, d, item);
