@@ -1,7 +1,7 @@
 // Activations to 8 bits and back (f2c_checkpoint_int8, f2c_checkpoint_values).  Bound by reading and writing the rows.
 //
 // A warp has a group - 128 columns of a row - four columns a lane: its extremes are one reduction instruction each, its codes 128 bytes
-// side by side.  Groups are taken kAhead at a time, all loads before the first use.
+// side by side.  Groups are taken kAhead at a time, all loads before the first use, their steps and reciprocals in a lane each.
 #include "checkpoint.cuh"
 
 namespace f2c {
@@ -14,7 +14,8 @@ struct Place { int64_t row; int group; };
 __device__ __forceinline__ Place place_of(int64_t i, uint32_t groups) { return Place{(int64_t)((uint32_t)i / groups), (int)((uint32_t)i % groups)}; }
 __device__ __forceinline__ Place behind(Place p, int groups) { return p.group + 1 < groups ? Place{p.row, p.group + 1} : Place{p.row + 1, 0}; }
 
-template <typename T, int ACCESS>
+// EVEN: all groups have 128 columns
+template <typename T, int ACCESS, bool EVEN>
 __global__ void __launch_bounds__(kThreads) encode_kernel(const T* __restrict__ x, int64_t ldx, int64_t m, int d, Codes out) {
   dependency_wait();
   release_dependents();
@@ -27,7 +28,7 @@ __global__ void __launch_bounds__(kThreads) encode_kernel(const T* __restrict__ 
   for (int a = 0; a < kAhead; ++a) {
     if (a > 0) at[a] = behind(at[a - 1], (int)out.groups);
     const int col = at[a].group * kGroup + 4 * lane;
-    v[a].load(x + at[a].row * ldx + col, first + a < total ? d - col : 0);
+    v[a].load(x + at[a].row * ldx + col, first + a < total ? (EVEN ? 4 : d - col) : 0);
   }
   Scale mine{0.0f, 0.0f};  // lane a: of group a
 #pragma unroll
@@ -37,9 +38,9 @@ __global__ void __launch_bounds__(kThreads) encode_kernel(const T* __restrict__ 
     v[a].get(f);
     Scale s;
     const int col = at[a].group * kGroup + 4 * lane;
-    const uint32_t codes = encode(f, d - col, s);
+    const uint32_t codes = encode(f, EVEN ? 4 : d - col, s);
     // rows have room for whole 16 bytes: a word that starts in front of the row's end is there
-    if (col < d) *reinterpret_cast<uint32_t*>(out.codes + at[a].row * out.ld + col) = codes;
+    if (EVEN || col < d) *reinterpret_cast<uint32_t*>(out.codes + at[a].row * out.ld + col) = codes;
     if (lane == a) mine = s;
   }
   if (lane < kAhead && first + lane < total) store_scale(out.scales + 2 * (first + lane), mine);
@@ -94,7 +95,13 @@ int check_codes(const char* op, const uint8_t* codes, int64_t ldq, const float* 
 template <typename T, int ACCESS>
 static void run_encode(const void* x, int64_t ldx, int64_t m, int64_t d, const Codes& out, cudaStream_t st) {
   const dim3 grid((unsigned)ceil_div(m * out.groups, kWarps * kAhead));
-  launch_dependent(encode_kernel<T, ACCESS>, grid, kThreads, 0, st, (const T*)x, ldx, m, (int)d, out);
+  if constexpr (ACCESS == 4 * (int)sizeof(T)) {
+    if (d % kGroup == 0) {
+      launch_dependent(encode_kernel<T, ACCESS, true>, grid, kThreads, 0, st, (const T*)x, ldx, m, (int)d, out);
+      return;
+    }
+  }
+  launch_dependent(encode_kernel<T, ACCESS, false>, grid, kThreads, 0, st, (const T*)x, ldx, m, (int)d, out);
 }
 template <typename T, int ACCESS>
 static void run_values(const Codes& in, void* out, int64_t ldo, int64_t m, int64_t d, cudaStream_t st) {

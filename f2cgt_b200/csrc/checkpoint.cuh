@@ -160,38 +160,52 @@ static __device__ __noinline__ uint32_t encode_by_division(float x0, float x1, f
   return codes;
 }
 
-// Codes of a group, four columns a lane of which `left` exist (the others' codes are 0); by whole warps.  The quotients are what division gives: the
-// product with the correctly rounded reciprocal, and two corrections with exact remainders (Markstein).  (Corrected only where the product lay near a tie: rows
-// of 16-bit numbers, whose quotients are ties as often as not somewhere in a group, took twice the time.)  2^23 + 2^22 added to a number below 2^22 rounds it to
-// even and leaves it in the last bits.
-__device__ __forceinline__ uint32_t encode(const f32x2 (&given)[2], int left, Scale& s) {
-  f32x2 x[2] = {given[0], given[1]};
+// A group's extremes, four columns a lane of which `left` exist: by whole warps, all lanes get them.  Columns that are not there get the first one's value.
+struct Extremes { float low, high; };
+__device__ __forceinline__ Extremes extremes_of(f32x2 (&x)[2], int left) {
   float low = min_nan(min_nan(lo32(x[0]), hi32(x[0]), lo32(x[1])), hi32(x[1])), high = max_nan(max_nan(lo32(x[0]), hi32(x[0]), lo32(x[1])), hi32(x[1]));
-  if (left < 4) {  // the columns that are not there have the first one's value; without any, nobody's extreme
+  if (left < 4) {
     const float first = lo32(x[0]);
     const float second = left > 1 ? hi32(x[0]) : first, third = left > 2 ? lo32(x[1]) : first;
     x[0] = pair_of(first, second);
     x[1] = pair_of(third, first);
-    low = left > 0 ? min_nan(first, second, third) : __int_as_float(0x7f800000);
+    low = left > 0 ? min_nan(first, second, third) : __int_as_float(0x7f800000);  // (without any: nobody's extreme)
     high = left > 0 ? max_nan(first, second, third) : __int_as_float(0xff800000);
   }
-  low = warp_min_nan(low);
-  high = warp_max_nan(high);
-  const float range = high - low;
-  s.low = low;
-  // range / 255 by two corrections with exact remainders; the ordinary division where they would not be exact
-  s.step = div_exact_fast(range, 255.0f, 1.0f / 255.0f);
-  const bool plain = range > 1e-25f && range < 1e30f;
-  if (!plain) {
-    if (!(range <= 3.402823466e38f)) {  // infinite, or no number
-      s.step = s.low = __int_as_float(0x7fffffff);
-      return 0u;
-    }
-    s.step = range / 255.0f;
-    if (s.step == 0.0f) return 0u;
-    return encode_by_division(lo32(x[0]), hi32(x[0]), lo32(x[1]), hi32(x[1]), low, s.step, left);
+  return Extremes{warp_min_nan(low), warp_max_nan(high)};
+}
+
+// Step and lowest value, the step's reciprocal, and whether the quotients are to be had with it (not where the range is so small or so large that remainders
+// would not be exact, or is none).
+struct Steps {
+  Scale s;
+  float by;
+  bool plain;
+};
+__device__ __forceinline__ Steps steps_of(Extremes e) {
+  Steps r;
+  const float range = e.high - e.low;
+  r.s.low = e.low;
+  r.s.step = div_exact_fast(range, 255.0f, 1.0f / 255.0f);  // two corrections with exact remainders
+  r.by = __frcp_rn(r.s.step);
+  r.plain = range > 1e-25f && range < 1e30f;
+  if (!r.plain) {
+    const bool none = !(range <= 3.402823466e38f);  // infinite, or no number
+    r.s.step = none ? __int_as_float(0x7fffffff) : range / 255.0f;
+    if (none) r.s.low = r.s.step;
   }
-  const f32x2 by = both(__frcp_rn(s.step)), less = both(-low), minus = both(-s.step), magic = both(12582912.0f);
+  return r;
+}
+
+// The codes of a lane's four columns (0 for those that are not there).  The quotients are what division gives: the product with the correctly rounded reciprocal, and two
+// corrections with exact remainders (Markstein).  (Corrected only where the product lay near a tie: rows of 16-bit numbers, whose quotients are ties as often as
+// not somewhere in a group, took twice the time.)  2^23 + 2^22 added to a number below 2^22 rounds it to even and leaves it in the last bits.
+__device__ __forceinline__ uint32_t codes_of(const f32x2 (&x)[2], int left, Scale s, float reciprocal, bool plain) {
+  if (!plain) {
+    if (!(s.step > 0.0f)) return 0u;
+    return encode_by_division(lo32(x[0]), hi32(x[0]), lo32(x[1]), hi32(x[1]), s.low, s.step, left);
+  }
+  const f32x2 by = both(reciprocal), less = both(-s.low), minus = both(-s.step), magic = both(12582912.0f);
   f32x2 m[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -203,6 +217,14 @@ __device__ __forceinline__ uint32_t encode(const f32x2 (&given)[2], int left, Sc
   }
   const uint32_t codes = __byte_perm(__byte_perm((uint32_t)m[0], (uint32_t)(m[0] >> 32), 0x0040), __byte_perm((uint32_t)m[1], (uint32_t)(m[1] >> 32), 0x0040), 0x5410);
   return left >= 4 ? codes : left <= 0 ? 0u : codes & ((1u << (8 * left)) - 1u);
+}
+
+// Codes and scale of a group; by whole warps.
+__device__ __forceinline__ uint32_t encode(const f32x2 (&given)[2], int left, Scale& s) {
+  f32x2 x[2] = {given[0], given[1]};
+  const Steps r = steps_of(extremes_of(x, left));
+  s = r.s;
+  return codes_of(x, left, r.s, r.by, r.plain);
 }
 
 // The codes as numbers: 2^23 + q, less 2^23.

@@ -144,7 +144,7 @@ PyObject* checkpoint_weight_grad(PyObject*, PyObject* const* a, Py_ssize_t n) { 
 }
 
 // x, weight, bias, eps, relu, keep (0: nothing, 1: what goes with the rows, 2: and the rows in 8 bits)
-// -> y, mean, rstd, active, codes, scales (None: not wanted)
+// -> y, or y, mean, rstd, active, codes, scales (None: not wanted)
 PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     arguments("layer_norm", n, 6);
@@ -174,6 +174,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (keep > 1) c.codes = c.codes.narrow(1, 0, d);
       return rc;
     }));
+    if (keep == 0) return THPVariable_Wrap(std::move(y));
     return tuple_of(std::move(y), std::move(mean), std::move(rstd), std::move(active), std::move(c.codes), std::move(c.scales));
   });
 }

@@ -400,7 +400,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over every row of ``x`` [rows, cols] (float32 / float16 / bfloat16), then ReLU if asked for;
     ``weight`` and ``bias`` float32 [cols] or None.  Statistics are single precision, the result is rounded once.  It has no gradient by itself:
     ``layer_norm_train`` keeps what ``layer_norm_backward`` needs, ``sage.LayerNorm`` is the module over them."""
-    return _native.layer_norm(x, weight, bias, eps, relu, 0)[0]
+    return _native.layer_norm(x, weight, bias, eps, relu, 0)
 
 
 def layer_norm_train(x, weight=None, bias=None, eps=1e-5, relu=False, int8=False):
