@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
   const uint32_t behind = start + n < s.m ? s.key[start + n] : s.rows;
   const uint32_t first = __ballot_sync(0xffffffffu, lane < n && (lane == 0 ? start == 0 || before != key : above != key));
   const int kept = __popc(__ballot_sync(0xffffffffu, key < s.rows));  // the places of no row are behind all others
-  int64_t number = 0;  // of the next segment that begins here
+  uint32_t row = key;  // of the result, for this lane's place (not where its segment begins in another stretch)
   if (s.looked_up != nullptr) {
     uint32_t tiles_before = 0u, all = 0u;
     const int tile = (int)(start / kTile);
@@ -342,8 +342,11 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
       if (t < tile) tiles_before += v;
     }
     all = __reduce_add_sync(0xffffffffu, all);
-    number = (int64_t)__reduce_add_sync(0xffffffffu, tiles_before) + s.in_tile[c];
-    if (c == 0 && blockIdx.y == 0 && lane == 0) *s.count = all;
+    row = __reduce_add_sync(0xffffffffu, tiles_before) + s.in_tile[c] + __popc(first & (0xffffffffu >> (31 - lane))) - 1u;
+    if (blockIdx.y == 0) {
+      if (c == 0 && lane == 0) *s.count = all;
+      if (key < s.rows && ((first >> lane) & 1u)) s.looked_up[row] = (int64_t)key;
+    }
     // rows behind the last segment's are zero
     for (int64_t r = max(start, (int64_t)all); r < start + n; ++r) {
       Four<T, ACCESS> zero;
@@ -353,28 +356,16 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
     }
   }
   f32x2 acc[2] = {};
-  bool head = (first & 1u) == 0u, opened = false;
-  const auto flush = [&](int last) {  // the segment whose last place here is `last`
-    const uint32_t k = __shfl_sync(0xffffffffu, key, last);
-    const bool goes_on = last == n - 1 && behind == k;
-    const int64_t row = s.looked_up != nullptr ? (head ? 0 : number) : (int64_t)k;
-    if (!head && s.looked_up != nullptr) {
-      if (lane == 0 && blockIdx.y == 0) s.looked_up[row] = (int64_t)k;
-      ++number;
-    }
-    if (head || goes_on) {
-      float* const to = (head ? open.head : open.tail) + c * open.width + blockIdx.y * kGroup + 4 * lane;
-      *reinterpret_cast<ulonglong2*>(to) = make_ulonglong2(acc[0], acc[1]);
-      if (!head) {
-        opened = true;
-        if (lane == 0 && blockIdx.y == 0) open.row[c] = row;
-      }
+  bool head = (first & 1u) == 0u;
+  const auto write = [&](int last) {  // the segment whose last place here is `last`, and which ends there
+    if (head) {
+      *reinterpret_cast<ulonglong2*>(open.head + c * open.width + blockIdx.y * kGroup + 4 * lane) = make_ulonglong2(acc[0], acc[1]);
     } else {
       acc[0] = mul2(acc[0], both(scale));
       acc[1] = mul2(acc[1], both(scale));
       Four<T, ACCESS> v;
       v.set(acc);
-      v.store(out + row * d + col, left);
+      v.store(out + (int64_t)__shfl_sync(0xffffffffu, row, last) * d + col, left);
     }
     head = false;
     acc[0] = acc[1] = 0ull;
@@ -390,15 +381,19 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
     for (int q = 0; q < kRowsAhead; ++q) {
       const int t = t0 + q;
       if (t >= kept) break;
-      if (t > 0 && ((first >> t) & 1u)) flush(t - 1);
+      if (t > 0 && ((first >> t) & 1u)) write(t - 1);
       f32x2 f[2];
       v[q].get(f);
       acc[0] = plus2(acc[0], f[0]);
       acc[1] = plus2(acc[1], f[1]);
     }
   }
-  if (kept > 0) flush(kept - 1);
-  if (!opened && lane == 0 && blockIdx.y == 0) open.row[c] = -1;
+  // the last segment may go on in the next stretch
+  const bool opened = kept == n && !head && behind == __shfl_sync(0xffffffffu, key, n - 1);
+  const int64_t opened_row = opened ? (int64_t)__shfl_sync(0xffffffffu, row, n - 1) : -1;
+  if (opened) *reinterpret_cast<ulonglong2*>(open.tail + c * open.width + blockIdx.y * kGroup + 4 * lane) = make_ulonglong2(acc[0], acc[1]);
+  else if (kept > 0) write(kept - 1);
+  if (lane == 0 && blockIdx.y == 0) open.row[c] = opened_row;
 }
 
 // Puts the segments together that lie in several stretches: the tail of the one in which they begin, then heads.  A warp does a short one by
@@ -498,8 +493,9 @@ static Plan plan(int64_t m, int64_t rows, int64_t d) {
   Plan p{};
   p.m = m;
   p.d = d;
-  // Short stretches where there are few places: a stretch's rows are added one after the other.
-  p.stretch = m <= 16384 ? 8 : 32;
+  // Short stretches where there are few places: a stretch's rows are added one after the other.  Long ones where segments go over many of them: 59,000 places of
+  // 172 rows took 29.9 us in stretches of 32 and 32.0 of 16, 121,000 of 2.4 M rows 84.7 and 79.6.
+  p.stretch = m <= 16384 ? 8 : rows < m / 8 ? 32 : 16;
   p.tiles = (int)ceil_div(m, kTile);
   int bits = 1;
   while ((rows >> bits) != 0) ++bits;
