@@ -1,4 +1,5 @@
-// Activations to 8 bits and back (f2c_checkpoint_int8, f2c_checkpoint_values).  Bound by reading and writing the rows.
+// Activations to 8 bits and back (f2c_checkpoint_int8, f2c_checkpoint_values).  Back: bound by memory (8192 x 4096 bfloat16 19 us, 5.3 TB/s).  To 8 bits: by
+// instructions, some hundred a group of a warp for 4 values a lane (the same 34 us, 2.9 TB/s; 59,000 x 128 float32 10.9 us, 3.5 TB/s).
 //
 // A warp has a group - 128 columns of a row - four columns a lane: its extremes are one reduction instruction each, its codes 128 bytes
 // side by side.  Groups are taken kAhead at a time, all loads before the first use, their steps and reciprocals in a lane each.

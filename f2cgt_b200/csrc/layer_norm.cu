@@ -1,7 +1,7 @@
 // Layer norm of rows, forward (f2c_layer_norm): y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps), with or without
 // ReLU; for training also mean, rstd, the ReLU's bits, and the rows in 8 bits (checkpoint.cuh), all of it in the one pass.
 //
-// Bound by reading and writing the rows.  A row's values stay in registers between the mean, the squares of the differences from it (no
+// Bound by reading and writing the rows (16,384 x 4096 bfloat16: 52 us, 5.2 TB/s; 59,000 x 128 float32: 12 us, 5.0 TB/s).  A row's values stay in registers between the mean, the squares of the differences from it (no
 // cancellation of large means) and the result: a warp has rows up to 1024 columns long, several at a time where they are short so that enough loads are on
 // the way; a CTA of four warps (eight beyond 4096 columns) has longer ones, one after the other, the next one's loads on the way: five or six of them to an SM
 // (two of eight warps, their columns' weights in registers, waited more than they worked: 16,384 x 4096 bfloat16 64 us); rows beyond 8192 columns it reads

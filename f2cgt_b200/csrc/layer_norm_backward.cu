@@ -2,7 +2,8 @@
 //   dx = rstd (g w - mean(g w) - h mean(g w h)),   dweight = sum over rows of g h,   dbias = sum over rows of g.
 // x is the rows themselves or their 8-bit codes (checkpoint.cuh), decoded on the way.
 //
-// Bound by reading dy and x and writing dx.  A lane has the same columns of every row that its warp (or CTA) takes, so the sums over rows stay in
+// Bound by reading dy and x and writing dx (59,000 x 128 float32: 15 us, 6.0 TB/s; 37,237 x 256 from 8 bits with the ReLU's bits: 18 us, 4.8 TB/s; the launch
+// that joins the sums 2 to 4 us).  A lane has the same columns of every row that its warp (or CTA) takes, so the sums over rows stay in
 // registers; each CTA leaves one part of them, and a second launch adds the parts up in their order: no atomics, the same bits every time.
 // What a row needs is on the way while the row before it is worked on.
 #include <type_traits>

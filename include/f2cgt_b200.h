@@ -490,7 +490,7 @@ int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, const void* 
  * out [m, d] = scale * table[ids[i]], rounded once; table [rows, d] of `dtype` (F32, F16, BF16), row stride ld, ids [m] int32 or int64.  An id outside
  * [0, rows) - a -1 that pads a batch - is a row of zeros and has no gradient. */
 int f2c_embedding(const void* table, int64_t ld, int dtype, int64_t rows, int64_t d, const void* ids, int index_dtype, int64_t m, float scale, void* out, void* stream);
-/* The table's gradient: row r is scale times the sum of dy[i] over ids[i] = r.  Sums are single precision in an order that m alone decides, rounded
+/* The table's gradient: row r is scale times the sum of dy[i] over ids[i] = r.  Sums are single precision in an order that m and rows decide, rounded
  * once to `dtype`.  count NULL: grad [rows, d], zeros where nothing was looked up.  Otherwise only the rows that were: looked_up [m] (int64) their ids,
  * ascending, grad [m, d] their rows, count [1] (int64) how many; behind them looked_up is -1 and grad zero.
  * workspace: f2c_embedding_backward_workspace(m, rows, d) bytes, 256-byte aligned. */

@@ -207,3 +207,61 @@ def test_training_command(monkeypatch):
         tg.train(epochs=1, max_steps=1, embedding=64, optimizer="muon")
     with pytest.raises(ValueError):
         tg.train(epochs=1, max_steps=1, activations="int4")
+
+
+def test_a_step_in_a_graph():
+    """Forward and backward of the modules, captured and replayed on other inputs: what eager calls give on them."""
+    from f2cgt_b200 import sage
+    torch.manual_seed(0)
+    rows, norm = sage.NodeEmbedding(300, 96, scale=2.0, device="cuda"), sage.LayerNorm(96, relu=True, int8=True).cuda()
+    ids, dy = torch.randint(-1, 300, (5000,), device="cuda"), torch.randn(5000, 96, device="cuda")
+    parameters = [rows.weight, norm.weight, norm.bias]
+
+    def step():
+        return torch.autograd.grad(norm(rows(ids)), parameters, dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    ids.copy_(torch.randint(-1, 300, (5000,), device="cuda"))
+    dy.copy_(torch.randn(5000, 96, device="cuda"))
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+
+
+def test_other_streams_and_threads():
+    """The modules' backward pass runs on the stream of the forward one, and from several threads at once."""
+    import threading
+    from f2cgt_b200 import sage
+    cm, blocks = minibatch()
+    model = network(cm, activations="int8")
+    dy = torch.randn(300, 10, device="cuda")
+    want = torch.autograd.grad(model(blocks), list(model.parameters()), dy)
+    torch.cuda.synchronize()
+    found, errors = [None] * 3, []
+
+    def one(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    found[i] = torch.autograd.grad(model(blocks), list(model.parameters()), dy)
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=one, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for got in found:
+        for a, b, (name, _) in zip(got, want, model.named_parameters()):
+            # the aggregation's gradient adds with atomics: everything behind it may differ in its roundings
+            assert float((a - b).norm()) <= 1e-5 * float(b.norm()), name
