@@ -34,7 +34,8 @@ struct Back {
   const uint8_t* active;       // null: no ReLU
   const float* weight;         // null: 1
   void* dx;                    // [m, d]
-  float* parts;                // [CTAs][2][d]
+  float *dw, *db;              // a CTA's sums, those of the next one `part` further: [CTAs][2][d], or the results where there is one CTA
+  int64_t part;
 };
 
 // A lane's four columns of a row, on their way
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : CHUNKS == 1 ? 3 
       out.store(dx + c * kStep, a.d - member * kGroup - 4 * lane - c * kStep);
     }
   }
-  float* const part = a.parts + (int64_t)blockIdx.x * 2 * a.d;
+  float *const part_dw = a.dw + blockIdx.x * a.part, *const part_db = a.db + blockIdx.x * a.part;
   if constexpr (kRows > 1) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
@@ -214,7 +215,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : CHUNKS == 1 ? 3 
       float sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < kRows; ++q) sum += joined[from][q];
-      part[i] = sum;
+      if (i < a.d) part_dw[i] = sum;
+      else part_db[i - a.d] = sum;
     }
   } else {
 #pragma unroll
@@ -223,8 +225,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : CHUNKS == 1 ? 3 
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (col + e < a.d) {
-          part[col + e] = e & 1 ? hi32(dw[c][e / 2]) : lo32(dw[c][e / 2]);
-          part[a.d + col + e] = e & 1 ? hi32(db[c][e / 2]) : lo32(db[c][e / 2]);
+          part_dw[col + e] = e & 1 ? hi32(dw[c][e / 2]) : lo32(dw[c][e / 2]);
+          part_db[col + e] = e & 1 ? hi32(db[c][e / 2]) : lo32(db[c][e / 2]);
         }
     }
   }
@@ -316,19 +318,19 @@ __global__ void __launch_bounds__(256) columns_kernel(const __grid_constant__ Ba
   float sum = 0.0f;
 #pragma unroll
   for (int q = 0; q < 8; ++q) sum += joined[which * kGroup + c][q];
-  if (at < a.d) a.parts[((int64_t)blockIdx.x * 2 + which) * a.d + at] = sum;
+  if (at < a.d) (which ? a.db : a.dw)[blockIdx.x * a.part + at] = sum;
 }
 
-// The parts' sums: eight columns a CTA, four parts a warp at a time.  (32 columns a CTA and a part a warp took 8 us for 888 parts of 256.)
+// The parts' sums: eight columns a CTA, four parts a warp at a time, a warp for every 16 parts.  (32 columns a CTA and a part a warp took 8 us for 888 parts of 256.)
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ parts, int count, int d, float* __restrict__ dweight, float* __restrict__ dbias) {
   __shared__ float of[32][8];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = blockIdx.x * 8 + (lane & 7);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, at = blockIdx.x * 8 + (lane & 7);
   float sum = 0.0f;
   if (at < 2 * d) {
 #pragma unroll 8
-    for (int p = warp * 4 + (lane >> 3); p < count; p += 128) sum += parts[(int64_t)p * 2 * d + at];
+    for (int p = warp * 4 + (lane >> 3); p < count; p += 4 * warps) sum += parts[(int64_t)p * 2 * d + at];
   }
   sum += __shfl_xor_sync(0xffffffffu, sum, 8);
   sum += __shfl_xor_sync(0xffffffffu, sum, 16);
@@ -336,8 +338,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ pa
   __syncthreads();
   if (threadIdx.x >= 8) return;
   sum = 0.0f;
-#pragma unroll
-  for (int q = 0; q < 32; ++q) sum += of[q][lane];
+  for (int q = 0; q < warps; ++q) sum += of[q][lane];
   if (at < d) {
     if (dweight != nullptr) dweight[at] = sum;
   } else if (at < 2 * d && dbias != nullptr) {
@@ -417,9 +418,10 @@ extern "C" int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, c
               (long long)need);
   cudaStream_t st = (cudaStream_t)stream;
   const ln::Deal how = ln::deal(m, d);
+  const bool alone = m > 0 && how.ctas == 1 && dweight != nullptr && dbias != nullptr;  // nothing to join
   if (m > 0) {
     const ln::Back a{dy, ldy, x, ckpt::Codes{const_cast<uint8_t*>(codes), ldq, const_cast<float*>(scales), ceil_div(d, ckpt::kGroup)}, ldx, m, (int)d, (float)(1.0 / (double)d), mean, rstd, active,
-                     weight, dx, (float*)workspace};
+                     weight, dx, alone ? dweight : (float*)workspace, alone ? dbias : (float*)workspace + d, 2 * d};
     const int item = dtype_size(dtype);
     int access = ckpt::access_of(dy, ldy, m, d, item), other = ckpt::access_of(dx, d, m, d, item);
     access = other < access ? other : access;
@@ -430,6 +432,8 @@ extern "C" int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, c
     F2C_BY_ROWS(ln::run, dtype, access, a, how, st);
     if (const int rc = check_launch(op)) return rc;
   }
-  launch_dependent(ln::join_kernel, dim3((unsigned)ceil_div(2 * d, 8)), 1024, 0, st, (const float*)workspace, m > 0 ? how.ctas : 0, (int)d, dweight, dbias);
+  if (alone) return F2C_OK;
+  const int parts = m > 0 ? how.ctas : 0;
+  launch_dependent(ln::join_kernel, dim3((unsigned)ceil_div(2 * d, 8)), 32 * (parts >= 512 ? 32 : parts / 16 + 1), 0, st, (const float*)workspace, parts, (int)d, dweight, dbias);
   return check_launch(op);
 }
