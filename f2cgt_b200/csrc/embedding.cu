@@ -4,12 +4,18 @@
 // the places i with ids[i] = r, in their order: the places are sorted by id (stable), every warp adds up a stretch of them, and a segment that lies in
 // several stretches is put together by a last launch.  No atomics on values: the same bits every time.  Sums are single precision, rounded once.
 //
+// Up to 1024 places it is one launch (few_kernel): every CTA sorts all of them, in registers and shared memory, and adds up its share of the segments; what
+// was not looked up is set to zero on the way.  (1024 places of 172 rows, 128 columns: 8.3 us in a graph, 7 in a row of calls; with
+// the launches below 8.3 and 12.4 (rows alone), and 19 in a row of calls, whose launches the host makes.)
+//
 // Sorting.  Up to 4096 places each place counts the ones in front of it, in one launch: the keys are few enough that all pairs cost
 // less than further launches.  Beyond, digits of up to 11 bits from the lowest on: counts of every tile of 1024 places, their sums over tiles, and the
 // placing, in which a warp ranks 32 places at a time by their equals in it and counts the next digit where the places go.  As many digits as the table
 // has rows need.  All of it is latency, 3 to 6 us a launch: the first one also clears what the others add to, and a whole table's gradient, on CTAs of its
 // own.  (With tiles of 4096 places that add up the other tiles' counts themselves, two launches less, 121,000 places took 62 us instead of 51: the work
 // was on too few SMs.)  121,000 places of 2.4 M rows, 128 columns: 51 us; 59,000 of 172: 19 us.
+#include <algorithm>
+
 #include "checkpoint.cuh"
 
 namespace f2c {
@@ -467,6 +473,135 @@ __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, cons
   }
 }
 
+// ---------------------------------------------------------------- few places
+constexpr int kOneLaunch = 1024, kFewWarps = kOneLaunch / 32, kShortSegment = 32;
+constexpr unsigned long long kNobody = ~0ull;
+
+// Sorts a number of every thread of the CTA, in ascending order (a bitonic network): partners up to 16 lanes away by shuffles, the others by shared memory.
+// `count` of them, from the first thread's on, are not kNobody.
+__device__ __forceinline__ unsigned long long sort_block(unsigned long long v, unsigned long long* room, int count) {
+  const int i = threadIdx.x;
+#pragma unroll
+  for (int size = 2; size <= kOneLaunch; size *= 2) {
+    if (size / 2 >= count) break;
+#pragma unroll
+    for (int apart = size / 2; apart > 0; apart /= 2) {
+      unsigned long long other;
+      if (apart >= 32) {
+        __syncthreads();
+        room[i] = v;
+        __syncthreads();
+        other = room[i ^ apart];
+      } else {
+        other = __shfl_xor_sync(0xffffffffu, v, apart);
+      }
+      const bool lower = ((i & apart) == 0) == ((i & size) == 0);
+      if ((v > other) == lower) v = other;
+    }
+  }
+  return v;
+}
+
+// CTA x of gridDim.x has every gridDim.x-th segment, 128 columns of it, and every gridDim.x-th row that is to be zero.
+template <typename T, typename I, int ACCESS>
+__global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict__ dy, int64_t ld, const I* __restrict__ ids, int m, uint32_t rows, int d, float scale, T* __restrict__ out,
+                                                            int64_t* __restrict__ looked_up, int64_t* __restrict__ count) {
+  __shared__ __align__(16) unsigned long long room[kOneLaunch];
+  __shared__ __align__(16) float sums[kFewWarps][kGroup];
+  __shared__ uint32_t key_of_segment[kOneLaunch], place_of[kOneLaunch], before_warp[kFewWarps];
+  __shared__ uint16_t start[kOneLaunch + 1];
+  dependency_wait();
+  release_dependents();
+  const int i = threadIdx.x, lane = i & 31, warp = i >> 5, col = blockIdx.y * kGroup + 4 * lane, left = d - col;
+  uint32_t key = i < m ? key_of(ids, i, rows) : rows;
+  const unsigned long long sorted = sort_block(key < rows ? (unsigned long long)key << 32 | (uint32_t)i : kNobody, room, m);
+  __syncthreads();
+  room[i] = sorted;
+  __syncthreads();
+  key = (uint32_t)(sorted >> 32);
+  place_of[i] = (uint32_t)sorted;
+  const bool there = sorted != kNobody, first = there && (i == 0 || (uint32_t)(room[i - 1] >> 32) != key);
+  const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) before_warp[warp] = __popc(firsts);
+  __syncthreads();
+  const uint32_t mine = before_warp[lane];  // (as many warps as lanes)
+  const uint32_t number = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0u) + __popc(firsts & ((1u << lane) - 1u));
+  if (first) {
+    start[number] = (uint16_t)i;
+    key_of_segment[number] = key;
+  }
+  const int kept = __syncthreads_count(there), segments = (int)__reduce_add_sync(0xffffffffu, mine);
+  if (i == 0) start[segments] = (uint16_t)kept;
+  __syncthreads();
+  const auto add = [&](f32x2 (&acc)[2], int from, int to) {
+    for (int p = from; p < to; p += kRowsAhead) {
+      Four<T, ACCESS> v[kRowsAhead];
+#pragma unroll
+      for (int q = 0; q < kRowsAhead; ++q) v[q].load(dy + (int64_t)place_of[min(p + q, kOneLaunch - 1)] * ld + col, p + q < to ? left : 0);
+#pragma unroll
+      for (int q = 0; q < kRowsAhead; ++q) {
+        f32x2 f[2];
+        v[q].get(f);
+        acc[0] = plus2(acc[0], f[0]);
+        acc[1] = plus2(acc[1], f[1]);
+      }
+    }
+  };
+  const auto write = [&](int s, f32x2 (&acc)[2]) {
+    acc[0] = mul2(acc[0], both(scale));
+    acc[1] = mul2(acc[1], both(scale));
+    Four<T, ACCESS> v;
+    v.set(acc);
+    v.store(out + (int64_t)(looked_up != nullptr ? (uint32_t)s : key_of_segment[s]) * d + col, left);
+  };
+  // short segments a warp each, long ones a 32nd of their places a warp
+  for (int s = blockIdx.x + warp * gridDim.x; s < segments; s += kFewWarps * gridDim.x) {
+    if (start[s + 1] - start[s] > kShortSegment) continue;
+    f32x2 acc[2] = {};
+    add(acc, start[s], start[s + 1]);
+    write(s, acc);
+  }
+  for (int s = blockIdx.x; s < segments; s += gridDim.x) {
+    const int from = start[s], places = start[s + 1] - from;
+    if (places <= kShortSegment) continue;  // for all threads alike
+    f32x2 acc[2] = {};
+    add(acc, from + places * warp / kFewWarps, from + places * (warp + 1) / kFewWarps);
+    *reinterpret_cast<ulonglong2*>(&sums[warp][4 * lane]) = make_ulonglong2(acc[0], acc[1]);
+    __syncthreads();
+    if (warp == 0) {
+      acc[0] = acc[1] = 0ull;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sums[w][4 * lane]);
+        acc[0] = plus2(acc[0], v.x);
+        acc[1] = plus2(acc[1], v.y);
+      }
+      write(s, acc);
+    }
+    __syncthreads();
+  }
+  Four<T, ACCESS> zero;
+  const f32x2 none[2] = {};
+  zero.set(none);
+  if (looked_up != nullptr) {
+    for (int r = segments + blockIdx.x + warp * gridDim.x; r < m; r += kFewWarps * gridDim.x) zero.store(out + (int64_t)r * d + col, left);
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+      if (i < m) looked_up[i] = i < segments ? (int64_t)key_of_segment[i] : -1;
+      if (i == 0) *count = segments;
+    }
+  } else {
+    for (int64_t r = blockIdx.x + (int64_t)warp * gridDim.x; r < (int64_t)rows; r += (int64_t)kFewWarps * gridDim.x) {
+      int low = 0, high = segments;  // the first segment whose row is not in front of this one
+      while (low < high) {
+        const int middle = (low + high) / 2;
+        if (key_of_segment[middle] < (uint32_t)r) low = middle + 1;
+        else high = middle;
+      }
+      if (low == segments || key_of_segment[low] != (uint32_t)r) zero.store(out + r * d + col, left);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- host
 template <typename T, typename I, int ACCESS>
 static void lookup_as(const void* table, int64_t ld, int64_t rows, int64_t d, const void* ids, int64_t m, float scale, void* out, cudaStream_t st) {
@@ -495,6 +630,7 @@ static Plan plan(int64_t m, int64_t rows, int64_t d) {
   Plan p{};
   p.m = m;
   p.d = d;
+  if (m <= kOneLaunch) return p;
   // Short stretches where there are few places: a stretch's rows are added one after the other.  Long ones where segments go over many of them: 59,000 places of
   // 172 rows took 29.9 us in stretches of 32 and 32.0 of 16, 121,000 of 2.4 M rows 84.7 and 79.6.
   p.stretch = m <= 16384 ? 8 : rows < m / 8 ? 32 : 16;
@@ -576,6 +712,18 @@ static void add_up(const Plan& p, const void* dy, int64_t ld, float scale, const
   launch_dependent(join_kernel<T, ACCESS>, grid, kThreads, 0, st, (int)p.d, scale, s, open, (T*)out);
 }
 
+// CTAs of few_kernel: a warp to a segment at most, and enough to write a table of zeros.
+template <typename T, int ACCESS>
+static void add_few(const void* dy, int64_t ld, const void* ids, int index_dtype, int64_t m, int64_t rows, int64_t d, float scale, void* out, int64_t* looked_up, int64_t* count, cudaStream_t st) {
+  const int64_t slabs = ceil_div(d, kGroup), zeros = count == nullptr ? rows : 0;
+  int64_t ctas = std::max(ceil_div(m, kFewWarps), ceil_div(zeros, 16 * kFewWarps));
+  ctas = std::min(ctas, std::max<int64_t>(1, kSmCount / slabs));
+  const dim3 grid((unsigned)ctas, (unsigned)slabs);
+  int64_t* const list = count != nullptr ? looked_up : nullptr;
+  if (index_dtype == F2C_I64) launch_dependent(few_kernel<T, int64_t, ACCESS>, grid, kOneLaunch, 0, st, (const T*)dy, ld, (const int64_t*)ids, (int)m, (uint32_t)rows, (int)d, scale, (T*)out, list, count);
+  else launch_dependent(few_kernel<T, int32_t, ACCESS>, grid, kOneLaunch, 0, st, (const T*)dy, ld, (const int32_t*)ids, (int)m, (uint32_t)rows, (int)d, scale, (T*)out, list, count);
+}
+
 static int check(const char* op, int dtype, int index_dtype, int64_t m, int64_t rows, int64_t d) {
   F2C_REQUIRE(is_float_dtype(dtype), F2C_ERR_UNSUPPORTED, "%s: rows must be float32, float16 or bfloat16", op);
   F2C_REQUIRE(is_index_dtype(index_dtype), F2C_ERR_UNSUPPORTED, "%s: ids must be int32 or int64", op);
@@ -624,7 +772,7 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
     F2C_REQUIRE(dy && ids && (grad || (dense && rows == 0)), F2C_ERR_INVALID, "%s: null pointer", op);
     F2C_REQUIRE(m == 1 || ldy >= d, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);
     const int64_t need = f2c_embedding_backward_workspace(m, rows, d);
-    F2C_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 256), F2C_ERR_INVALID, "%s: the workspace must have %lld bytes, 256-byte aligned", op, (long long)need);
+    F2C_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 256)), F2C_ERR_INVALID, "%s: the workspace must have %lld bytes, 256-byte aligned", op, (long long)need);
   }
   const int64_t bytes = dense ? rows * d * dtype_size(dtype) : 0;
   if (bytes > 0 && m == 0) {
@@ -637,6 +785,11 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
     if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
   }
   if (m == 0 || d == 0 || (dense && rows == 0)) return F2C_OK;
+  const int item = dtype_size(dtype), from = ckpt::access_of(dy, ldy, m, d, item), to = ckpt::access_of(grad, d, dense ? rows : m, d, item), access = from < to ? from : to;
+  if (m <= emb::kOneLaunch) {
+    F2C_BY_ROWS(emb::add_few, dtype, access, dy, ldy, ids, index_dtype, m, rows, d, scale, grad, looked_up, count, st);
+    return check_launch(op);
+  }
   char* const ws = (char*)workspace;
   const emb::Plan p = emb::plan(m, rows, d);
   const emb::Pairs sorted = index_dtype == F2C_I64 ? emb::sort(p, (const int64_t*)ids, (uint32_t)rows, ws, grad, bytes, st)
@@ -646,7 +799,6 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
     launch_dependent(emb::number_kernel, dim3((unsigned)p.tiles), emb::kThreads, 0, st, (const uint32_t*)sorted.key, m, (uint32_t)rows, p.stretch, in_tile, of_tile, looked_up);
   const emb::Segments s{sorted.key, sorted.place, m, (uint32_t)rows, p.stretch, p.stretches, in_tile, of_tile, p.tiles, dense ? nullptr : looked_up, count};
   const emb::Open open{(float*)(ws + p.head), (float*)(ws + p.tail), (int64_t*)(ws + p.row), p.width};
-  const int item = dtype_size(dtype), from = ckpt::access_of(dy, ldy, m, d, item), to = ckpt::access_of(grad, d, dense ? rows : m, d, item);
-  F2C_BY_ROWS(emb::add_up, dtype, (from < to ? from : to), p, dy, ldy, scale, s, open, grad, st);
+  F2C_BY_ROWS(emb::add_up, dtype, access, p, dy, ldy, scale, s, open, grad, st);
   return check_launch(op);
 }

@@ -87,7 +87,7 @@ def check_gradient(dy, ids, rows, scale):
 
 
 @pytest.mark.parametrize("how", ["any", "one", "skew", "outside", "nowhere", "descending"])
-@pytest.mark.parametrize("m,rows,d", [(1, 1, 1), (1, 1000, 128), (7, 3, 5), (8, 8, 128), (33, 5, 130), (255, 3000, 64), (1024, 172, 128), (4096, 100, 36), (4097, 100, 36),
+@pytest.mark.parametrize("m,rows,d", [(1, 1, 1), (1, 1000, 128), (7, 3, 5), (8, 8, 128), (33, 5, 130), (255, 3000, 64), (1024, 172, 128), (1024, 3, 4096), (1000, 100_000, 12), (1025, 172, 128), (4096, 100, 36), (4097, 100, 36),
                                       (5000, 2047, 8), (5000, 2048, 8), (20000, 5_000_000, 4), (16385, 172, 260), (40001, 7, 128), (70000, 60000, 16)])
 def test_gradient(m, rows, d, how):
     dy = table_of(m, d, torch.float32, seed=2)

@@ -61,7 +61,7 @@ def rows_gradient(dy=AT, ldy=8, dtype=_lib.F32, ids=AT, index=_lib.I64, m=4, row
     (lambda: lookup(ids=0), INVALID), (lambda: lookup(out=0), INVALID), (lambda: lookup(m=0, ids=0, out=0), OK), (lambda: lookup(d=0, out=0), OK),
     (lambda: rows_gradient(dtype=_lib.I8), UNSUPPORTED), (lambda: rows_gradient(index=_lib.U8), UNSUPPORTED), (lambda: rows_gradient(d=-1), INVALID), (lambda: rows_gradient(dy=0), INVALID),
     (lambda: rows_gradient(ids=0), INVALID), (lambda: rows_gradient(grad=0), INVALID), (lambda: rows_gradient(looked_up=0), INVALID), (lambda: rows_gradient(ldy=7), INVALID),
-    (lambda: rows_gradient(work=0), INVALID), (lambda: rows_gradient(work=AT + 8), INVALID), (lambda: rows_gradient(size=1000), INVALID),
+    (lambda: rows_gradient(m=5000, work=0), INVALID), (lambda: rows_gradient(m=5000, work=AT + 8), INVALID), (lambda: rows_gradient(m=5000, size=1000), INVALID),
     (lambda: rows_gradient(count=0, looked_up=0, rows=1 << 25, d=1 << 20, ldy=1 << 20, m=1), LIMIT), (lambda: rows_gradient(count=0, grad=0), INVALID),
     (lambda: rows_gradient(count=0, rows=0, m=0, dy=0, ids=0, work=0, grad=0), OK)])
 def test_learned_rows(call, status):
@@ -70,8 +70,8 @@ def test_learned_rows(call, status):
 
 
 def test_workspaces_of_learned_rows():
-    few, many, large = (lib.f2c_embedding_backward_workspace(m, rows, 128) for m, rows in ((100, 1000), (100_000, 1000), (100_000, 1 << 30)))
-    assert 0 < few < many < large and lib.f2c_embedding_backward_workspace(0, 10, 10) == 0
+    few, many, large = (lib.f2c_embedding_backward_workspace(m, rows, 128) for m, rows in ((1025, 1000), (100_000, 1000), (100_000, 1 << 30)))
+    assert 0 < few < many < large and lib.f2c_embedding_backward_workspace(0, 10, 10) == lib.f2c_embedding_backward_workspace(1024, 1000, 128) == 0
     assert many < 100_000 * 128 * 4  # less than the rows themselves
 
 
