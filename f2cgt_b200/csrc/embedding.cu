@@ -8,12 +8,15 @@
 // was not looked up is set to zero on the way.  (1024 places of 172 rows, 128 columns: 8.3 us in a graph, 7 in a row of calls; with
 // the launches below 8.3 and 12.4 (rows alone), and 19 in a row of calls, whose launches the host makes.)
 //
+// More places of few rows (labels): a CTA sorts 400 places at most while their rows of dy come to its shared memory, and leaves a sum for every row of the table
+// that it met; a second launch adds those up in the CTAs' order.  59,000 x 128 of 172 rows: 14 us, 24 with all places sorted.
+//
 // Sorting.  Up to 4096 places each place counts the ones in front of it, in one launch: the keys are few enough that all pairs cost
 // less than further launches.  Beyond, digits of up to 11 bits from the lowest on: counts of every tile of 1024 places, their sums over tiles, and the
 // placing, in which a warp ranks 32 places at a time by their equals in it and counts the next digit where the places go.  As many digits as the table
 // has rows need.  All of it is latency, 3 to 6 us a launch: the first one also clears what the others add to, and a whole table's gradient, on CTAs of its
 // own.  (With tiles of 4096 places that add up the other tiles' counts themselves, two launches less, 121,000 places took 62 us instead of 51: the work
-// was on too few SMs.)  121,000 places of 2.4 M rows, 128 columns: 51 us; 59,000 of 172: 19 us.
+// was on too few SMs.)  121,000 places of 2.4 M rows, 128 columns: 57 us in seven launches, 32 of them the sorting.
 #include <algorithm>
 
 #include "checkpoint.cuh"
@@ -476,17 +479,19 @@ __global__ void __launch_bounds__(kThreads) join_kernel(int d, float scale, cons
 // ---------------------------------------------------------------- few places
 constexpr int kOneLaunch = 1024, kFewWarps = kOneLaunch / 32, kShortSegment = 32;
 constexpr unsigned long long kNobody = ~0ull;
+constexpr int64_t kClearedBeside = 1 << 24;  // bytes of a table that this kernel clears itself
 
 // Sorts a number of every thread of the CTA, in ascending order (a bitonic network): partners up to 16 lanes away by shuffles, the others by shared memory.
-// `count` of them, from the first thread's on, are not kNobody.
-__device__ __forceinline__ unsigned long long sort_block(unsigned long long v, unsigned long long* room, int count) {
+// `count` of them, from the first thread's on, are not the largest number there is.
+template <int THREADS, typename N>
+__device__ __forceinline__ N sort_block(N v, N* room, int count) {
   const int i = threadIdx.x;
 #pragma unroll
-  for (int size = 2; size <= kOneLaunch; size *= 2) {
+  for (int size = 2; size <= THREADS; size *= 2) {
     if (size / 2 >= count) break;
 #pragma unroll
     for (int apart = size / 2; apart > 0; apart /= 2) {
-      unsigned long long other;
+      N other;
       if (apart >= 32) {
         __syncthreads();
         room[i] = v;
@@ -502,9 +507,9 @@ __device__ __forceinline__ unsigned long long sort_block(unsigned long long v, u
   return v;
 }
 
-// CTA x of gridDim.x has every gridDim.x-th segment, 128 columns of it, and every gridDim.x-th row that is to be zero.
+// CTA x of gridDim.x has every gridDim.x-th segment, 128 columns of it, and every gridDim.x-th row that is to be zero (of the first `clear` rows of a whole table).
 template <typename T, typename I, int ACCESS>
-__global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict__ dy, int64_t ld, const I* __restrict__ ids, int m, uint32_t rows, int d, float scale, T* __restrict__ out,
+__global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict__ dy, int64_t ld, const I* __restrict__ ids, int m, uint32_t rows, int64_t clear, int d, float scale, T* __restrict__ out,
                                                             int64_t* __restrict__ looked_up, int64_t* __restrict__ count) {
   __shared__ __align__(16) unsigned long long room[kOneLaunch];
   __shared__ __align__(16) float sums[kFewWarps][kGroup];
@@ -514,7 +519,7 @@ __global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict_
   release_dependents();
   const int i = threadIdx.x, lane = i & 31, warp = i >> 5, col = blockIdx.y * kGroup + 4 * lane, left = d - col;
   uint32_t key = i < m ? key_of(ids, i, rows) : rows;
-  const unsigned long long sorted = sort_block(key < rows ? (unsigned long long)key << 32 | (uint32_t)i : kNobody, room, m);
+  const unsigned long long sorted = sort_block<kOneLaunch>(key < rows ? (unsigned long long)key << 32 | (uint32_t)i : kNobody, room, m);
   __syncthreads();
   room[i] = sorted;
   __syncthreads();
@@ -590,7 +595,7 @@ __global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict_
       if (i == 0) *count = segments;
     }
   } else {
-    for (int64_t r = blockIdx.x + (int64_t)warp * gridDim.x; r < (int64_t)rows; r += (int64_t)kFewWarps * gridDim.x) {
+    for (int64_t r = blockIdx.x + (int64_t)warp * gridDim.x; r < clear; r += (int64_t)kFewWarps * gridDim.x) {
       int low = 0, high = segments;  // the first segment whose row is not in front of this one
       while (low < high) {
         const int middle = (low + high) / 2;
@@ -600,6 +605,162 @@ __global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict_
       if (low == segments || key_of_segment[low] != (uint32_t)r) zero.store(out + r * d + col, left);
     }
   }
+}
+
+// ---------------------------------------------------------------- few rows
+// A CTA has `each` places, 128 columns of them: it sorts them by row while they come to shared memory, and leaves a sum for every row that is among them.
+// (Places that need more than one CTA an SM: the sorting is not hidden any more, 236,000 of 1000 rows took 80 us and 68 with all of them sorted.  More rows
+// times pieces of 128 columns: as many CTAs join them, 6000 x 2048 of 3000 rows took 128 us and 37.)
+constexpr int kLabels = 2048, kLabelThreads = 512, kLabelWarps = kLabelThreads / 32, kMostPlaces = 400, kLeastPlaces = 32;
+constexpr uint16_t kNoSlot = 0xffffu;
+static_assert(kLabels <= 1 << 22 && kMostPlaces < kLabelThreads, "a row and a place are one number of 32 bits, and none is the largest");
+static_assert(kSmCount <= kLabelThreads, "a thread has a CTA's slot");
+
+struct Labels {
+  int64_t m, width;
+  uint32_t rows;
+  int d, each, ctas, slots;
+  float* part;      // [ctas][slots][width]
+  uint16_t* where;  // [rows][ctas]: a row's slot
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
+}
+
+template <typename T, typename I, int ACCESS>
+__global__ void __launch_bounds__(kLabelThreads, 1) labels_kernel(const T* __restrict__ dy, int64_t ld, const I* __restrict__ ids, const __grid_constant__ Labels a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ __align__(16) float sums[kLabelWarps][kGroup];
+  __shared__ uint32_t room[kLabelThreads], before_warp[kLabelWarps], long_of[kLabelWarps];
+  __shared__ uint16_t place_of[kLabelThreads], start[kLabelThreads + 1], slot[kLabels];
+  T* const tile = reinterpret_cast<T*>(smem_raw);  // [each][128]
+  dependency_wait();
+  release_dependents();
+  const int i = threadIdx.x, lane = i & 31, warp = i >> 5, col = blockIdx.y * kGroup + 4 * lane, left = a.d - col;
+  const int64_t from = (int64_t)blockIdx.x * a.each;
+  const int n = (int)min((int64_t)a.each, a.m - from);
+  uint32_t key = i < n ? key_of(ids, from + i, a.rows) : a.rows;
+  for (int p = warp; p < n; p += kLabelWarps) {
+    const T* const at = dy + (from + p) * ld + col;
+#pragma unroll
+    for (int q = 0; q < Four<T, ACCESS>::kPieces; ++q) {
+      constexpr int kEach = Four<T, ACCESS>::kEach;
+      T* const to = tile + p * kGroup + 4 * lane + q * kEach;
+      if (q * kEach >= left) continue;  // (what is there instead meets no column that exists)
+      if constexpr (ACCESS >= 4) copy_async<ACCESS>(to, at + q * kEach);
+      else *to = at[q];
+    }
+  }
+  for (int r = i; r < (int)a.rows; r += kLabelThreads) slot[r] = kNoSlot;
+  const uint32_t sorted = sort_block<kLabelThreads>(key < a.rows ? key << 9 | (uint32_t)i : ~0u, room, n);
+  __syncthreads();
+  room[i] = sorted;
+  __syncthreads();
+  key = sorted >> 9;
+  place_of[i] = (uint16_t)(sorted & 511u);
+  const bool there = sorted != ~0u, first = there && (i == 0 || room[i - 1] >> 9 != key);
+  const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) before_warp[warp] = __popc(firsts);
+  __syncthreads();
+  const uint32_t mine = lane < kLabelWarps ? before_warp[lane] : 0u;
+  const uint32_t number = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0u) + __popc(firsts & ((1u << lane) - 1u));
+  if (first) {
+    start[number] = (uint16_t)i;
+    slot[key] = (uint16_t)number;
+  }
+  const int kept = __syncthreads_count(there), segments = (int)__reduce_add_sync(0xffffffffu, mine);
+  if (i == 0) start[segments] = (uint16_t)kept;
+  __syncthreads();
+  const uint32_t longs = __ballot_sync(0xffffffffu, i < segments && start[i + 1] - start[i] > kShortSegment);
+  if (lane == 0) long_of[warp] = longs;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  const auto add = [&](f32x2 (&acc)[2], int from, int to) {
+#pragma unroll 4
+    for (int p = from; p < to; ++p) {
+      const Four<T, 4 * (int)sizeof(T)> v = *reinterpret_cast<const Four<T, 4 * (int)sizeof(T)>*>(tile + place_of[p] * kGroup + 4 * lane);
+      f32x2 f[2];
+      v.get(f);
+      acc[0] = plus2(acc[0], f[0]);
+      acc[1] = plus2(acc[1], f[1]);
+    }
+  };
+  const auto write = [&](int s, const f32x2 (&acc)[2]) {
+    *reinterpret_cast<ulonglong2*>(a.part + ((int64_t)blockIdx.x * a.slots + s) * a.width + blockIdx.y * kGroup + 4 * lane) = make_ulonglong2(acc[0], acc[1]);
+  };
+  // short segments a warp each, long ones a part of their places a warp
+  for (int s = warp; s < segments; s += kLabelWarps) {
+    if (start[s + 1] - start[s] > kShortSegment) continue;
+    f32x2 acc[2] = {};
+    add(acc, start[s], start[s + 1]);
+    write(s, acc);
+  }
+  for (int word = 0; word < kLabelWarps; ++word)
+    for (uint32_t bits = long_of[word]; bits != 0u; bits &= bits - 1u) {  // for all threads alike
+      const int s = 32 * word + __ffs((int)bits) - 1, from = start[s], places = start[s + 1] - from;
+      f32x2 acc[2] = {};
+      add(acc, from + places * warp / kLabelWarps, from + places * (warp + 1) / kLabelWarps);
+      *reinterpret_cast<ulonglong2*>(&sums[warp][4 * lane]) = make_ulonglong2(acc[0], acc[1]);
+      __syncthreads();
+      if (warp == 0) {
+        acc[0] = acc[1] = 0ull;
+#pragma unroll
+        for (int w = 0; w < kLabelWarps; ++w) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sums[w][4 * lane]);
+          acc[0] = plus2(acc[0], v.x);
+          acc[1] = plus2(acc[1], v.y);
+        }
+        write(s, acc);
+      }
+      __syncthreads();
+    }
+  if (blockIdx.y == 0)
+    for (int r = i; r < (int)a.rows; r += kLabelThreads) a.where[(int64_t)r * a.ctas + blockIdx.x] = slot[r];
+}
+
+// A row's sums over the CTAs, in their order: a CTA to a row, 128 columns of it.
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(kLabelThreads) label_rows_kernel(float scale, const __grid_constant__ Labels a, T* __restrict__ out) {
+  __shared__ __align__(16) float sums[kLabelWarps][kGroup];
+  __shared__ uint32_t list[kLabelThreads], before_warp[kLabelWarps];
+  dependency_wait();
+  release_dependents();
+  const int i = threadIdx.x, lane = i & 31, warp = i >> 5, row = blockIdx.x, col = blockIdx.y * kGroup + 4 * lane;
+  f32x2 acc[2] = {};
+  const uint16_t slot = i < a.ctas ? __ldg(a.where + (int64_t)row * a.ctas + i) : kNoSlot;
+  const uint32_t those = __ballot_sync(0xffffffffu, slot != kNoSlot);
+  if (lane == 0) before_warp[warp] = __popc(those);
+  __syncthreads();
+  const uint32_t mine = lane < kLabelWarps ? before_warp[lane] : 0u, before = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0u);
+  const int count = (int)__reduce_add_sync(0xffffffffu, mine);
+  if (slot != kNoSlot) list[before + __popc(those & ((1u << lane) - 1u))] = (uint32_t)(i * a.slots + slot);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < (kSmCount + kLabelWarps - 1) / kLabelWarps; ++u) {
+    const int q = warp + u * kLabelWarps;
+    if (q >= count) continue;
+    const float4 v = __ldg(reinterpret_cast<const float4*>(a.part + list[q] * a.width + blockIdx.y * kGroup + 4 * lane));
+    acc[0] = plus2(acc[0], pair_of(v.x, v.y));
+    acc[1] = plus2(acc[1], pair_of(v.z, v.w));
+  }
+  *reinterpret_cast<ulonglong2*>(&sums[warp][4 * lane]) = make_ulonglong2(acc[0], acc[1]);
+  __syncthreads();
+  if (warp != 0) return;
+  acc[0] = acc[1] = 0ull;
+#pragma unroll
+  for (int w = 0; w < kLabelWarps; ++w) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sums[w][4 * lane]);
+    acc[0] = plus2(acc[0], v.x);
+    acc[1] = plus2(acc[1], v.y);
+  }
+  acc[0] = mul2(acc[0], both(scale));
+  acc[1] = mul2(acc[1], both(scale));
+  Four<T, ACCESS> v;
+  v.set(acc);
+  v.store(out + (int64_t)row * a.d + col, a.d - col);
 }
 
 // ---------------------------------------------------------------- host
@@ -714,14 +875,45 @@ static void add_up(const Plan& p, const void* dy, int64_t ld, float scale, const
 
 // CTAs of few_kernel: a warp to a segment at most, and enough to write a table of zeros.
 template <typename T, int ACCESS>
-static void add_few(const void* dy, int64_t ld, const void* ids, int index_dtype, int64_t m, int64_t rows, int64_t d, float scale, void* out, int64_t* looked_up, int64_t* count, cudaStream_t st) {
-  const int64_t slabs = ceil_div(d, kGroup), zeros = count == nullptr ? rows : 0;
+static void add_few(const void* dy, int64_t ld, const void* ids, int index_dtype, int64_t m, bool clear, int64_t rows, int64_t d, float scale, void* out, int64_t* looked_up, int64_t* count, cudaStream_t st) {
+  const int64_t slabs = ceil_div(d, kGroup), zeros = count == nullptr && clear ? rows : 0;
   int64_t ctas = std::max(ceil_div(m, kFewWarps), ceil_div(zeros, 16 * kFewWarps));
   ctas = std::min(ctas, std::max<int64_t>(1, kSmCount / slabs));
   const dim3 grid((unsigned)ctas, (unsigned)slabs);
   int64_t* const list = count != nullptr ? looked_up : nullptr;
-  if (index_dtype == F2C_I64) launch_dependent(few_kernel<T, int64_t, ACCESS>, grid, kOneLaunch, 0, st, (const T*)dy, ld, (const int64_t*)ids, (int)m, (uint32_t)rows, (int)d, scale, (T*)out, list, count);
-  else launch_dependent(few_kernel<T, int32_t, ACCESS>, grid, kOneLaunch, 0, st, (const T*)dy, ld, (const int32_t*)ids, (int)m, (uint32_t)rows, (int)d, scale, (T*)out, list, count);
+  if (index_dtype == F2C_I64) launch_dependent(few_kernel<T, int64_t, ACCESS>, grid, kOneLaunch, 0, st, (const T*)dy, ld, (const int64_t*)ids, (int)m, (uint32_t)rows, zeros, (int)d, scale, (T*)out, list, count);
+  else launch_dependent(few_kernel<T, int32_t, ACCESS>, grid, kOneLaunch, 0, st, (const T*)dy, ld, (const int32_t*)ids, (int)m, (uint32_t)rows, zeros, (int)d, scale, (T*)out, list, count);
+}
+
+// Few rows: how the places are dealt out, and the workspace.  `ctas` 0: not for these sizes.
+static Labels labels(int64_t m, int64_t rows, int64_t d) {
+  Labels a{};
+  const int64_t slabs = ceil_div(d, kGroup);
+  if (m <= kOneLaunch || rows == 0 || rows * slabs > kLabels || ceil_div(m, kMostPlaces) * slabs > kSmCount) return a;
+  a.m = m;
+  a.width = slabs * kGroup;
+  a.rows = (uint32_t)rows;
+  a.d = (int)d;
+  a.each = (int)std::max<int64_t>(kLeastPlaces, ceil_div(m, kSmCount / slabs));
+  a.ctas = (int)ceil_div(m, a.each);
+  a.slots = (int)std::min<int64_t>(a.each, rows);
+  return a;
+}
+static int64_t label_parts(const Labels& a) { return ceil_div((int64_t)a.ctas * a.slots * a.width * 4, 256) * 256; }
+static int64_t label_bytes(const Labels& a) { return label_parts(a) + ceil_div((int64_t)a.ctas * a.rows * 2, 256) * 256; }
+
+template <typename T, int ACCESS>
+static void add_labels(const char* op, const void* dy, int64_t ld, const void* ids, int index_dtype, const Labels& a, float scale, void* out, cudaStream_t st, int* rc) {
+  const dim3 grid((unsigned)a.ctas, (unsigned)ceil_div(a.d, kGroup));
+  const int bytes = a.each * kGroup * (int)sizeof(T);
+  if (index_dtype == F2C_I64) {
+    if ((*rc = allow_smem(op, (const void*)labels_kernel<T, int64_t, ACCESS>, kMostPlaces * kGroup * (int)sizeof(T)))) return;
+    launch_dependent(labels_kernel<T, int64_t, ACCESS>, grid, kLabelThreads, bytes, st, (const T*)dy, ld, (const int64_t*)ids, a);
+  } else {
+    if ((*rc = allow_smem(op, (const void*)labels_kernel<T, int32_t, ACCESS>, kMostPlaces * kGroup * (int)sizeof(T)))) return;
+    launch_dependent(labels_kernel<T, int32_t, ACCESS>, grid, kLabelThreads, bytes, st, (const T*)dy, ld, (const int32_t*)ids, a);
+  }
+  launch_dependent(label_rows_kernel<T, ACCESS>, dim3(a.rows, grid.y), kLabelThreads, 0, st, scale, a, (T*)out);
 }
 
 static int check(const char* op, int dtype, int index_dtype, int64_t m, int64_t rows, int64_t d) {
@@ -754,7 +946,7 @@ extern "C" int f2c_embedding(const void* table, int64_t ld, int dtype, int64_t r
 
 extern "C" int64_t f2c_embedding_backward_workspace(int64_t m, int64_t rows, int64_t d) {
   if (m <= 0 || rows < 0 || d <= 0 || m > emb::kMaxPlaces || rows > emb::kMaxRows || d > emb::kMaxColumns) return 0;
-  return emb::plan(m, rows, d).bytes;
+  return std::max(emb::plan(m, rows, d).bytes, emb::label_bytes(emb::labels(m, rows, d)));
 }
 
 extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, const void* ids, int index_dtype, int64_t m, int64_t rows, int64_t d, float scale, void* grad,
@@ -775,7 +967,9 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
     F2C_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 256)), F2C_ERR_INVALID, "%s: the workspace must have %lld bytes, 256-byte aligned", op, (long long)need);
   }
   const int64_t bytes = dense ? rows * d * dtype_size(dtype) : 0;
-  if (bytes > 0 && m == 0) {
+  // (few places and a large table: cleared by itself.  The kernel's warps look every row up among the places': 2.4 M rows of 128 bytes took 364 us so, and 56 this way.)
+  const bool cleared = bytes > 0 && (m == 0 || d == 0 || (m <= emb::kOneLaunch && bytes > emb::kClearedBeside));
+  if (cleared) {
     const cudaError_t e = cudaMemsetAsync(grad, 0, (size_t)bytes, st);
     if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
   }
@@ -787,10 +981,18 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
   if (m == 0 || d == 0 || (dense && rows == 0)) return F2C_OK;
   const int item = dtype_size(dtype), from = ckpt::access_of(dy, ldy, m, d, item), to = ckpt::access_of(grad, d, dense ? rows : m, d, item), access = from < to ? from : to;
   if (m <= emb::kOneLaunch) {
-    F2C_BY_ROWS(emb::add_few, dtype, access, dy, ldy, ids, index_dtype, m, rows, d, scale, grad, looked_up, count, st);
+    F2C_BY_ROWS(emb::add_few, dtype, access, dy, ldy, ids, index_dtype, m, !cleared, rows, d, scale, grad, looked_up, count, st);
     return check_launch(op);
   }
   char* const ws = (char*)workspace;
+  emb::Labels few = emb::labels(m, rows, d);
+  if (dense && few.ctas > 0) {
+    few.part = (float*)ws;
+    few.where = (uint16_t*)(ws + emb::label_parts(few));
+    int rc = F2C_OK;
+    F2C_BY_ROWS(emb::add_labels, dtype, access, op, dy, ldy, ids, index_dtype, few, scale, grad, st, &rc);
+    return rc != F2C_OK ? rc : check_launch(op);
+  }
   const emb::Plan p = emb::plan(m, rows, d);
   const emb::Pairs sorted = index_dtype == F2C_I64 ? emb::sort(p, (const int64_t*)ids, (uint32_t)rows, ws, grad, bytes, st)
                                                        : emb::sort(p, (const int32_t*)ids, (uint32_t)rows, ws, grad, bytes, st);
