@@ -16,7 +16,7 @@
 //
 // What bounds it: bfloat16 shared memory, from which a stage's operand is read twice while its codes and steps are read and the next stages arrive (16,384 x 2048 x
 // 4096: 478 us, 575 TFLOP/s of the product, 1150 of the MMAs; half the MMAs, or no reading of codes and steps, each took 20% off); float32 the instructions that
-// split dy times the step, 650 a warp for a stage (4096 x 2048 x 1152: 87 us); few rows latency (59,000 x 128 x 128 float32: 17 us of 5.9 that memory takes).
+// split dy times the step, 650 a warp for a stage (4096 x 2048 x 1152: 74 us); few rows latency (59,000 x 128 x 128 float32: 17 us of 5.9 that memory takes).
 //
 // Many rows and few tiles: the rows are dealt out over all SMs; each leaves its part of the sums, and a second launch adds them up in their order.
 #include <algorithm>
@@ -49,9 +49,10 @@ struct Params {
   int64_t groups, m;
   int n, k;
   int n_tiles, splits;
+  int whole, rest;        // tiles that one CTA has all rows of, and the others, whose rows are split
   int64_t split_rows;     // a multiple of kRows
-  void *dw, *db;          // (splits == 1) of dy's type
-  float *part, *part_db;  // (splits > 1) [split][tile][columns / 4][128][4], [split][n_tiles * columns of dy]
+  void *dw, *db;          // of dy's type
+  float *part, *part_db;  // (splits > 1) [split][tile of the others][columns / 4][128][4], and (nothing whole) [split][n_tiles * columns of dy]
   uint32_t tries;
   int* error;
 };
@@ -133,16 +134,18 @@ struct Scales {
 };
 
 struct Place {
-  int tile, split, n0, group;
+  int split, n0, group;
+  int part;  // -1: the result itself
   int64_t row0, rows;
   int stages;
   __device__ __forceinline__ Place(const Params& p, int columns) {
-    tile = (int)blockIdx.x / p.splits;
-    split = (int)blockIdx.x % p.splits;
+    const int other = (int)blockIdx.x - p.whole, tile = other < 0 ? (int)blockIdx.x : p.whole + other / p.splits;
+    split = other < 0 ? 0 : other % p.splits;
+    part = other < 0 || p.splits == 1 ? -1 : split * p.rest + (tile - p.whole);
     n0 = tile % p.n_tiles * columns;
     group = tile / p.n_tiles;
     row0 = split * p.split_rows;
-    rows = min(p.split_rows, p.m - row0);
+    rows = other < 0 ? p.m : min(p.split_rows, p.m - row0);
     stages = (int)((rows + kRows - 1) / kRows);
   }
 };
@@ -326,8 +329,8 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
       uint32_t r[32];
       tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0, r);
       tmem_wait(r);
-      if (p.splits > 1) {
-        float4* const out = reinterpret_cast<float4*>(p.part) + ((int64_t)at.split * (gridDim.x / p.splits) + at.tile) * (kWide * 128 / 4) + c0 / 4 * 128 + quarter * 32 + lane;
+      if (at.part >= 0) {
+        float4* const out = reinterpret_cast<float4*>(p.part) + (int64_t)at.part * (kWide * 128 / 4) + c0 / 4 * 128 + quarter * 32 + lane;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           out[j * 128] = make_float4(__uint_as_float(r[4 * j]) + none, __uint_as_float(r[4 * j + 1]) + none, __uint_as_float(r[4 * j + 2]) + none, __uint_as_float(r[4 * j + 3]) + none);
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
     float sum = lost ? __int_as_float(0x7fffffff) : 0.0f;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) sum += columns[g * kWide + tid];
-    if (p.splits > 1) p.part_db[(int64_t)at.split * p.n_tiles * kWide + at.n0 + tid] = sum;
+    if (at.part >= 0) p.part_db[(int64_t)at.split * p.n_tiles * kWide + at.n0 + tid] = sum;
     else ((__nv_bfloat16*)p.db)[at.n0 + tid] = __float2bfloat16_rn(sum);
   }
 }
@@ -534,8 +537,8 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
   }
 #pragma unroll
   for (int j = 0; j < 16; ++j) sum[j] = plus2(sum[j], both(more));
-  if (p.splits > 1) {
-    ulonglong2* const out = reinterpret_cast<ulonglong2*>(p.part) + ((int64_t)at.split * (gridDim.x / p.splits) + at.tile) * (kTile * kTile / 4) + set * 8 * kTile + i;
+  if (at.part >= 0) {
+    ulonglong2* const out = reinterpret_cast<ulonglong2*>(p.part) + (int64_t)at.part * (kTile * kTile / 4) + set * 8 * kTile + i;
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j * kTile] = make_ulonglong2(sum[2 * j], sum[2 * j + 1]);
     if (at.group == 0 && set == 0) p.part_db[(int64_t)at.split * p.n_tiles * kTile + at.n0 + i] = bias;
@@ -567,17 +570,17 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
 }
 
 // Adds the parts up: 32 lanes and four columns of TMEM to a CTA, every 16th part (or as many as there are) to a
-// warp.  Behind the tiles' CTAs those of db.  The lanes are columns
+// warp.  Behind the tiles' CTAs those of db (where no tile is whole: otherwise those of the first group are).  The lanes are columns
 // of x (bfloat16) or of dy.
 constexpr int kJoinWarps = 16;
 template <typename T>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Params p, int tiles) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Params p) {
   constexpr bool kOfX = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kColumns = kOfX ? kWide : kTile, kPerTile = kColumns, kQuads = kColumns * 128 / 4;
   __shared__ float4 of[kJoinWarps][33];
   dependency_wait();
   release_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, tiles = p.rest;
   if ((int)blockIdx.x >= tiles * kPerTile) {
     const int i = ((int)blockIdx.x - tiles * kPerTile) * 32 + lane;
     float sum = 0.0f;
@@ -600,7 +603,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   }
   of[warp][lane] = sum;
   __syncthreads();
-  const int across = tile % p.n_tiles * kColumns, down = tile / p.n_tiles * kGroup;
+  const int across = (p.whole + tile) % p.n_tiles * kColumns, down = (p.whole + tile) / p.n_tiles * kGroup;
   const int n = across + (kOfX ? quad * 4 : i), col = down + (kOfX ? i : quad * 4);
   if (warp != 0 || n >= p.n || col >= p.k) return;
   sum = of[0][lane];
@@ -628,13 +631,15 @@ __global__ void __launch_bounds__(256) align_kernel(const T* __restrict__ src, i
 }
 
 struct Plan {
-  int columns, n_tiles, k_tiles, splits;
+  int columns, n_tiles, k_tiles, splits, whole, rest;
   int64_t split_rows, part_bytes, sum_bytes, copy_ld, bytes;  // copy_ld: 0 where dy can be read where it is
 };
 
 // How many ways the rows are split: the choice of least time, in cycles: a stage takes an SM 560 (bfloat16: its MMAs), 1200 (float32) or 900 (float16: what
 // the groups do for it); together the SMs get no more than 3500 bytes a cycle; a tile's start and end 4000, the parts' way through L2 and back 4000 bytes a
-// cycle for all SMs, and the launch that adds them up 4000.
+// cycle for all SMs, and the launch that adds them up 4000.  With more tiles than SMs those that fill the SMs are left whole and the rows of the others split, where
+// that is an eighth less: 196 tiles, 16,384 x 1700 x 1700 float32 509 us without and 370 so; 152 tiles, 8192 x 2048 x 2368 bfloat16 188 and 137; but 256 tiles,
+// 16,384 x 2048 x 4096 bfloat16 416 and 429 (SMs that wait leave the others power).
 static Plan plan(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k) {
   Plan p{};
   const int64_t item = dtype_size(dtype);
@@ -644,21 +649,27 @@ static Plan plan(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, i
   const int64_t tiles = (int64_t)p.n_tiles * p.k_tiles, stages = ceil_div(m, kRows), tile_bytes = (int64_t)p.columns * 128 * 4;
   const int64_t first = ceil_div(m, kMaxSplitRows);
   int64_t least = INT64_MAX;
-  for (int64_t s = first; s <= std::min<int64_t>(stages, std::max<int64_t>(first, kSmCount)); ++s) {
-    if (s > first && tiles * s > 2 * kSmCount) break;
-    const int64_t each = ceil_div(stages, s);
-    if (s > first && ceil_div(stages, each) != s) continue;  // (the last ones would have none)
-    const int64_t rounds = ceil_div(tiles * s, kSmCount), stage_bytes = kRows * ((int64_t)p.columns * item / p.k_tiles + 128 / p.n_tiles);
-    const int64_t stage = std::max<int64_t>(dtype == F2C_BF16 ? 560 : dtype == F2C_F32 ? 1200 : 900, std::min<int64_t>(tiles * s, kSmCount) * stage_bytes / 3500);
-    const int64_t cycles = rounds * (each * stage + 4000) + (s > 1 ? 4000 + tiles * s * 2 * tile_bytes / 4000 : 0);
-    if (cycles >= least) continue;
-    least = cycles;
+  const auto consider = [&](int64_t whole, int64_t s) {
+    const int64_t each = ceil_div(stages, s), rest = tiles - whole;
+    if (s > first && ceil_div(stages, each) != s) return;  // (the last ones would have none)
+    const int64_t stage_bytes = kRows * ((int64_t)p.columns * item / p.k_tiles + 128 / p.n_tiles);
+    const int64_t stage = std::max<int64_t>(dtype == F2C_BF16 ? 560 : dtype == F2C_F32 ? 1200 : 900, std::min<int64_t>(whole + rest * s, kSmCount) * stage_bytes / 3500);
+    const int64_t cycles = whole / kSmCount * (stages * stage + 4000) + ceil_div(rest * s, kSmCount) * (each * stage + 4000) + (s > 1 ? 4000 + rest * s * 2 * tile_bytes / 4000 : 0);
+    const int64_t cost = whole > 0 ? cycles + cycles / 8 : cycles;
+    if (cost >= least) return;
+    least = cost;
     p.split_rows = each * kRows;
     p.splits = (int)ceil_div(stages, each);
-  }
+    p.whole = (int)whole;
+    p.rest = (int)rest;
+  };
+  for (int64_t s = first; s <= std::min<int64_t>(stages, std::max<int64_t>(first, kSmCount)) && (s == first || tiles * s <= 2 * kSmCount); ++s) consider(0, s);
+  const int64_t whole = tiles / kSmCount * kSmCount;
+  if (first == 1 && whole >= p.n_tiles && whole < tiles)
+    for (int64_t s = 2; s <= stages && (tiles - whole) * s <= 4 * kSmCount; ++s) consider(whole, s);
   if (p.splits > 1) {
-    p.part_bytes = tiles * p.splits * tile_bytes;
-    p.sum_bytes = ceil_div((int64_t)p.splits * p.n_tiles * p.columns * 4, 256) * 256;
+    p.part_bytes = (int64_t)p.rest * p.splits * tile_bytes;
+    p.sum_bytes = p.whole > 0 ? 0 : ceil_div((int64_t)p.splits * p.n_tiles * p.columns * 4, 256) * 256;
   }
   p.bytes = p.part_bytes + p.sum_bytes;
   if (!aligned(dy, 16) || (m > 1 && ldy * item % 16 != 0)) {
@@ -677,8 +688,7 @@ static bool rows_map(CUtensorMap* map, const void* base, int64_t item, int64_t m
 
 template <typename T>
 static int run(const char* op, const CUtensorMap& dy, const CUtensorMap& codes, const Params& p, const Plan& how, cudaStream_t st) {
-  const int tiles = how.n_tiles * how.k_tiles;
-  const dim3 grid((unsigned)(tiles * how.splits));
+  const dim3 grid((unsigned)(how.whole + how.rest * how.splits));
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     if (const int rc = allow_smem(op, (const void*)rows_kernel, kWideSmem)) return rc;
     launch_dependent(rows_kernel, grid, kThreads, kWideSmem, st, dy, codes, p);
@@ -687,7 +697,7 @@ static int run(const char* op, const CUtensorMap& dy, const CUtensorMap& codes, 
     launch_dependent(scaled_kernel<T>, grid, kThreads, kTileSmem<T>, st, dy, codes, p);
   }
   if (how.splits > 1)
-    launch_dependent(join_kernel<T>, dim3((unsigned)(tiles * how.columns + how.n_tiles * how.columns / 32)), 32 * std::min(kJoinWarps, how.splits), 0, st, p, tiles);
+    launch_dependent(join_kernel<T>, dim3((unsigned)(how.rest * how.columns + (how.whole > 0 ? 0 : how.n_tiles * how.columns / 32))), 32 * std::min(kJoinWarps, how.splits), 0, st, p);
   return check_launch(op);
 }
 
@@ -738,7 +748,7 @@ extern "C" int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype
   }
   CUtensorMap maps[2] = {};
   F2C_REQUIRE(wg::rows_map(maps, dy, item, m, n, ldy) && wg::rows_map(maps + 1, codes, 1, m, k, ldq), F2C_ERR_CUDA, "%s: tensor map", op);
-  const wg::Params p{scales, ceil_div(k, ckpt::kGroup), m, (int)n, (int)k, how.n_tiles, how.splits, how.split_rows, dw, db, (float*)ws, (float*)(ws + how.part_bytes),
+  const wg::Params p{scales, ceil_div(k, ckpt::kGroup), m, (int)n, (int)k, how.n_tiles, how.splits, how.whole, how.rest, how.split_rows, dw, db, (float*)ws, (float*)(ws + how.part_bytes),
                      (flags & F2C_NO_WAITS) ? 0u : t5::kWaitLimit, stream_error_word()};
   if (dtype == F2C_F32) return wg::run<float>(op, maps[0], maps[1], p, how, st);
   if (dtype == F2C_F16) return wg::run<__half>(op, maps[0], maps[1], p, how, st);

@@ -41,7 +41,7 @@ def check(dy, c):
 
 @pytest.mark.parametrize("dtype", R.TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 128), (5, 3, 200), (31, 130, 16), (32, 128, 128), (33, 127, 129), (257, 64, 300), (1000, 172, 128), (1024, 172, 256), (4000, 41, 602),
-                                   (9000, 128, 128), (8200, 1, 128), (20000, 256, 256), (300, 1500, 1100), (2500, 2100, 1700)])
+                                   (9000, 128, 128), (8200, 1, 128), (20000, 256, 256), (300, 1500, 1100), (2500, 2100, 1700), (2001, 1700, 1665), (2100, 3350, 1700)])
 def test_gradients(m, n, k, dtype):
     x = matrix(m, k, dtype, seed=1).relu()
     x[:, ::3] -= 0.5  # groups whose lowest value is not zero
@@ -155,7 +155,7 @@ def test_the_same_bits_every_time_in_a_graph_and_beside_another():
 
 
 @pytest.mark.parametrize("dtype", R.TYPES)
-@pytest.mark.parametrize("m,n,k", [(5000, 128, 128), (300, 1500, 1500)])
+@pytest.mark.parametrize("m,n,k", [(5000, 128, 128), (300, 1500, 1500), (2000, 3400, 1700)])
 def test_waits_that_run_out_leave_nan_and_a_status(m, n, k, dtype):
     from f2cgt_b200 import _lib
     o = ops()
