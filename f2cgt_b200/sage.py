@@ -330,7 +330,7 @@ class _ReluBits(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return dy * ctx.saved_tensors[0]
+        return torch.where(ctx.saved_tensors[0], dy, 0.0)  # (as a product, an infinity at a closed place would be NaN)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -562,7 +562,8 @@ class Int8SAGE:
     """
 
     def __init__(self, model):
-        norms, embedding = model._modules.get("norms"), model._modules.get("embedding")
+        parts = getattr(model, "_modules", {})
+        norms, embedding = parts.get("norms"), parts.get("embedding")
         self.first_input = model.layers[0].sm if embedding is None else None
         self.layers, self.norms, self.embedding = [], None, None
         with torch.no_grad():

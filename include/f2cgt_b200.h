@@ -466,6 +466,7 @@ int f2c_checkpoint_values(const uint8_t* codes, int64_t ldq, const float* scales
 /* Gradient of a linear layer y = x W^T + b from dy [m, n] (`dtype`: F32, F16 or BF16, row stride ldy) and x [m, k] in 8 bits:
  *   dw [n, k] = dy^T x,  db [n] = the sums of dy's columns, both of `dtype`, rounded once; x is not written out.
  * dy times a code's step is held to 24 bits for F32 and to 16 for F16, x to 16 bits for BF16; sums are single precision in an order that the sizes decide.
+ * Where a row of dy or a group of x is not finite, neither are the results that it has a part in (NaN or infinities).
  * Codes as f2c_checkpoint_int8 leaves them (every row has whole 16 bytes).  m < 2^31 - 256, n and k up to 2^17.  flags: 0, or F2C_NO_WAITS.
  * workspace: f2c_checkpoint_weight_grad_workspace(...) bytes, 256-byte aligned; it depends on where dy starts and on its stride (rows that do not start on
  * 16 bytes are copied): ask with those of the call.  A bounded wait that runs out reports 8 and leaves NaN. */
@@ -492,7 +493,7 @@ int f2c_layer_norm_backward(const void* dy, int64_t ldy, int dtype, const void* 
 int f2c_embedding(const void* table, int64_t ld, int dtype, int64_t rows, int64_t d, const void* ids, int index_dtype, int64_t m, float scale, void* out, void* stream);
 /* The table's gradient: row r is scale times the sum of dy[i] over ids[i] = r.  Sums are single precision in an order that m and rows decide, rounded
  * once to `dtype`.  count NULL: grad [rows, d], zeros where nothing was looked up.  Otherwise only the rows that were: looked_up [m] (int64) their ids,
- * ascending, grad [m, d] their rows, count [1] (int64) how many; behind them looked_up is -1 and grad zero.
+ * ascending, grad [m, d] their rows, count [1] (int64) how many; behind them looked_up is -1 and grad zero (without columns: count 0).
  * workspace: f2c_embedding_backward_workspace(m, rows, d) bytes, 256-byte aligned. */
 int64_t f2c_embedding_backward_workspace(int64_t m, int64_t rows, int64_t d);
 int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, const void* ids, int index_dtype, int64_t m, int64_t rows, int64_t d, float scale, void* grad,

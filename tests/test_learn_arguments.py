@@ -95,3 +95,12 @@ def test_workspaces_of_weight_gradients():
     assert size(AT, 128, _lib.F32, 59_000, 128, 128) % (65536 + 512) == 0 and size(AT, 4096, _lib.BF16, 16_384, 4096, 4096) == 0
     # rows that do not start on 16 bytes are copied
     assert size(AT + 4, 128, _lib.F32, 32, 128, 128) == 32 * 512 and size(AT, 41, _lib.BF16, 100, 41, 128) >= 100 * 96 and size(AT, 41, _lib.F16, 1, 41, 16) == 0
+
+
+def test_relu_of_bits_keeps_infinities_where_it_is_open():
+    import torch
+    from f2cgt_b200 import sage
+    x = torch.tensor([-1.0, 2.0, 0.0, 3.0], requires_grad=True)
+    y = sage._ReluBits.apply(x)
+    y.backward(torch.tensor([float("inf"), float("inf"), float("nan"), -2.0]))
+    assert y.tolist() == [0.0, 2.0, 0.0, 3.0] and x.grad.tolist() == [0.0, float("inf"), 0.0, -2.0]
