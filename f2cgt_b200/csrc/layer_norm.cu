@@ -70,6 +70,11 @@ __device__ __forceinline__ f32x2 add_squares(const f32x2 (&x)[2], f32x2 less, in
   }
   return fma2(t[1], t[1], fma2(t[0], t[0], sum));
 }
+// 1 / sqrt(v), a step of Newton's behind the instruction's two units in the last place.  (With __frsqrt_rn, and the sum divided by the columns: 60 us instead of 54 at 16,384 x 4096.)
+__device__ __forceinline__ float rstd_of(float v) {
+  const float r = rsqrtf(v), off = fmaf(-(v * r), r, 1.0f);
+  return fabsf(off) < 1.0f ? fmaf(0.5f * r, off, r) : r;  // (v zero or infinite: as it is)
+}
 __device__ __forceinline__ float sum_of(f32x2 v) { return lo32(v) + hi32(v); }
 
 // Everything that a lane writes of four columns of a row, of which `left` exist; by whole warps.
@@ -145,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 3 : 2) warp_kernel(con
     const float mean = warp_sum(sum_of(sum)) * a.per_column;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) squares = add_squares(x[c], both(-mean), left_of(c), squares);
-    const float rstd = rsqrtf(fmaf(warp_sum(sum_of(squares)), a.per_column, a.eps));
+    const float rstd = rstd_of(fmaf(warp_sum(sum_of(squares)), a.per_column, a.eps));
     if (KEEP && lane == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
@@ -211,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, (KEEP ? 640 : 768) / THREADS) block_k
 #pragma unroll
     for (int k = 0; k < KEPT; ++k)
       if (k < mine) squares = add_squares(x[k], both(-mean), EVEN ? 4 : a.d - (warp + k * kWarps) * kGroup - 4 * lane, squares);
-    const float rstd = rsqrtf(fmaf(block_sum<THREADS>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
+    const float rstd = rstd_of(fmaf(block_sum<THREADS>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
     if (KEEP && threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
@@ -259,7 +264,7 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
   each([&](int, int, const f32x2 (&x)[2]) { sum = plus2(plus2(sum, x[0]), x[1]); });
   const float mean = block_sum<512>(sum_of(sum), of_warp[0]) * a.per_column;
   each([&](int, int col, const f32x2 (&x)[2]) { squares = add_squares(x, both(-mean), a.d - col, squares); });
-  const float rstd = rsqrtf(fmaf(block_sum<512>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
+  const float rstd = rstd_of(fmaf(block_sum<512>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
   if (KEEP && threadIdx.x == 0 && a.mean != nullptr) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
