@@ -108,9 +108,10 @@ __device__ __forceinline__ void finish(const Args& a, T* y, int64_t row, int chu
 
 constexpr int kThreads = 256;
 
-// ROWS rows of CHUNKS * 128 columns for every warp; the last chunk may have fewer, unless EVEN
+// ROWS rows of CHUNKS * 128 columns for every warp; the last chunk may have fewer, unless EVEN.  (Four CTAs an SM up to 640 columns, three beyond, though a few registers
+// spill: 16 M values with their codes, 256 columns 28 us and 31 with three, 768 columns 29 and 35 with two.)
 template <typename T, int ACCESS, int CHUNKS, int ROWS, bool EVEN, bool KEEP>
-__global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 3 : 2) warp_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 4 : 3) warp_kernel(const __grid_constant__ Args a) {
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31;
