@@ -9,7 +9,7 @@
 // the launches below 8.3 and 12.4 (rows alone), and 19 in a row of calls, whose launches the host makes.)
 //
 // More places of few rows (labels): a CTA sorts 400 places at most while their rows of dy come to its shared memory, and leaves a sum for every row of the table
-// that it met; a second launch adds those up in the CTAs' order.  59,000 x 128 of 172 rows: 14 us, 24 with all places sorted.
+// that it met; a second launch adds those up in the CTAs' order.  59,000 x 128 of 172 rows: 14 us, 24 with all places sorted (rows alone 20 and 27).
 //
 // Sorting.  Up to 4096 places each place counts the ones in front of it, in one launch: the keys are few enough that all pairs cost
 // less than further launches.  Beyond, digits of up to 11 bits from the lowest on: counts of every tile of 1024 places, their sums over tiles, and the
@@ -610,8 +610,8 @@ __global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict_
 // ---------------------------------------------------------------- few rows
 // A CTA has `each` places, 128 columns of them: it sorts them by row while they come to shared memory, and leaves a sum for every row that is among them.
 // (Places that need more than one CTA an SM: the sorting is not hidden any more, 236,000 of 1000 rows took 80 us and 68 with all of them sorted.  More rows
-// times pieces of 128 columns: as many CTAs join them, 6000 x 2048 of 3000 rows took 128 us and 37.)
-constexpr int kLabels = 2048, kLabelThreads = 512, kLabelWarps = kLabelThreads / 32, kMostPlaces = 400, kLeastPlaces = 32;
+// times pieces of 128 columns: as many CTAs join them, 2000 x 128 of 2000 rows took 16 us and 10, of 1000 rows 11 and 10.)
+constexpr int kLabels = 1024, kLabelThreads = 512, kLabelWarps = kLabelThreads / 32, kMostPlaces = 400, kLeastPlaces = 32;
 constexpr uint16_t kNoSlot = 0xffffu;
 static_assert(kLabels <= 1 << 22 && kMostPlaces < kLabelThreads, "a row and a place are one number of 32 bits, and none is the largest");
 static_assert(kSmCount <= kLabelThreads, "a thread has a CTA's slot");
@@ -622,6 +622,11 @@ struct Labels {
   int d, each, ctas, slots;
   float* part;      // [ctas][slots][width]
   uint16_t* where;  // [rows][ctas]: a row's slot
+  // only the rows that were looked up
+  int words;
+  uint32_t* seen;      // [words][ctas]: a bit for every row
+  int64_t* looked_up;  // null: the whole table
+  int64_t* count;
 };
 
 template <int BYTES>
@@ -717,18 +722,56 @@ __global__ void __launch_bounds__(kLabelThreads, 1) labels_kernel(const T* __res
       }
       __syncthreads();
     }
-  if (blockIdx.y == 0)
-    for (int r = i; r < (int)a.rows; r += kLabelThreads) a.where[(int64_t)r * a.ctas + blockIdx.x] = slot[r];
+  if (blockIdx.y != 0) return;
+  for (int r = i; r < 32 * a.words; r += kLabelThreads) {
+    const uint16_t s = r < (int)a.rows ? slot[r] : kNoSlot;
+    if (r < (int)a.rows) a.where[(int64_t)r * a.ctas + blockIdx.x] = s;
+    const uint32_t those = __ballot_sync(0xffffffffu, s != kNoSlot);
+    if (lane == 0 && a.looked_up != nullptr) a.seen[(r >> 5) * a.ctas + blockIdx.x] = those;
+  }
 }
 
-// A row's sums over the CTAs, in their order: a CTA to a row, 128 columns of it.
-template <typename T, int ACCESS>
-__global__ void __launch_bounds__(kLabelThreads) label_rows_kernel(float scale, const __grid_constant__ Labels a, T* __restrict__ out) {
+// A row's sums over the CTAs, in their order: a CTA to a row, 128 columns of it.  Where only the rows that were looked up are wanted (SOME) the CTAs behind those clear what
+// is behind the last of them.
+template <typename T, int ACCESS, bool SOME>
+__global__ void __launch_bounds__(kLabelThreads, 2) label_rows_kernel(float scale, const __grid_constant__ Labels a, T* __restrict__ out) {
   __shared__ __align__(16) float sums[kLabelWarps][kGroup];
-  __shared__ uint32_t list[kLabelThreads], before_warp[kLabelWarps];
+  __shared__ uint32_t list[kLabelThreads], before_warp[kLabelWarps], seen[SOME ? kLabels / 32 : 1];
   dependency_wait();
   release_dependents();
   const int i = threadIdx.x, lane = i & 31, warp = i >> 5, row = blockIdx.x, col = blockIdx.y * kGroup + 4 * lane;
+  int64_t to = row;
+  if constexpr (SOME) {
+    const int needed = row < (int)a.rows ? (row >> 5) + 1 : a.words;
+    for (int w = warp; w < needed; w += kLabelWarps) {
+      uint32_t any = 0u;
+      for (int c = lane; c < a.ctas; c += 32) any |= __ldg(a.seen + w * a.ctas + c);
+      any = __reduce_or_sync(0xffffffffu, any);
+      if (lane == 0) seen[w] = any;
+    }
+    __syncthreads();
+    uint32_t before = 0u, all = 0u;
+    for (int w = lane; w < needed; w += 32) {
+      all += __popc(seen[w]);
+      before += __popc(w < row >> 5 ? seen[w] : w == row >> 5 ? seen[w] & ((1u << (row & 31)) - 1u) : 0u);
+    }
+    to = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (row >= (int)a.rows) {
+      Four<T, ACCESS> zero;
+      const f32x2 none[2] = {};
+      zero.set(none);
+      const int cta = row - (int)a.rows, ctas = gridDim.x - (int)a.rows;
+      for (int64_t r = (int64_t)all + cta * kLabelWarps + warp; r < a.m; r += ctas * kLabelWarps) {
+        zero.store(out + r * a.d + col, a.d - col);
+        if (lane == 0 && blockIdx.y == 0) a.looked_up[r] = -1;
+      }
+      if (cta == 0 && blockIdx.y == 0 && i == 0) *a.count = all;
+      return;
+    }
+    if (((seen[row >> 5] >> (row & 31)) & 1u) == 0u) return;  // for all threads alike
+    if (i == 0 && blockIdx.y == 0) a.looked_up[to] = row;
+  }
   f32x2 acc[2] = {};
   const uint16_t slot = i < a.ctas ? __ldg(a.where + (int64_t)row * a.ctas + i) : kNoSlot;
   const uint32_t those = __ballot_sync(0xffffffffu, slot != kNoSlot);
@@ -760,7 +803,7 @@ __global__ void __launch_bounds__(kLabelThreads) label_rows_kernel(float scale, 
   acc[1] = mul2(acc[1], both(scale));
   Four<T, ACCESS> v;
   v.set(acc);
-  v.store(out + (int64_t)row * a.d + col, a.d - col);
+  v.store(out + to * a.d + col, a.d - col);
 }
 
 // ---------------------------------------------------------------- host
@@ -897,10 +940,12 @@ static Labels labels(int64_t m, int64_t rows, int64_t d) {
   a.each = (int)std::max<int64_t>(kLeastPlaces, ceil_div(m, kSmCount / slabs));
   a.ctas = (int)ceil_div(m, a.each);
   a.slots = (int)std::min<int64_t>(a.each, rows);
+  a.words = (int)ceil_div(rows, 32);
   return a;
 }
 static int64_t label_parts(const Labels& a) { return ceil_div((int64_t)a.ctas * a.slots * a.width * 4, 256) * 256; }
-static int64_t label_bytes(const Labels& a) { return label_parts(a) + ceil_div((int64_t)a.ctas * a.rows * 2, 256) * 256; }
+static int64_t label_slots(const Labels& a) { return ceil_div((int64_t)a.ctas * a.rows * 2, 256) * 256; }
+static int64_t label_bytes(const Labels& a) { return label_parts(a) + label_slots(a) + ceil_div((int64_t)a.ctas * a.words * 4, 256) * 256; }
 
 template <typename T, int ACCESS>
 static void add_labels(const char* op, const void* dy, int64_t ld, const void* ids, int index_dtype, const Labels& a, float scale, void* out, cudaStream_t st, int* rc) {
@@ -913,7 +958,9 @@ static void add_labels(const char* op, const void* dy, int64_t ld, const void* i
     if ((*rc = allow_smem(op, (const void*)labels_kernel<T, int32_t, ACCESS>, kMostPlaces * kGroup * (int)sizeof(T)))) return;
     launch_dependent(labels_kernel<T, int32_t, ACCESS>, grid, kLabelThreads, bytes, st, (const T*)dy, ld, (const int32_t*)ids, a);
   }
-  launch_dependent(label_rows_kernel<T, ACCESS>, dim3(a.rows, grid.y), kLabelThreads, 0, st, scale, a, (T*)out);
+  const unsigned more = a.looked_up == nullptr ? 0u : (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a.m, 8 * kLabelWarps), 2 * kSmCount / grid.y));
+  if (more == 0) launch_dependent(label_rows_kernel<T, ACCESS, false>, dim3(a.rows, grid.y), kLabelThreads, 0, st, scale, a, (T*)out);
+  else launch_dependent(label_rows_kernel<T, ACCESS, true>, dim3(a.rows + more, grid.y), kLabelThreads, 0, st, scale, a, (T*)out);
 }
 
 static int check(const char* op, int dtype, int index_dtype, int64_t m, int64_t rows, int64_t d) {
@@ -946,7 +993,8 @@ extern "C" int f2c_embedding(const void* table, int64_t ld, int dtype, int64_t r
 
 extern "C" int64_t f2c_embedding_backward_workspace(int64_t m, int64_t rows, int64_t d) {
   if (m <= 0 || rows < 0 || d <= 0 || m > emb::kMaxPlaces || rows > emb::kMaxRows || d > emb::kMaxColumns) return 0;
-  return std::max(emb::plan(m, rows, d).bytes, emb::label_bytes(emb::labels(m, rows, d)));
+  const emb::Labels few = emb::labels(m, rows, d);
+  return few.ctas > 0 ? emb::label_bytes(few) : emb::plan(m, rows, d).bytes;
 }
 
 extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, const void* ids, int index_dtype, int64_t m, int64_t rows, int64_t d, float scale, void* grad,
@@ -986,9 +1034,12 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
   }
   char* const ws = (char*)workspace;
   emb::Labels few = emb::labels(m, rows, d);
-  if (dense && few.ctas > 0) {
+  if (few.ctas > 0) {
     few.part = (float*)ws;
     few.where = (uint16_t*)(ws + emb::label_parts(few));
+    few.seen = (uint32_t*)(ws + emb::label_parts(few) + emb::label_slots(few));
+    few.looked_up = dense ? nullptr : looked_up;
+    few.count = count;
     int rc = F2C_OK;
     F2C_BY_ROWS(emb::add_labels, dtype, access, op, dy, ldy, ids, index_dtype, few, scale, grad, st, &rc);
     return rc != F2C_OK ? rc : check_launch(op);

@@ -80,6 +80,7 @@ def check_gradient(dy, ids, rows, scale):
     n = there.numel()
     assert looked_up.shape == (m,) and part.shape == (m, d) and int(count) == n
     assert torch.equal(looked_up[:n], there) and (looked_up[n:] == -1).all() and not part[n:].any()
+    assert torch.equal(part[:n], dense[there])
     R.near(part[:n], want[there] * by, (links * R.U * sizes[there] + 2 * R.U * want[there].abs()) * abs(by), dy.dtype)
     untouched = torch.ones(rows, dtype=torch.bool, device="cuda")
     untouched[there] = False
@@ -89,7 +90,7 @@ def check_gradient(dy, ids, rows, scale):
 
 @pytest.mark.parametrize("how", ["any", "one", "skew", "outside", "nowhere", "descending"])
 @pytest.mark.parametrize("m,rows,d", [(1, 1, 1), (1, 1000, 128), (7, 3, 5), (8, 8, 128), (33, 5, 130), (255, 3000, 64), (1024, 172, 128), (1024, 3, 4096), (1000, 100_000, 12), (1025, 172, 128), (4096, 100, 36), (4097, 100, 36),
-                                      (5000, 2047, 8), (5000, 2048, 8), (5000, 1024, 130), (5000, 1025, 130), (59001, 172, 128), (59200, 2048, 20), (59201, 2048, 20), (6400, 1, 1030), (1026, 9, 4100), (20000, 5_000_000, 4), (16385, 172, 260), (40001, 7, 128), (70000, 60000, 16)])
+                                      (5000, 2047, 8), (5000, 2048, 8), (5000, 512, 130), (5000, 513, 130), (59001, 172, 128), (59200, 1024, 20), (59201, 1024, 20), (59200, 1025, 20), (6400, 1, 1030), (1026, 9, 4100), (20000, 5_000_000, 4), (16385, 172, 260), (40001, 7, 128), (70000, 60000, 16)])
 def test_gradient(m, rows, d, how):
     dy = table_of(m, d, torch.float32, seed=2)
     check_gradient(dy, ids_of(m, rows, how), rows, 1.7)
