@@ -835,8 +835,8 @@ static Plan plan(int64_t m, int64_t rows, int64_t d) {
   p.m = m;
   p.d = d;
   if (m <= kOneLaunch) return p;
-  // Short stretches where there are few places: a stretch's rows are added one after the other.  Long ones where segments go over many of them: 59,000 places of
-  // 172 rows took 29.9 us in stretches of 32 and 32.0 of 16, 121,000 of 2.4 M rows 84.7 and 79.6.
+  // Short stretches where there are few places: a stretch's rows are added one after the other.  Long ones where segments go over many of them: 236,000 places of
+  // 172 rows took 69 us in stretches of 32 and 72 of 16, 121,000 of 2.4 M rows 84.7 and 79.6.
   p.stretch = m <= 16384 ? 8 : rows < m / 8 ? 32 : 16;
   p.tiles = (int)ceil_div(m, kTile);
   int bits = 1;

@@ -15,7 +15,7 @@
 // registers, while the MMAs go on in the other half of the accumulators; elsewhere every 16,384 rows (float16), and once a part of at most 65,536 rows.
 //
 // What bounds it: bfloat16 shared memory, from which a stage's operand is read twice while its codes and steps are read and the next stages arrive (16,384 x 2048 x
-// 4096: 478 us, 575 TFLOP/s of the product, 1150 of the MMAs; half the MMAs, or no reading of codes and steps, each took 20% off); float32 the instructions that
+// 4096: 490 us among other calls, 560 TFLOP/s of the product, 1120 of the MMAs, 420 by itself; half the MMAs, or no reading of codes and steps, each took 20% off); float32 the instructions that
 // split dy times the step, 650 a warp for a stage (4096 x 2048 x 1152: 74 us); few rows latency (59,000 x 128 x 128 float32: 17 us of 5.9 that memory takes).
 //
 // Many rows and few tiles: the rows are dealt out over all SMs; each leaves its part of the sums, and a second launch adds them up in their order.

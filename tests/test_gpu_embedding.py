@@ -159,6 +159,8 @@ def test_nothing():
     assert o.embedding_backward(torch.ones(2, 4, device="cuda"), ids, 0).shape == (0, 4)
     looked_up, rows, count = o.embedding_backward_rows(torch.ones(2, 4, device="cuda"), ids, 0)
     assert looked_up.tolist() == [-1, -1] and not rows.any() and int(count) == 0
+    looked_up, rows, count = o.embedding_backward_rows(torch.ones(5000, 4, device="cuda"), ids_of(5000, 3, "any"), 0)
+    assert (looked_up == -1).all() and not rows.any() and int(count) == 0
     looked_up, rows, count = o.embedding_backward_rows(torch.ones(2, 0, device="cuda"), ids, 5)
     assert int(count) == 0 and rows.shape == (2, 0)
 
