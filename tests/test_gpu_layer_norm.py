@@ -200,3 +200,37 @@ def test_refusals():
     with fwd.dual_level():
         with pytest.raises(RuntimeError, match="tangent"):
             o.layer_norm(fwd.make_dual(x, x))
+
+
+@pytest.mark.parametrize("m,d", [((1 << 21) + 3, 1100), ((1 << 25) + 3, 66)])
+def test_offsets_beyond_32_bits(m, d):
+    """More than 2^31 values, 2^32 bytes: the last rows are those of a call of their own."""
+    o = ops()
+    x = torch.zeros(m, d, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros(m, d, dtype=torch.bfloat16, device="cuda")
+    x[-300:], dy[-300:] = rows(300, d, torch.bfloat16, offset=0.5), rows(300, d, torch.bfloat16, seed=3)
+    w, b = vectors(d)
+    y, saved = o.layer_norm_train(x, w, b, relu=True, int8=True)
+    y_last, last = o.layer_norm_train(x[-300:], w, b, relu=True, int8=True)
+    assert torch.equal(y[-300:], y_last) and torch.equal(saved.x.codes[-300:], last.x.codes) and torch.equal(saved.x.scales[-300:], last.x.scales)
+    assert torch.equal(saved.mean[-300:], last.mean) and torch.equal(saved.rstd[-300:], last.rstd) and torch.equal(saved.active[-300:], last.active)
+    del y
+    dx, dw, db = o.layer_norm_backward(dy, saved, w)
+    dx_last, dw_last, db_last = o.layer_norm_backward(dy[-300:], last, w)
+    assert torch.equal(dx[-300:], dx_last) and not dx[:-300].any()
+    # the same 300 summands and zeros, added up in another order
+    h = (o.checkpoint_values(last.x).double() - last.mean.double()[:, None]) * last.rstd.double()[:, None]
+    assert ((dw - dw_last).abs() <= 2 * 303 * R.U * (dy[-300:].double() * h).abs().sum(0)).all() and ((db - db_last).abs() <= 2 * 303 * R.U * dy[-300:].double().abs().sum(0)).all()
+    del dx
+    kept = o.checkpoint_int8(x)
+    assert torch.equal(kept.codes[-300:], last.x.codes) and torch.equal(kept.scales[-300:], last.x.scales)
+    del x, saved
+    narrow = dy[:, :8].contiguous()
+    del dy
+    dweight, dbias = o.checkpoint_weight_grad(narrow, kept)
+    values, grads = o.checkpoint_values(last.x).double(), narrow[-300:].double()
+    # the values to 16 bits; the result and the sums of the last part's 300 rows
+    assert ((dweight.double() - grads.T @ values).abs() <= 2.0 ** -8 * (grads.T @ values).abs() + 2.0 ** -16 * grads.abs().T @ values.abs()).all()
+    assert ((dbias.double() - grads.sum(0)).abs() <= 2.0 ** -8 * grads.sum(0).abs() + 2.0 ** -16 * grads.abs().sum(0)).all()
+    values = o.checkpoint_values(kept, torch.bfloat16)
+    assert torch.equal(values[-300:], o.checkpoint_values(last.x, torch.bfloat16)) and not values[:-300].any()
