@@ -11,8 +11,10 @@
 //    float16, whose range bfloat16 has and float16 values of x might leave).  The second term is one number for every column of dy and group, summed in registers.  128
 //    columns of dy (the lanes) by a group.
 //
-// Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows.  So for float32 they are taken out every 256 rows and added up in
-// registers, while the MMAs go on in the other half of the accumulators; elsewhere every 16,384 rows (float16), and once a part of at most 65,536 rows.
+// Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows and all one way: 16,384 rows of bfloat16 lost 4e-5 of their sums, and so 4e-4 of
+// the norm of the rounded results.  So they are taken out and added up in single precision, every 256 rows (float32) or 16,384 (float16) in registers, while the MMAs go
+// on in the other half of the accumulators; for bfloat16, whose accumulators leave no room for a second half, every 2048 rows, in shared memory and TMEM, while the MMAs
+// wait (16,384 x 2048 x 4096, side by side: 488 us without, 495 every 4096 rows, 507 every 2048, 533 every 1024).
 //
 // What bounds it: bfloat16 shared memory, from which a stage's operand is read twice while its codes and steps are read and the next stages arrive (16,384 x 2048 x
 // 4096: 490 us among other calls, 560 TFLOP/s of the product, 1120 of the MMAs, 420 by itself; half the MMAs, or no reading of codes and steps, each took 20% off); float32 the instructions that
@@ -71,7 +73,7 @@ __device__ __forceinline__ void mma_f16_tmem(bool go, uint32_t d_tmem, uint32_t 
       "r"((uint32_t)go)
       : "memory");
 }
-// 16 or 8 columns of the 32 lanes that the warp owns
+// 32, 16 or 8 columns of the 32 lanes that the warp owns
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
@@ -80,6 +82,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+      "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -167,7 +178,7 @@ __device__ __forceinline__ void begin(Bars& bars, uint32_t empties) {
 }
 
 // The stages' loads, by a warp: `boxes` of dy, EACH columns apart, then the codes.
-template <int EACH>
+template <int STAGES, int EACH>
 __device__ __forceinline__ void load_stages(const CUtensorMap* dy, const CUtensorMap* codes, Bars& bars, uint32_t ring, uint32_t stage_bytes, uint32_t codes_at, int boxes, const Place& at,
                                             uint32_t& left, int& s, uint32_t& round) {
   const bool mine = elected() != 0u;
@@ -184,7 +195,7 @@ __device__ __forceinline__ void load_stages(const CUtensorMap* dy, const CUtenso
     expect_if(go, bars.full + s, (uint32_t)(boxes + 1) * kBox);
     for (int b = 0; b < boxes; ++b) tma_load(go, dy, stage + (uint32_t)b * kBox, bar, at.n0 + b * EACH, row);
     tma_load(go, codes, stage + codes_at, bar, at.group * kGroup, row);
-    if (++s == kStages) { s = 0; ++round; }
+    if (++s == STAGES) { s = 0; ++round; }
   }
 }
 
@@ -197,12 +208,13 @@ __device__ __forceinline__ bool settle(Bars& bars, uint32_t left) {
   return bars.failed != 0;
 }
 // The way out, after the last read of TMEM: when a wait has run out, what was issued is waited for (bounded) before TMEM is freed.
+template <int STAGES>
 __device__ __forceinline__ void leave(const Params& p, Bars& bars, bool lost, int s, uint32_t round) {
   const int wid = threadIdx.x >> 5;
   if (lost && p.tries != 0u) {
     uint32_t left = p.tries;
     if (wid == kWarps) {
-      for (int q = 0; q < kStages; ++q) {
+      for (int q = 0; q < STAGES; ++q) {
         const uint32_t uses = round + (q < s ? 1u : 0u);
         if (uses > 0) wait_bar(bars.full + q, (uses - 1) & 1, left);
       }
@@ -223,8 +235,9 @@ __device__ __forceinline__ void leave(const Params& p, Bars& bars, bool lost, in
 
 // ---------------------------------------------------------------- bfloat16: x decoded, in TMEM; dy as it is
 constexpr int kWide = 256;                                           // columns of dy in a tile
+constexpr int kWideTaken = 64;                                       // stages between two takings out
 constexpr uint32_t kWideStage = (kWide / 64 + 1) * kBox;             // four boxes of 64 columns, and the codes
-constexpr int kWideSmem = kStages * kWideStage + 1024;
+constexpr int kWideStages = 7, kWideSmem = kWideStages * kWideStage + 32 * 32 * kWarps * 4 + 1024;  // and sums that have been taken out
 
 __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant__ CUtensorMap dy, const __grid_constant__ CUtensorMap codes, const __grid_constant__ Params p) {
   extern __shared__ unsigned char smem_raw[];
@@ -239,19 +252,24 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
   uint32_t round = 0;
   begin(bars, 5);  // a stage is free when its MMAs are done and its group's warps have read it
   const uint32_t tmem = bars.tmem, ring = smem_u32(smem), a_tmem = tmem + kWide;
-  const int quarter = wid & 3, set = wid >> 2;
+  const int quarter = wid & 3, set = wid >> 2, takes = (at.stages + kWideTaken - 1) / kWideTaken;
+  // What has been taken out of a group's 64 columns of the accumulators: 32 in shared memory, four for all threads side by side, and 32 in the columns of TMEM that are left.
+  const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)set * 64, held = a_tmem + kGroups * 32 + ((uint32_t)(quarter * 32) << 16) + (uint32_t)set * 32;
+  float4* const sums = reinterpret_cast<float4*>(smem + kWideStages * kWideStage) + tid;
   f32x2 of_bias = 0ull;
   dependency_wait();
   release_dependents();
 
   if (wid == kWarps) {
-    load_stages<64>(&dy, &codes, bars, ring, kWideStage, (kWide / 64) * kBox, boxes, at, left, s, round);
+    load_stages<kWideStages, 64>(&dy, &codes, bars, ring, kWideStage, (kWide / 64) * kBox, boxes, at, left, s, round);
   } else if (wid == kWarps + 1) {
     // ================= MMAs
     const bool mine = elected() != 0u;
     const uint32_t idesc = instruction(kSumF32, kFormatBf16, 128, (uint32_t)(cols + 15) / 16 * 16) | kTurnedB, b_low = desc_low(ring, kBox);
     for (int i = 0; i < at.stages; ++i) {
-      const int slot = i % kGroups;
+      const int slot = i % kGroups, t = i / kWideTaken;
+      const bool starts = i % kWideTaken == 0;
+      if (starts && t > 0) wait_bar(bars.acc_empty, (t - 1) & 1, left);
       wait_bar(bars.full + s, round & 1, left);
       wait_bar(bars.ready + slot, (i / kGroups) & 1, left);
       fence_after();
@@ -259,15 +277,46 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
       const uint32_t b = b_low + (uint32_t)s * (kWideStage >> 4), a = a_tmem + (uint32_t)slot * 32;
 #pragma unroll
       for (uint32_t q = 0; q < kRows / 16; ++q) {
-        mma_f16_tmem(go, tmem, a + 8 * q, desc(b + q * kStepTurned), idesc, i != 0 || q != 0);
+        mma_f16_tmem(go, tmem, a + 8 * q, desc(b + q * kStepTurned), idesc, !starts || q != 0);
         mma_f16_tmem(go, tmem, a + 16 + 8 * q, desc(b + q * kStepTurned), idesc, true);
       }
       commit(go, bars.empty + s);
       commit(go, bars.taken + slot);
-      if (++s == kStages) { s = 0; ++round; }
+      if (i % kWideTaken == kWideTaken - 1 || i == at.stages - 1) commit(go, bars.acc_full);
+      if (++s == kWideStages) { s = 0; ++round; }
     }
-    commit(mine && left != 0u, bars.acc_full);
   } else {
+    const auto take = [&](int t) {  // sums out of TMEM
+      wait_bar(bars.acc_full, t & 1, left);
+      fence_after();
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint32_t r[32];
+        tmem_ld32(acc + 32 * part, r);
+        tmem_wait(r);
+        if (part == 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float4 v = t > 0 ? sums[j * 32 * kWarps] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v.x += __uint_as_float(r[4 * j]); v.y += __uint_as_float(r[4 * j + 1]); v.z += __uint_as_float(r[4 * j + 2]); v.w += __uint_as_float(r[4 * j + 3]);
+            sums[j * 32 * kWarps] = v;
+          }
+        } else {
+          if (t > 0) {
+            uint32_t before[32];
+            tmem_ld32(held, before);
+            tmem_wait(before);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(before[j]));
+          }
+          tmem_st32(held, r);
+        }
+      }
+      tmem_st_wait();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(bars.acc_empty);
+    };
     // ================= x as two bfloat16 numbers: a column a thread, a stage a group
     const int c = quarter * 32 + lane;
     uint32_t column[8];  // of row j of eight, in the 128-byte swizzle
@@ -276,12 +325,12 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
     const uint32_t to = a_tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)set * 32;
     Scales scale;
     scale.fetch(p, at.row0, at.rows, set, at.group);
-    int use = 0;
+    int use = 0, taken = 0;
     for (int i = set; i < at.stages; i += kGroups, ++use) {
-      s = i % kStages;
+      s = i % kWideStages;
       scale.tell(scales_s[wid]);
       scale.fetch(p, at.row0, at.rows, i + kGroups, at.group);
-      wait_bar(bars.full + s, (uint32_t)(i / kStages) & 1, left);
+      wait_bar(bars.full + s, (uint32_t)(i / kWideStages) & 1, left);
       const uint32_t stage = (uint32_t)s * kWideStage;
       uint32_t q[kRows];
 #pragma unroll
@@ -318,17 +367,41 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
       fence_before();
       __syncwarp();
       if (lane == 0) arrive(bars.ready + set);
+      // sums of stages that were handed over a round ago
+      if ((taken + 1) * kWideTaken <= i) take(taken++);
     }
-    wait_bar(bars.acc_full, 0, left);
+    while (taken + 1 < takes) take(taken++);
+    wait_bar(bars.acc_full, (takes - 1) & 1, left);
   }
   const bool lost = settle(bars, left);
   if (wid < kWarps) {  // a group has 64 columns of dy, a thread a column of x
     const float none = lost ? __int_as_float(0x7fffffff) : 0.0f;
     const int x_col = at.group * kGroup + quarter * 32 + lane;
-    for (int c0 = set * 64; c0 < min(cols, set * 64 + 64); c0 += 32) {
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const int c0 = set * 64 + 32 * part;
+      if (c0 >= cols) break;
       uint32_t r[32];
-      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0, r);
+      tmem_ld32(acc + 32 * part, r);
       tmem_wait(r);
+      if (takes > 1) {  // and what has been taken out before
+        if (part == 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 v = sums[j * 32 * kWarps];
+            r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) + v.x);
+            r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) + v.y);
+            r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) + v.z);
+            r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) + v.w);
+          }
+        } else {
+          uint32_t before[32];
+          tmem_ld32(held, before);
+          tmem_wait(before);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(before[j]));
+        }
+      }
       if (at.part >= 0) {
         float4* const out = reinterpret_cast<float4*>(p.part) + (int64_t)at.part * (kWide * 128 / 4) + c0 / 4 * 128 + quarter * 32 + lane;
 #pragma unroll
@@ -342,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant
       }
     }
   }
-  leave(p, bars, lost, s, round);
+  leave<kWideStages>(p, bars, lost, s, round);
   if (at.group != 0) return;
   float* const columns = reinterpret_cast<float*>(smem);  // [group][256]: the ring is free
   if (wid < kWarps) *reinterpret_cast<f32x2*>(columns + set * kWide + quarter * 64 + 2 * lane) = of_bias;
@@ -396,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
   release_dependents();
 
   if (wid == kWarps) {
-    load_stages<kEach>(&dy, &codes, bars, ring, kStage, kCodesAt, boxes, at, left, s, round);
+    load_stages<kStages, kEach>(&dy, &codes, bars, ring, kStage, kCodesAt, boxes, at, left, s, round);
   } else if (wid == kWarps + 1) {
     // ================= MMAs
     const bool mine = elected() != 0u;
@@ -520,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
     while (taken < takes) take(taken++);
   }
   const bool lost = settle(bars, left);
-  leave(p, bars, lost, s, round);
+  leave<kStages>(p, bars, lost, s, round);
   float(*const columns)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(smem);  // [group]: the ring is free, and behind them for the tile
   if (wid < kWarps) {
     columns[set][0][quarter * 32 + lane] = lo32(of_low) + hi32(of_low);

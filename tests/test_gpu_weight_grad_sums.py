@@ -1,0 +1,72 @@
+"""Sums of checkpoint_weight_grad over many rows: what the tensor cores' accumulators cut off is bounded by the rows between two takings out, not by all rows.
+
+S is the sum of |dy||x|.  An accumulator takes two products of 16 rows each (three beside float32), each of which leaves at most 2^-23 of the sizes that it adds;
+what is taken out is added up in single precision."""
+import pytest
+import torch
+
+import learn_reference as R
+
+pytestmark = pytest.mark.gpu
+
+TAKEN = {torch.float32: 256, torch.float16: 1024, torch.bfloat16: 2048}  # rows between two takings out
+CUTS = {torch.float32: 3 / 16, torch.float16: 2 / 16, torch.bfloat16: 2 / 16}  # a row
+# what the operands are rounded to, of one product: dy times the step to single precision, and to two numbers of eight bits; x to two such, and to single precision
+OPERANDS = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -18 + 2.0 ** -24, torch.bfloat16: 2.0 ** -18 + 2.0 ** -24}
+
+
+def ops():
+    from f2cgt_b200 import ops
+    return ops
+
+
+def positive(m, d, dtype, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.rand(m, d, generator=g, device="cuda").add_(0.5).to(dtype)
+
+
+def half_step(value, dtype):
+    """Half the distance between the type's numbers around a value (normal ones)."""
+    digits = {torch.float32: 24, torch.float16: 11, torch.bfloat16: 8}[dtype]
+    return torch.ldexp(torch.ones_like(value), torch.frexp(value).exponent - digits - 1)
+
+
+def rounded_once(got, want, off):
+    """Half a step of the type, exactly, and what the sum is off (1 % for what is of second order)."""
+    bad = ~((got.double() - want).abs() <= half_step(want, got.dtype) + 1.01 * off)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, by up to {float(((got.double() - want).abs() - half_step(want, got.dtype))[bad].max() / want.abs().max()):.3g} more than a rounding"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("m", [65536, 70_000, 9000])
+def test_summands_of_one_sign(m, dtype):
+    """148 tiles, one of each an SM, whose rows are not split but beyond 65,536: every sum is rounded once to the type, and is off by the cuts between two
+    takings out, the operands' roundings and an addition a taking out.  (Cut over all rows, sums of 9000 were 4e-5 off.)"""
+    n, k = 148 // 37 * (256 if dtype is torch.bfloat16 else 128), 37 * 128
+    x, dy = positive(m, k, dtype, 1), positive(m, n, dtype, 2)
+    c = ops().checkpoint_int8(x)
+    del x
+    dw, db = ops().checkpoint_weight_grad(dy, c)
+    want = dy.double().t() @ R.decode(c.codes, c.scales)
+    relative = CUTS[dtype] * min(m, TAKEN[dtype]) * 2.0 ** -23 + OPERANDS[dtype] + (m / TAKEN[dtype] + 4) * R.U
+    rounded_once(dw, want, relative * want)
+    R.near(db, dy.double().sum(0), (m / 32 + 24 + 160) * R.U * dy.double().sum(0), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("m", [2047, 2048, 2049, 2081, 4096, 4129, 10_000])
+def test_rows_around_a_taking_out(m, dtype):
+    """Whole numbers below 2^24 are exact however the rows fall into takings out: codes with a step of one and dy of -1, 0 and 1, the columns of dy and of x odd in number."""
+    n, k = 4 * 256 - 3, 37 * 128 - 5
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m)
+    codes = torch.randint(0, 256, (m, (k + 15) // 16 * 16), generator=g, device="cuda", dtype=torch.uint8)[:, :k]
+    scales = torch.ones(m, (k + 127) // 128, 2, device="cuda")
+    scales[:, :, 1] = -100.0 * torch.randint(0, 2, scales.shape[:2], generator=g, device="cuda")
+    dy = torch.randint(-1, 2, (m, n), generator=g, device="cuda").to(dtype)
+    want = dy.double().t() @ R.decode(codes, scales)
+    dw, db = ops().checkpoint_weight_grad(dy, ops().Int8Checkpoint(codes, scales))
+    assert torch.equal(dw, want.to(dtype)) and torch.equal(db, dy.double().sum(0).to(dtype))
+    again = ops().checkpoint_weight_grad(dy, ops().Int8Checkpoint(codes, scales))
+    assert torch.equal(again[0], dw) and torch.equal(again[1], db)
