@@ -227,13 +227,13 @@ __device__ __forceinline__ uint32_t encode(const f32x2 (&given)[2], int left, Sc
   return codes_of(x, left, r.s, r.by, r.plain);
 }
 
-// The codes as numbers: 2^23 + q, less 2^23.
-__device__ __forceinline__ void numbers_of(uint32_t codes, f32x2 (&q)[2]) {
-  q[0] = plus2(pair_of(__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7441))), both(-8388608.0f));
-  q[1] = plus2(pair_of(__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7443))), both(-8388608.0f));
+// The codes as numbers: 2^23 + q, and -2^23 (or another number that leaves whole ones).
+__device__ __forceinline__ void numbers_of(uint32_t codes, f32x2 less, f32x2 (&q)[2]) {
+  q[0] = plus2(pair_of(__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7441))), less);
+  q[1] = plus2(pair_of(__uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(codes, 0x4B000000u, 0x7443))), less);
 }
 __device__ __forceinline__ void decode(uint32_t codes, Scale s, f32x2 (&x)[2]) {
-  numbers_of(codes, x);
+  numbers_of(codes, both(-8388608.0f), x);
 #pragma unroll
   for (int h = 0; h < 2; ++h) x[h] = fma2(both(s.step), x[h], both(s.low));
 }

@@ -6,10 +6,12 @@
 //
 //  * bfloat16 dy (rows_kernel).  dy is an operand as it is.  x is two bfloat16 numbers, 16 bits, of a product that is rounded to 8: two MMAs of
 //    128 columns of x (the lanes of TMEM) by 256 of dy for every 16 rows.
-//  * float32 and float16 dy (scaled_kernel).  With the factors taken to the other side, dW = (step dy)^T q + (low dy)^T 1: the codes 0 .. 255 are
-//    bfloat16 numbers as they are, and step dy, rounded to single precision, is a sum of three of them (its 24 bits, eight each; float32) or two (16 bits;
-//    float16, whose range bfloat16 has and float16 values of x might leave).  The second term is one number for every column of dy and group, summed in registers.  128
-//    columns of dy (the lanes) by a group.
+//  * float32 and float16 dy (scaled_kernel).  With the factors taken to the other side, dW = (step dy)^T (q - z) + (base dy)^T 1, base = low + step z: differences of
+//    codes, -255 .. 255, are bfloat16 numbers as they are, and step dy, rounded to single precision, is a sum of three of them (its 24 bits, eight each; float32) or two
+//    (16 bits; float16, whose range bfloat16 has and float16 values of x might leave).  The second term is one number for every column of dy and group, summed in
+//    registers.  z is the code nearest to a value of zero: then no |base| is more than |x|, and no step |q - z| more than 2 |x|, so that neither sum is large where the result is
+//    not.  (With z = 0 both had the size of the groups' ranges and cancelled, and a small value beside large ones lost most of its digits; 16,384 x 1700 x 1700 float32
+//    358 us so and 368 with z.)  128 columns of dy (the lanes) by a group.
 //
 // Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows and all one way: 16,384 rows of bfloat16 lost 4e-5 of their sums, and so 4e-4 of
 // the norm of the rounded results.  So they are taken out and added up in single precision, every 256 rows (float32) or 16,384 (float16) in registers, while the MMAs go
@@ -140,6 +142,17 @@ struct Scales {
     __syncwarp();  // (the ones before have been read)
     mine[lane] = __uint_as_float(next.x);
     mine[32 + lane] = __uint_as_float(next.y);
+    __syncwarp();
+  }
+  // [steps of 32 rows][values of the codes z nearest to zero][2^23 + z]
+  __device__ __forceinline__ void tell_about_zero(float* mine) const {
+    const int lane = threadIdx.x & 31;
+    const float step = __uint_as_float(next.x), low = __uint_as_float(next.y);
+    const float z = fminf(fmaxf(rintf(__fdividef(-low, step)), 0.0f), 255.0f);  // (any code is right; 0 where there is no quotient)
+    __syncwarp();
+    mine[lane] = step;
+    mine[32 + lane] = fmaf(step, z, low);
+    mine[64 + lane] = 8388608.0f + z;
     __syncwarp();
   }
 };
@@ -451,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
   constexpr uint32_t kStage = Kind<T>::kStage, kCodesAt = kStage - kBox;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Bars bars;
-  __shared__ __align__(16) float scales_s[kWarps][64];
+  __shared__ __align__(16) float scales_s[kWarps][96];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
   const Place at(p, kTile);
@@ -462,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
   begin(bars, 4);  // a stage is free when its group's warps have read it
   const uint32_t tmem = bars.tmem, ring = smem_u32(smem), q_ring = ring + kStages * kStage, a_tmem = tmem + 2 * kTile;
   const int quarter = wid & 3, set = wid >> 2;
-  f32x2 sum[16], of_low = 0ull, of_bias = 0ull;
+  f32x2 sum[16], of_base = 0ull, of_bias = 0ull;
 #pragma unroll
   for (int j = 0; j < 16; ++j) sum[j] = 0ull;
   dependency_wait();
@@ -519,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
     int use = 0, taken = 0;
     for (int i = set; i < at.stages; i += kGroups, ++use) {
       s = i % kStages;
-      scale.tell(scales_s[wid]);
+      scale.tell_about_zero(scales_s[wid]);
       scale.fetch(p, at.row0, at.rows, i + kGroups, at.group);
       wait_bar(bars.full + s, (uint32_t)(i / kStages) & 1, left);
       const uint32_t stage = (uint32_t)s * kStage;
@@ -548,8 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
           const float4 step = *reinterpret_cast<const float4*>(step_of + r), base = *reinterpret_cast<const float4*>(step_of + 32 + r);
-          of_low = fma2(pair_of(base.x, base.y), d[r / 2], of_low);
-          of_low = fma2(pair_of(base.z, base.w), d[r / 2 + 1], of_low);
+          of_base = fma2(pair_of(base.x, base.y), d[r / 2], of_base);
+          of_base = fma2(pair_of(base.z, base.w), d[r / 2 + 1], of_base);
           d[r / 2] = mul2(pair_of(step.x, step.y), d[r / 2]);
           d[r / 2 + 1] = mul2(pair_of(step.z, step.w), d[r / 2 + 1]);
         }
@@ -568,16 +581,17 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
           tmem_st8(to + 16 * piece + 8 * half, w);
         }
       }
+      const f32x2 zero = both(-scales_s[wid][64 + q_row]);
 #pragma unroll
       for (uint32_t h = 0; h < 2; ++h) {  // 16 codes
         const uint4 q = lds_u128(ring + stage + kCodesAt + q_row * 128 + (((q_part * 2 + h) ^ (q_row & 7)) << 4));
         const uint32_t box = q_ring + (uint32_t)set * kCodesBytes + (q_part >> 1) * kBox + q_row * 128, first = (q_part & 1) * 4 + 2 * h;
         f32x2 a[2], b[2];
-        ckpt::numbers_of(q.x, a);
-        ckpt::numbers_of(q.y, b);
+        ckpt::numbers_of(q.x, zero, a);
+        ckpt::numbers_of(q.y, zero, b);
         sts_u128(box + ((first ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
-        ckpt::numbers_of(q.z, a);
-        ckpt::numbers_of(q.w, b);
+        ckpt::numbers_of(q.z, zero, a);
+        ckpt::numbers_of(q.w, zero, b);
         sts_u128(box + (((first + 1) ^ (q_row & 7)) << 4), pack_bf16(a[0]), pack_bf16(a[1]), pack_bf16(b[0]), pack_bf16(b[1]));
       }
       __syncwarp();
@@ -596,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) scaled_kernel(const __grid_consta
   leave<kStages>(p, bars, lost, s, round);
   float(*const columns)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(smem);  // [group]: the ring is free, and behind them for the tile
   if (wid < kWarps) {
-    columns[set][0][quarter * 32 + lane] = lo32(of_low) + hi32(of_low);
+    columns[set][0][quarter * 32 + lane] = lo32(of_base) + hi32(of_base);
     columns[set][1][quarter * 32 + lane] = lo32(of_bias) + hi32(of_bias);
   }
   __syncthreads();

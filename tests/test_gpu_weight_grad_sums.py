@@ -70,3 +70,57 @@ def test_rows_around_a_taking_out(m, dtype):
     assert torch.equal(dw, want.to(dtype)) and torch.equal(db, dy.double().sum(0).to(dtype))
     again = ops().checkpoint_weight_grad(dy, ops().Int8Checkpoint(codes, scales))
     assert torch.equal(again[0], dw) and torch.equal(again[1], db)
+
+
+def parts(c, dy):
+    """x, the sum's sizes S, and those of its two parts when the code nearest to zero is the origin: no more than S and twice S."""
+    x, d = R.decode(c.codes, c.scales), dy.double().abs()
+    step, low = (c.scales[:, :, i].double().repeat_interleave(128, 1)[:, :x.shape[1]] for i in (0, 1))
+    zero = torch.round(-low / step).clamp(0, 255)
+    whole, base, coded = d.t() @ x.abs(), d.t() @ (low + step * zero).abs(), d.t() @ (step * (c.codes.double() - zero)).abs()
+    assert (base <= 1.01 * whole).all() and (coded <= 2.01 * whole).all()
+    return x, whole, base, coded
+
+
+def check_about_zero(dy, c):
+    """Against sums in 64 bits, by the sizes of what is added up: takings out and their sum, and up to 160 parts; base times dy a thread's chain of a quarter of an eighth of the rows."""
+    dtype, m = dy.dtype, dy.shape[0]
+    x, whole, base, coded = parts(c, dy)
+    dw, _ = ops().checkpoint_weight_grad(dy, c)
+    if dtype is torch.bfloat16:
+        coded, base = whole, 0 * whole
+    off = (CUTS[dtype] * min(m, TAKEN[dtype]) * 2.0 ** -23 + OPERANDS[dtype]) * coded + (m / TAKEN[dtype] + 160) * R.U * (coded + base) + (m / 32 + 24) * R.U * base
+    R.near(dw, dy.double().t() @ x, off, dtype)
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+def test_small_values_beside_large_ones_of_both_signs(dtype):
+    """Two columns of every group 128 and -127 steps from zero, the others none or one: the sums of the others have the size of a step, whatever the range of their groups."""
+    m, n, k = 16_384, 100, 256
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    x = torch.randint(-1, 2, (m, k), generator=g, device="cuda").float()
+    x[:, ::128], x[:, 1::128] = 128, -127
+    x *= 0.1 + torch.rand(m, 1, generator=g, device="cuda")
+    check_about_zero(positive(m, n, dtype, 6) / 64, ops().checkpoint_int8(x.to(dtype)))
+
+
+@pytest.mark.parametrize("shift", [0.0, 0.7, 30.0, -30.0])
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("m,n,k", [(16_384, 100, 200), (3000, 1300, 1400), (70, 128, 128), (1, 5, 300)])
+def test_both_signs_and_one_sign_far_away(m, n, k, dtype, shift):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    x = torch.randn(m, k, generator=g, device="cuda") + shift
+    check_about_zero(positive(m, n, dtype, 8) / 64, ops().checkpoint_int8(x.to(dtype)))
+
+
+def test_groups_of_equal_values_and_of_none():
+    """No step: the value is the base.  A step beside which zero has no code: the nearest one."""
+    x = torch.full((500, 300), -3.25, device="cuda")
+    x[::2] = 0
+    x[1::4, 128:] = 1e-40
+    x[3::4, 256:] = 1e30
+    dy = positive(500, 40, torch.float32, 9)
+    dw, _ = ops().checkpoint_weight_grad(dy, ops().checkpoint_int8(x))
+    R.near(dw, dy.double().t() @ x.double(), (500 / 32 + 200) * R.U * (dy.double().abs().t() @ x.double().abs()))
