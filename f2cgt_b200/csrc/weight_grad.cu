@@ -14,9 +14,9 @@
 //    358 us so and 368 with z.)  128 columns of dy (the lanes) by a group.
 //
 // Sums.  The tensor cores cut sums off instead of rounding them, for every 16 rows and all one way: 16,384 rows of bfloat16 lost 4e-5 of their sums, and so 4e-4 of
-// the norm of the rounded results.  So they are taken out and added up in single precision, every 256 rows (float32) or 16,384 (float16) in registers, while the MMAs go
-// on in the other half of the accumulators; for bfloat16, whose accumulators leave no room for a second half, every 2048 rows, in shared memory and TMEM, while the MMAs
-// wait (16,384 x 2048 x 4096, side by side: 488 us without, 495 every 4096 rows, 507 every 2048, 533 every 1024).
+// the norm of the rounded results.  So they are taken out and added up in single precision, every 256 rows (float32) or 1024 (float16; 16,384 x 1700 x 1700 401 us, and
+// 395 every 16,384) in registers, while the MMAs go on in the other half of the accumulators; for bfloat16, whose accumulators leave no room for a second half, every
+// 2048 rows, in shared memory and TMEM, while the MMAs wait (16,384 x 2048 x 4096, side by side: 488 us without, 495 every 4096 rows, 507 every 2048, 533 every 1024).
 //
 // What bounds it: bfloat16 shared memory, from which a stage's operand is read twice while its codes and steps are read and the next stages arrive (16,384 x 2048 x
 // 4096: 490 us among other calls, 560 TFLOP/s of the product, 1120 of the MMAs, 420 by itself; half the MMAs, or no reading of codes and steps, each took 20% off); float32 the instructions that
@@ -453,7 +453,7 @@ template <> struct Kind<float> {
   static constexpr uint32_t kStage = 5 * kBox;
 };
 template <> struct Kind<__half> {
-  static constexpr int kPieces = 2, kTaken = 512, kEach = 64;
+  static constexpr int kPieces = 2, kTaken = 32, kEach = 64;
   static constexpr uint32_t kStage = 3 * kBox;
 };
 template <typename T> constexpr int kTileSmem = kStages * Kind<T>::kStage + kGroups * kCodesBytes + 1024;
