@@ -1,11 +1,18 @@
 // Layer norm of rows, forward (f2c_layer_norm): y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps), with or without
 // ReLU; for training also mean, rstd, the ReLU's bits, and the rows in 8 bits (checkpoint.cuh), all of it in the one pass.
 //
-// Bound by reading and writing the rows (16,384 x 4096 bfloat16: 52 us, 5.2 TB/s; 59,000 x 128 float32: 12 us, 5.0 TB/s).  A row's values stay in registers between the mean, the squares of the differences from it (no
-// cancellation of large means) and the result: a warp has rows up to 1024 columns long, several at a time where they are short so that enough loads are on
-// the way; a CTA of four warps (eight beyond 4096 columns) has longer ones, one after the other, the next one's loads on the way: five or six of them to an SM
-// (two of eight warps, their columns' weights in registers, waited more than they worked: 16,384 x 4096 bfloat16 64 us); rows beyond 8192 columns it reads
-// again for every step.
+// Bound by reading and writing the rows (16,384 x 4096 bfloat16: 53 us, 5.1 TB/s; 59,000 x 128 float32: 9.2 us, 6.6 TB/s, half of it from L2).  A row's values stay in registers
+// between the mean, the differences from it and their squares, and the result.
+//
+// Large means.  The sum and its division by the columns lose some last places of the mean, which every difference then has too: rows of nothing but 1000.3 came out 0.02
+// from their bias, with eps 1e-5, and rows of -3e4 +- 0.01 0.07.  The mean of the differences is what was lost: the result, the variance and the mean that is kept are
+// corrected by it.  (8 % of the time: 48.2 and 8.3 us without.  Only for rows whose mean is large it took 51.8 and 8.8, and 32.6 instead of 32.0 with codes, 62,500 x 256
+// float32: not worth results that depend on a limit.)  The mean that is kept is rounded to single precision, and the backward pass starts from it.
+//
+// A warp has rows up to 1024 columns long, several at a time where they are short so that enough loads are on the way; a CTA of four warps (eight beyond 4096 columns)
+// has longer ones, one after the other, the next one's loads on the way: five or six of them to an SM (two of eight warps, their columns' weights in registers, waited more
+// than they worked: 16,384 x 4096 bfloat16 64 us); rows beyond 8192 columns it reads again for every step (4000 x 16,384 bfloat16 116 us; with a few registers more, and one
+// CTA less an SM, 135).
 #include "checkpoint.cuh"
 
 namespace f2c {
@@ -39,6 +46,14 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float2 warp_sum(float2 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  return v;
+}
 
 // Four values of a vector, at `w` those of this lane's first columns (null: `otherwise`), where all four exist and start on 16 bytes
 __device__ __forceinline__ void of_columns(const float* w, float otherwise, f32x2 (&v)[2]) {
@@ -61,14 +76,16 @@ __device__ __forceinline__ void of_columns(const float* w, int at, int left, flo
   v[1] = pair_of(f.z, f.w);
 }
 
-// Squares of the differences from the mean, of the columns that there are.
-__device__ __forceinline__ f32x2 add_squares(const f32x2 (&x)[2], f32x2 less, int left, f32x2 sum) {
+// The differences from the mean and their squares, of the columns that there are.
+struct Spread { f32x2 off = 0ull, squares = 0ull; };
+__device__ __forceinline__ void add_spread(const f32x2 (&x)[2], f32x2 less, int left, Spread& sum) {
   f32x2 t[2] = {plus2(x[0], less), plus2(x[1], less)};
   if (left < 4) {
     t[0] = left > 1 ? t[0] : left > 0 ? pair_of(lo32(t[0]), 0.0f) : 0ull;
     t[1] = left > 2 ? pair_of(lo32(t[1]), 0.0f) : 0ull;
   }
-  return fma2(t[1], t[1], fma2(t[0], t[0], sum));
+  sum.off = plus2(plus2(sum.off, t[0]), t[1]);
+  sum.squares = fma2(t[1], t[1], fma2(t[0], t[0], sum.squares));
 }
 // 1 / sqrt(v), a step of Newton's behind the instruction's two units in the last place.  (With __frsqrt_rn, and the sum divided by the columns: 60 us instead of 54 at 16,384 x 4096.)
 __device__ __forceinline__ float rstd_of(float v) {
@@ -77,14 +94,28 @@ __device__ __forceinline__ float rstd_of(float v) {
 }
 __device__ __forceinline__ float sum_of(f32x2 v) { return lo32(v) + hi32(v); }
 
+// What a row's values are normalised by: the mean as the sum gave it, what it is off, and the reciprocal deviation.
+struct Norm {
+  float mean, off, rstd;
+  // from the sums of the differences and of their squares
+  __device__ __forceinline__ Norm(const Args& a, float mean, float2 sums) : mean(mean), off(sums.x * a.per_column) {
+    const float variance = fmaf(-off, off, sums.y * a.per_column);
+    rstd = rstd_of((variance < 0.0f ? 0.0f : variance) + a.eps);  // (a NaN stays one)
+  }
+  __device__ __forceinline__ void keep(const Args& a, int64_t row) const {
+    a.mean[row] = mean + off;
+    a.rstd[row] = rstd;
+  }
+};
+
 // Everything that a lane writes of four columns of a row, of which `left` exist; by whole warps.
 // KEEP: with what is wanted for the backward pass beside the result.
 template <typename T, int ACCESS, bool KEEP>
-__device__ __forceinline__ void finish(const Args& a, T* y, int64_t row, int chunk, int left, const f32x2 (&x)[2], float mean, float rstd, const f32x2 (&w)[2], const f32x2 (&b)[2]) {
+__device__ __forceinline__ void finish(const Args& a, T* y, int64_t row, int chunk, int left, const f32x2 (&x)[2], const Norm& n, const f32x2 (&w)[2], const f32x2 (&b)[2]) {
   const int lane = threadIdx.x & 31, col = chunk * kGroup + 4 * lane;
   f32x2 z[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) z[h] = fma2(mul2(plus2(x[h], both(-mean)), both(rstd)), w[h], b[h]);
+  for (int h = 0; h < 2; ++h) z[h] = fma2(fma2(plus2(x[h], both(-n.mean)), both(n.rstd), both(-n.off * n.rstd)), w[h], b[h]);
   if (KEEP && a.active != nullptr) {
     uint32_t bits = (lo32(z[0]) > 0.0f) | (hi32(z[0]) > 0.0f) << 1 | (lo32(z[1]) > 0.0f) << 2 | (hi32(z[1]) > 0.0f) << 3;
     if (left < 4) bits &= (1u << max(left, 0)) - 1u;
@@ -142,29 +173,27 @@ __global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 4 : 3) warp_kernel(con
   for (int r = 0; r < ROWS; ++r) {
     const int64_t row = first + r;
     if (row >= a.m) return;  // all threads of the warp
-    f32x2 x[CHUNKS][2], sum = 0ull, squares = 0ull;
+    f32x2 x[CHUNKS][2], sum = 0ull;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       raw[r][c].get(x[c]);
       sum = plus2(plus2(sum, x[c][0]), x[c][1]);
     }
     const float mean = warp_sum(sum_of(sum)) * a.per_column;
+    Spread spread;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) squares = add_squares(x[c], both(-mean), left_of(c), squares);
-    const float rstd = rstd_of(fmaf(warp_sum(sum_of(squares)), a.per_column, a.eps));
-    if (KEEP && lane == 0 && a.mean != nullptr) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
-    }
+    for (int c = 0; c < CHUNKS; ++c) add_spread(x[c], both(-mean), left_of(c), spread);
+    const Norm n(a, mean, warp_sum(make_float2(sum_of(spread.off), sum_of(spread.squares))));
+    if (KEEP && lane == 0 && a.mean != nullptr) n.keep(a, row);
     T* const y = (T*)a.y + row * a.d + 4 * lane;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       if constexpr (ROWS > 1) {
-        finish<T, ACCESS, KEEP>(a, y + c * kGroup, row, c, left_of(c), x[c], mean, rstd, w[c], b[c]);
+        finish<T, ACCESS, KEEP>(a, y + c * kGroup, row, c, left_of(c), x[c], n, w[c], b[c]);
       } else {  // the next chunk's weights are on the way meanwhile
         f32x2 w_next[2], b_next[2];
         if (c + 1 < CHUNKS) weights(c + 1, w_next, b_next);
-        finish<T, ACCESS, KEEP>(a, y + c * kGroup, row, c, left_of(c), x[c], mean, rstd, w[0], b[0]);
+        finish<T, ACCESS, KEEP>(a, y + c * kGroup, row, c, left_of(c), x[c], n, w[0], b[0]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           w[0][h] = w_next[h];
@@ -175,14 +204,21 @@ __global__ void __launch_bounds__(kThreads, CHUNKS <= 5 ? 4 : 3) warp_kernel(con
   }
 }
 
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float v, float* of_warp) {
+template <int THREADS, typename V>  // float or float2
+__device__ __forceinline__ V block_sum(V v, V* of_warp) {
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = v;
   __syncthreads();
   v = of_warp[threadIdx.x & (THREADS / 32 - 1)];
 #pragma unroll
-  for (int o = THREADS / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = THREADS / 64; o > 0; o >>= 1) {
+    if constexpr (sizeof(V) == sizeof(float)) {
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+    } else {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+  }
   return v;
 }
 
@@ -190,7 +226,8 @@ __device__ __forceinline__ float block_sum(float v, float* of_warp) {
 template <typename T, int ACCESS, int THREADS, int KEPT, bool EVEN, bool KEEP>
 __global__ void __launch_bounds__(THREADS, (KEEP ? 640 : 768) / THREADS) block_kernel(const __grid_constant__ Args a) {
   constexpr int kWarps = THREADS / 32;
-  __shared__ float of_warp[2][kWarps];
+  __shared__ float sums[kWarps];
+  __shared__ float2 spreads[kWarps];
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -205,7 +242,8 @@ __global__ void __launch_bounds__(THREADS, (KEEP ? 640 : 768) / THREADS) block_k
   const int mine = max(0, min(KEPT, ((a.d + kGroup - 1) / kGroup - warp + kWarps - 1) / kWarps));  // chunks that there are
   fetch(blockIdx.x);
   for (int64_t row = blockIdx.x; row < a.m; row += gridDim.x) {
-    f32x2 x[KEPT][2], sum = 0ull, squares = 0ull;
+    f32x2 x[KEPT][2], sum = 0ull;
+    Spread spread;
 #pragma unroll
     for (int k = 0; k < KEPT; ++k) {
       next[k].get(x[k]);
@@ -213,15 +251,12 @@ __global__ void __launch_bounds__(THREADS, (KEEP ? 640 : 768) / THREADS) block_k
     }
     fetch(row + gridDim.x);
     // (the barrier of one sum keeps the reads of the other's apart from the next row's writes)
-    const float mean = block_sum<THREADS>(sum_of(sum), of_warp[0]) * a.per_column;
+    const float mean = block_sum<THREADS>(sum_of(sum), sums) * a.per_column;
 #pragma unroll
     for (int k = 0; k < KEPT; ++k)
-      if (k < mine) squares = add_squares(x[k], both(-mean), EVEN ? 4 : a.d - (warp + k * kWarps) * kGroup - 4 * lane, squares);
-    const float rstd = rstd_of(fmaf(block_sum<THREADS>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
-    if (KEEP && threadIdx.x == 0 && a.mean != nullptr) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
-    }
+      if (k < mine) add_spread(x[k], both(-mean), EVEN ? 4 : a.d - (warp + k * kWarps) * kGroup - 4 * lane, spread);
+    const Norm n(a, mean, block_sum<THREADS>(make_float2(sum_of(spread.off), sum_of(spread.squares)), spreads));
+    if (KEEP && threadIdx.x == 0 && a.mean != nullptr) n.keep(a, row);
     T* const y = (T*)a.y + row * a.d + own;
 #pragma unroll
     for (int k = 0; k < KEPT; ++k) {
@@ -236,22 +271,24 @@ __global__ void __launch_bounds__(THREADS, (KEEP ? 640 : 768) / THREADS) block_k
         of_columns(a.weight, own + k * kStep, left, 1.0f, w);
         of_columns(a.bias, own + k * kStep, left, 0.0f, b);
       }
-      finish<T, ACCESS, KEEP>(a, y + k * kStep, row, warp + k * kWarps, left, x[k], mean, rstd, w, b);
+      finish<T, ACCESS, KEEP>(a, y + k * kStep, row, warp + k * kWarps, left, x[k], n, w, b);
     }
   }
 }
 
 // Longer rows, one a CTA, read three times.
 template <typename T, int ACCESS, bool KEEP>
-__global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(512, KEEP ? 3 : 4) long_kernel(const __grid_constant__ Args a) {
   constexpr int kWarps = 16;
-  __shared__ float of_warp[2][kWarps];
+  __shared__ float sums[kWarps];
+  __shared__ float2 spreads[kWarps];
   dependency_wait();
   release_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.d + kGroup - 1) / kGroup;
   const int64_t row = blockIdx.x;
   const T* const from = (const T*)a.x + row * a.ldx;
   const auto each = [&](auto&& body) {  // every chunk of this warp
+#pragma unroll 4
     for (int c = warp; c < chunks; c += kWarps) {
       Four<T, ACCESS> v;
       f32x2 x[2];
@@ -261,20 +298,18 @@ __global__ void __launch_bounds__(512) long_kernel(const __grid_constant__ Args 
       body(c, col, x);
     }
   };
-  f32x2 sum = 0ull, squares = 0ull;
+  f32x2 sum = 0ull;
+  Spread spread;
   each([&](int, int, const f32x2 (&x)[2]) { sum = plus2(plus2(sum, x[0]), x[1]); });
-  const float mean = block_sum<512>(sum_of(sum), of_warp[0]) * a.per_column;
-  each([&](int, int col, const f32x2 (&x)[2]) { squares = add_squares(x, both(-mean), a.d - col, squares); });
-  const float rstd = rstd_of(fmaf(block_sum<512>(sum_of(squares), of_warp[1]), a.per_column, a.eps));
-  if (KEEP && threadIdx.x == 0 && a.mean != nullptr) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
-  }
+  const float mean = block_sum<512>(sum_of(sum), sums) * a.per_column;
+  each([&](int, int col, const f32x2 (&x)[2]) { add_spread(x, both(-mean), a.d - col, spread); });
+  const Norm n(a, mean, block_sum<512>(make_float2(sum_of(spread.off), sum_of(spread.squares)), spreads));
+  if (KEEP && threadIdx.x == 0 && a.mean != nullptr) n.keep(a, row);
   each([&](int c, int col, const f32x2 (&x)[2]) {
     f32x2 w[2], b[2];
     of_columns(a.weight, col, a.d - col, 1.0f, w);
     of_columns(a.bias, col, a.d - col, 0.0f, b);
-    finish<T, ACCESS, KEEP>(a, (T*)a.y + row * a.d + col, row, c, a.d - col, x, mean, rstd, w, b);
+    finish<T, ACCESS, KEEP>(a, (T*)a.y + row * a.d + col, row, c, a.d - col, x, n, w, b);
   });
 }
 
