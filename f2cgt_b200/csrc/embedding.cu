@@ -287,9 +287,11 @@ struct Segments {
   uint32_t rows;                // keys of places without a row
   int stretch;                  // 8 to 32
   int64_t stretches;
-  // only the rows that were looked up: numbers of segments in front of a stretch in its tile, and of those that begin in each tile
+  // only the rows that were looked up: numbers of segments in front of a stretch in its tile, and of those that begin in each tile, or (summed) in the tiles in front of each
+  // and, last, in all of them
   const uint32_t *in_tile, *of_tile;
   int tiles;
+  bool summed;
   int64_t* looked_up;           // null: the whole table
   int64_t* count;
 };
@@ -316,6 +318,33 @@ __global__ void __launch_bounds__(kThreads) number_kernel(const uint32_t* __rest
   // a thread's four places are a part of one stretch
   if (first < m && first % stretch == 0) in_tile[first / stretch] = before;
   if (threadIdx.x == kThreads - 1) of_tile[blockIdx.x] = before + own;
+}
+
+// Beyond kTilesEach tiles their numbers are summed once, by a CTA; up to there every warp does so for itself, which saves a launch.  (Always so it was quadratic in the places:
+// 2^24 of them, 8 columns, took 7.1 ms and 2.7 this way; 2^20 176 us and 164; 2^19 98 and 96, and 128 columns 148 and 149.)
+constexpr int kTilesEach = 256, kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads) sum_kernel(uint32_t* __restrict__ of_tile, int tiles) {
+  __shared__ uint32_t of_warp[kSumThreads / 32];
+  dependency_wait();
+  release_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = (tiles + kSumThreads - 1) / kSumThreads, from = min(tiles, (int)threadIdx.x * each), to = min(tiles, from + each);
+  uint32_t own = 0u;
+  for (int t = from; t < to; ++t) own += of_tile[t];
+  uint32_t before = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  if (lane == 31) of_warp[warp] = before;
+  __syncthreads();
+  before = before - own + __reduce_add_sync(0xffffffffu, lane < warp ? of_warp[lane] : 0u);
+  for (int t = from; t < to; ++t) {
+    const uint32_t v = of_tile[t];
+    of_tile[t] = before;
+    before += v;
+  }
+  if (threadIdx.x == kSumThreads - 1) of_tile[tiles] = before;
 }
 
 constexpr int kRowsAhead = 8;
@@ -347,13 +376,19 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(const T* __restrict__
   if (s.looked_up != nullptr) {
     uint32_t tiles_before = 0u, all = 0u;
     const int tile = (int)(start / kTile);
-    for (int t = lane; t < s.tiles; t += 32) {
-      const uint32_t v = s.of_tile[t];
-      all += v;
-      if (t < tile) tiles_before += v;
+    if (s.summed) {
+      tiles_before = s.of_tile[tile];
+      all = s.of_tile[s.tiles];
+    } else {
+      for (int t = lane; t < s.tiles; t += 32) {
+        const uint32_t v = s.of_tile[t];
+        all += v;
+        if (t < tile) tiles_before += v;
+      }
+      all = __reduce_add_sync(0xffffffffu, all);
+      tiles_before = __reduce_add_sync(0xffffffffu, tiles_before);
     }
-    all = __reduce_add_sync(0xffffffffu, all);
-    row = __reduce_add_sync(0xffffffffu, tiles_before) + s.in_tile[c] + __popc(first & (0xffffffffu >> (31 - lane))) - 1u;
+    row = tiles_before + s.in_tile[c] + __popc(first & (0xffffffffu >> (31 - lane))) - 1u;
     if (blockIdx.y == 0) {
       if (c == 0 && lane == 0) *s.count = all;
       if (key < s.rows && ((first >> lane) & 1u)) s.looked_up[row] = (int64_t)key;
@@ -861,7 +896,7 @@ static Plan plan(int64_t m, int64_t rows, int64_t d) {
     p.totals = take((int64_t)4 << p.bits);
   }
   p.in_tile = take(4 * p.stretches);
-  p.of_tile = take(4 * (int64_t)p.tiles);
+  p.of_tile = take(4 * ((int64_t)p.tiles + 1));
   p.head = take(4 * p.stretches * p.width);
   p.tail = take(4 * p.stretches * p.width);
   p.row = take(8 * p.stretches);
@@ -1048,9 +1083,11 @@ extern "C" int f2c_embedding_backward(const void* dy, int64_t ldy, int dtype, co
   const emb::Pairs sorted = index_dtype == F2C_I64 ? emb::sort(p, (const int64_t*)ids, (uint32_t)rows, ws, grad, bytes, st)
                                                        : emb::sort(p, (const int32_t*)ids, (uint32_t)rows, ws, grad, bytes, st);
   uint32_t *const in_tile = (uint32_t*)(ws + p.in_tile), *const of_tile = (uint32_t*)(ws + p.of_tile);
+  const bool summed = !dense && p.tiles > emb::kTilesEach;
   if (!dense)
     launch_dependent(emb::number_kernel, dim3((unsigned)p.tiles), emb::kThreads, 0, st, (const uint32_t*)sorted.key, m, (uint32_t)rows, p.stretch, in_tile, of_tile, looked_up);
-  const emb::Segments s{sorted.key, sorted.place, m, (uint32_t)rows, p.stretch, p.stretches, in_tile, of_tile, p.tiles, dense ? nullptr : looked_up, count};
+  if (summed) launch_dependent(emb::sum_kernel, dim3(1), emb::kSumThreads, 0, st, of_tile, p.tiles);
+  const emb::Segments s{sorted.key, sorted.place, m, (uint32_t)rows, p.stretch, p.stretches, in_tile, of_tile, p.tiles, summed, dense ? nullptr : looked_up, count};
   const emb::Open open{(float*)(ws + p.head), (float*)(ws + p.tail), (int64_t*)(ws + p.row), p.width};
   F2C_BY_ROWS(emb::add_up, dtype, access, p, dy, ldy, scale, s, open, grad, st);
   return check_launch(op);
