@@ -29,9 +29,8 @@ def links(d):
 
 
 def norm(x, weight, bias, eps):
-    """y, mean, rstd in 64 bits, and the most that they are off.  The first mean is off by `first`.  Where it is more than four deviations (by variance and eps) it is corrected by the
-    mean of the differences, off by what a sum of that many links loses of the differences; elsewhere `first` is links times five roundings of a deviation at most.  A
-    difference of two near numbers, and the correction's product, are a rounding each."""
+    """y, mean, rstd in 64 bits, and the most that they are off.  The first mean is off by `first`; the mean of the differences from it corrects it, off by what a sum of that
+    many links loses of the differences.  A difference of two near numbers, and the correction's product, are a rounding each."""
     x = x.double()
     k = links(x.shape[1])
     mean = x.mean(1)
@@ -42,10 +41,10 @@ def norm(x, weight, bias, eps):
     y = h * weight.double() + bias.double()
     first = k * R.U * x.abs().mean(1)
     size = z.abs().mean(1) + first  # of a difference, on average
-    left = torch.maximum((k + 2) * R.U * size, torch.minimum(first, 5.5 * k * R.U / rstd))  # of the mean's error
+    left = (k + 2) * R.U * size  # of the mean's error
     z_off = left[:, None] + R.U * (2 * z.abs() + first[:, None])
-    # the variance: mean of the squares (less that of the correction), where the mean's error enters squared or is taken out
-    var_off = (k + 6) * R.U * (var + first ** 2) + 2 * first * (k + 2) * R.U * size + left ** 2
+    # the variance: mean of the squares less the square of the correction
+    var_off = (k + 6) * R.U * (var + first ** 2) + 2 * first * left
     rstd_off = rstd * (0.5 * var_off * rstd ** 2 + 4 * R.U)
     h_off = rstd[:, None] * (z_off + R.U * first[:, None]) + z.abs() * rstd_off[:, None] + 2 * R.U * h.abs()
     y_off = weight.double().abs() * h_off + 2 * R.U * (h * weight.double()).abs() + 2 * R.U * y.abs()
