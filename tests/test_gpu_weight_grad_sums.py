@@ -125,3 +125,26 @@ def test_groups_of_equal_values_and_of_none():
     dy = positive(500, 40, torch.float32, 9)
     dw, _ = ops().checkpoint_weight_grad(dy, ops().checkpoint_int8(x))
     R.near(dw, dy.double().t() @ x.double(), (500 / 8 + 200) * R.U * (dy.double().abs().t() @ x.double().abs()))
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("m,split", [(9000, False), (9000, True), (40, False)])
+def test_waits_that_run_out_around_a_taking_out(m, split, dtype):
+    """With all waits run out: NaN in all of both results, a status, and nothing of it in the next call."""
+    import ctypes as C
+
+    from f2cgt_b200 import _lib
+    o = ops()
+    n, k = (100, 200) if split else (4 * (256 if dtype is torch.bfloat16 else 128), 37 * 128)
+    dy, c = positive(m, n, dtype, 3), o.checkpoint_int8(positive(m, k, dtype, 4) - 1)
+    want = o.checkpoint_weight_grad(dy, c)
+    dw, db = torch.zeros(n, k, dtype=dtype, device="cuda"), torch.zeros(n, dtype=dtype, device="cuda")
+    tag = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}[dtype]
+    size = _lib.lib.f2c_checkpoint_weight_grad_workspace(dy.data_ptr(), n, tag, m, n, k)
+    assert (size > 0) is split
+    work = torch.empty(size + 256, dtype=torch.uint8, device="cuda")
+    rc = _lib.lib.f2c_checkpoint_weight_grad(dy.data_ptr(), n, tag, c.codes.data_ptr(), c.codes.stride(0), c.scales.data_ptr(), m, n, k, dw.data_ptr(), db.data_ptr(), _lib.NO_WAITS,
+                                             work.data_ptr(), size, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0 and o.device_status() == 8 and torch.isnan(dw).all() and torch.isnan(db).all()
+    got = o.checkpoint_weight_grad(dy, c)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and o.device_status() == 0
