@@ -363,6 +363,11 @@ extern "C" int f2c_layer_norm(const void* x, int64_t ldx, int dtype, int64_t m, 
   F2C_REQUIRE((mean == nullptr) == (rstd == nullptr), F2C_ERR_INVALID, "%s: mean and rstd go together", op);
   if (codes || scales)
     if (const int rc = ckpt::check_codes(op, codes, ldq, scales, m, d)) return rc;
+  if (m > 0 && d == 0 && mean != nullptr) {  // the mean of no values
+    cudaError_t e = cudaMemsetAsync(mean, 0xff, (size_t)m * sizeof(float), (cudaStream_t)stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(rstd, 0xff, (size_t)m * sizeof(float), (cudaStream_t)stream);
+    if (e != cudaSuccess) return set_error(F2C_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  }
   if (m == 0 || d == 0) return F2C_OK;
   F2C_REQUIRE(x && y, F2C_ERR_INVALID, "%s: null pointer", op);
   F2C_REQUIRE(m == 1 || ldx >= d, F2C_ERR_INVALID, "%s: a row stride is smaller than the row", op);

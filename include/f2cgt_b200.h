@@ -477,7 +477,7 @@ int f2c_checkpoint_weight_grad(const void* dy, int64_t ldy, int dtype, const uin
 /* y [m, d] = (x - mean) rstd weight + bias of every row, rstd = 1 / sqrt(mean((x - mean)^2) + eps); relu != 0: negative values become 0 (a NaN
  * stays one).  x and y of `dtype`, everything else float; weight, bias [d] or NULL (1, 0).  Wanted for the backward pass, or NULL: mean and
  * rstd [m]; active [m, ceil(d / 8)]: bit c % 8 of byte c / 8 says that y was positive before rounding (bits behind the columns are 0); codes and
- * scales: x in 8 bits, as f2c_checkpoint_int8 has it. */
+ * scales: x in 8 bits, as f2c_checkpoint_int8 has it.  Of rows without columns mean and rstd are NaN. */
 int f2c_layer_norm(const void* x, int64_t ldx, int dtype, int64_t m, int64_t d, const float* weight, const float* bias, float eps, int relu, void* y,
                    float* mean, float* rstd, uint8_t* active, uint8_t* codes, int64_t ldq, float* scales, void* stream);
 /* Gradients of it.  x or codes (with scales), mean, rstd and active (NULL: no ReLU) as f2c_layer_norm left them; dy and dx (and x) of `dtype`, dx

@@ -1,0 +1,25 @@
+"""Layer norm, 8-bit activations and learned rows at the ends of what they take."""
+import pytest
+import torch
+
+import learn_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def ops():
+    from f2cgt_b200 import ops
+    return ops
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("int8", [False, True])
+def test_rows_without_columns(int8, relu):
+    """The mean of no values is NaN, not what the memory held before."""
+    held = [torch.full((5,), 7.0, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    del held
+    y, saved = ops().layer_norm_train(torch.empty(5, 0, device="cuda"), relu=relu, int8=int8)
+    assert y.shape == (5, 0) and torch.isnan(saved.mean).all() and torch.isnan(saved.rstd).all()
+    dx, dweight, dbias = ops().layer_norm_backward(torch.empty(5, 0, device="cuda"), saved)
+    assert dx.shape == (5, 0) and dweight.shape == dbias.shape == (0,)
