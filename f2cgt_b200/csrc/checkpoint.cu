@@ -2,7 +2,7 @@
 // instructions, some hundred a group of a warp for 4 values a lane (the same 34 us, 2.9 TB/s; 59,000 x 128 float32 10.9 us, 3.5 TB/s).
 //
 // A warp has a group - 128 columns of a row - four columns a lane: its extremes are one reduction instruction each, its codes 128 bytes
-// side by side.  Groups are taken kAhead at a time, all loads before the first use, their steps and reciprocals in a lane each.
+// side by side, and every lane works out the step and its reciprocal.  Groups are taken kAhead at a time, all loads before the first use; lane a writes group a's step.
 #include "checkpoint.cuh"
 
 namespace f2c {

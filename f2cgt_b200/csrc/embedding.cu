@@ -9,14 +9,16 @@
 // the launches below 8.3 and 12.4 (rows alone), and 19 in a row of calls, whose launches the host makes.)
 //
 // More places of few rows (labels): a CTA sorts 400 places at most while their rows of dy come to its shared memory, and leaves a sum for every row of the table
-// that it met; a second launch adds those up in the CTAs' order.  59,000 x 128 of 172 rows: 14 us, 24 with all places sorted (rows alone 20 and 27).
+// that it met; a second launch adds those up in the CTAs' order.  59,000 x 128 of 172 rows: 13.4 us (rows alone 19.5); all places sorted, from
+// 59,201 of them on, 18.2 (26.7).
 //
 // Sorting.  Up to 4096 places each place counts the ones in front of it, in one launch: the keys are few enough that all pairs cost
 // less than further launches.  Beyond, digits of up to 11 bits from the lowest on: counts of every tile of 1024 places, their sums over tiles, and the
 // placing, in which a warp ranks 32 places at a time by their equals in it and counts the next digit where the places go.  As many digits as the table
 // has rows need.  All of it is latency, 3 to 6 us a launch: the first one also clears what the others add to, and a whole table's gradient, on CTAs of its
 // own.  (With tiles of 4096 places that add up the other tiles' counts themselves, two launches less, 121,000 places took 62 us instead of 51: the work
-// was on too few SMs.)  121,000 places of 2.4 M rows, 128 columns: 57 us in seven launches, 32 of them the sorting.
+// was on too few SMs.)  121,000 places of 2.4 M rows, 128 columns, the rows alone: 51 us in eight launches (57 beside a lookup), 32 of
+// them the sorting; the whole table in seven 256 us, of which clearing it is 168.
 #include <algorithm>
 
 #include "checkpoint.cuh"
@@ -644,7 +646,8 @@ __global__ void __launch_bounds__(kOneLaunch, 1) few_kernel(const T* __restrict_
 
 // ---------------------------------------------------------------- few rows
 // A CTA has `each` places, 128 columns of them: it sorts them by row while they come to shared memory, and leaves a sum for every row that is among them.
-// (Places that need more than one CTA an SM: the sorting is not hidden any more, 236,000 of 1000 rows took 80 us and 68 with all of them sorted.  More rows
+// (Places that need more than one CTA an SM: the sorting is not hidden any more, 236,000 of 1000 rows took 80 us and 68 with all of them sorted.  400 places are what float32
+// rows leave room for, with some to spare; twice as many of 16-bit rows were not tried.  More rows
 // times pieces of 128 columns: as many CTAs join them, 2000 x 128 of 2000 rows took 16 us and 10, of 1000 rows 11 and 10.)
 constexpr int kLabels = 1024, kLabelThreads = 512, kLabelWarps = kLabelThreads / 32, kMostPlaces = 400, kLeastPlaces = 32;
 constexpr uint16_t kNoSlot = 0xffffu;

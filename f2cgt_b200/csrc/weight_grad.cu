@@ -19,7 +19,7 @@
 // 2048 rows, in shared memory and TMEM, while the MMAs wait (16,384 x 2048 x 4096, side by side: 488 us without, 495 every 4096 rows, 507 every 2048, 533 every 1024).
 //
 // What bounds it: bfloat16 shared memory, from which a stage's operand is read twice while its codes and steps are read and the next stages arrive (16,384 x 2048 x
-// 4096: 490 us among other calls, 560 TFLOP/s of the product, 1120 of the MMAs, 420 by itself; half the MMAs, or no reading of codes and steps, each took 20% off); float32 the instructions that
+// 4096: 515 us among other calls, 534 TFLOP/s of the product, 1070 of the MMAs, 480 by itself; half the MMAs, or no reading of codes and steps, each took 20% off); float32 the instructions that
 // split dy times the step, 650 a warp for a stage (4096 x 2048 x 1152: 74 us); few rows latency (59,000 x 128 x 128 float32: 17 us of 5.9 that memory takes).
 //
 // Many rows and few tiles: the rows are dealt out over all SMs; each leaves its part of the sums, and a second launch adds them up in their order.
@@ -726,7 +726,7 @@ struct Plan {
 // the groups do for it); together the SMs get no more than 3500 bytes a cycle; a tile's start and end 4000, the parts' way through L2 and back 4000 bytes a
 // cycle for all SMs, and the launch that adds them up 4000.  With more tiles than SMs those that fill the SMs are left whole and the rows of the others split, where
 // that is an eighth less: 196 tiles, 16,384 x 1700 x 1700 float32 509 us without and 370 so; 152 tiles, 8192 x 2048 x 2368 bfloat16 188 and 137; but 256 tiles,
-// 16,384 x 2048 x 4096 bfloat16 416 and 429 (SMs that wait leave the others power).
+// 16,384 x 2048 x 4096 bfloat16 416 and 429 (SMs that wait leave the others power; both before its sums were taken out).
 static Plan plan(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k) {
   Plan p{};
   const int64_t item = dtype_size(dtype);

@@ -391,7 +391,7 @@ def checkpoint_values(checkpoint, dtype=torch.float32):
 
 def checkpoint_weight_grad(dy, checkpoint):
     """``(dweight, dbias)`` of a linear layer ``y = x @ weight.T + bias`` whose input was kept as an ``Int8Checkpoint``: ``dy.T @ x`` and the sums of
-    ``dy``'s columns, in the dtype of ``dy`` [rows, n] (float32 / float16 / bfloat16), without writing ``x`` out.  On the tensor cores; ``dy`` times a step is
+    ``dy``'s columns, in the dtype of ``dy`` [rows, n] (float32 / float16 / bfloat16), without writing ``x`` out (which has columns, where there are rows).  On the tensor cores; ``dy`` times a step is
     held to 24 bits (float32) or 16 (float16), the input to 16 bits beside bfloat16.  The tensor cores' sums are cut to 24 bits, for every 16 rows; they are taken out every
     256 rows (float32), 1024 (float16) or 2048 (bfloat16) and added up in single precision, in an order that the sizes alone decide."""
     return _native.checkpoint_weight_grad(dy, checkpoint[0], checkpoint[1])
@@ -421,7 +421,7 @@ def layer_norm_backward(dy, saved, weight=None):
 
 # ------------------------------------------------------------------ learned rows
 def embedding(table, ids, scale=1.0):
-    """``scale * table[ids]``, rounded once: rows of ``table`` [rows, cols] (float32 / float16 / bfloat16) for ``ids`` of any shape (int32 / int64).  An
+    """``scale * table[ids]``, rounded once: rows of ``table`` [rows, cols] (float32 / float16 / bfloat16) for contiguous ``ids`` of any shape (int32 / int64).  An
     id outside the table - the -1 that pads a batch - is a row of zeros.  It has no gradient by itself: see ``embedding_backward``;
     ``sage.NodeEmbedding`` is the module over them."""
     return _native.embedding(table, ids, scale)

@@ -386,7 +386,7 @@ class _Embedding(torch.autograd.Function):
 
 
 class NodeEmbedding(nn.Module):
-    """A learned row for every node: ``scale * weight[ids]`` (``ops.embedding``), zeros for ids outside the table.  The table's gradient is dense, or with
+    """A learned row for every node: ``scale * weight[ids]`` (``ops.embedding``; ``ids`` contiguous), zeros for ids outside the table.  The table's gradient is dense, or with
     ``sparse=True`` a sparse tensor of the rows that were looked up, each once, as ``torch.optim.SparseAdam`` and ``SGD`` take it.  Differentiable once."""
 
     def __init__(self, n_nodes, columns, scale=1.0, sparse=False, device=None, dtype=None):

@@ -468,7 +468,7 @@ int f2c_checkpoint_values(const uint8_t* codes, int64_t ldq, const float* scales
  * dy times a code's step is held to 24 bits for F32 and to 16 for F16, x to 16 bits for BF16.  The tensor cores' sums are cut to 24 bits, for every 16 rows; they are
  * taken out every 256 rows (F32), 1024 (F16) or 2048 (BF16) and added up in single precision, in an order that the sizes decide.
  * Where a row of dy or a group of x is not finite, neither are the results that it has a part in (NaN or infinities).
- * Codes as f2c_checkpoint_int8 leaves them (every row has whole 16 bytes).  m < 2^31 - 256, n and k up to 2^17.  flags: 0, or F2C_NO_WAITS.
+ * Codes as f2c_checkpoint_int8 leaves them (every row has whole 16 bytes).  m < 2^31 - 256, n and k up to 2^17; k = 0 only without rows.  flags: 0, or F2C_NO_WAITS.
  * workspace: f2c_checkpoint_weight_grad_workspace(...) bytes, 256-byte aligned; it depends on where dy starts and on its stride (rows that do not start on
  * 16 bytes are copied): ask with those of the call.  A bounded wait that runs out reports 8 and leaves NaN. */
 int64_t f2c_checkpoint_weight_grad_workspace(const void* dy, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k);

@@ -2,8 +2,6 @@
 import pytest
 import torch
 
-import learn_reference as R
-
 pytestmark = pytest.mark.gpu
 
 
@@ -23,3 +21,17 @@ def test_rows_without_columns(int8, relu):
     assert y.shape == (5, 0) and torch.isnan(saved.mean).all() and torch.isnan(saved.rstd).all()
     dx, dweight, dbias = ops().layer_norm_backward(torch.empty(5, 0, device="cuda"), saved)
     assert dx.shape == (5, 0) and dweight.shape == dbias.shape == (0,)
+
+
+def test_what_is_refused_at_the_ends():
+    from f2cgt_b200 import sage
+    o = ops()
+    with pytest.raises(RuntimeError, match="no columns"):
+        o.checkpoint_weight_grad(torch.ones(9, 3, device="cuda"), o.checkpoint_int8(torch.empty(9, 0, device="cuda")))
+    ids = torch.arange(12, device="cuda")[::2]
+    rows = sage.NodeEmbedding(20, 8, device="cuda")
+    for call in (lambda: rows(ids), lambda: o.embedding_backward(torch.ones(6, 8, device="cuda"), ids, 20), lambda: o.embedding_backward_rows(torch.ones(6, 8, device="cuda"), ids, 20)):
+        with pytest.raises(RuntimeError, match="contiguous"):
+            call()
+    rows(ids.contiguous()).sum().backward()
+    assert torch.equal(rows.weight.grad[:, 0], torch.bincount(ids, minlength=20).float())
