@@ -30,3 +30,23 @@ def test_time_grows_with_the_places():
         assert int(rows.float().sum() / 4) == m
         del looked_up, rows, dy, ids
     assert times[1] < 24 * times[0], times
+
+
+def test_the_same_in_a_graph_and_beside_another():
+    """Places whose tiles are numbered by a launch of its own, in captured calls and two at once."""
+    m, rows = 300_000, 1 << 20
+    ids, dy = ids_of(m, rows, "outside"), table_of(m, 4, torch.float32)
+    first = ops().embedding_backward_rows(dy, ids, rows)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        beside = [ops().embedding_backward_rows(dy, ids, rows) for _ in range(3)]
+    here = [ops().embedding_backward_rows(dy, ids, rows) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for got in beside + here for a, b in zip(got, first))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ops().embedding_backward_rows(dy, ids, rows)
+    ids.copy_(ids_of(m, rows, "skew", seed=5))
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(captured, ops().embedding_backward_rows(dy, ids, rows)))

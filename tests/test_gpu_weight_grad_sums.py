@@ -148,3 +148,40 @@ def test_waits_that_run_out_around_a_taking_out(m, split, dtype):
     assert rc == 0 and o.device_status() == 8 and torch.isnan(dw).all() and torch.isnan(db).all()
     got = o.checkpoint_weight_grad(dy, c)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and o.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+def test_numbers_that_are_none_before_a_taking_out(dtype):
+    """They stay in their column of dy and in their group of x."""
+    m, n, k = 5000, 4 * (256 if dtype is torch.bfloat16 else 128), 37 * 128
+    x, dy = positive(m, k, dtype, 1) - 1, positive(m, n, dtype, 2)
+    x[17, 200], x[4000, 1000], dy[5, 3] = float("inf"), float("nan"), float("nan")
+    dw, db = ops().checkpoint_weight_grad(dy, ops().checkpoint_int8(x))
+    want = torch.zeros(n, k, dtype=torch.bool, device="cuda")
+    want[:, 128:256] = want[:, 896:1024] = want[3] = True
+    assert torch.equal(torch.isnan(dw), want) and torch.isnan(db).nonzero().flatten().tolist() == [3]
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("tiles", [37, 40])
+def test_the_same_bits_beside_another_and_in_a_graph(tiles, dtype):
+    """148 tiles, whole, and 160, of which 12 have their rows split."""
+    m, n, k = 5000, 4 * (256 if dtype is torch.bfloat16 else 128), tiles * 128
+    x, dy = positive(m, k, dtype, 1) - 1, positive(m, n, dtype, 2)
+    c = ops().checkpoint_int8(x)
+    first = ops().checkpoint_weight_grad(dy, c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        beside = [ops().checkpoint_weight_grad(dy, c) for _ in range(3)]
+    here = [ops().checkpoint_weight_grad(dy, c) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(side)
+    for got in beside + here:
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ops().checkpoint_weight_grad(dy, c)
+    dy.copy_(positive(m, n, dtype, 41))
+    graph.replay()
+    again = ops().checkpoint_weight_grad(dy, c)
+    assert torch.equal(captured[0], again[0]) and torch.equal(captured[1], again[1])
